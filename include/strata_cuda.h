@@ -37,7 +37,7 @@ extern "C" {
 #define STRATA_ERR_HANDLE 4  /* not a live buffer of this context: src/backend.js:138-143 */
 #define STRATA_ERR_ALLOC 5   /* device allocation failed: wasm/runtime.js:7 "WASM allocation failed" */
 #define STRATA_ERR_CUDA 6    /* CUDA runtime error (the message names it) */
-#define STRATA_ERR_DEVICE 7  /* a kernel recorded an out-of-range index, an invalid routing, a timed-out wait or a non-finite PLE scale */
+#define STRATA_ERR_DEVICE 7  /* a kernel recorded an out-of-range index, an invalid routing, a timed-out wait, a non-finite PLE scale or cache value */
 
 #define STRATA_F32 0
 #define STRATA_I32 1
@@ -271,6 +271,86 @@ int strata_ep_loopback_release(strata_ctx *ctx, uint64_t hub);
  * non-finite scale ("Non-finite PLE scales", src/model.js:241) are reported by the next
  * synchronising call. Stream-ordered. */
 int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, int32_t rows, int32_t head_dim, strata_buf values);
+
+/* ---- attention over a paged key/value cache held in 8 bits (no reference counterpart) ----
+ * The reference keeps F32 caches of at most 2048 cells and leaves sparse selection out
+ * (src/model.js:13). These entries serve longer sessions and more of them: a cache of one byte
+ * per value, attention over it, and a selection of the blocks that a query attends to.
+ *
+ * Format. A page holds STRATA_KV8_BLOCK = 64 consecutive tokens (a block) of one sequence for every
+ * key/value head. With P = dim padded to 64, 128 or 256:
+ *   codes   int8 [pages][kv_heads][2][P * 64]: keys as [P / 64][64 tokens][64 channels], then values as
+ *           [P channels][64 tokens]; channels past dim are zero
+ *   marks   int8 [pages][kv_heads][2][P]: the lowest and the highest key code of each channel
+ *   scales  f32  [pages][kv_heads][2]: key scale, value scale; value = code * scale
+ *   open    f32  [sequences][2][64][kv_heads][dim]: the rows of each sequence's last, unfilled block,
+ *           from which its codes are formed again when a larger value makes its scale grow
+ *   table   i32  [sequences][blocks]: the page of each block (a page belongs to one sequence)
+ * With handles the codes and marks are u32 buffers of a quarter as many elements. `workspace` is
+ * scratch of STRATA_KV8_WORKSPACE_BYTES, zero-filled once by the caller and then left to these
+ * entries; calls that may overlap on the GPU need caches with workspaces of their own.
+ *
+ * Runs. A call works on segments * count tokens, `count` for each of `segments` runs. Run i belongs
+ * to sequence[i] and its first token stands at position start[i]; both are read on the device, so a
+ * captured graph can replay the call. sequence -1 marks an idle slot: nothing is appended, nothing is
+ * picked, its output is zero. Decode of a batch is count = 1; a prompt chunk is segments = 1.
+ * Rows of q, k and v are `row_stride` floats apart (0: contiguous).
+ *
+ * append: scale = amax / 127 over a block's rows so far (0 below 2^-100), code = x times the
+ *   reciprocal of scale, rounded to nearest even. A block's codes depend on its rows alone, not on how they
+ *   were split over calls. Appending goes on where the sequence ends; a run that starts at a block's
+ *   first token starts that block afresh. Rows dropped from an open block leave its scale and marks as they were.
+ *   A value that is not finite is stored as zero and reported. Runs of one call name different sequences.
+ * select: for each token and key/value head the `top` blocks (of those at or before the token) with the
+ *   largest bound on the summed logits of the group's queries, in ascending order, -1 past the last: i32
+ *   picks [tokens][kv_heads][top]. The bound is sum_d p_d hi_d + n_d lo_d times the block's key scale, where hi, lo
+ *   are the marks and p, n the group's positive and negative query parts: queries are rounded to
+ *   multiples of amax / 32767, added up as whole numbers and rounded to 8 bits, so that the choice does not
+ *   depend on the order of any sum. The `first` first and `last` last blocks are always picked; equal
+ *   bounds go to the lower block. A query value that is not finite counts as zero. Tables of at most
+ *   STRATA_KV8_SELECT_BLOCKS blocks.
+ * attend: y [tokens][heads * dim] = softmax(scale * q . k) v over the keys at or before the token's position, of
+ *   every block (picks null / 0) or of the blocks that picks [tokens][kv_heads][top] lists (distinct, -1 for
+ *   none). Query head h uses key/value head h / (heads / kv_heads). A token that sees no key gets zeros.
+ *   F32 in and out: products of two FP16 halves of each query and weight with the codes, which FP16
+ *   holds exactly; sums, maxima and weights in F32.
+ *
+ * heads / kv_heads is any whole number, dim is 1 .. 256. A sequence, page or position outside the cache
+ * is skipped and reported by the next synchronising call (STRATA_ERR_DEVICE), or, in the pointer forms, by
+ * bit 0 of *status (bit 4: a value that was not finite), which the caller clears. */
+#define STRATA_KV8_BLOCK 64
+#define STRATA_KV8_WORKSPACE_BYTES (32u << 20)
+#define STRATA_KV8_SELECT_BLOCKS 32768
+typedef struct {
+    int32_t kv_heads, dim, pages, sequences, blocks;
+    strata_buf codes, marks, scales, open, table, workspace;
+} strata_kv8_cache;
+int strata_kv8_append(strata_ctx *ctx, const strata_kv8_cache *cache, strata_buf k, strata_buf v, uint64_t row_stride, int32_t segments,
+                      int32_t count, strata_buf sequence, strata_buf start);
+int strata_kv8_select(strata_ctx *ctx, const strata_kv8_cache *cache, strata_buf q, uint64_t row_stride, int32_t heads, int32_t segments,
+                      int32_t count, strata_buf sequence, strata_buf start, int32_t top, int32_t first, int32_t last, strata_buf picks);
+int strata_kv8_attend(strata_ctx *ctx, const strata_kv8_cache *cache, strata_buf q, uint64_t row_stride, int32_t heads, int32_t segments,
+                      int32_t count, strata_buf sequence, strata_buf start, strata_buf picks, int32_t top, float scale, strata_buf y);
+/* The same on caller-owned device memory and a stream (a cudaStream_t as void*; NULL = the default
+ * stream) of the calling thread's current device. Nothing is allocated. codes, marks and workspace
+ * start on 16-byte boundaries, everything else on its element's. `status` (optional) is a device word
+ * that errors are added to; `msg` (optional) receives the reason for a non-zero return. */
+typedef struct {
+    int32_t kv_heads, dim, pages, sequences, blocks;
+    int8_t *codes, *marks;
+    float *scales, *open;
+    const int32_t *table;
+    void *workspace;
+    uint32_t *status;
+} strata_kv8_cache_dev;
+int strata_kv8_append_dev(const strata_kv8_cache_dev *cache, const float *k, const float *v, uint64_t row_stride, int32_t segments,
+                          int32_t count, const int32_t *sequence, const int32_t *start, void *stream, char *msg, size_t msg_cap);
+int strata_kv8_select_dev(const strata_kv8_cache_dev *cache, const float *q, uint64_t row_stride, int32_t heads, int32_t segments,
+                          int32_t count, const int32_t *sequence, const int32_t *start, int32_t top, int32_t first, int32_t last,
+                          int32_t *picks, void *stream, char *msg, size_t msg_cap);
+int strata_kv8_attend_dev(const strata_kv8_cache_dev *cache, const float *q, uint64_t row_stride, int32_t heads, int32_t segments,
+                          int32_t count, const int32_t *sequence, const int32_t *start, const int32_t *picks, int32_t top, float scale,
+                          float *y, void *stream, char *msg, size_t msg_cap);
 
 /* ---- CUDA graphs of the context's stream (no reference counterpart: the B200 runtime replays
  * captured work instead of relaunching it from the host) ----

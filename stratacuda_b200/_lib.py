@@ -36,6 +36,21 @@ class StrataMoeLayerDev(C.Structure):
                 ("shared_blob", C.c_void_p), ("shared_gate", C.c_void_p)]
 
 
+KV8_BLOCK, KV8_WORKSPACE_BYTES, KV8_SELECT_BLOCKS = 64, 32 << 20, 32768
+
+
+class StrataKv8Cache(C.Structure):
+    _fields_ = [("kv_heads", C.c_int32), ("dim", C.c_int32), ("pages", C.c_int32), ("sequences", C.c_int32), ("blocks", C.c_int32),
+                ("codes", C.c_uint64), ("marks", C.c_uint64), ("scales", C.c_uint64), ("open", C.c_uint64), ("table", C.c_uint64),
+                ("workspace", C.c_uint64)]
+
+
+class StrataKv8CacheDev(C.Structure):
+    _fields_ = [("kv_heads", C.c_int32), ("dim", C.c_int32), ("pages", C.c_int32), ("sequences", C.c_int32), ("blocks", C.c_int32),
+                ("codes", C.c_void_p), ("marks", C.c_void_p), ("scales", C.c_void_p), ("open", C.c_void_p), ("table", C.c_void_p),
+                ("workspace", C.c_void_p), ("status", C.c_void_p)]
+
+
 SIGNATURES = {
     "strata_create": ([_i, C.POINTER(_vp)], _i),
     "strata_destroy": ([_vp], _i),
@@ -71,6 +86,16 @@ SIGNATURES = {
     "strata_moe_forward": ([_vp, C.POINTER(StrataMoeLayer), _u64, C.c_int32, _u64, _u64, _u64, C.c_int32], _i),
     "strata_validate_experts": ([_vp, _u64, C.c_int32, C.c_int32, C.c_int32], _i),
     "strata_moe_forward_noalloc": ([C.POINTER(StrataMoeLayerDev), _vp, C.c_int32, _vp, _vp, _vp, _vp, C.c_char_p, _sz], _i),
+    "strata_kv8_append": ([_vp, C.POINTER(StrataKv8Cache), _u64, _u64, _u64, C.c_int32, C.c_int32, _u64, _u64], _i),
+    "strata_kv8_select": ([_vp, C.POINTER(StrataKv8Cache), _u64, _u64, C.c_int32, C.c_int32, C.c_int32, _u64, _u64, C.c_int32, C.c_int32,
+                           C.c_int32, _u64], _i),
+    "strata_kv8_attend": ([_vp, C.POINTER(StrataKv8Cache), _u64, _u64, C.c_int32, C.c_int32, C.c_int32, _u64, _u64, _u64, C.c_int32,
+                           C.c_float, _u64], _i),
+    "strata_kv8_append_dev": ([C.POINTER(StrataKv8CacheDev), _vp, _vp, _u64, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_char_p, _sz], _i),
+    "strata_kv8_select_dev": ([C.POINTER(StrataKv8CacheDev), _vp, _u64, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, C.c_int32, C.c_int32,
+                               C.c_int32, _vp, _vp, C.c_char_p, _sz], _i),
+    "strata_kv8_attend_dev": ([C.POINTER(StrataKv8CacheDev), _vp, _u64, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_int32,
+                               C.c_float, _vp, _vp, C.c_char_p, _sz], _i),
     "strata_synth_blobs": ([_vp, _u64, _u64, _u64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32], _i),
     "strata_synth_normals": ([_vp, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _d], _i),
 }

@@ -16,6 +16,7 @@
 
 #include "../../include/strata_cuda.h"
 #include "kernels.h"
+#include "kv8.h"
 
 using namespace strata;
 
@@ -109,6 +110,7 @@ int check_device_errors(strata_ctx *ctx) {
     if (e & kErrRouting) what += "invalid expert routing result; ";
     if (e & kErrWaitTimeout) what += "a bounded device wait timed out; ";
     if (e & kErrPleScale) what += "Non-finite PLE scales; ";
+    if (e & kErrKvValue) what += "Non-finite key or value; ";
     return fail(ctx, STRATA_ERR_DEVICE, "device check failed: %s", what.c_str());
 }
 
@@ -404,6 +406,57 @@ int validate(strata_ctx *ctx, const char *name, const std::vector<Param> &params
 bool blob_geometry_ok(int width, int ff) { return width > 0 && ff > 0 && width % 64 == 0 && ff % 64 == 0; }
 long long blob_words_of(int width, int ff) { return 3LL * ff * width / 16 + 3LL * ff * width / 128; }
 
+// ---- 8-bit paged key/value cache: handles to the device view the kernels take
+int kv8_buffer(strata_ctx *ctx, const char *what, strata_buf h, long long need, void **out) {
+    Buffer *b = find(ctx, h);
+    if (!b) return fail(ctx, STRATA_ERR_HANDLE, "cache %s is not a live buffer", what);
+    if (need < 0 || (long long)b->length < need) return fail(ctx, STRATA_ERR_LAYOUT, "cache %s needs %lld elements, the buffer has %llu", what, need, (unsigned long long)b->length);
+    *out = b->ptr;
+    return STRATA_OK;
+}
+int kv8_view(strata_ctx *ctx, const strata_kv8_cache *cache, int segments, int count, strata_buf sequence, strata_buf start, Kv8 *c, Kv8Runs *r) {
+    if (!cache) return fail(ctx, STRATA_ERR_RANGE, "null cache");
+    char msg[256];
+    if (int e = kv8_check_cache(cache->kv_heads, cache->dim, cache->pages, cache->sequences, cache->blocks, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = kv8_check_runs(segments, count, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    *c = Kv8{};
+    c->kv_heads = cache->kv_heads;
+    c->dim = cache->dim;
+    c->padded = kv8_padded(cache->dim);
+    c->pages = cache->pages;
+    c->sequences = cache->sequences;
+    c->blocks = cache->blocks;
+    c->err = ctx->err_dev;
+    const long long heads = (long long)c->pages * c->kv_heads;  // below 2^43: the products fit 64 bits
+    void *p = nullptr;
+    if (int e = kv8_buffer(ctx, "codes", cache->codes, heads * 2 * c->padded * kKvBlock / 4, &p)) return e;
+    c->codes = (int8_t *)p;
+    if (int e = kv8_buffer(ctx, "marks", cache->marks, heads * 2 * c->padded / 4, &p)) return e;
+    c->marks = (int8_t *)p;
+    if (int e = kv8_buffer(ctx, "scales", cache->scales, heads * 2, &p)) return e;
+    c->scales = (float *)p;
+    if (int e = kv8_buffer(ctx, "open", cache->open, (long long)c->sequences * 2 * kKvBlock * c->kv_heads * c->dim, &p)) return e;
+    c->open = (float *)p;
+    if (int e = kv8_buffer(ctx, "table", cache->table, (long long)c->sequences * c->blocks, &p)) return e;
+    c->table = (const int *)p;
+    if (int e = kv8_buffer(ctx, "workspace", cache->workspace, STRATA_KV8_WORKSPACE_BYTES / 4, &p)) return e;
+    c->workspace = p;
+    *r = Kv8Runs{segments, count, nullptr, nullptr};
+    if (int e = kv8_buffer(ctx, "sequence", sequence, segments, &p)) return e;
+    r->sequence = (const int *)p;
+    if (int e = kv8_buffer(ctx, "start", start, segments, &p)) return e;
+    r->start = (const int *)p;
+    return use_device(ctx);
+}
+// `tokens` rows of `width` floats, `stride` apart (0: contiguous), inside a buffer.
+int kv8_rows(strata_ctx *ctx, const char *what, strata_buf h, uint64_t *stride, long long tokens, long long width, void **out) {
+    if (!*stride) *stride = (uint64_t)width;
+    char msg[256];
+    if (*stride > (1ull << 40)) return fail(ctx, STRATA_ERR_LAYOUT, "row_stride is out of range");  // tokens < 2^25: no overflow below
+    if (int e = kv8_check_stride((long long)*stride, width, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    return kv8_buffer(ctx, what, h, (tokens - 1) * (long long)*stride + width, out);
+}
+
 }  // namespace
 
 extern "C" {
@@ -654,6 +707,63 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
     cudaError_t e = ple_gather_decode((const unsigned *)t->ptr, (long long)t->length, (const int *)d->ptr, (long long)d->length, rows, head_dim,
                                       (float *)v->ptr, (long long)v->length, ctx->stream, ctx->err_dev);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_ple_gather_decode");
+    return STRATA_OK;
+}
+
+int strata_kv8_append(strata_ctx *ctx, const strata_kv8_cache *cache, strata_buf k, strata_buf v, uint64_t row_stride, int32_t segments,
+                      int32_t count, strata_buf sequence, strata_buf start) {
+    if (!ctx) return STRATA_ERR_RANGE;
+    Kv8 c;
+    Kv8Runs r;
+    if (int e = kv8_view(ctx, cache, segments, count, sequence, start, &c, &r)) return e;
+    void *pk = nullptr, *pv = nullptr;
+    const long long tokens = (long long)segments * count, width = (long long)c.kv_heads * c.dim;
+    if (int e = kv8_rows(ctx, "k", k, &row_stride, tokens, width, &pk)) return e;
+    if (int e = kv8_rows(ctx, "v", v, &row_stride, tokens, width, &pv)) return e;
+    cudaError_t e = kv8_append(c, (const float *)pk, (const float *)pv, (long long)row_stride, r, ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_kv8_append");
+    ++ctx->dispatches;
+    return STRATA_OK;
+}
+
+int strata_kv8_select(strata_ctx *ctx, const strata_kv8_cache *cache, strata_buf q, uint64_t row_stride, int32_t heads, int32_t segments,
+                      int32_t count, strata_buf sequence, strata_buf start, int32_t top, int32_t first, int32_t last, strata_buf picks) {
+    if (!ctx) return STRATA_ERR_RANGE;
+    Kv8 c;
+    Kv8Runs r;
+    if (int e = kv8_view(ctx, cache, segments, count, sequence, start, &c, &r)) return e;
+    char msg[256];
+    if (int e = kv8_check_heads(heads, c.kv_heads, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = kv8_check_select(c.blocks, top, first, last, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    void *pq = nullptr, *pp = nullptr;
+    const long long tokens = (long long)segments * count;
+    if (int e = kv8_rows(ctx, "q", q, &row_stride, tokens, (long long)heads * c.dim, &pq)) return e;
+    if (int e = kv8_buffer(ctx, "picks", picks, tokens * c.kv_heads * top, &pp)) return e;
+    cudaError_t e = kv8_select(c, (const float *)pq, (long long)row_stride, heads, r, top, first, last, (int *)pp, ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_kv8_select");
+    ++ctx->dispatches;
+    return STRATA_OK;
+}
+
+int strata_kv8_attend(strata_ctx *ctx, const strata_kv8_cache *cache, strata_buf q, uint64_t row_stride, int32_t heads, int32_t segments,
+                      int32_t count, strata_buf sequence, strata_buf start, strata_buf picks, int32_t top, float scale, strata_buf y) {
+    if (!ctx) return STRATA_ERR_RANGE;
+    Kv8 c;
+    Kv8Runs r;
+    if (int e = kv8_view(ctx, cache, segments, count, sequence, start, &c, &r)) return e;
+    char msg[256];
+    if (int e = kv8_check_heads(heads, c.kv_heads, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (picks && top < 1) return fail(ctx, STRATA_ERR_RANGE, "top must be an integer >= 1");
+    if (!std::isfinite(scale)) return fail(ctx, STRATA_ERR_RANGE, "scale must be finite");
+    void *pq = nullptr, *pp = nullptr, *py = nullptr;
+    const long long tokens = (long long)segments * count, width = (long long)heads * c.dim;
+    if (int e = kv8_rows(ctx, "q", q, &row_stride, tokens, width, &pq)) return e;
+    if (picks)
+        if (int e = kv8_buffer(ctx, "picks", picks, tokens * c.kv_heads * top, &pp)) return e;
+    if (int e = kv8_buffer(ctx, "y", y, tokens * width, &py)) return e;
+    cudaError_t e = kv8_attend(c, (const float *)pq, (long long)row_stride, heads, r, (const int *)pp, top, scale, (float *)py, ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_kv8_attend");
+    ++ctx->dispatches;
     return STRATA_OK;
 }
 

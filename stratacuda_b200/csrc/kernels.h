@@ -15,6 +15,7 @@ enum : unsigned {
     kErrWaitTimeout = 2u,  // a bounded spin-wait gave up
     kErrRouting = 4u,      // a routed expert id was invalid or repeated (src/engine.js:138)
     kErrPleScale = 8u,     // a gathered PLE row has a non-finite FP16 scale (src/model.js:241)
+    kErrKvValue = 16u,     // a key or value appended to an 8-bit cache is not finite
 };
 
 // One resolved argument of a reference-compatible dispatch: a device buffer (ptr, length in

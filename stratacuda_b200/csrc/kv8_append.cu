@@ -1,0 +1,147 @@
+// Appending rows to the 8-bit paged cache (strata_kv8_append).
+#include "kv8.cuh"
+
+namespace strata {
+namespace {
+
+constexpr int kThreads = 256;
+
+// One CTA: one kind (keys or values) of one head's block of one run. The block's rows, those that
+// the sequence already holds (from `open`) and the new ones, are read into registers, the largest
+// magnitude fixes the scale, the codes are laid out in shared memory as the page holds them and
+// copied out whole.
+template <int P>
+__global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const float *k, const float *v, long long stride, const Kv8Runs runs) {
+    constexpr int kTiles = P / 64;  // 4 tokens x 4 channels a tile, 16 * P / 4 tiles
+    __shared__ __align__(16) int8_t page_s[P * kKvBlock];
+    __shared__ float red[kThreads / 32];
+    __shared__ int lo_s[4][P / 4], hi_s[4][P / 4];
+    const int tid = threadIdx.x, head = blockIdx.y >> 1, kind = blockIdx.y & 1;
+    const RunAt a = run_at(c, runs, blockIdx.z);
+    if (a.sequence < 0) return;
+    if (a.start < 0) {
+        if (tid == 0) raise_error(c.err, kErrIndex);
+        return;
+    }
+    const long long cells = (long long)c.blocks * kKvBlock;
+    long long end = (long long)a.start + runs.count;
+    if (end > cells) {
+        if (tid == 0) raise_error(c.err, kErrIndex);
+        end = cells;
+    }
+    const int block = a.start / kKvBlock + blockIdx.x;
+    if ((long long)block * kKvBlock >= end) return;
+    const int r0 = blockIdx.x == 0 ? a.start % kKvBlock : 0;
+    const int r1 = (int)min((long long)kKvBlock, end - (long long)block * kKvBlock);
+    const int page = page_of(c, a.sequence, block);
+    const float *x = kind ? v : k;
+    const size_t open_row = (size_t)c.kv_heads * c.dim;
+    float *open = c.open + ((size_t)a.sequence * 2 + kind) * kKvBlock * open_row + (size_t)head * c.dim;
+    const long long first = (long long)blockIdx.z * runs.count + (long long)block * kKvBlock - a.start;  // input row of the block's row 0
+    const float *in = x + first * stride + (size_t)head * c.dim;
+
+    // this thread's tiles: neighbouring lanes take neighbouring channels of a key row, and
+    // neighbouring token groups of a value channel, so that each kind's packed words lie side by side
+    float xs[kTiles][4][4];
+    float amax = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+        const int w = i * kThreads + tid;
+        const int t4 = kind ? w & 15 : w / (P / 4), c4 = kind ? w >> 4 : w % (P / 4);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = t4 * 4 + t, ch = c4 * 4 + e;
+                float f = 0.0f;
+                if (row < r1 && ch < c.dim) f = row < r0 ? open[row * open_row + ch] : in[(long long)row * stride + ch];
+                if (!isfinite(f)) {
+                    bad = true;
+                    f = 0.0f;
+                }
+                xs[i][t][e] = f;
+                amax = fmaxf(amax, fabsf(f));
+            }
+    }
+    if (bad) raise_error(c.err, kErrKvValue);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
+    if (tid % 32 == 0) red[tid / 32] = amax;
+    __syncthreads();  // also: every read of `open` above is done
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) amax = fmaxf(amax, red[i]);
+    const float scale = amax < 0x1p-100f ? 0.0f : __fdiv_rn(amax, 127.0f);
+    const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+        const int w = i * kThreads + tid;
+        const int t4 = kind ? w & 15 : w / (P / 4), c4 = kind ? w >> 4 : w % (P / 4);
+        int q[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[t][e] = max(-127, min(127, __float2int_rn(__fmul_rn(xs[i][t][e], inv)))) & 255;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (kind)
+                *reinterpret_cast<int *>(page_s + (c4 * 4 + j) * kKvBlock + t4 * 4) = q[0][j] | q[1][j] << 8 | q[2][j] << 16 | q[3][j] << 24;
+            else
+                *reinterpret_cast<int *>(page_s + key_byte(t4 * 4 + j, c4 * 4)) = q[j][0] | q[j][1] << 8 | q[j][2] << 16 | q[j][3] << 24;
+        }
+    }
+    __syncthreads();
+    if (page >= 0) {
+        uint4 *dst = reinterpret_cast<uint4 *>(page_codes(c, page, head, kind));
+        for (int i = tid; i < P * kKvBlock / 16; i += kThreads) dst[i] = reinterpret_cast<const uint4 *>(page_s)[i];
+        if (tid == 0) page_scales(c, page, head)[kind] = scale;
+    }
+    if (!kind) {  // lowest and highest code of each channel over the rows there are
+        for (int w = tid; w < P; w += kThreads) {
+            const int quarter = w / (P / 4), c4 = w % (P / 4);
+            int lo = 0x7f7f7f7f, hi = (int)0x81818181u;
+            for (int t = quarter * 16; t < min(r1, quarter * 16 + 16); ++t) {
+                const int codes = *reinterpret_cast<const int *>(page_s + key_byte(t, c4 * 4));
+                lo = __vmins4(lo, codes);
+                hi = __vmaxs4(hi, codes);
+            }
+            lo_s[quarter][c4] = lo;
+            hi_s[quarter][c4] = hi;
+        }
+        __syncthreads();
+        if (page >= 0 && tid < P / 4) {
+            int lo = lo_s[0][tid], hi = hi_s[0][tid];
+            for (int i = 1; i < 4; ++i) {
+                lo = __vmins4(lo, lo_s[i][tid]);
+                hi = __vmaxs4(hi, hi_s[i][tid]);
+            }
+            int8_t *m = page_marks(c, page, head);
+            reinterpret_cast<int *>(m)[tid] = lo;
+            reinterpret_cast<int *>(m + P)[tid] = hi;
+        }
+    }
+    // the run's last block keeps its new rows in 32 bits while it is unfilled. The first block's
+    // CTA writes them, after its own reads: it is the only one that reads this head's open rows.
+    if (blockIdx.x == 0 && end % kKvBlock) {
+        const int last = (int)(end / kKvBlock), rows = (int)(end % kKvBlock);
+        const int from = last == block ? r0 : 0;
+        const float *src = x + ((long long)blockIdx.z * runs.count + (long long)last * kKvBlock - a.start) * stride + (size_t)head * c.dim;
+        for (int i = tid; i < (rows - from) * c.dim; i += kThreads) {
+            const int row = from + i / c.dim, ch = i % c.dim;
+            const float f = src[(long long)row * stride + ch];
+            open[row * open_row + ch] = isfinite(f) ? f : 0.0f;
+        }
+    }
+}
+
+}  // namespace
+
+cudaError_t kv8_append(const Kv8 &c, const float *k, const float *v, long long stride, const Kv8Runs &r, cudaStream_t s) {
+    const dim3 grid((r.count + kKvBlock - 2) / kKvBlock + 1, c.kv_heads * 2, r.segments);
+    if (c.padded == 64) k_kv8_append<64><<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
+    else if (c.padded == 128) k_kv8_append<128><<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
+    else k_kv8_append<256><<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
+    return cudaGetLastError();
+}
+
+}  // namespace strata

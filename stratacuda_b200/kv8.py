@@ -1,0 +1,142 @@
+"""Attention over a paged key/value cache held in 8 bits (include/strata_cuda.h, strata_kv8_*).
+
+The reference keeps F32 caches of at most 2048 cells (src/model.js:13). Here a cache holds one byte
+per value with a scale for each block of 64 tokens and head, in pages that sequences take from one
+pool, so that sessions can be longer and more of them fit. Three operators work on it:
+
+* ``append`` — quantise new key and value rows into the sequences' pages;
+* ``select`` — choose, for each token and key/value head, the blocks with the largest bound on the
+  logits, from two 8-bit marks per block and channel;
+* ``attend`` — softmax attention over all blocks or over the chosen ones, F32 in and out, for single
+  tokens of many sequences and for prompt chunks.
+
+``Kv8Cache`` owns its buffers on a CudaBackend and works on its stream. ``DeviceCache`` is a view of
+caller-owned device memory (torch tensors, or plain addresses) on a stream of the caller's.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+
+from . import _lib as L
+from .backend import StrataError, StrataRangeError
+
+BLOCK = L.KV8_BLOCK
+
+
+def padded(dim: int) -> int:
+    """Channels that a page stores for heads of `dim`."""
+    return 64 if dim <= 64 else 128 if dim <= 128 else 256
+
+
+def sizes(kv_heads: int, dim: int, pages: int, sequences: int, blocks: int) -> dict:
+    """Elements of a cache's parts: codes and marks in bytes, the others in 4-byte elements."""
+    p = padded(dim)
+    return dict(codes=pages * kv_heads * 2 * p * BLOCK, marks=pages * kv_heads * 2 * p, scales=pages * kv_heads * 2,
+                open=sequences * 2 * BLOCK * kv_heads * dim, table=sequences * blocks, workspace=L.KV8_WORKSPACE_BYTES // 4)
+
+
+class Kv8Cache:
+    """One layer's cache on a CudaBackend. `pages` defaults to a page for every block of every
+    sequence, in order; with fewer, the caller hands pages out with ``write_table``."""
+
+    def __init__(self, backend, kv_heads: int, dim: int, sequences: int, blocks: int, pages: int | None = None, workspace=None):
+        self.b = backend
+        self.kv_heads, self.dim, self.sequences, self.blocks = kv_heads, dim, sequences, blocks
+        self.pages = sequences * blocks if pages is None else pages
+        n = sizes(kv_heads, dim, self.pages, sequences, blocks)
+        self._owned = []
+
+        def keep(length, type="f32"):
+            buf = backend.alloc(length, type, zero=True)
+            self._owned.append(buf)
+            return buf
+
+        self.codes, self.marks = keep(n["codes"] // 4, "u32"), keep(n["marks"] // 4, "u32")
+        self.scales, self.open, self.table = keep(n["scales"]), keep(n["open"]), keep(n["table"], "i32")
+        # caches whose calls follow one another on the backend's stream may share one workspace
+        self.workspace = keep(n["workspace"], "u32") if workspace is None else workspace
+        if pages is None:
+            self.write_table(np.arange(self.pages, dtype=np.int32).reshape(sequences, blocks))
+        else:
+            self.write_table(np.full((sequences, blocks), -1, np.int32))
+
+    def write_table(self, table) -> None:
+        """The page of every block of every sequence, int [sequences][blocks]; -1 where there is none yet."""
+        table = np.ascontiguousarray(table, np.int32)
+        if table.shape != (self.sequences, self.blocks):
+            raise StrataError(L.ERR_LAYOUT, f"the page table is [{self.sequences}][{self.blocks}]")
+        self.b.write(self.table, table.ravel())
+
+    def _struct(self) -> L.StrataKv8Cache:
+        return L.StrataKv8Cache(self.kv_heads, self.dim, self.pages, self.sequences, self.blocks, self.codes.handle, self.marks.handle,
+                                self.scales.handle, self.open.handle, self.table.handle, self.workspace.handle)
+
+    def append(self, k, v, sequence, start, segments: int = 1, count: int = 1, row_stride: int = 0) -> None:
+        """Append rows k and v [segments * count][kv_heads * dim] (strata_kv8_append)."""
+        self.b._check(self.b.lib.strata_kv8_append(self.b.ctx, C.byref(self._struct()), k.handle, v.handle, row_stride, segments, count,
+                                                   sequence.handle, start.handle))
+
+    def select(self, q, heads: int, picks, sequence, start, segments: int = 1, count: int = 1, top: int = 32, first: int = 1, last: int = 2,
+               row_stride: int = 0) -> None:
+        """picks [segments * count][kv_heads][top] (i32): the chosen blocks (strata_kv8_select)."""
+        self.b._check(self.b.lib.strata_kv8_select(self.b.ctx, C.byref(self._struct()), q.handle, row_stride, heads, segments, count,
+                                                   sequence.handle, start.handle, top, first, last, picks.handle))
+
+    def attend(self, q, heads: int, y, sequence, start, segments: int = 1, count: int = 1, picks=None, top: int = 0,
+               scale: float | None = None, row_stride: int = 0) -> None:
+        """y [segments * count][heads * dim]: attention over all blocks, or those in `picks` (strata_kv8_attend).
+        `scale` defaults to 1 / sqrt(dim)."""
+        self.b._check(self.b.lib.strata_kv8_attend(self.b.ctx, C.byref(self._struct()), q.handle, row_stride, heads, segments, count,
+                                                   sequence.handle, start.handle, 0 if picks is None else picks.handle, top,
+                                                   1 / math.sqrt(self.dim) if scale is None else scale, y.handle))
+
+    def free(self) -> None:
+        for buf in self._owned:
+            self.b.free(buf)
+        self._owned = []
+
+
+def _address(x):
+    if x is None or isinstance(x, int):
+        return x
+    ptr = getattr(x, "data_ptr", None)
+    return ptr() if ptr is not None else x.device_ptr
+
+
+class DeviceCache:
+    """A cache in caller-owned device memory: torch tensors, Buffers or addresses of the layouts in
+    include/strata_cuda.h. Calls go to `stream` (a cudaStream_t as an integer; 0 is the default
+    stream) of the current device, allocate nothing and do not synchronise. `status`, where given, is
+    a zeroed 32-bit device word that device-side errors are added to. The parts must stay alive."""
+
+    def __init__(self, kv_heads: int, dim: int, pages: int, sequences: int, blocks: int, codes, marks, scales, open, table, workspace,
+                 status=None):
+        self.lib = L.load()
+        self.kv_heads, self.dim = kv_heads, dim
+        self.parts = (codes, marks, scales, open, table, workspace, status)
+        self._cache = L.StrataKv8CacheDev(kv_heads, dim, pages, sequences, blocks, *[_address(x) for x in self.parts])
+        self._ref = C.byref(self._cache)
+        self._msg = C.create_string_buffer(256)
+        self._scale = 1 / math.sqrt(dim) if dim > 0 else 0.0
+
+    def _check(self, rc: int) -> None:
+        if rc != L.OK:
+            raise (StrataRangeError if rc == L.ERR_RANGE else StrataError)(rc, self._msg.value.decode(errors="replace"))
+
+    def append(self, k, v, sequence, start, segments: int = 1, count: int = 1, row_stride: int = 0, stream: int = 0) -> None:
+        self._check(self.lib.strata_kv8_append_dev(self._ref, _address(k), _address(v), row_stride, segments, count, _address(sequence),
+                                                   _address(start), stream, self._msg, 256))
+
+    def select(self, q, heads: int, picks, sequence, start, segments: int = 1, count: int = 1, top: int = 32, first: int = 1, last: int = 2,
+               row_stride: int = 0, stream: int = 0) -> None:
+        self._check(self.lib.strata_kv8_select_dev(self._ref, _address(q), row_stride, heads, segments, count, _address(sequence),
+                                                   _address(start), top, first, last, _address(picks), stream, self._msg, 256))
+
+    def attend(self, q, heads: int, y, sequence, start, segments: int = 1, count: int = 1, picks=None, top: int = 0,
+               scale: float | None = None, row_stride: int = 0, stream: int = 0) -> None:
+        self._check(self.lib.strata_kv8_attend_dev(self._ref, _address(q), row_stride, heads, segments, count, _address(sequence),
+                                                   _address(start), _address(picks), top, self._scale if scale is None else scale,
+                                                   _address(y), stream, self._msg, 256))
