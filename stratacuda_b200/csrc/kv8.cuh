@@ -3,6 +3,8 @@
 #include "common.cuh"
 #include "kv8.h"
 
+#include <cuda_fp16.h>
+
 namespace strata {
 
 // A run's sequence and first position, or sequence -1 for an idle slot (a sequence outside the
@@ -42,5 +44,28 @@ __device__ __forceinline__ int8_t *page_marks(const Kv8 &c, int page, int head) 
 __device__ __forceinline__ float *page_scales(const Kv8 &c, int page, int head) { return c.scales + ((size_t)page * c.kv_heads + head) * 2; }
 // Byte of key channel ch of token t in a page: panels of 64 channels, token rows of 64 bytes.
 __device__ __forceinline__ int key_byte(int t, int ch) { return ((ch >> 6) * kKvBlock + t) * 64 + (ch & 63); }
+
+// Four signed codes as two FP16 pairs: the bits 0x6400 | (c + 128) are 1152 + c, less 1152 is c, exactly.
+__device__ __forceinline__ void codes_to_half(unsigned w, unsigned &b0, unsigned &b1) {
+    const unsigned u = w ^ 0x80808080u, k1152 = 0x64806480u;
+    const unsigned p0 = __byte_perm(u, 0x64646464u, 0x4140), p1 = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 k = *reinterpret_cast<const __half2 *>(&k1152);
+    const __half2 h0 = __hsub2(*reinterpret_cast<const __half2 *>(&p0), k), h1 = __hsub2(*reinterpret_cast<const __half2 *>(&p1), k);
+    b0 = *reinterpret_cast<const unsigned *>(&h0);
+    b1 = *reinterpret_cast<const unsigned *>(&h1);
+}
+// a pair of floats as FP16 halves: x = hi + lo to 2^-22 of x (2^-25 absolute for small x)
+__device__ __forceinline__ void split_pair(float x, float y, unsigned &hi, unsigned &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const unsigned *>(&h);
+    lo = *reinterpret_cast<const unsigned *>(&l);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 }  // namespace strata

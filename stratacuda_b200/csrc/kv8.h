@@ -46,5 +46,8 @@ cudaError_t kv8_select(const Kv8 &c, const float *q, long long stride, int heads
 // picks null: every block. `scale` multiplies q . k.
 cudaError_t kv8_attend(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, const int *picks, int top, float scale,
                        float *y, cudaStream_t s);
+// The same for many tokens a run, every block: 128-row tiles (kv8_prompt.cu), taken by kv8_attend.
+cudaError_t kv8_attend_prompt(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, float scale, float *y,
+                              cudaStream_t s);
 
 }  // namespace strata

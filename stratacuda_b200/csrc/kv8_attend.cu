@@ -20,8 +20,6 @@
 // second kernel joins them in CTA order, so results repeat bit for bit.
 #include "kv8.cuh"
 
-#include <cuda_fp16.h>
-
 #include <atomic>
 #include <cmath>
 
@@ -116,29 +114,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsig
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Four signed codes as two FP16 pairs: the bits 0x6400 | (c + 128) are 1152 + c, less 1152 is c, exactly.
-__device__ __forceinline__ void codes_to_half(unsigned w, unsigned &b0, unsigned &b1) {
-    const unsigned u = w ^ 0x80808080u, k1152 = 0x64806480u;
-    const unsigned p0 = __byte_perm(u, 0x64646464u, 0x4140), p1 = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 k = *reinterpret_cast<const __half2 *>(&k1152);
-    const __half2 h0 = __hsub2(*reinterpret_cast<const __half2 *>(&p0), k), h1 = __hsub2(*reinterpret_cast<const __half2 *>(&p1), k);
-    b0 = *reinterpret_cast<const unsigned *>(&h0);
-    b1 = *reinterpret_cast<const unsigned *>(&h1);
-}
-// a pair of floats as FP16 halves: x = hi + lo to 2^-22 of x (2^-25 absolute for small x)
-__device__ __forceinline__ void split_pair(float x, float y, unsigned &hi, unsigned &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const unsigned *>(&h);
-    lo = *reinterpret_cast<const unsigned *>(&l);
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 // Entries of a token's page list: every block in sight, or its picks.
 __device__ __forceinline__ int entries(const Args &A, int token, int *sequence, int *seen) {
     const RunAt at = run_at(A.c, A.runs, token / A.runs.count);
@@ -561,6 +536,7 @@ cudaError_t launch(Args A, cudaStream_t s) {
 cudaError_t kv8_attend(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, const int *picks, int top, float scale,
                        float *y, cudaStream_t s) {
     const int group = heads / c.kv_heads;
+    if (!picks && r.count > 1 && (long long)r.count * group >= 64) return kv8_attend_prompt(c, q, stride, heads, r, scale, y, s);
     const Args A{c, q, stride, heads, group, (group + kRows - 1) / kRows, r, picks, top, scale * 1.4426950408889634f, y, 0};
     if (c.padded == 64) return launch<64>(A, s);
     if (c.padded == 128) return launch<128>(A, s);

@@ -1,0 +1,665 @@
+// Attention over the 8-bit paged cache for prompt chunks (strata_kv8_attend, many tokens a run): tiles of
+// 128 query rows on the 5th-generation tensor cores (tcgen05 + TMEM).
+//
+// A tile is 128 consecutive (token, query head) pairs of one run and key/value head, so that groups of any
+// size fill it. Its keys and values pass by page by page (64 tokens):
+//   S[128][64] = Q K^T     Q as two FP16 halves in shared memory, the codes converted to FP16 (exact)
+//   O[128][P] += W V       the weights as two FP16 halves in TMEM, the A operand of the second product
+// Both products run twice, for the high and the low half, which gives F32's accuracy at half of the FP16
+// rate. Accumulators, maxima and sums are F32.
+//
+// Warps:
+//   0-3  softmax: a thread owns one row (its TMEM lane): logits from S, running maximum and sum,
+//        weights back into the TMEM columns of S. O is rescaled only when a row's maximum has grown by more than
+//        2^5 (weights are kept times 2^10, so that both ends stay inside FP16), so seldom after the
+//        first pages
+//   4-7  converters: 8-bit codes from global memory (the next item's loads in flight) to FP16 in the
+//        128-byte-swizzled layout of the MMA operands; keys and values alternate through one ring of slots
+//   8    one thread issues the MMAs: S of page j + 1 before O of page j, so that the softmax of
+//        a page runs under the products of its neighbours
+// A value scale cannot be applied after the product, since pages add up in one accumulator: weights are
+// multiplied by scale / (largest scale of the tile's pages).
+//
+// Every wait is bounded; past the limit all roles leave and the error word is set.
+#include "kv8.cuh"
+#include "pf_gemm.cuh"
+
+#include <atomic>
+#include <cmath>
+
+namespace strata {
+namespace {
+
+using namespace pf;
+
+constexpr int kPromptThreads = 288;
+constexpr int kTileRows = 128;
+constexpr int kBufs = 4;             // S / weight buffers in TMEM, 64 columns each
+constexpr float kLiftP = 10.0f;      // weights are stored times 2^10
+constexpr float kGrow = 5.0f;        // growth of a maximum (log2) that O's scale bears
+constexpr long long kLimit = 2000000000;  // clocks, about a second
+
+constexpr int kFlush = 16;           // pages that add up in TMEM before the sum moves to 32-bit adds
+constexpr int kMaxGrid = 160;        // CTAs, each with a slot in the workspace
+constexpr int kMaxPairs = 1024;      // (run, tile) pairs of a split call
+constexpr int kMaxUnits = 65536;
+
+template <int P>
+struct __align__(1024) PromptSmem {
+    static constexpr int slots = P == 256 ? 3 : 6;
+    unsigned char q[2][P / 64][kTileRows * 128];  // high and low halves: panels of 64 channels, rows of 128 bytes, swizzled
+    unsigned char slot[slots][P * 128];           // keys [P / 64][64 tokens][128 bytes] or values [P channels][128 bytes], swizzled
+    float row_scale[kTileRows];
+    float red[9];
+    unsigned long long full[slots], empty[slots], s_full[kBufs], w_full[kBufs], o_done[kBufs], o_free, drained;
+    unsigned tmem;
+    int abort_flag;
+};
+
+struct PromptArgs {
+    Kv8 c;
+    const float *q;
+    long long stride;
+    int heads, group, tiles;  // tiles of 128 rows a run and key/value head
+    Kv8Runs runs;
+    float scale;  // times log2 e
+    float *y;
+    int split;
+};
+// Workspace: a CTA's sum of more than kFlush pages, or of the part of a unit that an earlier CTA began,
+// as [P / 4][128 rows] float4; per row maximum, sum and value scale of such a part and of a begun one (whose sum is
+// in y); the CTAs that share a unit.
+struct PromptParts {
+    float4 *sum;      // [kMaxGrid][P / 4][128]
+    float4 *tail_ml;  // [kMaxGrid][128]
+    float4 *head_ml;  // [kMaxGrid][128]
+    int2 *cover;      // [units]
+};
+__host__ __device__ inline PromptParts prompt_parts(void *ws, int P) {
+    char *p = static_cast<char *>(ws);
+    PromptParts r;
+    r.sum = reinterpret_cast<float4 *>(p);
+    p += (size_t)kMaxGrid * P * kTileRows * 4;
+    r.tail_ml = reinterpret_cast<float4 *>(p);
+    p += (size_t)kMaxGrid * kTileRows * 16;
+    r.head_ml = reinterpret_cast<float4 *>(p);
+    p += (size_t)kMaxGrid * kTileRows * 16;
+    r.cover = reinterpret_cast<int2 *>(p);
+    return r;
+}
+static_assert((size_t)kMaxGrid * (256 * kTileRows * 4 + 2 * kTileRows * 16) + (size_t)kMaxUnits * 8 <= (32u << 20), "fits the workspace");
+
+// Pages that a tile of a run attends to: those of its last row.
+__device__ __forceinline__ int pair_pages(const PromptArgs &A, int run, int tile) {
+    const int last = min(A.runs.count * A.group, (tile + 1) * kTileRows) - 1;
+    return (visible_keys(A.c, run_at(A.c, A.runs, run), last / A.group) + kKvBlock - 1) / kKvBlock;
+}
+__device__ __forceinline__ float *prompt_row(const PromptArgs &A, int run, int head, int r) {
+    return A.y + (((size_t)run * A.runs.count + r / A.group) * A.heads + head * A.group + r % A.group) * A.c.dim;
+}
+
+// 32 TMEM columns of this thread's lane, without the wait.
+__device__ __forceinline__ void tmem_ld32_async(unsigned taddr, unsigned (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// 16 of them.
+__device__ __forceinline__ void tmem_ld16_async(unsigned taddr, unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+struct Piece {
+    int run, tile, head;
+    int first, stop, n;  // pages [first, stop) of the unit's n
+};
+
+template <int P>
+__global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_constant__ PromptArgs A) {
+    using Sm = PromptSmem<P>;
+    extern __shared__ unsigned char raw[];
+    Sm &M = *reinterpret_cast<Sm *>(raw + ((1024 - (su32(raw) & 1023)) & 1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int pairs = A.runs.segments * A.tiles;
+    const PromptParts W = prompt_parts(A.c.workspace, P);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- this CTA's work: units (pair, head) blockIdx.x, + gridDim.x, ... or pages [work, work_end) of all units' list
+    long long unit = blockIdx.x, work = 0, work_end = 0, chunk = 1;
+    int at_pair = 0, at_head = 0, at_page = 0;
+    if (A.split) {
+        long long *before = reinterpret_cast<long long *>(M.slot[0]);  // used before the ring is
+        long long *part = before + kMaxPairs + 1;
+        static_assert(sizeof(M.slot) >= (kMaxPairs + 1 + 9) * 8, "the page counts fit");
+        for (int base = 0; base < pairs; base += 256) {  // before[i]: a head's pages before pair i
+            long long sum = tid < 256 && base + tid < pairs ? pair_pages(A, (base + tid) / A.tiles, (base + tid) % A.tiles) : 0;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const long long o = __shfl_up_sync(0xffffffffu, sum, s);
+                if (lane >= s) sum += o;
+            }
+            if (lane == 31) part[warp] = sum;
+            __syncthreads();
+            long long carry = base ? before[base] : 0;
+            for (int w = 0; w < warp; ++w) carry += part[w];
+            if (base == 0 && tid == 0) before[0] = 0;
+            if (tid < 256 && base + tid < pairs) before[base + tid + 1] = carry + sum;
+            __syncthreads();
+        }
+        const long long total = before[pairs] * A.c.kv_heads;
+        chunk = (total + gridDim.x - 1) / gridDim.x;
+        work = chunk * blockIdx.x;
+        work_end = min(total, work + chunk);
+        if (work >= work_end) return;
+        int lo = 0, hi = pairs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (before[mid + 1] * A.c.kv_heads > work) hi = mid;
+            else lo = mid + 1;
+        }
+        const long long n = before[lo + 1] - before[lo], in = work - before[lo] * A.c.kv_heads;
+        at_pair = lo;
+        at_head = (int)(in / n);
+        at_page = (int)(in % n);
+    }
+    if (tid == 0) {
+        for (int i = 0; i < Sm::slots; ++i) {
+            bar_init(&M.full[i], 128);
+            bar_init(&M.empty[i], 1);
+        }
+        for (int i = 0; i < kBufs; ++i) {
+            bar_init(&M.s_full[i], 1);
+            bar_init(&M.w_full[i], 128);
+            bar_init(&M.o_done[i], 1);
+        }
+        bar_init(&M.o_free, 128);
+        bar_init(&M.drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        M.abort_flag = 0;
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&M.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = M.tmem;
+    auto wait = [&](unsigned long long *b, unsigned parity) -> bool {
+        for (const long long began = clock64();;) {
+            if (bar_try(b, parity)) return true;
+            if (*(volatile int *)&M.abort_flag) return false;
+            if (clock64() - began > kLimit) {
+                atomicOr(&M.abort_flag, 1);
+                return false;
+            }
+        }
+    };
+
+    // The next piece of the CTA's work. The part of a unit that an earlier CTA began comes last: its sum stays
+    // in the CTA's workspace slot, which the other pieces use in passing.
+    Piece tail{0, 0, 0, 0, 0, 0};
+    bool has_tail = false;
+    auto next = [&](Piece &p) -> bool {
+        if (!A.split) {
+            if (unit >= (long long)pairs * A.c.kv_heads) return false;
+            const int a_tile = A.runs.segments * A.c.kv_heads, rest = (int)(unit % a_tile);  // the tiles with the most keys first
+            p.tile = A.tiles - 1 - (int)(unit / a_tile);
+            p.run = rest / A.c.kv_heads;
+            p.head = rest % A.c.kv_heads;
+            p.first = 0;
+            p.n = p.stop = pair_pages(A, p.run, p.tile);
+            unit += gridDim.x;
+            return true;
+        }
+        while (work < work_end) {
+            p.run = at_pair / A.tiles;
+            p.tile = at_pair % A.tiles;
+            p.head = at_head;
+            p.n = pair_pages(A, p.run, p.tile);
+            if (p.n == 0) {  // nothing in sight: the joining kernel writes the zeros
+                ++at_pair;
+                continue;
+            }
+            p.first = at_page;
+            p.stop = (int)min((long long)p.n, at_page + (work_end - work));
+            if (at_page == 0 && tid == 0)
+                W.cover[at_pair * A.c.kv_heads + at_head] = make_int2(blockIdx.x, (int)((work + p.n - 1) / chunk));
+            work += p.stop - p.first;
+            at_page = 0;
+            if (++at_head == A.c.kv_heads) {
+                at_head = 0;
+                ++at_pair;
+            }
+            if (p.first == 0) return true;
+            tail = p;
+            has_tail = true;
+        }
+        if (!has_tail) return false;
+        p = tail;
+        has_tail = false;
+        return true;
+    };
+
+    // counters that go on from piece to piece: pages (S buffers), ring items, flushes
+    int pages = 0, used = 0, flushes = 0;
+    Piece p;
+    while (next(p)) {
+        const RunAt at = run_at(A.c, A.runs, p.run);
+        const int row0 = p.tile * kTileRows, rows = min(kTileRows, A.runs.count * A.group - row0), n = p.stop - p.first, head = p.head;
+        if (n == 0) {  // no row of the tile sees a key
+            for (int i = tid; i < rows * A.c.dim; i += kPromptThreads) prompt_row(A, p.run, head, row0 + i / A.c.dim)[i % A.c.dim] = 0.0f;
+            continue;
+        }
+        auto page_at = [&](int j) { return page_of(A.c, at.sequence, p.first + j); };
+        // queries: a row is P / 8 lanes of 8 channels; scaled by a power of two to 2^9 .. 2^10 at most
+        if (warp < 8) {
+            constexpr int kLanes = P / 8, kAtOnce = 32 / kLanes;
+            const int l = lane % kLanes, ch0 = 8 * l;
+            for (int i = warp * kAtOnce + lane / kLanes; i < kTileRows; i += 8 * kAtOnce) {
+                float x[8], big = 0.0f;
+                const int r = row0 + i;
+                const float *src = A.q + (p.run * (long long)A.runs.count + r / A.group) * A.stride + (size_t)(head * A.group + r % A.group) * A.c.dim + ch0;
+                if (i < rows && ch0 + 8 <= A.c.dim && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                    const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
+                    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = i < rows && ch0 + k < A.c.dim ? src[k] : 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(x[k]));
+#pragma unroll
+                for (int s = kLanes / 2; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+                const unsigned field = min(263u - (__float_as_uint(big) >> 23), 253u);
+                const float up = __uint_as_float(field << 23);
+                if (l == 0) M.row_scale[i] = __uint_as_float((254u - field) << 23) * A.scale;
+                uint4 hi, lo;
+                split_pair(x[0] * up, x[1] * up, hi.x, lo.x);
+                split_pair(x[2] * up, x[3] * up, hi.y, lo.y);
+                split_pair(x[4] * up, x[5] * up, hi.z, lo.z);
+                split_pair(x[6] * up, x[7] * up, hi.w, lo.w);
+                const int where = i * 128 + (((l & 7) ^ (i & 7)) << 4);
+                *reinterpret_cast<uint4 *>(M.q[0][l >> 3] + where) = hi;
+                *reinterpret_cast<uint4 *>(M.q[1][l >> 3] + where) = lo;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        // the largest value scale of the unit's pages
+        float most = 0.0f;
+        for (int j = tid; j < p.n; j += kPromptThreads) {
+            const int page = page_of(A.c, at.sequence, j);
+            if (page >= 0) most = fmaxf(most, page_scales(A.c, page, head)[1]);
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+        if (lane == 0) M.red[warp] = most;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 9; ++i) most = fmaxf(most, M.red[i]);
+
+        if (warp < 4) {
+            // ---------------------------------------------------------------- softmax
+            const int i = warp * 32 + lane;
+            const int seen = i < rows ? visible_keys(A.c, at, (row0 + i) / A.group) - p.first * kKvBlock : 0;
+            const unsigned mine = tmem + ((unsigned)(warp * 32) << 16);
+            const float row_scale = M.row_scale[i], over = most > 0.0f ? __fdiv_rn(1.0f, most) : 0.0f;
+            float4 *kept = W.sum + (size_t)blockIdx.x * (P / 4) * kTileRows + i;  // this row's sum of flushed pages, every 128th
+            float m = -INFINITY, sum = 0.0f, kept_m = -INFINITY;
+            bool ok = true;
+            auto scales_of = [&](int j) {
+                const int page = page_at(j);
+                const float *s = page >= 0 ? page_scales(A.c, page, head) : nullptr;
+                return s ? make_float2(s[0], s[1]) : make_float2(-1.0f, 0.0f);  // -1: no page
+            };
+            // O of local page j's group, complete, joins the kept sum
+            auto flush = [&](int j) -> bool {
+                const int g = pages + j;
+                if (!__all_sync(0xffffffffu, wait(&M.o_done[g % kBufs], g / kBufs & 1))) return false;
+                tc_fence_after();
+                const bool fresh = j < kFlush;
+                const float alpha = fresh || kept_m >= m ? 1.0f : exp2_fast(kept_m - m);
+                kept_m = m;
+#pragma unroll 1
+                for (int k = 0; k < P; k += 16) {
+                    unsigned x[16];
+                    float4 f[4];
+                    tmem_ld16_async(mine + k, x);
+                    if (!fresh) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] = kept[(k / 4 + e) * kTileRows];
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float4 o = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
+                                               __uint_as_float(x[4 * e + 3]));
+                        if (!fresh) o = make_float4(f[e].x * alpha + o.x, f[e].y * alpha + o.y, f[e].z * alpha + o.z, f[e].w * alpha + o.w);
+                        kept[(k / 4 + e) * kTileRows] = o;
+                    }
+                }
+                tc_fence_before();
+                bar_arrive(&M.o_free);
+                return true;
+            };
+            float2 sc = scales_of(0);
+            for (int j = 0; j < n; ++j) {
+                const int g = pages + j, buf = g % kBufs;
+                const unsigned cols = mine + P + 64 * buf;
+                const int left = sc.x >= 0.0f ? seen - j * kKvBlock : 0;
+                const float c = sc.x * row_scale, fv = sc.y * over;
+                if (j + 1 < n) sc = scales_of(j + 1);  // under this page's work
+                if (!(ok = __all_sync(0xffffffffu, wait(&M.s_full[buf], g / kBufs & 1)))) break;
+                tc_fence_after();
+                float a[64];
+#pragma unroll
+                for (int k = 0; k < 64; k += 32) {
+                    unsigned x[32];
+                    tmem_ld32_async(cols + k, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) a[k + e] = __uint_as_float(x[e]) * c;
+                }
+                if (__any_sync(0xffffffffu, left < kKvBlock)) {
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) a[k] = k < left ? a[k] : -INFINITY;
+                }
+                float big[4] = {a[0], a[1], a[2], a[3]};
+#pragma unroll
+                for (int k = 4; k < 64; ++k) big[k & 3] = fmaxf(big[k & 3], a[k]);
+                const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+                bool due = j > 0 && j % kFlush == 0;  // the group of pages before this one is to be kept
+                if (__any_sync(0xffffffffu, top > m + kGrow)) {
+                    if (due) {
+                        if (!(ok = flush(j - 1))) break;
+                        due = false;
+                    }
+                    const float now = fmaxf(m, top), alpha = now > m ? exp2_fast(m - now) : 1.0f;
+                    m = now;
+                    sum *= alpha;
+                    if (j % kFlush) {
+                        if (!(ok = __all_sync(0xffffffffu, wait(&M.o_done[(g - 1) % kBufs], (g - 1) / kBufs & 1)))) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int k = 0; k < P; k += 16) {
+                            unsigned x[16];
+                            tmem_ld16_async(mine + k, x);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+                            tmem_st16(mine + k, x);
+                        }
+                    }
+                }
+                const float from = (m == -INFINITY ? 0.0f : m) - kLiftP;
+                float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {  // 32 weights to 16 columns of high and 16 of low halves
+                    unsigned hi[16], lo[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float p0 = exp2_fast(a[16 * k + 2 * e] - from), p1 = exp2_fast(a[16 * k + 2 * e + 1] - from);
+                        add[(2 * e) & 3] += p0;
+                        add[(2 * e + 1) & 3] += p1;
+                        split_pair(p0 * fv, p1 * fv, hi[e], lo[e]);
+                    }
+                    tmem_st16(cols + 8 * k, hi);
+                    tmem_st16(cols + 32 + 8 * k, lo);
+                }
+                sum += (add[0] + add[1]) + (add[2] + add[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                bar_arrive(&M.w_full[buf]);
+                if (due && !(ok = flush(j - 1))) break;
+            }
+            const int g = pages + n - 1;
+            if (ok && (ok = __all_sync(0xffffffffu, wait(&M.o_done[g % kBufs], g / kBufs & 1)))) {
+                tc_fence_after();
+                const bool whole = n == p.n, flushed = n > kFlush;
+                const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum), by = whole ? most : 1.0f;
+                const float alpha = !flushed || kept_m >= m ? 1.0f : exp2_fast(kept_m - m);
+                float *dst = i < rows ? prompt_row(A, p.run, head, row0 + i) : nullptr;
+                const bool wide = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+                if (!whole) (p.first ? W.tail_ml : W.head_ml)[blockIdx.x * kTileRows + i] = make_float4(m, sum, most, 0.0f);
+#pragma unroll 1
+                for (int k = 0; k < P; k += 32) {
+                    unsigned x[32];
+                    float4 f[8];
+                    __syncwarp();
+                    tmem_ld32_async(mine + k, x);
+                    if (flushed) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = kept[(k / 4 + e) * kTileRows];
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float4 o = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
+                                               __uint_as_float(x[4 * e + 3]));
+                        if (flushed) o = make_float4(f[e].x * alpha + o.x, f[e].y * alpha + o.y, f[e].z * alpha + o.z, f[e].w * alpha + o.w);
+                        if (p.first) {
+                            kept[(k / 4 + e) * kTileRows] = o;
+                        } else if (dst) {
+                            const int ch = k + 4 * e;
+                            o = make_float4(o.x * inv * by, o.y * inv * by, o.z * inv * by, o.w * inv * by);
+                            if (wide && ch + 4 <= A.c.dim) {
+                                *reinterpret_cast<float4 *>(dst + ch) = o;
+                            } else {
+                                if (ch < A.c.dim) dst[ch] = o.x;
+                                if (ch + 1 < A.c.dim) dst[ch + 1] = o.y;
+                                if (ch + 2 < A.c.dim) dst[ch + 2] = o.z;
+                                if (ch + 3 < A.c.dim) dst[ch + 3] = o.w;
+                            }
+                        }
+                    }
+                }
+            }
+        } else if (warp < 8) {
+            // ---------------------------------------------------------------- converters
+            // items in the order of use: keys 0, then keys j + 1 and values j for each j. A thread takes every
+            // 128th 16-byte piece: piece w is codes 16 (w % 4) .. of row w / 4, two swizzled 16-byte chunks
+            constexpr int kPieces = P * 64 / 16 / 128;
+            const int ct = tid - 128;
+            auto load = [&](int item, uint4(&w)[kPieces]) {
+                // item 0: keys 0; 2 j + 1: keys j + 1 (no item after the last page); 2 j + 2: values j
+                const int kind = item > 0 && item % 2 == 0, j = kind ? item / 2 - 1 : (item + 1) / 2;
+                const int page = page_at(j);
+                const uint4 *src = page >= 0 ? reinterpret_cast<const uint4 *>(page_codes(A.c, page, head, kind)) : nullptr;
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) w[k] = src ? src[k * 128 + ct] : make_uint4(0, 0, 0, 0);
+            };
+            uint4 w[kPieces];
+            load(0, w);
+            int count = used;
+            for (int item = 0; item <= 2 * n; ++item) {
+                if (item == 2 * n - 1) continue;  // there are no keys past the last page
+                const int s = count % Sm::slots, following = item + 1 == 2 * n - 1 ? item + 2 : item + 1;
+                uint4 ahead[kPieces];
+                if (following <= 2 * n) load(following, ahead);
+                if (!wait(&M.empty[s], (count / Sm::slots & 1) ^ 1)) break;
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) {
+                    const int piece = k * 128 + ct, row = piece >> 2, ch = (piece & 3) * 2;
+                    uint4 x, z;
+                    codes_to_half(w[k].x, x.x, x.y);
+                    codes_to_half(w[k].y, x.z, x.w);
+                    codes_to_half(w[k].z, z.x, z.y);
+                    codes_to_half(w[k].w, z.z, z.w);
+                    unsigned char *dst = M.slot[s] + row * 128;
+                    *reinterpret_cast<uint4 *>(dst + ((ch ^ (row & 7)) << 4)) = x;
+                    *reinterpret_cast<uint4 *>(dst + (((ch + 1) ^ (row & 7)) << 4)) = z;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bar_arrive(&M.full[s]);
+                ++count;
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) w[k] = ahead[k];
+            }
+        } else {
+            // ---------------------------------------------------------------- MMA issuer
+            const unsigned id_s = idesc_f16(kTileRows, kKvBlock), id_o = idesc_f16(kTileRows, P);
+            const unsigned long long qd[2] = {sw128_desc(su32(M.q[0][0])), sw128_desc(su32(M.q[1][0]))};
+            int count = used, freed = flushes;
+            bool ok = true;
+            auto scores = [&](int j) {
+                const int s = count % Sm::slots, g = pages + j, buf = g % kBufs;
+                ok = ok && __all_sync(0xffffffffu, wait(&M.full[s], count / Sm::slots & 1));
+                if (ok && g >= kBufs) ok = __all_sync(0xffffffffu, wait(&M.o_done[buf], (g - kBufs) / kBufs & 1));  // that page's weights are used
+                if (!ok) return;
+                tc_fence_after();
+                const unsigned long long kd = sw128_desc(su32(M.slot[s]));
+                if (elect_one()) {
+                    // the low halves first: the accumulator is then small, and what an addition drops as well
+#pragma unroll
+                    for (int h = 1; h >= 0; --h)
+#pragma unroll
+                        for (int b = 0; b < P / 64; ++b)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_f16(tmem + P + 64 * buf, qd[h] + b * (kTileRows * 128 >> 4) + 2 * k, kd + b * (kKvBlock * 128 >> 4) + 2 * k,
+                                        id_s, b > 0 || k > 0 || h == 0);
+                    mma_commit(&M.empty[s]);
+                    mma_commit(&M.s_full[buf]);
+                }
+                __syncwarp();
+                ++count;
+            };
+            scores(0);
+            for (int j = 0; j < n && ok; ++j) {
+                if (j + 1 < n) scores(j + 1);
+                const int s = count % Sm::slots, g = pages + j, buf = g % kBufs;
+                ok = ok && __all_sync(0xffffffffu, wait(&M.full[s], count / Sm::slots & 1) && wait(&M.w_full[buf], g / kBufs & 1));
+                if (ok && j > 0 && j % kFlush == 0) ok = __all_sync(0xffffffffu, wait(&M.o_free, freed++ & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const unsigned w = tmem + P + 64 * buf;
+                const unsigned long long vd = sw128_desc(su32(M.slot[s]));
+                if (elect_one()) {
+#pragma unroll
+                    for (int h = 1; h >= 0; --h)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma_f16_ts(tmem, w + 32 * h + 8 * k, vd + 2 * k, id_o, j % kFlush > 0 || k > 0 || h == 0);
+                    mma_commit(&M.empty[s]);
+                    mma_commit(&M.o_done[buf]);
+                }
+                __syncwarp();
+                ++count;
+            }
+        }
+        pages += n;
+        used += 2 * n;
+        flushes += (n - 1) / kFlush;
+        tc_fence_before();
+        __syncthreads();  // the piece is done: its queries, its S and O are free
+        tc_fence_after();
+        if (*(volatile int *)&M.abort_flag) break;
+    }
+    __syncthreads();
+    if (tid == 0 && M.abort_flag) raise_error(A.c.err, kErrWaitTimeout);
+    if (warp == 8) {
+        // every MMA issued must complete before TMEM is released, whether or not the others have given up
+        if (elect_one()) mma_commit(&M.drained);
+        __syncwarp();
+        for (const long long began = clock64(); !bar_try(&M.drained, 0) && clock64() - began < kLimit;) {
+        }
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Joins the parts of a unit that several CTAs worked on: the begun one in y and the tails in the workspace, all of
+// them sums of 2^(logit - m_i) v / most; 32 rows of a tile a block.
+template <int P>
+__global__ void __launch_bounds__(256) k_kv8_prompt_join(const __grid_constant__ PromptArgs A) {
+    const int tid = threadIdx.x, unit = blockIdx.x, pair = unit / A.c.kv_heads, head = unit % A.c.kv_heads;
+    const int run = pair / A.tiles, tile = pair % A.tiles, i = blockIdx.y * 32 + tid % 32, r = tile * kTileRows + i;
+    const bool there = i < kTileRows && r < A.runs.count * A.group;
+    const int n = pair_pages(A, run, tile);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float *dst = there ? prompt_row(A, run, head, r) : nullptr;
+    if (n == 0) {
+        for (int ch = tid / 32; there && ch < A.c.dim; ch += 8) dst[ch] = 0.0f;
+        return;
+    }
+    const PromptParts W = prompt_parts(A.c.workspace, P);
+    const int2 cover = W.cover[unit];
+    if (cover.x == cover.y || !there) return;
+    const float4 begun = W.head_ml[cover.x * kTileRows + i];
+    float m = begun.x;
+    for (int c = cover.x + 1; c <= cover.y; ++c) m = fmaxf(m, W.tail_ml[c * kTileRows + i].x);
+    if (m == -INFINITY) m = 0.0f;
+    const float w0 = exp2_fast(begun.x - m);
+    float sum = begun.y * w0;
+    for (int c = cover.x + 1; c <= cover.y; ++c) {
+        const float4 t = W.tail_ml[c * kTileRows + i];
+        sum += t.y * exp2_fast(t.x - m);
+    }
+    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    for (int k = tid / 32; k < P / 4; k += 8) {
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = 4 * k + e < A.c.dim ? dst[4 * k + e] * w0 : 0.0f;
+        for (int c = cover.x + 1; c <= cover.y; ++c) {
+            const float w = exp2_fast(W.tail_ml[c * kTileRows + i].x - m);
+            const float4 f = W.sum[((size_t)c * (P / 4) + k) * kTileRows + i];
+            o[0] += f.x * w, o[1] += f.y * w, o[2] += f.z * w, o[3] += f.w * w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (4 * k + e < A.c.dim) dst[4 * k + e] = o[e] * inv * begun.z;
+    }
+}
+
+template <int P>
+cudaError_t launch(PromptArgs A, cudaStream_t s) {
+    // at least half of an SM's shared memory: two CTAs on one SM would wait for each other's TMEM
+    constexpr size_t kSmem = sizeof(PromptSmem<P>) + 1024 > 120 * 1024 ? sizeof(PromptSmem<P>) + 1024 : 120 * 1024;
+    static_assert(kSmem <= 227 * 1024, "fits an SM");
+    int device = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_kv8_prompt<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    if (e != cudaSuccess) return e;
+    const long long pairs = (long long)A.tiles * A.runs.segments, units = pairs * A.c.kv_heads;
+    const int most = sms < kMaxGrid ? sms : kMaxGrid;
+    // Units shared page by page where whole ones would leave the last round of CTAs uneven
+    A.split = pairs <= kMaxPairs && units <= kMaxUnits && units < 8LL * most;
+    const long long work = A.split ? units * A.c.blocks : units;
+    k_kv8_prompt<P><<<(unsigned)(work < most ? work : most), kPromptThreads, kSmem, s>>>(A);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !A.split) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)units, kTileRows / 32);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_kv8_prompt_join<P>, A);
+}
+
+}  // namespace
+
+cudaError_t kv8_attend_prompt(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, float scale, float *y, cudaStream_t s) {
+    const int group = heads / c.kv_heads;
+    const long long rows = (long long)r.count * group;
+    const PromptArgs A{c, q, stride, heads, group, (int)((rows + kTileRows - 1) / kTileRows), r, scale * 1.4426950408889634f, y, 0};
+    if (c.padded == 64) return launch<64>(A, s);
+    if (c.padded == 128) return launch<128>(A, s);
+    return launch<256>(A, s);
+}
+
+}  // namespace strata
