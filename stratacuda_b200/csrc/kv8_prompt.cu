@@ -8,14 +8,14 @@
 // Both products run twice, for the high and the low half, which gives F32's accuracy at half of the FP16
 // rate. Accumulators, maxima and sums are F32.
 //
-// Warps:
-//   0-3  softmax: a thread owns one row (its TMEM lane): logits from S, running maximum and sum,
-//        weights back into the TMEM columns of S. O is rescaled only when a row's maximum has grown by more than
+// Warps (8, so that a thread may hold a whole row's logits in its registers):
+//   0-3  softmax: a thread owns one row (its TMEM lane): logits from S, running maximum and sum, weights
+//        back into the TMEM columns of S. O is rescaled only when a row's maximum has grown by more than
 //        2^5 (weights are kept times 2^10, so that both ends stay inside FP16), so seldom after the
 //        first pages
-//   4-7  converters: 8-bit codes from global memory (the next item's loads in flight) to FP16 in the
+//   4-6  converters: 8-bit codes from global memory (the next item's loads in flight) to FP16 in the
 //        128-byte-swizzled layout of the MMA operands; keys and values alternate through one ring of slots
-//   8    one thread issues the MMAs: S of page j + 1 before O of page j, so that the softmax of
+//   7    one thread issues the MMAs: S of page j + 1 before O of page j, so that the softmax of
 //        a page runs under the products of its neighbours
 // A value scale cannot be applied after the product, since pages add up in one accumulator: weights are
 // multiplied by scale / (largest scale of the tile's pages).
@@ -32,7 +32,9 @@ namespace {
 
 using namespace pf;
 
-constexpr int kPromptThreads = 288;
+constexpr int kSoftWarps = 4, kConvWarps = 3, kMmaWarp = kSoftWarps + kConvWarps;
+constexpr int kPromptThreads = 32 * (kMmaWarp + 1);
+constexpr int kConvThreads = 32 * kConvWarps;
 constexpr int kTileRows = 128;
 constexpr int kBufs = 4;             // S / weight buffers in TMEM, 64 columns each
 constexpr float kLiftP = 10.0f;      // weights are stored times 2^10
@@ -44,13 +46,25 @@ constexpr int kMaxGrid = 160;        // CTAs, each with a slot in the workspace
 constexpr int kMaxPairs = 1024;      // (run, tile) pairs of a split call
 constexpr int kMaxUnits = 65536;
 
+// Pages [first, stop) of the n that a unit (run, tile, key/value head) attends to; n < 0: no piece is left.
+struct Piece {
+    int run, tile, head;
+    int first, stop, n;
+};
+
 template <int P>
 struct __align__(1024) PromptSmem {
     static constexpr int slots = P == 256 ? 3 : 6;
     unsigned char q[2][P / 64][kTileRows * 128];  // high and low halves: panels of 64 channels, rows of 128 bytes, swizzled
     unsigned char slot[slots][P * 128];           // keys [P / 64][64 tokens][128 bytes] or values [P channels][128 bytes], swizzled
     float row_scale[kTileRows];
-    float red[9];
+    float red[kPromptThreads / 32];
+    struct Walk {
+        long long unit, work, work_end, chunk;
+        int pair, head, page, has_tail;
+        Piece tail;
+    } walk;  // thread 0's
+    Piece piece;
     unsigned long long full[slots], empty[slots], s_full[kBufs], w_full[kBufs], o_done[kBufs], o_free, drained;
     unsigned tmem;
     int abort_flag;
@@ -120,30 +134,23 @@ __device__ __forceinline__ void tmem_ld16_async(unsigned taddr, unsigned (&r)[16
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-struct Piece {
-    int run, tile, head;
-    int first, stop, n;  // pages [first, stop) of the unit's n
-};
-
 template <int P>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_constant__ PromptArgs A) {
     using Sm = PromptSmem<P>;
-    extern __shared__ unsigned char raw[];
-    Sm &M = *reinterpret_cast<Sm *>(raw + ((1024 - (su32(raw) & 1023)) & 1023));
+    extern __shared__ __align__(1024) unsigned char raw[];  // the swizzled operands repeat every 1024 bytes
+    Sm &M = *reinterpret_cast<Sm *>(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pairs = A.runs.segments * A.tiles;
     const PromptParts W = prompt_parts(A.c.workspace, P);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ---- this CTA's work: units (pair, head) blockIdx.x, + gridDim.x, ... or pages [work, work_end) of all units' list
-    long long unit = blockIdx.x, work = 0, work_end = 0, chunk = 1;
-    int at_pair = 0, at_head = 0, at_page = 0;
     if (A.split) {
         long long *before = reinterpret_cast<long long *>(M.slot[0]);  // used before the ring is
         long long *part = before + kMaxPairs + 1;
-        static_assert(sizeof(M.slot) >= (kMaxPairs + 1 + 9) * 8, "the page counts fit");
-        for (int base = 0; base < pairs; base += 256) {  // before[i]: a head's pages before pair i
-            long long sum = tid < 256 && base + tid < pairs ? pair_pages(A, (base + tid) / A.tiles, (base + tid) % A.tiles) : 0;
+        static_assert(sizeof(M.slot) >= (kMaxPairs + 1 + kPromptThreads / 32) * 8, "the page counts fit");
+        for (int base = 0; base < pairs; base += kPromptThreads) {  // before[i]: a head's pages before pair i
+            long long sum = base + tid < pairs ? pair_pages(A, (base + tid) / A.tiles, (base + tid) % A.tiles) : 0;
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1) {
                 const long long o = __shfl_up_sync(0xffffffffu, sum, s);
@@ -154,41 +161,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
             long long carry = base ? before[base] : 0;
             for (int w = 0; w < warp; ++w) carry += part[w];
             if (base == 0 && tid == 0) before[0] = 0;
-            if (tid < 256 && base + tid < pairs) before[base + tid + 1] = carry + sum;
+            if (base + tid < pairs) before[base + tid + 1] = carry + sum;
             __syncthreads();
         }
-        const long long total = before[pairs] * A.c.kv_heads;
-        chunk = (total + gridDim.x - 1) / gridDim.x;
-        work = chunk * blockIdx.x;
-        work_end = min(total, work + chunk);
-        if (work >= work_end) return;
-        int lo = 0, hi = pairs - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (before[mid + 1] * A.c.kv_heads > work) hi = mid;
-            else lo = mid + 1;
+        const long long total = before[pairs] * A.c.kv_heads, chunk = (total + gridDim.x - 1) / gridDim.x, work = chunk * blockIdx.x;
+        if (work >= total) return;
+        if (tid == 0) {
+            int lo = 0, hi = pairs - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (before[mid + 1] * A.c.kv_heads > work) hi = mid;
+                else lo = mid + 1;
+            }
+            const long long n = before[lo + 1] - before[lo], in = work - before[lo] * A.c.kv_heads;
+            M.walk.work = work;
+            M.walk.work_end = min(total, work + chunk);
+            M.walk.chunk = chunk;
+            M.walk.pair = lo;
+            M.walk.head = (int)(in / n);
+            M.walk.page = (int)(in % n);
         }
-        const long long n = before[lo + 1] - before[lo], in = work - before[lo] * A.c.kv_heads;
-        at_pair = lo;
-        at_head = (int)(in / n);
-        at_page = (int)(in % n);
     }
     if (tid == 0) {
         for (int i = 0; i < Sm::slots; ++i) {
-            bar_init(&M.full[i], 128);
+            bar_init(&M.full[i], kConvThreads);
             bar_init(&M.empty[i], 1);
         }
         for (int i = 0; i < kBufs; ++i) {
             bar_init(&M.s_full[i], 1);
-            bar_init(&M.w_full[i], 128);
+            bar_init(&M.w_full[i], 32 * kSoftWarps);
             bar_init(&M.o_done[i], 1);
         }
-        bar_init(&M.o_free, 128);
+        bar_init(&M.o_free, 32 * kSoftWarps);
         bar_init(&M.drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         M.abort_flag = 0;
+        M.walk.unit = blockIdx.x;
+        M.walk.has_tail = 0;
     }
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&M.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -207,67 +218,80 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
         }
     };
 
-    // The next piece of the CTA's work. The part of a unit that an earlier CTA began comes last: its sum stays
-    // in the CTA's workspace slot, which the other pieces use in passing.
-    Piece tail{0, 0, 0, 0, 0, 0};
-    bool has_tail = false;
-    auto next = [&](Piece &p) -> bool {
+    // The next piece of the CTA's work (thread 0). The part of a unit that an earlier CTA began comes last: its
+    // sum stays in the CTA's workspace slot, which the other pieces use in passing.
+    auto next = [&]() {
+        auto &w = M.walk;
+        Piece p{0, 0, 0, 0, 0, -1};
         if (!A.split) {
-            if (unit >= (long long)pairs * A.c.kv_heads) return false;
-            const int a_tile = A.runs.segments * A.c.kv_heads, rest = (int)(unit % a_tile);  // the tiles with the most keys first
-            p.tile = A.tiles - 1 - (int)(unit / a_tile);
-            p.run = rest / A.c.kv_heads;
-            p.head = rest % A.c.kv_heads;
-            p.first = 0;
-            p.n = p.stop = pair_pages(A, p.run, p.tile);
-            unit += gridDim.x;
-            return true;
+            if (w.unit < (long long)pairs * A.c.kv_heads) {
+                const int a_tile = A.runs.segments * A.c.kv_heads, rest = (int)(w.unit % a_tile);  // the tiles with the most keys first
+                p.tile = A.tiles - 1 - (int)(w.unit / a_tile);
+                p.run = rest / A.c.kv_heads;
+                p.head = rest % A.c.kv_heads;
+                p.n = p.stop = pair_pages(A, p.run, p.tile);
+                w.unit += gridDim.x;
+            }
+            M.piece = p;
+            return;
         }
-        while (work < work_end) {
-            p.run = at_pair / A.tiles;
-            p.tile = at_pair % A.tiles;
-            p.head = at_head;
+        while (w.work < w.work_end) {
+            p.run = w.pair / A.tiles;
+            p.tile = w.pair % A.tiles;
+            p.head = w.head;
             p.n = pair_pages(A, p.run, p.tile);
             if (p.n == 0) {  // nothing in sight: the joining kernel writes the zeros
-                ++at_pair;
+                ++w.pair;
                 continue;
             }
-            p.first = at_page;
-            p.stop = (int)min((long long)p.n, at_page + (work_end - work));
-            if (at_page == 0 && tid == 0)
-                W.cover[at_pair * A.c.kv_heads + at_head] = make_int2(blockIdx.x, (int)((work + p.n - 1) / chunk));
-            work += p.stop - p.first;
-            at_page = 0;
-            if (++at_head == A.c.kv_heads) {
-                at_head = 0;
-                ++at_pair;
+            p.first = w.page;
+            p.stop = (int)min((long long)p.n, w.page + (w.work_end - w.work));
+            if (w.page == 0) W.cover[w.pair * A.c.kv_heads + w.head] = make_int2(blockIdx.x, (int)((w.work + p.n - 1) / w.chunk));
+            w.work += p.stop - p.first;
+            w.page = 0;
+            if (++w.head == A.c.kv_heads) {
+                w.head = 0;
+                ++w.pair;
             }
-            if (p.first == 0) return true;
-            tail = p;
-            has_tail = true;
+            if (p.first == 0) {
+                M.piece = p;
+                return;
+            }
+            w.tail = p;
+            w.has_tail = 1;
         }
-        if (!has_tail) return false;
-        p = tail;
-        has_tail = false;
-        return true;
+        if (w.has_tail) M.piece = w.tail;
+        else M.piece.n = -1;
+        w.has_tail = 0;
     };
 
     // counters that go on from piece to piece: pages (S buffers), ring items, flushes
     int pages = 0, used = 0, flushes = 0;
-    Piece p;
-    while (next(p)) {
+    for (;;) {
+        if (tid == 0) next();
+        __syncthreads();
+        const Piece p = M.piece;
+        if (p.n < 0) break;
         const RunAt at = run_at(A.c, A.runs, p.run);
         const int row0 = p.tile * kTileRows, rows = min(kTileRows, A.runs.count * A.group - row0), n = p.stop - p.first, head = p.head;
         if (n == 0) {  // no row of the tile sees a key
             for (int i = tid; i < rows * A.c.dim; i += kPromptThreads) prompt_row(A, p.run, head, row0 + i / A.c.dim)[i % A.c.dim] = 0.0f;
+            __syncthreads();
             continue;
         }
-        auto page_at = [&](int j) { return page_of(A.c, at.sequence, p.first + j); };
+        // the table's entry of local page j, to be looked at an iteration later
+        const int *table = A.c.table + (size_t)at.sequence * A.c.blocks + p.first;
+        auto entry_at = [&](int j) { return j < n ? table[j] : -1; };
+        auto checked = [&](int j, int page) {  // an entry of a page that is needed
+            if (page >= 0 && page < A.c.pages) return page;
+            if (j < n) raise_error(A.c.err, kErrIndex);
+            return -1;
+        };
         // queries: a row is P / 8 lanes of 8 channels; scaled by a power of two to 2^9 .. 2^10 at most
-        if (warp < 8) {
+        {
             constexpr int kLanes = P / 8, kAtOnce = 32 / kLanes;
             const int l = lane % kLanes, ch0 = 8 * l;
-            for (int i = warp * kAtOnce + lane / kLanes; i < kTileRows; i += 8 * kAtOnce) {
+            for (int i = warp * kAtOnce + lane / kLanes; i < kTileRows; i += kPromptThreads / 32 * kAtOnce) {
                 float x[8], big = 0.0f;
                 const int r = row0 + i;
                 const float *src = A.q + (p.run * (long long)A.runs.count + r / A.group) * A.stride + (size_t)(head * A.group + r % A.group) * A.c.dim + ch0;
@@ -307,9 +331,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
         if (lane == 0) M.red[warp] = most;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 9; ++i) most = fmaxf(most, M.red[i]);
+        for (int i = 0; i < kPromptThreads / 32; ++i) most = fmaxf(most, M.red[i]);
 
-        if (warp < 4) {
+        if (warp < kSoftWarps) {
             // ---------------------------------------------------------------- softmax
             const int i = warp * 32 + lane;
             const int seen = i < rows ? visible_keys(A.c, at, (row0 + i) / A.group) - p.first * kKvBlock : 0;
@@ -318,10 +342,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
             float4 *kept = W.sum + (size_t)blockIdx.x * (P / 4) * kTileRows + i;  // this row's sum of flushed pages, every 128th
             float m = -INFINITY, sum = 0.0f, kept_m = -INFINITY;
             bool ok = true;
-            auto scales_of = [&](int j) {
-                const int page = page_at(j);
+            auto scales_of = [&](int page) {  // -1: no page
                 const float *s = page >= 0 ? page_scales(A.c, page, head) : nullptr;
-                return s ? make_float2(s[0], s[1]) : make_float2(-1.0f, 0.0f);  // -1: no page
+                return s ? make_float2(s[0], s[1]) : make_float2(-1.0f, 0.0f);
             };
             // O of local page j's group, complete, joins the kept sum
             auto flush = [&](int j) -> bool {
@@ -332,17 +355,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                 const float alpha = fresh || kept_m >= m ? 1.0f : exp2_fast(kept_m - m);
                 kept_m = m;
 #pragma unroll 1
-                for (int k = 0; k < P; k += 16) {
-                    unsigned x[16];
-                    float4 f[4];
-                    tmem_ld16_async(mine + k, x);
+                for (int k = 0; k < P; k += 32) {
+                    unsigned x[32];
+                    float4 f[8];
+                    tmem_ld32_async(mine + k, x);
                     if (!fresh) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) f[e] = kept[(k / 4 + e) * kTileRows];
+                        for (int e = 0; e < 8; ++e) f[e] = kept[(k / 4 + e) * kTileRows];
                     }
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int e = 0; e < 8; ++e) {
                         float4 o = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
                                                __uint_as_float(x[4 * e + 3]));
                         if (!fresh) o = make_float4(f[e].x * alpha + o.x, f[e].y * alpha + o.y, f[e].z * alpha + o.z, f[e].w * alpha + o.w);
@@ -353,23 +376,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                 bar_arrive(&M.o_free);
                 return true;
             };
-            float2 sc = scales_of(0);
+            // scales are loaded two pages ahead, table entries three
+            float2 sc = scales_of(checked(0, entry_at(0))), sc1 = scales_of(checked(1, entry_at(1)));
+            int entry2 = entry_at(2);
             for (int j = 0; j < n; ++j) {
                 const int g = pages + j, buf = g % kBufs;
                 const unsigned cols = mine + P + 64 * buf;
                 const int left = sc.x >= 0.0f ? seen - j * kKvBlock : 0;
                 const float c = sc.x * row_scale, fv = sc.y * over;
-                if (j + 1 < n) sc = scales_of(j + 1);  // under this page's work
+                sc = sc1;
+                sc1 = scales_of(checked(j + 2, entry2));
+                entry2 = entry_at(j + 3);
                 if (!(ok = __all_sync(0xffffffffu, wait(&M.s_full[buf], g / kBufs & 1)))) break;
                 tc_fence_after();
                 float a[64];
-#pragma unroll
-                for (int k = 0; k < 64; k += 32) {
-                    unsigned x[32];
-                    tmem_ld32_async(cols + k, x);
+                {
+                    unsigned x[32], z[32];
+                    tmem_ld32_async(cols, x);
+                    tmem_ld32_async(cols + 32, z);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) a[k + e] = __uint_as_float(x[e]) * c;
+                    for (int e = 0; e < 32; ++e) {
+                        a[e] = __uint_as_float(x[e]) * c;
+                        a[32 + e] = __uint_as_float(z[e]) * c;
+                    }
                 }
                 if (__any_sync(0xffffffffu, left < kKvBlock)) {
 #pragma unroll
@@ -405,17 +435,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                 const float from = (m == -INFINITY ? 0.0f : m) - kLiftP;
                 float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int k = 0; k < 4; k += 2) {  // 32 weights to 16 columns of high and 16 of low halves
+                for (int k = 0; k < 2; ++k) {  // 32 weights to 16 columns of high and 16 of low halves
                     unsigned hi[16], lo[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float p0 = exp2_fast(a[16 * k + 2 * e] - from), p1 = exp2_fast(a[16 * k + 2 * e + 1] - from);
+                        const float p0 = exp2_fast(a[32 * k + 2 * e] - from), p1 = exp2_fast(a[32 * k + 2 * e + 1] - from);
                         add[(2 * e) & 3] += p0;
                         add[(2 * e + 1) & 3] += p1;
                         split_pair(p0 * fv, p1 * fv, hi[e], lo[e]);
                     }
-                    tmem_st16(cols + 8 * k, hi);
-                    tmem_st16(cols + 32 + 8 * k, lo);
+                    tmem_st16(cols + 16 * k, hi);
+                    tmem_st16(cols + 32 + 16 * k, lo);
                 }
                 sum += (add[0] + add[1]) + (add[2] + add[3]);
                 tmem_wait_st();
@@ -465,32 +495,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                     }
                 }
             }
-        } else if (warp < 8) {
+        } else if (warp < kMmaWarp) {
             // ---------------------------------------------------------------- converters
             // items in the order of use: keys 0, then keys j + 1 and values j for each j. A thread takes every
-            // 128th 16-byte piece: piece w is codes 16 (w % 4) .. of row w / 4, two swizzled 16-byte chunks
-            constexpr int kPieces = P * 64 / 16 / 128;
-            const int ct = tid - 128;
-            auto load = [&](int item, uint4(&w)[kPieces]) {
-                // item 0: keys 0; 2 j + 1: keys j + 1 (no item after the last page); 2 j + 2: values j
-                const int kind = item > 0 && item % 2 == 0, j = kind ? item / 2 - 1 : (item + 1) / 2;
-                const int page = page_at(j);
+            // 96th 16-byte piece: piece w is codes 16 (w % 4) .. of row w / 4, two swizzled 16-byte chunks
+            constexpr int kAll = P * 64 / 16, kPieces = (kAll + kConvThreads - 1) / kConvThreads;
+            const int ct = tid - 32 * kSoftWarps;
+            auto load = [&](int page, int kind, uint4(&w)[kPieces]) {
                 const uint4 *src = page >= 0 ? reinterpret_cast<const uint4 *>(page_codes(A.c, page, head, kind)) : nullptr;
 #pragma unroll
-                for (int k = 0; k < kPieces; ++k) w[k] = src ? src[k * 128 + ct] : make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < kPieces; ++k)
+                    w[k] = src && k * kConvThreads + ct < kAll ? src[k * kConvThreads + ct] : make_uint4(0, 0, 0, 0);
             };
-            uint4 w[kPieces];
-            load(0, w);
             int count = used;
-            for (int item = 0; item <= 2 * n; ++item) {
-                if (item == 2 * n - 1) continue;  // there are no keys past the last page
-                const int s = count % Sm::slots, following = item + 1 == 2 * n - 1 ? item + 2 : item + 1;
-                uint4 ahead[kPieces];
-                if (following <= 2 * n) load(following, ahead);
-                if (!wait(&M.empty[s], (count / Sm::slots & 1) ^ 1)) break;
+            auto store = [&](const uint4(&w)[kPieces]) -> bool {
+                const int s = count % Sm::slots;
+                if (!wait(&M.empty[s], (count / Sm::slots & 1) ^ 1)) return false;
 #pragma unroll
                 for (int k = 0; k < kPieces; ++k) {
-                    const int piece = k * 128 + ct, row = piece >> 2, ch = (piece & 3) * 2;
+                    const int piece = k * kConvThreads + ct, row = piece >> 2, ch = (piece & 3) * 2;
+                    if (piece >= kAll) break;
                     uint4 x, z;
                     codes_to_half(w[k].x, x.x, x.y);
                     codes_to_half(w[k].y, x.z, x.w);
@@ -503,8 +527,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 bar_arrive(&M.full[s]);
                 ++count;
+                return true;
+            };
+            // each item's loads are in flight while the item before it is converted
+            uint4 keys[kPieces], values[kPieces];
+            int page = checked(0, entry_at(0)), page1 = checked(1, entry_at(1)), entry2 = entry_at(2);
+            load(page, 0, keys);
+            load(page1, 0, values);  // (the next keys, for the first step)
+            bool ok = store(keys);
 #pragma unroll
-                for (int k = 0; k < kPieces; ++k) w[k] = ahead[k];
+            for (int k = 0; k < kPieces; ++k) keys[k] = values[k];
+            for (int j = 0; j < n && ok; ++j) {
+                load(page, 1, values);
+                if (j + 1 < n) ok = store(keys);
+                page = page1;
+                page1 = checked(j + 2, entry2);
+                entry2 = entry_at(j + 3);
+                if (j + 2 < n) load(page1, 0, keys);
+                ok = ok && store(values);
             }
         } else {
             // ---------------------------------------------------------------- MMA issuer
@@ -567,7 +607,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
     }
     __syncthreads();
     if (tid == 0 && M.abort_flag) raise_error(A.c.err, kErrWaitTimeout);
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         // every MMA issued must complete before TMEM is released, whether or not the others have given up
         if (elect_one()) mma_commit(&M.drained);
         __syncwarp();
@@ -624,7 +664,7 @@ __global__ void __launch_bounds__(256) k_kv8_prompt_join(const __grid_constant__
 template <int P>
 cudaError_t launch(PromptArgs A, cudaStream_t s) {
     // at least half of an SM's shared memory: two CTAs on one SM would wait for each other's TMEM
-    constexpr size_t kSmem = sizeof(PromptSmem<P>) + 1024 > 120 * 1024 ? sizeof(PromptSmem<P>) + 1024 : 120 * 1024;
+    constexpr size_t kSmem = sizeof(PromptSmem<P>) > 120 * 1024 ? sizeof(PromptSmem<P>) : 120 * 1024;
     static_assert(kSmem <= 227 * 1024, "fits an SM");
     int device = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&device);
