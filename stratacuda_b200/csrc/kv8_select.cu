@@ -1,151 +1,331 @@
 // Choosing the blocks that a query attends to (strata_kv8_select).
+//
+// A block's bound for a token and key/value head is an integer product: the group's queries as two rows
+// of 8-bit codes (negative and positive parts) with the block's two rows of marks, 2 P terms, times the
+// block's key scale. Products and sums are whole numbers, so any order gives the same bound, and the
+// choice repeats exactly.
+//   * 16 tokens of a run are the rows of an integer tensor-core tile (mma.sync m16n8k32) against 8 blocks a
+//     step, whose marks come from global memory in fragment order: 16 consecutive bytes are a lane's operands
+//     of two k-steps. One token alone pays for the tile but not for memory: each block's marks are read once.
+//   * the bounds, as words that order like the numbers, stay in shared memory; the words' range is halved
+//     until exactly `top` of them lie above, which takes a dozen steps instead of 32 when few are equal.
+//   * few tokens: a cluster of up to 8 CTAs shares a token's blocks and sends the bounds to its first CTA.
 #include "kv8.cuh"
+
+#include <cooperative_groups.h>
 
 namespace strata {
 namespace {
 
-constexpr int kThreads = 256;
+namespace cg = cooperative_groups;
 
-__device__ __forceinline__ float block_max(float x, float *red) {
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) x = fmaxf(x, red[i]);
-    return x;
-}
-// A float's bits in an order that compares as unsigned words.
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kTile = 16;
+constexpr unsigned kForced = 0xffffffffu;
+
+struct Args {
+    Kv8 c;
+    const float *q;
+    long long stride;
+    int heads, group;
+    Kv8Runs runs;
+    int top, first, last;
+    int *picks;
+    int rows;     // tokens of a CTA (of a cluster), 1 .. 16
+    int tiles;    // CTAs (clusters) a run
+    int row_len;  // words between the rows of bounds in shared memory
+};
+
+// A float's bits in an order that compares as unsigned words; 0 is below every number.
 __device__ __forceinline__ unsigned ordered(float f) {
     const unsigned u = __float_as_uint(f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float finite_or_zero(float f) { return isfinite(f) ? f : 0.0f; }
+__device__ __forceinline__ void mma_s8(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
-// One CTA: one token and key/value head. The group's queries become two rows of 8-bit codes
-// (positive and negative parts), every block's bound is an integer product with its marks, and the
-// top-th largest ordered bound is found bit by bit; blocks above it and the lowest of those equal to
-// it are written in ascending order.
-template <int P>
-__global__ void __launch_bounds__(kThreads) k_kv8_select(const Kv8 c, const float *q, long long stride, int heads, const Kv8Runs runs, int top,
-                                                         int first, int last, int *picks) {
-    extern __shared__ unsigned key_s[];  // [blocks in sight]
-    __shared__ float red[kThreads / 32];
-    __shared__ __align__(16) int8_t pos_s[P], neg_s[P];
-    __shared__ int count_s, taken_s[kThreads];
-    const int tid = threadIdx.x, head = blockIdx.y;
-    const int token = blockIdx.x, run = token / runs.count;
-    const RunAt a = run_at(c, runs, run);
-    const int nb = (visible_keys(c, a, token % runs.count) + kKvBlock - 1) / kKvBlock;
-    int *out = picks + ((size_t)token * c.kv_heads + head) * top;
-    if (nb <= top) {
-        for (int i = tid; i < top; i += kThreads) out[i] = i < nb ? i : -1;
-        return;
-    }
-    const int group = heads / c.kv_heads;
-    const float *x = q + (long long)token * stride + (size_t)head * group * c.dim;
-    float amax = 0.0f;
-    for (int i = tid; i < group * c.dim; i += kThreads) amax = fmaxf(amax, isfinite(x[i]) ? fabsf(x[i]) : 0.0f);
-    amax = block_max(amax, red);
-    const float unit = amax < 0x1p-100f ? 0.0f : __fdiv_rn(32767.0f, amax);
-    int pos = 0, neg = 0;
-    if (tid < c.dim)
-        for (int h = 0; h < group; ++h) {
-            const float f = x[h * c.dim + tid];
-            const int r = isfinite(f) ? __float2int_rn(__fmul_rn(f, unit)) : 0;
-            pos += max(r, 0);
-            neg += min(r, 0);
-        }
-    const float big = block_max((float)max(pos, -neg), red);
-    const float fine = big > 0.0f ? __fdiv_rn(127.0f, big) : 0.0f;
-    if (tid < P) {
-        pos_s[tid] = (int8_t)__float2int_rn(__fmul_rn((float)pos, fine));
-        neg_s[tid] = (int8_t)__float2int_rn(__fmul_rn((float)neg, fine));
-    }
+// The largest of x over the warps that share a row: the whole block, or this warp.
+template <bool WIDE>
+__device__ __forceinline__ float row_max(float x, float *red) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
+    if (!WIDE) return x;
     __syncthreads();
-    for (int b = tid; b < nb; b += kThreads) {
-        unsigned key = 0xffffffffu;
-        if (b >= first && b < nb - last) {
-            const int page = page_of(c, a.sequence, b);
-            int dot = 0;
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) x = fmaxf(x, red[i]);
+    return x;
+}
+
+// WIDE: one token a CTA (cluster), all warps on it. Otherwise up to 16 tokens of a run, a warp to a token.
+template <int P, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constant__ Args A) {
+    extern __shared__ unsigned key_s[];  // [rows][row_len]
+    __shared__ __align__(16) int8_t code_s[kTile][2 * P + 16];  // negative parts, positive parts
+    __shared__ float red[kWarps];
+    __shared__ int count_s[2][kWarps], equal_s[kWarps], have_s[kTile];
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int unit = blockIdx.x / ranks, head = unit % A.c.kv_heads, tile = unit / A.c.kv_heads % A.tiles, run = unit / A.c.kv_heads / A.tiles;
+    const RunAt at = run_at(A.c, A.runs, run);
+    const int j0 = tile * A.rows, rows = min(A.rows, A.runs.count - j0);
+    const long long token0 = (long long)run * A.runs.count + j0;
+    if (tid < rows) have_s[tid] = (visible_keys(A.c, at, j0 + tid) + kKvBlock - 1) / kKvBlock;
+
+    // the group's queries of each row as two rows of codes
+    constexpr int kEach = WIDE ? (P + kThreads - 1) / kThreads : P / 32;  // channels a thread
+    const int me = WIDE ? tid : lane, step = WIDE ? kThreads : 32;
+    for (int r = WIDE ? 0 : warp; r < (WIDE ? 1 : kTile); r += kWarps) {
+        int pos[kEach] = {}, neg[kEach] = {};
+        if (r < rows) {
+            const float *x = A.q + (token0 + r) * A.stride + (size_t)head * A.group * A.c.dim;
+            float amax = 0.0f;
+            for (int h = 0; h < A.group; ++h)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int ch = me + i * step;
+                    if (ch < A.c.dim) amax = fmaxf(amax, fabsf(finite_or_zero(x[h * A.c.dim + ch])));
+                }
+            amax = row_max<WIDE>(amax, red);
+            const float unit_of = amax < 0x1p-100f ? 0.0f : __fdiv_rn(32767.0f, amax);
+            for (int h = 0; h < A.group; ++h)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int ch = me + i * step;
+                    const int v = ch < A.c.dim ? __float2int_rn(__fmul_rn(finite_or_zero(x[h * A.c.dim + ch]), unit_of)) : 0;
+                    pos[i] += max(v, 0);
+                    neg[i] += min(v, 0);
+                }
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) big = fmaxf(big, (float)max(pos[i], -neg[i]));
+            big = row_max<WIDE>(big, red);
+            const float fine = big > 0.0f ? __fdiv_rn(127.0f, big) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                pos[i] = __float2int_rn(__fmul_rn((float)pos[i], fine));
+                neg[i] = __float2int_rn(__fmul_rn((float)neg[i], fine));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (me + i * step < P) {
+                code_s[r][me + i * step] = (int8_t)neg[i];
+                code_s[r][P + me + i * step] = (int8_t)pos[i];
+            }
+    }
+    if (WIDE)  // the tile's other rows
+        for (int i = tid; i < (kTile - 1) * (2 * P + 16) / 4; i += kThreads) reinterpret_cast<int *>(code_s[1])[i] = 0;
+    __syncthreads();
+    const int most = have_s[rows - 1];
+    if (most > A.top) {
+        unsigned a[P / 32][2][4];  // 64-byte segments of the code rows, two k-steps each
+#pragma unroll
+        for (int i = 0; i < P / 32; ++i) {
+            const uint4 lo = *reinterpret_cast<const uint4 *>(&code_s[g][i * 64 + t * 16]);
+            const uint4 hi = *reinterpret_cast<const uint4 *>(&code_s[g + 8][i * 64 + t * 16]);
+            a[i][0][0] = lo.x, a[i][0][2] = lo.y, a[i][1][0] = lo.z, a[i][1][2] = lo.w;
+            a[i][0][1] = hi.x, a[i][0][3] = hi.y, a[i][1][1] = hi.z, a[i][1][3] = hi.w;
+        }
+        unsigned *keys = cluster.map_shared_rank(key_s, 0);
+        const int *table = A.c.table + (size_t)at.sequence * A.c.blocks;
+        const int stride_b = 8 * kWarps * ranks;
+        int b0 = (rank * kWarps + warp) * 8;
+        int entry = b0 + g < most ? table[b0 + g] : -1;
+        for (; b0 < most; b0 += stride_b) {
+            const int b = b0 + g;
+            int page = entry;
+            if (b < most && (page < 0 || page >= A.c.pages)) {
+                raise_error(A.c.err, kErrIndex);
+                page = -1;
+            }
+            entry = b + stride_b < most ? table[b + stride_b] : -1;
+            uint4 m[P / 32];
             float scale = 0.0f;
             if (page >= 0) {
-                const uint4 *m = reinterpret_cast<const uint4 *>(page_marks(c, page, head));
-                for (int i = 0; i < P / 16; ++i) {
-                    const uint4 lo = m[i], hi = m[P / 16 + i];
-                    const uint4 n = reinterpret_cast<const uint4 *>(neg_s)[i], p = reinterpret_cast<const uint4 *>(pos_s)[i];
-                    dot = __dp4a((int)lo.x, (int)n.x, dot), dot = __dp4a((int)lo.y, (int)n.y, dot);
-                    dot = __dp4a((int)lo.z, (int)n.z, dot), dot = __dp4a((int)lo.w, (int)n.w, dot);
-                    dot = __dp4a((int)hi.x, (int)p.x, dot), dot = __dp4a((int)hi.y, (int)p.y, dot);
-                    dot = __dp4a((int)hi.z, (int)p.z, dot), dot = __dp4a((int)hi.w, (int)p.w, dot);
-                }
-                scale = page_scales(c, page, head)[0];
+                const uint4 *src = reinterpret_cast<const uint4 *>(page_marks(A.c, page, head)) + t;
+#pragma unroll
+                for (int i = 0; i < P / 32; ++i) m[i] = src[i * 4];
+                scale = page_scales(A.c, page, head)[0];
+            } else {
+#pragma unroll
+                for (int i = 0; i < P / 32; ++i) m[i] = make_uint4(0, 0, 0, 0);
             }
-            key = min(ordered(__fmul_rn((float)dot, scale)), 0xfffffffeu);
-        }
-        key_s[b] = key;
-    }
-    // the largest threshold that at least `top` keys reach, from its highest bit down
-    unsigned least = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned trial = least | 1u << bit;
-        __syncthreads();
-        if (tid == 0) count_s = 0;
-        __syncthreads();
-        int n = 0;
-        for (int b = tid; b < nb; b += kThreads) n += key_s[b] >= trial;
-        atomicAdd(&count_s, n);
-        __syncthreads();
-        if (count_s >= top) least = trial;
-    }
-    // each thread writes a run of blocks of its own; keys equal to the threshold fill what is left, lowest first
-    const int each = (nb + kThreads - 1) / kThreads, b0 = tid * each, b1 = min(nb, b0 + each);
-    int above = 0, equal = 0;
-    for (int b = b0; b < b1; ++b) {
-        above += key_s[b] > least;
-        equal += key_s[b] == least;
-    }
-    taken_s[tid] = above | equal << 16;
-    __syncthreads();
-    if (tid == 0) {
-        int room = top;
-        for (int i = 0; i < kThreads; ++i) room -= taken_s[i] & 65535;
-        int at = 0;
-        for (int i = 0; i < kThreads; ++i) {
-            const int up = taken_s[i] & 65535, eq = min(room, taken_s[i] >> 16);
-            taken_s[i] = at | eq << 16;
-            at += up + eq;
-            room -= eq;
+            int d[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < P / 32; ++i) {
+                mma_s8(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], m[i].x, m[i].y);
+                mma_s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], m[i].z, m[i].w);
+            }
+            const float s0 = __shfl_sync(0xffffffffu, scale, 8 * t), s1 = __shfl_sync(0xffffffffu, scale, 8 * t + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = g + (e >> 1) * 8, block = b0 + 2 * t + (e & 1);
+                if (r >= rows || block >= most) continue;
+                const int have = have_s[r];
+                unsigned key = min(ordered(__fmul_rn((float)d[e], e & 1 ? s1 : s0)), kForced - 1);
+                if (block < A.first || block >= have - A.last) key = kForced;
+                if (block >= have) key = 0;
+                keys[r * A.row_len + block] = key;
+            }
         }
     }
-    __syncthreads();
-    int at = taken_s[tid] & 65535, eq = taken_s[tid] >> 16;
-    for (int b = b0; b < b1; ++b) {
-        const bool same = key_s[b] == least;
-        if (key_s[b] > least || (same && eq > 0)) {
-            out[at++] = b;
-            eq -= same;
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+    if (rank) return;
+
+    for (int r = WIDE ? 0 : warp; r < rows; r += kWarps) {
+        const int have = have_s[r];
+        int *out = A.picks + ((size_t)(token0 + r) * A.c.kv_heads + head) * A.top;
+        if (have <= A.top) {
+            for (int i = me; i < A.top; i += step) out[i] = i < have ? i : -1;
+            continue;
+        }
+        const unsigned *key = key_s + r * A.row_len;
+        // this warp's blocks: all, or an eighth in whole groups of 128
+        const int share = WIDE ? (have + 128 * kWarps - 1) / (128 * kWarps) * 128 : have;
+        const int from = WIDE ? min(have, warp * share) : 0, to = WIDE ? min(have, from + share) : have;
+        auto row_sum = [&](int n, int which) {  // over the warps on this row; two places, so one barrier a call is enough
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (!WIDE) return n;
+            if (lane == 0) count_s[which][warp] = n;
+            __syncthreads();
+            n = 0;
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) n += count_s[which][i];
+            return n;
+        };
+        unsigned lo = kForced, hi = 0;
+        int forced = 0;
+        for (int b = from + lane; b < to; b += 32) {
+            const unsigned k = key[b];
+            forced += k == kForced;
+            if (k != kForced) {
+                lo = min(lo, k);
+                hi = max(hi, k);
+            }
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        if (WIDE) {
+            if (lane == 0) {
+                count_s[1][warp] = (int)lo;
+                equal_s[warp] = (int)hi;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+                lo = min(lo, (unsigned)count_s[1][i]);
+                hi = max(hi, (unsigned)equal_s[i]);
+            }
+        }
+        // at least `top` words reach lo, `above` <= top reach hi; halve until as many as wanted do, or equal words
+        // (lo, all of them) are left to fill up with
+        int above = row_sum(forced, 0), turn = 1;
+        hi += 1;
+        while (above != A.top && hi - lo > 1) {
+            const unsigned mid = lo + (hi - lo) / 2;
+            int n = 0;
+            for (int b = from + 4 * lane; b < to; b += 128) {  // (words past the row's last block are zero up to a multiple of 4)
+                const uint4 k = *reinterpret_cast<const uint4 *>(key + b);
+                n += (k.x >= mid) + (b + 1 < to && k.y >= mid) + (b + 2 < to && k.z >= mid) + (b + 3 < to && k.w >= mid);
+            }
+            n = row_sum(n, turn);
+            turn ^= 1;
+            if (n >= A.top && n != A.top) {
+                lo = mid;
+            } else {
+                hi = mid;
+                above = n;
+            }
+        }
+        int room = A.top - above, at_out = 0;
+        if (WIDE) {  // where this warp's picks begin, and how many equal ones earlier warps take
+            int up = 0, eq = 0;
+            for (int b = from + lane; b < to; b += 32) {
+                up += key[b] >= hi;
+                eq += key[b] == lo && key[b] < hi;
+            }
+            up = __reduce_add_sync(0xffffffffu, up);
+            eq = __reduce_add_sync(0xffffffffu, eq);
+            __syncthreads();
+            if (lane == 0) {
+                count_s[0][warp] = up;
+                equal_s[warp] = eq;
+            }
+            __syncthreads();
+            for (int i = 0; i < warp; ++i) {
+                const int take = min(room, equal_s[i]);
+                at_out += count_s[0][i] + take;
+                room -= take;
+            }
+        }
+        for (int b = from; b < to; b += 32) {
+            const unsigned k = b + lane < to ? key[b + lane] : 0;
+            const bool up = k >= hi, eq = !up && k == lo && b + lane < to;
+            const unsigned equals = __ballot_sync(0xffffffffu, eq);
+            const bool take = up || (eq && __popc(equals & ((1u << lane) - 1)) < room);
+            const unsigned all = __ballot_sync(0xffffffffu, take);
+            if (take) out[at_out + __popc(all & ((1u << lane) - 1))] = b + lane;
+            at_out += __popc(all);
+            room -= min(room, __popc(equals));
         }
     }
 }
 
-template <int P>
-cudaError_t launch(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, int top, int first, int last, int *picks,
-                   cudaStream_t s) {
-    const size_t smem = (size_t)c.blocks * 4;
-    cudaError_t e = cudaFuncSetAttribute(k_kv8_select<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <int P, bool WIDE>
+cudaError_t launch(const Args &A, int ranks, size_t smem, cudaStream_t s) {
+    cudaError_t e = cudaFuncSetAttribute(k_kv8_select<P, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    k_kv8_select<P><<<dim3(r.segments * r.count, c.kv_heads), kThreads, smem, s>>>(c, q, stride, heads, r, top, first, last, picks);
-    return cudaGetLastError();
+    const long long ctas = (long long)A.runs.segments * A.tiles * A.c.kv_heads * ranks;
+    if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ranks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_kv8_select<P, WIDE>, A);
 }
 
 }  // namespace
 
 cudaError_t kv8_select(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, int top, int first, int last, int *picks,
                        cudaStream_t s) {
-    if (c.padded == 64) return launch<64>(c, q, stride, heads, r, top, first, last, picks, s);
-    if (c.padded == 128) return launch<128>(c, q, stride, heads, r, top, first, last, picks, s);
-    return launch<256>(c, q, stride, heads, r, top, first, last, picks, s);
+    constexpr int kSms = 148, kKeyBytes = 96 * 1024;  // two CTAs' bounds fit an SM
+    Args A{c, q, stride, heads, heads / c.kv_heads, r, top, first, last, picks, 1, r.count, (c.blocks + 3) / 4 * 4};
+    const long long tokens = (long long)r.segments * r.count * c.kv_heads;
+    // Tiles of up to 16 tokens where they give every multiprocessor one: marks are then read once for 16 tokens
+    int rows = kKeyBytes / (A.row_len * 4);
+    rows = rows > kTile ? kTile : rows;
+    if (rows > r.count) rows = r.count;
+    if (rows > 1 && tokens >= (long long)rows * kSms) {
+        A.rows = rows;
+        A.tiles = (r.count + rows - 1) / rows;
+        const size_t smem = (size_t)rows * A.row_len * 4;
+        if (c.padded == 64) return launch<64, false>(A, 1, smem, s);
+        if (c.padded == 128) return launch<128, false>(A, 1, smem, s);
+        return launch<256, false>(A, 1, smem, s);
+    }
+    // A token a cluster; as many CTAs in it as leave each 64 blocks and the device two rounds of CTAs at most
+    int ranks = 1;
+    while (ranks < 8 && tokens * ranks * 2 <= 4 * kSms && c.blocks >= 128 * ranks) ranks *= 2;
+    const size_t smem = (size_t)A.row_len * 4;
+    if (c.padded == 64) return launch<64, true>(A, ranks, smem, s);
+    if (c.padded == 128) return launch<128, true>(A, ranks, smem, s);
+    return launch<256, true>(A, ranks, smem, s);
 }
 
 }  // namespace strata
