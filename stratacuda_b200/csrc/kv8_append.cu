@@ -6,11 +6,15 @@ namespace {
 
 constexpr int kThreads = 256;
 
+constexpr int kFew = 4;  // new rows of an open block that are worth trying to add without forming the block again
+
 // One CTA: one kind (keys or values) of one head's block of one run. The block's rows, those that
 // the sequence already holds (from `open`) and the new ones, are read into registers, the largest
 // magnitude fixes the scale, the codes are laid out in shared memory as the page holds them and
-// copied out whole.
-template <int P>
+// copied out whole. Bound by memory: 4 bytes read and 1 written a value.
+// A few rows added to an open block (decode) mostly leave its scale as it is; then all other codes stand
+// and only the new rows' are written, with the same result. Bound by the latency of the look-ups.
+template <int P, bool WIDE>
 __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const float *k, const float *v, long long stride, const Kv8Runs runs) {
     constexpr int kTiles = P / 64;  // 4 tokens x 4 channels a tile, 16 * P / 4 tiles
     __shared__ __align__(16) int8_t page_s[P * kKvBlock];
@@ -40,6 +44,64 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
     const long long first = (long long)blockIdx.z * runs.count + (long long)block * kKvBlock - a.start;  // input row of the block's row 0
     const float *in = x + first * stride + (size_t)head * c.dim;
 
+    // the run's last block keeps its new rows in 32 bits while it is unfilled. The first block's
+    // CTA writes them, after its own reads: it is the only one that reads this head's open rows.
+    auto keep = [&]() {
+        if (blockIdx.x != 0 || end % kKvBlock == 0) return;
+        const int last = (int)(end / kKvBlock), rows = (int)(end % kKvBlock), from = last == block ? r0 : 0;
+        const float *src = x + ((long long)blockIdx.z * runs.count + (long long)last * kKvBlock - a.start) * stride + (size_t)head * c.dim;
+        for (int i = tid; i < (rows - from) * c.dim; i += kThreads) {
+            const int row = from + i / c.dim, ch = i % c.dim;
+            const float f = src[(long long)row * stride + ch];
+            open[row * open_row + ch] = isfinite(f) ? f : 0.0f;
+        }
+    };
+    if (r0 > 0 && r1 - r0 <= kFew) {
+        static_assert(P <= kThreads, "a thread a channel");
+        const int ch = tid;
+        float f[kFew], amax = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kFew; ++i) {
+            f[i] = r0 + i < r1 && ch < c.dim ? in[(long long)(r0 + i) * stride + ch] : 0.0f;
+            if (!isfinite(f[i])) {
+                bad = true;
+                f[i] = 0.0f;
+            }
+            amax = fmaxf(amax, fabsf(f[i]));
+        }
+        const float scale = page >= 0 ? page_scales(c, page, head)[kind] : 0.0f;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
+        if (tid % 32 == 0) red[tid / 32] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) amax = fmaxf(amax, red[i]);
+        if (page >= 0 && (amax < 0x1p-100f ? 0.0f : __fdiv_rn(amax, 127.0f)) <= scale) {
+            if (bad) raise_error(c.err, kErrKvValue);
+            if (ch < c.dim) {
+                const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+                int8_t *codes = page_codes(c, page, head, kind), *m = page_marks(c, page, head);
+                int lo = 127, hi = -127;
+#pragma unroll
+                for (int i = 0; i < kFew; ++i) {
+                    if (r0 + i >= r1) continue;
+                    const int q = max(-127, min(127, __float2int_rn(__fmul_rn(f[i], inv))));
+                    codes[kind ? ch * kKvBlock + r0 + i : key_byte(r0 + i, ch)] = (int8_t)q;
+                    lo = min(lo, q);
+                    hi = max(hi, q);
+                }
+                if (!kind) {
+                    if (lo < m[ch]) m[ch] = (int8_t)lo;
+                    if (hi > m[P + ch]) m[P + ch] = (int8_t)hi;
+                }
+            }
+            keep();
+            return;
+        }
+        __syncthreads();  // red is written again below
+    }
+
     // this thread's tiles: neighbouring lanes take neighbouring channels of a key row, and
     // neighbouring token groups of a value channel, so that each kind's packed words lie side by side
     float xs[kTiles][4][4];
@@ -50,20 +112,30 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
         const int w = i * kThreads + tid;
         const int t4 = kind ? w & 15 : w / (P / 4), c4 = kind ? w >> 4 : w % (P / 4);
 #pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int row = t4 * 4 + t, ch = c4 * 4;
+            const float *src = row < r0 ? open + row * open_row + ch : in + (long long)row * stride + ch;
+            if (WIDE) {
+                const float4 f = row < r1 && ch < c.dim ? *reinterpret_cast<const float4 *>(src) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                xs[i][t][0] = f.x, xs[i][t][1] = f.y, xs[i][t][2] = f.z, xs[i][t][3] = f.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xs[i][t][e] = row < r1 && ch + e < c.dim ? src[e] : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = t4 * 4 + t, ch = c4 * 4 + e;
-                float f = 0.0f;
-                if (row < r1 && ch < c.dim) f = row < r0 ? open[row * open_row + ch] : in[(long long)row * stride + ch];
-                if (!isfinite(f)) {
+                if (!isfinite(xs[i][t][e])) {
                     bad = true;
-                    f = 0.0f;
+                    xs[i][t][e] = 0.0f;
                 }
-                xs[i][t][e] = f;
-                amax = fmaxf(amax, fabsf(f));
+                amax = fmaxf(amax, fabsf(xs[i][t][e]));
             }
-    }
     if (bad) raise_error(c.err, kErrKvValue);
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
@@ -120,27 +192,23 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
             reinterpret_cast<int *>(m + P)[tid] = hi;
         }
     }
-    // the run's last block keeps its new rows in 32 bits while it is unfilled. The first block's
-    // CTA writes them, after its own reads: it is the only one that reads this head's open rows.
-    if (blockIdx.x == 0 && end % kKvBlock) {
-        const int last = (int)(end / kKvBlock), rows = (int)(end % kKvBlock);
-        const int from = last == block ? r0 : 0;
-        const float *src = x + ((long long)blockIdx.z * runs.count + (long long)last * kKvBlock - a.start) * stride + (size_t)head * c.dim;
-        for (int i = tid; i < (rows - from) * c.dim; i += kThreads) {
-            const int row = from + i / c.dim, ch = i % c.dim;
-            const float f = src[(long long)row * stride + ch];
-            open[row * open_row + ch] = isfinite(f) ? f : 0.0f;
-        }
-    }
+    keep();
 }
 
 }  // namespace
 
 cudaError_t kv8_append(const Kv8 &c, const float *k, const float *v, long long stride, const Kv8Runs &r, cudaStream_t s) {
     const dim3 grid((r.count + kKvBlock - 2) / kKvBlock + 1, c.kv_heads * 2, r.segments);
-    if (c.padded == 64) k_kv8_append<64><<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
-    else if (c.padded == 128) k_kv8_append<128><<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
-    else k_kv8_append<256><<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
+    // 16-byte loads where every row of a head starts on such a boundary
+    const uintptr_t starts = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(c.open);
+    const bool wide = starts % 16 == 0 && stride % 4 == 0 && c.dim % 4 == 0;
+    auto launch = [&](auto narrow_kernel, auto wide_kernel) {
+        if (wide) wide_kernel<<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
+        else narrow_kernel<<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
+    };
+    if (c.padded == 64) launch(k_kv8_append<64, false>, k_kv8_append<64, true>);
+    else if (c.padded == 128) launch(k_kv8_append<128, false>, k_kv8_append<128, true>);
+    else launch(k_kv8_append<256, false>, k_kv8_append<256, true>);
     return cudaGetLastError();
 }
 

@@ -100,10 +100,10 @@ class Kv8Cache:
 
 
 def _address(x):
-    if x is None or isinstance(x, int):
-        return x
-    ptr = getattr(x, "data_ptr", None)
-    return ptr() if ptr is not None else x.device_ptr
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return x if x is None or isinstance(x, int) else x.device_ptr
 
 
 class DeviceCache:
