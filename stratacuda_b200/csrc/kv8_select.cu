@@ -4,7 +4,7 @@
 // of 8-bit codes (negative and positive parts) with the block's two rows of marks, 2 P terms, times the
 // block's key scale. Products and sums are whole numbers, so any order gives the same bound, and the
 // choice repeats exactly.
-//   * 16 tokens of a run are the rows of an integer tensor-core tile (mma.sync m16n8k32) against 8 blocks a
+//   * 16 tokens of a run (two such tiles a CTA) are the rows of an integer tensor-core tile (mma.sync m16n8k32) against 8 blocks a
 //     step, whose marks come from global memory in fragment order: 16 consecutive bytes are a lane's operands
 //     of two k-steps. One token alone pays for the tile but not for memory: each block's marks are read once.
 //   * the bounds, as words that order like the numbers, stay in shared memory; the words' range is halved
@@ -19,8 +19,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kTile = 16;
+constexpr int kTile = 16;       // tokens of a tensor-core tile
+constexpr int kTileRows = 32;   // of a CTA: two tiles, whose warps read the same marks soon after one another (L1)
+constexpr int kCandidates = 256;
+template <bool WIDE>
+struct Shape {
+    static constexpr int threads = WIDE ? 256 : 512, warps = threads / 32, rows = WIDE ? kTile : kTileRows;
+};
 constexpr unsigned kForced = 0xffffffffu;
 
 struct Args {
@@ -31,7 +36,7 @@ struct Args {
     Kv8Runs runs;
     int top, first, last;
     int *picks;
-    int rows;     // tokens of a CTA (of a cluster), 1 .. 16
+    int rows;     // tokens of a CTA (of a cluster), 1 .. 32
     int tiles;    // CTAs (clusters) a run
     int row_len;  // words between the rows of bounds in shared memory
 };
@@ -59,17 +64,19 @@ __device__ __forceinline__ float row_max(float x, float *red) {
     if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) x = fmaxf(x, red[i]);
+    for (int i = 0; i < Shape<true>::warps; ++i) x = fmaxf(x, red[i]);
     return x;
 }
 
-// WIDE: one token a CTA (cluster), all warps on it. Otherwise up to 16 tokens of a run, a warp to a token.
+// WIDE: one token a CTA (cluster), all warps on it. Otherwise up to 32 tokens of a run, a warp to a token.
 template <int P, bool WIDE>
-__global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constant__ Args A) {
-    extern __shared__ unsigned key_s[];  // [rows][row_len]
-    __shared__ __align__(16) int8_t code_s[kTile][2 * P + 16];  // negative parts, positive parts
+__global__ void __launch_bounds__(Shape<WIDE>::threads, WIDE ? 2 : 1) k_kv8_select(const __grid_constant__ Args A) {
+    constexpr int kThreads = Shape<WIDE>::threads, kWarps = Shape<WIDE>::warps, kRows = Shape<WIDE>::rows;
+    extern __shared__ __align__(16) unsigned key_s[];  // [rows][row_len]
+    __shared__ __align__(16) int8_t code_s[kRows][2 * P + 16];  // negative parts, positive parts
     __shared__ float red[kWarps];
-    __shared__ int count_s[2][kWarps], equal_s[kWarps], have_s[kTile];
+    __shared__ int count_s[2][kWarps], equal_s[kWarps], have_s[kRows];
+    __shared__ unsigned short block_s[WIDE ? 1 : kWarps][kCandidates];
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -80,29 +87,53 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
     if (tid < rows) have_s[tid] = (visible_keys(A.c, at, j0 + tid) + kKvBlock - 1) / kKvBlock;
 
     // the group's queries of each row as two rows of codes
-    constexpr int kEach = WIDE ? (P + kThreads - 1) / kThreads : P / 32;  // channels a thread
-    const int me = WIDE ? tid : lane, step = WIDE ? kThreads : 32;
-    for (int r = WIDE ? 0 : warp; r < (WIDE ? 1 : kTile); r += kWarps) {
+    constexpr int kEach = WIDE ? (P + kThreads - 1) / kThreads : P / 32;  // neighbouring channels of a thread
+    constexpr int kHeads = WIDE ? 16 : 4;                                 // heads whose loads are in flight at a time
+    const int me = WIDE ? tid : lane, step = WIDE ? kThreads : 32, ch0 = me * kEach;
+    for (int r = WIDE ? 0 : warp; r < (WIDE ? 1 : kRows); r += kWarps) {
         int pos[kEach] = {}, neg[kEach] = {};
         if (r < rows) {
-            const float *x = A.q + (token0 + r) * A.stride + (size_t)head * A.group * A.c.dim;
-            float amax = 0.0f;
-            for (int h = 0; h < A.group; ++h)
+            const float *x = A.q + (token0 + r) * A.stride + (size_t)head * A.group * A.c.dim + ch0;
+            const bool wide = kEach % 4 == 0 && ch0 + kEach <= A.c.dim && A.c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+            auto load = [&](int h0, float(&f)[kHeads][kEach]) {
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    const int ch = me + i * step;
-                    if (ch < A.c.dim) amax = fmaxf(amax, fabsf(finite_or_zero(x[h * A.c.dim + ch])));
+                for (int h = 0; h < kHeads; ++h) {
+                    const float *src = x + (size_t)(h0 + h) * A.c.dim;
+                    if (wide) {
+#pragma unroll
+                        for (int i = 0; i < kEach / 4; ++i) {
+                            const float4 v = h0 + h < A.group ? reinterpret_cast<const float4 *>(src)[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            f[h][4 * i] = v.x, f[h][4 * i + 1] = v.y, f[h][4 * i + 2] = v.z, f[h][4 * i + 3] = v.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kEach; ++i) f[h][i] = h0 + h < A.group && ch0 + i < A.c.dim ? src[i] : 0.0f;
+                    }
                 }
+            };
+            float amax = 0.0f;
+            for (int h0 = 0; h0 < A.group; h0 += kHeads) {
+                float f[kHeads][kEach];
+                load(h0, f);
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) amax = fmaxf(amax, fabsf(finite_or_zero(f[h][i])));
+            }
             amax = row_max<WIDE>(amax, red);
             const float unit_of = amax < 0x1p-100f ? 0.0f : __fdiv_rn(32767.0f, amax);
-            for (int h = 0; h < A.group; ++h)
+            for (int h0 = 0; h0 < A.group; h0 += kHeads) {
+                float f[kHeads][kEach];
+                load(h0, f);
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    const int ch = me + i * step;
-                    const int v = ch < A.c.dim ? __float2int_rn(__fmul_rn(finite_or_zero(x[h * A.c.dim + ch]), unit_of)) : 0;
-                    pos[i] += max(v, 0);
-                    neg[i] += min(v, 0);
-                }
+                for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        const int v = __float2int_rn(__fmul_rn(finite_or_zero(f[h][i]), unit_of));
+                        pos[i] += max(v, 0);
+                        neg[i] += min(v, 0);
+                    }
+            }
             float big = 0.0f;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) big = fmaxf(big, (float)max(pos[i], -neg[i]));
@@ -116,28 +147,29 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
         }
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            if (me + i * step < P) {
-                code_s[r][me + i * step] = (int8_t)neg[i];
-                code_s[r][P + me + i * step] = (int8_t)pos[i];
+            if (ch0 + i < P) {
+                code_s[r][ch0 + i] = (int8_t)neg[i];
+                code_s[r][P + ch0 + i] = (int8_t)pos[i];
             }
     }
     if (WIDE)  // the tile's other rows
         for (int i = tid; i < (kTile - 1) * (2 * P + 16) / 4; i += kThreads) reinterpret_cast<int *>(code_s[1])[i] = 0;
     __syncthreads();
     const int most = have_s[rows - 1];
-    if (most > A.top) {
+    const int r0 = WIDE ? 0 : warp / 8 * kTile;  // this warp's tile of rows
+    if (most > A.top && r0 < rows) {
         unsigned a[P / 32][2][4];  // 64-byte segments of the code rows, two k-steps each
 #pragma unroll
         for (int i = 0; i < P / 32; ++i) {
-            const uint4 lo = *reinterpret_cast<const uint4 *>(&code_s[g][i * 64 + t * 16]);
-            const uint4 hi = *reinterpret_cast<const uint4 *>(&code_s[g + 8][i * 64 + t * 16]);
+            const uint4 lo = *reinterpret_cast<const uint4 *>(&code_s[r0 + g][i * 64 + t * 16]);
+            const uint4 hi = *reinterpret_cast<const uint4 *>(&code_s[r0 + g + 8][i * 64 + t * 16]);
             a[i][0][0] = lo.x, a[i][0][2] = lo.y, a[i][1][0] = lo.z, a[i][1][2] = lo.w;
             a[i][0][1] = hi.x, a[i][0][3] = hi.y, a[i][1][1] = hi.z, a[i][1][3] = hi.w;
         }
         unsigned *keys = cluster.map_shared_rank(key_s, 0);
         const int *table = A.c.table + (size_t)at.sequence * A.c.blocks;
-        const int stride_b = 8 * kWarps * ranks;
-        int b0 = (rank * kWarps + warp) * 8;
+        const int stride_b = 64 * ranks;
+        int b0 = (rank * 8 + warp % 8) * 8;
         int entry = b0 + g < most ? table[b0 + g] : -1;
         for (; b0 < most; b0 += stride_b) {
             const int b = b0 + g;
@@ -158,16 +190,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
 #pragma unroll
                 for (int i = 0; i < P / 32; ++i) m[i] = make_uint4(0, 0, 0, 0);
             }
-            int d[4] = {0, 0, 0, 0};
+            int d[4] = {0, 0, 0, 0}, d1[4] = {0, 0, 0, 0};  // two chains, so that one product need not wait for the last
 #pragma unroll
             for (int i = 0; i < P / 32; ++i) {
                 mma_s8(d, a[i][0][0], a[i][0][1], a[i][0][2], a[i][0][3], m[i].x, m[i].y);
-                mma_s8(d, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], m[i].z, m[i].w);
+                mma_s8(d1, a[i][1][0], a[i][1][1], a[i][1][2], a[i][1][3], m[i].z, m[i].w);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] += d1[e];
             const float s0 = __shfl_sync(0xffffffffu, scale, 8 * t), s1 = __shfl_sync(0xffffffffu, scale, 8 * t + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = g + (e >> 1) * 8, block = b0 + 2 * t + (e & 1);
+                const int r = r0 + g + (e >> 1) * 8, block = b0 + 2 * t + (e & 1);
                 if (r >= rows || block >= most) continue;
                 const int have = have_s[r];
                 unsigned key = min(ordered(__fmul_rn((float)d[e], e & 1 ? s1 : s0)), kForced - 1);
@@ -188,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
             for (int i = me; i < A.top; i += step) out[i] = i < have ? i : -1;
             continue;
         }
-        const unsigned *key = key_s + r * A.row_len;
+        unsigned *key = key_s + r * A.row_len;
         // this warp's blocks: all, or an eighth in whole groups of 128
         const int share = WIDE ? (have + 128 * kWarps - 1) / (128 * kWarps) * 128 : have;
         const int from = WIDE ? min(have, warp * share) : 0, to = WIDE ? min(have, from + share) : have;
@@ -202,7 +236,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
             for (int i = 0; i < kWarps; ++i) n += count_s[which][i];
             return n;
         };
-        unsigned lo = kForced, hi = 0;
+        // words in a few registers where they fit
+        constexpr int kHold = 8;
+        unsigned held[kHold];
+        unsigned lo = kForced, hi = 0, first_max = 0, second_max = 0;
         int forced = 0;
         for (int b = from + lane; b < to; b += 32) {
             const unsigned k = key[b];
@@ -211,9 +248,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
                 lo = min(lo, k);
                 hi = max(hi, k);
             }
+            second_max = max(second_max, min(first_max, k));
+            first_max = max(first_max, k);
         }
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
+        int n_words = to - from;
+        unsigned *words = key + from;
+        bool compact = false;
         if (WIDE) {
             if (lane == 0) {
                 count_s[1][warp] = (int)lo;
@@ -225,6 +267,43 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
                 lo = min(lo, (unsigned)count_s[1][i]);
                 hi = max(hi, (unsigned)equal_s[i]);
             }
+        } else if (A.top <= 64) {
+            // 32 (64) words at least reach the least of the lanes' largest (second largest): only those that do are
+            // candidates, and are moved to the front in their order, with their blocks
+            const unsigned least = __reduce_min_sync(0xffffffffu, A.top <= 32 ? first_max : second_max);
+            if (least > lo) {
+                int n = 0;
+                for (int b = lane; b < have; b += 32) n += key[b] >= least;
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (n <= kCandidates && n > A.top) {
+                    compact = true;
+                    lo = least == kForced ? lo : least;
+                    int at = 0;
+                    for (int b = 0; b < have; b += 128) {
+                        unsigned k[4], ballot[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) k[i] = b + 32 * i + lane < have ? key[b + 32 * i + lane] : 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ballot[i] = __ballot_sync(0xffffffffu, k[i] >= least);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (k[i] >= least) {
+                                const int to_at = at + __popc(ballot[i] & ((1u << lane) - 1));
+                                key[to_at] = k[i];
+                                block_s[warp][to_at] = (unsigned short)(b + 32 * i + lane);
+                            }
+                            at += __popc(ballot[i]);
+                        }
+                        __syncwarp();
+                    }
+                    n_words = n;
+                }
+            }
+        }
+        const bool hold = n_words <= 32 * kHold;  // (of every warp on the row: they share alike)
+        if (hold) {
+#pragma unroll
+            for (int i = 0; i < kHold; ++i) held[i] = i * 32 + lane < n_words ? words[i * 32 + lane] : 0;
         }
         // at least `top` words reach lo, `above` <= top reach hi; halve until as many as wanted do, or equal words
         // (lo, all of them) are left to fill up with
@@ -233,9 +312,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
         while (above != A.top && hi - lo > 1) {
             const unsigned mid = lo + (hi - lo) / 2;
             int n = 0;
-            for (int b = from + 4 * lane; b < to; b += 128) {  // (words past the row's last block are zero up to a multiple of 4)
-                const uint4 k = *reinterpret_cast<const uint4 *>(key + b);
-                n += (k.x >= mid) + (b + 1 < to && k.y >= mid) + (b + 2 < to && k.z >= mid) + (b + 3 < to && k.w >= mid);
+            if (hold) {
+#pragma unroll
+                for (int i = 0; i < kHold; ++i) n += held[i] >= mid;
+            } else {
+                for (int b = 4 * lane; b < n_words; b += 128) {
+                    const uint4 k = *reinterpret_cast<const uint4 *>(words + b);
+                    n += (k.x >= mid) + (b + 1 < n_words && k.y >= mid) + (b + 2 < n_words && k.z >= mid) + (b + 3 < n_words && k.w >= mid);
+                }
             }
             n = row_sum(n, turn);
             turn ^= 1;
@@ -267,13 +351,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_select(const __grid_constan
                 room -= take;
             }
         }
-        for (int b = from; b < to; b += 32) {
-            const unsigned k = b + lane < to ? key[b + lane] : 0;
-            const bool up = k >= hi, eq = !up && k == lo && b + lane < to;
+        for (int b = 0; b < n_words; b += 32) {
+            const unsigned k = b + lane < n_words ? words[b + lane] : 0;
+            const bool up = k >= hi, eq = !up && k == lo && b + lane < n_words;
             const unsigned equals = __ballot_sync(0xffffffffu, eq);
             const bool take = up || (eq && __popc(equals & ((1u << lane) - 1)) < room);
             const unsigned all = __ballot_sync(0xffffffffu, take);
-            if (take) out[at_out + __popc(all & ((1u << lane) - 1))] = b + lane;
+            if (take) out[at_out + __popc(all & ((1u << lane) - 1))] = compact ? block_s[WIDE ? 0 : warp][b + lane] : from + b + lane;
             at_out += __popc(all);
             room -= min(room, __popc(equals));
         }
@@ -288,7 +372,7 @@ cudaError_t launch(const Args &A, int ranks, size_t smem, cudaStream_t s) {
     if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(Shape<WIDE>::threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr;
@@ -304,14 +388,14 @@ cudaError_t launch(const Args &A, int ranks, size_t smem, cudaStream_t s) {
 
 cudaError_t kv8_select(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, int top, int first, int last, int *picks,
                        cudaStream_t s) {
-    constexpr int kSms = 148, kKeyBytes = 96 * 1024;  // two CTAs' bounds fit an SM
+    constexpr int kSms = 148, kKeyBytes = 184 * 1024;  // of a CTA's bounds, beside the codes and candidates
     Args A{c, q, stride, heads, heads / c.kv_heads, r, top, first, last, picks, 1, r.count, (c.blocks + 3) / 4 * 4};
     const long long tokens = (long long)r.segments * r.count * c.kv_heads;
-    // Tiles of up to 16 tokens where they give every multiprocessor one: marks are then read once for 16 tokens
+    // Tiles of up to 32 tokens where half of the multiprocessors get one: marks are then read once for 16 or 32 tokens
     int rows = kKeyBytes / (A.row_len * 4);
-    rows = rows > kTile ? kTile : rows;
+    rows = rows > kTileRows ? kTileRows : rows;
     if (rows > r.count) rows = r.count;
-    if (rows > 1 && tokens >= (long long)rows * kSms) {
+    if (rows > 1 && tokens >= (long long)rows * kSms / 2) {
         A.rows = rows;
         A.tiles = (r.count + rows - 1) / rows;
         const size_t smem = (size_t)rows * A.row_len * 4;
