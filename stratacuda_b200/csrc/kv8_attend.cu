@@ -10,12 +10,13 @@
 //       TMEM over up to 256 pages
 // A thread of the softmax warps has one of the step's tokens (its TMEM lane): it puts the rows' logits together
 // from their digits, takes the exponentials, and writes the weights' digits as the second product's operand.
-// Logits, maxima and sums of weights are F32. A row's weights refer to a maximum that follows the true one only
-// when a weight would pass 8; then, and at the unit's end, the sums move from TMEM to F32 registers.
+// Logits, references and sums of weights are F32. A row's weights refer to a power of two some way above its maximum,
+// which moves only when a weight would pass 8; then, and at the unit's end, the sums move from TMEM to F32 registers.
 //
-// Warps: 0-3 softmax, sums and results; 4 looks pages up and fetches keys and values by TMA (64-byte swizzle) into
-// two rings, ahead across units; 5 issues the products, S of the next step before O of this; 6-7 make the
-// next unit's query digits. One CTA a multiprocessor; every wait is bounded, and past the limit all leave.
+// Warps: 0-3 and 4-7 are two softmax groups that take the steps in turn, each with references and sums of its own
+// (joined at the unit's end), so that one's latencies run under the other's work; 8 looks pages up and fetches
+// keys and values by TMA (64-byte swizzle), ahead across units; one thread of 9 issues S, up to four steps ahead, one
+// of 11 O; 10 makes the next unit's query digits. One CTA a multiprocessor; every wait is bounded, and past the limit all leave.
 //
 // Few units (`split`): the pages of all units form one list that the CTAs share evenly, whatever the
 // lengths; a unit cut by a CTA border leaves unnormalised partial sums in the workspace and a
@@ -34,14 +35,16 @@ namespace {
 
 using namespace pf;
 
-constexpr int kSoft = 128, kFetchWarp = 4, kIssueWarp = 5, kQueryWarp = 6, kThreads = 256;
+constexpr int kSoft = 128, kKeyWarp = 8, kIssueWarp = 9, kSumWarp = 11, kThreads = 384;  // kSoft: threads of a softmax group
+constexpr int kSteps = 8;         // steps looked up ahead
 constexpr int kJoinThreads = 256;
 constexpr int kRows = 16;
 constexpr int kMaxTokens = 1024;  // tokens of a split call (their page counts are summed up in shared memory)
 constexpr int kMaxCtas = 640;     // CTAs of a split call: two partial results each in the workspace
 constexpr int kFlushSteps = 128;  // steps that TMEM's 32-bit sums bear (255 * 127 * 128 tokens a step)
-constexpr float kGrow = 8.0f;     // weights stay below this, times
+constexpr float kGrow = 8.0f;          // weights stay below this, times
 constexpr float kUnit = 268435456.0f;  // 2^28, below 2^32
+constexpr float kRoom = 3.0f;          // log2 of the room that a new reference leaves above the maximum, so that it seldom moves again
 constexpr long long kWaitClocks = 2000000000;  // about a second
 
 // Workspace of a split call: page counts are not kept, only what the joining kernel reads.
@@ -80,13 +83,12 @@ struct Shape {
     static constexpr int panels = P / 64;
     static constexpr int blocks = P <= 128 ? 1 : 2;             // of 128 channels
     static constexpr int ns = (3 * R + 15) / 16 * 16, nw = 4 * R;  // columns of S and O
-    static constexpr int k_ring = 3, v_ring = P == 256 ? 5 : 6;  // steps (two pages), pages
+    static constexpr int k_ring = P == 256 ? 2 : 3, v_ring = P == 256 ? 3 : 4;  // steps
 };
-// What a slot of the key ring holds: 1 or 2 pages, the end of a unit (0), or the end of all (-1).
+// A step: 1 or 2 pages, the end of a unit (0), or the end of all (-1).
 struct Step {
-    int pages, block[2];
+    int pages, unit, block[2];
     float k_scale[2], v_scale[2];
-    int pad;
 };
 struct Unit {  // or the part of it that this CTA works on: entries [entry, stop) of its n
     int token, sub, entry, stop, n, seen, sequence, last_cta;
@@ -95,10 +97,10 @@ template <int P, int R>
 struct __align__(1024) Smem {
     using Z = Shape<P, R>;
     unsigned char k[Z::k_ring][Z::panels][128 * 64];  // tokens of two pages, 64 channels a row
-    unsigned char v[Z::v_ring][P * 64];               // channels, 64 tokens a row
+    unsigned char v[Z::v_ring][2][P * 64];            // two pages: channels, 64 tokens a row
     unsigned char v_end[P == 64 ? 4096 : 1024];       // (a 64-channel page is read as 128 rows)
     unsigned char q[2][Z::panels][Z::ns * 64];        // row 3 r + digit: 64 channels
-    unsigned char w[2][2][Z::nw * 64];                // by step parity and page: row 4 r + digit: 64 tokens
+    unsigned char w[2][2][Z::nw * 64];                // by group and page: row 4 r + digit: 64 tokens
     union {
         struct {
             long long before[kMaxTokens + 1];  // used before the first page is
@@ -106,20 +108,23 @@ struct __align__(1024) Smem {
         };
         struct {
             float row_scale[2][kRows];
-            float row_top[4][kRows];
+            float row_top[2][4][kRows];
+            float2 group_row[kRows];  // the second group's reference and sum of weights
             Unit unit[2];
-            Step step[Z::k_ring];
-            int fresh[2];  // by step parity: O starts from zero
+            Step step[kSteps];
+            float4 list[32];  // pages looked up: page, block (bits), key scale, value scale
+            float group_ref;
+            int what[2];  // by group: pages whose weights are there (-1: no more), plus 4 where O starts from zero
         };
     };
-    unsigned long long k_full[Z::k_ring], k_empty[Z::k_ring], v_full[Z::v_ring], v_empty[Z::v_ring];
-    unsigned long long q_full[2], q_empty[2], s_full[2], s_free[2], w_full[2], o_done[2], drained;
+    unsigned long long step_full[kSteps], step_empty[kSteps], k_full[Z::k_ring], k_empty[Z::k_ring], v_full[Z::v_ring], v_empty[Z::v_ring];
+    unsigned long long q_full[2], q_empty[2], s_full[4], s_free[4], w_full[2], o_done[2], hand_full, hand_free, drained[2];
     unsigned tmem;
     int abort_flag;
 };
 
 struct RowArgs : Args {
-    CUtensorMap codes;  // {64 bytes, rows of a page, pages}, boxes of 64 rows, 64-byte swizzle
+    CUtensorMap keys, values;  // {64 bytes, rows of a page, pages}, 64-byte swizzle; boxes of 64 rows, of P rows
 };
 
 // Entries of a token's page list: every block in sight, or its picks.
@@ -195,18 +200,24 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, int *r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // 2^x for a whole x <= 0 or -infinity, exactly; NaN (-infinity less itself) is 1.
 __device__ __forceinline__ float two_to(float x) { return x < -126.0f ? 0.0f : isnan(x) ? 1.0f : __uint_as_float((unsigned)(127 + (int)x) << 23); }
-// OR of x over the softmax warps (named barrier 1).
-__device__ __forceinline__ bool soft_or(bool x) {
+// OR of x over a named barrier's threads: a softmax group's (barriers 1 and 2).
+__device__ __forceinline__ bool bar_or(int barrier, int threads, bool x) {
     unsigned r;
     asm volatile(
         "{\n\t.reg .pred pi, po;\n\t"
         "setp.ne.u32 pi, %1, 0;\n\t"
-        "bar.red.or.pred po, 1, 128, pi;\n\t"
+        "bar.red.or.pred po, %2, %3, pi;\n\t"
         "selp.u32 %0, 1, 0, po;\n\t}"
         : "=r"(r)
-        : "r"((unsigned)x)
+        : "r"((unsigned)x), "r"(barrier), "r"(threads)
         : "memory");
     return r != 0;
+}
+// The largest of x over the warp; NaN only where all are.
+__device__ __forceinline__ float warp_max(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 template <int P, int R>
@@ -218,13 +229,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
     const int tokens = A.runs.segments * A.runs.count, per_token = A.c.kv_heads * A.tiles;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
-        for (int i = 0; i < Z::k_ring; ++i) bar_init(&M.k_full[i], 1), bar_init(&M.k_empty[i], 1 + kSoft / 32);
+        for (int i = 0; i < Z::k_ring; ++i) bar_init(&M.k_full[i], 1), bar_init(&M.k_empty[i], 1);
+        // read by the softmax warps and the one that issues S
+        for (int i = 0; i < kSteps; ++i) bar_init(&M.step_full[i], 1), bar_init(&M.step_empty[i], 2 * kSoft / 32 + 1);
         for (int i = 0; i < Z::v_ring; ++i) bar_init(&M.v_full[i], 1), bar_init(&M.v_empty[i], 1);
         for (int i = 0; i < 2; ++i) {
-            bar_init(&M.q_full[i], 64), bar_init(&M.q_empty[i], 1 + kSoft / 32);
-            bar_init(&M.s_full[i], 1), bar_init(&M.s_free[i], kSoft), bar_init(&M.w_full[i], kSoft), bar_init(&M.o_done[i], 1);
+            bar_init(&M.q_full[i], 32), bar_init(&M.q_empty[i], 1 + 2 * kSoft / 32);
+            bar_init(&M.w_full[i], kSoft), bar_init(&M.o_done[i], 1);
         }
-        bar_init(&M.drained, 1);
+        for (int i = 0; i < 4; ++i) bar_init(&M.s_full[i], 1), bar_init(&M.s_free[i], kSoft);
+        bar_init(&M.hand_full, kSoft), bar_init(&M.hand_free, kSoft);
+        bar_init(&M.drained[0], 1), bar_init(&M.drained[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         M.abort_flag = 0;
     }
@@ -265,14 +280,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
         walk.sub = (int)(in / n);
         walk.entry = (int)(in % n);
     }
-    if (warp == kIssueWarp) {  // TMEM: two buffers of S, 64 columns each, and O, 64 columns a block of 128 channels
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(su32(&M.tmem)) : "memory");
+    if (warp == kIssueWarp) {  // TMEM: four buffers of S, 64 columns each, and each group's O, 64 columns a block of 128 channels
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&M.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const unsigned tmem = M.tmem, tmem_o = tmem + 128;
+    const unsigned tmem = M.tmem, tmem_o = tmem + 256;
     auto wait = [&](unsigned long long *b, unsigned parity) -> bool {
         if (bar_try(b, parity)) return true;
         for (const long long began = clock64(); clock64() - began < kWaitClocks;) {
@@ -283,23 +298,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
         return false;
     };
     auto wait_all = [&](unsigned long long *b, unsigned parity) { return (bool)__all_sync(0xffffffffu, wait(b, parity)); };
+    auto wait_out = [&](unsigned long long *b, unsigned parity) {  // the same where others have failed: only the limit ends it
+        for (const long long began = clock64(); clock64() - began < kWaitClocks && !bar_try(b, parity);) {
+        }
+    };
 
-    if (warp < kSoft / 32) {
+    if (warp < kKeyWarp) {
         // ---------------------------------------------------------------- softmax, sums and results
-        const int page = warp >> 1, token_in = (warp & 1) * 32 + lane;  // this thread's token of a step
-        const unsigned mine = (unsigned)(warp * 32) << 16;
-        unsigned kc = 0, sc = 0;  // key slots, and of them steps with pages, used
-        bool ok = true;
+        const int group = warp >> 2, quarter = warp & 3, page = quarter >> 1, token_in = (quarter & 1) * 32 + lane;  // this thread's token of a step
+        const int thread = tid & (kSoft - 1);
+        const unsigned mine = (unsigned)(quarter * 32) << 16, own_o = tmem_o + 128 * group;
+        unsigned kc = 0, sc = 0;  // steps, and of them those with pages, so far
+        bool ok = true, handed = false;  // handed: the second group's last hand-over may not be taken yet
         // Every barrier of these warps is a vote; when it is not unanimous, a second one says whether to leave, so that all
-        // leave together, wherever each of them is
-        auto leave = [&]() { return soft_or(!ok || *(volatile int *)&M.abort_flag); };
-        auto meet = [&]() { return !soft_or(!ok) || !leave(); };
+        // leave together, wherever each of them is. Between the groups there are only bounded waits.
+        auto leave = [&]() { return bar_or(1 + group, kSoft, !ok || *(volatile int *)&M.abort_flag); };
+        auto meet = [&]() { return !bar_or(1 + group, kSoft, !ok) || !leave(); };
         for (unsigned un = 0;; ++un) {
             const unsigned qb = un & 1;
             ok = wait_all(&M.q_full[qb], un >> 1 & 1);
             if (!meet()) break;
             const Unit u = M.unit[qb];
-            if (u.token < 0) break;
+            if (u.token < 0) {  // the group whose step would be next says so to the warp that issues O
+                if ((sc & 1) == group) {
+                    if (sc >= 2) ok = wait_all(&M.o_done[group], (sc - 2) >> 1 & 1);
+                    if (thread == 0) M.what[group] = -1;
+                    bar_arrive(&M.w_full[group]);
+                }
+                break;
+            }
             float m[R], sum[R], rs[R], o[Z::blocks][R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
@@ -311,49 +338,59 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
             if (lane == 0) bar_arrive(&M.q_empty[qb]);
             float ref = 0.0f;  // a power of two near the first page's value scale: what a weight's digits refer to
             int held = 0;      // steps whose products are in TMEM's sums
-            // TMEM's sums of all steps before step number sc join o
+            unsigned last = 0;  // the group's last step
+            // TMEM's sums join o
             auto flush = [&]() {
-                const unsigned last = sc - 1;
-                if (!wait_all(&M.o_done[last & 1], last >> 1 & 1)) return false;
+                if (!wait_all(&M.o_done[group], last >> 1 & 1)) return false;
                 tc_fence_after();
 #pragma unroll
-                for (int b = 0; b < Z::blocks; ++b)
+                for (int b = 0; b < Z::blocks; ++b) {
+                    int x[Z::nw];
 #pragma unroll
-                    for (int c = 0; c < Z::nw; c += 16) {
-                        int x[16];
-                        tmem_ld16(tmem_o + mine + 64 * b + c, x);
-                        tmem_wait_ld();
+                    for (int c = 0; c < Z::nw; c += 16) tmem_ld16(own_o + mine + 64 * b + c, x + c);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            o[b][c / 4 + r] += fmaf(fmaf(fmaf((float)x[4 * r + 3], 256.0f, (float)x[4 * r + 2]), 256.0f, (float)x[4 * r + 1]), 256.0f,
-                                                    (float)x[4 * r]);
-                    }
+                    for (int r = 0; r < R; ++r)
+                        o[b][r] += fmaf(fmaf(fmaf((float)x[4 * r + 3], 256.0f, (float)x[4 * r + 2]), 256.0f, (float)x[4 * r + 1]), 256.0f,
+                                        (float)x[4 * r]);
+                }
                 tc_fence_before();
                 held = 0;
                 return true;
             };
+            auto taken = [&]() {  // before O's columns of TMEM or the other places are written again
+                if (handed) ok = ok && wait_all(&M.hand_free, (un - 1) & 1);
+                handed = false;
+            };
             bool gone = false;
             for (;;) {
-                const unsigned ks = kc % Z::k_ring, buf = sc & 1;
-                float a[R], p[R], f = 0.0f;
+                const unsigned ks = kc % kSteps, buf = sc & 3;
+                float a[R], f = 0.0f, lift = 0.0f;
                 bool grows = false, here = false;
-                ok = ok && wait_all(&M.k_full[ks], kc / Z::k_ring & 1);
+                int pages_now = 0;
+                ok = ok && wait_all(&M.step_full[ks], kc / kSteps & 1);
                 if (ok) {
                     const int pages = M.step[ks].pages, block = M.step[ks].block[page];
                     const float by_k = M.step[ks].k_scale[page], by_v = M.step[ks].v_scale[page], first_v = M.step[ks].v_scale[0];
                     __syncwarp();
-                    if (lane == 0) bar_arrive(&M.k_empty[ks]);
+                    if (lane == 0) bar_arrive(&M.step_empty[ks]);
                     ++kc;
                     if (pages == 0) break;
+                    if ((sc & 1) != group) {  // the other group's step
+                        ++sc;
+                        continue;
+                    }
                     if (ref == 0.0f) ref = first_v > 0x1p-120f ? __uint_as_float(__float_as_uint(first_v) & 0x7f800000u) : 1.0f;
                     f = by_v / ref;
                     here = page < pages;
+                    pages_now = pages;
                     const int left = here ? u.seen - block * kKvBlock - token_in : 0;
-                    ok = wait_all(&M.s_full[buf], sc >> 1 & 1);
+                    ok = wait_all(&M.s_full[buf], sc >> 2 & 1);
                     tc_fence_after();
                     int s[Z::ns];
 #pragma unroll
                     for (int c = 0; c < Z::ns; c += 16) tmem_ld16(tmem + mine + 64 * buf + c, s + c);
+                    lift = fmaxf(f > 0.0f ? log2f(f) : -40.0f, -40.0f);
                     tmem_wait_ld();
                     tc_fence_before();
                     bar_arrive(&M.s_free[buf]);
@@ -362,25 +399,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
                         // 256 d1 + d0 stays inside 31 bits for 256 channels of codes
                         a[r] = fmaf((float)s[3 * r + 2], 65536.0f, (float)(s[3 * r + 1] * 256 + s[3 * r])) * (by_k * rs[r]);
                         a[r] = left > 0 ? a[r] : -INFINITY;
-                        const float e = a[r] - m[r];
-                        p[r] = exp2_fast(e);
-                        grows |= p[r] * f > kGrow || e > 60.0f;
+                        grows |= a[r] + lift > m[r] + kGrow;
                     }
                 }
-                if (soft_or(grows || !ok)) {
+                if (bar_or(1 + group, kSoft, grows || !ok)) {
                     if (leave()) {
                         gone = true;
                         break;
                     }
                     // all rows move to their maximum over the step
                     if (held) ok = flush();
-                    const float lift = fmaxf(f > 0.0f ? log2f(f) : -40.0f, -40.0f);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        float top = a[r] + lift;
-#pragma unroll
-                        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        if (lane == 0) M.row_top[warp][r] = top;
+                        const float top = warp_max(a[r] + lift);
+                        if (lane == 0) M.row_top[group][quarter][r] = top;
                     }
                     if (!meet()) {
                         gone = true;
@@ -388,235 +420,265 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
                     }
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        const float now = fmaxf(m[r], ceilf(fmaxf(fmaxf(M.row_top[0][r], M.row_top[1][r]), fmaxf(M.row_top[2][r], M.row_top[3][r]))));
+                        const float(*top)[kRows] = M.row_top[group];
+                        const float now = fmaxf(m[r], ceilf(fmaxf(fmaxf(top[0][r], top[1][r]), fmaxf(top[2][r], top[3][r]))) + kRoom);
                         const float alpha = two_to(m[r] - now);
                         m[r] = now;
                         sum[r] *= alpha;
 #pragma unroll
                         for (int b = 0; b < Z::blocks; ++b) o[b][r] *= alpha;
-                        p[r] = exp2_fast(a[r] - (now == -INFINITY ? 0.0f : now));
                     }
                 } else if (held == kFlushSteps) {
                     ok = flush();
                 }
                 // the weights' digits; the buffer's last use is over when that step's products are
-                if (sc >= 2) ok = ok && wait_all(&M.o_done[buf], (sc - 2) >> 1 & 1);
+                if (sc >= 2) ok = ok && wait_all(&M.o_done[group], (sc - 2) >> 1 & 1);
+                taken();
                 if (here && ok) {
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        sum[r] += p[r];
-                        const unsigned w = __float2uint_rn(p[r] * f * kUnit);
+                        const float p = exp2_fast(a[r] - (m[r] == -INFINITY ? 0.0f : m[r]));
+                        sum[r] += p;
+                        const unsigned w = __float2uint_rn(p * f * kUnit);
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) M.w[buf][page][sw64_byte(4 * r + d, token_in)] = (unsigned char)(w >> (8 * d));
+                        for (int d = 0; d < 4; ++d) M.w[group][page][sw64_byte(4 * r + d, token_in)] = (unsigned char)(w >> (8 * d));
                     }
                 }
-                if (tid == 0) M.fresh[buf] = held == 0;
+                if (thread == 0) M.what[group] = pages_now + (held == 0 ? 4 : 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(&M.w_full[buf]);
+                bar_arrive(&M.w_full[group]);
+                last = sc;
                 ++held;
                 ++sc;
             }
             if (gone) break;
             if (held) ok = flush();
-            // ---- the unit is done: the rows' sums over the tokens, then the result or its part
+            // ---- the unit is done: the rows' sums over the group's tokens
 #pragma unroll
             for (int r = 0; r < R; ++r) {
 #pragma unroll
                 for (int x = 16; x > 0; x >>= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], x);
-                if (lane == 0) M.row_top[warp][r] = sum[r];
+                if (lane == 0) M.row_top[group][quarter][r] = sum[r];
             }
             if (!meet()) break;
 #pragma unroll
-            for (int r = 0; r < R; ++r) sum[r] = (M.row_top[0][r] + M.row_top[1][r]) + (M.row_top[2][r] + M.row_top[3][r]);
-            const int head = u.sub / A.tiles, row0 = u.sub % A.tiles * kRows, rows = min(kRows, A.group - row0);
-            const float scale = ref / kUnit;
-            if (u.entry == 0 && u.stop == u.n) {
-                float *dst = A.y + ((size_t)u.token * A.heads + head * A.group + row0) * A.c.dim;
+            for (int r = 0; r < R; ++r) {
+                const float(*part)[kRows] = M.row_top[group];
+                sum[r] = (part[0][r] + part[1][r]) + (part[2][r] + part[3][r]);
+            }
+            // the second group hands its own over, O through its columns of TMEM, and the first writes the result
+            if (group == 1) {
+                taken();
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float inv = sum[r] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[r]);
+                for (int b = 0; b < Z::blocks; ++b) {
+                    unsigned x[16];
 #pragma unroll
-                    for (int b = 0; b < Z::blocks; ++b) {
-                        const int ch = 128 * b + tid;
-                        if (r < rows && ch < A.c.dim) dst[(size_t)r * A.c.dim + ch] = o[b][r] * inv * scale;
-                    }
+                    for (int r = 0; r < 16; ++r) x[r] = r < R ? __float_as_uint(o[b][r < R ? r : 0]) : 0u;
+                    tmem_st16(own_o + mine + 64 * b, x);
                 }
-            } else {
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (thread == r) M.group_row[r] = make_float2(m[r], sum[r]);
+                if (thread == 0) M.group_ref = ref;
+                bar_arrive(&M.hand_full);
+                handed = true;
+                continue;
+            }
+            ok = wait_all(&M.hand_full, un & 1);
+            if (!meet()) break;
+            {
+                tc_fence_after();
+                const float other_ref = M.group_ref / kUnit, own_ref = ref / kUnit;
+                const int head = u.sub / A.tiles, row0 = u.sub % A.tiles * kRows, rows = min(kRows, A.group - row0);
+                const bool whole = u.entry == 0 && u.stop == u.n;
                 const Parts W = parts_of(A.c.workspace, P);
                 const int slot = 2 * blockIdx.x + (u.entry == 0);  // a CTA's first unit may have begun earlier, its last may go on
+                float *dst = A.y + ((size_t)u.token * A.heads + head * A.group + row0) * A.c.dim;
+                float f0[R], f1[R];
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    if (tid == 0) W.ml[slot * kRows + r] = make_float2(m[r], sum[r]);
+                    const float2 x = M.group_row[r];
+                    const float now = fmaxf(m[r], x.x), l0 = two_to(m[r] - now), l1 = two_to(x.x - now);
+                    sum[r] = sum[r] * l0 + x.y * l1;
+                    m[r] = now;
+                    const float by = !whole ? 1.0f : sum[r] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[r]);
+                    f0[r] = l0 * by;
+                    f1[r] = l1 * by;
+                }
 #pragma unroll
-                    for (int b = 0; b < Z::blocks; ++b)
-                        if (128 * b + tid < P) W.acc[((size_t)slot * kRows + r) * P + 128 * b + tid] = o[b][r] * scale;
+                for (int b = 0; b < Z::blocks; ++b) {
+                    int x[16];
+                    tmem_ld16(tmem_o + 128 + mine + 64 * b, x);
+                    tmem_wait_ld();
+                    const int ch = 128 * b + thread;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float out = o[b][r] * f0[r] * own_ref + __int_as_float(x[r]) * f1[r] * other_ref;
+                        if (whole) {
+                            if (r < rows && ch < A.c.dim) dst[(size_t)r * A.c.dim + ch] = out;
+                        } else if (ch < P) {
+                            W.acc[((size_t)slot * kRows + r) * P + ch] = out;
+                        }
+                    }
+                }
+                if (!whole && thread == 0)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) W.ml[slot * kRows + r] = make_float2(m[r], sum[r]);
+                if (u.last_cta >= 0 && thread == 0) W.cover[u.token * per_token + u.sub] = make_int2(blockIdx.x, u.last_cta);
+                tc_fence_before();
+                bar_arrive(&M.hand_free);
+            }
+        }
+    } else if (warp == kKeyWarp) {
+        // ---------------------------------------------------------------- pages, keys and values
+        unsigned kc = 0, sc = 0, vc = 0;  // steps; of them those with pages, and those whose values have been asked for
+        bool ok = true;
+        // a batch: up to 32 entries of a unit, an entry a lane, looked up while the batch before it is being fetched
+        struct {
+            int unit, head, page, block;  // unit -1: there is no more
+            float k_scale, v_scale;
+            bool end;  // of the unit
+        } batch;
+        Unit u;
+        int unit = -1, base = 0;
+        u.stop = 0;
+        auto look_up = [&]() {
+            if (base >= u.stop) {
+                if (!walk.next(A, per_token, tokens, u)) {
+                    batch.unit = -1;
+                    return;
+                }
+                ++unit;
+                base = u.entry;
+            }
+            batch.unit = unit;
+            batch.head = u.sub / A.tiles;
+            batch.page = -1;
+            if (base + lane < u.stop) {
+                batch.block = A.picks ? A.picks[((size_t)u.token * A.c.kv_heads + batch.head) * A.top + base + lane] : base + lane;
+                if (batch.block >= 0 && batch.block < (u.seen + kKvBlock - 1) / kKvBlock) batch.page = page_of(A.c, u.sequence, batch.block);
+                if (batch.page >= 0) {
+                    const float *f = page_scales(A.c, batch.page, batch.head);
+                    batch.k_scale = f[0], batch.v_scale = f[1];
                 }
             }
-            if (u.last_cta >= 0 && tid == 0) parts_of(A.c.workspace, P).cover[u.token * per_token + u.sub] = make_int2(blockIdx.x, u.last_cta);
-            if (!meet()) break;  // row_top is free
-        }
-    } else if (warp == kFetchWarp) {
-        // ---------------------------------------------------------------- pages
-        unsigned kc = 0, vc = 0;  // key and value slots asked for
-        bool ok = true;
-        Unit u;
-        auto keys = [&](int n, const int(&page)[2], const int(&block)[2], const float2(&sc)[2], int head) {
-            const unsigned s = kc % Z::k_ring;
-            if (!wait_all(&M.k_empty[s], (kc / Z::k_ring & 1) ^ 1)) return false;
+            base += 32;
+            batch.end = base >= u.stop;
+        };
+        // a step's copies: a lane a box, of 64 key rows or of a page's values
+        auto post = [&](int n, int unit_of, int head, int at) {
+            const unsigned s = kc % kSteps, k = sc % Z::k_ring, v = vc % Z::v_ring;
+            if (!wait_all(&M.step_empty[s], (kc / kSteps & 1) ^ 1)) return false;
             if (lane == 0) {
-                M.step[s] = Step{n, {block[0], block[1]}, {sc[0].x, sc[1].x}, {sc[0].y, sc[1].y}, 0};
-                if (n > 0) {
-                    bar_expect(&M.k_full[s], n * P * kKvBlock);
-                    for (int i = 0; i < n; ++i)
-                        for (int b = 0; b < Z::panels; ++b) tma3(M.k[s][b] + i * 4096, &A.codes, 0, head * 2 * P + 64 * b, page[i], &M.k_full[s]);
-                } else {
-                    bar_arrive(&M.k_full[s]);
-                }
+                const float4 x = M.list[at & 31], y = M.list[(at + 1) & 31];
+                M.step[s] = Step{n, unit_of, {__float_as_int(x.y), __float_as_int(y.y)}, {x.z, y.z}, {x.w, y.w}};
+                bar_arrive(&M.step_full[s]);
             }
             ++kc;
-            return true;
-        };
-        auto values = [&](int page, int head) {
-            const unsigned s = vc % Z::v_ring;
-            if (!wait_all(&M.v_empty[s], (vc / Z::v_ring & 1) ^ 1)) return false;
-            if (lane == 0) {
-                bar_expect(&M.v_full[s], P * kKvBlock);
-                for (int b = 0; b < Z::panels; ++b) tma3(M.v[s] + b * 4096, &A.codes, 0, head * 2 * P + P + 64 * b, page, &M.v_full[s]);
-            }
+            if (n <= 0) return true;
+            if (!wait_all(&M.k_empty[k], (sc / Z::k_ring & 1) ^ 1)) return false;
+            if (lane == 0) bar_expect(&M.k_full[k], n * P * kKvBlock);
+            __syncwarp();
+            if (lane < n * Z::panels)
+                tma3(M.k[k][lane % Z::panels] + lane / Z::panels * 4096, &A.keys, 0, head * 2 * P + 64 * (lane % Z::panels),
+                     __float_as_int(M.list[at + lane / Z::panels].x), &M.k_full[k]);
+            ++sc;
+            if (!wait_all(&M.v_empty[v], (vc / Z::v_ring & 1) ^ 1)) return false;
+            if (lane == 0) bar_expect(&M.v_full[v], n * P * kKvBlock);
+            __syncwarp();
+            if (lane < n) tma3(M.v[v][lane], &A.values, 0, head * 2 * P + P, __float_as_int(M.list[at + lane].x), &M.v_full[v]);
             ++vc;
             return true;
         };
-        const int none[2] = {-1, -1};
-        const float2 zero[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        while (ok && walk.next(A, per_token, tokens, u)) {
-            const int head = u.sub / A.tiles, nb = (u.seen + kKvBlock - 1) / kKvBlock;
-            int page2[2] = {-1, -1}, block2[2] = {0, 0}, n = 0, behind[2] = {-1, -1};  // the step at hand; values still to be asked for
-            float2 scale2[2] = {zero[0], zero[1]};
-            auto step = [&]() {  // this step's keys, then the last step's values, which are wanted a step later
-                ok = keys(n, page2, block2, scale2, head);
+        look_up();
+        while (ok && batch.unit >= 0) {
+            const int this_unit = batch.unit, head = batch.head;
+            const bool end = batch.end;
+            const unsigned there = __ballot_sync(0xffffffffu, batch.page >= 0);
+            const int count = __popc(there);
+            if (batch.page >= 0)
+                M.list[__popc(there & ((1u << lane) - 1))] =
+                    make_float4(__int_as_float(batch.page), __int_as_float(batch.block), batch.k_scale, batch.v_scale);
+            __syncwarp();
+            for (int at = 0; at < count && ok; at += 2) {
+                ok = post(min(2, count - at), this_unit, head, at);
+                if (at == 2) look_up();  // the rings are full for a while
+            }
+            if (count <= 2) look_up();
+            if (ok && end) ok = post(0, this_unit, head, 0);
+        }
+        if (ok) ok = post(-1, unit + 1, 0, 0);
+        if (!ok && lane == 0) {  // let what is in flight land: the last copy of each slot, within the limit
+            for (unsigned i = 1; i <= Z::k_ring && i <= sc; ++i) wait_out(&M.k_full[(sc - i) % Z::k_ring], (sc - i) / Z::k_ring & 1);
+            for (unsigned i = 1; i <= Z::v_ring && i <= vc; ++i) wait_out(&M.v_full[(vc - i) % Z::v_ring], (vc - i) / Z::v_ring & 1);
+        }
+    } else if (warp == kSumWarp) {
+        // ---------------------------------------------------------------- O
+        if (lane == 0) {
+            const unsigned id_o = idesc_i8(Z::nw, false);
+            for (unsigned sc = 0;; ++sc) {
+                const unsigned group = sc & 1, s = sc % Z::v_ring;
+                if (!wait(&M.w_full[group], sc >> 1 & 1)) break;
+                const int what = M.what[group], pages = what & 3;
+                if (what < 0 || !wait(&M.v_full[s], sc / Z::v_ring & 1)) break;
+                tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (ok && behind[i] >= 0) ok = values(behind[i], head);
-                    behind[i] = i < n ? page2[i] : -1;
-                }
-                n = 0;
-            };
-            for (int base = u.entry; base < u.stop && ok; base += 32) {
-                // 32 entries looked up at a time, then those that are there in order
-                int page = -1, block = -1;
-                float2 sc = zero[0];
-                if (base + lane < u.stop) {
-                    block = A.picks ? A.picks[((size_t)u.token * A.c.kv_heads + head) * A.top + base + lane] : base + lane;
-                    if (block >= 0 && block < nb) page = page_of(A.c, u.sequence, block);
-                    if (page >= 0) {
-                        const float *f = page_scales(A.c, page, head);
-                        sc = make_float2(f[0], f[1]);
-                    }
-                }
-                unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-                while (there && ok) {
-                    const int l = __ffs(there) - 1;
-                    there &= there - 1;
-                    const int pg = __shfl_sync(0xffffffffu, page, l), bl = __shfl_sync(0xffffffffu, block, l);
-                    const float2 s2 = make_float2(__shfl_sync(0xffffffffu, sc.x, l), __shfl_sync(0xffffffffu, sc.y, l));
-                    if (n == 0) page2[0] = pg, block2[0] = bl, scale2[0] = s2;
-                    else page2[1] = pg, block2[1] = bl, scale2[1] = s2;
-                    if (++n == 2) step();
-                }
-            }
-            if (ok && n) step();
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (ok && behind[i] >= 0) ok = values(behind[i], head);
-            if (ok) ok = keys(0, none, none, zero, head);  // the end of the unit
-        }
-        if (ok) ok = keys(-1, none, none, zero, 0);
-        if (!ok && lane == 0) {  // let what is in flight land: the last copy of each slot, within the limit
-            auto out = [&](unsigned long long *b, unsigned parity) {
-                for (const long long began = clock64(); clock64() - began < kWaitClocks && !bar_try(b, parity);) {
-                }
-            };
-            for (unsigned i = 1; i <= Z::k_ring && i <= kc; ++i) out(&M.k_full[(kc - i) % Z::k_ring], (kc - i) / Z::k_ring & 1);
-            for (unsigned i = 1; i <= Z::v_ring && i <= vc; ++i) out(&M.v_full[(vc - i) % Z::v_ring], (vc - i) / Z::v_ring & 1);
-        }
-    } else if (warp == kIssueWarp) {
-        // ---------------------------------------------------------------- products
-        const unsigned id_s = idesc_i8(Z::ns, true), id_o = idesc_i8(Z::nw, false);
-        unsigned kc = 0, vc = 0, sc = 0, un = 0;
-        int behind = 0;  // pages of the step whose O is still to be issued
-        bool ok = true, begun = false;
-        auto sums = [&]() {  // O of step sc - 1
-            const unsigned s = sc - 1, buf = s & 1;
-            if (!wait_all(&M.w_full[buf], s >> 1 & 1)) return false;
-            for (int i = 0; i < behind; ++i)
-                if (!wait_all(&M.v_full[(vc + i) % Z::v_ring], (vc + i) / Z::v_ring & 1)) return false;
-            tc_fence_after();
-            const int fresh = M.fresh[buf];
-            if (elect_one()) {
-                for (int i = 0; i < behind; ++i) {
-                    const unsigned long long v = sw64_desc(su32(M.v[(vc + i) % Z::v_ring])), w = sw64_desc(su32(M.w[buf][i]));
+                    if (i >= pages) continue;
+                    const unsigned long long v = sw64_desc(su32(M.v[s][i])), w = sw64_desc(su32(M.w[group][i]));
 #pragma unroll
                     for (int b = 0; b < Z::blocks; ++b)
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
-                            mma_i8(tmem_o + 64 * b, v + b * (8192 >> 4) + 2 * k, w + 2 * k, id_o, !fresh || i > 0 || k > 0);
-                    mma_commit(&M.v_empty[(vc + i) % Z::v_ring]);
+                            mma_i8(tmem_o + 128 * group + 64 * b, v + b * (8192 >> 4) + 2 * k, w + 2 * k, id_o, !(what & 4) || i > 0 || k > 0);
                 }
-                mma_commit(&M.o_done[buf]);
+                mma_commit(&M.v_empty[s]);
+                mma_commit(&M.o_done[group]);
             }
-            __syncwarp();
-            vc += behind;
-            behind = 0;
-            return true;
-        };
-        for (;;) {
-            const unsigned ks = kc % Z::k_ring;
-            if (!(ok = wait_all(&M.k_full[ks], kc / Z::k_ring & 1))) break;
-            const int pages = M.step[ks].pages;
-            __syncwarp();
-            if (pages > 0) {
-                const unsigned qb = un & 1, buf = sc & 1;
-                if (!begun) {
-                    begun = true;
-                    if (!(ok = wait_all(&M.q_full[qb], un >> 1 & 1))) break;
-                }
-                if (!(ok = sc < 2 || wait_all(&M.s_free[buf], (sc - 2) >> 1 & 1))) break;
-                tc_fence_after();
-                const unsigned long long k = sw64_desc(su32(M.k[ks][0])), q = sw64_desc(su32(M.q[qb][0]));
-                if (elect_one()) {
-#pragma unroll
-                    for (int b = 0; b < Z::panels; ++b)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            mma_i8(tmem + 64 * buf, k + b * (8192 >> 4) + 2 * h, q + b * (Z::ns * 64 >> 4) + 2 * h, id_s, b > 0 || h > 0);
-                    mma_commit(&M.k_empty[ks]);
-                    mma_commit(&M.s_full[buf]);
-                }
-                __syncwarp();
-                if (behind && !(ok = sums())) break;
-                behind = pages;
-                ++sc;
-            } else {
-                if (pages == 0 && !begun && !(ok = wait_all(&M.q_full[un & 1], un >> 1 & 1))) break;  // a unit without pages
-                if (behind && !(ok = sums())) break;
-                if (elect_one()) {
-                    bar_arrive(&M.k_empty[ks]);
-                    mma_commit(&M.q_empty[un & 1]);  // the unit's queries have been used
-                }
-                __syncwarp();
-                begun = false;
-                ++un;
-                if (pages < 0) break;
-            }
-            ++kc;
+            mma_commit(&M.drained[1]);
+            wait_out(&M.drained[1], 0);
         }
-        if (elect_one()) mma_commit(&M.drained);
         __syncwarp();
-        for (const long long began = clock64(); !bar_try(&M.drained, 0) && clock64() - began < kWaitClocks;) {
+    } else if (warp == kIssueWarp) {
+        // ---------------------------------------------------------------- S
+        if (lane == 0) {
+            const unsigned id_s = idesc_i8(Z::ns, true);
+            unsigned sc = 0;
+            int unit = -1;  // whose queries are in use
+            for (unsigned kc = 0;; ++kc) {
+                const unsigned st = kc % kSteps, ks = sc % Z::k_ring, buf = sc & 3;
+                if (!wait(&M.step_full[st], kc / kSteps & 1)) break;
+                const int pages = M.step[st].pages, next_unit = M.step[st].unit;
+                bar_arrive(&M.step_empty[st]);
+                if (pages < 0) break;
+                if (unit != next_unit && !wait(&M.q_full[next_unit & 1], next_unit >> 1 & 1)) break;
+                unit = next_unit;
+                if (pages == 0) {
+                    mma_commit(&M.q_empty[unit & 1]);  // the unit's queries have been used
+                    continue;
+                }
+                if (sc >= 4 && !wait(&M.s_free[buf], (sc - 4) >> 2 & 1)) break;
+                if (!wait(&M.k_full[ks], sc / Z::k_ring & 1)) break;
+                tc_fence_after();
+                const unsigned long long k = sw64_desc(su32(M.k[ks][0])), q = sw64_desc(su32(M.q[unit & 1][0]));
+#pragma unroll
+                for (int b = 0; b < Z::panels; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        mma_i8(tmem + 64 * buf, k + b * (8192 >> 4) + 2 * h, q + b * (Z::ns * 64 >> 4) + 2 * h, id_s, b > 0 || h > 0);
+                mma_commit(&M.k_empty[ks]);
+                mma_commit(&M.s_full[buf]);
+                ++sc;
+            }
+            mma_commit(&M.drained[0]);
+            wait_out(&M.drained[0], 0);
         }
+        __syncwarp();
     } else {
         // ---------------------------------------------------------------- query digits, a unit ahead
-        // a row is P / 8 lanes of 8 channels; rows dealt over the two warps
+        // a row is P / 8 lanes of 8 channels
         constexpr int kLanes = P / 8, kAtOnce = 32 / kLanes;
         const int l = lane % kLanes;
         Unit u;
@@ -626,38 +688,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
             if (!wait_all(&M.q_empty[b], (n >> 1 & 1) ^ 1)) break;
             if (!more) u.token = -1;
             const int head = u.sub / A.tiles, row0 = u.sub % A.tiles * kRows, rows = min(kRows, A.group - row0);
-            for (int i = (warp - kQueryWarp) * kAtOnce; more && i < R; i += 2 * kAtOnce) {
-                const int r = i + lane / kLanes;
-                const bool there = r < rows;
-                const float *src = A.q + (long long)u.token * A.stride + (size_t)(head * A.group + row0 + r) * A.c.dim + 8 * l;
-                float x[8], big = 0.0f;
-                if (there && 8 * l + 8 <= A.c.dim && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                    const float4 a = reinterpret_cast<const float4 *>(src)[0], c = reinterpret_cast<const float4 *>(src)[1];
-                    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
-                } else {
+            constexpr int kBatch = 4;  // row groups whose loads are in flight together
+            for (int i0 = 0; more && i0 < R; i0 += kBatch * kAtOnce) {
+                float x[kBatch][8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = there && 8 * l + k < A.c.dim ? src[k] : 0.0f;
-                }
-                bool bad = false;
+                for (int j = 0; j < kBatch; ++j) {
+                    const int r = i0 + j * kAtOnce + lane / kLanes;
+                    const bool there = r < rows;
+                    const float *src = A.q + (long long)u.token * A.stride + (size_t)(head * A.group + row0 + r) * A.c.dim + 8 * l;
+                    if (there && 8 * l + 8 <= A.c.dim && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                        const float4 a = reinterpret_cast<const float4 *>(src)[0], c = reinterpret_cast<const float4 *>(src)[1];
+                        x[j][0] = a.x, x[j][1] = a.y, x[j][2] = a.z, x[j][3] = a.w, x[j][4] = c.x, x[j][5] = c.y, x[j][6] = c.z, x[j][7] = c.w;
+                    } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    bad |= !isfinite(x[k]);
-                    big = fmaxf(big, fabsf(x[k]));
+                        for (int k = 0; k < 8; ++k) x[j][k] = there && 8 * l + k < A.c.dim ? src[k] : 0.0f;
+                    }
                 }
 #pragma unroll
-                for (int s = kLanes / 2; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
-                const unsigned all_bad = __ballot_sync(0xffffffffu, bad);
-                const bool spoilt = (all_bad >> (lane / kLanes * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << (kLanes & 31)) - 1)) != 0;
-                // a power of two that brings the row's largest value to 2^21 .. 2^22: three signed digits
-                const unsigned field = min(275u - (__float_as_uint(big) >> 23), 253u);
-                const float up = __uint_as_float(field << 23);
-                if (r < R) {
+                for (int j = 0; j < kBatch; ++j) {
+                    const int r = i0 + j * kAtOnce + lane / kLanes;
+                    float big = 0.0f;
+                    bool bad = false;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        bad |= !isfinite(x[j][k]);
+                        big = fmaxf(big, fabsf(x[j][k]));
+                    }
+#pragma unroll
+                    for (int s = kLanes / 2; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+                    const unsigned all_bad = __ballot_sync(0xffffffffu, bad);
+                    const bool spoilt = (all_bad >> (lane / kLanes * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << (kLanes & 31)) - 1)) != 0;
+                    // a power of two that brings the row's largest value to 2^21 .. 2^22: three signed digits
+                    const unsigned field = min(275u - (__float_as_uint(big) >> 23), 253u);
+                    const float up = __uint_as_float(field << 23);
+                    if (r >= R) continue;
                     // a row with a value that is not finite has no result
                     if (l == 0) M.row_scale[b][r] = spoilt ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - field) << 23) * A.scale;
                     uint2 d[3] = {};
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        int v = __float2int_rn(x[k] * up);
+                        int v = __float2int_rn(x[j][k] * up);
 #pragma unroll
                         for (int e = 0; e < 3; ++e) {
                             const int digit = e < 2 ? ((v + 128) & 255) - 128 : v;
@@ -668,8 +738,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 3; ++e) *reinterpret_cast<uint2 *>(M.q[b][l >> 3] + sw64_byte(3 * r + e, 8 * (l & 7))) = d[e];
                 }
+                __syncwarp();
             }
-            if (warp == kQueryWarp && lane == 0) M.unit[b] = u;
+            if (lane == 0) M.unit[b] = u;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             bar_arrive(&M.q_full[b]);
             if (!more) break;
@@ -680,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
     if (tid == 0 && M.abort_flag) raise_error(A.c.err, kErrWaitTimeout);
     if (warp == kIssueWarp) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 
@@ -787,12 +858,13 @@ cudaError_t launch(const Args &args, cudaStream_t s) {
     if (slots > kMaxCtas) slots = kMaxCtas;
     const auto encode = encoder();
     if (!encode) return cudaErrorNotSupported;
-    const unsigned long long rows = 2ull * A.c.kv_heads * P;
-    const cuuint64_t dims[3] = {64, rows, (cuuint64_t)A.c.pages}, strides[2] = {64, rows * 64};
-    const cuuint32_t box[3] = {64, 64, 1}, steps[3] = {1, 1, 1};
-    if (encode(&A.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, A.c.codes, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return cudaErrorInvalidValue;
+    const cuuint64_t dims[3] = {64, 2ull * A.c.kv_heads * P, (cuuint64_t)A.c.pages}, strides[2] = {64, dims[1] * 64};
+    const cuuint32_t key_box[3] = {64, 64, 1}, value_box[3] = {64, P, 1}, steps[3] = {1, 1, 1};
+    for (int i = 0; i < 2; ++i)
+        if (encode(i ? &A.values : &A.keys, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, A.c.codes, dims, strides, i ? value_box : key_box, steps,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
     const long long tokens = (long long)A.runs.segments * A.runs.count, units = tokens * A.c.kv_heads * A.tiles;
     A.split = tokens <= kMaxTokens && units < 8LL * slots && units <= 65536;
     const long long most = A.split ? units * (A.picks ? A.top : A.c.blocks) : units;
