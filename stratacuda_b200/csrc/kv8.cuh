@@ -7,6 +7,31 @@
 
 namespace strata {
 
+// Programmatic dependent launch, by all of these kernels: a kernel may be placed while the one before it still runs, and
+// its first act is to wait until that has finished and its writes are visible; then it lets the next one be placed. Only
+// launch latency overlaps: about 2 us a kernel of a token step.
+__device__ __forceinline__ void kv8_enter() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... KT, typename... AT>
+inline cudaError_t kv8_launch(void (*k)(KT...), dim3 grid, dim3 block, size_t smem, unsigned cluster, cudaStream_t s, AT &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, static_cast<AT &&>(args)...);
+}
+
 // A run's sequence and first position, or sequence -1 for an idle slot (a sequence outside the
 // cache is reported and treated as idle).
 struct RunAt {

@@ -21,6 +21,7 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
     __shared__ float red[kThreads / 32];
     __shared__ int lo_s[4][P / 4], hi_s[4][P / 4];
     const int tid = threadIdx.x, head = blockIdx.y >> 1, kind = blockIdx.y & 1;
+    kv8_enter();
     const RunAt a = run_at(c, runs, blockIdx.z);
     if (a.sequence < 0) return;
     if (a.start < 0) {
@@ -203,13 +204,11 @@ cudaError_t kv8_append(const Kv8 &c, const float *k, const float *v, long long s
     const uintptr_t starts = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(c.open);
     const bool wide = starts % 16 == 0 && stride % 4 == 0 && c.dim % 4 == 0;
     auto launch = [&](auto narrow_kernel, auto wide_kernel) {
-        if (wide) wide_kernel<<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
-        else narrow_kernel<<<grid, kThreads, 0, s>>>(c, k, v, stride, r);
+        return kv8_launch(wide ? wide_kernel : narrow_kernel, grid, dim3(kThreads), 0, 1, s, c, k, v, stride, r);
     };
-    if (c.padded == 64) launch(k_kv8_append<64, false>, k_kv8_append<64, true>);
-    else if (c.padded == 128) launch(k_kv8_append<128, false>, k_kv8_append<128, true>);
-    else launch(k_kv8_append<256, false>, k_kv8_append<256, true>);
-    return cudaGetLastError();
+    if (c.padded == 64) return launch(k_kv8_append<64, false>, k_kv8_append<64, true>);
+    if (c.padded == 128) return launch(k_kv8_append<128, false>, k_kv8_append<128, true>);
+    return launch(k_kv8_append<256, false>, k_kv8_append<256, true>);
 }
 
 }  // namespace strata

@@ -227,7 +227,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
     Smem<P, R> &M = *reinterpret_cast<Smem<P, R> *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tokens = A.runs.segments * A.runs.count, per_token = A.c.kv_heads * A.tiles;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int i = 0; i < Z::k_ring; ++i) bar_init(&M.k_full[i], 1), bar_init(&M.k_empty[i], 1);
         // read by the softmax warps and the one that issues S
@@ -243,6 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         M.abort_flag = 0;
     }
+    kv8_enter();
     // this CTA's pages [work, work_end) of the list of all units' pages, or units blockIdx.x, + gridDim.x, ...
     Walk walk{};
     walk.unit = blockIdx.x;
@@ -557,7 +557,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
             batch.head = u.sub / A.tiles;
             batch.page = -1;
             if (base + lane < u.stop) {
-                batch.block = A.picks ? A.picks[((size_t)u.token * A.c.kv_heads + batch.head) * A.top + base + lane] : base + lane;
+                // the list is walked from its second entry on: the first is mostly the session's first block, which selection
+                // picks for its place, and a reference taken from it would soon have to move
+                const int e = base + lane + 1 < u.n ? base + lane + 1 : 0;
+                batch.block = A.picks ? A.picks[((size_t)u.token * A.c.kv_heads + batch.head) * A.top + e] : e;
                 if (batch.block >= 0 && batch.block < (u.seen + kKvBlock - 1) / kKvBlock) batch.page = page_of(A.c, u.sequence, batch.block);
                 if (batch.page >= 0) {
                     const float *f = page_scales(A.c, batch.page, batch.head);
@@ -755,22 +758,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
     }
 }
 
-// Joins the partial results of a unit's row: out = sum_i 2^(m_i - max) acc_i / sum_i 2^(m_i - max) l_i.
-template <int P>
+// Joins the partial results of a unit's rows: out = sum_i 2^(m_i - max) acc_i / sum_i 2^(m_i - max) l_i. DEEP parts
+// are read at a time by as many groups of threads, and the other threads of the block take further rows.
+template <int P, int DEEP>
 __global__ void __launch_bounds__(kJoinThreads) k_kv8_join(const __grid_constant__ Args A) {
-    constexpr int kAcross = P / 4, kDeep = kJoinThreads / kAcross;  // threads a row, parts at a time
-    __shared__ float weight_s[kMaxCtas], red[kJoinThreads / 32];
+    constexpr int kAcross = P / 4, kRowsHere = kJoinThreads / kAcross / DEEP;
     __shared__ float4 acc_s[kJoinThreads];
-    __shared__ float sum_s[kDeep];
-    const int tid = threadIdx.x, per_token = A.c.kv_heads * A.tiles, unit = blockIdx.x, row = blockIdx.y;
+    __shared__ float sum_s[kJoinThreads];
+    const int tid = threadIdx.x, per_token = A.c.kv_heads * A.tiles, unit = blockIdx.x;
+    const int at = tid % kAcross, deep = tid / kAcross % DEEP, row = blockIdx.y * kRowsHere + tid / kAcross / DEEP;
     const int token = unit / per_token, sub = unit % per_token, head = sub / A.tiles, row0 = sub % A.tiles * kRows;
-    if (row >= min(kRows, A.group - row0)) return;
+    const bool there = row < min(kRows, A.group - row0);
     int sequence, seen;
+    kv8_enter();
     const int n = entries(A, token, &sequence, &seen);
     float *dst = A.y + ((size_t)token * A.heads + head * A.group + row0 + row) * A.c.dim;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (n == 0) {  // nothing in sight: no CTA had this unit
-        for (int i = tid; i < A.c.dim; i += kJoinThreads) dst[i] = 0.0f;
+        for (int i = at; there && deep == 0 && i < A.c.dim; i += kAcross) dst[i] = 0.0f;
         return;
     }
     const Parts W = parts_of(A.c.workspace, P);
@@ -779,38 +783,34 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv8_join(const __grid_constant
     if (count <= 1) return;
     // the unit begins in its first CTA's second slot and goes on in the first slots of the others
     auto slot = [&](int i) { return (size_t)2 * (cover.x + i) + (i == 0); };
-    float m = -INFINITY;
-    for (int i = tid; i < count; i += kJoinThreads) {
-        weight_s[i] = W.ml[slot(i) * kRows + row].x;
-        m = fmaxf(m, weight_s[i]);
-    }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-    if (tid % 32 == 0) red[tid / 32] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, red[i]);
-    if (m == -INFINITY) m = 0.0f;
-    const int at = tid % kAcross, deep = tid / kAcross;
-    float4 acc = make_float4(0, 0, 0, 0);
-    float sum = 0.0f;
+    float m = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (there) {
 #pragma unroll 8
-    for (int i = deep; i < count; i += kDeep) {
-        const float w = exp2_fast(weight_s[i] - m);
-        const float4 f = *reinterpret_cast<const float4 *>(W.acc + (slot(i) * kRows + row) * P + at * 4);
-        sum += w * W.ml[slot(i) * kRows + row].y;
-        acc.x += w * f.x, acc.y += w * f.y, acc.z += w * f.z, acc.w += w * f.w;
+        for (int i = 0; i < count; ++i) m = fmaxf(m, W.ml[slot(i) * kRows + row].x);
+        if (m == -INFINITY) m = 0.0f;
+#pragma unroll 8
+        for (int i = deep; i < count; i += DEEP) {
+            const float2 ml = W.ml[slot(i) * kRows + row];
+            const float4 f = *reinterpret_cast<const float4 *>(W.acc + (slot(i) * kRows + row) * P + at * 4);
+            const float w = exp2_fast(ml.x - m);
+            sum += w * ml.y;
+            acc.x += w * f.x, acc.y += w * f.y, acc.z += w * f.z, acc.w += w * f.w;
+        }
     }
-    acc_s[tid] = acc;
-    if (at == 0) sum_s[deep] = sum;
-    __syncthreads();
-    if (deep) return;
+    if (DEEP > 1) {
+        acc_s[tid] = acc;
+        sum_s[tid] = sum;
+        __syncthreads();
+        if (deep) return;
 #pragma unroll
-    for (int i = 1; i < kDeep; ++i) {
-        const float4 f = acc_s[i * kAcross + at];
-        acc.x += f.x, acc.y += f.y, acc.z += f.z, acc.w += f.w;
-        sum += sum_s[i];
+        for (int i = 1; i < DEEP; ++i) {
+            const float4 f = acc_s[tid + i * kAcross];
+            acc.x += f.x, acc.y += f.y, acc.z += f.z, acc.w += f.w;
+            sum += sum_s[tid + i * kAcross];
+        }
     }
+    if (!there) return;
     const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum), v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -868,19 +868,14 @@ cudaError_t launch(const Args &args, cudaStream_t s) {
     const long long tokens = (long long)A.runs.segments * A.runs.count, units = tokens * A.c.kv_heads * A.tiles;
     A.split = tokens <= kMaxTokens && units < 8LL * slots && units <= 65536;
     const long long most = A.split ? units * (A.picks ? A.top : A.c.blocks) : units;
-    k_kv8_rows<P, R><<<(unsigned)(most < slots ? most : slots), kThreads, kSmem, s>>>(A);
-    e = cudaGetLastError();
+    e = kv8_launch(k_kv8_rows<P, R>, dim3((unsigned)(most < slots ? most : slots)), dim3(kThreads), kSmem, 1, s, A);
     if (e != cudaSuccess || !A.split) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)units, A.group < kRows ? A.group : kRows);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_kv8_join<P>, static_cast<const Args &>(A));
+    // few units have many parts each, which a block's threads share; many units have few
+    constexpr int kSpread = kJoinThreads / (P / 4);
+    const int rows = A.group < kRows ? A.group : kRows;
+    const bool deep = units * rows < 2LL * slots;
+    return kv8_launch(deep ? k_kv8_join<P, kSpread> : k_kv8_join<P, 1>, dim3((unsigned)units, deep ? rows : (rows + kSpread - 1) / kSpread),
+                      dim3(kJoinThreads), 0, 1, s, static_cast<const Args &>(A));
 }
 template <int P>
 cudaError_t launch_rows(const Args &A, cudaStream_t s) {  // room for as many rows as the group has, to the next four

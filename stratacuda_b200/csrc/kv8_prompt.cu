@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pairs = A.runs.segments * A.tiles;
     const PromptParts W = prompt_parts(A.c.workspace, P);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    kv8_enter();
 
     // ---- this CTA's work: units (pair, head) blockIdx.x, + gridDim.x, ... or pages [work, work_end) of all units' list
     if (A.split) {
@@ -625,8 +625,8 @@ __global__ void __launch_bounds__(256) k_kv8_prompt_join(const __grid_constant__
     const int tid = threadIdx.x, unit = blockIdx.x, pair = unit / A.c.kv_heads, head = unit % A.c.kv_heads;
     const int run = pair / A.tiles, tile = pair % A.tiles, i = blockIdx.y * 32 + tid % 32, r = tile * kTileRows + i;
     const bool there = i < kTileRows && r < A.runs.count * A.group;
+    kv8_enter();
     const int n = pair_pages(A, run, tile);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     float *dst = there ? prompt_row(A, run, head, r) : nullptr;
     if (n == 0) {
         for (int ch = tid / 32; there && ch < A.c.dim; ch += 8) dst[ch] = 0.0f;
@@ -676,19 +676,9 @@ cudaError_t launch(PromptArgs A, cudaStream_t s) {
     // Units shared page by page where whole ones would leave the last round of CTAs uneven
     A.split = pairs <= kMaxPairs && units <= kMaxUnits && units < 8LL * most;
     const long long work = A.split ? units * A.c.blocks : units;
-    k_kv8_prompt<P><<<(unsigned)(work < most ? work : most), kPromptThreads, kSmem, s>>>(A);
-    e = cudaGetLastError();
+    e = kv8_launch(k_kv8_prompt<P>, dim3((unsigned)(work < most ? work : most)), dim3(kPromptThreads), kSmem, 1, s, A);
     if (e != cudaSuccess || !A.split) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)units, kTileRows / 32);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_kv8_prompt_join<P>, A);
+    return kv8_launch(k_kv8_prompt_join<P>, dim3((unsigned)units, kTileRows / 32), dim3(256), 0, 1, s, A);
 }
 
 }  // namespace

@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(Shape<WIDE>::threads, WIDE ? 2 : 1) k_kv8_sele
     __shared__ float red[kWarps];
     __shared__ int count_s[2][kWarps], equal_s[kWarps], have_s[kRows];
     __shared__ unsigned short block_s[WIDE ? 1 : kWarps][kCandidates];
+    kv8_enter();
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -370,18 +371,7 @@ cudaError_t launch(const Args &A, int ranks, size_t smem, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const long long ctas = (long long)A.runs.segments * A.tiles * A.c.kv_heads * ranks;
     if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(Shape<WIDE>::threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ranks;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_kv8_select<P, WIDE>, A);
+    return kv8_launch(k_kv8_select<P, WIDE>, dim3((unsigned)ctas), dim3(Shape<WIDE>::threads), smem, ranks, s, A);
 }
 
 }  // namespace
