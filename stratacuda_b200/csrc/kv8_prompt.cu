@@ -619,45 +619,65 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
 }
 
 // Joins the parts of a unit that several CTAs worked on: the begun one in y and the tails in the workspace, all of
-// them sums of 2^(logit - m_i) v / most; 32 rows of a tile a block.
+// them sums of 2^(logit - m_i) v / most; 32 rows of a tile a block. A warp's lanes are 32 rows in the tails, as they lie
+// there, and 32 channels of a row in y; the tails' sum turns in shared memory.
 template <int P>
 __global__ void __launch_bounds__(256) k_kv8_prompt_join(const __grid_constant__ PromptArgs A) {
-    const int tid = threadIdx.x, unit = blockIdx.x, pair = unit / A.c.kv_heads, head = unit % A.c.kv_heads;
-    const int run = pair / A.tiles, tile = pair % A.tiles, i = blockIdx.y * 32 + tid % 32, r = tile * kTileRows + i;
-    const bool there = i < kTileRows && r < A.runs.count * A.group;
+    __shared__ float4 tails[P / 4][33];
+    __shared__ float2 by[32];  // of a row: what its part in y and what the tails' sum is taken by
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, unit = blockIdx.x, pair = unit / A.c.kv_heads, head = unit % A.c.kv_heads;
+    const int run = pair / A.tiles, tile = pair % A.tiles, first = blockIdx.y * 32, i = first + lane;
+    const int rows = min(32, A.runs.count * A.group - tile * kTileRows - first);  // of this block, none or fewer at the end
     kv8_enter();
+    if (rows <= 0) return;
     const int n = pair_pages(A, run, tile);
-    float *dst = there ? prompt_row(A, run, head, r) : nullptr;
     if (n == 0) {
-        for (int ch = tid / 32; there && ch < A.c.dim; ch += 8) dst[ch] = 0.0f;
+        for (int r = warp; r < rows; r += 8) {
+            float *dst = prompt_row(A, run, head, tile * kTileRows + first + r);
+            for (int ch = lane; ch < A.c.dim; ch += 32) dst[ch] = 0.0f;
+        }
         return;
     }
     const PromptParts W = prompt_parts(A.c.workspace, P);
     const int2 cover = W.cover[unit];
-    if (cover.x == cover.y || !there) return;
-    const float4 begun = W.head_ml[cover.x * kTileRows + i];
-    float m = begun.x;
-    for (int c = cover.x + 1; c <= cover.y; ++c) m = fmaxf(m, W.tail_ml[c * kTileRows + i].x);
-    if (m == -INFINITY) m = 0.0f;
-    const float w0 = exp2_fast(begun.x - m);
-    float sum = begun.y * w0;
-    for (int c = cover.x + 1; c <= cover.y; ++c) {
-        const float4 t = W.tail_ml[c * kTileRows + i];
-        sum += t.y * exp2_fast(t.x - m);
-    }
-    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-    for (int k = tid / 32; k < P / 4; k += 8) {
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = 4 * k + e < A.c.dim ? dst[4 * k + e] * w0 : 0.0f;
+    if (cover.x == cover.y) return;
+    float m = -INFINITY;
+    if (lane < rows) {
+        const float4 begun = W.head_ml[cover.x * kTileRows + i];
+        m = begun.x;
+        for (int c = cover.x + 1; c <= cover.y; ++c) m = fmaxf(m, W.tail_ml[c * kTileRows + i].x);
+        if (m == -INFINITY) m = 0.0f;
+        if (warp == 0) {
+            const float w0 = exp2_fast(begun.x - m);
+            float sum = begun.y * w0;
+            for (int c = cover.x + 1; c <= cover.y; ++c) {
+                const float4 t = W.tail_ml[c * kTileRows + i];
+                sum += t.y * exp2_fast(t.x - m);
+            }
+            const float inv = (sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum)) * begun.z;
+            by[lane] = make_float2(w0 * inv, inv);
+        }
+        float4 o[P / 32] = {};
         for (int c = cover.x + 1; c <= cover.y; ++c) {
             const float w = exp2_fast(W.tail_ml[c * kTileRows + i].x - m);
-            const float4 f = W.sum[((size_t)c * (P / 4) + k) * kTileRows + i];
-            o[0] += f.x * w, o[1] += f.y * w, o[2] += f.z * w, o[3] += f.w * w;
+#pragma unroll
+            for (int j = 0; j < P / 32; ++j) {
+                const float4 f = W.sum[((size_t)c * (P / 4) + 8 * j + warp) * kTileRows + i];
+                o[j].x += f.x * w, o[j].y += f.y * w, o[j].z += f.z * w, o[j].w += f.w * w;
+            }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (4 * k + e < A.c.dim) dst[4 * k + e] = o[e] * inv * begun.z;
+        for (int j = 0; j < P / 32; ++j) tails[8 * j + warp][lane] = o[j];
+    }
+    __syncthreads();
+    for (int r = warp; r < rows; r += 8) {
+        float *dst = prompt_row(A, run, head, tile * kTileRows + first + r);
+        const float2 w = by[r];
+#pragma unroll
+        for (int j = 0; j < P / 32; ++j) {
+            const int ch = 32 * j + lane;
+            if (ch < A.c.dim) dst[ch] = dst[ch] * w.x + reinterpret_cast<const float *>(&tails[ch / 4][r])[ch % 4] * w.y;
+        }
     }
 }
 
