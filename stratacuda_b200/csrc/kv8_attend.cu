@@ -21,13 +21,10 @@
 // Few units (`split`): the pages of all units form one list that the CTAs share evenly, whatever the
 // lengths; a unit cut by a CTA border leaves unnormalised partial sums in the workspace and a
 // second kernel joins them in CTA order, so results repeat bit for bit.
+#include "kv8_mma.cuh"
 #include "kv8_rows.cuh"
-#include "pf_gemm.cuh"
-
-#include <cudaTypedefs.h>
 
 #include <atomic>
-#include <mutex>
 
 namespace strata {
 namespace {
@@ -38,7 +35,7 @@ using namespace kv8_rows;
 constexpr int kSoft = 128, kKeyWarp = 8, kIssueWarp = 9, kSumWarp = 11, kThreads = 384;  // kSoft: threads of a softmax group
 constexpr int kSteps = 8;         // steps looked up ahead
 constexpr int kFlushSteps = 128;  // steps that TMEM's 32-bit sums bear (255 * 127 * 128 tokens a step)
-constexpr float kGrow = 8.0f;          // weights stay below this, times
+constexpr float kGrow = 3.0f;          // log2 of what weights stay below, times
 constexpr float kUnit = 268435456.0f;  // 2^28, below 2^32
 constexpr float kRoom = 3.0f;          // log2 of the room that a new reference leaves above the maximum, so that it seldom moves again
 constexpr long long kWaitClocks = 2000000000;  // about a second
@@ -126,26 +123,6 @@ struct Walk {
     }
 };
 
-
-// Shared-memory matrix descriptor: K-major, 64-byte rows and swizzle, 8-row groups 512 bytes apart.
-__device__ __forceinline__ unsigned long long sw64_desc(unsigned smem_addr) {
-    return (unsigned long long)((smem_addr & 0x3FFFFu) >> 4) | (1ull << 16) | (32ull << 32) | (1ull << 46) | (4ull << 61);
-}
-// Byte of a 64-byte row in that layout.
-__device__ __forceinline__ int sw64_byte(int row, int at) { return row * 64 + ((((at >> 4) ^ (row >> 1)) & 3) << 4) + (at & 15); }
-// Instruction descriptor, kind::i8: S32 sums (bits 4-5 = 2), A signed (bits 7-9 = 1), B signed or not (bits 10-12), both
-// K-major, M = 128.
-__device__ __forceinline__ unsigned idesc_i8(int N, bool b_signed) {
-    return (2u << 4) | (1u << 7) | ((unsigned)b_signed << 10) | ((unsigned)(N >> 3) << 17) | (8u << 24);
-}
-__device__ __forceinline__ void mma_i8(unsigned tmem_d, unsigned long long a, unsigned long long b, unsigned idesc, int accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 // 16 consecutive columns of this thread's TMEM lane, without the wait.
 __device__ __forceinline__ void tmem_ld16(unsigned taddr, int *r) {
     asm volatile(
@@ -715,18 +692,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
     }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
-}
-
 // What the current device needs set or asked once.
 template <int P, int R>
 cudaError_t multiprocessors(size_t smem, int *out) {
@@ -753,17 +718,9 @@ cudaError_t launch(const Args &args, cudaStream_t s) {
     cudaError_t e = multiprocessors<P, R>(kSmem, &slots);
     if (e != cudaSuccess) return e;
     if (slots > kMaxCtas) slots = kMaxCtas;
-    if (kv8_short_fits(A, slots)) return kv8_attend_short(A, slots, s);
-    const auto encode = encoder();
-    if (!encode) return cudaErrorNotSupported;
-    const cuuint64_t dims[3] = {64, 2ull * A.c.kv_heads * P, (cuuint64_t)A.c.pages}, strides[2] = {64, dims[1] * 64};
-    const cuuint32_t key_box[3] = {64, 64, 1}, value_box[3] = {64, P, 1}, steps[3] = {1, 1, 1};
-    for (int i = 0; i < 2; ++i)
-        if (encode(i ? &A.values : &A.keys, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, A.c.codes, dims, strides, i ? value_box : key_box, steps,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return cudaErrorInvalidValue;
     const long long tokens = (long long)A.runs.segments * A.runs.count, units = tokens * A.c.kv_heads * A.tiles;
+    if (kv8_short_fits(A, slots)) return kv8_attend_short(A, slots, s);
+    if (!page_map(A.c, 64, &A.keys) || !page_map(A.c, P, &A.values)) return cudaErrorInvalidValue;
     A.split = tokens <= kMaxTokens && units < 8LL * slots && units <= 65536;
     const long long most = A.split ? units * (A.picks ? A.top : A.c.blocks) : units;
     e = kv8_launch(k_kv8_rows<P, R>, dim3((unsigned)(most < slots ? most : slots)), dim3(kThreads), kSmem, 1, s, A);

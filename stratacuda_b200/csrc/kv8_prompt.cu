@@ -3,26 +3,32 @@
 //
 // A tile is 128 consecutive (token, query head) pairs of one run and key/value head, so that groups of any
 // size fill it. Its keys and values pass by page by page (64 tokens):
-//   S[128][64] = Q K^T     Q as two FP16 halves in shared memory, the codes converted to FP16 (exact)
-//   O[128][P] += W V       the weights as two FP16 halves in TMEM, the A operand of the second product
-// Both products run twice, for the high and the low half, which gives F32's accuracy at half of the FP16
-// rate. Accumulators, maxima and sums are F32.
+//   S[128][64] = Q K^T     on integer products (kind::i8): a query row, scaled by a power of two, is 23 bits in three
+//                          signed 8-bit digits in shared memory, and the keys' codes are taken as they lie in memory; a digit's
+//                          sums are whole numbers in TMEM, exact, and join in F32
+//   O[128][P] += W V       the weights as two FP16 halves in TMEM, the A operand, against codes converted to FP16 (exact)
+// which gives F32's accuracy at three integer passes for the first product and two FP16 passes for the second. (The
+// second on integers would want as many sums as weights have digits, more than TMEM holds.) Maxima and sums are F32.
 //
-// Warps (8, so that a thread may hold a whole row's logits in its registers):
-//   0-3  softmax: a thread owns one row (its TMEM lane): logits from S, running maximum and sum, weights
-//        back into the TMEM columns of S. O is rescaled only when a row's maximum has grown by more than
-//        2^5 (weights are kept times 2^10, so that both ends stay inside FP16), so seldom after the
-//        first pages
-//   4-6  converters: 8-bit codes from global memory (the next item's loads in flight) to FP16 in the
-//        128-byte-swizzled layout of the MMA operands; keys and values alternate through one ring of slots
-//   7    one thread issues the MMAs: S of page j + 1 before O of page j, so that the softmax of
-//        a page runs under the products of its neighbours
+// Warps:
+//   0-7  softmax: a row (TMEM lane) is two threads', 32 of a page's tokens each: logits from S, running maximum (the two
+//        exchange theirs) and sum, weights into TMEM. O is rescaled only when a row's maximum has grown by more than
+//        2^5 (weights are kept times 2^10, so that both ends stay inside FP16), so seldom after the first pages
+//   8-9  converters: values to FP16 in the 128-byte-swizzled layout of the MMA operands
+//   10   fetches keys by TMA (64-byte swizzle) and values by bulk copies
+//   11   one thread issues the MMAs: S of page j + 1 before O of page j, so that S's columns are read and free
+//        again while O is computed
 // A value scale cannot be applied after the product, since pages add up in one accumulator: weights are
-// multiplied by scale / (largest scale of the tile's pages).
+// multiplied by scale / (largest scale of the tile's pages), in their exponents.
+//
+// Measured: 2048 tokens over 16384 keys, 24 heads over 2 of 256 channels, 1307 us, 600 TFLOP/s of the two products as they
+// are defined, at a page about every 4100 clocks a CTA. S takes 1250 of them (24 instructions of 128 x 64 x 32, bound by
+// reading their operands from shared memory) and O 1000; the rest are the hand-overs between products and softmax, for
+// which TMEM has no second set of S's columns. The form with queries in FP16 halves and keys converted as well took
+// 1546 us, since its converters and operands take twice the shared-memory traffic.
 //
 // Every wait is bounded; past the limit all roles leave and the error word is set.
-#include "kv8.cuh"
-#include "pf_gemm.cuh"
+#include "kv8_mma.cuh"
 
 #include <atomic>
 #include <cmath>
@@ -32,16 +38,17 @@ namespace {
 
 using namespace pf;
 
-constexpr int kSoftWarps = 4, kConvWarps = 3, kMmaWarp = kSoftWarps + kConvWarps;
+constexpr int kSoftWarps = 8, kConvWarps = 2, kKeyWarp = kSoftWarps + kConvWarps, kMmaWarp = kKeyWarp + 1;
 constexpr int kPromptThreads = 32 * (kMmaWarp + 1);
 constexpr int kConvThreads = 32 * kConvWarps;
 constexpr int kTileRows = 128;
-constexpr int kBufs = 4;             // S / weight buffers in TMEM, 64 columns each
+constexpr int kDigits = 3;           // of a query
 constexpr float kLiftP = 10.0f;      // weights are stored times 2^10
 constexpr float kGrow = 5.0f;        // growth of a maximum (log2) that O's scale bears
 constexpr long long kLimit = 2000000000;  // clocks, about a second
 
 constexpr int kFlush = 16;           // pages that add up in TMEM before the sum moves to 32-bit adds
+constexpr int kScales = 8;           // pages whose scales are kept: more than are fetched ahead of the softmax
 constexpr int kMaxGrid = 160;        // CTAs, each with a slot in the workspace
 constexpr int kMaxPairs = 1024;      // (run, tile) pairs of a split call
 constexpr int kMaxUnits = 65536;
@@ -53,11 +60,15 @@ struct Piece {
 };
 
 template <int P>
-struct __align__(1024) PromptSmem {
-    static constexpr int slots = P == 256 ? 3 : 6;
-    unsigned char q[2][P / 64][kTileRows * 128];  // high and low halves: panels of 64 channels, rows of 128 bytes, swizzled
-    unsigned char slot[slots][P * 128];           // keys [P / 64][64 tokens][128 bytes] or values [P channels][128 bytes], swizzled
+struct PromptSmem {  // 1024-byte aligned
+    static constexpr int k_ring = P == 256 ? 2 : 3, v_ring = k_ring;
+    unsigned char q[kDigits][P / 64][kTileRows * 64];  // panels of 64 channels, a row 64 bytes, swizzled
+    unsigned char k[k_ring][P * 64];                   // keys [P / 64][64 tokens][64 bytes], swizzled
+    unsigned char v[v_ring][P * 128];                  // values as FP16 [P channels][128 bytes], swizzled
+    unsigned char raw[v_ring][P * 64];                 // values as they lie in memory
     float row_scale[kTileRows];
+    float2 page_scale[kScales];       // of keys (-1: no page) and values, by page
+    float half_row[2][2][kTileRows];  // by page's parity and half: what a row's two threads exchange
     float red[kPromptThreads / 32];
     struct Walk {
         long long unit, work, work_end, chunk;
@@ -65,7 +76,8 @@ struct __align__(1024) PromptSmem {
         Piece tail;
     } walk;  // thread 0's
     Piece piece;
-    unsigned long long full[slots], empty[slots], s_full[kBufs], w_full[kBufs], o_done[kBufs], o_free, drained;
+    unsigned long long k_full[k_ring], k_empty[k_ring], raw_full[v_ring], raw_empty[v_ring], v_full[v_ring], v_empty[v_ring];
+    unsigned long long s_full, s_free, w_full, o_done, o_free, drained;
     unsigned tmem;
     int abort_flag;
 };
@@ -79,6 +91,7 @@ struct PromptArgs {
     float scale;  // times log2 e
     float *y;
     int split;
+    CUtensorMap keys;  // boxes of P rows
 };
 // Workspace: a CTA's sum of more than kFlush pages, or of the part of a unit that an earlier CTA began,
 // as [P / 4][128 rows] float4; per row maximum, sum and value scale of such a part and of a begun one (whose sum is
@@ -131,6 +144,21 @@ __device__ __forceinline__ void tmem_ld16_async(unsigned taddr, unsigned (&r)[16
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
+// OR of x over a named barrier's two warps.
+__device__ __forceinline__ bool pair_or(int barrier, bool x) {
+    unsigned r;
+    asm volatile(
+        "{\n\t.reg .pred pi, po;\n\t"
+        "setp.ne.u32 pi, %1, 0;\n\t"
+        "bar.red.or.pred po, %2, 64, pi;\n\t"
+        "selp.u32 %0, 1, 0, po;\n\t}"
+        : "=r"(r)
+        : "r"((unsigned)x), "r"(barrier)
+        : "memory");
+    return r != 0;
+}
+// A whole number of |x| < 2^22 in two additions: 1.5 * 2^23 + x is the float whose bits are 0x4b400000 + x.
+__device__ __forceinline__ float whole_float(unsigned x) { return __uint_as_float(0x4b400000u + x) - 12582912.0f; }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -146,9 +174,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
 
     // ---- this CTA's work: units (pair, head) blockIdx.x, + gridDim.x, ... or pages [work, work_end) of all units' list
     if (A.split) {
-        long long *before = reinterpret_cast<long long *>(M.slot[0]);  // used before the ring is
+        long long *before = reinterpret_cast<long long *>(M.v[0]);  // used before the ring is
         long long *part = before + kMaxPairs + 1;
-        static_assert(sizeof(M.slot) >= (kMaxPairs + 1 + kPromptThreads / 32) * 8, "the page counts fit");
+        static_assert(sizeof(M.v) >= (kMaxPairs + 1 + kPromptThreads / 32) * 8, "the page counts fit");
         for (int base = 0; base < pairs; base += kPromptThreads) {  // before[i]: a head's pages before pair i
             long long sum = base + tid < pairs ? pair_pages(A, (base + tid) / A.tiles, (base + tid) % A.tiles) : 0;
 #pragma unroll
@@ -183,15 +211,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
         }
     }
     if (tid == 0) {
-        for (int i = 0; i < Sm::slots; ++i) {
-            bar_init(&M.full[i], kConvThreads);
-            bar_init(&M.empty[i], 1);
-        }
-        for (int i = 0; i < kBufs; ++i) {
-            bar_init(&M.s_full[i], 1);
-            bar_init(&M.w_full[i], 32 * kSoftWarps);
-            bar_init(&M.o_done[i], 1);
-        }
+        for (int i = 0; i < Sm::k_ring; ++i) bar_init(&M.k_full[i], 1), bar_init(&M.k_empty[i], 1);
+        for (int i = 0; i < Sm::v_ring; ++i) bar_init(&M.v_full[i], kConvThreads), bar_init(&M.v_empty[i], 1);
+        for (int i = 0; i < Sm::v_ring; ++i) bar_init(&M.raw_full[i], 1), bar_init(&M.raw_empty[i], kConvWarps);
+        bar_init(&M.s_full, 1), bar_init(&M.s_free, 32 * kSoftWarps);
+        bar_init(&M.w_full, 32 * kSoftWarps), bar_init(&M.o_done, 1);
         bar_init(&M.o_free, 32 * kSoftWarps);
         bar_init(&M.drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -265,8 +289,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
         w.has_tail = 0;
     };
 
-    // counters that go on from piece to piece: pages (S buffers), ring items, flushes
-    int pages = 0, used = 0, flushes = 0;
+    // counters that go on from piece to piece
+    int pages = 0, flushes = 0;
     for (;;) {
         if (tid == 0) next();
         __syncthreads();
@@ -287,7 +311,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
             if (j < n) raise_error(A.c.err, kErrIndex);
             return -1;
         };
-        // queries: a row is P / 8 lanes of 8 channels; scaled by a power of two to 2^9 .. 2^10 at most
+        auto scales_of = [&](int page) {
+            const float *s = page >= 0 ? page_scales(A.c, page, head) : nullptr;
+            return s ? make_float2(s[0], s[1]) : make_float2(-1.0f, 0.0f);
+        };
+        const int first_page = tid < p.n ? page_of(A.c, at.sequence, tid) : -1;
+        const float first_most = first_page >= 0 ? page_scales(A.c, first_page, head)[1] : 0.0f;
+        // queries: a row is P / 8 lanes of 8 channels; scaled by a power of two to 2^21 .. 2^22 at most
         {
             constexpr int kLanes = P / 8, kAtOnce = 32 / kLanes;
             const int l = lane % kLanes, ch0 = 8 * l;
@@ -302,27 +332,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = i < rows && ch0 + k < A.c.dim ? src[k] : 0.0f;
                 }
+                bool bad = false;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(x[k]));
+                for (int k = 0; k < 8; ++k) {
+                    bad |= !isfinite(x[k]);
+                    big = fmaxf(big, fabsf(x[k]));
+                }
 #pragma unroll
-                for (int s = kLanes / 2; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
-                const unsigned field = min(263u - (__float_as_uint(big) >> 23), 253u);
-                const float up = __uint_as_float(field << 23);
-                if (l == 0) M.row_scale[i] = __uint_as_float((254u - field) << 23) * A.scale;
-                uint4 hi, lo;
-                split_pair(x[0] * up, x[1] * up, hi.x, lo.x);
-                split_pair(x[2] * up, x[3] * up, hi.y, lo.y);
-                split_pair(x[4] * up, x[5] * up, hi.z, lo.z);
-                split_pair(x[6] * up, x[7] * up, hi.w, lo.w);
-                const int where = i * 128 + (((l & 7) ^ (i & 7)) << 4);
-                *reinterpret_cast<uint4 *>(M.q[0][l >> 3] + where) = hi;
-                *reinterpret_cast<uint4 *>(M.q[1][l >> 3] + where) = lo;
+                for (int s = kLanes / 2; s > 0; s >>= 1) {
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+                    bad |= __shfl_xor_sync(0xffffffffu, (int)bad, s) != 0;
+                }
+                const unsigned field = min(275u - (__float_as_uint(big) >> 23), 253u);
+                const float up = copysignf(__uint_as_float(field << 23), A.scale);
+                // a row with a value that is not finite has no result
+                if (l == 0) M.row_scale[i] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - field) << 23) * fabsf(A.scale);
+                uint2 d[kDigits] = {};
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    int v = __float2int_rn(x[k] * up);
+#pragma unroll
+                    for (int e = 0; e < kDigits; ++e) {
+                        const int digit = e < kDigits - 1 ? ((v + 128) & 255) - 128 : v;
+                        v = (v - digit) >> 8;
+                        (k < 4 ? d[e].x : d[e].y) |= (unsigned)(digit & 255) << (8 * (k & 3));
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < kDigits; ++e) *reinterpret_cast<uint2 *>(M.q[e][l >> 3] + sw64_byte(i, 8 * (l & 7))) = d[e];
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         // the largest value scale of the unit's pages
-        float most = 0.0f;
-        for (int j = tid; j < p.n; j += kPromptThreads) {
+        float most = first_most;
+        for (int j = tid + kPromptThreads; j < p.n; j += kPromptThreads) {
             const int page = page_of(A.c, at.sequence, j);
             if (page >= 0) most = fmaxf(most, page_scales(A.c, page, head)[1]);
         }
@@ -335,94 +378,98 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
 
         if (warp < kSoftWarps) {
             // ---------------------------------------------------------------- softmax
-            const int i = warp * 32 + lane;
-            const int seen = i < rows ? visible_keys(A.c, at, (row0 + i) / A.group) - p.first * kKvBlock : 0;
-            const unsigned mine = tmem + ((unsigned)(warp * 32) << 16);
-            const float row_scale = M.row_scale[i], over = most > 0.0f ? __fdiv_rn(1.0f, most) : 0.0f;
+            const int half = warp >> 2, i = (warp & 3) * 32 + lane;
+            const int in_sight = i < rows ? visible_keys(A.c, at, (row0 + i) / A.group) : 0;
+            const int seen = in_sight - p.first * kKvBlock - 32 * half;  // from this half of the first page on
+            const unsigned mine = tmem + ((unsigned)((warp & 3) * 32) << 16), cols = mine + P + 64 * kDigits + 16 * half;  // O, and the weights
+            const float row_scale = in_sight ? M.row_scale[i] : 0.0f, over = most > 0.0f ? __fdiv_rn(1.0f, most) : 0.0f;
             float4 *kept = W.sum + (size_t)blockIdx.x * (P / 4) * kTileRows + i;  // this row's sum of flushed pages, every 128th
             float m = -INFINITY, sum = 0.0f, kept_m = -INFINITY;
             bool ok = true;
-            auto scales_of = [&](int page) {  // -1: no page
-                const float *s = page >= 0 ? page_scales(A.c, page, head) : nullptr;
-                return s ? make_float2(s[0], s[1]) : make_float2(-1.0f, 0.0f);
-            };
+            // The two warps of 32 rows meet at a vote; they leave at the same one, which a warp whose wait has failed still comes to.
+            auto vote = [&](bool x) -> bool { return pair_or(1 + (warp & 3), x); };
+            auto leave = [&]() -> bool { return vote(!ok || *(volatile int *)&M.abort_flag); };
+            bool gone = false;
             // O of local page j's group, complete, joins the kept sum
             auto flush = [&](int j) -> bool {
-                const int g = pages + j;
-                if (!__all_sync(0xffffffffu, wait(&M.o_done[g % kBufs], g / kBufs & 1))) return false;
+                if (!__all_sync(0xffffffffu, wait(&M.o_done, (pages + j) & 1))) return false;
                 tc_fence_after();
                 const bool fresh = j < kFlush;
                 const float alpha = fresh || kept_m >= m ? 1.0f : exp2_fast(kept_m - m);
                 kept_m = m;
+                const bool scaled = __any_sync(0xffffffffu, alpha != 1.0f);  // seldom: else the sum is added where it lies
 #pragma unroll 1
-                for (int k = 0; k < P; k += 32) {
-                    unsigned x[32];
-                    float4 f[8];
-                    tmem_ld32_async(mine + k, x);
-                    if (!fresh) {
+                for (int k = half * (P / 2); k < (half + 1) * (P / 2); k += 16) {
+                    unsigned x[16];
+                    float4 f[4];
+                    tmem_ld16_async(mine + k, x);
+                    if (scaled) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = kept[(k / 4 + e) * kTileRows];
+                        for (int e = 0; e < 4; ++e) f[e] = __ldcg(kept + (k / 4 + e) * kTileRows);
                     }
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
+                    for (int e = 0; e < 4; ++e) {
                         float4 o = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
                                                __uint_as_float(x[4 * e + 3]));
-                        if (!fresh) o = make_float4(f[e].x * alpha + o.x, f[e].y * alpha + o.y, f[e].z * alpha + o.z, f[e].w * alpha + o.w);
-                        kept[(k / 4 + e) * kTileRows] = o;
+                        if (scaled) o = make_float4(f[e].x * alpha + o.x, f[e].y * alpha + o.y, f[e].z * alpha + o.z, f[e].w * alpha + o.w);
+                        if (fresh || scaled) kept[(k / 4 + e) * kTileRows] = o;
+                        else atomicAdd(kept + (k / 4 + e) * kTileRows, o);  // (this thread alone adds to it)
                     }
                 }
                 tc_fence_before();
                 bar_arrive(&M.o_free);
                 return true;
             };
-            // scales are loaded two pages ahead, table entries three
-            float2 sc = scales_of(checked(0, entry_at(0))), sc1 = scales_of(checked(1, entry_at(1)));
-            int entry2 = entry_at(2);
             for (int j = 0; j < n; ++j) {
-                const int g = pages + j, buf = g % kBufs;
-                const unsigned cols = mine + P + 64 * buf;
-                const int left = sc.x >= 0.0f ? seen - j * kKvBlock : 0;
-                const float c = sc.x * row_scale, fv = sc.y * over;
-                sc = sc1;
-                sc1 = scales_of(checked(j + 2, entry2));
-                entry2 = entry_at(j + 3);
-                if (!(ok = __all_sync(0xffffffffu, wait(&M.s_full[buf], g / kBufs & 1)))) break;
+                const int g = pages + j;
+                ok = ok && __all_sync(0xffffffffu, wait(&M.s_full, g & 1));
                 tc_fence_after();
-                float a[64];
+                const float2 sc = M.page_scale[g % kScales];
+                const int left = sc.x >= 0.0f ? seen - j * kKvBlock : 0;
+                float a[32];  // digits' sums joined: logits but for the positive factor c
                 {
-                    unsigned x[32], z[32];
-                    tmem_ld32_async(cols, x);
-                    tmem_ld32_async(cols + 32, z);
+                    unsigned x[kDigits][32];
+#pragma unroll
+                    for (int e = 0; e < kDigits; ++e) tmem_ld32_async(mine + P + 64 * e + 32 * half, x[e]);
                     tmem_wait_ld();
+                    tc_fence_before();
+                    bar_arrive(&M.s_free);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        a[e] = __uint_as_float(x[e]) * c;
-                        a[32 + e] = __uint_as_float(z[e]) * c;
-                    }
+                    for (int e = 0; e < 32; ++e)
+                        a[e] = __fmaf_rn(whole_float(x[2][e]), 65536.0f, (float)((int)x[1][e] * 256 + (int)x[0][e]));
                 }
-                if (__any_sync(0xffffffffu, left < kKvBlock)) {
+                // a positive factor, so that -infinity stays that; what would be below this makes logits of 0
+                const float c = isnan(row_scale) ? row_scale : fmaxf(sc.x * row_scale, 1e-30f);
+                // weights take the page's value scale in the exponent. One of 0 has values of 0, and one below 2^-60 of the
+                // largest counts as that, which FP16 weights would not hold either
+                const float fv = fmaxf(sc.y * over, 0x1p-60f);
+                if (__any_sync(0xffffffffu, left < 32)) {
 #pragma unroll
-                    for (int k = 0; k < 64; ++k) a[k] = k < left ? a[k] : -INFINITY;
+                    for (int k = 0; k < 32; ++k) a[k] = k < left ? a[k] : -INFINITY;
                 }
                 float big[4] = {a[0], a[1], a[2], a[3]};
 #pragma unroll
-                for (int k = 4; k < 64; ++k) big[k & 3] = fmaxf(big[k & 3], a[k]);
-                const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+                for (int k = 4; k < 32; ++k) big[k & 3] = fmaxf(big[k & 3], a[k]);
+                float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+                top *= c;
                 bool due = j > 0 && j % kFlush == 0;  // the group of pages before this one is to be kept
-                if (__any_sync(0xffffffffu, top > m + kGrow)) {
+                if (vote(!ok || top > m + kGrow)) {  // seldom
+                    M.half_row[j & 1][half][i] = top;
+                    if ((gone = leave())) break;
+                    top = fmaxf(top, M.half_row[j & 1][half ^ 1][i]);
                     if (due) {
-                        if (!(ok = flush(j - 1))) break;
+                        if (!(ok = flush(j - 1))) continue;
                         due = false;
                     }
                     const float now = fmaxf(m, top), alpha = now > m ? exp2_fast(m - now) : 1.0f;
                     m = now;
                     sum *= alpha;
                     if (j % kFlush) {
-                        if (!(ok = __all_sync(0xffffffffu, wait(&M.o_done[(g - 1) % kBufs], (g - 1) / kBufs & 1)))) break;
+                        if (!(ok = __all_sync(0xffffffffu, wait(&M.o_done, (g - 1) & 1)))) continue;
                         tc_fence_after();
 #pragma unroll 1
-                        for (int k = 0; k < P; k += 16) {
+                        for (int k = half * (P / 2); k < (half + 1) * (P / 2); k += 16) {
                             unsigned x[16];
                             tmem_ld16_async(mine + k, x);
                             tmem_wait_ld();
@@ -432,45 +479,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                         }
                     }
                 }
-                const float from = (m == -INFINITY ? 0.0f : m) - kLiftP;
+                const float from = kLiftP - (m == -INFINITY ? 0.0f : m) + log2f(fv);
                 float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                unsigned hi[16], lo[16];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {  // 32 weights to 16 columns of high and 16 of low halves
-                    unsigned hi[16], lo[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p0 = exp2_fast(a[32 * k + 2 * e] - from), p1 = exp2_fast(a[32 * k + 2 * e + 1] - from);
-                        add[(2 * e) & 3] += p0;
-                        add[(2 * e + 1) & 3] += p1;
-                        split_pair(p0 * fv, p1 * fv, hi[e], lo[e]);
-                    }
-                    tmem_st16(cols + 16 * k, hi);
-                    tmem_st16(cols + 32 + 16 * k, lo);
+                for (int e = 0; e < 16; ++e) {
+                    const float p0 = exp2_fast(__fmaf_rn(a[2 * e], c, from)), p1 = exp2_fast(__fmaf_rn(a[2 * e + 1], c, from));
+                    add[(2 * e) & 3] += p0;
+                    add[(2 * e + 1) & 3] += p1;
+                    split_pair(p0, p1, hi[e], lo[e]);
                 }
-                sum += (add[0] + add[1]) + (add[2] + add[3]);
+                if (g > 0 && !(ok = __all_sync(0xffffffffu, wait(&M.o_done, (g - 1) & 1)))) continue;  // the weights before are used
+                tc_fence_after();
+                tmem_st16(cols, hi);
+                tmem_st16(cols + 32, lo);
+                sum += __fdividef((add[0] + add[1]) + (add[2] + add[3]), fv);
                 tmem_wait_st();
                 tc_fence_before();
-                bar_arrive(&M.w_full[buf]);
-                if (due && !(ok = flush(j - 1))) break;
+                bar_arrive(&M.w_full);
+                if (due) ok = flush(j - 1);
             }
-            const int g = pages + n - 1;
-            if (ok && (ok = __all_sync(0xffffffffu, wait(&M.o_done[g % kBufs], g / kBufs & 1)))) {
+            if (!gone) {
+                M.half_row[n & 1][half][i] = sum;
+                gone = leave();
+            }
+            if (!gone && (ok = __all_sync(0xffffffffu, wait(&M.o_done, (pages + n - 1) & 1)))) {
+                sum += M.half_row[n & 1][half ^ 1][i];
                 tc_fence_after();
                 const bool whole = n == p.n, flushed = n > kFlush;
                 const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum), by = whole ? most : 1.0f;
                 const float alpha = !flushed || kept_m >= m ? 1.0f : exp2_fast(kept_m - m);
                 float *dst = i < rows ? prompt_row(A, p.run, head, row0 + i) : nullptr;
                 const bool wide = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-                if (!whole) (p.first ? W.tail_ml : W.head_ml)[blockIdx.x * kTileRows + i] = make_float4(m, sum, most, 0.0f);
+                if (!whole && half == 0) (p.first ? W.tail_ml : W.head_ml)[blockIdx.x * kTileRows + i] = make_float4(m, sum, most, 0.0f);
 #pragma unroll 1
-                for (int k = 0; k < P; k += 32) {
+                for (int k = half * (P / 2); k < (half + 1) * (P / 2); k += 32) {
                     unsigned x[32];
                     float4 f[8];
                     __syncwarp();
                     tmem_ld32_async(mine + k, x);
                     if (flushed) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = kept[(k / 4 + e) * kTileRows];
+                        for (int e = 0; e < 8; ++e) f[e] = __ldcg(kept + (k / 4 + e) * kTileRows);
                     }
                     tmem_wait_ld();
 #pragma unroll
@@ -495,110 +545,126 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                     }
                 }
             }
-        } else if (warp < kMmaWarp) {
+        } else if (warp < kKeyWarp) {
             // ---------------------------------------------------------------- converters
-            // items in the order of use: keys 0, then keys j + 1 and values j for each j. A thread takes every
-            // 96th 16-byte piece: piece w is codes 16 (w % 4) .. of row w / 4, two swizzled 16-byte chunks
-            constexpr int kAll = P * 64 / 16, kPieces = (kAll + kConvThreads - 1) / kConvThreads;
+            // piece w of a page's values is codes 16 (w % 4) .. of row w / 4, two swizzled 16-byte chunks of FP16
             const int ct = tid - 32 * kSoftWarps;
-            auto load = [&](int page, int kind, uint4(&w)[kPieces]) {
-                const uint4 *src = page >= 0 ? reinterpret_cast<const uint4 *>(page_codes(A.c, page, head, kind)) : nullptr;
-#pragma unroll
-                for (int k = 0; k < kPieces; ++k)
-                    w[k] = src && k * kConvThreads + ct < kAll ? src[k * kConvThreads + ct] : make_uint4(0, 0, 0, 0);
-            };
-            int count = used;
-            auto store = [&](const uint4(&w)[kPieces]) -> bool {
-                const int s = count % Sm::slots;
-                if (!wait(&M.empty[s], (count / Sm::slots & 1) ^ 1)) return false;
-#pragma unroll
-                for (int k = 0; k < kPieces; ++k) {
-                    const int piece = k * kConvThreads + ct, row = piece >> 2, ch = (piece & 3) * 2;
-                    if (piece >= kAll) break;
+            for (int j = 0; j < n; ++j) {
+                const int g = pages + j, s = g % Sm::v_ring;
+                const unsigned turn = g / Sm::v_ring & 1;
+                if (!__all_sync(0xffffffffu, wait(&M.raw_full[s], turn) && wait(&M.v_empty[s], turn ^ 1))) break;
+#pragma unroll 8
+                for (int piece = ct; piece < P * 4; piece += kConvThreads) {
+                    const int row = piece >> 2, ch = (piece & 3) * 2;
+                    const uint4 w = reinterpret_cast<const uint4 *>(M.raw[s])[piece];
                     uint4 x, z;
-                    codes_to_half(w[k].x, x.x, x.y);
-                    codes_to_half(w[k].y, x.z, x.w);
-                    codes_to_half(w[k].z, z.x, z.y);
-                    codes_to_half(w[k].w, z.z, z.w);
-                    unsigned char *dst = M.slot[s] + row * 128;
+                    codes_to_half(w.x, x.x, x.y);
+                    codes_to_half(w.y, x.z, x.w);
+                    codes_to_half(w.z, z.x, z.y);
+                    codes_to_half(w.w, z.z, z.w);
+                    unsigned char *dst = M.v[s] + row * 128;
                     *reinterpret_cast<uint4 *>(dst + ((ch ^ (row & 7)) << 4)) = x;
                     *reinterpret_cast<uint4 *>(dst + (((ch + 1) ^ (row & 7)) << 4)) = z;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(&M.full[s]);
-                ++count;
-                return true;
-            };
-            // each item's loads are in flight while the item before it is converted
-            uint4 keys[kPieces], values[kPieces];
-            int page = checked(0, entry_at(0)), page1 = checked(1, entry_at(1)), entry2 = entry_at(2);
-            load(page, 0, keys);
-            load(page1, 0, values);  // (the next keys, for the first step)
-            bool ok = store(keys);
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) keys[k] = values[k];
-            for (int j = 0; j < n && ok; ++j) {
-                load(page, 1, values);
-                if (j + 1 < n) ok = store(keys);
-                page = page1;
-                page1 = checked(j + 2, entry2);
-                entry2 = entry_at(j + 3);
-                if (j + 2 < n) load(page1, 0, keys);
-                ok = ok && store(values);
+                bar_arrive(&M.v_full[s]);
+                __syncwarp();
+                if (lane == 0) bar_arrive(&M.raw_empty[s]);
+            }
+        } else if (warp == kKeyWarp) {
+            // ---------------------------------------------------------------- keys and values
+            // 32 pages at a time, a page a lane, the next ones looked up on the way
+            int next_page = checked(lane, entry_at(lane));
+            float2 next_scale = scales_of(next_page);
+            bool ok = true;
+            int asked[2] = {0, 0};
+            for (int base = 0; base < n && ok; base += 32) {
+                const int page = next_page;
+                const float2 scale = next_scale;
+                next_page = checked(base + 32 + lane, entry_at(base + 32 + lane));
+                next_scale = scales_of(next_page);
+                for (int e = 0; e < min(32, n - base); ++e) {
+                    const int g = pages + base + e, k = g % Sm::k_ring, v = g % Sm::v_ring, at_page = __shfl_sync(0xffffffffu, page, e);
+                    if (!(ok = __all_sync(0xffffffffu, wait(&M.k_empty[k], (g / Sm::k_ring & 1) ^ 1)))) break;
+                    if (lane == 0 && at_page >= 0) {  // (no key of a page that is not there is in sight: what lies in the rings has no weight)
+                        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(su32(&M.k_full[k])), "r"(P * kKvBlock) : "memory");
+                        tma3(M.k[k], &A.keys, 0, head * 2 * P, at_page, &M.k_full[k]);
+                    }
+                    __syncwarp();
+                    if (lane == e) {
+                        M.page_scale[g % kScales] = scale;
+                        bar_arrive(&M.k_full[k]);
+                    }
+                    ++asked[0];
+                    if (!(ok = __all_sync(0xffffffffu, wait(&M.raw_empty[v], (g / Sm::v_ring & 1) ^ 1)))) break;
+                    if (lane == 0) {
+                        if (at_page >= 0) {
+                            bar_expect(&M.raw_full[v], P * kKvBlock);
+                            bulk(M.raw[v], page_codes(A.c, at_page, head, 1), P * kKvBlock, &M.raw_full[v]);
+                        } else {
+                            bar_arrive(&M.raw_full[v]);
+                        }
+                    }
+                    ++asked[1];
+                }
+            }
+            if (*(volatile int *)&M.abort_flag) {  // what was asked for lands before the CTA leaves
+                auto land = [&](unsigned long long *bars, int ring, int count) {
+                    for (int a = max(0, count - ring); a < count; ++a)
+                        for (const long long began = clock64(); !bar_try(&bars[(pages + a) % ring], (pages + a) / ring & 1) && clock64() - began < kLimit;) {
+                        }
+                };
+                land(M.k_full, Sm::k_ring, asked[0]);
+                land(M.raw_full, Sm::v_ring, asked[1]);
             }
         } else {
             // ---------------------------------------------------------------- MMA issuer
-            const unsigned id_s = idesc_f16(kTileRows, kKvBlock), id_o = idesc_f16(kTileRows, P);
-            const unsigned long long qd[2] = {sw128_desc(su32(M.q[0][0])), sw128_desc(su32(M.q[1][0]))};
-            int count = used, freed = flushes;
+            const unsigned id_s = idesc_i8(kKvBlock, true), id_o = idesc_f16(kTileRows, P);
+            int freed = flushes;
             bool ok = true;
             auto scores = [&](int j) {
-                const int s = count % Sm::slots, g = pages + j, buf = g % kBufs;
-                ok = ok && __all_sync(0xffffffffu, wait(&M.full[s], count / Sm::slots & 1));
-                if (ok && g >= kBufs) ok = __all_sync(0xffffffffu, wait(&M.o_done[buf], (g - kBufs) / kBufs & 1));  // that page's weights are used
+                const int g = pages + j, s = g % Sm::k_ring;
+                ok = ok && __all_sync(0xffffffffu, wait(&M.k_full[s], g / Sm::k_ring & 1));
+                if (ok && g > 0) ok = __all_sync(0xffffffffu, wait(&M.s_free, (g - 1) & 1));
                 if (!ok) return;
                 tc_fence_after();
-                const unsigned long long kd = sw128_desc(su32(M.slot[s]));
+                if (elect_one()) {
+#pragma unroll
+                    for (int e = 0; e < kDigits; ++e)
+#pragma unroll
+                        for (int b = 0; b < P / 64; ++b) {
+                            const unsigned long long qd = sw64_desc(su32(M.q[e][b])), kd = sw64_desc(su32(M.k[s] + b * 4096));
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) mma_i8(tmem + P + 64 * e, qd + 2 * k, kd + 2 * k, id_s, b > 0 || k > 0);
+                        }
+                    mma_commit(&M.k_empty[s]);
+                    mma_commit(&M.s_full);
+                }
+                __syncwarp();
+            };
+            scores(0);
+            for (int j = 0; j < n && ok; ++j) {
+                if (j + 1 < n) scores(j + 1);
+                const int g = pages + j, s = g % Sm::v_ring;
+                ok = ok && __all_sync(0xffffffffu, wait(&M.v_full[s], g / Sm::v_ring & 1) && wait(&M.w_full, g & 1));
+                if (ok && j > 0 && j % kFlush == 0) ok = __all_sync(0xffffffffu, wait(&M.o_free, freed++ & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const unsigned w = tmem + P + 64 * kDigits;
+                const unsigned long long vd = sw128_desc(su32(M.v[s]));
                 if (elect_one()) {
                     // the low halves first: the accumulator is then small, and what an addition drops as well
 #pragma unroll
                     for (int h = 1; h >= 0; --h)
 #pragma unroll
-                        for (int b = 0; b < P / 64; ++b)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                mma_f16(tmem + P + 64 * buf, qd[h] + b * (kTileRows * 128 >> 4) + 2 * k, kd + b * (kKvBlock * 128 >> 4) + 2 * k,
-                                        id_s, b > 0 || k > 0 || h == 0);
-                    mma_commit(&M.empty[s]);
-                    mma_commit(&M.s_full[buf]);
-                }
-                __syncwarp();
-                ++count;
-            };
-            scores(0);
-            for (int j = 0; j < n && ok; ++j) {
-                if (j + 1 < n) scores(j + 1);
-                const int s = count % Sm::slots, g = pages + j, buf = g % kBufs;
-                ok = ok && __all_sync(0xffffffffu, wait(&M.full[s], count / Sm::slots & 1) && wait(&M.w_full[buf], g / kBufs & 1));
-                if (ok && j > 0 && j % kFlush == 0) ok = __all_sync(0xffffffffu, wait(&M.o_free, freed++ & 1));
-                if (!ok) break;
-                tc_fence_after();
-                const unsigned w = tmem + P + 64 * buf;
-                const unsigned long long vd = sw128_desc(su32(M.slot[s]));
-                if (elect_one()) {
-#pragma unroll
-                    for (int h = 1; h >= 0; --h)
-#pragma unroll
                         for (int k = 0; k < 4; ++k) mma_f16_ts(tmem, w + 32 * h + 8 * k, vd + 2 * k, id_o, j % kFlush > 0 || k > 0 || h == 0);
-                    mma_commit(&M.empty[s]);
-                    mma_commit(&M.o_done[buf]);
+                    mma_commit(&M.v_empty[s]);
+                    mma_commit(&M.o_done);
                 }
                 __syncwarp();
-                ++count;
             }
         }
         pages += n;
-        used += 2 * n;
         flushes += (n - 1) / kFlush;
         tc_fence_before();
         __syncthreads();  // the piece is done: its queries, its S and O are free
@@ -607,12 +673,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
     }
     __syncthreads();
     if (tid == 0 && M.abort_flag) raise_error(A.c.err, kErrWaitTimeout);
-    if (warp == kMmaWarp) {
-        // every MMA issued must complete before TMEM is released, whether or not the others have given up
-        if (elect_one()) mma_commit(&M.drained);
-        __syncwarp();
+    // every MMA issued must complete before TMEM is released, whether or not the others have given up
+    if (warp == kMmaWarp && lane == 0) {
+        mma_commit(&M.drained);
         for (const long long began = clock64(); !bar_try(&M.drained, 0) && clock64() - began < kLimit;) {
         }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
@@ -691,6 +760,7 @@ cudaError_t launch(PromptArgs A, cudaStream_t s) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_kv8_prompt<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
     if (e != cudaSuccess) return e;
+    if (!page_map(A.c, P, &A.keys)) return cudaErrorInvalidValue;
     const long long pairs = (long long)A.tiles * A.runs.segments, units = pairs * A.c.kv_heads;
     const int most = sms < kMaxGrid ? sms : kMaxGrid;
     // Units shared page by page where whole ones would leave the last round of CTAs uneven
@@ -706,7 +776,7 @@ cudaError_t launch(PromptArgs A, cudaStream_t s) {
 cudaError_t kv8_attend_prompt(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, float scale, float *y, cudaStream_t s) {
     const int group = heads / c.kv_heads;
     const long long rows = (long long)r.count * group;
-    const PromptArgs A{c, q, stride, heads, group, (int)((rows + kTileRows - 1) / kTileRows), r, scale * 1.4426950408889634f, y, 0};
+    const PromptArgs A{c, q, stride, heads, group, (int)((rows + kTileRows - 1) / kTileRows), r, scale * 1.4426950408889634f, y, 0, {}};
     if (c.padded == 64) return launch<64>(A, s);
     if (c.padded == 128) return launch<128>(A, s);
     return launch<256>(A, s);
