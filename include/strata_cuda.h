@@ -299,7 +299,7 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
  * append: scale = amax / 127 over a block's rows so far (0 below 2^-100), code = x times the
  *   reciprocal of scale, rounded to nearest even. A block's codes depend on its rows alone, not on how they
  *   were split over calls. Appending goes on where the sequence ends; a run that starts at a block's
- *   first token starts that block afresh. Rows dropped from an open block leave its scale and marks as they were.
+ *   first token starts that block afresh, and one that starts inside the open block drops its rows from there on.
  *   A value that is not finite is stored as zero and reported. Runs of one call name different sequences.
  * select: for each token and key/value head the `top` blocks (of those at or before the token) with the
  *   largest bound on the summed logits of the group's queries, in ascending order, -1 past the last: i32

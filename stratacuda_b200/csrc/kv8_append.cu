@@ -12,8 +12,8 @@ constexpr int kFew = 4;  // new rows of an open block that are worth trying to a
 // the sequence already holds (from `open`) and the new ones, are read into registers, the largest
 // magnitude fixes the scale, the codes are laid out in shared memory as the page holds them and
 // copied out whole. Bound by memory: 4 bytes read and 1 written a value.
-// A few rows added to an open block (decode) mostly leave its scale as it is; then all other codes stand
-// and only the new rows' are written, with the same result. Bound by the latency of the look-ups.
+// A few rows added to an open block (decode) mostly leave its scale as it is; then all other codes stand and only the
+// new rows' and the marks are written, with the same result. Bound by the latency of the look-ups and of the open rows.
 template <int P, bool WIDE>
 __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const float *k, const float *v, long long stride, const Kv8Runs runs) {
     constexpr int kTiles = P / 64;  // 4 tokens x 4 channels a tile, 16 * P / 4 tiles
@@ -57,44 +57,63 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
             open[row * open_row + ch] = isfinite(f) ? f : 0.0f;
         }
     };
-    if (r0 > 0 && r1 - r0 <= kFew) {
-        static_assert(P <= kThreads, "a thread a channel");
-        const int ch = tid;
-        float f[kFew], amax = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < kFew; ++i) {
-            f[i] = r0 + i < r1 && ch < c.dim ? in[(long long)(r0 + i) * stride + ch] : 0.0f;
-            if (!isfinite(f[i])) {
-                bad = true;
-                f[i] = 0.0f;
-            }
-            amax = fmaxf(amax, fabsf(f[i]));
-        }
+    // (a run that goes on past this block leaves another's rows in `open`, with which it could not be repeated)
+    if (r0 > 0 && r1 - r0 <= kFew && end - (long long)block * kKvBlock <= kKvBlock) {
+        // The block's values by channel: the largest magnitude fixes the scale, and the lowest and highest the marks, since
+        // rounding keeps order. A page whose scale is that one holds the other rows' codes already.
+        constexpr int kDeep = kThreads / P;  // threads a channel
+        static_assert(kDeep * P == kThreads, "whole channels");
+        __shared__ float lowest_s[kThreads], highest_s[kThreads];
+        const int ch = tid % P, deep = tid / P;
         const float scale = page >= 0 ? page_scales(c, page, head)[kind] : 0.0f;
+        float f[kFew], lowest = INFINITY, highest = -INFINITY;
+        bool bad = false;
+        auto take = [&](float &x) {
+            if (!isfinite(x)) {
+                bad = true;
+                x = 0.0f;
+            }
+            lowest = fminf(lowest, x);
+            highest = fmaxf(highest, x);
+        };
+#pragma unroll
+        for (int i = 0; i < kFew; ++i) f[i] = r0 + i < r1 && ch < c.dim ? in[(long long)(r0 + i) * stride + ch] : 0.0f;
+        if (ch < c.dim) {
+#pragma unroll 16
+            for (int row = deep; row < r0; row += kDeep) {
+                float x = open[row * open_row + ch];
+                take(x);
+            }
+#pragma unroll
+            for (int i = 0; i < kFew; ++i)
+                if (r0 + i < r1) take(f[i]);
+        }
+        lowest_s[tid] = lowest;
+        highest_s[tid] = highest;
+        float amax = ch < c.dim ? fmaxf(-lowest, highest) : 0.0f;
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
         if (tid % 32 == 0) red[tid / 32] = amax;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kThreads / 32; ++i) amax = fmaxf(amax, red[i]);
-        if (page >= 0 && (amax < 0x1p-100f ? 0.0f : __fdiv_rn(amax, 127.0f)) <= scale) {
+        if (page >= 0 && (amax < 0x1p-100f ? 0.0f : __fdiv_rn(amax, 127.0f)) == scale) {
             if (bad) raise_error(c.err, kErrKvValue);
-            if (ch < c.dim) {
+            if (ch < c.dim && deep == 0) {
                 const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+                auto code = [&](float x) { return (int8_t)max(-127, min(127, __float2int_rn(__fmul_rn(x, inv)))); };
                 int8_t *codes = page_codes(c, page, head, kind), *m = page_marks(c, page, head);
-                int lo = 127, hi = -127;
 #pragma unroll
-                for (int i = 0; i < kFew; ++i) {
-                    if (r0 + i >= r1) continue;
-                    const int q = max(-127, min(127, __float2int_rn(__fmul_rn(f[i], inv))));
-                    codes[kind ? ch * kKvBlock + r0 + i : key_byte(r0 + i, ch)] = (int8_t)q;
-                    lo = min(lo, q);
-                    hi = max(hi, q);
-                }
+                for (int i = 0; i < kFew; ++i)
+                    if (r0 + i < r1) codes[kind ? ch * kKvBlock + r0 + i : key_byte(r0 + i, ch)] = code(f[i]);
                 if (!kind) {
-                    if (lo < m[ch]) m[ch] = (int8_t)lo;
-                    if (hi > m[P + ch]) m[P + ch] = (int8_t)hi;
+#pragma unroll
+                    for (int d = 1; d < kDeep; ++d) {
+                        lowest = fminf(lowest, lowest_s[d * P + ch]);
+                        highest = fmaxf(highest, highest_s[d * P + ch]);
+                    }
+                    m[ch] = code(lowest);
+                    m[P + ch] = code(highest);
                 }
             }
             keep();

@@ -574,3 +574,144 @@ def test_handles_graph_replay_and_device_errors():
             from stratacuda_b200.backend import Buffer
             c.attend(bufs[2], heads, Buffer(b, 123456, 4, "f32"), seq, start)
         b.idle()
+
+
+# ---------------------------------------------------------------- later additions
+@pytest.mark.parametrize("kv,dim", [(1, 16), (2, 96), (2, 256)])
+def test_append_again_from_inside_an_open_block(kv, dim):
+    """A run that starts inside the open block takes the place of its rows from there on: scale, codes and marks are
+    those of the rows that remain and the new ones, also where a dropped row had set the scale or a mark."""
+    c = Cache(kv, dim, 1, 2)
+    rng = np.random.default_rng(4)
+    k, v = (rng.normal(0, 1, (40, kv, dim)).astype(np.float32) for _ in range(2))
+    c.append(k[None], v[None], [0], [0])
+    for at, rows, size in ((38, 2, 1.0), (30, 1, 50.0), (30, 1, 0.01), (29, 3, 1.0), (10, 2, 1e-3)):
+        k2, v2 = (rng.normal(0, size, (rows, kv, dim)).astype(np.float32) for _ in range(2))
+        c.append(k2[None], v2[None], [0], [at])
+        k, v = np.concatenate([k[:at], k2]), np.concatenate([v[:at], v2])
+        page, p = c.order[0, 0], R.padded(dim)
+        for h in range(kv):
+            keys = c.codes[page, h, 0].cpu().numpy().reshape(p // 64, BLOCK, 64).transpose(1, 0, 2).reshape(BLOCK, p)
+            values = c.codes[page, h, 1].cpu().numpy().reshape(p, BLOCK).T
+            for kind, (got, x) in enumerate(((keys, k), (values, v))):
+                want, scale = R.quantise(x[:, h])
+                assert c.scales[page, h, kind].item() == scale, (at, h, kind)
+                np.testing.assert_array_equal(got[:at + rows, :dim], want)
+                if kind == 0:
+                    np.testing.assert_array_equal(c.marks[page, h].cpu().numpy()[:, :dim], [want.min(0), want.max(0)])
+
+
+class WideCache(Cache):
+    """A cache whose table has room for more blocks than there are pages; the test fills the table."""
+
+    def __init__(self, kv, dim, sequences, blocks, pages):
+        from stratacuda_b200.kv8 import DeviceCache
+        super().__init__(kv, dim, 1, pages - 2)
+        self.sequences, self.blocks = sequences, blocks
+        self.open = self.torch.full((sequences, 2, BLOCK, kv, dim), float("nan"), device="cuda")
+        self.table = self.torch.full((sequences, blocks), -1, dtype=self.torch.int32, device="cuda")
+        self.view = DeviceCache(kv, dim, self.pages, sequences, blocks, self.codes, self.marks, self.scales, self.open, self.table,
+                                self.workspace, self.status)
+
+
+def _rising(rng, n, kv, dim, q, slope):
+    """Keys whose logits with the queries' common direction rise by about `slope` (log2) every 128 tokens, and values whose
+    blocks differ in size."""
+    k = rng.normal(0, 0.2, (n, kv, dim))
+    direction = q / np.sum(q * q)
+    k += (np.arange(n) / 128 * slope * math.log(2) * math.sqrt(dim))[:, None, None] * direction
+    v = rng.normal(0, 1, (n, kv, dim)) * 2.0 ** rng.integers(-3, 4, (n + 63) // 64).repeat(64)[:n, None, None]
+    return k.astype(np.float32), v.astype(np.float32)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(5, 1, 64), (16, 2, 96), (12, 1, 256), (17, 1, 40)])
+@pytest.mark.parametrize("slope", [0.0, 2.5, 5.0, 7.5, 30.0, -6.0])
+def test_attend_long_lists_with_a_rising_maximum(heads, kv, dim, slope):
+    """One sequence of some dozens of pages in a table of many more, so that the form for long lists takes it, and a
+    short one beside it."""
+    c = WideCache(kv, dim, 2, 1600 // kv, 64)
+    rng = np.random.default_rng(8)
+    direction = rng.normal(0, 1, dim)
+    n, short = 64 * 45 + 17, 70
+    k, v = _rising(rng, n, kv, dim, direction, slope)
+    c.table[0, :46] = c.i32(np.arange(46))
+    c.table[1, :2] = c.i32([50, 49])
+    c.append(k[None], v[None], [0], [0])
+    c.append(k[None, :short], v[None, :short], [1], [0])
+    q = (direction + rng.normal(0, 0.05, (2, 1, heads, dim))).astype(np.float32)
+    got = c.attend(q, heads, [0, 1], [n - 1, short - 1])
+    c.check_attend(got[0], q[0], k, v, n - 1, 1 / math.sqrt(dim))
+    c.check_attend(got[1], q[1], k[:short], v[:short], short - 1, 1 / math.sqrt(dim))
+    assert c.errors() == 0
+    # the same list as picks
+    top = 46
+    picks = np.arange(top)[None, None].repeat(kv, 1)
+    again = c.attend(q[:1], heads, [0], [n - 1], picks=picks.reshape(1, kv, top), top=top)
+    c.check_attend(again[0], q[0], k, v, n - 1, 1 / math.sqrt(dim))
+
+
+def test_attend_more_steps_than_whole_number_sums_hold():
+    """A unit of more than 256 pages on one CTA: its whole-number sums have to move on the way."""
+    kv, dim, heads, n = 1, 16, 2, 64 * 300
+    sequences = 160  # as many units as keep a unit on one CTA or two
+    c = WideCache(kv, dim, sequences, 300, 300)
+    rng = np.random.default_rng(9)
+    k = rng.normal(0, 0.05, (n, kv, dim)).astype(np.float32)
+    v = rng.normal(1, 0.01, (n, kv, dim)).astype(np.float32)
+    c.table[:] = c.i32(np.arange(300))
+    c.append(k[None], v[None], [0], [0])
+    q = rng.normal(0, 1, (sequences, 1, heads, dim)).astype(np.float32)
+    got = c.attend(q, heads, np.arange(sequences), np.full(sequences, n - 1))
+    for s in (0, 1, 77, 159):
+        c.check_attend(got[s], q[s], k, v, n - 1, 1 / math.sqrt(dim))
+
+
+def test_sparse_prompt_of_more_tokens_than_are_counted_up():
+    kv, dim, heads, count, top = 1, 24, 3, 1100, 5
+    c = Cache(kv, dim, 1, 18)
+    ks, vs = c.fill([count])
+    rng = np.random.default_rng(3)
+    q = rng.normal(0, 1, (1, count, heads, dim)).astype(np.float32)
+    picks = np.full((1, count, kv, top), -1, np.int32)
+    for t in range(count):
+        have = rng.permutation(t // 64 + 1)[:top]
+        picks[0, t, 0, :len(have)] = np.sort(have)
+    got = c.attend(q, heads, [0], [0], picks=picks.reshape(count, kv, top), top=top)
+    c.check_attend(got[0], q[0], ks[0], vs[0], 0, 1 / math.sqrt(dim), picks[0])
+
+
+@pytest.mark.parametrize("heads,kv,dim,count", [(1, 1, 64, 130), (6, 2, 96, 64), (12, 1, 256, 40)])
+@pytest.mark.parametrize("slope", [0.0, 3.0, 9.0, -6.0])
+def test_attend_prompt_after_many_pages(heads, kv, dim, count, slope):
+    """More pages than add up in one accumulator, on as few CTAs as there are units' pages to share."""
+    c = Cache(kv, dim, 1, 90)
+    rng = np.random.default_rng(12)
+    direction = rng.normal(0, 1, dim)
+    n = 64 * 88 + 11
+    k, v = _rising(rng, n, kv, dim, direction, slope)
+    c.append(k[None], v[None], [0], [0])
+    q = (direction + rng.normal(0, 0.05, (1, count, heads, dim))).astype(np.float32)
+    got = c.attend(q, heads, [0], [n - count])
+    c.check_attend(got[0], q[0], k, v, n - count, 1 / math.sqrt(dim))
+    assert c.errors() == 0
+
+
+@pytest.mark.parametrize("dim,segments,count,blocks", [(16, 300, 70, 3), (256, 40, 70, 40)])
+def test_attend_prompts_of_many_sequences(dim, segments, count, blocks):
+    """Whole units a CTA (many sequences), and long lists that one CTA walks over more than one accumulator."""
+    kv = 4 if segments > 100 else 2
+    c = Cache(kv, dim, segments, blocks) if segments > 100 else WideCache(kv, dim, segments, blocks, blocks + 2)
+    rng = np.random.default_rng(6)
+    n = 64 * blocks - 20
+    if segments <= 100:  # all read one sequence's pages
+        c.table[:] = c.i32(np.arange(blocks))
+        ks, vs = c.fill([n])
+        ks, vs = ks * segments, vs * segments
+    else:
+        ks, vs = c.fill([n] * segments)
+    q = rng.normal(0, 1, (segments, count, kv, dim)).astype(np.float32)
+    start = [(n - count) - (i % 7) for i in range(segments)]
+    got = c.attend(q, kv, np.arange(segments), start)
+    for s in range(0, segments, 13):
+        c.check_attend(got[s], q[s], ks[s], vs[s], start[s], 1 / math.sqrt(dim))
+    assert c.errors() == 0
