@@ -627,27 +627,26 @@ def _rising(rng, n, kv, dim, q, slope):
 @pytest.mark.parametrize("heads,kv,dim", [(5, 1, 64), (16, 2, 96), (12, 1, 256), (17, 1, 40)])
 @pytest.mark.parametrize("slope", [0.0, 2.5, 5.0, 7.5, 30.0, -6.0])
 def test_attend_long_lists_with_a_rising_maximum(heads, kv, dim, slope):
-    """One sequence of some dozens of pages in a table of many more, so that the form for long lists takes it, and a
-    short one beside it."""
-    c = WideCache(kv, dim, 2, 1600 // kv, 64)
+    """Sequences of some dozens of pages, all of one sequence's, and short ones between them: units that begin and end
+    anywhere in a CTA's list, and whose references have to move by little and by much."""
+    sequences, n, short, blocks = 96, 64 * 45 + 17, 70, 46
+    c = WideCache(kv, dim, sequences, blocks, blocks + 2)
     rng = np.random.default_rng(8)
     direction = rng.normal(0, 1, dim)
-    n, short = 64 * 45 + 17, 70
     k, v = _rising(rng, n, kv, dim, direction, slope)
-    c.table[0, :46] = c.i32(np.arange(46))
-    c.table[1, :2] = c.i32([50, 49])
+    c.table[:] = c.i32(np.arange(blocks))
     c.append(k[None], v[None], [0], [0])
-    c.append(k[None, :short], v[None, :short], [1], [0])
-    q = (direction + rng.normal(0, 0.05, (2, 1, heads, dim))).astype(np.float32)
-    got = c.attend(q, heads, [0, 1], [n - 1, short - 1])
-    c.check_attend(got[0], q[0], k, v, n - 1, 1 / math.sqrt(dim))
-    c.check_attend(got[1], q[1], k[:short], v[:short], short - 1, 1 / math.sqrt(dim))
+    q = (direction + rng.normal(0, 0.05, (sequences, 1, heads, dim))).astype(np.float32)
+    start = np.where(np.arange(sequences) % 5 == 3, short - 1, n - 1 - np.arange(sequences))
+    got = c.attend(q, heads, np.arange(sequences), start)
+    # the same lists as picks
+    picks = np.arange(blocks)[None, None].repeat(kv, 1).repeat(sequences, 0)
+    picks = np.where(picks <= (start // BLOCK)[:, None, None], picks, -1)
+    again = c.attend(q, heads, np.arange(sequences), start, picks=picks, top=blocks)
+    for s in (0, 1, 3, 31, 32, 50, 95):
+        for y in (got, again):
+            c.check_attend(y[s], q[s], k, v, start[s], 1 / math.sqrt(dim))
     assert c.errors() == 0
-    # the same list as picks
-    top = 46
-    picks = np.arange(top)[None, None].repeat(kv, 1)
-    again = c.attend(q[:1], heads, [0], [n - 1], picks=picks.reshape(1, kv, top), top=top)
-    c.check_attend(again[0], q[0], k, v, n - 1, 1 / math.sqrt(dim))
 
 
 def test_attend_more_steps_than_whole_number_sums_hold():
