@@ -61,36 +61,42 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
     if (r0 > 0 && r1 - r0 <= kFew && end - (long long)block * kKvBlock <= kKvBlock) {
         // The block's values by channel: the largest magnitude fixes the scale, and the lowest and highest the marks, since
         // rounding keeps order. A page whose scale is that one holds the other rows' codes already.
-        constexpr int kDeep = kThreads / P;  // threads a channel
-        static_assert(kDeep * P == kThreads, "whole channels");
-        __shared__ float lowest_s[kThreads], highest_s[kThreads];
-        const int ch = tid % P, deep = tid / P;
+        constexpr int kAcross = P / 4, kDeep = kThreads / kAcross, kRowsEach = kKvBlock / kDeep;  // a thread: 4 channels, every kDeep-th row
+        static_assert(kDeep * kAcross == kThreads && kRowsEach * kDeep == kKvBlock, "whole channels and rows");
+        __shared__ __align__(16) float lowest_s[kDeep][P], highest_s[kDeep][P];
+        const int ch4 = tid % kAcross * 4, deep = tid / kAcross, ch = tid;
         const float scale = page >= 0 ? page_scales(c, page, head)[kind] : 0.0f;
-        float f[kFew], lowest = INFINITY, highest = -INFINITY;
+        float amax = 0.0f;
         bool bad = false;
-        auto take = [&](float &x) {
-            if (!isfinite(x)) {
-                bad = true;
-                x = 0.0f;
-            }
-            lowest = fminf(lowest, x);
-            highest = fmaxf(highest, x);
-        };
+        {
+            float f[kRowsEach][4], lowest[4], highest[4];
 #pragma unroll
-        for (int i = 0; i < kFew; ++i) f[i] = r0 + i < r1 && ch < c.dim ? in[(long long)(r0 + i) * stride + ch] : 0.0f;
-        if (ch < c.dim) {
-#pragma unroll 16
-            for (int row = deep; row < r0; row += kDeep) {
-                float x = open[row * open_row + ch];
-                take(x);
+            for (int i = 0; i < kRowsEach; ++i) {
+                const int row = i * kDeep + deep;
+                const float *src = row < r0 ? open + row * open_row + ch4 : in + (long long)row * stride + ch4;
+                if (WIDE) {
+                    const float4 x = row < r1 && ch4 < c.dim ? *reinterpret_cast<const float4 *>(src) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    f[i][0] = x.x, f[i][1] = x.y, f[i][2] = x.z, f[i][3] = x.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[i][e] = row < r1 && ch4 + e < c.dim ? src[e] : 0.0f;
+                }
             }
 #pragma unroll
-            for (int i = 0; i < kFew; ++i)
-                if (r0 + i < r1) take(f[i]);
+            for (int e = 0; e < 4; ++e) {
+                lowest[e] = INFINITY, highest[e] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kRowsEach; ++i) {
+                    const bool finite = isfinite(f[i][e]);
+                    const float x = finite ? f[i][e] : 0.0f;
+                    bad |= !finite;
+                    amax = fmaxf(amax, fabsf(x));
+                    if (i * kDeep + deep < r1) lowest[e] = fminf(lowest[e], x), highest[e] = fmaxf(highest[e], x);
+                }
+            }
+            *reinterpret_cast<float4 *>(&lowest_s[deep][ch4]) = make_float4(lowest[0], lowest[1], lowest[2], lowest[3]);
+            *reinterpret_cast<float4 *>(&highest_s[deep][ch4]) = make_float4(highest[0], highest[1], highest[2], highest[3]);
         }
-        lowest_s[tid] = lowest;
-        highest_s[tid] = highest;
-        float amax = ch < c.dim ? fmaxf(-lowest, highest) : 0.0f;
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
         if (tid % 32 == 0) red[tid / 32] = amax;
@@ -99,18 +105,20 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
         for (int i = 0; i < kThreads / 32; ++i) amax = fmaxf(amax, red[i]);
         if (page >= 0 && (amax < 0x1p-100f ? 0.0f : __fdiv_rn(amax, 127.0f)) == scale) {
             if (bad) raise_error(c.err, kErrKvValue);
-            if (ch < c.dim && deep == 0) {
+            if (ch < c.dim) {
                 const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
                 auto code = [&](float x) { return (int8_t)max(-127, min(127, __float2int_rn(__fmul_rn(x, inv)))); };
                 int8_t *codes = page_codes(c, page, head, kind), *m = page_marks(c, page, head);
-#pragma unroll
-                for (int i = 0; i < kFew; ++i)
-                    if (r0 + i < r1) codes[kind ? ch * kKvBlock + r0 + i : key_byte(r0 + i, ch)] = code(f[i]);
+                for (int row = r0; row < r1; ++row) {
+                    const float x = in[(long long)row * stride + ch];
+                    codes[kind ? ch * kKvBlock + row : key_byte(row, ch)] = code(isfinite(x) ? x : 0.0f);
+                }
                 if (!kind) {
+                    float lowest = INFINITY, highest = -INFINITY;
 #pragma unroll
-                    for (int d = 1; d < kDeep; ++d) {
-                        lowest = fminf(lowest, lowest_s[d * P + ch]);
-                        highest = fmaxf(highest, highest_s[d * P + ch]);
+                    for (int d = 0; d < kDeep; ++d) {
+                        lowest = fminf(lowest, lowest_s[d][ch]);
+                        highest = fmaxf(highest, highest_s[d][ch]);
                     }
                     m[ch] = code(lowest);
                     m[P + ch] = code(highest);
