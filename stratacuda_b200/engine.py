@@ -951,24 +951,42 @@ class SequenceBatch(PromptBatch):
     prefilled there, then its state is copied into the slot) and can be copied back (``export``).
     With ``graph`` the step body is captured once and replayed; each later step writes the
     tokens, positions and PLE row ids (4 + 4 + 4 pleHeads bytes per sequence) and reads the
-    next tokens back."""
+    next tokens back.
 
-    def __init__(self, engine: StrataEngine, capacity: int, graph: bool = False):
+    With ``kv8`` the attention layers keep their keys and values in 8 bits (stratacuda_b200.kv8, a
+    quarter of the memory): each step appends to the cache and attends over it. With ``top`` as well, a
+    token attends to the ``top`` blocks of 64 tokens that strata_kv8_select picks for each key/value
+    head. A slot's values then differ from its own engine's by the cache's rounding, and a slot
+    cannot be exported."""
+
+    def __init__(self, engine: StrataEngine, capacity: int, graph: bool = False, kv8: bool = False, top: int = 0):
         require_integer(capacity, "batch capacity", 1, 1024)
+        require_integer(top, "picked blocks", 0, 512)
+        if top and not kv8:
+            raise ValueError("Blocks are picked from an 8-bit cache: top needs kv8")
+        if 0 < top < 3:
+            raise ValueError("The first and the last two blocks are always picked: top is 0 or at least 3")
         engine._check_ready()
         super().__init__(engine, [0] * capacity)
         g, b = self.g, self.b
         self.capacity = capacity
         self.use_graph = bool(graph) and getattr(engine.store, "moe_layer", None) is not None
-        self.persistent = []
+        self.persistent, self.caches = [], []
         self.disposed = False
+        self.kv8, self.top = bool(kv8), top
         hc, c = g["width"] * g["streams"], (2 * g["keyHeads"] + g["valueHeads"]) * g["ssmDim"]
         try:
             self.residual = self._keep(capacity * hc)
             self.ple_history = self._keep(capacity * (g["pleTaps"] - 1) * g["pleDilation"] * hc)
             self.states = []
             for layer in range(g["layers"]):
-                if engine.is_attention(layer):
+                if engine.is_attention(layer) and kv8:
+                    from .kv8 import BLOCK, Kv8Cache
+                    cache = Kv8Cache(b, g["kvHeads"], g["headDim"], capacity, (g["context"] + BLOCK - 1) // BLOCK,
+                                     workspace=self.caches[0].workspace if self.caches else None)
+                    self.caches.append(cache)
+                    self.states.append(dict(cache=cache))
+                elif engine.is_attention(layer):
                     kv = capacity * g["context"] * g["kvHeads"] * g["headDim"]
                     self.states.append(dict(keys=self._keep(kv), values=self._keep(kv)))
                 else:
@@ -976,6 +994,9 @@ class SequenceBatch(PromptBatch):
                                             conv=self._keep(capacity * c * 3)))
             self.dev = dict(tokens=self._keep(capacity, "i32"), positions=self._keep(capacity, "i32"),
                             ple=self._keep(capacity * g["pleHeads"], "i32"))
+            if kv8:  # the sequences of a step, and the one that is being admitted
+                self.dev.update(sequences=self._keep(capacity, "i32"), admitted=self._keep(1, "i32"), begin=self._keep(1, "i32"))
+                b.write(self.dev["sequences"], np.arange(capacity, dtype=np.int32))
         except Exception:
             self.dispose()
             raise
@@ -994,6 +1015,8 @@ class SequenceBatch(PromptBatch):
         """(engine buffer, batch buffer, elements per sequence) for every piece of sequence state."""
         out = [(engine.ple_history, self.ple_history, engine.ple_history.length)]
         for mine, theirs in zip(self.states, engine.states):
+            if "cache" in mine:
+                continue
             for key, buf in theirs.items():
                 out.append((buf, mine[key], buf.length))
         return out
@@ -1011,12 +1034,19 @@ class SequenceBatch(PromptBatch):
         engine._check_ready()
         for src, dst, n in self._regions(engine):
             self.b.copy(src, dst, n, 0, slot * n)
+        if self.kv8 and engine.position:
+            self.b.write(self.dev["admitted"], np.array([slot], np.int32))
+            for mine, theirs in zip(self.states, engine.states):
+                if "cache" in mine:
+                    mine["cache"].append(theirs["keys"], theirs["values"], self.dev["admitted"], self.dev["begin"], 1, engine.position)
         self.positions[slot] = engine.position
         self.previous[slot] = list(engine.previous)
 
     def export(self, slot: int, engine: StrataEngine) -> None:
         """Copy the sequence in `slot` back into a single-sequence engine, which continues it."""
         self._check_engine(slot, engine)
+        if self.kv8:
+            raise ValueError("An 8-bit cache holds rounded values: its sequences cannot be exported")
         if self.positions[slot] is None:
             raise ValueError("Slot is empty")
         for dst, src, n in self._regions(engine):
@@ -1086,16 +1116,29 @@ class SequenceBatch(PromptBatch):
         kr = self.mat(p + "attn_k.weight", x)
         k = rotate(o.norm(kr, o.vector(p + "attn_k_norm.weight"), hd, n * g["kvHeads"]), g["kvHeads"])
         v = self.mat(p + "attn_v.weight", x)
-        b.run("strata_kv_append_seqs", dict(K=k, V=v, Keys=st["keys"], Values=st["values"], Positions=pos, width=g["kvHeads"] * hd,
-                                            cells=g["context"], tokens=n), grid(n * g["kvHeads"] * hd))
         attn = o.alloc(n * g["heads"] * hd)
+        if self.kv8:
+            cache, seqs, picks = st["cache"], self.dev["sequences"], None
+            cache.append(k, v, seqs, pos, n, 1)
+            if self.top:
+                picks = o.alloc(n * g["kvHeads"] * self.top, "i32")
+                cache.select(q, g["heads"], picks, seqs, pos, n, 1, self.top)
+            cache.attend(q, g["heads"], attn, seqs, pos, n, 1, picks, self.top, _f32(1 / math.sqrt(hd)))
+        else:
+            self._attend(st, q, k, v, attn)
         gated = o.alloc(attn.length)
-        b.run("strata_attention_seqs", dict(Q=q, Keys=st["keys"], Values=st["values"], Positions=pos, Y=attn, dim=hd, heads=g["heads"],
-                                            kvHeads=g["kvHeads"], cells=g["context"], scale=_f32(1 / math.sqrt(hd))),
-              [g["heads"], (hd + 63) // 64, n])
         b.run("strata_attention_gate_batch", dict(Attention=attn, FullQ=full, Y=gated, dim=hd, heads=g["heads"], tokens=n),
               grid(attn.length))
         return self.mat(p + "attn_output.weight", gated)
+
+    def _attend(self, st, q, k, v, attn) -> None:
+        """Append to the F32 caches and attend over them."""
+        g, b, n, hd, pos = self.g, self.b, self.n, self.g["headDim"], self.dev["positions"]
+        b.run("strata_kv_append_seqs", dict(K=k, V=v, Keys=st["keys"], Values=st["values"], Positions=pos, width=g["kvHeads"] * hd,
+                                            cells=g["context"], tokens=n), grid(n * g["kvHeads"] * hd))
+        b.run("strata_attention_seqs", dict(Q=q, Keys=st["keys"], Values=st["values"], Positions=pos, Y=attn, dim=hd, heads=g["heads"],
+                                            kvHeads=g["kvHeads"], cells=g["context"], scale=_f32(1 / math.sqrt(hd))),
+              [g["heads"], (hd + 63) // 64, n])
 
     # ---- the step
     def _body(self):
@@ -1171,6 +1214,9 @@ class SequenceBatch(PromptBatch):
             self.b.graph_free(self._graph)
             self._graph = None
         self.b.idle()
+        for cache in self.caches[::-1]:  # (the first one's workspace is shared)
+            cache.free()
+        self.caches = []
         for buf in self.persistent:
             self.b.free(buf)
         self.persistent = []

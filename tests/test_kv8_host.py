@@ -98,3 +98,17 @@ def test_reference_quantisation():
     codes, scale = R.quantise(x)
     assert np.abs(codes).max() == 127 and np.abs(codes * np.float64(scale) - x).max() <= 0.5001 * scale
     assert R.quantise(np.zeros((3, 4), np.float32))[1] == 0
+
+
+def test_sequence_batch_refuses_what_an_8_bit_cache_cannot_do():
+    from oracle.backend import OracleBackend
+    from oracle.oracle import Oracle
+    from stratacuda_b200.engine import SequenceBatch, StrataEngine
+    from stratacuda_b200.model import create_fixture
+    engine = StrataEngine.create(create_fixture(), OracleBackend(Oracle("port")))
+    with pytest.raises(ValueError, match="top needs kv8"):
+        SequenceBatch(engine, 2, top=8)
+    with pytest.raises(ValueError, match="at least 3"):
+        SequenceBatch(engine, 2, kv8=True, top=2)
+    with pytest.raises((TypeError, ValueError, RuntimeError)):
+        SequenceBatch(engine, 2, kv8=True, top=1.5)
