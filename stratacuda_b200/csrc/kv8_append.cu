@@ -6,7 +6,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-constexpr int kFew = 4;  // new rows of an open block that are worth trying to add without forming the block again
+constexpr int kFew = 4;  // rows of a run, up to which it is worth trying to add them without forming the block again (FEW)
 
 // One CTA: one kind (keys or values) of one head's block of one run. The block's rows, those that
 // the sequence already holds (from `open`) and the new ones, are read into registers, the largest
@@ -16,7 +16,7 @@ constexpr int kFew = 4;  // new rows of an open block that are worth trying to a
 // new rows' and the marks are written, with the same result. Bound by the latency of the look-ups and of the open rows.
 // Measured at 2 heads of 256 channels: a prompt of 8191 tokens 15.5 us (2.7 TB/s; a CTA a block, kind and head is one
 // wave, so that loads and stores of a CTA do not overlap), 64 sessions' tokens 8.8 us, of which the host takes most.
-template <int P, bool WIDE>
+template <int P, bool WIDE, bool FEW>
 __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const float *k, const float *v, long long stride, const Kv8Runs runs) {
     constexpr int kTiles = P / 64;  // 4 tokens x 4 channels a tile, 16 * P / 4 tiles
     __shared__ __align__(16) int8_t page_s[P * kKvBlock];
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const floa
         }
     };
     // (a run that goes on past this block leaves another's rows in `open`, with which it could not be repeated)
-    if (r0 > 0 && r1 - r0 <= kFew && end - (long long)block * kKvBlock <= kKvBlock) {
+    if (FEW && r0 > 0 && end - (long long)block * kKvBlock <= kKvBlock) {
         // The block's values by channel: the largest magnitude fixes the scale, and the lowest and highest the marks, since
         // rounding keeps order. A page whose scale is that one holds the other rows' codes already.
         constexpr int kAcross = P / 4, kDeep = kThreads / kAcross, kRowsEach = kKvBlock / kDeep;  // a thread: 4 channels, every kDeep-th row
@@ -232,12 +232,17 @@ cudaError_t kv8_append(const Kv8 &c, const float *k, const float *v, long long s
     // 16-byte loads where every row of a head starts on such a boundary
     const uintptr_t starts = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(c.open);
     const bool wide = starts % 16 == 0 && stride % 4 == 0 && c.dim % 4 == 0;
-    auto launch = [&](auto narrow_kernel, auto wide_kernel) {
-        return kv8_launch(wide ? wide_kernel : narrow_kernel, grid, dim3(kThreads), 0, 1, s, c, k, v, stride, r);
+    const bool few = r.count <= kFew;
+    auto launch = [&](auto... kernels) {
+        decltype(&k_kv8_append<64, false, false>) all[] = {kernels...};
+        return kv8_launch(all[2 * few + wide], grid, dim3(kThreads), 0, 1, s, c, k, v, stride, r);
     };
-    if (c.padded == 64) return launch(k_kv8_append<64, false>, k_kv8_append<64, true>);
-    if (c.padded == 128) return launch(k_kv8_append<128, false>, k_kv8_append<128, true>);
-    return launch(k_kv8_append<256, false>, k_kv8_append<256, true>);
+    if (c.padded == 64)
+        return launch(k_kv8_append<64, false, false>, k_kv8_append<64, true, false>, k_kv8_append<64, false, true>, k_kv8_append<64, true, true>);
+    if (c.padded == 128)
+        return launch(k_kv8_append<128, false, false>, k_kv8_append<128, true, false>, k_kv8_append<128, false, true>,
+                      k_kv8_append<128, true, true>);
+    return launch(k_kv8_append<256, false, false>, k_kv8_append<256, true, false>, k_kv8_append<256, false, true>, k_kv8_append<256, true, true>);
 }
 
 }  // namespace strata
