@@ -30,6 +30,17 @@ __device__ __forceinline__ void mma_i8(unsigned tmem_d, unsigned long long a, un
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// Three signed 8-bit digits of four whole numbers |v| <= 2^22, digit e of v[k] in byte k of d[e]: with 128 added at each
+// digit's place the digits are the bytes, less 128 each.
+__device__ __forceinline__ void digits_of(const int (&v)[4], unsigned (&d)[3]) {
+    unsigned w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (unsigned)(v[k] + 0x808080) ^ 0x808080u;
+    const unsigned a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+    d[0] = __byte_perm(a, b, 0x5410);
+    d[1] = __byte_perm(a, b, 0x7632);
+    d[2] = __byte_perm(__byte_perm(w[0], w[1], 0x0062), __byte_perm(w[2], w[3], 0x0062), 0x5410);
+}
 inline PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;

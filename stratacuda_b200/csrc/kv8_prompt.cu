@@ -347,19 +347,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                 const float up = copysignf(__uint_as_float(field << 23), A.scale);
                 // a row with a value that is not finite has no result
                 if (l == 0) M.row_scale[i] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - field) << 23) * fabsf(A.scale);
-                uint2 d[kDigits] = {};
+                unsigned d[2][kDigits];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    int v = __float2int_rn(x[k] * up);
-#pragma unroll
-                    for (int e = 0; e < kDigits; ++e) {
-                        const int digit = e < kDigits - 1 ? ((v + 128) & 255) - 128 : v;
-                        v = (v - digit) >> 8;
-                        (k < 4 ? d[e].x : d[e].y) |= (unsigned)(digit & 255) << (8 * (k & 3));
-                    }
+                for (int k = 0; k < 2; ++k) {
+                    const int v[4] = {__float2int_rn(x[4 * k] * up), __float2int_rn(x[4 * k + 1] * up), __float2int_rn(x[4 * k + 2] * up),
+                                      __float2int_rn(x[4 * k + 3] * up)};
+                    digits_of(v, d[k]);
                 }
 #pragma unroll
-                for (int e = 0; e < kDigits; ++e) *reinterpret_cast<uint2 *>(M.q[e][l >> 3] + sw64_byte(i, 8 * (l & 7))) = d[e];
+                for (int e = 0; e < kDigits; ++e)
+                    *reinterpret_cast<uint2 *>(M.q[e][l >> 3] + sw64_byte(i, 8 * (l & 7))) = make_uint2(d[0][e], d[1][e]);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
