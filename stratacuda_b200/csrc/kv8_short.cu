@@ -1,4 +1,4 @@
-// Attention over the 8-bit paged cache, token by token, where the CTAs have few pages each.
+// Attention over the 8-bit paged cache, token by token, where units have few pages on a CTA or little to read a query row.
 //
 // The same sums as the form on tcgen05, on 16-row tiles of mma.sync (m16n8k16), whose products answer at once: no tensor
 // maps, no TMEM, no digits to prepare, two CTAs a multiprocessor. A unit is one token and key/value head with up to 16
@@ -407,15 +407,26 @@ cudaError_t launch(Args A, int multiprocessors, cudaStream_t s) {
 
 }  // namespace
 
-// Up to this many pages a multiprocessor, counting every block of the table where there are no picks (lengths are known
-// on the device alone). Microseconds of this form and the other, cold, for picks of 32 blocks over 2 heads of 256 channels:
-// 1.7 pages 23.6 and 29.6, 6.9 pages 31.8 and 42.0, 10.4 pages 42.1 and 44.0, 13.8 pages 48.1 and 48.2, 27.7 pages 66.6 and
-// 58.4; one session over 8 heads of 128 channels: 6.9 pages 23.6 and 27.7, 13.8 pages 33.8 and 29.7.
+// Chosen for up to kShortPages pages a multiprocessor, and for up to kShortPart pages a part, a unit's pages on one CTA. All
+// counts take every block of the table where there are no picks (lengths are known on the device alone).
+// A multiprocessor's time in microseconds, fitted to 1000 tokens over 2 heads with 8 and 32 picked blocks: this form takes
+// 3 a part and 0.58, 0.74, 1.29 a page at 64, 128, 256 channels whatever the group. The other takes by the group's rows
+//            64 channels           128 channels          256 channels
+//   4 rows   3.9 and 0.32 a page   4.1 and 0.33          4.8 and 0.42
+//   8        5.5 and 0.41          5.8 and 0.39         10.5 and 0.45
+//   12       9.2 and 0.48         12.0 and 0.41         16.0 and 0.55
+//   16      13.4 and 0.61         14.8 and 0.65         19.2 and 0.81
+// so that both are even at kShortPart pages. Where calls are small the other form's fixed costs (its operands' set-up) decide: one
+// session over 8 heads of 128 channels takes 23.6 and 27.7 us at 6.9 pages a multiprocessor, 33.8 and 29.7 at 13.8.
 constexpr long long kShortPages = 10;
+constexpr long long kShortPart[3][4] = {{4, 16, 64, 1LL << 40}, {3, 8, 27, 127}, {2, 8, 17, 33}};
 
 bool kv8_short_fits(const Args &A, int multiprocessors) {
     const long long tokens = (long long)A.runs.segments * A.runs.count, units = tokens * A.c.kv_heads * A.tiles;
-    return tokens <= kMaxTokens && units <= 65536 && units * (A.picks ? A.top : A.c.blocks) <= kShortPages * multiprocessors;
+    if (tokens > kMaxTokens || units > 65536) return false;
+    const long long pages = units * (A.picks ? A.top : A.c.blocks);
+    const int rows = A.group < kRows ? (A.group + 3) / 4 - 1 : 3;
+    return pages <= kShortPages * multiprocessors || pages <= kShortPart[A.c.padded == 64 ? 0 : A.c.padded == 128 ? 1 : 2][rows] * (units + multiprocessors);
 }
 
 cudaError_t kv8_attend_short(Args A, int multiprocessors, cudaStream_t s) {

@@ -714,3 +714,24 @@ def test_attend_prompts_of_many_sequences(dim, segments, count, blocks):
     for s in range(0, segments, 13):
         c.check_attend(got[s], q[s], ks[s], vs[s], start[s], 1 / math.sqrt(dim))
     assert c.errors() == 0
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 1, 128), (16, 1, 256), (33, 1, 100), (3, 1, 200)])
+@pytest.mark.parametrize("slope", [0.5, 5.0, 12.0, -6.0])
+def test_attend_groups_of_many_heads_in_wide_tables(heads, kv, dim, slope):
+    """Tables with room for long sessions, as many of whose blocks as a session has are read: 16 rows a unit, and units of
+    16 and of fewer rows side by side (33 heads)."""
+    sequences, n, used = 70, 64 * 20 + 3, 21
+    c = WideCache(kv, dim, sequences, 500, used + 2)
+    rng = np.random.default_rng(10)
+    direction = rng.normal(0, 1, dim)
+    k, v = _rising(rng, n, kv, dim, direction, slope)
+    c.table[:, :used] = c.i32(np.arange(used))
+    c.append(k[None], v[None], [0], [0])
+    q = (direction + rng.normal(0, 0.05, (sequences, 1, heads, dim))).astype(np.float32)
+    start = n - 1 - 3 * np.arange(sequences)
+    start[5] = 0
+    got = c.attend(q, heads, np.arange(sequences), start)
+    for s in (0, 5, 6, 41, 69):
+        c.check_attend(got[s], q[s], k, v, start[s], 1 / math.sqrt(dim))
+    assert c.errors() == 0
