@@ -44,11 +44,16 @@ constexpr int kConvThreads = 32 * kConvWarps;
 constexpr int kTileRows = 128;
 constexpr int kDigits = 3;           // of a query
 constexpr float kLiftP = 10.0f;      // weights are stored times 2^10
+constexpr float kRoomP = 4.0f;       // log2 of a new reference over its maximum: weights begin at 2^6, far above FP16's subnormals
 constexpr float kGrow = 5.0f;        // growth of a maximum (log2) that O's scale bears
 constexpr long long kLimit = 2000000000;  // clocks, about a second
 
 constexpr int kFlush = 16;           // pages that add up in TMEM before the sum moves to 32-bit adds
 constexpr int kScales = 8;           // pages whose scales are kept: more than are fetched ahead of the softmax
+// A unit counts as this many pages more when pages are shared: beginning one takes longer than a page. (Without it
+// the CTAs of a prompt's first tiles, which have a page or two each, came last: 1497 tokens from the start, 36 heads over 3
+// of 64 channels, took 221 us instead of 84; 98 with 3.)
+constexpr int kBegin = 6;
 constexpr int kMaxGrid = 160;        // CTAs, each with a slot in the workspace
 constexpr int kMaxPairs = 1024;      // (run, tile) pairs of a split call
 constexpr int kMaxUnits = 65536;
@@ -177,8 +182,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
         long long *before = reinterpret_cast<long long *>(M.v[0]);  // used before the ring is
         long long *part = before + kMaxPairs + 1;
         static_assert(sizeof(M.v) >= (kMaxPairs + 1 + kPromptThreads / 32) * 8, "the page counts fit");
-        for (int base = 0; base < pairs; base += kPromptThreads) {  // before[i]: a head's pages before pair i
+        for (int base = 0; base < pairs; base += kPromptThreads) {  // before[i]: a head's pages, and kBegin a unit, before pair i
             long long sum = base + tid < pairs ? pair_pages(A, (base + tid) / A.tiles, (base + tid) % A.tiles) : 0;
+            if (sum) sum += kBegin;
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1) {
                 const long long o = __shfl_up_sync(0xffffffffu, sum, s);
@@ -268,9 +274,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                 ++w.pair;
                 continue;
             }
-            p.first = w.page;
-            p.stop = (int)min((long long)p.n, w.page + (w.work_end - w.work));
-            if (w.page == 0) W.cover[w.pair * A.c.kv_heads + w.head] = make_int2(blockIdx.x, (int)((w.work + p.n - 1) / w.chunk));
+            if (w.page < kBegin) {  // the CTA that has the first page begins the unit
+                w.work += kBegin - w.page;
+                w.page = kBegin;
+                continue;
+            }
+            p.first = w.page - kBegin;
+            p.stop = (int)min((long long)p.n, p.first + (w.work_end - w.work));
+            if (p.first == 0) W.cover[w.pair * A.c.kv_heads + w.head] = make_int2(blockIdx.x, (int)((w.work + p.n - 1) / w.chunk));
             w.work += p.stop - p.first;
             w.page = 0;
             if (++w.head == A.c.kv_heads) {
@@ -459,7 +470,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                         if (!(ok = flush(j - 1))) continue;
                         due = false;
                     }
-                    const float now = fmaxf(m, top), alpha = now > m ? exp2_fast(m - now) : 1.0f;
+                    const float now = top > m ? top + kRoomP : m, alpha = now > m ? exp2_fast(m - now) : 1.0f;
                     m = now;
                     sum *= alpha;
                     if (j % kFlush) {
