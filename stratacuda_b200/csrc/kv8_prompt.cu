@@ -21,8 +21,8 @@
 // A value scale cannot be applied after the product, since pages add up in one accumulator: weights are
 // multiplied by scale / (largest scale of the tile's pages), in their exponents.
 //
-// Measured: 2048 tokens over 16384 keys, 24 heads over 2 of 256 channels, 1395 us, 555 TFLOP/s of the two products as they
-// are defined (1307 us with the cache in L2), at a page about every 4200 clocks a CTA. S takes 1250 of them (24 instructions of 128 x 64 x 32, bound by
+// Measured: 2048 tokens over 16384 keys, 24 heads over 2 of 256 channels, 1365 us, 567 TFLOP/s of the two products as they
+// are defined (1287 us with the cache in L2), at a page about every 4200 clocks a CTA. S takes 1250 of them (24 instructions of 128 x 64 x 32, bound by
 // reading their operands from shared memory) and O 1000; the rest are the hand-overs between products and softmax, for
 // which TMEM has no second set of S's columns. The form with queries in FP16 halves and keys converted as well took
 // 1546 us, since its converters and operands take twice the shared-memory traffic.
