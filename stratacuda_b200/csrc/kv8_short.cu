@@ -191,9 +191,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_short(const __grid_constant
         float m = -INFINITY, sum = 0.0f;  // of row 2 warp + lane / 16; the sum over this lane's four tokens of each page
         const int srow = warp * 2 + (lane >> 4), stok = (lane & 15) * 4;
         float o[Z::o_tiles][4] = {};
-        for (int base = entry; base < stop && ok; base += kList) {
-            // look up to 256 pages up, those that are there in order
-            __syncthreads();
+        for (int base = entry; base < stop; base += kList) {
+            // look up to 256 pages up, those that are there in order. (A thread's last wait may have failed where others' did
+            // not, and all must meet at the same barriers: so they leave together)
+            if (!(ok = __syncthreads_and(ok))) break;
             int page = -1, block = -1;
             if (base + tid < stop) {
                 block = A.picks ? A.picks[((size_t)token * A.c.kv_heads + head) * A.top + base + tid] : base + tid;

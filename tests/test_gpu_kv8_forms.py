@@ -92,3 +92,27 @@ def test_select_prompt_from_the_first_token_on():
         for t in list(range(0, 450, 7)) + list(range(450, count, 211)):
             _check_picks(got[0, t], q[0, t], lo, hi, scales, order[0], heads, (start + t + 64) // BLOCK, top, 1, 2)
     assert c.errors() == 0
+
+
+# ---------------------------------------------------------------- attend
+
+@pytest.mark.parametrize("holes", [False, True])
+def test_short_form_over_more_pages_than_it_looks_up_at_a_time(holes):
+    """16 heads of 64 channels on mma.sync tiles with more than 256 pages of a unit on one CTA, also with gaps among them."""
+    heads, kv, dim, blocks, sequences = 16, 1, 64, 600, 160
+    c = WideCache(kv, dim, sequences, blocks, blocks)
+    rng = np.random.default_rng(3)
+    n = blocks * BLOCK - 5
+    k, v = rng.normal(0, 1, (2, n, kv, dim)).astype(np.float32)
+    c.table[:] = c.i32(rng.permutation(blocks))
+    c.append(k[None], v[None], [0], [0])
+    q = rng.normal(0, 1, (sequences, 1, heads, dim)).astype(np.float32)
+    start = n - 1 - np.arange(sequences)
+    picks = None
+    if holes:
+        picks = np.arange(blocks)[None, None].repeat(sequences, 0)
+        picks[rng.random(picks.shape) < 0.3] = -1
+    got = c.attend(q, heads, np.arange(sequences), start, picks=picks, top=blocks if holes else 0)
+    for s in (0, 1, 80, 159):
+        c.check_attend(got[s], q[s], k, v, start[s], 1 / math.sqrt(dim), None if picks is None else picks[s:s + 1])
+    assert c.errors() == 0
