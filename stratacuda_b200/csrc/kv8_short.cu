@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_short(const __grid_constant
         for (int base = entry; base < stop; base += kList) {
             // look up to 256 pages up, those that are there in order. (A thread's last wait may have failed where others' did
             // not, and all must meet at the same barriers: so they leave together)
-            if (!(ok = __syncthreads_and(ok))) break;
+            if (!__syncthreads_and(ok)) break;
             int page = -1, block = -1;
             if (base + tid < stop) {
                 block = A.picks ? A.picks[((size_t)token * A.c.kv_heads + head) * A.top + base + tid] : base + tid;
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_short(const __grid_constant
                     *reinterpret_cast<float2 *>(&M.s[panel][g + 8][tok]) = make_float2(acc[j][2], acc[j][3]);
                 }
                 // every warp has read this page's keys and the last page's values
-                if (!(ok = __syncthreads_and(ok))) break;
+                if (!__syncthreads_and(ok)) break;
                 if (tid == 0) {
                     if (i + Z::stages < count) get(i + Z::stages, 0);
                     if (i > 0 && i - 1 + Z::stages < count) get(i - 1 + Z::stages, 1);
@@ -319,8 +319,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv8_short(const __grid_constant
             }
             if (ok) fetched = first + count;
         }
-        ok = __syncthreads_and(ok);
-        if (!ok) {  // a copy did not land in time: report, let what is in flight land, leave
+        if (!__syncthreads_and(ok)) {  // a copy did not land in time: report, let what is in flight land, leave
             if (tid == 0) {
                 raise_error(A.c.err, kErrWaitTimeout);
                 for (unsigned i = 0; i < Z::stages; ++i) {  // the last copy of each stage
