@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(Shape<WIDE>::threads, WIDE ? 2 : 1) k_kv8_sele
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     // bounds go to the first CTA's shared memory, which is there once that CTA has begun: every CTA says so here, and
     // waits for the others before its first store, with the queries' rounding between
-    if (ranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int unit = blockIdx.x / ranks, head = unit % A.c.kv_heads, tile = unit / A.c.kv_heads % A.tiles, run = unit / A.c.kv_heads / A.tiles;
     const RunAt at = run_at(A.c, A.runs, run);
