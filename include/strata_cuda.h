@@ -311,7 +311,7 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
  *   STRATA_KV8_SELECT_BLOCKS blocks.
  * attend: y [tokens][heads * dim] = softmax(scale * q . k) v over the keys at or before the token's position, of
  *   every block (picks null / 0) or of the blocks that picks [tokens][kv_heads][top] lists (distinct, -1 for
- *   none). Query head h uses key/value head h / (heads / kv_heads). A token that sees no key gets zeros.
+ *   none; top at most 33554431, the blocks that a table can have). Query head h uses key/value head h / (heads / kv_heads). A token that sees no key gets zeros.
  *   F32 in and out. Queries and weights keep 22 bits or more of their row's largest (8-bit digits or two FP16
  *   halves, by the kernel's form) and meet the codes without rounding these; maxima, sums and results are F32 or wider.
  *   Prompt chunks sum weights times (a page's value scale / the largest of the pages in a tile's sight): values smaller

@@ -46,6 +46,10 @@ int kv8_check_select(int blocks, int top, int first, int last, char *msg, size_t
         return say(msg, cap, STRATA_ERR_RANGE, "first and last must be integers >= 0 with first + last <= top");
     return STRATA_OK;
 }
+int kv8_check_picks(int top, char *msg, size_t cap) {
+    // as many blocks as a table can have: lists are walked with 32-bit indices
+    return top < 1 || top > 0x7fffffff / kKvBlock ? say(msg, cap, STRATA_ERR_RANGE, "top must be an integer in [1, 33554431]") : STRATA_OK;
+}
 int kv8_check_stride(long long stride, long long width, char *msg, size_t cap) {
     if (stride < width || stride > (1LL << 40)) return say(msg, cap, STRATA_ERR_LAYOUT, "row_stride is smaller than a row");
     return STRATA_OK;
@@ -124,7 +128,8 @@ extern "C" int strata_kv8_attend_dev(const strata_kv8_cache_dev *cache, const fl
     if (int e = rows(q, &row_stride, (long long)heads * c.dim, msg, msg_cap)) return e;
     if (!y) return say(msg, msg_cap, STRATA_ERR_RANGE, "null device pointer");
     if (!aligned(y, 4) || !aligned(picks, 4)) return say(msg, msg_cap, STRATA_ERR_LAYOUT, "picks and y must start on 4-byte boundaries");
-    if (picks && top < 1) return say(msg, msg_cap, STRATA_ERR_RANGE, "top must be an integer >= 1");
+    if (picks)
+        if (int e = kv8_check_picks(top, msg, msg_cap)) return e;
     if (!std::isfinite(scale)) return say(msg, msg_cap, STRATA_ERR_RANGE, "scale must be finite");
     return done(kv8_attend(c, q, (long long)row_stride, heads, r, picks, top, scale, y, static_cast<cudaStream_t>(stream)), msg, msg_cap);
 }
