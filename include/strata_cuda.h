@@ -317,7 +317,8 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
  *   Prompt chunks sum weights times (a page's value scale / the largest of the pages in a tile's sight): values smaller
  *   than that largest by 2^24 and more lose bits there. A query value that is not finite makes its own row NaN.
  *
- * heads / kv_heads is any whole number, dim is 1 .. 256. A sequence, page or position outside the cache
+ * heads / kv_heads is any whole number, dim is 1 .. 256. A run that attends to every block has at most 2^31 - 128 rows
+ * (count * heads / kv_heads). A sequence, page or position outside the cache
  * is skipped and reported by the next synchronising call (STRATA_ERR_DEVICE), or, in the pointer forms, by
  * bit 0 of *status (bit 4: a value that was not finite), which the caller clears. */
 #define STRATA_KV8_BLOCK 64

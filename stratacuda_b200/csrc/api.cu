@@ -753,8 +753,7 @@ int strata_kv8_attend(strata_ctx *ctx, const strata_kv8_cache *cache, strata_buf
     if (int e = kv8_view(ctx, cache, segments, count, sequence, start, &c, &r)) return e;
     char msg[256];
     if (int e = kv8_check_heads(heads, c.kv_heads, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
-    if (picks)
-        if (int e = kv8_check_picks(top, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = picks ? kv8_check_picks(top, msg, sizeof msg) : kv8_check_rows(count, heads, c.kv_heads, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
     if (!std::isfinite(scale)) return fail(ctx, STRATA_ERR_RANGE, "scale must be finite");
     void *pq = nullptr, *pp = nullptr, *py = nullptr;
     const long long tokens = (long long)segments * count, width = (long long)heads * c.dim;

@@ -37,6 +37,7 @@ int kv8_check_cache(int kv_heads, int dim, int pages, int sequences, int blocks,
 int kv8_check_runs(int segments, int count, char *msg, size_t cap);
 int kv8_check_heads(int heads, int kv_heads, char *msg, size_t cap);
 int kv8_check_select(int blocks, int top, int first, int last, char *msg, size_t cap);
+int kv8_check_rows(int count, int heads, int kv_heads, char *msg, size_t cap);
 int kv8_check_picks(int top, char *msg, size_t cap);
 int kv8_check_stride(long long stride, long long width, char *msg, size_t cap);
 int kv8_check_alignment(const Kv8 &c, char *msg, size_t cap);

@@ -46,6 +46,12 @@ int kv8_check_select(int blocks, int top, int first, int last, char *msg, size_t
         return say(msg, cap, STRATA_ERR_RANGE, "first and last must be integers >= 0 with first + last <= top");
     return STRATA_OK;
 }
+int kv8_check_rows(int count, int heads, int kv_heads, char *msg, size_t cap) {
+    // a prompt's rows, whole tiles of 128, are counted in 32 bits
+    return (long long)count * (heads / kv_heads) > 0x80000000LL - 128
+               ? say(msg, cap, STRATA_ERR_RANGE, "count * heads / kv_heads must be at most 2^31 - 128 rows where every block is attended to")
+               : STRATA_OK;
+}
 int kv8_check_picks(int top, char *msg, size_t cap) {
     // as many blocks as a table can have: lists are walked with 32-bit indices
     return top < 1 || top > 0x7fffffff / kKvBlock ? say(msg, cap, STRATA_ERR_RANGE, "top must be an integer in [1, 33554431]") : STRATA_OK;
@@ -128,8 +134,7 @@ extern "C" int strata_kv8_attend_dev(const strata_kv8_cache_dev *cache, const fl
     if (int e = rows(q, &row_stride, (long long)heads * c.dim, msg, msg_cap)) return e;
     if (!y) return say(msg, msg_cap, STRATA_ERR_RANGE, "null device pointer");
     if (!aligned(y, 4) || !aligned(picks, 4)) return say(msg, msg_cap, STRATA_ERR_LAYOUT, "picks and y must start on 4-byte boundaries");
-    if (picks)
-        if (int e = kv8_check_picks(top, msg, msg_cap)) return e;
+    if (int e = picks ? kv8_check_picks(top, msg, msg_cap) : kv8_check_rows(count, heads, c.kv_heads, msg, msg_cap)) return e;
     if (!std::isfinite(scale)) return say(msg, msg_cap, STRATA_ERR_RANGE, "scale must be finite");
     return done(kv8_attend(c, q, (long long)row_stride, heads, r, picks, top, scale, y, static_cast<cudaStream_t>(stream)), msg, msg_cap);
 }
