@@ -452,7 +452,7 @@ int kv8_view(strata_ctx *ctx, const strata_kv8_cache *cache, int segments, int c
 int kv8_rows(strata_ctx *ctx, const char *what, strata_buf h, uint64_t *stride, long long tokens, long long width, void **out) {
     if (!*stride) *stride = (uint64_t)width;
     char msg[256];
-    if (*stride > (1ull << 40)) return fail(ctx, STRATA_ERR_LAYOUT, "row_stride is out of range");  // tokens < 2^25: no overflow below
+    if (*stride > (1ull << 38)) return fail(ctx, STRATA_ERR_LAYOUT, "row_stride is out of range");  // at most 2^24 tokens: below 2^63
     if (int e = kv8_check_stride((long long)*stride, width, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
     return kv8_buffer(ctx, what, h, (tokens - 1) * (long long)*stride + width, out);
 }
