@@ -12,8 +12,10 @@
 //   * few tokens: a cluster of up to 8 CTAs shares a token's blocks and sends the bounds to its first CTA.
 // Measured at 24 heads over 2 of 256 channels: 32 of 1024 blocks for 2048 tokens 47 us (90 T operations/s), bound by the search
 // among a token's bounds and by loading marks in fragment order; for 16 sessions 13 us, bound by latency.
+#include "../../include/strata_cuda.h"
 #include "kv8.cuh"
 
+#include <atomic>
 #include <cooperative_groups.h>
 
 namespace strata {
@@ -371,9 +373,25 @@ __global__ void __launch_bounds__(Shape<WIDE>::threads, WIDE ? 2 : 1) k_kv8_sele
     }
 }
 
+constexpr int kKeyBytes = 184 * 1024;  // of a tile's bounds, beside the codes and candidates
+constexpr int kWideBytes = STRATA_KV8_SELECT_BLOCKS * 4;  // of a token's
+
+// The limit on a kernel's shared memory is the function's, whichever thread's call it serves: the largest, once a device.
+template <int P, bool WIDE>
+cudaError_t allow_shared_memory() {
+    constexpr int kDevices = 64;
+    static std::atomic<bool> done[kDevices];
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < kDevices && done[device].load(std::memory_order_relaxed))) return e;
+    e = cudaFuncSetAttribute(k_kv8_select<P, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, WIDE ? kWideBytes : kKeyBytes);
+    if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
+    return e;
+}
+
 template <int P, bool WIDE>
 cudaError_t launch(const Args &A, int ranks, size_t smem, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(k_kv8_select<P, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_shared_memory<P, WIDE>();
     if (e != cudaSuccess) return e;
     const long long ctas = (long long)A.runs.segments * A.tiles * A.c.kv_heads * ranks;
     if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
@@ -384,7 +402,7 @@ cudaError_t launch(const Args &A, int ranks, size_t smem, cudaStream_t s) {
 
 cudaError_t kv8_select(const Kv8 &c, const float *q, long long stride, int heads, const Kv8Runs &r, int top, int first, int last, int *picks,
                        cudaStream_t s) {
-    constexpr int kSms = 148, kKeyBytes = 184 * 1024;  // of a CTA's bounds, beside the codes and candidates
+    constexpr int kSms = 148;
     Args A{c, q, stride, heads, heads / c.kv_heads, r, top, first, last, picks, 1, r.count, (c.blocks + 3) / 4 * 4};
     const long long tokens = (long long)r.segments * r.count * c.kv_heads;
     // Tiles of up to 32 tokens where half of the multiprocessors get one: marks are then read once for 16 or 32 tokens

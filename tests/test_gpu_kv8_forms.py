@@ -116,3 +116,65 @@ def test_short_form_over_more_pages_than_it_looks_up_at_a_time(holes):
     for s in (0, 1, 80, 159):
         c.check_attend(got[s], q[s], k, v, start[s], 1 / math.sqrt(dim), None if picks is None else picks[s:s + 1])
     assert c.errors() == 0
+
+
+# ---------------------------------------------------------------- calls from several threads
+
+# One thread a call, each its own `times` times; returns the calls that were refused. (Python's threads overlap too seldom.)
+_THREADS = """
+#include <atomic>
+#include <cstdint>
+#include <thread>
+#include <vector>
+struct Call { const void *cache; const float *q; const int32_t *sequence, *start; int32_t *picks; void *stream; int32_t heads, top; };
+using Select = int (*)(const void *, const float *, uint64_t, int32_t, int32_t, int32_t, const int32_t *, const int32_t *, int32_t, int32_t, int32_t,
+                       int32_t *, void *, char *, size_t);
+extern "C" long hammer(Select select, const Call *calls, int n, long times) {
+    std::atomic<long> refused{0};
+    std::vector<std::thread> threads;
+    for (int i = 0; i < n; ++i)
+        threads.emplace_back([&, i] {
+            const Call c = calls[i];
+            for (long k = 0; k < times; ++k)
+                refused += select(c.cache, c.q, 0, c.heads, 1, 1, c.sequence, c.start, c.top, 1, 2, c.picks, c.stream, nullptr, 0) != 0;
+        });
+    for (auto &t : threads) t.join();
+    return refused;
+}
+"""
+
+
+def test_select_from_several_threads_over_tables_of_different_widths(tmp_path):
+    """A selection's shared memory goes by the table's width; what one thread's call needs must not depend on another's."""
+    import ctypes as C
+    import shutil
+    import subprocess
+
+    from stratacuda_b200 import _lib as L
+
+    if not shutil.which("g++"):
+        pytest.skip("no C++ compiler for the calling threads")
+    (tmp_path / "hammer.cc").write_text(_THREADS)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-pthread", str(tmp_path / "hammer.cc"), "-o", str(tmp_path / "hammer.so")],
+                   check=True)
+
+    class Call(C.Structure):
+        _fields_ = [(n, C.c_void_p) for n in ("cache", "q", "sequence", "start", "picks", "stream")] + [("heads", C.c_int32), ("top", C.c_int32)]
+
+    widths, keep, calls = (32768, 40, 32768, 100), [], []
+    for blocks in widths:
+        c, lo, hi, scales, order, rng = _marked(1, 16, 1, blocks, 1)
+        torch = c.torch
+        q = rng.normal(0, 1, (2, 16)).astype(np.float32)
+        dq, seq, start = torch.from_numpy(q.reshape(1, -1)).cuda(), c.i32([0]), c.i32([blocks * BLOCK - 1])
+        picks, stream = torch.full((1, 1, 8), -9, dtype=torch.int32, device="cuda"), torch.cuda.Stream()
+        keep.append((c, lo, hi, scales, order, q, dq, seq, start, picks, stream))
+        calls.append(Call(C.addressof(c.view._cache), dq.data_ptr(), seq.data_ptr(), start.data_ptr(), picks.data_ptr(), stream.cuda_stream, 2, 8))
+    torch.cuda.synchronize()
+    hammer = C.CDLL(str(tmp_path / "hammer.so")).hammer
+    hammer.restype, hammer.argtypes = C.c_long, [C.c_void_p, C.POINTER(Call), C.c_int, C.c_long]
+    refused = hammer(C.cast(L.load().strata_kv8_select_dev, C.c_void_p), (Call * len(calls))(*calls), len(calls), 20000)
+    torch.cuda.synchronize()
+    assert refused == 0
+    for blocks, (c, lo, hi, scales, order, q, dq, seq, start, picks, stream) in zip(widths, keep):
+        _check_picks(picks.cpu().numpy()[0], q, lo, hi, scales, order[0], 2, blocks, 8, 1, 2)
