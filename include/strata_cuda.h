@@ -314,8 +314,8 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
  *   none; top at most 33554431, the blocks that a table can have). Query head h uses key/value head h / (heads / kv_heads). A token that sees no key gets zeros.
  *   F32 in and out. Queries and weights keep 22 bits or more of their row's largest (8-bit digits or two FP16
  *   halves, by the kernel's form) and meet the codes without rounding these; maxima, sums and results are F32 or wider.
- *   Prompt chunks sum weights times (a page's value scale / the largest of the pages in a tile's sight): values smaller
- *   than that largest by 2^24 and more lose bits there. A query value that is not finite makes its own row NaN.
+ *   Prompt chunks keep weights times their page's value scale to 2^-31 of the row's largest such product; values of a page
+ *   whose scale is below 2^-90 of the largest in sight of the 128 rows of a tile count as zeros there. A query value that is not finite makes its own row NaN.
  *
  * heads / kv_heads is any whole number, dim is 1 .. 256. A run that attends to every block has at most 2^31 - 128 rows
  * (count * heads / kv_heads). A sequence, page or position outside the cache

@@ -19,7 +19,8 @@
 //   11   one thread issues the MMAs: S of page j + 1 before O of page j, so that S's columns are read and free
 //        again while O is computed
 // A value scale cannot be applied after the product, since pages add up in one accumulator: weights are
-// multiplied by scale / (largest scale of the tile's pages), in their exponents.
+// multiplied by scale / (largest scale of the tile's pages), in their exponents, and a row's running reference is that of
+// the products. So FP16's steps are 2^-31 of the row's largest product at most, also for rows that see only small scales.
 //
 // Measured: 2048 tokens over 16384 keys, 24 heads over 2 of 256 channels, 1365 us, 567 TFLOP/s of the two products as they
 // are defined (1287 us with the cache in L2), at a page about every 4200 clocks a CTA. S takes 1250 of them (24 instructions of 128 x 64 x 32, bound by
@@ -449,9 +450,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                 }
                 // a positive factor, so that -infinity stays that; what would be below this makes logits of 0
                 const float c = isnan(row_scale) ? row_scale : fmaxf(sc.x * row_scale, 1e-30f);
-                // weights take the page's value scale in the exponent. One of 0 has values of 0, and one below 2^-60 of the
-                // largest counts as that, which FP16 weights would not hold either
-                const float fv = fmaxf(sc.y * over, 0x1p-60f);
+                // weights take the page's value scale over the tile's largest in the exponent, and a row's reference is that of
+                // its largest weight so taken: its weights begin at 2^6 whatever scales other rows' pages have. Values of
+                // a scale below 2^-90 of the largest, none among them, count as none
+                const float by_v = sc.y * over, fv = fmaxf(by_v, 0x1p-90f), lift = log2f(fv);
                 if (__any_sync(0xffffffffu, left < 32)) {
 #pragma unroll
                     for (int k = 0; k < 32; ++k) a[k] = k < left ? a[k] : -INFINITY;
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
 #pragma unroll
                 for (int k = 4; k < 32; ++k) big[k & 3] = fmaxf(big[k & 3], a[k]);
                 float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-                top *= c;
+                top = top * c + lift;
                 bool due = j > 0 && j % kFlush == 0;  // the group of pages before this one is to be kept
                 if (vote(!ok || top > m + kGrow)) {  // seldom
                     M.half_row[j & 1][half][i] = top;
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                         }
                     }
                 }
-                const float from = kLiftP - (m == -INFINITY ? 0.0f : m) + log2f(fv);
+                const float from = kLiftP - ((m == -INFINITY ? 0.0f : m) - lift);
                 float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 unsigned hi[16], lo[16];
 #pragma unroll
@@ -496,6 +498,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv8_prompt(const __grid_c
                     add[(2 * e) & 3] += p0;
                     add[(2 * e + 1) & 3] += p1;
                     split_pair(p0, p1, hi[e], lo[e]);
+                }
+                if (by_v < 0x1p-90f) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) hi[e] = lo[e] = 0;
                 }
                 if (g > 0 && !(ok = __all_sync(0xffffffffu, wait(&M.o_done, (g - 1) & 1)))) continue;  // the weights before are used
                 tc_fence_after();

@@ -178,3 +178,49 @@ def test_select_from_several_threads_over_tables_of_different_widths(tmp_path):
     assert refused == 0
     for blocks, (c, lo, hi, scales, order, q, dq, seq, start, picks, stream) in zip(widths, keep):
         _check_picks(picks.cpu().numpy()[0], q, lo, hi, scales, order[0], 2, blocks, 8, 1, 2)
+
+
+# ---------------------------------------------------------------- value scales far apart
+
+@pytest.mark.parametrize("heads,kv,dim,start,count", [(1, 1, 64, 0, 200), (5, 1, 128, 0, 150), (6, 2, 256, 0, 140), (3, 1, 40, 64 * 9 + 30, 300)])
+@pytest.mark.parametrize("growth", [12, 20, 33, 60])
+def test_prompt_rows_do_not_lose_bits_to_values_they_cannot_see(heads, kv, dim, start, count, growth):
+    """Each block's values are 2^growth times those of the block before (from the chunk's on, at most 2^60 in all): every row
+    is within the bound that the largest value in its own sight gives."""
+    c = WideCache(kv, dim, 1, 20, 20)
+    rng = np.random.default_rng(growth)
+    n = start + count
+    k, v = rng.normal(0, 1, (2, n, kv, dim))
+    v *= 2.0 ** np.minimum(growth * np.maximum(np.arange(n) // BLOCK - start // BLOCK, 0), 60)[:, None, None] * 1e-9
+    k, v = k.astype(np.float32), v.astype(np.float32)
+    c.table[0] = c.i32(rng.permutation(20))
+    c.append(k[None], v[None], [0], [0])
+    q = rng.normal(0, 1, (1, count, heads, dim)).astype(np.float32)
+    got = c.attend(q, heads, [0], [start])
+    c.check_attend(got[0], q[0], k, v, start, 1 / math.sqrt(dim))
+    assert c.errors() == 0
+
+
+@pytest.mark.parametrize("count", [1, 70])
+@pytest.mark.parametrize("heads,kv,dim,blocks", [(4, 1, 64, 12), (6, 2, 128, 40), (12, 1, 256, 300)])
+@pytest.mark.parametrize("small", [9, 16, 24, 40])
+def test_results_from_blocks_of_small_values(heads, kv, dim, blocks, small, count):
+    """Rows whose weight lies on blocks with values 2^-small of the other blocks', which have weights below 2^-100: the result is
+    as exact against the small values as it would be without the others."""
+    c = WideCache(kv, dim, 1, blocks, blocks)
+    rng = np.random.default_rng(small)
+    n = blocks * BLOCK - 3
+    heavy = np.arange(n) // BLOCK % 3 == 1  # these have the weight
+    direction = rng.normal(0, 1, dim)
+    k = rng.normal(0, 0.1, (n, kv, dim)) - 100 * math.sqrt(dim) * np.where(heavy, 0, 1)[:, None, None] * direction / np.sum(direction ** 2)
+    v = rng.normal(0, 1, (n, kv, dim)) * np.where(heavy, 2.0 ** -small, 1.0)[:, None, None]
+    k, v = k.astype(np.float32), v.astype(np.float32)
+    c.table[0] = c.i32(rng.permutation(blocks))
+    c.append(k[None], v[None], [0], [0])
+    q = (direction + rng.normal(0, 0.01, (1, count, heads, dim))).astype(np.float32)
+    start = n - count
+    got = c.attend(q, heads, [0], [start])
+    heavy_blocks = np.arange(1, blocks, 3)
+    picks = np.broadcast_to(heavy_blocks, (count, kv, len(heavy_blocks)))
+    c.check_attend(got[0], q[0], k, v, start, 1 / math.sqrt(dim), picks)  # (the others' share is below 2^-100)
+    assert c.errors() == 0
