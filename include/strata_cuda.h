@@ -37,7 +37,7 @@ extern "C" {
 #define STRATA_ERR_HANDLE 4  /* not a live buffer of this context: src/backend.js:138-143 */
 #define STRATA_ERR_ALLOC 5   /* device allocation failed: wasm/runtime.js:7 "WASM allocation failed" */
 #define STRATA_ERR_CUDA 6    /* CUDA runtime error (the message names it) */
-#define STRATA_ERR_DEVICE 7  /* a kernel recorded an out-of-range index, an invalid routing, a timed-out wait, a non-finite PLE scale or cache value */
+#define STRATA_ERR_DEVICE 7  /* a kernel recorded an out-of-range index, an invalid routing, a timed-out wait, a non-finite PLE scale or cache value, cache scales too far apart */
 
 #define STRATA_F32 0
 #define STRATA_I32 1
@@ -315,12 +315,14 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
  *   F32 in and out. Queries and weights keep 22 bits or more of their row's largest (8-bit digits or two FP16
  *   halves, by the kernel's form) and meet the codes without rounding these; maxima, sums and results are F32 or wider.
  *   Prompt chunks keep weights times their page's value scale to 2^-31 of the row's largest such product; values of a page
- *   whose scale is below 2^-90 of the largest in sight of the 128 rows of a tile count as zeros there. A query value that is not finite makes its own row NaN.
+ *   whose scale is below 2^-90 of the largest in sight of the 128 rows of a tile count as zeros there. Tokens
+ *   taken one by one refer to the largest value scale of the first 32 pages of a list (of each part that a CTA has): scales
+ *   below 2^-40 of it lose bits, and one above 2^80 times it is reported. A query value that is not finite makes its own row NaN.
  *
  * heads / kv_heads is any whole number, dim is 1 .. 256. A run that attends to every block has at most 2^31 - 128 rows
  * (count * heads / kv_heads). A sequence, page or position outside the cache
  * is skipped and reported by the next synchronising call (STRATA_ERR_DEVICE), or, in the pointer forms, by
- * bit 0 of *status (bit 4: a value that was not finite), which the caller clears. */
+ * bit 0 of *status (bit 4: a value that was not finite, bit 5: value scales too far apart), which the caller clears. */
 #define STRATA_KV8_BLOCK 64
 #define STRATA_KV8_WORKSPACE_BYTES (32u << 20)
 #define STRATA_KV8_SELECT_BLOCKS 32768

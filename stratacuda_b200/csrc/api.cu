@@ -111,6 +111,7 @@ int check_device_errors(strata_ctx *ctx) {
     if (e & kErrWaitTimeout) what += "a bounded device wait timed out; ";
     if (e & kErrPleScale) what += "Non-finite PLE scales; ";
     if (e & kErrKvValue) what += "Non-finite key or value; ";
+    if (e & kErrKvScale) what += "value scales too far apart; ";
     return fail(ctx, STRATA_ERR_DEVICE, "device check failed: %s", what.c_str());
 }
 

@@ -16,6 +16,7 @@ enum : unsigned {
     kErrRouting = 4u,      // a routed expert id was invalid or repeated (src/engine.js:138)
     kErrPleScale = 8u,     // a gathered PLE row has a non-finite FP16 scale (src/model.js:241)
     kErrKvValue = 16u,     // a key or value appended to an 8-bit cache is not finite
+    kErrKvScale = 32u,     // value scales in one list of an 8-bit cache are too far apart
 };
 
 // One resolved argument of a reference-compatible dispatch: a device buffer (ptr, length in

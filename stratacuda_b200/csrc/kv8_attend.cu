@@ -45,6 +45,10 @@ constexpr float kUnit = 268435456.0f;  // 2^28, below 2^32
 // is then 2^-4 at least, and rounding to a whole unit exact to 2^-25 of it. (5, 2^26 and room 4 moved less often, a sparse
 // prompt of 1024 tokens 426 instead of 445 us, but doubled the result's error to 2e-6.)
 constexpr float kRoom = 3.0f;
+// What weights refer to: a power of two near the largest value scale of the first 32 pages (of a unit's pages on this CTA) that
+// have one but zero. A page's scale counts as 2^kLeastLift of it at least when a row's reference is chosen, and may be up to kFar
+// times as large (past that it is reported): references and maxima so stay close enough for F32's exponents, also where parts are joined.
+constexpr float kLeastLift = -40.0f, kFar = 0x1p80f;
 constexpr long long kWaitClocks = 2000000000;  // about a second
 
 // P stored channels; R rows that the operands have room for, 4 .. 16.
@@ -58,7 +62,8 @@ struct Shape {
 // A step: 1 or 2 pages, the end of a unit (0), or the end of all (-1).
 struct Step {
     int pages, unit, block[2];
-    float k_scale[2], v_scale[2];
+    float k_scale[2], v_scale[2];  // values' over the unit's `ref`
+    float ref;
 };
 struct Unit {  // or the part of it that this CTA works on: entries [entry, stop) of its n
     int token, sub, entry, stop, n, seen, sequence, last_cta;
@@ -82,7 +87,7 @@ struct __align__(1024) Smem {
             float2 group_row[kRows];  // the second group's reference and sum of weights
             Unit unit[2];
             Step step[kSteps];
-            float4 list[32];  // pages looked up: page, block (bits), key scale, value scale
+            float4 list[32];  // pages looked up: page, block (bits), key scale, value scale over the unit's reference
             float group_ref;
             int what[2];  // by group: pages whose weights are there (-1: no more), plus 4 where O starts from zero
         };
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
             }
             __syncwarp();
             if (lane == 0) bar_arrive(&M.q_empty[qb]);
-            float ref = 0.0f;  // a power of two near the first page's value scale: what a weight's digits refer to
+            float ref = 0.0f;  // a power of two near the first pages' value scales: what a weight's digits refer to
             int held = 0;      // steps whose products are in TMEM's sums
             unsigned last = 0;  // the group's last step
             // TMEM's sums join o
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
                 ok = ok && wait_all(&M.step_full[ks], kc / kSteps & 1);
                 if (ok) {
                     const int pages = M.step[ks].pages, block = M.step[ks].block[page];
-                    const float by_k = M.step[ks].k_scale[page], by_v = M.step[ks].v_scale[page], first_v = M.step[ks].v_scale[0];
+                    const float by_k = M.step[ks].k_scale[page], by_v = M.step[ks].v_scale[page], of_unit = M.step[ks].ref;
                     __syncwarp();
                     if (lane == 0) bar_arrive(&M.step_empty[ks]);
                     ++kc;
@@ -321,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
                         ++sc;
                         continue;
                     }
-                    if (ref == 0.0f) ref = first_v > 0x1p-120f ? __uint_as_float(__float_as_uint(first_v) & 0x7f800000u) : 1.0f;
-                    f = by_v / ref;
+                    ref = of_unit;
+                    f = by_v;
                     here = page < pages;
                     pages_now = pages;
                     const int left = here ? u.seen - block * kKvBlock - token_in : 0;
@@ -331,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
                     int s[Z::ns];
 #pragma unroll
                     for (int c = 0; c < Z::ns; c += 16) tmem_ld16(tmem + mine + 64 * buf + c, s + c);
-                    lift = fmaxf(f > 0.0f ? log2f(f) : -40.0f, -40.0f);
+                    lift = fmaxf(f > 0.0f ? log2f(f) : kLeastLift, kLeastLift);
                     tmem_wait_ld();
                     tc_fence_before();
                     bar_arrive(&M.s_free[buf]);
@@ -511,13 +516,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
             base += 32;
             batch.end = base >= u.stop;
         };
+        float ref = 0.0f, per_ref = 0.0f;  // of the unit whose pages are being fetched
+        int ref_unit = -1;
         // a step's copies: a lane a box, of 64 key rows or of a page's values
         auto post = [&](int n, int unit_of, int head, int at) {
             const unsigned s = kc % kSteps, k = sc % Z::k_ring, v = vc % Z::v_ring;
             if (!wait_all(&M.step_empty[s], (kc / kSteps & 1) ^ 1)) return false;
             if (lane == 0) {
                 const float4 x = M.list[at & 31], y = M.list[(at + 1) & 31];
-                M.step[s] = Step{n, unit_of, {__float_as_int(x.y), __float_as_int(y.y)}, {x.z, y.z}, {x.w, y.w}};
+                M.step[s] = Step{n, unit_of, {__float_as_int(x.y), __float_as_int(y.y)}, {x.z, y.z}, {x.w, y.w}, ref};
                 bar_arrive(&M.step_full[s]);
             }
             ++kc;
@@ -542,9 +549,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv8_rows(const __grid_constant_
             const bool end = batch.end;
             const unsigned there = __ballot_sync(0xffffffffu, batch.page >= 0);
             const int count = __popc(there);
+            if (this_unit != ref_unit) {  // while all values are zero, nothing refers to it
+                const float most = warp_max(batch.page >= 0 ? batch.v_scale : 0.0f);
+                ref = most > 0.0f ? __uint_as_float(__float_as_uint(most) & 0x7f800000u) : 1.0f;
+                per_ref = __fdiv_rn(1.0f, ref);
+                if (most > 0.0f) ref_unit = this_unit;
+            }
+            if (batch.page >= 0 && batch.v_scale * per_ref > kFar) raise_error(A.c.err, kErrKvScale);
             if (batch.page >= 0)
                 M.list[__popc(there & ((1u << lane) - 1))] =
-                    make_float4(__int_as_float(batch.page), __int_as_float(batch.block), batch.k_scale, batch.v_scale);
+                    make_float4(__int_as_float(batch.page), __int_as_float(batch.block), batch.k_scale, batch.v_scale * per_ref);
             __syncwarp();
             for (int at = 0; at < count && ok; at += 2) {
                 ok = post(min(2, count - at), this_unit, head, at);

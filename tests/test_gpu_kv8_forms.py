@@ -224,3 +224,40 @@ def test_results_from_blocks_of_small_values(heads, kv, dim, blocks, small, coun
     picks = np.broadcast_to(heavy_blocks, (count, kv, len(heavy_blocks)))
     c.check_attend(got[0], q[0], k, v, start, 1 / math.sqrt(dim), picks)  # (the others' share is below 2^-100)
     assert c.errors() == 0
+
+
+@pytest.mark.parametrize("heads,kv,dim,blocks,sequences", [(4, 1, 64, 300, 16), (12, 1, 256, 200, 24), (8, 2, 128, 300, 9), (4, 1, 64, 20, 2)])
+@pytest.mark.parametrize("sizes", [(0.0, 2.0 ** -60), (2.0 ** -90, 2.0 ** 60), (0.0, 2.0 ** -90, 2.0 ** 20), (2.0 ** -60, 2.0 ** -20, 2.0 ** 20, 2.0 ** 60, 0.0)])
+def test_tokens_over_blocks_of_zeros_and_of_very_different_values(heads, kv, dim, blocks, sequences, sizes):
+    """Token steps over long lists (and a short one) whose blocks' values are of the given sizes, in no order."""
+    c = WideCache(kv, dim, sequences, blocks, blocks)
+    rng = np.random.default_rng(len(sizes))
+    n = blocks * BLOCK - 7
+    k, v = rng.normal(0, 1, (2, n, kv, dim))
+    v *= rng.choice(sizes, blocks).repeat(BLOCK)[:n, None, None]
+    k, v = k.astype(np.float32), v.astype(np.float32)
+    c.table[:] = c.i32(rng.permutation(blocks))
+    c.append(k[None], v[None], [0], [0])
+    q = rng.normal(0, 1, (sequences, 1, heads, dim)).astype(np.float32)
+    start = n - 1 - 50 * np.arange(sequences)
+    got = c.attend(q, heads, np.arange(sequences), start)
+    for s in (0, 1, sequences - 1):
+        c.check_attend(got[s], q[s], k, v, start[s], 1 / math.sqrt(dim))
+    assert c.errors() == 0
+
+
+def test_value_scales_too_far_apart_are_reported():
+    """A list whose later values are 2^150 times those of its first pages has no result in F32's exponents, and says so."""
+    heads, kv, dim, blocks, sequences = 4, 1, 64, 300, 40
+    c = WideCache(kv, dim, sequences, blocks, blocks)
+    rng = np.random.default_rng(1)
+    n = blocks * BLOCK
+    k, v = rng.normal(0, 1, (2, n, kv, dim))
+    v *= np.where(np.arange(n) < n // 2, 2.0 ** -90, 2.0 ** 60)[:, None, None]
+    c.table[:] = c.i32(np.arange(blocks))
+    c.append(k[None].astype(np.float32), v[None].astype(np.float32), [0], [0])
+    q = rng.normal(0, 1, (sequences, 1, heads, dim)).astype(np.float32)
+    c.attend(q, heads, np.arange(sequences), np.full(sequences, n // 2 - 1))  # small ones alone
+    assert c.errors() == 0
+    c.attend(q, heads, np.arange(sequences), np.full(sequences, n - 1))
+    assert c.errors() == 32
