@@ -54,14 +54,18 @@ class Kv8Cache:
             self._owned.append(buf)
             return buf
 
-        self.codes, self.marks = keep(n["codes"] // 4, "u32"), keep(n["marks"] // 4, "u32")
-        self.scales, self.open, self.table = keep(n["scales"]), keep(n["open"]), keep(n["table"], "i32")
-        # caches whose calls follow one another on the backend's stream may share one workspace
-        self.workspace = keep(n["workspace"], "u32") if workspace is None else workspace
-        if pages is None:
-            self.write_table(np.arange(self.pages, dtype=np.int32).reshape(sequences, blocks))
-        else:
-            self.write_table(np.full((sequences, blocks), -1, np.int32))
+        try:
+            self.codes, self.marks = keep(n["codes"] // 4, "u32"), keep(n["marks"] // 4, "u32")
+            self.scales, self.open, self.table = keep(n["scales"]), keep(n["open"]), keep(n["table"], "i32")
+            # caches whose calls follow one another on the backend's stream may share one workspace
+            self.workspace = keep(n["workspace"], "u32") if workspace is None else workspace
+            if pages is None:
+                self.write_table(np.arange(self.pages, dtype=np.int32).reshape(sequences, blocks))
+            else:
+                self.write_table(np.full((sequences, blocks), -1, np.int32))
+        except BaseException:  # nobody else has them
+            self.free()
+            raise
 
     def write_table(self, table) -> None:
         """The page of every block of every sequence, int [sequences][blocks]; -1 where there is none yet."""

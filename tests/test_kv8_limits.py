@@ -16,3 +16,48 @@ def test_attend_refuses_longer_lists_than_a_table_has_blocks(top):
 def test_attend_refuses_runs_of_more_rows_than_32_bits_count(count, heads):
     """A prompt's rows, tokens times query heads a key/value head, are counted in 32 bits."""
     assert refuse(kv8.StrataRangeError, "2\\^31", lambda: CALLS["attend"](cache(kv_heads=1, dim=1), count=count, heads=heads)) == L.ERR_RANGE
+
+
+class Backend:
+    """Hands out buffers and takes them back; the `fails`-th allocation (or the first write) does not succeed."""
+    kind = "cuda"
+
+    def __init__(self, fails=None, writes=True):
+        self.fails, self.writes, self.made, self.live = fails, writes, 0, set()
+
+    def alloc(self, length, type="f32", zero=True):
+        self.made += 1
+        if self.made == self.fails:
+            raise kv8.StrataError(L.ERR_ALLOC, "device allocation failed")
+        self.live.add(self.made)
+        return self.made
+
+    def write(self, buf, data, offset=0):
+        if not self.writes:
+            raise kv8.StrataError(L.ERR_CUDA, "write failed")
+
+    def free(self, buf):
+        self.live.remove(buf)
+
+
+@pytest.mark.parametrize("fails", [1, 2, 3, 4, 5, 6, None])
+def test_a_cache_that_cannot_be_had_leaves_no_buffer_behind(fails):
+    backend = Backend(fails, writes=False)
+    with pytest.raises(kv8.StrataError):
+        kv8.Kv8Cache(backend, kv_heads=2, dim=64, sequences=3, blocks=5)
+    assert backend.made == (fails or 6) and not backend.live
+    shared = Backend()
+    workspace = shared.alloc(8)
+    shared.fails = 4
+    with pytest.raises(kv8.StrataError):
+        kv8.Kv8Cache(shared, kv_heads=2, dim=64, sequences=3, blocks=5, workspace=workspace)
+    assert shared.live == {workspace}  # a workspace that others use stays
+
+
+def test_a_cache_gives_its_buffers_back_once():
+    backend = Backend()
+    c = kv8.Kv8Cache(backend, kv_heads=2, dim=64, sequences=3, blocks=5)
+    assert len(backend.live) == 6
+    c.free()
+    c.free()
+    assert not backend.live
