@@ -43,6 +43,8 @@ class Kv8Cache:
     sequence, in order; with fewer, the caller hands pages out with ``write_table``."""
 
     def __init__(self, backend, kv_heads: int, dim: int, sequences: int, blocks: int, pages: int | None = None, workspace=None):
+        if getattr(backend, "kind", None) != "cuda":
+            raise StrataRangeError(L.ERR_RANGE, "an 8-bit cache needs the CUDA backend")
         self.b = backend
         self.kv_heads, self.dim, self.sequences, self.blocks = kv_heads, dim, sequences, blocks
         self.pages = sequences * blocks if pages is None else pages

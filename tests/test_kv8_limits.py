@@ -61,3 +61,19 @@ def test_a_cache_gives_its_buffers_back_once():
     c.free()
     c.free()
     assert not backend.live
+
+
+def test_a_cache_asks_for_the_cuda_backend():
+    """Its operators have no other: a batch on a host backend is refused when it is made, not at its first step."""
+    from oracle.backend import OracleBackend
+    from oracle.oracle import Oracle
+    from stratacuda_b200.engine import SequenceBatch, StrataEngine
+    from stratacuda_b200.model import create_fixture
+    host = OracleBackend(Oracle("port"))
+    with pytest.raises(ValueError, match="CUDA backend"):
+        kv8.Kv8Cache(host, kv_heads=2, dim=64, sequences=3, blocks=5)
+    engine = StrataEngine.create(create_fixture(), host)
+    for top in (0, 8):
+        with pytest.raises(ValueError, match="CUDA backend"):
+            SequenceBatch(engine, 2, kv8=True, top=top)
+    SequenceBatch(engine, 2).dispose()
