@@ -972,6 +972,7 @@ class SequenceBatch(PromptBatch):
         self.capacity = capacity
         self.use_graph = bool(graph) and getattr(engine.store, "moe_layer", None) is not None
         self.persistent, self.caches = [], []
+        self._graph = self._graph_head = None
         self.disposed = False
         self.kv8, self.top = bool(kv8), top
         hc, c = g["width"] * g["streams"], (2 * g["keyHeads"] + g["valueHeads"]) * g["ssmDim"]
@@ -1002,8 +1003,6 @@ class SequenceBatch(PromptBatch):
             raise
         self.positions = [None] * capacity  # None: an empty slot
         self.previous = [[] for _ in range(capacity)]
-        self._graph = None
-        self._graph_head = None
         self.failed = False
 
     def _keep(self, n: int, type: str = "f32"):

@@ -77,3 +77,26 @@ def test_a_cache_asks_for_the_cuda_backend():
         with pytest.raises(ValueError, match="CUDA backend"):
             SequenceBatch(engine, 2, kv8=True, top=top)
     SequenceBatch(engine, 2).dispose()
+
+
+@pytest.mark.parametrize("fails", [1, 2, 5, 9])
+def test_a_batch_that_cannot_be_had_leaves_no_buffer_behind(fails):
+    """The allocation's own error comes through, and the buffers made before it are given back."""
+    from oracle.backend import OracleBackend
+    from oracle.oracle import Oracle
+    from stratacuda_b200.engine import SequenceBatch, StrataEngine
+    from stratacuda_b200.model import create_fixture
+    host = OracleBackend(Oracle("port"))
+    engine = StrataEngine.create(create_fixture(), host)
+    live, alloc, free = [], host.alloc, host.free
+
+    def counted(*args, **kw):
+        if len(live) + 1 == fails:
+            raise MemoryError("no more")
+        live.append(alloc(*args, **kw))
+        return live[-1]
+
+    host.alloc, host.free = counted, lambda buf: (live.remove(buf), free(buf))
+    with pytest.raises(MemoryError, match="no more"):
+        SequenceBatch(engine, 2)
+    assert not live
