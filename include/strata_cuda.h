@@ -356,6 +356,25 @@ int strata_kv8_select_dev(const strata_kv8_cache_dev *cache, const float *q, uin
 int strata_kv8_attend_dev(const strata_kv8_cache_dev *cache, const float *q, uint64_t row_stride, int32_t heads, int32_t segments,
                           int32_t count, const int32_t *sequence, const int32_t *start, const int32_t *picks, int32_t top, float scale,
                           float *y, void *stream, char *msg, size_t msg_cap);
+/* The same three with their arguments in a structure, for bindings that pay for each argument. `rows` is k or q; members
+ * that an operator does not take are ignored. */
+#define STRATA_KV8_APPEND 0
+#define STRATA_KV8_SELECT 1
+#define STRATA_KV8_ATTEND 2
+typedef struct {
+    const strata_kv8_cache_dev *cache;
+    const float *rows, *v;
+    uint64_t row_stride;
+    const int32_t *sequence, *start;
+    int32_t *picks; /* select: written; attend: read, or null */
+    float *y;
+    void *stream;
+    char *msg;
+    uint64_t msg_cap;
+    int32_t op, segments, count, heads, top, first, last;
+    float scale;
+} strata_kv8_call;
+int strata_kv8_call_dev(const strata_kv8_call *call);
 
 /* ---- CUDA graphs of the context's stream (no reference counterpart: the B200 runtime replays
  * captured work instead of relaunching it from the host) ----

@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import pathlib
+import struct
 
 PKG = pathlib.Path(__file__).resolve().parent
 LIB_PATH = pathlib.Path(os.environ.get("STRATA_CUDA_LIB", PKG / "libstrata_cuda.so"))
@@ -37,6 +38,8 @@ class StrataMoeLayerDev(C.Structure):
 
 
 KV8_BLOCK, KV8_WORKSPACE_BYTES, KV8_SELECT_BLOCKS = 64, 32 << 20, 32768
+KV8_APPEND, KV8_SELECT, KV8_ATTEND = 0, 1, 2
+KV8_CALL = struct.Struct("@11Q7if")  # strata_kv8_call: cache .. msg_cap, op .. last, scale
 
 
 class StrataKv8Cache(C.Structure):
@@ -96,6 +99,7 @@ SIGNATURES = {
                                C.c_int32, _vp, _vp, C.c_char_p, _sz], _i),
     "strata_kv8_attend_dev": ([C.POINTER(StrataKv8CacheDev), _vp, _u64, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_int32,
                                C.c_float, _vp, _vp, C.c_char_p, _sz], _i),
+    "strata_kv8_call_dev": ([C.c_char_p], _i),
     "strata_synth_blobs": ([_vp, _u64, _u64, _u64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32], _i),
     "strata_synth_normals": ([_vp, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _d], _i),
 }

@@ -138,3 +138,19 @@ extern "C" int strata_kv8_attend_dev(const strata_kv8_cache_dev *cache, const fl
     if (!std::isfinite(scale)) return say(msg, msg_cap, STRATA_ERR_RANGE, "scale must be finite");
     return done(kv8_attend(c, q, (long long)row_stride, heads, r, picks, top, scale, y, static_cast<cudaStream_t>(stream)), msg, msg_cap);
 }
+
+extern "C" int strata_kv8_call_dev(const strata_kv8_call *a) {
+    if (!a) return STRATA_ERR_RANGE;
+    switch (a->op) {
+    case STRATA_KV8_APPEND:
+        return strata_kv8_append_dev(a->cache, a->rows, a->v, a->row_stride, a->segments, a->count, a->sequence, a->start, a->stream, a->msg,
+                                     a->msg_cap);
+    case STRATA_KV8_SELECT:
+        return strata_kv8_select_dev(a->cache, a->rows, a->row_stride, a->heads, a->segments, a->count, a->sequence, a->start, a->top, a->first,
+                                     a->last, a->picks, a->stream, a->msg, a->msg_cap);
+    case STRATA_KV8_ATTEND:
+        return strata_kv8_attend_dev(a->cache, a->rows, a->row_stride, a->heads, a->segments, a->count, a->sequence, a->start, a->picks, a->top,
+                                     a->scale, a->y, a->stream, a->msg, a->msg_cap);
+    }
+    return say(a->msg, a->msg_cap, STRATA_ERR_RANGE, "op must be STRATA_KV8_APPEND, _SELECT or _ATTEND");
+}

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import numpy as np
 
@@ -38,6 +39,12 @@ def sizes(kv_heads: int, dim: int, pages: int, sequences: int, blocks: int) -> d
                 open=sequences * 2 * BLOCK * kv_heads * dim, table=sequences * blocks, workspace=L.KV8_WORKSPACE_BYTES // 4)
 
 
+def _int32(**values) -> None:
+    for name, x in values.items():
+        if not -(1 << 31) <= x < 1 << 31:
+            raise StrataRangeError(L.ERR_RANGE, f"{name} must be a 32-bit integer")
+
+
 class Kv8Cache:
     """One layer's cache on a CudaBackend. `pages` defaults to a page for every block of every
     sequence, in order; with fewer, the caller hands pages out with ``write_table``."""
@@ -45,6 +52,7 @@ class Kv8Cache:
     def __init__(self, backend, kv_heads: int, dim: int, sequences: int, blocks: int, pages: int | None = None, workspace=None):
         if getattr(backend, "kind", None) != "cuda":
             raise StrataRangeError(L.ERR_RANGE, "an 8-bit cache needs the CUDA backend")
+        _int32(kv_heads=kv_heads, dim=dim, sequences=sequences, blocks=blocks, pages=sequences * blocks if pages is None else pages)
         self.b = backend
         self.kv_heads, self.dim, self.sequences, self.blocks = kv_heads, dim, sequences, blocks
         self.pages = sequences * blocks if pages is None else pages
@@ -82,12 +90,14 @@ class Kv8Cache:
 
     def append(self, k, v, sequence, start, segments: int = 1, count: int = 1, row_stride: int = 0) -> None:
         """Append rows k and v [segments * count][kv_heads * dim] (strata_kv8_append)."""
+        _int32(segments=segments, count=count)
         self.b._check(self.b.lib.strata_kv8_append(self.b.ctx, C.byref(self._struct()), k.handle, v.handle, row_stride, segments, count,
                                                    sequence.handle, start.handle))
 
     def select(self, q, heads: int, picks, sequence, start, segments: int = 1, count: int = 1, top: int = 32, first: int = 1, last: int = 2,
                row_stride: int = 0) -> None:
         """picks [segments * count][kv_heads][top] (i32): the chosen blocks (strata_kv8_select)."""
+        _int32(segments=segments, count=count, heads=heads, top=top, first=first, last=last)
         self.b._check(self.b.lib.strata_kv8_select(self.b.ctx, C.byref(self._struct()), q.handle, row_stride, heads, segments, count,
                                                    sequence.handle, start.handle, top, first, last, picks.handle))
 
@@ -95,6 +105,7 @@ class Kv8Cache:
                scale: float | None = None, row_stride: int = 0) -> None:
         """y [segments * count][heads * dim]: attention over all blocks, or those in `picks` (strata_kv8_attend).
         `scale` defaults to 1 / sqrt(dim)."""
+        _int32(segments=segments, count=count, heads=heads, top=top)
         self.b._check(self.b.lib.strata_kv8_attend(self.b.ctx, C.byref(self._struct()), q.handle, row_stride, heads, segments, count,
                                                    sequence.handle, start.handle, 0 if picks is None else picks.handle, top,
                                                    1 / math.sqrt(self.dim) if scale is None else scale, y.handle))
@@ -106,10 +117,12 @@ class Kv8Cache:
 
 
 def _address(x):
+    if x is None:
+        return 0
     try:
         return x.data_ptr()
     except AttributeError:
-        return x if x is None or isinstance(x, int) else x.device_ptr
+        return x if isinstance(x, int) else x.device_ptr
 
 
 class DeviceCache:
@@ -123,26 +136,32 @@ class DeviceCache:
         self.lib = L.load()
         self.kv_heads, self.dim = kv_heads, dim
         self.parts = (codes, marks, scales, open, table, workspace, status)
+        _int32(kv_heads=kv_heads, dim=dim, pages=pages, sequences=sequences, blocks=blocks)
         self._cache = L.StrataKv8CacheDev(kv_heads, dim, pages, sequences, blocks, *[_address(x) for x in self.parts])
-        self._ref = C.byref(self._cache)
+        self._at = C.addressof(self._cache)
         self._msg = C.create_string_buffer(256)
+        self._msg_at = C.addressof(self._msg)
         self._scale = 1 / math.sqrt(dim) if dim > 0 else 0.0
 
-    def _check(self, rc: int) -> None:
+    def _call(self, rows, v, row_stride, sequence, start, picks, y, stream, op, segments, count, heads=0, top=0, first=0, last=0, scale=0.0) -> None:
+        try:
+            call = L.KV8_CALL.pack(self._at, rows, v, row_stride, sequence, start, picks, y, stream, self._msg_at, 256, op, segments, count, heads,
+                                   top, first, last, scale)
+        except (struct.error, OverflowError) as e:
+            raise StrataRangeError(L.ERR_RANGE, f"an argument is not a number of its type: {e}") from None
+        rc = self.lib.strata_kv8_call_dev(call)
         if rc != L.OK:
             raise (StrataRangeError if rc == L.ERR_RANGE else StrataError)(rc, self._msg.value.decode(errors="replace"))
 
     def append(self, k, v, sequence, start, segments: int = 1, count: int = 1, row_stride: int = 0, stream: int = 0) -> None:
-        self._check(self.lib.strata_kv8_append_dev(self._ref, _address(k), _address(v), row_stride, segments, count, _address(sequence),
-                                                   _address(start), stream, self._msg, 256))
+        self._call(_address(k), _address(v), row_stride, _address(sequence), _address(start), 0, 0, stream, L.KV8_APPEND, segments, count)
 
     def select(self, q, heads: int, picks, sequence, start, segments: int = 1, count: int = 1, top: int = 32, first: int = 1, last: int = 2,
                row_stride: int = 0, stream: int = 0) -> None:
-        self._check(self.lib.strata_kv8_select_dev(self._ref, _address(q), row_stride, heads, segments, count, _address(sequence),
-                                                   _address(start), top, first, last, _address(picks), stream, self._msg, 256))
+        self._call(_address(q), 0, row_stride, _address(sequence), _address(start), _address(picks), 0, stream, L.KV8_SELECT, segments, count,
+                   heads, top, first, last)
 
     def attend(self, q, heads: int, y, sequence, start, segments: int = 1, count: int = 1, picks=None, top: int = 0,
                scale: float | None = None, row_stride: int = 0, stream: int = 0) -> None:
-        self._check(self.lib.strata_kv8_attend_dev(self._ref, _address(q), row_stride, heads, segments, count, _address(sequence),
-                                                   _address(start), _address(picks), top, self._scale if scale is None else scale,
-                                                   _address(y), stream, self._msg, 256))
+        self._call(_address(q), 0, row_stride, _address(sequence), _address(start), _address(picks), _address(y), stream, L.KV8_ATTEND, segments,
+                   count, heads, top, 0, 0, self._scale if scale is None else scale)

@@ -100,3 +100,45 @@ def test_a_batch_that_cannot_be_had_leaves_no_buffer_behind(fails):
     with pytest.raises(MemoryError, match="no more"):
         SequenceBatch(engine, 2)
     assert not live
+
+
+@pytest.mark.parametrize("name,bad", [("append", dict(segments=(1 << 32) + 1)), ("append", dict(count=(1 << 32) + 1)), ("select", dict(top=(1 << 32) + 4)),
+                                      ("select", dict(first=1 << 32)), ("attend", dict(heads=(1 << 32) + 4)), ("attend", dict(count=-(1 << 32) + 1)),
+                                      ("attend", dict(picks=A, top=(1 << 33) + 1)), ("append", dict(row_stride=-1)), ("attend", dict(scale=1e300))])
+def test_refuses_integers_past_their_range(name, bad):
+    """2^32 + 1 rows are not one row."""
+    with pytest.raises(kv8.StrataError) as e:
+        CALLS[name](cache(), **bad)
+    assert e.value.code in (L.ERR_RANGE, L.ERR_LAYOUT)
+
+
+def test_a_cache_refuses_integers_past_their_range():
+    for bad in (dict(kv_heads=(1 << 32) + 2), dict(dim=(1 << 32) + 64), dict(pages=1 << 32), dict(sequences=(1 << 32) + 1), dict(blocks=-(1 << 32) + 4)):
+        with pytest.raises(kv8.StrataError) as e:
+            CALLS["append"](cache(**bad))
+        assert e.value.code == L.ERR_RANGE
+
+
+def test_a_cache_on_the_backend_refuses_integers_past_their_range():
+    class Library:
+        def __getattr__(self, name):
+            raise AssertionError("the call went through")
+
+    class Buf:
+        handle = 1
+
+    big = (1 << 32) + 1
+    backend = Backend()
+    with pytest.raises(kv8.StrataRangeError, match="sequences"):
+        kv8.Kv8Cache(backend, kv_heads=2, dim=64, sequences=big, blocks=1)
+    with pytest.raises(kv8.StrataRangeError, match="pages"):
+        kv8.Kv8Cache(backend, kv_heads=2, dim=64, sequences=1 << 20, blocks=1 << 20)
+    assert not backend.live
+    c = kv8.Kv8Cache(backend, kv_heads=2, dim=64, sequences=3, blocks=5)
+    backend.lib = Library()
+    b = Buf()
+    for name, call in (("segments", lambda: c.append(b, b, b, b, big)), ("count", lambda: c.append(b, b, b, b, 1, big)),
+                       ("top", lambda: c.select(b, 4, b, b, b, top=big)), ("last", lambda: c.select(b, 4, b, b, b, last=big)),
+                       ("heads", lambda: c.attend(b, big, b, b, b)), ("top", lambda: c.attend(b, 4, b, b, b, picks=b, top=big))):
+        with pytest.raises(kv8.StrataRangeError, match=name):
+            call()
