@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+import threading
 
 import numpy as np
 
@@ -125,6 +126,17 @@ def _address(x):
         return x if isinstance(x, int) else x.device_ptr
 
 
+class _Message(threading.local):
+    """Where a thread's calls leave the reason for a refusal."""
+
+    def __init__(self):
+        self.text = C.create_string_buffer(256)
+        self.at = C.addressof(self.text)
+
+
+_message = _Message()
+
+
 class DeviceCache:
     """A cache in caller-owned device memory: torch tensors, Buffers or addresses of the layouts in
     include/strata_cuda.h. Calls go to `stream` (a cudaStream_t as an integer; 0 is the default
@@ -139,19 +151,17 @@ class DeviceCache:
         _int32(kv_heads=kv_heads, dim=dim, pages=pages, sequences=sequences, blocks=blocks)
         self._cache = L.StrataKv8CacheDev(kv_heads, dim, pages, sequences, blocks, *[_address(x) for x in self.parts])
         self._at = C.addressof(self._cache)
-        self._msg = C.create_string_buffer(256)
-        self._msg_at = C.addressof(self._msg)
         self._scale = 1 / math.sqrt(dim) if dim > 0 else 0.0
 
     def _call(self, rows, v, row_stride, sequence, start, picks, y, stream, op, segments, count, heads=0, top=0, first=0, last=0, scale=0.0) -> None:
         try:
-            call = L.KV8_CALL.pack(self._at, rows, v, row_stride, sequence, start, picks, y, stream, self._msg_at, 256, op, segments, count, heads,
+            call = L.KV8_CALL.pack(self._at, rows, v, row_stride, sequence, start, picks, y, stream, _message.at, 256, op, segments, count, heads,
                                    top, first, last, scale)
         except (struct.error, OverflowError) as e:
             raise StrataRangeError(L.ERR_RANGE, f"an argument is not a number of its type: {e}") from None
         rc = self.lib.strata_kv8_call_dev(call)
         if rc != L.OK:
-            raise (StrataRangeError if rc == L.ERR_RANGE else StrataError)(rc, self._msg.value.decode(errors="replace"))
+            raise (StrataRangeError if rc == L.ERR_RANGE else StrataError)(rc, _message.text.value.decode(errors="replace"))
 
     def append(self, k, v, sequence, start, segments: int = 1, count: int = 1, row_stride: int = 0, stream: int = 0) -> None:
         self._call(_address(k), _address(v), row_stride, _address(sequence), _address(start), 0, 0, stream, L.KV8_APPEND, segments, count)

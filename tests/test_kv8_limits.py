@@ -142,3 +142,23 @@ def test_a_cache_on_the_backend_refuses_integers_past_their_range():
                        ("heads", lambda: c.attend(b, big, b, b, b)), ("top", lambda: c.attend(b, 4, b, b, b, picks=b, top=big))):
         with pytest.raises(kv8.StrataRangeError, match=name):
             call()
+
+
+def test_a_refusals_message_is_its_own_threads():
+    """Another thread's refusal by the same cache, between a call's return and its message's reading, changes nothing."""
+    import threading
+    c = cache()
+    entry, inside = c.lib.strata_kv8_call_dev, []
+
+    class Library:
+        def strata_kv8_call_dev(self, call):
+            rc = entry(call)
+            if not inside:
+                inside.append(1)
+                other = threading.Thread(target=lambda: refuse(kv8.StrataRangeError, "divisible", lambda: CALLS["attend"](c, heads=5)))
+                other.start()
+                other.join()
+            return rc
+
+    c.lib = Library()
+    refuse(kv8.StrataRangeError, "segments", lambda: CALLS["append"](c, segments=0))
