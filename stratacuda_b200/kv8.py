@@ -23,7 +23,7 @@ import threading
 import numpy as np
 
 from . import _lib as L
-from .backend import StrataError, StrataRangeError
+from .backend import Buffer, StrataError, StrataRangeError
 
 BLOCK = L.KV8_BLOCK
 
@@ -117,13 +117,57 @@ class Kv8Cache:
         self._owned = []
 
 
-def _address(x):
-    if x is None:
-        return 0
-    try:
-        return x.data_ptr()
-    except AttributeError:
-        return x if isinstance(x, int) else x.device_ptr
+class _Types:
+    """torch's element types, once a tensor has been seen."""
+    int8 = int32 = float32 = None
+
+    @classmethod
+    def known(cls):
+        if cls.int8 is None:
+            import torch
+            cls.int8, cls.int32, cls.float32 = torch.int8, torch.int32, torch.float32
+        return cls
+
+
+def _memory(x, what: str, need: int, device):
+    """Device address of a tensor's elements, `need` or more that follow one another."""
+    if x.get_device() < 0 or (device is not None and x.get_device() != device):
+        raise StrataError(L.ERR_LAYOUT, f"{what} must be on the cache's CUDA device, not on {x.device}")
+    if not x.is_contiguous():
+        raise StrataError(L.ERR_LAYOUT, f"{what} must be contiguous (rows of k, v and q may be row_stride apart)")
+    if x.numel() < need:
+        raise StrataError(L.ERR_LAYOUT, f"{what} needs {need} elements, the tensor has {x.numel()}")
+    return x.data_ptr()
+
+
+def _address(x, what: str, need: int, dtype: str, device):
+    """Device address of `need` elements: of a tensor of that type or a Buffer that has them, or as given."""
+    if x is None or isinstance(x, int):
+        return x or 0
+    if isinstance(x, Buffer):
+        if x.length < need:
+            raise StrataError(L.ERR_LAYOUT, f"{what} needs {need} elements, the buffer has {x.length}")
+        return x.device_ptr
+    if x.dtype is not getattr(_Types.known(), dtype):
+        raise StrataError(L.ERR_LAYOUT, f"{what} must be a tensor of torch.{dtype}, not {x.dtype}")
+    return _memory(x, what, need, device)
+
+
+def _words(x, what: str, need: int, device):
+    """The same of `need` 32-bit words, in a tensor of any type."""
+    if hasattr(x, "element_size"):
+        return _memory(x, what, -(-4 * need // x.element_size()), device)
+    return _address(x, what, need, "int32", device)
+
+
+def _strided(x, what: str, rows: int, width: int, row_stride: int, device):
+    """The same of `rows` rows of `width` floats, `row_stride` apart."""
+    if x is None or isinstance(x, (int, Buffer)) or x.is_contiguous():
+        return _address(x, what, (rows - 1) * row_stride + width, "float32", device)
+    # a view of some columns of longer rows
+    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) != row_stride or x.shape[0] < max(rows, 1) or x.shape[1] < width:
+        raise StrataError(L.ERR_LAYOUT, f"{what} must be {rows} rows of {width} elements, {row_stride} apart")
+    return _address(x[0], what, width, "float32", device)
 
 
 class _Message(threading.local):
@@ -139,7 +183,8 @@ _message = _Message()
 
 class DeviceCache:
     """A cache in caller-owned device memory: torch tensors, Buffers or addresses of the layouts in
-    include/strata_cuda.h. Calls go to `stream` (a cudaStream_t as an integer; 0 is the default
+    include/strata_cuda.h. Tensors are checked for their type, device, order and size and Buffers for their size; addresses
+    are the caller's word. Calls go to `stream` (a cudaStream_t as an integer; 0 is the default
     stream) of the current device, allocate nothing and do not synchronise. `status`, where given, is
     a zeroed 32-bit device word that device-side errors are added to. The parts must stay alive."""
 
@@ -149,7 +194,16 @@ class DeviceCache:
         self.kv_heads, self.dim = kv_heads, dim
         self.parts = (codes, marks, scales, open, table, workspace, status)
         _int32(kv_heads=kv_heads, dim=dim, pages=pages, sequences=sequences, blocks=blocks)
-        self._cache = L.StrataKv8CacheDev(kv_heads, dim, pages, sequences, blocks, *[_address(x) for x in self.parts])
+        self._device = d = codes.get_device() if hasattr(codes, "get_device") else None
+        n = sizes(kv_heads, dim, pages, sequences, blocks)
+
+        def codes_at(x, what):  # a Buffer has them four to an element
+            return _address(x, what, n[what] // 4 if isinstance(x, Buffer) else n[what], "int8", d)
+
+        self._cache = L.StrataKv8CacheDev(kv_heads, dim, pages, sequences, blocks, codes_at(codes, "codes"), codes_at(marks, "marks"),
+                                          _address(scales, "scales", n["scales"], "float32", d),
+                                          _address(open, "open", n["open"], "float32", d), _address(table, "table", n["table"], "int32", d),
+                                          _words(workspace, "workspace", n["workspace"], d), _words(status, "status", 1, d))
         self._at = C.addressof(self._cache)
         self._scale = 1 / math.sqrt(dim) if dim > 0 else 0.0
 
@@ -163,15 +217,40 @@ class DeviceCache:
         if rc != L.OK:
             raise (StrataRangeError if rc == L.ERR_RANGE else StrataError)(rc, _message.text.value.decode(errors="replace"))
 
+    # most calls' tensors are as they should be: these look at that at once, and leave the rest to _address
+    def _floats(self, x, what: str, need: int):
+        try:
+            if x.dtype is _Types.float32 and x.get_device() == self._device and x.numel() >= need and x.is_contiguous():
+                return x.data_ptr()
+        except AttributeError:  # an address or a Buffer
+            pass
+        return _address(x, what, need, "float32", self._device)
+
+    def _ints(self, x, what: str, need: int):
+        try:
+            if x.dtype is _Types.int32 and x.get_device() == self._device and x.numel() >= need and x.is_contiguous():
+                return x.data_ptr()
+        except AttributeError:  # an address or a Buffer
+            pass
+        return _address(x, what, need, "int32", self._device)
+
     def append(self, k, v, sequence, start, segments: int = 1, count: int = 1, row_stride: int = 0, stream: int = 0) -> None:
-        self._call(_address(k), _address(v), row_stride, _address(sequence), _address(start), 0, 0, stream, L.KV8_APPEND, segments, count)
+        n, w = segments * count, self.kv_heads * self.dim
+        self._call(_strided(k, "k", n, w, row_stride, self._device) if row_stride else self._floats(k, "k", n * w),
+                   _strided(v, "v", n, w, row_stride, self._device) if row_stride else self._floats(v, "v", n * w), row_stride,
+                   self._ints(sequence, "sequence", segments), self._ints(start, "start", segments), 0, 0, stream, L.KV8_APPEND, segments, count)
 
     def select(self, q, heads: int, picks, sequence, start, segments: int = 1, count: int = 1, top: int = 32, first: int = 1, last: int = 2,
                row_stride: int = 0, stream: int = 0) -> None:
-        self._call(_address(q), 0, row_stride, _address(sequence), _address(start), _address(picks), 0, stream, L.KV8_SELECT, segments, count,
-                   heads, top, first, last)
+        n, w = segments * count, heads * self.dim
+        self._call(_strided(q, "q", n, w, row_stride, self._device) if row_stride else self._floats(q, "q", n * w), 0, row_stride,
+                   self._ints(sequence, "sequence", segments), self._ints(start, "start", segments),
+                   self._ints(picks, "picks", n * self.kv_heads * top), 0, stream, L.KV8_SELECT, segments, count, heads, top, first, last)
 
     def attend(self, q, heads: int, y, sequence, start, segments: int = 1, count: int = 1, picks=None, top: int = 0,
                scale: float | None = None, row_stride: int = 0, stream: int = 0) -> None:
-        self._call(_address(q), 0, row_stride, _address(sequence), _address(start), _address(picks), _address(y), stream, L.KV8_ATTEND, segments,
-                   count, heads, top, 0, 0, self._scale if scale is None else scale)
+        n, w = segments * count, heads * self.dim
+        self._call(_strided(q, "q", n, w, row_stride, self._device) if row_stride else self._floats(q, "q", n * w), 0, row_stride,
+                   self._ints(sequence, "sequence", segments), self._ints(start, "start", segments),
+                   0 if picks is None else self._ints(picks, "picks", n * self.kv_heads * top), self._floats(y, "y", n * w), stream,
+                   L.KV8_ATTEND, segments, count, heads, top, 0, 0, self._scale if scale is None else scale)

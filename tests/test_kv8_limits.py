@@ -162,3 +162,132 @@ def test_a_refusals_message_is_its_own_threads():
 
     c.lib = Library()
     refuse(kv8.StrataRangeError, "segments", lambda: CALLS["append"](c, segments=0))
+
+
+# ---------------------------------------------------------------- tensors
+
+class Calls:
+    """Stands in for the library: keeps the calls that would have gone through."""
+
+    def __init__(self):
+        self.made = []
+
+    def strata_kv8_call_dev(self, call):
+        self.made.append(L.KV8_CALL.unpack(call))
+        return L.OK
+
+
+def tensors(device=0, **kw):
+    """A DeviceCache of tensors (2 heads of 72, 3 sequences of 5 blocks, 17 pages) that say they are on `device`, and the
+    arguments of a call on 3 runs of 4 tokens, by name; `kw` changes some of either."""
+    import torch
+
+    class On(torch.Tensor):
+        def get_device(self):
+            return getattr(self, "claimed", device)
+
+    def make(shape, dtype=torch.float32):
+        return torch.zeros(shape, dtype=dtype).as_subclass(On)
+
+    parts = dict(codes=make((17, 2, 2, 128 * 64), torch.int8), marks=make((17, 2, 2, 128), torch.int8), scales=make((17, 2, 2)),
+                 open=make((3, 2, 64, 2, 72)), table=make((3, 5), torch.int32), workspace=make(L.KV8_WORKSPACE_BYTES, torch.uint8),
+                 status=make(1, torch.int32))
+    arguments = dict(k=make((12, 144)), v=make((12, 144)), q=make((12, 6 * 72)), y=make((12, 6 * 72)), sequence=make(3, torch.int32),
+                     start=make(3, torch.int32), picks=make((12, 2, 4), torch.int32))
+    for name, change in kw.items():
+        where = parts if name in parts else arguments
+        where[name] = change(where[name])
+    c = kv8.DeviceCache(2, 72, 17, 3, 5, **parts)
+    c.lib = Calls()
+    return c, arguments
+
+
+def every_call(c, a, **kw):
+    common = dict(sequence=a["sequence"], start=a["start"], segments=3, count=4, **kw)
+    return {"append": lambda: c.append(a["k"], a["v"], **common), "select": lambda: c.select(a["q"], 6, a["picks"], top=4, **common),
+            "attend": lambda: c.attend(a["q"], 6, a["y"], **common), "sparse": lambda: c.attend(a["q"], 6, a["y"], picks=a["picks"], top=4, **common)}
+
+
+def elsewhere(where):
+    def change(t):
+        t.claimed = where
+        return t
+    return change
+
+
+def test_tensors_as_they_should_be_go_through():
+    c, a = tensors()
+    for call in every_call(c, a).values():
+        call()
+    assert len(c.lib.made) == 4
+    made = c.lib.made[0]
+    assert made[1:3] == (a["k"].data_ptr(), a["v"].data_ptr()) and made[4:6] == (a["sequence"].data_ptr(), a["start"].data_ptr())
+    assert c.lib.made[3][6:8] == (a["picks"].data_ptr(), a["y"].data_ptr()) and c.lib.made[2][6] == 0
+
+
+@pytest.mark.parametrize("part", ["codes", "marks", "scales", "open", "table", "workspace", "status"])
+def test_a_cache_of_tensors_refuses_parts_that_are_none(part):
+    import torch
+    cut = dict(codes=lambda t: t[:-1], marks=lambda t: t[:-1], scales=lambda t: t[1:], open=lambda t: t[:2], table=lambda t: t[:, :4].contiguous(),
+               workspace=lambda t: t[1:], status=lambda t: t[:0])
+    changes = [("needs", cut[part]), ("CUDA device", elsewhere(-1)), ("CUDA device", elsewhere(1))]
+    if part not in ("workspace", "status"):
+        changes += [("torch", lambda t: t.to(torch.float64)), ("torch", lambda t: t.to(torch.int16))]
+        changes += [("contiguous", lambda t: t.transpose(0, 1))]
+    for text, change in changes:
+        assert refuse(kv8.StrataError, text, lambda: tensors(**{part: change})) == L.ERR_LAYOUT, text
+
+
+def test_tensors_on_the_host_are_refused():
+    for where in (-1, None):
+        kw = dict(device=-1) if where else {n: elsewhere(-1) for n in ("codes",)}
+        assert refuse(kv8.StrataError, "CUDA device", lambda: tensors(**kw)) == L.ERR_LAYOUT
+
+
+@pytest.mark.parametrize("name,calls", [("k", ["append"]), ("v", ["append"]), ("q", ["select", "attend", "sparse"]), ("y", ["attend", "sparse"]),
+                                        ("picks", ["select", "sparse"]), ("sequence", None), ("start", None)])
+def test_calls_refuse_tensors_that_do_not_hold_their_argument(name, calls):
+    import torch
+    changes = [("needs", lambda t: t[:-1]), ("CUDA device", elsewhere(-1)), ("CUDA device", elsewhere(1)), ("torch", lambda t: t.to(torch.float16)),
+               ("torch", lambda t: t.to(torch.int64)), ("torch", lambda t: t.double()),
+               ("contiguous", lambda t: t.repeat(*[1] * (t.dim() - 1), 2)[..., ::2])]
+    for text, change in changes:
+        c, a = tensors(**{name: change})
+        for which, call in every_call(c, a).items():
+            if calls is None or which in calls:
+                assert refuse(kv8.StrataError, text, call) == L.ERR_LAYOUT, (which, text)
+            else:
+                call()
+        assert len(c.lib.made) == (4 - len(calls) if calls else 0)
+
+
+def test_rows_some_way_apart():
+    """row_stride says how far: of a view of longer rows, or of a tensor that has them whole; of nothing else."""
+    import torch
+    for change, stride, text in ((lambda t: t.repeat(1, 3)[:, 5:149], 432, None), (lambda t: t.repeat(1, 3), 432, None),
+                                 (lambda t: t.repeat(1, 3)[:, 5:149], 431, "apart"), (lambda t: t.repeat(1, 3)[:, 5:148], 432, "apart"),
+                                 (lambda t: t.repeat(1, 3)[:11, 5:149], 432, "apart"), (lambda t: t.repeat(3, 1)[::3], 432, None),
+                                 (lambda t: t.repeat(1, 2)[:, ::2], 288, "apart"), (lambda t: t.repeat(1, 3)[:11], 432, "needs"),
+                                 (lambda t: t, 145, "needs"), (lambda t: t.half().repeat(1, 3)[:, 5:149], 432, "torch"),
+                                 (lambda t: t.repeat(1, 3)[:, 5:149].unsqueeze(0), 432, "apart")):
+        c, a = tensors(k=change, v=change)
+        call = every_call(c, a, row_stride=stride)["append"]
+        if text is None:
+            call()
+            assert c.lib.made[0][1] == a["k"].data_ptr() and c.lib.made[0][3] == stride
+        else:
+            assert refuse(kv8.StrataError, text, call) == L.ERR_LAYOUT
+            assert not c.lib.made
+
+
+def test_addresses_and_tensors_mix():
+    """Addresses are the caller's word; tensors beside them are still looked at."""
+    c, a = tensors()
+    d = cache(kv_heads=2, dim=72, pages=17, sequences=3, blocks=5)
+    d.lib = Calls()
+    for call in every_call(d, a).values():
+        call()
+    every_call(c, dict.fromkeys(a, A))["sparse"]()
+    assert len(d.lib.made) == 4 and len(c.lib.made) == 1
+    a["q"] = a["q"].half()
+    assert refuse(kv8.StrataError, "torch", every_call(d, a)["attend"]) == L.ERR_LAYOUT
