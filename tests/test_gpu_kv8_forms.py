@@ -261,3 +261,89 @@ def test_value_scales_too_far_apart_are_reported():
     assert c.errors() == 0
     c.attend(q, heads, np.arange(sequences), np.full(sequences, n - 1))
     assert c.errors() == 32
+
+
+# ---------------------------------------------------------------- token steps on tcgen05, by heads and channels
+
+def _strided_attend(c, q, heads, sequence, start, picks=None, top=0, off=1):
+    """c.attend with queries in rows three floats longer than they need be, `off` floats past a 16-byte boundary."""
+    s, n = q.shape[:2]
+    w = heads * c.dim
+    wide = c.torch.zeros(s * n * (w + 3) + off, device="cuda")
+    rows = wide[off:].reshape(s * n, w + 3)
+    rows[:, :w] = c.torch.from_numpy(q.reshape(s * n, w)).cuda()
+    y = c.torch.full((s * n * w + 1,), float("nan"), device="cuda")[1:]
+    c.view.attend(rows, heads, y, c.i32(sequence), c.i32(start), s, n, None if picks is None else c.i32(picks), top, row_stride=w + 3)
+    return y.cpu().numpy().reshape(s, n, heads, c.dim)
+
+
+@pytest.mark.parametrize("heads,dim,blocks", [(3, 64, 45), (8, 40, 85), (11, 64, 310), (3, 128, 45), (7, 72, 60), (12, 128, 140), (16, 100, 600),
+                                              (4, 256, 40), (8, 256, 60), (10, 200, 90), (15, 256, 160)])
+def test_tokens_of_long_sessions_by_heads_and_channels(heads, dim, blocks):
+    """Pages of 40 sessions shared over the CTAs, for every width of the operands that a call of this kind takes: queries off the
+    16-byte grid, one that is not finite, blocks of zeros, garbage past each token's position and in the table past its block."""
+    kv, sequences = 1, 40
+    c = WideCache(kv, dim, sequences, blocks + 3, blocks)
+    rng = np.random.default_rng(dim + heads)
+    n = blocks * BLOCK - 21
+    k, v = rng.normal(0, 1, (2, n, kv, dim)).astype(np.float32)
+    for b in (1, 6, 7, blocks // 2):
+        k[b * BLOCK:(b + 1) * BLOCK] = 0
+        v[(b + 1) * BLOCK:(b + 2) * BLOCK] = 0
+    c.table[:, :blocks] = c.i32(rng.permutation(blocks))
+    c.table[:, blocks:] = c.i32([-1, 1 << 30, -7])
+    c.append(k[None], v[None], [0], [0])
+    last = int(c.table[0, blocks - 1])
+    c.codes[last, :, 0].reshape(kv, -1, BLOCK, 64)[:, :, n % BLOCK:] = -128
+    c.codes[last, :, 1].reshape(kv, -1, BLOCK)[:, :, n % BLOCK:] = 127
+    q = rng.normal(0, 1, (sequences, 1, heads, dim)).astype(np.float32)
+    start = n - 1 - 70 * np.arange(sequences) % (n // 2)
+    sequence = np.arange(sequences)
+    sequence[3], start[4] = -1, -1
+    want = _strided_attend(c, q, heads, sequence, start)
+    assert c.errors() == 0 and not want[3].any() and not want[4].any()
+    for s in (0, 1, 5, sequences - 1):
+        c.check_attend(want[s], q[s], k, v, start[s], 1 / math.sqrt(dim))
+    for bad in (np.nan, -np.inf):
+        p = q.copy()
+        p[5, 0, heads - 1, dim // 2] = bad
+        got = _strided_attend(c, p, heads, sequence, start, off=4)
+        assert np.isnan(got[5, 0, heads - 1]).all()
+        got[5, 0, heads - 1] = want[5, 0, heads - 1]
+        assert np.array_equal(got.view(np.uint32), want.view(np.uint32))
+    # a block whose page is none is left out and reported; others' tokens stay as they are
+    c.table[7, 2] = blocks
+    got = _strided_attend(c, q, heads, sequence, start)
+    assert c.errors() == 1
+    listed = np.setdiff1d(np.arange(blocks), [2])[None, None]
+    c.check_attend(got[7], q[7], k, v, start[7], 1 / math.sqrt(dim), listed)
+    assert np.array_equal(got[:7].view(np.uint32), want[:7].view(np.uint32))
+
+
+@pytest.mark.parametrize("heads,dim", [(3, 64), (8, 40), (11, 64), (16, 64), (3, 128), (7, 72), (12, 128), (16, 100), (4, 256), (8, 256), (12, 256),
+                                       (15, 200)])
+@pytest.mark.parametrize("picked", [True, False])
+def test_more_tokens_than_share_pages_by_heads_and_channels(heads, dim, picked):
+    """1200 tokens, each of whose units one CTA has whole: lists of picks with gaps, or all blocks of sessions of all lengths."""
+    kv, blocks, top, tokens = 1, 30, 7, 1200
+    c = WideCache(kv, dim, tokens, blocks, blocks)
+    rng = np.random.default_rng(dim + heads)
+    n = blocks * BLOCK
+    k, v = rng.normal(0, 1, (2, n, kv, dim)).astype(np.float32)
+    c.table[:] = c.i32(rng.permutation(blocks))
+    c.append(k[None], v[None], [0], [0])
+    q = rng.normal(0, 1, (tokens, 1, heads, dim)).astype(np.float32)
+    start, sequence, picks = rng.integers(0, n, tokens), np.arange(tokens), None
+    sequence[11], start[12], start[13] = -1, -1, 0
+    if picked:
+        picks = np.full((tokens, kv, top), -1)
+        for t in range(tokens):
+            some = np.sort(rng.permutation(max(start[t] // BLOCK + 1, 1))[:top])
+            picks[t, 0, rng.permutation(top)[:len(some)]] = some
+        picks[14] = -1
+    q[15, 0, 0, 0] = np.nan
+    got = _strided_attend(c, q, heads, sequence, start, picks, top if picked else 0)
+    assert c.errors() == 0
+    assert not got[11].any() and not got[12].any() and np.isnan(got[15, 0, 0]).all() and not np.isnan(np.delete(got, 15, 0)).any()
+    for t in list(range(0, tokens, 61)) + [13, 14, tokens - 1]:
+        c.check_attend(got[t], q[t], k, v, start[t], 1 / math.sqrt(dim), None if picks is None else picks[t][None])
