@@ -299,19 +299,22 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
  * append: scale = amax / 127 over a block's rows so far (0 below 2^-100), code = x times the
  *   reciprocal of scale, rounded to nearest even. A block's codes depend on its rows alone, not on how they
  *   were split over calls. Appending goes on where the sequence ends; a run that starts at a block's
- *   first token starts that block afresh, and one that starts inside the open block drops its rows from there on.
+ *   first token starts that block afresh, and one that starts inside the open block drops its rows from there on (a block
+ *   that has been filled is not open any more: only its first token starts it anew).
  *   A value that is not finite is stored as zero and reported. Runs of one call name different sequences.
  * select: for each token and key/value head the `top` blocks (of those at or before the token) with the
- *   largest bound on the summed logits of the group's queries, in ascending order, -1 past the last: i32
- *   picks [tokens][kv_heads][top]. The bound is sum_d p_d hi_d + n_d lo_d times the block's key scale, where hi, lo
+ *   largest score, in ascending order, -1 past the last: i32
+ *   picks [tokens][kv_heads][top]. The score is sum_d p_d hi_d + n_d lo_d times the block's key scale, where hi, lo
  *   are the marks and p, n the group's positive and negative query parts: queries are rounded to
  *   multiples of amax / 32767, added up as whole numbers and rounded to 8 bits, so that the choice does not
- *   depend on the order of any sum. The `first` first and `last` last blocks are always picked; equal
- *   bounds go to the lower block. A query value that is not finite counts as zero. Tables of at most
+ *   depend on the order of any sum. Without the rounding it is an upper bound on the summed logits of the group's queries;
+ *   rounding p and n moves it by half of sum_d |hi_d| + |lo_d| units at most. The `first` first and `last` last blocks
+ *   are always picked; equal scores go to the lower block. A query value that is not finite counts as zero. Tables of at most
  *   STRATA_KV8_SELECT_BLOCKS blocks.
  * attend: y [tokens][heads * dim] = softmax(scale * q . k) v over the keys at or before the token's position, of
  *   every block (picks null / 0) or of the blocks that picks [tokens][kv_heads][top] lists (distinct, -1 for
- *   none; top at most 33554431, the blocks that a table can have). Query head h uses key/value head h / (heads / kv_heads). A token that sees no key gets zeros.
+ *   none; top at most 33554431, the blocks that a table can have). Query head h uses key/value head
+ *   h / (heads / kv_heads). A token that sees no key gets zeros.
  *   F32 in and out. Queries and weights keep 22 bits or more of their row's largest (8-bit digits or two FP16
  *   halves, by the kernel's form) and meet the codes without rounding these; maxima, sums and results are F32 or wider.
  *   Prompt chunks keep weights times their page's value scale to 2^-31 of the row's largest such product; values of a page
@@ -322,7 +325,8 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
  * heads / kv_heads is any whole number, dim is 1 .. 256. A run that attends to every block has at most 2^31 - 128 rows
  * (count * heads / kv_heads). A sequence, page or position outside the cache
  * is skipped and reported by the next synchronising call (STRATA_ERR_DEVICE), or, in the pointer forms, by
- * bit 0 of *status (bit 4: a value that was not finite, bit 5: value scales too far apart), which the caller clears. */
+ * bit 0 of *status (bit 1: a bounded wait in a kernel ran out, bit 4: a value that was not finite, bit 5: value scales too
+ * far apart), which the caller clears. */
 #define STRATA_KV8_BLOCK 64
 #define STRATA_KV8_WORKSPACE_BYTES (32u << 20)
 #define STRATA_KV8_SELECT_BLOCKS 32768

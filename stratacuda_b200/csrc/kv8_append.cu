@@ -14,8 +14,8 @@ constexpr int kFew = 4;  // rows of a run, up to which it is worth trying to add
 // copied out whole. Bound by memory: 4 bytes read and 1 written a value.
 // A few rows added to an open block (decode) mostly leave its scale as it is; then all other codes stand and only the
 // new rows' and the marks are written, with the same result. Bound by the latency of the look-ups and of the open rows.
-// Measured at 2 heads of 256 channels: a prompt of 8191 tokens 15.5 us (2.7 TB/s; a CTA a block, kind and head is one
-// wave, so that loads and stores of a CTA do not overlap), 64 sessions' tokens 8.8 us, of which the host takes most.
+// Measured at 2 heads of 256 channels: a prompt of 8191 tokens 15.7 us (2.7 TB/s; 516 CTAs, a block, kind and head each, are
+// 1.2 waves, and loads and stores of a CTA do not overlap), 64 sessions' tokens 7.6 us (9 with the call, which the host bounds).
 template <int P, bool WIDE, bool FEW>
 __global__ void __launch_bounds__(kThreads) k_kv8_append(const Kv8 c, const float *k, const float *v, long long stride, const Kv8Runs runs) {
     constexpr int kTiles = P / 64;  // 4 tokens x 4 channels a tile, 16 * P / 4 tiles

@@ -18,9 +18,9 @@
 // keys and values by TMA (64-byte swizzle), ahead across units; one thread of 9 issues S, up to four steps ahead, one
 // of 11 O; 10 makes the next unit's query digits. One CTA a multiprocessor; every wait is bounded, and past the limit all leave.
 //
-// Measured: 64 sessions of up to 16384 tokens, 24 heads over 2 of 256 channels, 117 us, 4.7 TB/s of what has to be read; one
-// session of 200001 tokens, 32 heads over 8 of 128, 84 us, 4.9 TB/s. A step of two pages takes a group about 6000 clocks
-// and the two groups together 3000, in which memory could bring one and a third; copies alone run at 100 and 75 us.
+// Measured: 64 sessions of up to 16384 tokens, 24 heads over 2 of 256 channels, 115 us, 4.7 TB/s of what has to be read; one
+// session of 200001 tokens, 32 heads over 8 of 128, 85 us, 4.8 TB/s. In the first a CTA has 56 steps of two pages in 212
+// thousand clocks, 3800 a step with units' beginnings and ends; copies alone ran at 100 and 75 us.
 //
 // Few units (`split`): the pages of all units form one list that the CTAs share evenly, whatever the
 // lengths; a unit cut by a CTA border leaves unnormalised partial sums in the workspace and a

@@ -23,9 +23,9 @@
 // the products. So FP16's steps are 2^-31 of the row's largest product at most, also for rows that see only small scales.
 //
 // Measured: 2048 tokens over 16384 keys, 24 heads over 2 of 256 channels, 1365 us, 567 TFLOP/s of the two products as they
-// are defined (1287 us with the cache in L2), at a page about every 4200 clocks a CTA. S takes 1250 of them (24 instructions of 128 x 64 x 32, bound by
-// reading their operands from shared memory) and O 1000; the rest are the hand-overs between products and softmax, for
-// which TMEM has no second set of S's columns. The form with queries in FP16 halves and keys converted as well took
+// are defined, at a page every 3900 clocks a CTA (2.2 us), the tensor pipe busy for 47%. S alone takes 1250 clocks (24
+// instructions of 128 x 64 x 32, bound by reading their operands from shared memory) and O 1000; the rest are the hand-overs
+// between products and softmax, for which TMEM has no second set of S's columns at 256 channels. The form with queries in FP16 halves and keys converted as well took
 // 1546 us, since its converters and operands take twice the shared-memory traffic.
 //
 // Every wait is bounded; past the limit all roles leave and the error word is set.

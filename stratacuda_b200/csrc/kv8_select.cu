@@ -1,9 +1,9 @@
 // Choosing the blocks that a query attends to (strata_kv8_select).
 //
-// A block's bound for a token and key/value head is an integer product: the group's queries as two rows
+// A block's score for a token and key/value head is an integer product: the group's queries as two rows
 // of 8-bit codes (negative and positive parts) with the block's two rows of marks, 2 P terms, times the
-// block's key scale. Products and sums are whole numbers, so any order gives the same bound, and the
-// choice repeats exactly.
+// block's key scale: the upper bound that the marks give on the group's summed logits, but for the rounding of the codes
+// ("bound" below). Products and sums are whole numbers, so any order gives the same score, and the choice repeats exactly.
 //   * 16 tokens of a run (two such tiles a CTA) are the rows of an integer tensor-core tile (mma.sync m16n8k32) against 8 blocks a
 //     step, whose marks come from global memory in fragment order: 16 consecutive bytes are a lane's operands
 //     of two k-steps. One token alone pays for the tile but not for memory: each block's marks are read once.
@@ -11,7 +11,7 @@
 //     until exactly `top` of them lie above, which takes a dozen steps instead of 32 when few are equal.
 //   * few tokens: a cluster of up to 8 CTAs shares a token's blocks and sends the bounds to its first CTA.
 // Measured at 24 heads over 2 of 256 channels: 32 of 1024 blocks for 2048 tokens 47 us (90 T operations/s), bound by the search
-// among a token's bounds and by loading marks in fragment order; for 16 sessions 13 us, bound by latency.
+// among a token's bounds and by loading marks in fragment order; for 16 sessions 14 us, bound by latency.
 #include "../../include/strata_cuda.h"
 #include "kv8.cuh"
 

@@ -16,10 +16,10 @@
 // value row (tokens) are one lane's operands of four k-steps, the k order being the same on both sides.
 // The pages of all units form one list that the CTAs share evenly, as in the other form.
 //
-// Bound by latency, not by bytes: a page is a copy, a product, a softmax and a product one after the other, with three
+// Bound by latency, not by bytes: a page is a copy, a product, a softmax and a product one after the other, with two
 // block barriers (about 1.5 us a page and CTA), before that the look-ups and after it the joining kernel. Measured for
-// 24 query heads over 2 key/value heads of 256 channels: one session of 2048 tokens 14.4 us (18.6 by the other form),
-// 16 sessions with 32 picked blocks each 25.9 us (34.0), 1.2 TB/s.
+// 24 query heads over 2 key/value heads of 256 channels: one session of 2048 tokens 14.2 us (18.6 by the other form),
+// 16 sessions with 32 picked blocks each 24.8 us (34.0), 1.3 TB/s.
 #include "kv8_rows.cuh"
 
 #include <atomic>

@@ -179,6 +179,7 @@ class _Message(threading.local):
 
 
 _message = _Message()
+_pack = L.KV8_CALL.pack
 
 
 class DeviceCache:
@@ -209,7 +210,7 @@ class DeviceCache:
 
     def _call(self, rows, v, row_stride, sequence, start, picks, y, stream, op, segments, count, heads=0, top=0, first=0, last=0, scale=0.0) -> None:
         try:
-            call = L.KV8_CALL.pack(self._at, rows, v, row_stride, sequence, start, picks, y, stream, _message.at, 256, op, segments, count, heads,
+            call = _pack(self._at, rows, v, row_stride, sequence, start, picks, y, stream, _message.at, 256, op, segments, count, heads,
                                    top, first, last, scale)
         except (struct.error, OverflowError) as e:
             raise StrataRangeError(L.ERR_RANGE, f"an argument is not a number of its type: {e}") from None

@@ -291,3 +291,31 @@ def test_addresses_and_tensors_mix():
     assert len(d.lib.made) == 4 and len(c.lib.made) == 1
     a["q"] = a["q"].half()
     assert refuse(kv8.StrataError, "torch", every_call(d, a)["attend"]) == L.ERR_LAYOUT
+
+
+# ---------------------------------------------------------------- the selection's rounding
+
+@pytest.mark.parametrize("dim,group,blocks,top", [(256, 12, 1024, 32), (128, 4, 512, 16), (64, 1, 300, 8)])
+def test_rounded_scores_pick_what_the_marks_bound_picks(dim, group, blocks, top):
+    """Queries rounded to 8 bits choose at least 15 of 16 blocks that the bound itself would choose, with keys some of whose channels
+    are loud; and the bound is one: no block's summed logits pass it."""
+    import numpy as np
+
+    import kv8_reference as R
+    rng = np.random.default_rng(1)
+    loud, size = 1 + 3 * (rng.random(dim) < 0.06), np.exp(0.3 * rng.normal(size=(blocks, 1, 1)))
+    keys = (rng.normal(size=(blocks, 64, dim)) + rng.normal(size=(blocks, 1, dim))) * size * loud
+    scales = (np.abs(keys).max((1, 2)) / 127).astype(np.float32)
+    codes = np.clip(np.rint(keys / scales[:, None, None]), -127, 127)
+    lo, hi = codes.min(1), codes.max(1)
+    same = []
+    for _ in range(16):
+        q = rng.normal(size=(group, dim)).astype(np.float32)
+        bound = (hi @ np.maximum(q, 0).sum(0) + lo @ np.minimum(q, 0).sum(0)) * scales
+        logits = ((codes * scales[:, None, None]) @ q.T.astype(np.float64)).sum(-1)
+        assert (logits.max(1) <= bound * (1 + 1e-6) + 1e-6).all()
+        order = bound.copy()
+        order[:1] = order[-2:] = np.inf
+        want = np.argsort(-order, kind="stable")[:top]
+        same.append(np.isin(want, R.select(q, (lo, hi), scales, blocks, top, 1, 2)).mean())
+    assert np.mean(same) >= 15 / 16
