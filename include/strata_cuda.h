@@ -380,6 +380,116 @@ typedef struct {
 } strata_kv8_call;
 int strata_kv8_call_dev(const strata_kv8_call *call);
 
+/* ---- token mixers over runs of many sequences (no reference counterpart) ----
+ * The reference walks the delta rule token after token (kernels/strata.cu:304-313, :432-444) and dispatches its inputs and the
+ * queries and keys of attention in five steps each (src/engine.js, src/prefill.js). These entries take several tokens of
+ * several sequences in one call, single tokens and long prompts alike. F32 in and out, every sum in F32; results agree with the
+ * reference's entries to F32 rounding, not bit for bit.
+ *
+ * Runs. A call works on segments * count rows, `count` for each of `segments` runs; run i belongs to sequence[i], and has
+ * lengths[i] tokens (lengths null / 0: count each). Both are read on the device, so a captured graph can replay a call. Rows
+ * behind a run's tokens are left as they were. sequence -1 marks an idle slot: its rows become zero, what it holds stays. Runs
+ * of one call name different sequences: one that an earlier run has too is reported and treated as idle. Rows of x, q, k and v
+ * are `..._stride` floats apart (0: contiguous); results are contiguous and do not overlap what is read.
+ *
+ * delta_inputs: from a layer's [q | k | v] projection x [rows][channels], channels = (2 key_heads + value_heads) * dim, a causal
+ *   convolution of each channel, c_t = sum_m weight[c][m] x_{t - (taps - 1) + m}, which goes on from the sequence's last
+ *   taps - 1 inputs (history, oldest first) and leaves the new ones there; s = c / (1 + exp(-c)); for each head of q and k
+ *   s / sqrt(sum s^2 + epsilon), q's times q_scale (0: 1 / sqrt(dim)); v = s.
+ * delta_rule: with the state S [dim key][dim value] of each value head of the run's sequence, token after token
+ *     S <- decay S;  d = beta (v - S^T k);  S <- S + k d^T;  y = S^T q
+ *   Value head h reads key head h % key_heads. decay, beta [rows][value_heads]; y [rows][value_heads * dim]. Runs of many
+ *   tokens are taken in chunks of 64 on the tensor cores: factors keep 22 bits of what is largest in their row or tile, sums
+ *   are F32. A chunk in which a value is not finite (or past 2^60 in magnitude) is walked token by token, so that no token before it
+ *   sees it.
+ * qk_rope: for each head of q and k x / sqrt(mean x^2 + epsilon) times the kind's weight [dim], its first `rotary` channels
+ *   rotated (channel d with d + rotary / 2) by the row start[i] + j of cos and sin [cells][rotary / 2], as strata_norm and then
+ *   strata_rope_position. Heads of q may lie q_head_stride floats apart (0: dim), as in a projection of [q | gate] for each head.
+ *   A position outside the tables gives a row of zeros and is reported. sequence may be null / 0: no idle slots. y may be what is
+ *   read where that is contiguous.
+ *
+ * dim is 1 .. 256 and value_heads a multiple of key_heads; taps is 1 .. 8. The workspace is scratch of delta_rule of
+ * STRATA_DELTA_WORKSPACE_BYTES; calls that may overlap on the GPU need workspaces of their own, calls that follow one another on
+ * a stream may share one. A sequence outside [-1, sequences), a length outside [0, count] or a position outside the tables is
+ * reported by the next synchronising call (STRATA_ERR_DEVICE), or, in the pointer forms, by bit 0 of *status (bit 1: a bounded
+ * wait in a kernel ran out), which the caller clears. */
+#define STRATA_DELTA_WORKSPACE_BYTES (128u << 20)
+typedef struct {
+    int32_t key_heads, value_heads, dim, taps, sequences;
+    strata_buf state;     /* f32 [sequences][dim key][value_heads][dim value]; delta_rule */
+    strata_buf history;   /* f32 [sequences][channels][taps - 1]; delta_inputs with taps > 1 */
+    strata_buf weight;    /* f32 [channels][taps]; delta_inputs */
+    strata_buf workspace; /* delta_rule */
+} strata_delta_net;
+int strata_delta_inputs(strata_ctx *ctx, const strata_delta_net *net, strata_buf x, uint64_t row_stride, int32_t segments, int32_t count,
+                        strata_buf sequence, strata_buf lengths, float q_scale, float epsilon, strata_buf q, strata_buf k, strata_buf v);
+int strata_delta_rule(strata_ctx *ctx, const strata_delta_net *net, strata_buf q, uint64_t q_stride, strata_buf k, uint64_t k_stride,
+                      strata_buf v, uint64_t v_stride, strata_buf decay, strata_buf beta, int32_t segments, int32_t count,
+                      strata_buf sequence, strata_buf lengths, strata_buf y);
+typedef struct {
+    int32_t heads, kv_heads, dim, rotary, cells, sequences;
+    strata_buf q_weight, k_weight; /* f32 [dim] */
+    strata_buf cos, sin;           /* f32 [cells][rotary / 2]; ignored where rotary is 0 */
+} strata_qk_rope_weights;
+int strata_qk_rope(strata_ctx *ctx, const strata_qk_rope_weights *weights, strata_buf q, uint64_t q_stride, uint64_t q_head_stride,
+                   strata_buf k, uint64_t k_stride, int32_t segments, int32_t count, strata_buf sequence, strata_buf start,
+                   strata_buf lengths, float epsilon, strata_buf yq, strata_buf yk);
+/* The same on caller-owned device memory and a stream (a cudaStream_t as void*; NULL = the default stream) of the calling
+ * thread's current device, with the arguments in a structure. Nothing is allocated. The workspace starts on a 128-byte boundary,
+ * everything else on its element's. `status` (optional) is a device word that errors are added to; `msg` (optional) receives
+ * the reason for a non-zero return. */
+typedef struct {
+    int32_t key_heads, value_heads, dim, taps, sequences;
+    float *state, *history;
+    const float *weight;
+    void *workspace;
+    uint32_t *status;
+} strata_delta_net_dev;
+typedef struct {
+    const strata_delta_net_dev *net;
+    const float *x;
+    uint64_t row_stride;
+    const int32_t *sequence, *lengths;
+    float *q, *k, *v;
+    void *stream;
+    char *msg;
+    uint64_t msg_cap;
+    int32_t segments, count;
+    float q_scale, epsilon;
+} strata_delta_inputs_call;
+typedef struct {
+    const strata_delta_net_dev *net;
+    const float *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride;
+    const float *decay, *beta;
+    const int32_t *sequence, *lengths;
+    float *y;
+    void *stream;
+    char *msg;
+    uint64_t msg_cap;
+    int32_t segments, count;
+} strata_delta_rule_call;
+typedef struct {
+    int32_t heads, kv_heads, dim, rotary, cells, sequences;
+    const float *q_weight, *k_weight, *cos, *sin;
+    uint32_t *status;
+} strata_qk_rope_weights_dev;
+typedef struct {
+    const strata_qk_rope_weights_dev *weights;
+    const float *q, *k;
+    uint64_t q_stride, q_head_stride, k_stride;
+    const int32_t *sequence, *start, *lengths;
+    float *yq, *yk;
+    void *stream;
+    char *msg;
+    uint64_t msg_cap;
+    int32_t segments, count;
+    float epsilon;
+} strata_qk_rope_call;
+int strata_delta_inputs_dev(const strata_delta_inputs_call *call);
+int strata_delta_rule_dev(const strata_delta_rule_call *call);
+int strata_qk_rope_dev(const strata_qk_rope_call *call);
+
 /* ---- CUDA graphs of the context's stream (no reference counterpart: the B200 runtime replays
  * captured work instead of relaunching it from the host) ----
  * strata_capture_begin starts capturing the context's stream (thread-local mode): the calls

@@ -54,6 +54,33 @@ class StrataKv8CacheDev(C.Structure):
                 ("workspace", C.c_void_p), ("status", C.c_void_p)]
 
 
+DELTA_WORKSPACE_BYTES = 128 << 20
+DELTA_INPUTS_CALL = struct.Struct("@11Q2i2f")  # strata_delta_inputs_call: net .. v, stream, msg, msg_cap; segments, count; q_scale, epsilon
+DELTA_RULE_CALL = struct.Struct("@15Q2i")  # strata_delta_rule_call: net .. stream, msg, msg_cap; segments, count
+QK_ROPE_CALL = struct.Struct("@14Q2if")  # strata_qk_rope_call: weights .. stream, msg, msg_cap; segments, count; epsilon
+
+
+class StrataDeltaNet(C.Structure):
+    _fields_ = [("key_heads", C.c_int32), ("value_heads", C.c_int32), ("dim", C.c_int32), ("taps", C.c_int32), ("sequences", C.c_int32),
+                ("state", C.c_uint64), ("history", C.c_uint64), ("weight", C.c_uint64), ("workspace", C.c_uint64)]
+
+
+class StrataDeltaNetDev(C.Structure):
+    _fields_ = [("key_heads", C.c_int32), ("value_heads", C.c_int32), ("dim", C.c_int32), ("taps", C.c_int32), ("sequences", C.c_int32),
+                ("state", C.c_void_p), ("history", C.c_void_p), ("weight", C.c_void_p), ("workspace", C.c_void_p), ("status", C.c_void_p)]
+
+
+class StrataQkRopeWeights(C.Structure):
+    _fields_ = [("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("rotary", C.c_int32), ("cells", C.c_int32),
+                ("sequences", C.c_int32), ("q_weight", C.c_uint64), ("k_weight", C.c_uint64), ("cos", C.c_uint64), ("sin", C.c_uint64)]
+
+
+class StrataQkRopeWeightsDev(C.Structure):
+    _fields_ = [("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("rotary", C.c_int32), ("cells", C.c_int32),
+                ("sequences", C.c_int32), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("cos", C.c_void_p), ("sin", C.c_void_p),
+                ("status", C.c_void_p)]
+
+
 SIGNATURES = {
     "strata_create": ([_i, C.POINTER(_vp)], _i),
     "strata_destroy": ([_vp], _i),
@@ -100,6 +127,15 @@ SIGNATURES = {
     "strata_kv8_attend_dev": ([C.POINTER(StrataKv8CacheDev), _vp, _u64, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_int32,
                                C.c_float, _vp, _vp, C.c_char_p, _sz], _i),
     "strata_kv8_call_dev": ([C.c_char_p], _i),
+    "strata_delta_inputs": ([_vp, C.POINTER(StrataDeltaNet), _u64, _u64, C.c_int32, C.c_int32, _u64, _u64, C.c_float, C.c_float, _u64, _u64,
+                             _u64], _i),
+    "strata_delta_rule": ([_vp, C.POINTER(StrataDeltaNet), _u64, _u64, _u64, _u64, _u64, _u64, _u64, _u64, C.c_int32, C.c_int32, _u64, _u64,
+                           _u64], _i),
+    "strata_qk_rope": ([_vp, C.POINTER(StrataQkRopeWeights), _u64, _u64, _u64, _u64, _u64, C.c_int32, C.c_int32, _u64, _u64, _u64, C.c_float,
+                        _u64, _u64], _i),
+    "strata_delta_inputs_dev": ([C.c_char_p], _i),
+    "strata_delta_rule_dev": ([C.c_char_p], _i),
+    "strata_qk_rope_dev": ([C.c_char_p], _i),
     "strata_synth_blobs": ([_vp, _u64, _u64, _u64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32], _i),
     "strata_synth_normals": ([_vp, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _d], _i),
 }

@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdlib>
 #include <cstdio>
+#include <initializer_list>
 #include <cstring>
 #include <mutex>
 #include <cmath>
@@ -17,6 +18,7 @@
 #include "../../include/strata_cuda.h"
 #include "kernels.h"
 #include "kv8.h"
+#include "mixers.h"
 
 using namespace strata;
 
@@ -458,6 +460,45 @@ int kv8_rows(strata_ctx *ctx, const char *what, strata_buf h, uint64_t *stride, 
     return kv8_buffer(ctx, what, h, (tokens - 1) * (long long)*stride + width, out);
 }
 
+// ---- token mixers: handles to the device views the kernels take
+struct MixNeed {
+    const char *what;
+    strata_buf h;
+    long long need;  // elements
+    void **out;
+    bool optional;   // 0 stands for null
+};
+int mix_buffers(strata_ctx *ctx, std::initializer_list<MixNeed> all) {
+    for (const MixNeed &n : all) {
+        *n.out = nullptr;
+        if (n.optional && !n.h) continue;
+        Buffer *b = find(ctx, n.h);
+        if (!b) return fail(ctx, STRATA_ERR_HANDLE, "%s is not a live buffer", n.what);
+        if ((long long)b->length < n.need)
+            return fail(ctx, STRATA_ERR_LAYOUT, "%s needs %lld elements, the buffer has %llu", n.what, n.need, (unsigned long long)b->length);
+        *n.out = b->ptr;
+    }
+    return STRATA_OK;
+}
+int mix_stride(strata_ctx *ctx, const char *what, uint64_t *stride, long long width) {
+    if (!*stride) *stride = (uint64_t)width;
+    char msg[256];
+    if (int e = mix_check_stride(what, *stride > (1ull << 38) ? -1 : (long long)*stride, width, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    return STRATA_OK;
+}
+// The geometry and the runs of a delta-rule call; its buffers follow.
+int delta_view(strata_ctx *ctx, const strata_delta_net *net, int segments, int count, strata_buf sequence, strata_buf lengths, DeltaNet *n, MixRuns *r) {
+    if (!net) return fail(ctx, STRATA_ERR_RANGE, "null net");
+    char msg[256];
+    if (int e = delta_check(net->key_heads, net->value_heads, net->dim, net->taps, net->sequences, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = mix_check_runs(segments, count, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    *n = DeltaNet{net->key_heads, net->value_heads, net->dim, net->taps, net->sequences, nullptr, nullptr, nullptr, nullptr, ctx->err_dev};
+    *r = MixRuns{segments, count, nullptr, nullptr};
+    if (int e = mix_buffers(ctx, {{"sequence", sequence, segments, (void **)&r->sequence, false}, {"lengths", lengths, segments, (void **)&r->lengths, true}}))
+        return e;
+    return use_device(ctx);
+}
+
 }  // namespace
 
 extern "C" {
@@ -708,6 +749,94 @@ int strata_ple_gather_decode(strata_ctx *ctx, strata_buf table, strata_buf ids, 
     cudaError_t e = ple_gather_decode((const unsigned *)t->ptr, (long long)t->length, (const int *)d->ptr, (long long)d->length, rows, head_dim,
                                       (float *)v->ptr, (long long)v->length, ctx->stream, ctx->err_dev);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_ple_gather_decode");
+    return STRATA_OK;
+}
+
+int strata_delta_inputs(strata_ctx *ctx, const strata_delta_net *net, strata_buf x, uint64_t row_stride, int32_t segments, int32_t count,
+                        strata_buf sequence, strata_buf lengths, float q_scale, float epsilon, strata_buf q, strata_buf k, strata_buf v) {
+    if (!ctx) return STRATA_ERR_RANGE;
+    DeltaNet n;
+    MixRuns r;
+    if (int e = delta_view(ctx, net, segments, count, sequence, lengths, &n, &r)) return e;
+    char msg[256];
+    if (int e = mix_check_numbers(q_scale, epsilon, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = mix_stride(ctx, "row_stride", &row_stride, n.channels())) return e;
+    const long long rows = (long long)segments * count, kd = (long long)n.key_heads * n.dim, vd = (long long)n.value_heads * n.dim;
+    DeltaInputs a{nullptr, (long long)row_stride, q_scale, epsilon, nullptr, nullptr, nullptr};
+    if (int e = mix_buffers(ctx, {{"x", x, (rows - 1) * a.row_stride + n.channels(), (void **)&a.x, false},
+                                  {"q", q, rows * kd, (void **)&a.q, false},
+                                  {"k", k, rows * kd, (void **)&a.k, false},
+                                  {"v", v, rows * vd, (void **)&a.v, false},
+                                  {"weight", net->weight, n.channels() * n.taps, (void **)&n.weight, false},
+                                  {"history", net->history, n.sequences * n.channels() * (n.taps - 1), (void **)&n.history, n.taps == 1}}))
+        return e;
+    cudaError_t e = delta_inputs(n, a, r, ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_delta_inputs");
+    ++ctx->dispatches;
+    return STRATA_OK;
+}
+
+int strata_delta_rule(strata_ctx *ctx, const strata_delta_net *net, strata_buf q, uint64_t q_stride, strata_buf k, uint64_t k_stride,
+                      strata_buf v, uint64_t v_stride, strata_buf decay, strata_buf beta, int32_t segments, int32_t count,
+                      strata_buf sequence, strata_buf lengths, strata_buf y) {
+    if (!ctx) return STRATA_ERR_RANGE;
+    DeltaNet n;
+    MixRuns r;
+    if (int e = delta_view(ctx, net, segments, count, sequence, lengths, &n, &r)) return e;
+    const long long rows = (long long)segments * count, kd = (long long)n.key_heads * n.dim, vd = (long long)n.value_heads * n.dim;
+    if (int e = mix_stride(ctx, "q_stride", &q_stride, kd)) return e;
+    if (int e = mix_stride(ctx, "k_stride", &k_stride, kd)) return e;
+    if (int e = mix_stride(ctx, "v_stride", &v_stride, vd)) return e;
+    DeltaRule a{nullptr, nullptr, nullptr, nullptr, nullptr, (long long)q_stride, (long long)k_stride, (long long)v_stride, nullptr};
+    if (int e = mix_buffers(ctx, {{"q", q, (rows - 1) * a.q_stride + kd, (void **)&a.q, false},
+                                  {"k", k, (rows - 1) * a.k_stride + kd, (void **)&a.k, false},
+                                  {"v", v, (rows - 1) * a.v_stride + vd, (void **)&a.v, false},
+                                  {"decay", decay, rows * n.value_heads, (void **)&a.decay, false},
+                                  {"beta", beta, rows * n.value_heads, (void **)&a.beta, false},
+                                  {"y", y, rows * vd, (void **)&a.y, false},
+                                  {"state", net->state, n.sequences * n.dim * vd, (void **)&n.state, false},
+                                  {"workspace", net->workspace, STRATA_DELTA_WORKSPACE_BYTES / 4, &n.workspace, false}}))
+        return e;
+    cudaError_t e = delta_rule(n, a, r, ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_delta_rule");
+    ++ctx->dispatches;
+    return STRATA_OK;
+}
+
+int strata_qk_rope(strata_ctx *ctx, const strata_qk_rope_weights *w, strata_buf q, uint64_t q_stride, uint64_t q_head_stride, strata_buf k,
+                   uint64_t k_stride, int32_t segments, int32_t count, strata_buf sequence, strata_buf start, strata_buf lengths, float epsilon,
+                   strata_buf yq, strata_buf yk) {
+    if (!ctx) return STRATA_ERR_RANGE;
+    if (!w) return fail(ctx, STRATA_ERR_RANGE, "null weights");
+    char msg[256];
+    if (int e = qk_check(w->heads, w->kv_heads, w->dim, w->rotary, w->cells, sequence ? w->sequences : 1, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = mix_check_runs(segments, count, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = mix_check_numbers(0, epsilon, msg, sizeof msg)) return fail(ctx, e, "%s", msg);
+    if (int e = mix_stride(ctx, "q_head_stride", &q_head_stride, w->dim)) return e;
+    if (q_head_stride > (1ull << 24)) return fail(ctx, STRATA_ERR_LAYOUT, "q_head_stride is out of range");
+    const long long reach = (w->heads - 1) * (long long)q_head_stride + w->dim;  // from a row's first head to the end of its last
+    if (int e = mix_stride(ctx, "q_stride", &q_stride, q_stride ? reach : w->heads * (long long)q_head_stride)) return e;
+    if (int e = mix_stride(ctx, "k_stride", &k_stride, (long long)w->kv_heads * w->dim)) return e;
+    const long long rows = (long long)segments * count, table = (long long)w->cells * (w->rotary / 2);
+    QkRope n{w->heads, w->kv_heads, w->dim, w->rotary, w->cells, w->sequences, nullptr, nullptr, nullptr, nullptr, ctx->err_dev};
+    QkRopeRows a{nullptr, nullptr, (long long)q_stride, (long long)q_head_stride, (long long)k_stride, nullptr, epsilon, nullptr, nullptr};
+    MixRuns r{segments, count, nullptr, nullptr};
+    if (int e = mix_buffers(ctx, {{"q", q, (rows - 1) * a.q_stride + reach, (void **)&a.q, false},
+                                  {"k", k, (rows - 1) * a.k_stride + (long long)w->kv_heads * w->dim, (void **)&a.k, false},
+                                  {"yq", yq, rows * w->heads * w->dim, (void **)&a.yq, false},
+                                  {"yk", yk, rows * w->kv_heads * w->dim, (void **)&a.yk, false},
+                                  {"sequence", sequence, segments, (void **)&r.sequence, true},
+                                  {"start", start, segments, (void **)&a.start, false},
+                                  {"lengths", lengths, segments, (void **)&r.lengths, true},
+                                  {"q_weight", w->q_weight, w->dim, (void **)&n.q_weight, false},
+                                  {"k_weight", w->k_weight, w->dim, (void **)&n.k_weight, false},
+                                  {"cos", w->cos, table, (void **)&n.cos, w->rotary == 0},
+                                  {"sin", w->sin, table, (void **)&n.sin, w->rotary == 0}}))
+        return e;
+    if (int e = use_device(ctx)) return e;
+    cudaError_t e = qk_rope(n, a, r, ctx->stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "strata_qk_rope");
+    ++ctx->dispatches;
     return STRATA_OK;
 }
 
