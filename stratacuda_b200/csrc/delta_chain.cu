@@ -1,0 +1,347 @@
+// The chunked delta rule's second kernel: a run's state of one value head, from chunk to chunk (delta_chunk.cuh).
+//
+// A block has a run's value head. A thread of its eight working warps has a value channel (its TMEM lane) with half of the
+// state's keys, in F32 registers; the state and the differences go to TMEM as the products' 128-row operand straight from
+// there, and what kernel one left comes through bulk copies as the narrow one:
+//   Z^T = S^T W^T,  R^T = S^T Q^T        128 value channels by 64 tokens, sums over keys
+//   D = U - Z;  new state's part = (E D)^T K        128 by D keys, sums over tokens; K's tile read the other way round
+//   Y^T = D^T G^T;  y = P R + Y          128 by 64 tokens
+// One warp fetches, one issues; results of a chunk are written while the next one's first product runs.
+#include "delta_chunk.cuh"
+
+#include <atomic>
+
+namespace strata {
+namespace {
+
+using namespace delta;
+
+constexpr int kWork = 256, kChainThreads = kWork + 64, kFetchWarp = 8, kIssueWarp = 9;
+
+template <int D>
+struct __align__(1024) ChainSmem {
+    unsigned char w[2][2 * D / 64][64 * 128];  // by stage: hi panels, lo panels
+    unsigned char q[2][2 * D / 64][64 * 128];
+    unsigned char k[2][2 * D / 64][64 * 128];
+    unsigned char g[2][64 * 128];  // hi, lo
+    DeltaFactors factors[2];
+    float s_max[2][128];
+    float2 d_max[2][128];
+    float2 walk[2][128];
+    unsigned long long w_full[2], w_empty[2], q_full[2], q_empty[2], k_full[2], k_empty[2], f_full[2], f_empty[2], g_full, g_empty;
+    unsigned long long s_ready, r_free, d_ready, y_ready, z_done, r_done, d_done, y_done;
+    unsigned tmem;
+    int abort_flag;
+};
+
+__device__ __forceinline__ void pair_sync(int w4) { asm volatile("bar.sync %0, 64;" ::"r"(1 + w4) : "memory"); }
+__device__ __forceinline__ void work_sync() { asm volatile("bar.sync 5, 256;" ::: "memory"); }
+
+template <int D>
+__global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
+    using Slot = DeltaSlot<D>;
+    constexpr int kPanels = D / 64, kHalf = D / 2;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    ChainSmem<D> &M = *reinterpret_cast<ChainSmem<D> *>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    kv8_enter();
+    const int m = (int)(blockIdx.x % slab.ratio), head_l = (int)(blockIdx.x / slab.ratio % slab.heads), run_l = (int)(blockIdx.x / slab.ratio / slab.heads);
+    const int h = slab.head0 + head_l + m * n.key_heads, run = slab.run0 + run_l;
+    const MixRun me = mix_run_alone(r, n.sequences, run, n.err);
+    const long long first = (long long)run * r.count, vw = (long long)n.value_heads * n.dim;
+    const int begin = slab.chunk0 * kChunk;
+    if (me.sequence < 0) {
+        const long long end = min((long long)r.count, (long long)begin + (long long)slab.chunks * kChunk), rows = end - begin;
+        for (long long i = tid; i < rows * n.dim; i += kChainThreads) A.y[(first + begin + i / n.dim) * vw + (long long)h * n.dim + i % n.dim] = 0.0f;
+        return;
+    }
+    if (begin >= me.tokens) return;
+    const int chunks = min(slab.chunks, (me.tokens - begin + kChunk - 1) / kChunk);
+    const unsigned char *slots = slab.slots + ((long long)run_l * slab.heads + head_l) * slab.chunks * slab.slot_bytes;
+    const long long mine = Slot::heads + (long long)m * Slot::head_bytes;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&M.w_full[i], 1), bar_init(&M.w_empty[i], 1), bar_init(&M.q_full[i], 1), bar_init(&M.q_empty[i], 1);
+            bar_init(&M.k_full[i], 1), bar_init(&M.k_empty[i], 1), bar_init(&M.f_full[i], 1), bar_init(&M.f_empty[i], kWork / 32 + 1);
+        }
+        bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
+        bar_init(&M.s_ready, kWork / 32), bar_init(&M.r_free, kWork / 32), bar_init(&M.d_ready, kWork / 32), bar_init(&M.y_ready, kWork / 32);
+        bar_init(&M.z_done, 1), bar_init(&M.r_done, 1), bar_init(&M.d_done, 1), bar_init(&M.y_done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        M.abort_flag = 0;
+    }
+    if (warp == kIssueWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&M.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = M.tmem;
+    // columns: the state's halves, under whose place Y's operand goes once R has been formed; E D's; Z, R, Y, the new state's part
+    constexpr unsigned kS = 0, kSLo = D / 2, kD = 128, kZ = 192, kR = 256, kY = 320, kNew = 384;
+    const Waits wait{&M.abort_flag, n.err};
+
+    if (warp == kFetchWarp) {
+        if (lane == 0) {
+            const auto fetch = [&](void *to, const unsigned char *from, unsigned bytes, unsigned long long *full) {
+                bar_expect(full, bytes);
+                bulk(to, from, bytes, full);
+            };
+            for (int c = 0; c < chunks; ++c) {
+                const int st = c & 1;
+                const unsigned again = (c >> 1 & 1) ^ 1;
+                const unsigned char *slot = slots + c * slab.slot_bytes;
+                wait(&M.f_empty[st], again);
+                fetch(&M.factors[st], slot + mine + Slot::factors, sizeof(DeltaFactors), &M.f_full[st]);
+                wait(&M.w_empty[st], again);
+                fetch(M.w[st], slot + mine + Slot::w, Slot::tile, &M.w_full[st]);
+                wait(&M.q_empty[st], again);
+                fetch(M.q[st], slot + Slot::q, Slot::tile, &M.q_full[st]);
+                wait(&M.k_empty[st], again);
+                fetch(M.k[st], slot + Slot::k, Slot::tile, &M.k_full[st]);
+                wait(&M.g_empty, (c & 1) ^ 1);
+                fetch(M.g, slot + mine + Slot::g, Slot::attn, &M.g_full);
+            }
+        }
+        __syncwarp();
+    } else if (warp == kIssueWarp) {
+        if (elect_one()) {
+            unsigned live = 0;  // chunks on the tensor cores so far
+            for (int c = 0; c < chunks; ++c) {
+                const int st = c & 1;
+                const unsigned ph = c >> 1 & 1;
+                wait(&M.f_full[st], ph);
+                const bool walk = M.factors[st].walk != 0;
+                bar_arrive(&M.f_empty[st]);
+                if (walk) {  // nothing of it is used
+                    wait(&M.w_full[st], ph), wait(&M.q_full[st], ph), wait(&M.k_full[st], ph), wait(&M.g_full, c & 1);
+                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.q_empty[st]), bar_arrive(&M.k_empty[st]), bar_arrive(&M.g_empty);
+                    continue;
+                }
+                const unsigned now = live & 1;
+                ++live;
+                wait(&M.w_full[st], ph);
+                wait(&M.s_ready, now);
+                tc_fence_after();
+#pragma unroll
+                for (int product = 0; product < 3; ++product)  // lo hi, hi lo, hi hi
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_f16_ts(tmem + kZ, tmem + (product == 0 ? kSLo : kS) + k * 8,
+                                   sw128_desc(su32(M.w[st][(product == 1 ? kPanels : 0) + k / 4])) + k % 4 * 2, idesc_f16(128, 64), product || k);
+                mma_commit(&M.w_empty[st]);
+                mma_commit(&M.z_done);
+                wait(&M.q_full[st], ph);
+                wait(&M.r_free, now);
+                tc_fence_after();
+#pragma unroll
+                for (int product = 0; product < 3; ++product)
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8,
+                                   sw128_desc(su32(M.q[st][(product == 1 ? kPanels : 0) + k / 4])) + k % 4 * 2, idesc_f16(128, 64), product || k);
+                mma_commit(&M.q_empty[st]);
+                mma_commit(&M.r_done);
+                wait(&M.k_full[st], ph);
+                wait(&M.d_ready, now);
+                tc_fence_after();
+#pragma unroll
+                for (int product = 0; product < 3; ++product)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f16_ts(tmem + kNew, tmem + kD + (product == 0) * 32 + k * 8,
+                                   turned_desc(su32(M.k[st][product == 1 ? kPanels : 0]) + k * 2048, 8192), turned_idesc(128, D), product || k);
+                mma_commit(&M.k_empty[st]);
+                mma_commit(&M.d_done);
+                wait(&M.g_full, c & 1);
+                wait(&M.y_ready, now);
+                tc_fence_after();
+#pragma unroll
+                for (int product = 0; product < 3; ++product)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f16_ts(tmem + kY, tmem + kS + (product == 0) * 32 + k * 8, sw128_desc(su32(M.g[product == 1])) + k * 2, idesc_f16(128, 64),
+                                   product || k);
+                mma_commit(&M.g_empty);
+                mma_commit(&M.y_done);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int w4 = warp & 3, half = warp >> 2, v = w4 * 32 + lane;
+        const unsigned lanes = tmem + ((unsigned)(w4 * 32) << 16);
+        const bool in = v < n.dim;
+        const auto arrive = [&](unsigned long long *b) {
+            __syncwarp();
+            if (lane == 0) bar_arrive(b);
+        };
+        float *state = n.state + ((long long)me.sequence * n.dim + half * kHalf) * vw + (long long)h * n.dim + v;
+        float S[kHalf];
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i) S[i] = in && half * kHalf + i < n.dim ? state[i * vw] : 0.0f;
+        unsigned live = 0;
+        bool owed = false;            // the chunk before has results in TMEM
+        float inv_r = 0, inv_y = 0;   // their scales taken back
+        // results of chunk c: its tokens half * 32 ..
+        const auto write_y = [&](int c) {
+            const DeltaFactors &f = M.factors[c & 1];
+            float R[32], Y[32];
+            tmem_read(lanes + kR + half * 32, R);
+            tmem_read(lanes + kY + half * 32, Y);
+            const int t0 = begin + c * kChunk + half * 32;
+            float *y = A.y + (first + t0) * vw + (long long)h * n.dim + v;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float value = R[i] * inv_r * f.q[half * 32 + i] + Y[i] * inv_y * f.attn[half * 32 + i];
+                if (in && t0 + i < me.tokens) y[i * vw] = value;
+            }
+            arrive(&M.f_empty[c & 1]);
+        };
+        for (int c = 0; c < chunks; ++c) {
+            const int st = c & 1;
+            const unsigned char *slot = slots + c * slab.slot_bytes;
+            wait(&M.f_full[st], c >> 1 & 1);
+            const DeltaFactors &f = M.factors[st];
+            if (owed) wait(&M.y_done, (live - 1) & 1), tc_fence_after();
+            if (f.walk) {
+                if (owed) write_y(c - 1);
+                owed = false;
+                // token by token: a channel's two threads add up their halves of the keys
+                const int t0 = begin + c * kChunk, tokens = min(kChunk, me.tokens - t0);
+                for (int t = 0; t < tokens; ++t) {
+                    const long long row = first + t0 + t;
+                    const float *kp = A.k + row * A.k_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
+                    const float *qp = A.q + row * A.q_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
+                    const float a = A.decay[row * n.value_heads + h], b = A.beta[row * n.value_heads + h];
+                    const float value = in ? A.v[row * A.v_stride + (long long)h * n.dim + v] : 0.0f;
+                    float p = 0.0f, y = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kHalf; ++i) {
+                        S[i] *= a;
+                        p = fmaf(S[i], half * kHalf + i < n.dim ? kp[i] : 0.0f, p);
+                    }
+                    M.walk[half][v].x = p;
+                    pair_sync(w4);
+                    const float d = b * (value - (M.walk[0][v].x + M.walk[1][v].x));
+#pragma unroll
+                    for (int i = 0; i < kHalf; ++i) {
+                        if (half * kHalf + i < n.dim) {
+                            S[i] = fmaf(kp[i], d, S[i]);
+                            y = fmaf(S[i], qp[i], y);
+                        }
+                    }
+                    M.walk[half][v].y = y;
+                    pair_sync(w4);
+                    if (half == 0 && in) A.y[row * vw + (long long)h * n.dim + v] = M.walk[0][v].y + M.walk[1][v].y;
+                }
+                arrive(&M.f_empty[st]);
+                continue;
+            }
+            const unsigned now = live & 1;
+            ++live;
+            float u[32];
+            const float *up = reinterpret_cast<const float *>(slot + mine + Slot::uu) + half * 32 * D + (v < D ? v : 0);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = __ldcg(up + i * D);
+            // the state as an operand
+            M.s_max[half][v] = largest(S);
+            pair_sync(w4);
+            const int es = exponent_of(__uint_as_float(max(__float_as_uint(M.s_max[0][v]), __float_as_uint(M.s_max[1][v]))));
+            const float inv_s = unscale_of(es);
+            {
+                unsigned hi[kHalf / 2], lo[kHalf / 2];
+                split(S, scale_of(es), hi, lo);
+                tmem_write(lanes + kS + half * (kHalf / 2), hi);
+                tmem_write(lanes + kSLo + half * (kHalf / 2), lo);
+                tmem_written();
+            }
+            arrive(&M.s_ready);
+            if (owed) {
+                write_y(c - 1);
+                tc_fence_before();
+            }
+            arrive(&M.r_free);
+            inv_r = inv_s;
+            // differences, and as the decays to the chunk's end leave them
+            wait(&M.z_done, now);
+            tc_fence_after();
+            float d[32], e[32];
+            tmem_read(lanes + kZ + half * 32, d);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                d[i] = fmaf(-d[i] * inv_s, f.z[half * 32 + i], u[i]);
+                if (v >= D) d[i] = 0.0f;
+                e[i] = d[i] * f.k[half * 32 + i];
+            }
+            M.d_max[half][v] = float2{largest(d), largest(e)};
+            pair_sync(w4);
+            const float2 m0 = M.d_max[0][v], m1 = M.d_max[1][v];
+            const int ed = exponent_of(__uint_as_float(max(__float_as_uint(m0.x), __float_as_uint(m1.x))));
+            const int ee = exponent_of(__uint_as_float(max(__float_as_uint(m0.y), __float_as_uint(m1.y))));
+            unsigned hi[16], lo[16];
+            split(e, scale_of(ee), hi, lo);
+            tmem_write(lanes + kD + half * 16, hi);
+            tmem_write(lanes + kD + 32 + half * 16, lo);
+            tmem_written();
+            arrive(&M.d_ready);
+            split(d, scale_of(ed), hi, lo);
+            wait(&M.r_done, now);  // the state's halves have been read
+            tc_fence_after();
+            tmem_write(lanes + kS + half * 16, hi);
+            tmem_write(lanes + kS + 32 + half * 16, lo);
+            tmem_written();
+            arrive(&M.y_ready);
+            inv_y = unscale_of(ed);
+            // the new state
+            wait(&M.d_done, now);
+            tc_fence_after();
+            const float inv_e = unscale_of(ee), end = f.end;
+            float x[kHalf];
+            tmem_read(lanes + kNew + half * kHalf, x);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) S[i] = fmaf(x[i], inv_e, S[i] * end);
+            tc_fence_before();
+            owed = true;
+        }
+        if (owed) {
+            wait(&M.y_done, (live - 1) & 1);
+            tc_fence_after();
+            write_y(chunks - 1);
+        }
+        work_sync();
+        if (!*(volatile int *)&M.abort_flag) {
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i)
+                if (in && half * kHalf + i < n.dim) state[i * vw] = S[i];
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    settle(&M.abort_flag);
+    if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <int D>
+cudaError_t launch_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
+    constexpr int kDevices = 64;
+    static std::atomic<bool> done[kDevices];
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && (device >= kDevices || !done[device].load(std::memory_order_relaxed))) {
+        e = cudaFuncSetAttribute(k_delta_chain<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChainSmem<D>));
+        if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
+    }
+    if (e != cudaSuccess) return e;
+    return kv8_launch(k_delta_chain<D>, dim3((unsigned)(slab.runs * slab.heads * slab.ratio)), dim3(kChainThreads), sizeof(ChainSmem<D>), 1, s, n, a, r,
+                      slab);
+}
+
+}  // namespace
+
+cudaError_t delta_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
+    return n.dim <= 64 ? launch_chain<64>(n, a, r, slab, s) : launch_chain<128>(n, a, r, slab, s);
+}
+
+}  // namespace strata

@@ -1,0 +1,147 @@
+// The gated delta rule in chunks of 64 tokens on the 5th-generation tensor cores: what its two kernels share.
+//
+// With P_i the product of a chunk's decays up to token i, G_ij that of those after j up to i, E_i that of those after i:
+//   A_ij = beta_i G_ij (k_i . k_j) for j < i,   T = (I + A)^-1,   U = T diag(beta) V,   W = T diag(beta P) K        delta_prepare.cu
+//   D = U - W S,   y_i = P_i q_i S + sum_{j <= i} G_ij (q_i . k_j) D_j,   S <- P_63 S + sum_i E_i k_i D_i^T          delta_chain.cu
+// The first line needs no state: all chunks of all heads at once. The second goes from chunk to chunk. Products of decays are
+// formed by multiplication alone, so that zero decays need no care.
+//
+// Products. Each F32 factor is two FP16 halves, times a power of two that brings the largest value of its row (or of its
+// TMEM lane, or tile) to 2^13: 22 bits for whatever is within 2^-17 of that, and 2^-38 of it below. lo hi + hi lo + hi hi are three
+// FP16 products with F32 sums; lo lo would be 2^-22 of the result. The large product comes last: sums in TMEM are cut, not
+// rounded, and each step at full size costs up to 2^-24 of the sum, always towards zero (with hi hi first a prompt's result was 9.4e-7
+// off in the 2-norm, so it is 2.8e-7).
+//
+// Workspace: a slot for each run, key head and chunk of a slab, in the layout that the second kernel's tensor-core operands
+// have in shared memory (rows of 128 bytes, 128-byte swizzle): Q and K [64 tokens][D], hi and lo; then for each of the key
+// head's value heads W [64][D], hi and lo, the products G (q . k) [64][64], hi and lo, U [64][D] in F32 and the rows' factors.
+#pragma once
+#include "mixers.cuh"
+#include "pf_gemm.cuh"
+
+namespace strata {
+
+constexpr int kChunk = 64;
+constexpr float kDeltaLarge = 0x1p60f;  // past this, or not finite: the chunk is walked token by token
+
+struct DeltaFactors {  // of a chunk's rows, for one value head
+    float z[64];       // W's scale taken back
+    float q[64];       // P over Q's scale
+    float attn[64];    // G (q . k)'s scale taken back
+    float k[64];       // E over K's scale
+    float end;         // P of the last token
+    int walk;          // token by token
+    int pad[30];
+};
+struct DeltaSlab {  // runs, key heads and chunks [first, first + n) of a call
+    int run0, runs, head0, heads, chunk0, chunks;
+    int ratio;  // value heads of a key head
+    unsigned char *slots;
+    long long slot_bytes;
+};
+template <int D>
+struct DeltaSlot {
+    static constexpr int tile = 64 * D * 2 * 2, attn = 64 * 64 * 2 * 2, u = 64 * D * 4;  // bytes; hi and lo
+    static constexpr int q = 0, k = tile, heads = 2 * tile;
+    static constexpr int w = 0, g = tile, uu = tile + attn, factors = uu + u, head_bytes = factors + (int)sizeof(DeltaFactors);
+    __host__ __device__ static long long bytes(int ratio) { return heads + (long long)ratio * head_bytes; }
+};
+
+cudaError_t delta_step(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s);
+cudaError_t delta_prepare(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, bool vec, cudaStream_t s);
+cudaError_t delta_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s);
+
+#ifdef __CUDACC__
+namespace delta {
+
+using namespace pf;
+
+// 32 or 64 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
+__device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[64]) {
+    float a[32], b[32];
+    tmem_ld32(taddr, a);
+    tmem_ld32(taddr + 32, b);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = a[i], v[32 + i] = b[i];
+}
+template <int N>
+__device__ __forceinline__ void tmem_write(unsigned taddr, const unsigned (&r)[N]) {
+#pragma unroll
+    for (int at = 0; at < N; at += 16) {
+        unsigned part[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[i] = r[at + i];
+        tmem_st16(taddr + at, part);
+    }
+}
+__device__ __forceinline__ void tmem_written() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    tc_fence_before();
+}
+__device__ __forceinline__ void to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// The power of two that brings a largest magnitude to [2^13, 2^14), and its reciprocal.
+__device__ __forceinline__ int exponent_of(float largest) { return min(max((int)(__float_as_uint(largest) >> 23) - 127, -113), 127); }
+__device__ __forceinline__ float scale_of(int e) { return __uint_as_float((unsigned)(140 - e) << 23); }
+__device__ __forceinline__ float unscale_of(int e) { return __uint_as_float((unsigned)(114 + e) << 23); }
+// The larger magnitude, as bits order it: NaN above all.
+__device__ __forceinline__ unsigned larger(unsigned m, float x) { return max(m, __float_as_uint(x) & 0x7fffffffu); }
+template <int N>
+__device__ __forceinline__ float largest(const float (&x)[N]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = larger(m, x[i]);
+    return __uint_as_float(m);
+}
+__device__ __forceinline__ bool past(float largest) { return !(largest <= kDeltaLarge); }
+// x times a power of two as pairs of FP16 halves, hi and lo
+template <int N>
+__device__ __forceinline__ void split(const float (&x)[N], float scale, unsigned (&hi)[N / 2], unsigned (&lo)[N / 2]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) split_pair(x[2 * i] * scale, x[2 * i + 1] * scale, hi[i], lo[i]);
+}
+// Byte of 16-byte piece c of row r: rows of 128 bytes, 128-byte swizzle.
+__device__ __forceinline__ int piece(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+// Pieces [first, first + N / 4) of row r of a tile from pairs.
+template <int N>
+__device__ __forceinline__ void put_pieces(unsigned char *tile, int r, int first, const unsigned (&x)[N]) {
+#pragma unroll
+    for (int c = 0; c < N / 4; ++c) *reinterpret_cast<uint4 *>(tile + piece(r, first + c)) = uint4{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+}
+// Operand with its rows along the sum (a tile [sum][64 channels a panel] read the other way round): 64 channels of 8 rows are
+// an atom; panels are `panel` bytes apart, the next 8 rows 1024.
+__device__ __forceinline__ unsigned long long turned_desc(unsigned smem_addr, unsigned panel) {
+    return (unsigned long long)((smem_addr & 0x3FFFFu) >> 4) | ((unsigned long long)(panel >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ unsigned turned_idesc(int M, int N) { return idesc_f16(M, N) | (1u << 16); }
+
+// Waits of a block's threads, with a limit; past it, all of them let everything through and the block reports.
+struct Waits {
+    int *abort_flag;
+    unsigned *err;
+    __device__ __forceinline__ void operator()(unsigned long long *b, unsigned parity) const {
+        if (bar_try(b, parity)) return;
+        const long long began = clock64();
+        while (!bar_try(b, parity)) {
+            if (*(volatile int *)abort_flag) return;
+            if (clock64() - began > 2000000000LL) {  // about a second
+                atomicExch(abort_flag, 1);
+                raise_error(err, kErrWaitTimeout);
+                return;
+            }
+        }
+    }
+};
+// After a wait has run out: time for copies and products in flight, before shared memory and TMEM go.
+__device__ __forceinline__ void settle(const int *abort_flag) {
+    if (!*(volatile const int *)abort_flag) return;
+    const long long began = clock64();
+    while (clock64() - began < 4000000) {
+    }
+}
+
+}  // namespace delta
+#endif
+
+}  // namespace strata

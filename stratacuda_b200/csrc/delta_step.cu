@@ -4,7 +4,7 @@
 //   d = b (v - a S^T k),  y = a S^T q + (k . q) d,  S <- a S + k d^T
 // so that prediction and result come from one pass over the state as it was: one exchange between warps a token.
 // A block has 32 value columns of a head (columns do not meet), its 128 threads 4 columns by ROWS keys each, in registers.
-#include "mixers.cuh"
+#include "delta_chunk.cuh"
 
 namespace strata {
 namespace {
@@ -125,7 +125,7 @@ cudaError_t launch_step(const DeltaNet &n, const DeltaRule &a, const MixRuns &r,
 
 }  // namespace
 
-cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s) {
+cudaError_t delta_step(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s) {
     const bool vec = n.dim % 4 == 0 && a.v_stride % 4 == 0 && mix_aligned16(n.state) && mix_aligned16(a.v) && mix_aligned16(a.y);
     return vec ? launch_step<true>(n, a, r, s) : launch_step<false>(n, a, r, s);
 }
