@@ -16,19 +16,20 @@ namespace {
 
 using namespace delta;
 
-constexpr int kWork = 256, kChainThreads = kWork + 64, kFetchWarp = 8, kIssueWarp = 9;
+constexpr int kWork = 256, kChainThreads = kWork + 128, kFetchWarp = 8, kIssueWarp = 9;
 
 template <int D>
 struct __align__(1024) ChainSmem {
     unsigned char w[2][2 * D / 64][64 * 128];  // by stage: hi panels, lo panels
     unsigned char q[2][2 * D / 64][64 * 128];
-    unsigned char k[2][2 * D / 64][64 * 128];
+    unsigned char k[2 * D / 64][64 * 128];
     unsigned char g[2][64 * 128];  // hi, lo
+    float u[64 * D];
     DeltaFactors factors[2];
     float s_max[2][128];
     float2 d_max[2][128];
     float2 walk[2][128];
-    unsigned long long w_full[2], w_empty[2], q_full[2], q_empty[2], k_full[2], k_empty[2], f_full[2], f_empty[2], g_full, g_empty;
+    unsigned long long w_full[2], w_empty[2], q_full[2], q_empty[2], f_full[2], f_empty[2], k_full, k_empty, g_full, g_empty, u_full, u_empty;
     unsigned long long s_ready, r_free, d_ready, y_ready, z_done, r_done, d_done, y_done;
     unsigned tmem;
     int abort_flag;
@@ -40,7 +41,7 @@ __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 5, 256;" ::
 template <int D>
 __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
-    constexpr int kPanels = D / 64, kHalf = D / 2;
+    constexpr int kHalf = D / 2;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     ChainSmem<D> &M = *reinterpret_cast<ChainSmem<D> *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -63,9 +64,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             bar_init(&M.w_full[i], 1), bar_init(&M.w_empty[i], 1), bar_init(&M.q_full[i], 1), bar_init(&M.q_empty[i], 1);
-            bar_init(&M.k_full[i], 1), bar_init(&M.k_empty[i], 1), bar_init(&M.f_full[i], 1), bar_init(&M.f_empty[i], kWork / 32 + 1);
+            bar_init(&M.f_full[i], 1), bar_init(&M.f_empty[i], kWork / 32 + 1);
         }
-        bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
+        bar_init(&M.k_full, 1), bar_init(&M.k_empty, 1), bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
+        bar_init(&M.u_full, 1), bar_init(&M.u_empty, kWork / 32);
         bar_init(&M.s_ready, kWork / 32), bar_init(&M.r_free, kWork / 32), bar_init(&M.d_ready, kWork / 32), bar_init(&M.y_ready, kWork / 32);
         bar_init(&M.z_done, 1), bar_init(&M.r_done, 1), bar_init(&M.d_done, 1), bar_init(&M.y_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -83,6 +85,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
     constexpr unsigned kS = 0, kSLo = D / 2, kD = 128, kZ = 192, kR = 256, kY = 320, kNew = 384;
     const Waits wait{&M.abort_flag, n.err};
 
+    // of 64512 registers, 168 a thread at the start, the working threads take 216 and the others keep 72
+    if (warp >= kFetchWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == kFetchWarp) {
         if (lane == 0) {
             const auto fetch = [&](void *to, const unsigned char *from, unsigned bytes, unsigned long long *full) {
@@ -99,8 +103,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
                 fetch(M.w[st], slot + mine + Slot::w, Slot::tile, &M.w_full[st]);
                 wait(&M.q_empty[st], again);
                 fetch(M.q[st], slot + Slot::q, Slot::tile, &M.q_full[st]);
-                wait(&M.k_empty[st], again);
-                fetch(M.k[st], slot + Slot::k, Slot::tile, &M.k_full[st]);
+                wait(&M.u_empty, (c & 1) ^ 1);
+                fetch(M.u, slot + mine + Slot::uu, Slot::u, &M.u_full);
+                wait(&M.k_empty, (c & 1) ^ 1);
+                fetch(M.k, slot + Slot::k, Slot::tile, &M.k_full);
                 wait(&M.g_empty, (c & 1) ^ 1);
                 fetch(M.g, slot + mine + Slot::g, Slot::attn, &M.g_full);
             }
@@ -116,44 +122,45 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
                 const bool walk = M.factors[st].walk != 0;
                 bar_arrive(&M.f_empty[st]);
                 if (walk) {  // nothing of it is used
-                    wait(&M.w_full[st], ph), wait(&M.q_full[st], ph), wait(&M.k_full[st], ph), wait(&M.g_full, c & 1);
-                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.q_empty[st]), bar_arrive(&M.k_empty[st]), bar_arrive(&M.g_empty);
+                    wait(&M.w_full[st], ph), wait(&M.q_full[st], ph), wait(&M.k_full, c & 1), wait(&M.g_full, c & 1);
+                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.q_empty[st]), bar_arrive(&M.k_empty), bar_arrive(&M.g_empty);
                     continue;
                 }
                 const unsigned now = live & 1;
                 ++live;
+                constexpr unsigned kLoTile = D / 64 * 512;  // from a tile's hi panels to its lo ones, in 16-byte units
                 wait(&M.w_full[st], ph);
                 wait(&M.s_ready, now);
                 tc_fence_after();
+                const auto over_keys = [&](unsigned to, const void *tile) {  // lo hi, hi lo, hi hi
+                    const unsigned long long b = sw128_desc(su32(tile));
 #pragma unroll
-                for (int product = 0; product < 3; ++product)  // lo hi, hi lo, hi hi
+                    for (int product = 0; product < 3; ++product)
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_f16_ts(tmem + kZ, tmem + (product == 0 ? kSLo : kS) + k * 8,
-                                   sw128_desc(su32(M.w[st][(product == 1 ? kPanels : 0) + k / 4])) + k % 4 * 2, idesc_f16(128, 64), product || k);
+                        for (int k = 0; k < D / 16; ++k)
+                            mma_f16_ts(tmem + to, tmem + (product == 0 ? kSLo : kS) + k * 8, b + (product == 1) * kLoTile + k / 4 * 512 + k % 4 * 2,
+                                       idesc_f16(128, 64), product || k);
+                };
+                over_keys(kZ, M.w[st]);
                 mma_commit(&M.w_empty[st]);
                 mma_commit(&M.z_done);
                 wait(&M.q_full[st], ph);
                 wait(&M.r_free, now);
                 tc_fence_after();
-#pragma unroll
-                for (int product = 0; product < 3; ++product)
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8,
-                                   sw128_desc(su32(M.q[st][(product == 1 ? kPanels : 0) + k / 4])) + k % 4 * 2, idesc_f16(128, 64), product || k);
+                over_keys(kR, M.q[st]);
                 mma_commit(&M.q_empty[st]);
                 mma_commit(&M.r_done);
-                wait(&M.k_full[st], ph);
+                wait(&M.k_full, c & 1);
                 wait(&M.d_ready, now);
                 tc_fence_after();
+                const unsigned long long keys = turned_desc(su32(M.k[0]), 8192), g = sw128_desc(su32(M.g[0]));
 #pragma unroll
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + kNew, tmem + kD + (product == 0) * 32 + k * 8,
-                                   turned_desc(su32(M.k[st][product == 1 ? kPanels : 0]) + k * 2048, 8192), turned_idesc(128, D), product || k);
-                mma_commit(&M.k_empty[st]);
+                        mma_f16_ts(tmem + kNew, tmem + kD + (product == 0) * 32 + k * 8, keys + (product == 1) * kLoTile + k * 128, turned_idesc(128, D),
+                                   product || k);
+                mma_commit(&M.k_empty);
                 mma_commit(&M.d_done);
                 wait(&M.g_full, c & 1);
                 wait(&M.y_ready, now);
@@ -162,14 +169,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + kY, tmem + kS + (product == 0) * 32 + k * 8, sw128_desc(su32(M.g[product == 1])) + k * 2, idesc_f16(128, 64),
-                                   product || k);
+                        mma_f16_ts(tmem + kY, tmem + kS + (product == 0) * 32 + k * 8, g + (product == 1) * 512 + k * 2, idesc_f16(128, 64), product || k);
                 mma_commit(&M.g_empty);
                 mma_commit(&M.y_done);
             }
         }
         __syncwarp();
-    } else {
+    } else if (warp < kFetchWarp) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int w4 = warp & 3, half = warp >> 2, v = w4 * 32 + lane;
         const unsigned lanes = tmem + ((unsigned)(w4 * 32) << 16);
         const bool in = v < n.dim;
@@ -186,22 +193,29 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
         float inv_r = 0, inv_y = 0;   // their scales taken back
         // results of chunk c: its tokens half * 32 ..
         const auto write_y = [&](int c) {
-            const DeltaFactors &f = M.factors[c & 1];
-            float R[32], Y[32];
-            tmem_read(lanes + kR + half * 32, R);
-            tmem_read(lanes + kY + half * 32, Y);
-            const int t0 = begin + c * kChunk + half * 32;
+            const float *fq = M.factors[c & 1].q + half * 32, *fa = M.factors[c & 1].attn + half * 32;
+            const int t0 = begin + c * kChunk + half * 32, left = in ? me.tokens - t0 : 0;
             float *y = A.y + (first + t0) * vw + (long long)h * n.dim + v;
+#pragma unroll 1
+            for (int at = 0; at < 32; at += 16) {
+                float R[16], Y[16];
+                tmem_read(lanes + kR + half * 32 + at, R);
+                tmem_read(lanes + kY + half * 32 + at, Y);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float value = R[i] * inv_r * f.q[half * 32 + i] + Y[i] * inv_y * f.attn[half * 32 + i];
-                if (in && t0 + i < me.tokens) y[i * vw] = value;
+                for (int i = 0; i < 16; ++i) R[i] = fmaf(R[i] * inv_r, fq[at + i], Y[i] * inv_y * fa[at + i]);
+                if (left >= at + 16) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i, y += vw) *y = R[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i, y += vw)
+                        if (at + i < left) *y = R[i];
+                }
             }
             arrive(&M.f_empty[c & 1]);
         };
         for (int c = 0; c < chunks; ++c) {
             const int st = c & 1;
-            const unsigned char *slot = slots + c * slab.slot_bytes;
             wait(&M.f_full[st], c >> 1 & 1);
             const DeltaFactors &f = M.factors[st];
             if (owed) wait(&M.y_done, (live - 1) & 1), tc_fence_after();
@@ -212,8 +226,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
                 const int t0 = begin + c * kChunk, tokens = min(kChunk, me.tokens - t0);
                 for (int t = 0; t < tokens; ++t) {
                     const long long row = first + t0 + t;
-                    const float *kp = A.k + row * A.k_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
-                    const float *qp = A.q + row * A.q_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
+                    // (volatile: one after another, not 128 registers of them)
+                    const volatile float *kp = A.k + row * A.k_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
+                    const volatile float *qp = A.q + row * A.q_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
                     const float a = A.decay[row * n.value_heads + h], b = A.beta[row * n.value_heads + h];
                     const float value = in ? A.v[row * A.v_stride + (long long)h * n.dim + v] : 0.0f;
                     float p = 0.0f, y = 0.0f;
@@ -237,26 +252,28 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
                     if (half == 0 && in) A.y[row * vw + (long long)h * n.dim + v] = M.walk[0][v].y + M.walk[1][v].y;
                 }
                 arrive(&M.f_empty[st]);
+                wait(&M.u_full, c & 1);
+                arrive(&M.u_empty);
                 continue;
             }
             const unsigned now = live & 1;
             ++live;
-            float u[32];
-            const float *up = reinterpret_cast<const float *>(slot + mine + Slot::uu) + half * 32 * D + (v < D ? v : 0);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __ldcg(up + i * D);
             // the state as an operand
-            M.s_max[half][v] = largest(S);
+            M.s_max[half][v] = largest(0.0f, S);
             pair_sync(w4);
-            const int es = exponent_of(__uint_as_float(max(__float_as_uint(M.s_max[0][v]), __float_as_uint(M.s_max[1][v]))));
+            const int es = exponent_of(larger(M.s_max[0][v], M.s_max[1][v], 0.0f));
             const float inv_s = unscale_of(es);
-            {
-                unsigned hi[kHalf / 2], lo[kHalf / 2];
-                split(S, scale_of(es), hi, lo);
-                tmem_write(lanes + kS + half * (kHalf / 2), hi);
-                tmem_write(lanes + kSLo + half * (kHalf / 2), lo);
-                tmem_written();
+#pragma unroll
+            for (int i = 0; i < kHalf; i += 16) {
+                float x[16];
+                unsigned hi[8], lo[8];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = S[i + e];
+                split(x, scale_of(es), hi, lo);
+                tmem_write(lanes + kS + (half * kHalf + i) / 2, hi);
+                tmem_write(lanes + kSLo + (half * kHalf + i) / 2, lo);
             }
+            tmem_written();
             arrive(&M.s_ready);
             if (owed) {
                 write_y(c - 1);
@@ -265,32 +282,50 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
             arrive(&M.r_free);
             inv_r = inv_s;
             // differences, and as the decays to the chunk's end leave them
+            wait(&M.u_full, c & 1);
             wait(&M.z_done, now);
             tc_fence_after();
-            float d[32], e[32];
+            float d[32];
+            const float *u = M.u + half * 32 * D + (v < D ? v : 0), *fz = f.z + half * 32, *fk = f.k + half * 32;
+            const float by = v < D ? -inv_s : 0.0f;
+            float most_d = 0.0f, most_e = 0.0f;
             tmem_read(lanes + kZ + half * 32, d);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                d[i] = fmaf(-d[i] * inv_s, f.z[half * 32 + i], u[i]);
-                if (v >= D) d[i] = 0.0f;
-                e[i] = d[i] * f.k[half * 32 + i];
+            for (int i = 0; i < 32; i += 2) {
+                d[i] = fmaf(d[i] * by, fz[i], v < D ? u[i * D] : 0.0f);
+                d[i + 1] = fmaf(d[i + 1] * by, fz[i + 1], v < D ? u[i * D + D] : 0.0f);
+                most_d = larger(most_d, d[i], d[i + 1]);
+                most_e = larger(most_e, d[i] * fk[i], d[i + 1] * fk[i + 1]);
             }
-            M.d_max[half][v] = float2{largest(d), largest(e)};
+            arrive(&M.u_empty);
+            M.d_max[half][v] = float2{most_d, most_e};
             pair_sync(w4);
             const float2 m0 = M.d_max[0][v], m1 = M.d_max[1][v];
-            const int ed = exponent_of(__uint_as_float(max(__float_as_uint(m0.x), __float_as_uint(m1.x))));
-            const int ee = exponent_of(__uint_as_float(max(__float_as_uint(m0.y), __float_as_uint(m1.y))));
-            unsigned hi[16], lo[16];
-            split(e, scale_of(ee), hi, lo);
-            tmem_write(lanes + kD + half * 16, hi);
-            tmem_write(lanes + kD + 32 + half * 16, lo);
+            const int ed = exponent_of(larger(m0.x, m1.x, 0.0f)), ee = exponent_of(larger(m0.y, m1.y, 0.0f));
+#pragma unroll
+            for (int i = 0; i < 32; i += 16) {
+                float x[16];
+                unsigned hi[8], lo[8];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = d[i + e] * fk[i + e];
+                split(x, scale_of(ee), hi, lo);
+                tmem_write(lanes + kD + (half * 32 + i) / 2, hi);
+                tmem_write(lanes + kD + 32 + (half * 32 + i) / 2, lo);
+            }
             tmem_written();
             arrive(&M.d_ready);
-            split(d, scale_of(ed), hi, lo);
             wait(&M.r_done, now);  // the state's halves have been read
             tc_fence_after();
-            tmem_write(lanes + kS + half * 16, hi);
-            tmem_write(lanes + kS + 32 + half * 16, lo);
+#pragma unroll
+            for (int i = 0; i < 32; i += 16) {
+                float x[16];
+                unsigned hi[8], lo[8];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = d[i + e];
+                split(x, scale_of(ed), hi, lo);
+                tmem_write(lanes + kS + (half * 32 + i) / 2, hi);
+                tmem_write(lanes + kS + 32 + (half * 32 + i) / 2, lo);
+            }
             tmem_written();
             arrive(&M.y_ready);
             inv_y = unscale_of(ed);
@@ -298,10 +333,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
             wait(&M.d_done, now);
             tc_fence_after();
             const float inv_e = unscale_of(ee), end = f.end;
-            float x[kHalf];
-            tmem_read(lanes + kNew + half * kHalf, x);
 #pragma unroll
-            for (int i = 0; i < kHalf; ++i) S[i] = fmaf(x[i], inv_e, S[i] * end);
+            for (int i = 0; i < kHalf; i += 16) {
+                float x[16];
+                tmem_read(lanes + kNew + half * kHalf + i, x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) S[i + e] = fmaf(x[e], inv_e, S[i + e] * end);
+            }
             tc_fence_before();
             owed = true;
         }

@@ -56,24 +56,28 @@ namespace delta {
 
 using namespace pf;
 
-// 32 or 64 columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
-__device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[64]) {
-    float a[32], b[32];
-    tmem_ld32(taddr, a);
-    tmem_ld32(taddr + 32, b);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = a[i], v[32 + i] = b[i];
+// 16 or 32 columns of this thread's TMEM lane, and 8 or more written.
+__device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+          "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
 }
-template <int N>
-__device__ __forceinline__ void tmem_write(unsigned taddr, const unsigned (&r)[N]) {
+__device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
+__device__ __forceinline__ void tmem_write(unsigned taddr, const unsigned (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_write(unsigned taddr, const unsigned (&r)[16]) { tmem_st16(taddr, r); }
+__device__ __forceinline__ void tmem_write(unsigned taddr, const float (&v)[16]) {
+    unsigned r[16];
 #pragma unroll
-    for (int at = 0; at < N; at += 16) {
-        unsigned part[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[i] = r[at + i];
-        tmem_st16(taddr + at, part);
-    }
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+    tmem_st16(taddr, r);
 }
 __device__ __forceinline__ void tmem_written() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -85,21 +89,42 @@ __device__ __forceinline__ void to_async() { asm volatile("fence.proxy.async.sha
 __device__ __forceinline__ int exponent_of(float largest) { return min(max((int)(__float_as_uint(largest) >> 23) - 127, -113), 127); }
 __device__ __forceinline__ float scale_of(int e) { return __uint_as_float((unsigned)(140 - e) << 23); }
 __device__ __forceinline__ float unscale_of(int e) { return __uint_as_float((unsigned)(114 + e) << 23); }
-// The larger magnitude, as bits order it: NaN above all.
-__device__ __forceinline__ unsigned larger(unsigned m, float x) { return max(m, __float_as_uint(x) & 0x7fffffffu); }
+// Largest magnitudes; NaN where one is.
+__device__ __forceinline__ float larger(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 template <int N>
-__device__ __forceinline__ float largest(const float (&x)[N]) {
-    unsigned m = 0;
+__device__ __forceinline__ float largest(float m, const float (&x)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = larger(m, x[i]);
-    return __uint_as_float(m);
+    for (int i = 0; i + 1 < N; i += 2) m = larger(m, x[i], x[i + 1]);
+    return m;
+}
+__device__ __forceinline__ float warp_largest(float x) {
+    float r;
+    asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
 }
 __device__ __forceinline__ bool past(float largest) { return !(largest <= kDeltaLarge); }
 // x times a power of two as pairs of FP16 halves, hi and lo
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[N], float scale, unsigned (&hi)[N / 2], unsigned (&lo)[N / 2]) {
+    const unsigned long long by = pack2(scale, scale), less = pack2(-1.0f, -1.0f);
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) split_pair(x[2 * i] * scale, x[2 * i + 1] * scale, hi[i], lo[i]);
+    for (int i = 0; i < N / 2; ++i) {
+        const unsigned long long s = mul2_rn(pack2(x[2 * i], x[2 * i + 1]), by);
+        float a, b;
+        unpack2(s, a, b);
+        const __half2 h = __floats2half2_rn(a, b);
+        const float2 f = __half22float2(h);
+        unsigned long long d;
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pack2(f.x, f.y)), "l"(less), "l"(s));
+        unpack2(d, a, b);
+        const __half2 l = __floats2half2_rn(a, b);
+        hi[i] = *reinterpret_cast<const unsigned *>(&h);
+        lo[i] = *reinterpret_cast<const unsigned *>(&l);
+    }
 }
 // Byte of 16-byte piece c of row r: rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ int piece(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }

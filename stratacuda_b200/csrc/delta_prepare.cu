@@ -3,9 +3,12 @@
 // A block has a run's chunk and key head, and takes the head's value heads two at a time, one by each warpgroup:
 //   [Q; K] K^T      128 rows by 64, once for all of them
 //   A, G (q . k)    a thread a row, from its TMEM lane
-//   T = (I + A)^-1  halves' inverses by substitution, a column a lane, then -T22 (A21 T11); F32 throughout
-//   U^T = V^T (T diag(beta))^T   a lane a value channel, V straight from memory to TMEM
+//   T = (I + A)^-1  of blocks of 16 by substitution, a column a lane, then of blocks twice as large twice, F32 throughout
+//   U^T = V^T (T diag(beta))^T   a lane a value channel
 //   W = (T diag(beta P)) K       both heads' 64 rows as one operand; K's tile as it lies, read the other way round
+// Bound by instructions, most of them the splits into halves: what a row needs twice (its largest value first) waits in TMEM,
+// and columns go by 16 in loops that are not unrolled, since code that a block runs once comes slower than it executes (with all
+// 64 columns unrolled a prompt of 2048 tokens over 32 heads of 128 took 210 us, most of them without an instruction to issue).
 #include "delta_chunk.cuh"
 
 #include <atomic>
@@ -20,11 +23,18 @@ constexpr int kPrepareThreads = 256, kPitch = 68;
 template <int D>
 struct __align__(1024) PrepareSmem {
     unsigned char qk[2][D / 64][128 * 128];  // hi, lo: panels of 64 channels; rows 0-63 Q, 64-127 K
-    unsigned char tw[2][128 * 128];          // T diag(beta P) over K's scales: two heads' 64 rows
-    unsigned char tu[2][2][64 * 128];        // by head: T diag(beta)
-    float a[2][64 * kPitch];                 // A, then T; the upper right quarter has A21 T11
-    float inv[128];                          // Q's and K's scales taken back
-    float decay[2][64], beta[2][64], upto[2][64];
+    union {                                  // V's rows until they are in TMEM, then T's
+        float v[2][64 * D];                  // by head
+        struct {
+            unsigned char tw[2][128 * 128];    // T diag(beta P) over K's scales: hi, lo; two heads' 64 rows
+            unsigned char tu[2][2][64 * 128];  // by head: T diag(beta), hi, lo
+        };
+    };
+    float a[2][64 * kPitch];  // A, then T
+    float inv[128];           // Q's and K's scales taken back
+    // by head: decays; products of decays up to a token in its half; strengths, and times decays up to the token over K's scale;
+    // K's scales taken back, the lower half's times the decays after a token in it
+    float decay[2][64], upto[2][64], beta[2][64], beta_w[2][64], inv_k[2][64];
     float inv_tw[2][64], inv_tu[2][64];
     float w_max[2][128];
     int bad_key, bad[2], abort_flag;
@@ -33,11 +43,15 @@ struct __align__(1024) PrepareSmem {
 };
 
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
+__device__ __forceinline__ void add2(unsigned long long &d, unsigned long long a, unsigned long long b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ ulonglong2 load22(const float *p) { return *reinterpret_cast<const ulonglong2 *>(p); }
 
-// x[j] of the unit triangular system (I + L) x = e_c, L the strictly lower part of 32 rows at l
-__device__ __forceinline__ void substitute(const float *l, int c, float (&x)[32]) {
+// x of (I + L) x = e_c, L the strictly lower part of 16 rows at l
+__device__ __forceinline__ void substitute(const float *l, int c, float (&x)[16]) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 16; ++i) {
         float s[4] = {i == c ? 1.0f : 0.0f, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < i; j += 4) {
@@ -50,20 +64,49 @@ __device__ __forceinline__ void substitute(const float *l, int c, float (&x)[32]
         x[i] = (s[0] + s[1]) + (s[2] + s[3]);
     }
 }
-// eight columns of row r of sign * X Y, 32 by 32 at x and y; X's row has `terms` values that count
-__device__ __forceinline__ void times(const float *x, const float *y, int r, int c, int terms, float (&out)[8]) {
+// W columns (4 or 8) from c of row r of sign X Y: rows of X at x, Y at y; `terms` (a multiple of 4) of X's row count
+template <int W>
+__device__ __forceinline__ void times(const float *x, const float *y, int r, int c, int terms, float sign, float *to) {
+    unsigned long long s[W / 2] = {};
+#pragma unroll 2
+    for (int j = 0; j < terms; j += 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(x + r * kPitch + j);
+        const float g[4] = {f.x * sign, f.y * sign, f.z * sign, f.w * sign};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = 0.0f;
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) {
-        const float f = j < terms ? x[r * kPitch + j] : 0.0f;
-        const float4 a = *reinterpret_cast<const float4 *>(y + j * kPitch + c), b = *reinterpret_cast<const float4 *>(y + j * kPitch + c + 4);
-        out[0] = fmaf(f, a.x, out[0]), out[1] = fmaf(f, a.y, out[1]), out[2] = fmaf(f, a.z, out[2]), out[3] = fmaf(f, a.w, out[3]);
-        out[4] = fmaf(f, b.x, out[4]), out[5] = fmaf(f, b.y, out[5]), out[6] = fmaf(f, b.z, out[6]), out[7] = fmaf(f, b.w, out[7]);
+        for (int e = 0; e < 4; ++e) {
+            const float *row = y + (j + e) * kPitch + c;
+#pragma unroll
+            for (int w = 0; w < W; w += 4) {
+                const ulonglong2 b = load22(row + w);
+                add2(s[w / 2], pack2(g[e], g[e]), b.x);
+                add2(s[w / 2 + 1], pack2(g[e], g[e]), b.y);
+            }
+        }
     }
+#pragma unroll
+    for (int w = 0; w < W; w += 4) *reinterpret_cast<ulonglong2 *>(to + r * kPitch + c + w) = ulonglong2{s[w / 2], s[w / 2 + 1]};
+}
+// Products over lanes: of this one's and those before, and of those after.
+__device__ __forceinline__ float product_upto(float x, int lane) {
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const float o = __shfl_up_sync(0xffffffffu, x, s);
+        if (lane >= s) x *= o;
+    }
+    return x;
+}
+__device__ __forceinline__ float product_after(float x, int lane) {
+    x = __shfl_down_sync(0xffffffffu, x, 1);
+    if (lane == 31) x = 1.0f;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const float o = __shfl_down_sync(0xffffffffu, x, s);
+        if (lane + s < 32) x *= o;
+    }
+    return x;
 }
 
-// VEC: rows of q and k can be read four channels at a time.
+// VEC: rows of q, k and v can be read four channels at a time.
 template <int D, bool VEC>
 __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
@@ -80,6 +123,21 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
     const long long row0 = (long long)run * r.count + t0;
     unsigned char *slot = slab.slots + blockIdx.x * slab.slot_bytes;
 
+    // V's rows of a value head to shared memory, by its warpgroup; zeros behind the run's end and past dim
+    const auto fetch_v = [&](int h) {
+        const float *from = A.v + row0 * A.v_stride + (long long)h * n.dim;
+        constexpr int kPiece = VEC ? 4 : 1;
+#pragma unroll 4
+        for (int at = gt * kPiece; at < 64 * D; at += 128 * kPiece) {
+            const int j = at / D, c = at % D;
+            const bool in = j < tokens && c < n.dim;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(su32(&M.v[g][at])), "l"(in ? from + j * A.v_stride + c : A.v),
+                         "n"(kPiece * 4), "r"(in ? kPiece * 4 : 0)
+                         : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (g < slab.ratio) fetch_v(head + g * n.key_heads);
     if (tid == 0) {
         bar_init(&M.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -93,12 +151,14 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = M.tmem, mine = tmem + ((unsigned)(w4 * 32) << 16);
-    const unsigned kRaw = 0, kV = 64 + 64 * g, kWAt = 192, kU = 320 + 64 * g;  // columns
+    // columns: [Q; K] K^T; by head V's halves; W; by head U^T, whose place and W's keep rows until they are split
+    const unsigned kRaw = 0, kV = 64 + 64 * g, kWAt = 192, kU = 320 + 64 * g;
     const Waits wait{&M.abort_flag, n.err};
     unsigned phase = 0;
 
     // Q's and K's rows, a power of two each
     constexpr int kLanes = D / 4, kRows = 32 / kLanes;
+#pragma unroll 1
     for (int at = 0; at < 16; at += 8 * kRows) {
         float f[8][4];
         const int ch = 4 * (lane % kLanes);
@@ -119,12 +179,16 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int row = warp * 16 + at + u * kRows + lane / kLanes;
-            unsigned m = __float_as_uint(largest(f[u]));
+            float m = largest(0.0f, f[u]);
+            if (kLanes == 32) {
+                m = warp_largest(m);
+            } else {
 #pragma unroll
-            for (int s = kLanes / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
-            const int e = exponent_of(__uint_as_float(m));
+                for (int s = kLanes / 2; s > 0; s >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, s), 0.0f);
+            }
+            const int e = exponent_of(m);
             if (lane % kLanes == 0) M.inv[row] = unscale_of(e);
-            if (past(__uint_as_float(m))) M.bad_key = 1;
+            if (past(m)) M.bad_key = 1;
             unsigned hi[2], lo[2];
             split(f[u], scale_of(e), hi, lo);
             const int to = piece(row, ch % 64 / 8) + ch % 8 * 2;
@@ -136,11 +200,13 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
     __syncthreads();
     if (warp == 0) {
         if (elect_one()) {
+            const unsigned long long q = sw128_desc(su32(M.qk[0][0]));
+#pragma unroll 1
             for (int product = 0; product < 3; ++product) {  // lo hi, hi lo, hi hi
-                const int x = product == 0, y = product == 1;
+                const unsigned long long x = q + (product == 0) * (kPanels * 1024), y = q + 512 + (product == 1) * (kPanels * 1024);
+#pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_f16(tmem + kRaw, sw128_desc(su32(M.qk[x][k / 4])) + k % 4 * 2, sw128_desc(su32(M.qk[y][k / 4]) + 8192) + k % 4 * 2,
-                            idesc_f16(128, 64), product || k);
+                    mma_f16(tmem + kRaw, x + k / 4 * 1024 + k % 4 * 2, y + k / 4 * 1024 + k % 4 * 2, idesc_f16(128, 64), product || k);
             }
             mma_commit(&M.done);
         }
@@ -156,6 +222,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
         __syncwarp();
     }
 
+#pragma unroll 1
     for (int pair = 0; pair < slab.ratio; pair += 2) {
         const int m = pair + g, h = head + m * n.key_heads;
         const bool there = m < slab.ratio;
@@ -164,100 +231,184 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
         if (gt == 0) M.bad[g] = 0;
         float inv_v = 0.0f;
         if (there) {
-            // decays and strengths; rows behind the run's end change nothing
-            const int t = gt & 63;
-            const bool in = t < tokens;
-            const long long at = (row0 + t) * n.value_heads + h;
-            const float x = gt < 64 ? (in ? A.decay[at] : 1.0f) : (in ? A.beta[at] : 0.0f);
-            (gt < 64 ? M.decay[g] : M.beta[g])[t] = x;
-            // V's column of this lane to TMEM
-            float v[64];
-            const float *p = A.v + row0 * A.v_stride + (long long)h * n.dim + gt;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            group_sync(g);  // V is there, and bad[g] has been cleared
+            if (w4 == 0) {
+                // decays and strengths, two tokens a lane; rows behind the run's end change nothing
+                float a[2], b[2];
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = gt < n.dim && j < tokens ? p[j * A.v_stride] : 0.0f;
-            group_sync(g);  // bad[g] has been cleared
-            const float most = largest(v);
+                for (int e = 0; e < 2; ++e) {
+                    const bool in = lane + 32 * e < tokens;
+                    const long long at = (row0 + lane + 32 * e) * n.value_heads + h;
+                    a[e] = in ? A.decay[at] : 1.0f;
+                    b[e] = in ? A.beta[at] : 0.0f;
+                }
+                if (past(larger(larger(a[0], a[1], b[0]), b[1], 0.0f))) M.bad[g] = 1;
+                const float upto[2] = {product_upto(a[0], lane), product_upto(a[1], lane)};
+                const float after[2] = {product_after(a[0], lane), product_after(a[1], lane)};
+                const float low = __shfl_sync(0xffffffffu, upto[0], 31), high = __shfl_sync(0xffffffffu, upto[1], 31);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int t = lane + 32 * e;
+                    const float p = e ? upto[1] * low : upto[0], inv_k = M.inv[64 + t];
+                    M.decay[g][t] = a[e];
+                    M.upto[g][t] = upto[e];
+                    M.beta[g][t] = b[e];
+                    M.beta_w[g][t] = b[e] * p * inv_k;
+                    M.inv_k[g][t] = e ? inv_k : inv_k * after[0];
+                    factors->q[t] = p * M.inv[t];
+                    factors->k[t] = (e ? after[1] : after[0] * high) * inv_k;
+                    if (t == 63) factors->end = p;
+                }
+            }
+            // V's column of this lane to TMEM
+            const float *column = M.v[g] + (gt < D ? gt : 0);
+            float most = 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < 64; j += 16) {
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = column[(j + e) * D];
+                most = largest(most, v);
+            }
             const int e = exponent_of(most);
             inv_v = unscale_of(e);
-            if (past(most) || past(fabsf(x))) M.bad[g] = 1;
-            unsigned hi[32], lo[32];
-            split(v, scale_of(e), hi, lo);
-            tmem_write(mine + kV, hi);
-            tmem_write(mine + kV + 32, lo);
+            if (past(most)) M.bad[g] = 1;
+#pragma unroll 1
+            for (int j = 0; j < 64; j += 16) {
+                float v[16];
+                unsigned hi[8], lo[8];
+#pragma unroll
+                for (int u = 0; u < 16; ++u) v[u] = column[(j + u) * D];
+                split(v, scale_of(e), hi, lo);
+                tmem_write(mine + kV + j / 2, hi);
+                tmem_write(mine + kV + 32 + j / 2, lo);
+            }
             tmem_written();
         }
         if (pair == 0) wait(&M.done, phase & 1), ++phase;
         tc_fence_after();
         if (there) {
-            float x[64];
-            tmem_read(mine + kRaw, x);
+            group_sync(g);  // the decays are there
+            // rows 0-63: products of queries, 64-127: of keys, each times G over the column's scale. Row i of the upper half: the
+            // decays up to it in that half times those after column j in the lower one; else their product grows from j = i down.
             const int i = gt & 63;
-            const bool key = gt >= 64;
-            // x_j G_ij over the scales; the product of decays grows from j = i down
-            const float inv_i = M.inv[gt];
-            float p = 1.0f;
+            const bool key = gt >= 64, upper = w4 & 1;
+            const float row_factor = key ? M.inv[gt] * M.beta[g][i] : 1.0f, far = M.upto[g][i];
+            float *a_row = &M.a[g][i * kPitch];
+            float p = 1.0f, most = 0.0f;
+            const int last = upper ? 48 : 16;  // the last columns that count
+#pragma unroll 1
+            for (int j = last; j >= 0; j -= 16) {
+                float x[16];
+                tmem_read(mine + kRaw + j, x);
+                if (upper && j < 32) {
 #pragma unroll
-            for (int j = 63; j >= 0; --j) {
-                if (j < i) p *= M.decay[g][(j + 1) & 63];
-                if (key && i == 63) factors->k[j] = p * M.inv[64 + j];
-                x[j] = j < i || (j == i && !key) ? x[j] * M.inv[64 + j] * p * inv_i : 0.0f;
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 c = *reinterpret_cast<const float4 *>(&M.inv_k[g][j + e]);
+                        x[e] *= c.x * far, x[e + 1] *= c.y * far, x[e + 2] *= c.z * far, x[e + 3] *= c.w * far;
+                    }
+                } else {
+                    const int limit = key ? i - 1 : i;
+#pragma unroll
+                    for (int e = 15; e >= 0; --e) {
+                        if (j + e < i) p *= M.decay[g][j + e + 1];
+                        x[e] = j + e <= limit ? x[e] * M.inv[64 + j + e] * p : 0.0f;
+                    }
+                }
+                if (key) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4 *>(a_row + j + e) =
+                            float4{x[e] * row_factor, x[e + 1] * row_factor, x[e + 2] * row_factor, x[e + 3] * row_factor};
+                } else {
+                    most = largest(most, x);
+                    tmem_write(mine + kU + j, x);
+                }
             }
-            const float upto = p * M.decay[g][0];
-            if (key) {
-                const float b = M.beta[g][i];
-#pragma unroll
-                for (int j = 0; j < 64; j += 4)
-                    *reinterpret_cast<float4 *>(&M.a[g][i * kPitch + j]) = float4{x[j] * b, x[j + 1] * b, x[j + 2] * b, x[j + 3] * b};
-                M.upto[g][i] = upto;
-                if (i == 63) factors->end = upto;
-            } else {
-                const int e = exponent_of(largest(x));
-                unsigned hi[32], lo[32];
-                split(x, scale_of(e), hi, lo);
-                put_pieces(mine_out + Slot::g, i, 0, hi);
-                put_pieces(mine_out + Slot::g + 8192, i, 0, lo);
-                factors->attn[i] = unscale_of(e);
-                factors->q[i] = upto * inv_i;
+            if (!key) {
+                const int e = exponent_of(most);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+#pragma unroll 1
+                for (int j = 0; j < 64; j += 16) {
+                    unsigned hi[8] = {}, lo[8] = {};
+                    if (j <= last) {
+                        float x[16];
+                        tmem_read(mine + kU + j, x);
+                        split(x, scale_of(e), hi, lo);
+                    }
+                    put_pieces(mine_out + Slot::g, i, j / 8, hi);
+                    put_pieces(mine_out + Slot::g + 8192, i, j / 8, lo);
+                }
+                factors->attn[i] = unscale_of(e) * M.inv[i];
             }
             group_sync(g);
-            float *a = M.a[g], *a21 = a + 32 * kPitch, *a12 = a + 32, *a22 = a21 + 32;
-            if (w4 >= 2) {  // a warp each: the inverses of the two quarters on the diagonal
-                float *block = w4 == 2 ? a : a22;
-                float c[32];
-                substitute(block, lane, c);
+            // T: inverses of the four blocks of 16 on the diagonal, by two warps; then of pairs of them: the lower left of
+            // [B 0; A C]^-1 is -C^-1 (A B^-1), whose second factor waits in the upper right
+            float *a = M.a[g];
+            const auto at = [&](int row, int col) { return a + row * kPitch + col; };
+            if (w4 >= 2) {
+                const int block = 32 * (w4 - 2) + (lane & 16);
+                float c[16];
+                substitute(at(block, block), lane & 15, c);
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) block[j * kPitch + lane] = c[j];
+                for (int j = 0; j < 16; ++j) *at(block + j, block + (lane & 15)) = c[j];
             }
             group_sync(g);
-            float out[8];
-            const int row = gt >> 2, col = gt % 4 * 8;
-            times(a21, a, row, col, 32, out);
-            *reinterpret_cast<float4 *>(a12 + row * kPitch + col) = float4{out[0], out[1], out[2], out[3]};
-            *reinterpret_cast<float4 *>(a12 + row * kPitch + col + 4) = float4{out[4], out[5], out[6], out[7]};
-            group_sync(g);
-            times(a22, a12, row, col, row + 1, out);
-            *reinterpret_cast<float4 *>(a21 + row * kPitch + col) = float4{-out[0], -out[1], -out[2], -out[3]};
-            *reinterpret_cast<float4 *>(a21 + row * kPitch + col + 4) = float4{-out[4], -out[5], -out[6], -out[7]};
-            group_sync(g);
-            // T's rows as operands: threads 0-63 for U, 64-127 for W
+            {
+                const int two = gt >> 6, row = (gt & 63) >> 2, col = (gt & 3) * 4;  // 64 threads each of two pairs
+                float *b = at(32 * two, 32 * two);
+                times<4>(b + 16 * kPitch, b, row, col, 16, 1.0f, b + 16);
+                group_sync(g);
+                times<4>(b + 16 * kPitch + 16, b + 16, row, col, 16, -1.0f, b + 16 * kPitch);
+                group_sync(g);
+                *reinterpret_cast<float4 *>(b + 16 + row * kPitch + col) = float4{0, 0, 0, 0};
+            }
+            {
+                const int row = gt >> 2, col = (gt & 3) * 8;
+                group_sync(g);
+                times<8>(at(32, 0), at(0, 0), row, col, 32, 1.0f, at(0, 32));
+                group_sync(g);
+                times<8>(at(32, 32), at(0, 32), row, col, 8 * w4 + 8, -1.0f, at(32, 0));
+                group_sync(g);
+            }
+        }
+        __syncthreads();  // T's rows take V's place
+        if (there) {
+            // as operands: threads 0-63 for U, 64-127 for W. They wait in W's place.
+            const int i = gt & 63, last = w4 & 1 ? 48 : 16;
+            const bool key = gt >= 64;
+            const float *a_row = &M.a[g][i * kPitch], *by = key ? M.beta_w[g] : M.beta[g];
+            const unsigned waiting = mine + kWAt + 64 * g;
+            float most = 0.0f;
+#pragma unroll 1
+            for (int j = 0; j <= last; j += 16) {
+                float x[16];
 #pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(a + i * kPitch + j);
-                x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 t = *reinterpret_cast<const float4 *>(a_row + j + e), b = *reinterpret_cast<const float4 *>(by + j + e);
+                    x[e] = t.x * b.x, x[e + 1] = t.y * b.y, x[e + 2] = t.z * b.z, x[e + 3] = t.w * b.w;
+                }
+                most = largest(most, x);
+                tmem_write(waiting + j, x);
             }
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                const float by = key ? M.beta[g][j] * M.upto[g][j] * M.inv[64 + j] : M.beta[g][j];
-                x[j] = j <= i ? x[j] * by : 0.0f;
-            }
-            const float most = largest(x);
             if (past(most)) M.bad[g] = 1;
             const int e = exponent_of(most);
-            unsigned hi[32], lo[32];
-            split(x, scale_of(e), hi, lo);
-            put_pieces(key ? M.tw[0] : M.tu[g][0], key ? g * 64 + i : i, 0, hi);
-            put_pieces(key ? M.tw[1] : M.tu[g][1], key ? g * 64 + i : i, 0, lo);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            unsigned char *t_hi = key ? M.tw[0] : M.tu[g][0], *t_lo = key ? M.tw[1] : M.tu[g][1];
+            const int t_row = key ? g * 64 + i : i;
+#pragma unroll 1
+            for (int j = 0; j < 64; j += 16) {
+                unsigned hi[8] = {}, lo[8] = {};
+                if (j <= last) {
+                    float x[16];
+                    tmem_read(waiting + j, x);
+                    split(x, scale_of(e), hi, lo);
+                }
+                put_pieces(t_hi, t_row, j / 8, hi);
+                put_pieces(t_lo, t_row, j / 8, lo);
+            }
             (key ? M.inv_tw[g] : M.inv_tu[g])[i] = unscale_of(e);
         } else if (gt >= 64) {  // rows that no head has
             const unsigned zero[32] = {};
@@ -271,50 +422,66 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
         tc_fence_after();
         if (warp == 0) {
             if (elect_one()) {
-                for (int w = 0; w < 2 && pair + w < slab.ratio; ++w)  // U^T: lanes are value channels
-                    for (int product = 0; product < 3; ++product)
+                const unsigned long long tu = sw128_desc(su32(M.tu[0][0])), tw = sw128_desc(su32(M.tw[0]));
+                const unsigned long long keys = turned_desc(su32(M.qk[0][0]) + 8192, 16384);
+#pragma unroll 1
+                for (int product = 0; product < 3; ++product) {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)  // U^T: lanes are value channels (of no head: nobody looks)
+#pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_f16_ts(tmem + 320 + 64 * w, tmem + 64 + 64 * w + (product == 0) * 32 + k * 8,
-                                       sw128_desc(su32(M.tu[w][product == 1])) + k * 2, idesc_f16(128, 64), product || k);
-                for (int product = 0; product < 3; ++product)
+                            mma_f16_ts(tmem + 320 + 64 * w, tmem + 64 + 64 * w + (product == 0) * 32 + k * 8, tu + w * 1024 + (product == 1) * 512 + k * 2,
+                                       idesc_f16(128, 64), product || k);
+#pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16(tmem + kWAt, sw128_desc(su32(M.tw[product == 0])) + k * 2,
-                                turned_desc(su32(M.qk[product == 1][0]) + 8192 + k * 2048, 16384), turned_idesc(128, D), product || k);
+                        mma_f16(tmem + kWAt, tw + (product == 0) * 1024 + k * 2, keys + (product == 1) * (kPanels * 1024) + k * 128, turned_idesc(128, D),
+                                product || k);
+                }
                 mma_commit(&M.done);
             }
             __syncwarp();
         }
         wait(&M.done, phase & 1), ++phase;
         tc_fence_after();
-        if (there) {
-            float u[64];
-            tmem_read(mine + kU, u);
+        if (pair + 2 + g < slab.ratio) fetch_v(h + 2 * n.key_heads);  // T's rows have been read
+        if (there && w4 < D / 32) {
             float *to = reinterpret_cast<float *>(mine_out + Slot::uu) + gt;
-            if (gt < D) {
+#pragma unroll 1
+            for (int i = 0; i < 64; i += 16) {
+                float u[16];
+                tmem_read(mine + kU + i, u);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) to[i * D] = u[i] * inv_v * M.inv_tu[g][i];
+                for (int e = 0; e < 16; ++e) to[(i + e) * D] = u[e] * inv_v * M.inv_tu[g][i + e];
             }
         }
         // W's rows: lane w4 * 32 + lane is row i of the pair's head `of`; this warpgroup has half of its channels
-        float w[kW];
-        tmem_read(mine + kWAt + g * kW, w);
         const int of = w4 >> 1, i = gt & 63;
-        const float inv = M.inv_tw[of][i];
-#pragma unroll
-        for (int c = 0; c < kW; ++c) w[c] *= inv;
-        M.w_max[g][gt] = largest(w);
+        float most = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < kW; c += 16) {
+            float w[16];
+            tmem_read(mine + kWAt + g * kW + c, w);
+            most = largest(most, w);
+        }
+        M.w_max[g][gt] = most;
         __syncthreads();
-        const float most = fmaxf(M.w_max[0][gt], M.w_max[1][gt]);
-        if (past(M.w_max[0][gt]) || past(M.w_max[1][gt])) M.bad[of] = 1;
+        most = larger(M.w_max[0][gt], M.w_max[1][gt], 0.0f);
+        const float inv_t = M.inv_tw[of][i];
+        if (past(most * inv_t)) M.bad[of] = 1;
         if (pair + of < slab.ratio) {
             unsigned char *out = slot + Slot::heads + (long long)(pair + of) * Slot::head_bytes;
             const int e = exponent_of(most);
-            unsigned hi[kW / 2], lo[kW / 2];
-            split(w, scale_of(e), hi, lo);
             const int panel = D == 128 ? g : 0, first = D == 128 ? 0 : g * 4;
-            put_pieces(out + Slot::w + panel * 8192, i, first, hi);
-            put_pieces(out + Slot::w + (kPanels + panel) * 8192, i, first, lo);
-            if (g == 0) reinterpret_cast<DeltaFactors *>(out + Slot::factors)->z[i] = unscale_of(e);
+#pragma unroll 1
+            for (int c = 0; c < kW; c += 16) {
+                float w[16];
+                unsigned hi[8], lo[8];
+                tmem_read(mine + kWAt + g * kW + c, w);
+                split(w, scale_of(e), hi, lo);
+                put_pieces(out + Slot::w + panel * 8192, i, first + c / 8, hi);
+                put_pieces(out + Slot::w + (kPanels + panel) * 8192, i, first + c / 8, lo);
+            }
+            if (g == 0) reinterpret_cast<DeltaFactors *>(out + Slot::factors)->z[i] = unscale_of(e) * inv_t;
         }
         tc_fence_before();
         __syncthreads();

@@ -16,7 +16,8 @@ cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, 
     const long long bytes = n.dim <= 64 ? DeltaSlot<64>::bytes(ratio) : DeltaSlot<128>::bytes(ratio);
     const int room = (int)((long long)STRATA_DELTA_WORKSPACE_BYTES / bytes);  // slots
     if (n.dim > 128 || r.count <= kShortRun || room < 1) return delta_step(n, a, r, s);
-    const bool vec = n.dim % 4 == 0 && a.q_stride % 4 == 0 && a.k_stride % 4 == 0 && mix_aligned16(a.q) && mix_aligned16(a.k);
+    const bool vec = n.dim % 4 == 0 && a.q_stride % 4 == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 && mix_aligned16(a.q) &&
+                     mix_aligned16(a.k) && mix_aligned16(a.v);
     // Whole runs where they fit; else as many runs as give each multiprocessor two value heads, and their chunks in turn.
     const int all = (r.count + kChunk - 1) / kChunk, heads = std::min(n.key_heads, room);
     int runs = std::max(1, std::min({r.segments, room / heads, (2 * 148 + heads * ratio - 1) / (heads * ratio)}));
