@@ -1,7 +1,7 @@
 // The chunked delta rule's second kernel: a run's state of one value head, from chunk to chunk (delta_chunk.cuh).
 //
-// A block has a run's value head. A thread of its eight working warps has a value channel (its TMEM lane) with half of the
-// state's keys, in F32 registers; the state and the differences go to TMEM as the products' 128-row operand straight from
+// A block has a run's value head. A thread of its sixteen working warps has a value channel (its TMEM lane) with a quarter of
+// the state's keys, in F32 registers; the state and the differences go to TMEM as the products' 128-row operand straight from
 // there, and what kernel one left comes through bulk copies as the narrow one:
 //   Z^T = S^T W^T,  R^T = S^T Q^T        128 value channels by 64 tokens, sums over keys
 //   D = U - Z;  new state's part = (E D)^T K        128 by D keys, sums over tokens; K's tile read the other way round
@@ -16,32 +16,31 @@ namespace {
 
 using namespace delta;
 
-constexpr int kWork = 256, kChainThreads = kWork + 128, kFetchWarp = 8, kIssueWarp = 9;
+constexpr int kWork = 512, kChainThreads = kWork + 64, kFetchWarp = 16, kIssueWarp = 17;
 
 template <int D>
 struct __align__(1024) ChainSmem {
-    unsigned char w[2][2 * D / 64][64 * 128];  // by stage: hi panels, lo panels
-    unsigned char q[2][2 * D / 64][64 * 128];
+    unsigned char w[2][2][D * 128];            // by stage: hi, lo; rows are key channels
+    unsigned char q[2][2 * D / 64][64 * 128];  // by stage: hi panels, lo panels
     unsigned char k[2 * D / 64][64 * 128];
     unsigned char g[2][64 * 128];  // hi, lo
     float u[64 * D];
     DeltaFactors factors[2];
-    float s_max[2][128];
-    float2 d_max[2][128];
-    float2 walk[2][128];
+    float s_max[4][128];
+    float2 d_max[4][128];  // also the sums of chunks that are walked
     unsigned long long w_full[2], w_empty[2], q_full[2], q_empty[2], f_full[2], f_empty[2], k_full, k_empty, g_full, g_empty, u_full, u_empty;
     unsigned long long s_ready, r_free, d_ready, y_ready, z_done, r_done, d_done, y_done;
     unsigned tmem;
     int abort_flag;
 };
 
-__device__ __forceinline__ void pair_sync(int w4) { asm volatile("bar.sync %0, 64;" ::"r"(1 + w4) : "memory"); }
-__device__ __forceinline__ void work_sync() { asm volatile("bar.sync 5, 256;" ::: "memory"); }
+__device__ __forceinline__ void lane_sync(int w4) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w4) : "memory"); }  // of the same lanes
+__device__ __forceinline__ void work_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
 
 template <int D>
 __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
-    constexpr int kHalf = D / 2;
+    constexpr int kPart = D / 4;  // keys of a thread; and 16 tokens
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     ChainSmem<D> &M = *reinterpret_cast<ChainSmem<D> *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -85,8 +84,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
     constexpr unsigned kS = 0, kSLo = D / 2, kD = 128, kZ = 192, kR = 256, kY = 320, kNew = 384;
     const Waits wait{&M.abort_flag, n.err};
 
-    // of 64512 registers, 168 a thread at the start, the working threads take 216 and the others keep 72
-    if (warp >= kFetchWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == kFetchWarp) {
         if (lane == 0) {
             const auto fetch = [&](void *to, const unsigned char *from, unsigned bytes, unsigned long long *full) {
@@ -132,22 +129,24 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
                 wait(&M.w_full[st], ph);
                 wait(&M.s_ready, now);
                 tc_fence_after();
-                const auto over_keys = [&](unsigned to, const void *tile) {  // lo hi, hi lo, hi hi
-                    const unsigned long long b = sw128_desc(su32(tile));
+                const unsigned long long w = turned_desc(su32(M.w[st]), 0), q = sw128_desc(su32(M.q[st]));
 #pragma unroll
-                    for (int product = 0; product < 3; ++product)
+                for (int product = 0; product < 3; ++product)  // lo hi, hi lo, hi hi
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k)
-                            mma_f16_ts(tmem + to, tmem + (product == 0 ? kSLo : kS) + k * 8, b + (product == 1) * kLoTile + k / 4 * 512 + k % 4 * 2,
-                                       idesc_f16(128, 64), product || k);
-                };
-                over_keys(kZ, M.w[st]);
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_f16_ts(tmem + kZ, tmem + (product == 0 ? kSLo : kS) + k * 8, w + (product == 1) * kLoTile + k * 128, turned_idesc(128, 64),
+                                   product || k);
                 mma_commit(&M.w_empty[st]);
                 mma_commit(&M.z_done);
                 wait(&M.q_full[st], ph);
                 wait(&M.r_free, now);
                 tc_fence_after();
-                over_keys(kR, M.q[st]);
+#pragma unroll
+                for (int product = 0; product < 3; ++product)
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8, q + (product == 1) * kLoTile + k / 4 * 512 + k % 4 * 2,
+                                   idesc_f16(128, 64), product || k);
                 mma_commit(&M.q_empty[st]);
                 mma_commit(&M.r_done);
                 wait(&M.k_full, c & 1);
@@ -176,41 +175,44 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
         }
         __syncwarp();
     } else if (warp < kFetchWarp) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int w4 = warp & 3, half = warp >> 2, v = w4 * 32 + lane;
+        const int w4 = warp & 3, part = warp >> 2, v = w4 * 32 + lane;
         const unsigned lanes = tmem + ((unsigned)(w4 * 32) << 16);
         const bool in = v < n.dim;
         const auto arrive = [&](unsigned long long *b) {
             __syncwarp();
             if (lane == 0) bar_arrive(b);
         };
-        float *state = n.state + ((long long)me.sequence * n.dim + half * kHalf) * vw + (long long)h * n.dim + v;
-        float S[kHalf];
+        float *state = n.state + ((long long)me.sequence * n.dim + part * kPart) * vw + (long long)h * n.dim + v;
+        float S[kPart];
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) S[i] = in && half * kHalf + i < n.dim ? state[i * vw] : 0.0f;
+        for (int i = 0; i < kPart; ++i) S[i] = in && part * kPart + i < n.dim ? state[i * vw] : 0.0f;
         unsigned live = 0;
         bool owed = false;            // the chunk before has results in TMEM
         float inv_r = 0, inv_y = 0;   // their scales taken back
-        // results of chunk c: its tokens half * 32 ..
+        // results of chunk c: its tokens part * 16 ..
         const auto write_y = [&](int c) {
-            const float *fq = M.factors[c & 1].q + half * 32, *fa = M.factors[c & 1].attn + half * 32;
-            const int t0 = begin + c * kChunk + half * 32, left = in ? me.tokens - t0 : 0;
+            const float4 *fq = reinterpret_cast<const float4 *>(M.factors[c & 1].q + part * 16);
+            const float4 *fa = reinterpret_cast<const float4 *>(M.factors[c & 1].attn + part * 16);
+            const int t0 = begin + c * kChunk + part * 16, left = in ? me.tokens - t0 : 0;
             float *y = A.y + (first + t0) * vw + (long long)h * n.dim + v;
-#pragma unroll 1
-            for (int at = 0; at < 32; at += 16) {
-                float R[16], Y[16];
-                tmem_read(lanes + kR + half * 32 + at, R);
-                tmem_read(lanes + kY + half * 32 + at, Y);
+            float R[16], Y[16];
+            tmem_read(lanes + kR + part * 16, R);
+            tmem_read(lanes + kY + part * 16, Y);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) R[i] = fmaf(R[i] * inv_r, fq[at + i], Y[i] * inv_y * fa[at + i]);
-                if (left >= at + 16) {
+            for (int i = 0; i < 4; ++i) {
+                const float4 q = fq[i], a = fa[i];
+                R[4 * i] = fmaf(R[4 * i] * inv_r, q.x, Y[4 * i] * inv_y * a.x);
+                R[4 * i + 1] = fmaf(R[4 * i + 1] * inv_r, q.y, Y[4 * i + 1] * inv_y * a.y);
+                R[4 * i + 2] = fmaf(R[4 * i + 2] * inv_r, q.z, Y[4 * i + 2] * inv_y * a.z);
+                R[4 * i + 3] = fmaf(R[4 * i + 3] * inv_r, q.w, Y[4 * i + 3] * inv_y * a.w);
+            }
+            if (left >= 16) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i, y += vw) *y = R[i];
-                } else {
+                for (int i = 0; i < 16; ++i, y += vw) *y = R[i];
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i, y += vw)
-                        if (at + i < left) *y = R[i];
-                }
+                for (int i = 0; i < 16; ++i, y += vw)
+                    if (i < left) *y = R[i];
             }
             arrive(&M.f_empty[c & 1]);
         };
@@ -222,34 +224,35 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
             if (f.walk) {
                 if (owed) write_y(c - 1);
                 owed = false;
-                // token by token: a channel's two threads add up their halves of the keys
+                // token by token: a channel's four threads add up their parts of the keys
                 const int t0 = begin + c * kChunk, tokens = min(kChunk, me.tokens - t0);
                 for (int t = 0; t < tokens; ++t) {
                     const long long row = first + t0 + t;
                     // (volatile: one after another, not 128 registers of them)
-                    const volatile float *kp = A.k + row * A.k_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
-                    const volatile float *qp = A.q + row * A.q_stride + (long long)(slab.head0 + head_l) * n.dim + half * kHalf;
+                    const volatile float *kp = A.k + row * A.k_stride + (long long)(slab.head0 + head_l) * n.dim + part * kPart;
+                    const volatile float *qp = A.q + row * A.q_stride + (long long)(slab.head0 + head_l) * n.dim + part * kPart;
                     const float a = A.decay[row * n.value_heads + h], b = A.beta[row * n.value_heads + h];
                     const float value = in ? A.v[row * A.v_stride + (long long)h * n.dim + v] : 0.0f;
                     float p = 0.0f, y = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < kHalf; ++i) {
+                    for (int i = 0; i < kPart; ++i) {
                         S[i] *= a;
-                        p = fmaf(S[i], half * kHalf + i < n.dim ? kp[i] : 0.0f, p);
+                        p = fmaf(S[i], part * kPart + i < n.dim ? kp[i] : 0.0f, p);
                     }
-                    M.walk[half][v].x = p;
-                    pair_sync(w4);
-                    const float d = b * (value - (M.walk[0][v].x + M.walk[1][v].x));
+                    M.d_max[part][v].x = p;
+                    lane_sync(w4);
+                    const float d = b * (value - ((M.d_max[0][v].x + M.d_max[1][v].x) + (M.d_max[2][v].x + M.d_max[3][v].x)));
 #pragma unroll
-                    for (int i = 0; i < kHalf; ++i) {
-                        if (half * kHalf + i < n.dim) {
+                    for (int i = 0; i < kPart; ++i) {
+                        if (part * kPart + i < n.dim) {
                             S[i] = fmaf(kp[i], d, S[i]);
                             y = fmaf(S[i], qp[i], y);
                         }
                     }
-                    M.walk[half][v].y = y;
-                    pair_sync(w4);
-                    if (half == 0 && in) A.y[row * vw + (long long)h * n.dim + v] = M.walk[0][v].y + M.walk[1][v].y;
+                    M.d_max[part][v].y = y;
+                    lane_sync(w4);
+                    if (part == 0 && in)
+                        A.y[row * vw + (long long)h * n.dim + v] = (M.d_max[0][v].y + M.d_max[1][v].y) + (M.d_max[2][v].y + M.d_max[3][v].y);
                 }
                 arrive(&M.f_empty[st]);
                 wait(&M.u_full, c & 1);
@@ -259,19 +262,19 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
             const unsigned now = live & 1;
             ++live;
             // the state as an operand
-            M.s_max[half][v] = largest(0.0f, S);
-            pair_sync(w4);
-            const int es = exponent_of(larger(M.s_max[0][v], M.s_max[1][v], 0.0f));
+            M.s_max[part][v] = largest(0.0f, S);
+            lane_sync(w4);
+            const int es = exponent_of(larger(larger(M.s_max[0][v], M.s_max[1][v], M.s_max[2][v]), M.s_max[3][v], 0.0f));
             const float inv_s = unscale_of(es);
 #pragma unroll
-            for (int i = 0; i < kHalf; i += 16) {
+            for (int i = 0; i < kPart; i += 16) {
                 float x[16];
                 unsigned hi[8], lo[8];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[e] = S[i + e];
                 split(x, scale_of(es), hi, lo);
-                tmem_write(lanes + kS + (half * kHalf + i) / 2, hi);
-                tmem_write(lanes + kSLo + (half * kHalf + i) / 2, lo);
+                tmem_write(lanes + kS + (part * kPart + i) / 2, hi);
+                tmem_write(lanes + kSLo + (part * kPart + i) / 2, lo);
             }
             tmem_written();
             arrive(&M.s_ready);
@@ -285,47 +288,34 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
             wait(&M.u_full, c & 1);
             wait(&M.z_done, now);
             tc_fence_after();
-            float d[32];
-            const float *u = M.u + half * 32 * D + (v < D ? v : 0), *fz = f.z + half * 32, *fk = f.k + half * 32;
-            const float by = v < D ? -inv_s : 0.0f;
-            float most_d = 0.0f, most_e = 0.0f;
-            tmem_read(lanes + kZ + half * 32, d);
+            float d[16], e[16];
+            const float *u = M.u + part * 16 * D + (v < D ? v : 0);
+            const float4 *fz = reinterpret_cast<const float4 *>(f.z + part * 16), *fk = reinterpret_cast<const float4 *>(f.k + part * 16);
+            const float by = v < D ? -inv_s : 0.0f, keep = v < D ? 1.0f : 0.0f;
+            tmem_read(lanes + kZ + part * 16, d);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                d[i] = fmaf(d[i] * by, fz[i], v < D ? u[i * D] : 0.0f);
-                d[i + 1] = fmaf(d[i + 1] * by, fz[i + 1], v < D ? u[i * D + D] : 0.0f);
-                most_d = larger(most_d, d[i], d[i + 1]);
-                most_e = larger(most_e, d[i] * fk[i], d[i + 1] * fk[i + 1]);
+            for (int i = 0; i < 16; i += 4) {
+                const float4 z = fz[i / 4], k = fk[i / 4];
+                d[i] = fmaf(d[i] * by, z.x, u[i * D] * keep), d[i + 1] = fmaf(d[i + 1] * by, z.y, u[i * D + D] * keep);
+                d[i + 2] = fmaf(d[i + 2] * by, z.z, u[i * D + 2 * D] * keep), d[i + 3] = fmaf(d[i + 3] * by, z.w, u[i * D + 3 * D] * keep);
+                e[i] = d[i] * k.x, e[i + 1] = d[i + 1] * k.y, e[i + 2] = d[i + 2] * k.z, e[i + 3] = d[i + 3] * k.w;
             }
             arrive(&M.u_empty);
-            M.d_max[half][v] = float2{most_d, most_e};
-            pair_sync(w4);
-            const float2 m0 = M.d_max[0][v], m1 = M.d_max[1][v];
-            const int ed = exponent_of(larger(m0.x, m1.x, 0.0f)), ee = exponent_of(larger(m0.y, m1.y, 0.0f));
-#pragma unroll
-            for (int i = 0; i < 32; i += 16) {
-                float x[16];
-                unsigned hi[8], lo[8];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = d[i + e] * fk[i + e];
-                split(x, scale_of(ee), hi, lo);
-                tmem_write(lanes + kD + (half * 32 + i) / 2, hi);
-                tmem_write(lanes + kD + 32 + (half * 32 + i) / 2, lo);
-            }
+            M.d_max[part][v] = float2{largest(0.0f, d), largest(0.0f, e)};
+            lane_sync(w4);
+            const float2 m0 = M.d_max[0][v], m1 = M.d_max[1][v], m2 = M.d_max[2][v], m3 = M.d_max[3][v];
+            const int ed = exponent_of(larger(larger(m0.x, m1.x, m2.x), m3.x, 0.0f)), ee = exponent_of(larger(larger(m0.y, m1.y, m2.y), m3.y, 0.0f));
+            unsigned hi[8], lo[8];
+            split(e, scale_of(ee), hi, lo);
+            tmem_write(lanes + kD + part * 8, hi);
+            tmem_write(lanes + kD + 32 + part * 8, lo);
             tmem_written();
             arrive(&M.d_ready);
+            split(d, scale_of(ed), hi, lo);
             wait(&M.r_done, now);  // the state's halves have been read
             tc_fence_after();
-#pragma unroll
-            for (int i = 0; i < 32; i += 16) {
-                float x[16];
-                unsigned hi[8], lo[8];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = d[i + e];
-                split(x, scale_of(ed), hi, lo);
-                tmem_write(lanes + kS + (half * 32 + i) / 2, hi);
-                tmem_write(lanes + kS + 32 + (half * 32 + i) / 2, lo);
-            }
+            tmem_write(lanes + kS + part * 8, hi);
+            tmem_write(lanes + kS + 32 + part * 8, lo);
             tmem_written();
             arrive(&M.y_ready);
             inv_y = unscale_of(ed);
@@ -334,9 +324,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
             tc_fence_after();
             const float inv_e = unscale_of(ee), end = f.end;
 #pragma unroll
-            for (int i = 0; i < kHalf; i += 16) {
+            for (int i = 0; i < kPart; i += 16) {
                 float x[16];
-                tmem_read(lanes + kNew + half * kHalf + i, x);
+                tmem_read(lanes + kNew + part * kPart + i, x);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) S[i + e] = fmaf(x[e], inv_e, S[i + e] * end);
             }
@@ -351,8 +341,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
         work_sync();
         if (!*(volatile int *)&M.abort_flag) {
 #pragma unroll
-            for (int i = 0; i < kHalf; ++i)
-                if (in && half * kHalf + i < n.dim) state[i * vw] = S[i];
+            for (int i = 0; i < kPart; ++i)
+                if (in && part * kPart + i < n.dim) state[i * vw] = S[i];
         }
     }
     tc_fence_before();

@@ -14,7 +14,7 @@
 //
 // Workspace: a slot for each run, key head and chunk of a slab, in the layout that the second kernel's tensor-core operands
 // have in shared memory (rows of 128 bytes, 128-byte swizzle): Q and K [64 tokens][D], hi and lo; then for each of the key
-// head's value heads W [64][D], hi and lo, the products G (q . k) [64][64], hi and lo, U [64][D] in F32 and the rows' factors.
+// head's value heads W^T [D][64], hi and lo, the products G (q . k) [64][64], hi and lo, U [64][D] in F32 and the rows' factors.
 #pragma once
 #include "mixers.cuh"
 #include "pf_gemm.cuh"
@@ -139,7 +139,8 @@ __device__ __forceinline__ void put_pieces(unsigned char *tile, int r, int first
 __device__ __forceinline__ unsigned long long turned_desc(unsigned smem_addr, unsigned panel) {
     return (unsigned long long)((smem_addr & 0x3FFFFu) >> 4) | ((unsigned long long)(panel >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ unsigned turned_idesc(int M, int N) { return idesc_f16(M, N) | (1u << 16); }
+__device__ __forceinline__ unsigned turned_idesc(int M, int N) { return idesc_f16(M, N) | (1u << 16); }  // the narrow operand
+constexpr unsigned kTurnedWide = 1u << 15;                                                                // the 128-row one
 
 // Waits of a block's threads, with a limit; past it, all of them let everything through and the block reports.
 struct Waits {

@@ -1,14 +1,16 @@
 // The chunked delta rule's first kernel: what a chunk needs that does not depend on the state (delta_chunk.cuh).
 //
-// A block has a run's chunk and key head, and takes the head's value heads two at a time, one by each warpgroup:
+// A block has a run's chunk and key head, and takes the head's value heads one after another:
 //   [Q; K] K^T      128 rows by 64, once for all of them
-//   A, G (q . k)    a thread a row, from its TMEM lane
+//   A, G (q . k)    a row's two threads have half of its columns each, from their TMEM lane
 //   T = (I + A)^-1  of blocks of 16 by substitution, a column a lane, then of blocks twice as large twice, F32 throughout
-//   U^T = V^T (T diag(beta))^T   a lane a value channel
-//   W = (T diag(beta P)) K       both heads' 64 rows as one operand; K's tile as it lies, read the other way round
-// Bound by instructions, most of them the splits into halves: what a row needs twice (its largest value first) waits in TMEM,
-// and columns go by 16 in loops that are not unrolled, since code that a block runs once comes slower than it executes (with all
-// 64 columns unrolled a prompt of 2048 tokens over 32 heads of 128 took 210 us, most of them without an instruction to issue).
+//   U^T = V^T (T diag(beta))^T      a lane a value channel
+//   W^T = K^T (T diag(beta P))^T    a lane a key channel; K's tile as it lies, read the other way round
+// Bound by instructions, most of them the splits into halves, and by the way from one step to the next: two blocks a
+// multiprocessor, 100 KB and half of TMEM each, so that one's steps run in the other's waits. What becomes operands goes
+// through shared memory and bulk copies. Code that a block runs once comes slower than it executes, so it is kept short: with a
+// thread for a whole row, all 64 columns unrolled, a prompt of 2048 tokens over 32 heads of 128 took 210 us, most of them
+// without an instruction to issue.
 #include "delta_chunk.cuh"
 
 #include <atomic>
@@ -19,34 +21,41 @@ namespace {
 using namespace delta;
 
 constexpr int kPrepareThreads = 256, kPitch = 68;
+constexpr float kWScale = 0x1p-19f;  // of W's sums, which are 2^34 at most: 64 terms of two factors below 2^14
 
 template <int D>
 struct __align__(1024) PrepareSmem {
     unsigned char qk[2][D / 64][128 * 128];  // hi, lo: panels of 64 channels; rows 0-63 Q, 64-127 K
-    union {                                  // V's rows until they are in TMEM, then T's
-        float v[2][64 * D];                  // by head
-        struct {
-            unsigned char tw[2][128 * 128];    // T diag(beta P) over K's scales: hi, lo; two heads' 64 rows
-            unsigned char tu[2][2][64 * 128];  // by head: T diag(beta), hi, lo
-        };
+    unsigned char more[D == 64 ? 4 : 1][D == 64 ? 64 * 128 : 16];
+    union {  // a value head's V, until it is in TMEM; A, then T; W^T, hi and lo
+        float v[64 * D];
+        float a[64 * kPitch];
+        unsigned char w[2][D * 128];
     };
-    float a[2][64 * kPitch];  // A, then T
-    float inv[128];           // Q's and K's scales taken back
-    // by head: decays; products of decays up to a token in its half; strengths, and times decays up to the token over K's scale;
-    // K's scales taken back, the lower half's times the decays after a token in it
-    float decay[2][64], upto[2][64], beta[2][64], beta_w[2][64], inv_k[2][64];
-    float inv_tw[2][64], inv_tu[2][64];
-    float w_max[2][128];
-    int bad_key, bad[2], abort_flag;
+    float inv[128];  // Q's and K's scales taken back
+    // decays; products of decays up to a token in its half; strengths, and times decays up to the token over K's scale; K's
+    // scales taken back, the lower half's times the decays after a token in it
+    float decay[64], upto[64], beta[64], beta_w[64], inv_k[64];
+    float inv_tu[64];
+    float most[2][2][128];  // a row's largest values, by warpgroup; two that are used in turn
+    int bad_key, bad, abort_flag;
     unsigned tmem;
     unsigned long long done;
+
+    // Tiles [64][64] of halves, in Q's place once it is not needed any more: G (q . k), hi and lo, and when that has been copied
+    // out T diag(beta P) over K's scales; T diag(beta)
+    __device__ __forceinline__ unsigned char *tile(int i) { return D == 128 ? qk[i >> 1][i & 1] : more[i]; }
 };
 
-__device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
 __device__ __forceinline__ void add2(unsigned long long &d, unsigned long long a, unsigned long long b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
 }
 __device__ __forceinline__ ulonglong2 load22(const float *p) { return *reinterpret_cast<const ulonglong2 *>(p); }
+__device__ __forceinline__ void bulk_out(void *to, const void *from, unsigned bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(su32(from)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_out_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_out_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 // x of (I + L) x = e_c, L the strictly lower part of 16 rows at l
 __device__ __forceinline__ void substitute(const float *l, int c, float (&x)[16]) {
@@ -64,27 +73,21 @@ __device__ __forceinline__ void substitute(const float *l, int c, float (&x)[16]
         x[i] = (s[0] + s[1]) + (s[2] + s[3]);
     }
 }
-// W columns (4 or 8) from c of row r of sign X Y: rows of X at x, Y at y; `terms` (a multiple of 4) of X's row count
-template <int W>
+// Four columns from c of row r of sign X Y: rows of X at x, Y at y; `terms` (a multiple of 4) of X's row count
 __device__ __forceinline__ void times(const float *x, const float *y, int r, int c, int terms, float sign, float *to) {
-    unsigned long long s[W / 2] = {};
+    unsigned long long s0 = 0, s1 = 0;
 #pragma unroll 2
     for (int j = 0; j < terms; j += 4) {
         const float4 f = *reinterpret_cast<const float4 *>(x + r * kPitch + j);
         const float g[4] = {f.x * sign, f.y * sign, f.z * sign, f.w * sign};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float *row = y + (j + e) * kPitch + c;
-#pragma unroll
-            for (int w = 0; w < W; w += 4) {
-                const ulonglong2 b = load22(row + w);
-                add2(s[w / 2], pack2(g[e], g[e]), b.x);
-                add2(s[w / 2 + 1], pack2(g[e], g[e]), b.y);
-            }
+            const ulonglong2 b = load22(y + (j + e) * kPitch + c);
+            add2(s0, pack2(g[e], g[e]), b.x);
+            add2(s1, pack2(g[e], g[e]), b.y);
         }
     }
-#pragma unroll
-    for (int w = 0; w < W; w += 4) *reinterpret_cast<ulonglong2 *>(to + r * kPitch + c + w) = ulonglong2{s[w / 2], s[w / 2 + 1]};
+    *reinterpret_cast<ulonglong2 *>(to + r * kPitch + c) = ulonglong2{s0, s1};
 }
 // Products over lanes: of this one's and those before, and of those after.
 __device__ __forceinline__ float product_upto(float x, int lane) {
@@ -108,12 +111,13 @@ __device__ __forceinline__ float product_after(float x, int lane) {
 
 // VEC: rows of q, k and v can be read four channels at a time.
 template <int D, bool VEC>
-__global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
+__global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
-    constexpr int kPanels = D / 64, kW = D / 2;
+    constexpr int kPanels = D / 64;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     PrepareSmem<D> &M = *reinterpret_cast<PrepareSmem<D> *>(smem_raw);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = tid >> 7, gt = tid & 127, w4 = warp & 3;
+    // half of the columns, row
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = tid >> 7, gt = tid & 127, w4 = warp & 3;
     kv8_enter();
     const int chunk = slab.chunk0 + (int)(blockIdx.x % slab.chunks), head = slab.head0 + (int)(blockIdx.x / slab.chunks % slab.heads);
     const int run = slab.run0 + (int)(blockIdx.x / slab.chunks / slab.heads), t0 = chunk * kChunk;
@@ -123,40 +127,39 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
     const long long row0 = (long long)run * r.count + t0;
     unsigned char *slot = slab.slots + blockIdx.x * slab.slot_bytes;
 
-    // V's rows of a value head to shared memory, by its warpgroup; zeros behind the run's end and past dim
+    // V's rows of a value head to shared memory; zeros behind the run's end and past dim
     const auto fetch_v = [&](int h) {
         const float *from = A.v + row0 * A.v_stride + (long long)h * n.dim;
         constexpr int kPiece = VEC ? 4 : 1;
 #pragma unroll 4
-        for (int at = gt * kPiece; at < 64 * D; at += 128 * kPiece) {
+        for (int at = tid * kPiece; at < 64 * D; at += kPrepareThreads * kPiece) {
             const int j = at / D, c = at % D;
             const bool in = j < tokens && c < n.dim;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(su32(&M.v[g][at])), "l"(in ? from + j * A.v_stride + c : A.v),
-                         "n"(kPiece * 4), "r"(in ? kPiece * 4 : 0)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(su32(&M.v[at])), "l"(in ? from + j * A.v_stride + c : A.v), "n"(kPiece * 4),
+                         "r"(in ? kPiece * 4 : 0)
                          : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (g < slab.ratio) fetch_v(head + g * n.key_heads);
+    fetch_v(head);
     if (tid == 0) {
         bar_init(&M.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         M.abort_flag = M.bad_key = 0;
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&M.tmem)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(su32(&M.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = M.tmem, mine = tmem + ((unsigned)(w4 * 32) << 16);
-    // columns: [Q; K] K^T; by head V's halves; W; by head U^T, whose place and W's keep rows until they are split
-    const unsigned kRaw = 0, kV = 64 + 64 * g, kWAt = 192, kU = 320 + 64 * g;
+    constexpr unsigned kRaw = 0, kV = 64, kU = 128, kW = 192;  // columns: [Q; K] K^T; V's halves; U^T; W^T
     const Waits wait{&M.abort_flag, n.err};
     unsigned phase = 0;
 
-    // Q's and K's rows, a power of two each
+    // Q's and K's rows, a power of two each: 16 a warp
     constexpr int kLanes = D / 4, kRows = 32 / kLanes;
 #pragma unroll 1
     for (int at = 0; at < 16; at += 8 * kRows) {
@@ -213,208 +216,178 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
         if (lane == 0) {
             for (int i = 0; i < 4 * kPanels; ++i) {  // Q: hi, lo; K: hi, lo
                 const int part = i % (2 * kPanels);
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], 8192;" ::"l"(slot + i * 8192),
-                             "r"(su32(M.qk[part / kPanels][part % kPanels]) + (i / (2 * kPanels)) * 8192)
-                             : "memory");
+                bulk_out(slot + i * 8192, M.qk[part / kPanels][part % kPanels] + (i / (2 * kPanels)) * 8192, 8192);
             }
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            bulk_out_commit();
         }
         __syncwarp();
     }
 
 #pragma unroll 1
-    for (int pair = 0; pair < slab.ratio; pair += 2) {
-        const int m = pair + g, h = head + m * n.key_heads;
-        const bool there = m < slab.ratio;
-        unsigned char *mine_out = slot + Slot::heads + (long long)m * Slot::head_bytes;
-        DeltaFactors *factors = reinterpret_cast<DeltaFactors *>(mine_out + Slot::factors);
-        if (gt == 0) M.bad[g] = 0;
-        float inv_v = 0.0f;
-        if (there) {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            group_sync(g);  // V is there, and bad[g] has been cleared
-            if (w4 == 0) {
-                // decays and strengths, two tokens a lane; rows behind the run's end change nothing
-                float a[2], b[2];
+    for (int m = 0; m < slab.ratio; ++m) {
+        const int h = head + m * n.key_heads;
+        unsigned char *out = slot + Slot::heads + (long long)m * Slot::head_bytes;
+        DeltaFactors *factors = reinterpret_cast<DeltaFactors *>(out + Slot::factors);
+        if (tid == 0) M.bad = 0;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();  // V is there, and bad has been cleared
+        if (warp == 0) {
+            // decays and strengths, two tokens a lane; rows behind the run's end change nothing
+            float a[2], b[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const bool in = lane + 32 * e < tokens;
-                    const long long at = (row0 + lane + 32 * e) * n.value_heads + h;
-                    a[e] = in ? A.decay[at] : 1.0f;
-                    b[e] = in ? A.beta[at] : 0.0f;
-                }
-                if (past(larger(larger(a[0], a[1], b[0]), b[1], 0.0f))) M.bad[g] = 1;
-                const float upto[2] = {product_upto(a[0], lane), product_upto(a[1], lane)};
-                const float after[2] = {product_after(a[0], lane), product_after(a[1], lane)};
-                const float low = __shfl_sync(0xffffffffu, upto[0], 31), high = __shfl_sync(0xffffffffu, upto[1], 31);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int t = lane + 32 * e;
-                    const float p = e ? upto[1] * low : upto[0], inv_k = M.inv[64 + t];
-                    M.decay[g][t] = a[e];
-                    M.upto[g][t] = upto[e];
-                    M.beta[g][t] = b[e];
-                    M.beta_w[g][t] = b[e] * p * inv_k;
-                    M.inv_k[g][t] = e ? inv_k : inv_k * after[0];
-                    factors->q[t] = p * M.inv[t];
-                    factors->k[t] = (e ? after[1] : after[0] * high) * inv_k;
-                    if (t == 63) factors->end = p;
-                }
+            for (int e = 0; e < 2; ++e) {
+                const bool in = lane + 32 * e < tokens;
+                const long long at = (row0 + lane + 32 * e) * n.value_heads + h;
+                a[e] = in ? A.decay[at] : 1.0f;
+                b[e] = in ? A.beta[at] : 0.0f;
             }
-            // V's column of this lane to TMEM
-            const float *column = M.v[g] + (gt < D ? gt : 0);
-            float most = 0.0f;
-#pragma unroll 1
-            for (int j = 0; j < 64; j += 16) {
-                float v[16];
+            if (past(larger(larger(a[0], a[1], b[0]), b[1], 0.0f))) M.bad = 1;
+            const float upto[2] = {product_upto(a[0], lane), product_upto(a[1], lane)};
+            const float after[2] = {product_after(a[0], lane), product_after(a[1], lane)};
+            const float low = __shfl_sync(0xffffffffu, upto[0], 31), high = __shfl_sync(0xffffffffu, upto[1], 31);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = column[(j + e) * D];
-                most = largest(most, v);
+            for (int e = 0; e < 2; ++e) {
+                const int t = lane + 32 * e;
+                const float p = e ? upto[1] * low : upto[0], inv_k = M.inv[64 + t];
+                M.decay[t] = a[e];
+                M.upto[t] = upto[e];
+                M.beta[t] = b[e];
+                M.beta_w[t] = b[e] * p * inv_k;
+                M.inv_k[t] = e ? inv_k : inv_k * after[0];
+                factors->q[t] = p * M.inv[t];
+                factors->k[t] = (e ? after[1] : after[0] * high) * inv_k;
+                if (t == 63) factors->end = p;
             }
+        }
+        float inv_v;
+        {  // V's column of this lane to TMEM, 32 tokens
+            const float *column = M.v + half * 32 * D + (gt < D ? gt : 0);
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = column[j * D];
+            M.most[0][half][gt] = largest(0.0f, v);
+            __syncthreads();  // the decays are there, too
+            const float most = larger(M.most[0][0][gt], M.most[0][1][gt], 0.0f);
             const int e = exponent_of(most);
             inv_v = unscale_of(e);
-            if (past(most)) M.bad[g] = 1;
-#pragma unroll 1
-            for (int j = 0; j < 64; j += 16) {
-                float v[16];
-                unsigned hi[8], lo[8];
-#pragma unroll
-                for (int u = 0; u < 16; ++u) v[u] = column[(j + u) * D];
-                split(v, scale_of(e), hi, lo);
-                tmem_write(mine + kV + j / 2, hi);
-                tmem_write(mine + kV + 32 + j / 2, lo);
-            }
+            if (past(most)) M.bad = 1;
+            unsigned hi[16], lo[16];
+            split(v, scale_of(e), hi, lo);
+            tmem_write(mine + kV + half * 16, hi);
+            tmem_write(mine + kV + 32 + half * 16, lo);
             tmem_written();
         }
-        if (pair == 0) wait(&M.done, phase & 1), ++phase;
+        if (m == 0) wait(&M.done, phase & 1), ++phase;
         tc_fence_after();
-        if (there) {
-            group_sync(g);  // the decays are there
-            // rows 0-63: products of queries, 64-127: of keys, each times G over the column's scale. Row i of the upper half: the
-            // decays up to it in that half times those after column j in the lower one; else their product grows from j = i down.
+        if (tid == 0) bulk_out_read();  // Q's tile, or the last head's T
+        {
+            // Rows 0-63: products of queries, 64-127: of keys, each times G over the column's scale. Where row and column are of the
+            // same half of the tokens, the product of decays grows from the diagonal; else it is that up to the row in its half times
+            // that after the column in its own. Columns of the upper half mean nothing to rows of the lower one.
             const int i = gt & 63;
-            const bool key = gt >= 64, upper = w4 & 1;
-            const float row_factor = key ? M.inv[gt] * M.beta[g][i] : 1.0f, far = M.upto[g][i];
-            float *a_row = &M.a[g][i * kPitch];
-            float p = 1.0f, most = 0.0f;
-            const int last = upper ? 48 : 16;  // the last columns that count
-#pragma unroll 1
-            for (int j = last; j >= 0; j -= 16) {
-                float x[16];
-                tmem_read(mine + kRaw + j, x);
-                if (upper && j < 32) {
+            const bool key = gt >= 64, upper = w4 & 1, empty = !upper && half;
+            float *a_row = &M.a[i * kPitch + 32 * half];
+            float x[32], most = 0.0f;
+            if (!empty) {
+                tmem_read(mine + kRaw + 32 * half, x);
+                if (upper && !half) {
+                    const float far = M.upto[i];
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const float4 c = *reinterpret_cast<const float4 *>(&M.inv_k[g][j + e]);
-                        x[e] *= c.x * far, x[e + 1] *= c.y * far, x[e + 2] *= c.z * far, x[e + 3] *= c.w * far;
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 c = *reinterpret_cast<const float4 *>(&M.inv_k[j]);
+                        x[j] *= c.x * far, x[j + 1] *= c.y * far, x[j + 2] *= c.z * far, x[j + 3] *= c.w * far;
                     }
                 } else {
-                    const int limit = key ? i - 1 : i;
+                    const int row = i & 31, limit = key ? row - 1 : row;
+                    const float *decay = &M.decay[32 * half], *inv = &M.inv[64 + 32 * half];
+                    float p = 1.0f;
 #pragma unroll
-                    for (int e = 15; e >= 0; --e) {
-                        if (j + e < i) p *= M.decay[g][j + e + 1];
-                        x[e] = j + e <= limit ? x[e] * M.inv[64 + j + e] * p : 0.0f;
+                    for (int j = 31; j >= 0; --j) {
+                        if (j < row) p *= decay[j + 1 < 32 ? j + 1 : 31];
+                        x[j] = j <= limit ? x[j] * inv[j] * p : 0.0f;
                     }
                 }
                 if (key) {
+                    const float f = M.inv[gt] * M.beta[i];
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<float4 *>(a_row + j + e) =
-                            float4{x[e] * row_factor, x[e + 1] * row_factor, x[e + 2] * row_factor, x[e + 3] * row_factor};
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(a_row + j) = float4{x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
                 } else {
-                    most = largest(most, x);
-                    tmem_write(mine + kU + j, x);
+                    most = largest(0.0f, x);
                 }
             }
+            M.most[1][half][gt] = most;
+            __syncthreads();
             if (!key) {
-                const int e = exponent_of(most);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-#pragma unroll 1
-                for (int j = 0; j < 64; j += 16) {
-                    unsigned hi[8] = {}, lo[8] = {};
-                    if (j <= last) {
-                        float x[16];
-                        tmem_read(mine + kU + j, x);
-                        split(x, scale_of(e), hi, lo);
-                    }
-                    put_pieces(mine_out + Slot::g, i, j / 8, hi);
-                    put_pieces(mine_out + Slot::g + 8192, i, j / 8, lo);
-                }
-                factors->attn[i] = unscale_of(e) * M.inv[i];
+                const int e = exponent_of(larger(M.most[1][0][gt], M.most[1][1][gt], 0.0f));
+                unsigned hi[16] = {}, lo[16] = {};
+                if (!empty) split(x, scale_of(e), hi, lo);
+                put_pieces(M.tile(0), i, half * 4, hi);
+                put_pieces(M.tile(1), i, half * 4, lo);
+                if (!half) factors->attn[i] = unscale_of(e) * M.inv[i];
+                to_async();
             }
-            group_sync(g);
+        }
+        {
             // T: inverses of the four blocks of 16 on the diagonal, by two warps; then of pairs of them: the lower left of
             // [B 0; A C]^-1 is -C^-1 (A B^-1), whose second factor waits in the upper right
-            float *a = M.a[g];
+            float *a = M.a;
             const auto at = [&](int row, int col) { return a + row * kPitch + col; };
-            if (w4 >= 2) {
-                const int block = 32 * (w4 - 2) + (lane & 16);
+            if (warp == 2 || warp == 3) {
+                const int block = 32 * (warp - 2) + (lane & 16);
                 float c[16];
                 substitute(at(block, block), lane & 15, c);
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) *at(block + j, block + (lane & 15)) = c[j];
             }
-            group_sync(g);
-            {
-                const int two = gt >> 6, row = (gt & 63) >> 2, col = (gt & 3) * 4;  // 64 threads each of two pairs
-                float *b = at(32 * two, 32 * two);
-                times<4>(b + 16 * kPitch, b, row, col, 16, 1.0f, b + 16);
-                group_sync(g);
-                times<4>(b + 16 * kPitch + 16, b + 16, row, col, 16, -1.0f, b + 16 * kPitch);
-                group_sync(g);
-                *reinterpret_cast<float4 *>(b + 16 + row * kPitch + col) = float4{0, 0, 0, 0};
+            __syncthreads();
+            if (tid == 0) {
+                bulk_out(out + Slot::g, M.tile(0), 8192);
+                bulk_out(out + Slot::g + 8192, M.tile(1), 8192);
+                bulk_out_commit();
             }
-            {
-                const int row = gt >> 2, col = (gt & 3) * 8;
-                group_sync(g);
-                times<8>(at(32, 0), at(0, 0), row, col, 32, 1.0f, at(0, 32));
-                group_sync(g);
-                times<8>(at(32, 32), at(0, 32), row, col, 8 * w4 + 8, -1.0f, at(32, 0));
-                group_sync(g);
-            }
+            const int two = gt >> 6, row16 = (gt & 63) >> 2, col16 = (gt & 3) * 4;  // 64 threads each of two pairs
+            float *b = at(32 * two, 32 * two);
+            if (half) times(b + 16 * kPitch, b, row16, col16, 16, 1.0f, b + 16);
+            __syncthreads();
+            if (half) times(b + 16 * kPitch + 16, b + 16, row16, col16, 16, -1.0f, b + 16 * kPitch);
+            __syncthreads();
+            if (half) *reinterpret_cast<float4 *>(b + 16 + row16 * kPitch + col16) = float4{0, 0, 0, 0};
+            __syncthreads();
+            const int row = tid >> 3, col = (tid & 7) * 4;
+            times(at(32, 0), at(0, 0), row, col, 32, 1.0f, at(0, 32));
+            __syncthreads();
+            times(at(32, 32), at(0, 32), row, col, warp * 4 + 4, -1.0f, at(32, 0));
+            if (tid == 0) bulk_out_read();  // G
+            __syncthreads();
         }
-        __syncthreads();  // T's rows take V's place
-        if (there) {
-            // as operands: threads 0-63 for U, 64-127 for W. They wait in W's place.
-            const int i = gt & 63, last = w4 & 1 ? 48 : 16;
-            const bool key = gt >= 64;
-            const float *a_row = &M.a[g][i * kPitch], *by = key ? M.beta_w[g] : M.beta[g];
-            const unsigned waiting = mine + kWAt + 64 * g;
-            float most = 0.0f;
-#pragma unroll 1
-            for (int j = 0; j <= last; j += 16) {
-                float x[16];
+        {
+            // T's rows as operands: threads 0-63 for U, 64-127 for W
+            const int i = gt & 63;
+            const bool key = gt >= 64, empty = !(w4 & 1) && half;
+            const float *a_row = &M.a[i * kPitch + 32 * half], *by = (key ? M.beta_w : M.beta) + 32 * half;
+            float x[32], most = 0.0f;
+            if (!empty) {
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const float4 t = *reinterpret_cast<const float4 *>(a_row + j + e), b = *reinterpret_cast<const float4 *>(by + j + e);
-                    x[e] = t.x * b.x, x[e + 1] = t.y * b.y, x[e + 2] = t.z * b.z, x[e + 3] = t.w * b.w;
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 t = *reinterpret_cast<const float4 *>(a_row + j), b = *reinterpret_cast<const float4 *>(by + j);
+                    x[j] = t.x * b.x, x[j + 1] = t.y * b.y, x[j + 2] = t.z * b.z, x[j + 3] = t.w * b.w;
                 }
-                most = largest(most, x);
-                tmem_write(waiting + j, x);
+                most = largest(0.0f, x);
             }
-            if (past(most)) M.bad[g] = 1;
+            M.most[0][half][gt] = most;
+            __syncthreads();
+            most = larger(M.most[0][0][gt], M.most[0][1][gt], 0.0f);
+            if (past(most)) M.bad = 1;
             const int e = exponent_of(most);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            unsigned char *t_hi = key ? M.tw[0] : M.tu[g][0], *t_lo = key ? M.tw[1] : M.tu[g][1];
-            const int t_row = key ? g * 64 + i : i;
-#pragma unroll 1
-            for (int j = 0; j < 64; j += 16) {
-                unsigned hi[8] = {}, lo[8] = {};
-                if (j <= last) {
-                    float x[16];
-                    tmem_read(waiting + j, x);
-                    split(x, scale_of(e), hi, lo);
-                }
-                put_pieces(t_hi, t_row, j / 8, hi);
-                put_pieces(t_lo, t_row, j / 8, lo);
+            unsigned hi[16] = {}, lo[16] = {};
+            if (!empty) split(x, scale_of(e), hi, lo);
+            put_pieces(M.tile(key ? 0 : 2), i, half * 4, hi);
+            put_pieces(M.tile(key ? 1 : 3), i, half * 4, lo);
+            if (!half) {
+                if (key) factors->z[i] = unscale_of(e) * (1.0f / kWScale);
+                else M.inv_tu[i] = unscale_of(e);
             }
-            (key ? M.inv_tw[g] : M.inv_tu[g])[i] = unscale_of(e);
-        } else if (gt >= 64) {  // rows that no head has
-            const unsigned zero[32] = {};
-            put_pieces(M.tw[0], 64 + (gt & 63), 0, zero);
-            put_pieces(M.tw[1], 64 + (gt & 63), 0, zero);
-            M.inv_tw[g][gt & 63] = 0.0f;
         }
         to_async();
         tc_fence_before();
@@ -422,77 +395,63 @@ __global__ void __launch_bounds__(kPrepareThreads, 1) k_delta_prepare(DeltaNet n
         tc_fence_after();
         if (warp == 0) {
             if (elect_one()) {
-                const unsigned long long tu = sw128_desc(su32(M.tu[0][0])), tw = sw128_desc(su32(M.tw[0]));
-                const unsigned long long keys = turned_desc(su32(M.qk[0][0]) + 8192, 16384);
-#pragma unroll 1
-                for (int product = 0; product < 3; ++product) {
+                // (of 64 channels the wide operand's second 64 rows are the first ones again, and nobody looks)
+                const unsigned long long keys = turned_desc(su32(M.qk[0][0]) + 8192, D == 128 ? 16384 : 0);
+                const unsigned long long tw[2] = {sw128_desc(su32(M.tile(0))), sw128_desc(su32(M.tile(1)))};
+                const unsigned long long tu[2] = {sw128_desc(su32(M.tile(2))), sw128_desc(su32(M.tile(3)))};
 #pragma unroll
-                    for (int w = 0; w < 2; ++w)  // U^T: lanes are value channels (of no head: nobody looks)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_f16_ts(tmem + 320 + 64 * w, tmem + 64 + 64 * w + (product == 0) * 32 + k * 8, tu + w * 1024 + (product == 1) * 512 + k * 2,
-                                       idesc_f16(128, 64), product || k);
+                for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16(tmem + kWAt, tw + (product == 0) * 1024 + k * 2, keys + (product == 1) * (kPanels * 1024) + k * 128, turned_idesc(128, D),
+                        mma_f16_ts(tmem + kU, tmem + kV + (product == 0) * 32 + k * 8, tu[product == 1] + k * 2, idesc_f16(128, 64), product || k);
+#pragma unroll
+                for (int product = 0; product < 3; ++product)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f16(tmem + kW, keys + (product == 0) * (kPanels * 1024) + k * 128, tw[product == 1] + k * 2, idesc_f16(128, 64) | kTurnedWide,
                                 product || k);
-                }
                 mma_commit(&M.done);
             }
             __syncwarp();
         }
         wait(&M.done, phase & 1), ++phase;
         tc_fence_after();
-        if (pair + 2 + g < slab.ratio) fetch_v(h + 2 * n.key_heads);  // T's rows have been read
-        if (there && w4 < D / 32) {
-            float *to = reinterpret_cast<float *>(mine_out + Slot::uu) + gt;
-#pragma unroll 1
-            for (int i = 0; i < 64; i += 16) {
-                float u[16];
-                tmem_read(mine + kU + i, u);
+        if (w4 < D / 32) {
+            float x[32];
+            tmem_read(mine + kU + half * 32, x);
+            float *to = reinterpret_cast<float *>(out + Slot::uu) + half * 32 * D + gt;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) to[(i + e) * D] = u[e] * inv_v * M.inv_tu[g][i + e];
+            for (int i = 0; i < 32; i += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(&M.inv_tu[half * 32 + i]);
+                to[i * D] = x[i] * inv_v * f.x, to[i * D + D] = x[i + 1] * inv_v * f.y;
+                to[i * D + 2 * D] = x[i + 2] * inv_v * f.z, to[i * D + 3 * D] = x[i + 3] * inv_v * f.w;
             }
+            unsigned hi[16], lo[16];
+            tmem_read(mine + kW + half * 32, x);
+            split(x, kWScale, hi, lo);
+            put_pieces(M.w[0], gt, half * 4, hi);
+            put_pieces(M.w[1], gt, half * 4, lo);
         }
-        // W's rows: lane w4 * 32 + lane is row i of the pair's head `of`; this warpgroup has half of its channels
-        const int of = w4 >> 1, i = gt & 63;
-        float most = 0.0f;
-#pragma unroll 1
-        for (int c = 0; c < kW; c += 16) {
-            float w[16];
-            tmem_read(mine + kWAt + g * kW + c, w);
-            most = largest(most, w);
-        }
-        M.w_max[g][gt] = most;
-        __syncthreads();
-        most = larger(M.w_max[0][gt], M.w_max[1][gt], 0.0f);
-        const float inv_t = M.inv_tw[of][i];
-        if (past(most * inv_t)) M.bad[of] = 1;
-        if (pair + of < slab.ratio) {
-            unsigned char *out = slot + Slot::heads + (long long)(pair + of) * Slot::head_bytes;
-            const int e = exponent_of(most);
-            const int panel = D == 128 ? g : 0, first = D == 128 ? 0 : g * 4;
-#pragma unroll 1
-            for (int c = 0; c < kW; c += 16) {
-                float w[16];
-                unsigned hi[8], lo[8];
-                tmem_read(mine + kWAt + g * kW + c, w);
-                split(w, scale_of(e), hi, lo);
-                put_pieces(out + Slot::w + panel * 8192, i, first + c / 8, hi);
-                put_pieces(out + Slot::w + (kPanels + panel) * 8192, i, first + c / 8, lo);
-            }
-            if (g == 0) reinterpret_cast<DeltaFactors *>(out + Slot::factors)->z[i] = unscale_of(e) * inv_t;
-        }
+        to_async();
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        if (there && gt == 0) factors->walk = M.bad[g] | M.bad_key;
+        if (tid == 0) {
+            factors->walk = M.bad | M.bad_key;
+            bulk_out(out + Slot::w, M.w[0], Slot::tile);
+            bulk_out_commit();
+        }
+        if (m + 1 < slab.ratio) {
+            if (tid == 0) bulk_out_read();
+            __syncthreads();
+            fetch_v(h + n.key_heads);
+        }
     }
     if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     settle(&M.abort_flag);
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
 }
 
 template <int D, bool VEC>
