@@ -7,6 +7,9 @@
 //   D = U - Z;  new state's part = (E D)^T K        128 by D keys, sums over tokens; K's tile read the other way round
 //   Y^T = D^T G^T;  y = P R + Y          128 by 64 tokens
 // One warp fetches, one issues; results of a chunk are written while the next one's first product runs.
+//
+// Bound by the way round: a product, its differences, the next product and the new state cannot overlap one another. The four
+// products take 2700 clocks of the tensor cores a chunk of 128 channels, half of them on that way.
 #include "delta_chunk.cuh"
 
 #include <atomic>
@@ -20,16 +23,18 @@ constexpr int kWork = 512, kChainThreads = kWork + 64, kFetchWarp = 16, kIssueWa
 
 template <int D>
 struct __align__(1024) ChainSmem {
-    unsigned char w[2][2][D * 128];            // by stage: hi, lo; rows are key channels
-    unsigned char q[2][2 * D / 64][64 * 128];  // by stage: hi panels, lo panels
+    unsigned char w[2][2][D * 128];         // by stage: hi, lo; rows are key channels
+    unsigned char q[2 * D / 64][64 * 128];  // hi panels, lo panels
     unsigned char k[2 * D / 64][64 * 128];
     unsigned char g[2][64 * 128];  // hi, lo
-    float u[64 * D];
-    DeltaFactors factors[2];
+    struct {
+        float u[64 * D];
+        DeltaFactors f;
+    } row[2];  // by stage, as they follow one another in a slot
     float s_max[4][128];
     float2 d_max[4][128];  // also the sums of chunks that are walked
-    unsigned long long w_full[2], w_empty[2], q_full[2], q_empty[2], f_full[2], f_empty[2], k_full, k_empty, g_full, g_empty, u_full, u_empty;
-    unsigned long long s_ready, r_free, d_ready, y_ready, z_done, r_done, d_done, y_done;
+    unsigned long long w_full[2], w_empty[2], row_full[2], row_empty[2], q_full, q_empty, k_full, k_empty, g_full, g_empty;
+    unsigned long long s_ready, r_free, d_ready, y_ready, z_done, d_done, y_done;
     unsigned tmem;
     int abort_flag;
 };
@@ -37,8 +42,38 @@ struct __align__(1024) ChainSmem {
 __device__ __forceinline__ void lane_sync(int w4) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w4) : "memory"); }  // of the same lanes
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
 
+// A chunk token by token, on the state in memory: a channel's four threads add up their parts of the keys.
 template <int D>
-__global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
+__device__ __noinline__ void walk_chunk(const DeltaNet &n, const DeltaRule &A, ChainSmem<D> &M, float *state, long long row, int tokens, int h, int part, int v) {
+    constexpr int kPart = D / 4;
+    const long long vw = (long long)n.value_heads * n.dim, key = (long long)(h % n.key_heads) * n.dim + part * kPart;
+    const bool in = v < n.dim;
+    const int keys = in ? min(kPart, n.dim - part * kPart) : 0;
+    for (int t = 0; t < tokens; ++t, ++row) {
+        const float *kp = A.k + row * A.k_stride + key, *qp = A.q + row * A.q_stride + key;
+        const float a = A.decay[row * n.value_heads + h], b = A.beta[row * n.value_heads + h];
+        float p = 0.0f, y = 0.0f;
+        for (int i = 0; i < keys; ++i) {
+            state[i * vw] *= a;
+            p = fmaf(state[i * vw], kp[i], p);
+        }
+        M.d_max[part][v].x = p;
+        lane_sync(v >> 5);
+        const float d = b * ((in ? A.v[row * A.v_stride + (long long)h * n.dim + v] : 0.0f) -
+                             ((M.d_max[0][v].x + M.d_max[1][v].x) + (M.d_max[2][v].x + M.d_max[3][v].x)));
+        for (int i = 0; i < keys; ++i) {
+            state[i * vw] = fmaf(kp[i], d, state[i * vw]);
+            y = fmaf(state[i * vw], qp[i], y);
+        }
+        M.d_max[part][v].y = y;
+        lane_sync(v >> 5);
+        if (part == 0 && in) A.y[row * vw + (long long)h * n.dim + v] = (M.d_max[0][v].y + M.d_max[1][v].y) + (M.d_max[2][v].y + M.d_max[3][v].y);
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A,
+                                                                  const __grid_constant__ MixRuns r, const __grid_constant__ DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
     constexpr int kPart = D / 4;  // keys of a thread; and 16 tokens
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -57,18 +92,15 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
     }
     if (begin >= me.tokens) return;
     const int chunks = min(slab.chunks, (me.tokens - begin + kChunk - 1) / kChunk);
-    const unsigned char *slots = slab.slots + ((long long)run_l * slab.heads + head_l) * slab.chunks * slab.slot_bytes;
-    const long long mine = Slot::heads + (long long)m * Slot::head_bytes;
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            bar_init(&M.w_full[i], 1), bar_init(&M.w_empty[i], 1), bar_init(&M.q_full[i], 1), bar_init(&M.q_empty[i], 1);
-            bar_init(&M.f_full[i], 1), bar_init(&M.f_empty[i], kWork / 32 + 1);
+            bar_init(&M.w_full[i], 1), bar_init(&M.w_empty[i], 1);
+            bar_init(&M.row_full[i], 1), bar_init(&M.row_empty[i], kWork / 32 + 1);
         }
-        bar_init(&M.k_full, 1), bar_init(&M.k_empty, 1), bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
-        bar_init(&M.u_full, 1), bar_init(&M.u_empty, kWork / 32);
+        bar_init(&M.q_full, 1), bar_init(&M.q_empty, 1), bar_init(&M.k_full, 1), bar_init(&M.k_empty, 1), bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
         bar_init(&M.s_ready, kWork / 32), bar_init(&M.r_free, kWork / 32), bar_init(&M.d_ready, kWork / 32), bar_init(&M.y_ready, kWork / 32);
-        bar_init(&M.z_done, 1), bar_init(&M.r_done, 1), bar_init(&M.d_done, 1), bar_init(&M.y_done, 1);
+        bar_init(&M.z_done, 1), bar_init(&M.d_done, 1), bar_init(&M.y_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         M.abort_flag = 0;
     }
@@ -80,65 +112,65 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = M.tmem;
-    // columns: the state's halves, under whose place Y's operand goes once R has been formed; E D's; Z, R, Y, the new state's part
-    constexpr unsigned kS = 0, kSLo = D / 2, kD = 128, kZ = 192, kR = 256, kY = 320, kNew = 384;
+    // columns: the state's halves; E D's; Z, and when it has been read D's halves; R, Y, the new state's part
+    constexpr unsigned kS = 0, kSLo = D / 2, kE = 128, kZ = 192, kR = 256, kY = 320, kNew = 384;
     const Waits wait{&M.abort_flag, n.err};
 
     if (warp == kFetchWarp) {
         if (lane == 0) {
+            const unsigned char *slot = slab.slots + ((long long)run_l * slab.heads + head_l) * slab.chunks * slab.slot_bytes;
+            const long long mine = Slot::heads + (long long)m * Slot::head_bytes;
             const auto fetch = [&](void *to, const unsigned char *from, unsigned bytes, unsigned long long *full) {
                 bar_expect(full, bytes);
                 bulk(to, from, bytes, full);
             };
-            for (int c = 0; c < chunks; ++c) {
+            for (int c = 0; c < chunks; ++c, slot += slab.slot_bytes) {
                 const int st = c & 1;
-                const unsigned again = (c >> 1 & 1) ^ 1;
-                const unsigned char *slot = slots + c * slab.slot_bytes;
-                wait(&M.f_empty[st], again);
-                fetch(&M.factors[st], slot + mine + Slot::factors, sizeof(DeltaFactors), &M.f_full[st]);
+                const unsigned again = (c >> 1 & 1) ^ 1, again1 = (c & 1) ^ 1;
                 wait(&M.w_empty[st], again);
                 fetch(M.w[st], slot + mine + Slot::w, Slot::tile, &M.w_full[st]);
-                wait(&M.q_empty[st], again);
-                fetch(M.q[st], slot + Slot::q, Slot::tile, &M.q_full[st]);
-                wait(&M.u_empty, (c & 1) ^ 1);
-                fetch(M.u, slot + mine + Slot::uu, Slot::u, &M.u_full);
-                wait(&M.k_empty, (c & 1) ^ 1);
+                wait(&M.row_empty[st], again);
+                fetch(&M.row[st], slot + mine + Slot::uu, sizeof M.row[st], &M.row_full[st]);
+                wait(&M.q_empty, again1);
+                fetch(M.q, slot + Slot::q, Slot::tile, &M.q_full);
+                wait(&M.k_empty, again1);
                 fetch(M.k, slot + Slot::k, Slot::tile, &M.k_full);
-                wait(&M.g_empty, (c & 1) ^ 1);
+                wait(&M.g_empty, again1);
                 fetch(M.g, slot + mine + Slot::g, Slot::attn, &M.g_full);
             }
         }
         __syncwarp();
     } else if (warp == kIssueWarp) {
         if (elect_one()) {
+            constexpr unsigned kLoTile = D / 64 * 512;  // from a tile's hi panels to its lo ones, in 16-byte units
+            const unsigned long long q = sw128_desc(su32(M.q)), keys = turned_desc(su32(M.k), 8192), g = sw128_desc(su32(M.g));
             unsigned live = 0;  // chunks on the tensor cores so far
             for (int c = 0; c < chunks; ++c) {
                 const int st = c & 1;
-                const unsigned ph = c >> 1 & 1;
-                wait(&M.f_full[st], ph);
-                const bool walk = M.factors[st].walk != 0;
-                bar_arrive(&M.f_empty[st]);
+                const unsigned ph = c >> 1 & 1, ph1 = c & 1;
+                wait(&M.row_full[st], ph);
+                const bool walk = M.row[st].f.walk != 0;
+                bar_arrive(&M.row_empty[st]);
                 if (walk) {  // nothing of it is used
-                    wait(&M.w_full[st], ph), wait(&M.q_full[st], ph), wait(&M.k_full, c & 1), wait(&M.g_full, c & 1);
-                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.q_empty[st]), bar_arrive(&M.k_empty), bar_arrive(&M.g_empty);
+                    wait(&M.w_full[st], ph), wait(&M.q_full, ph1), wait(&M.k_full, ph1), wait(&M.g_full, ph1);
+                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.q_empty), bar_arrive(&M.k_empty), bar_arrive(&M.g_empty);
                     continue;
                 }
                 const unsigned now = live & 1;
                 ++live;
-                constexpr unsigned kLoTile = D / 64 * 512;  // from a tile's hi panels to its lo ones, in 16-byte units
+                const unsigned long long w = turned_desc(su32(M.w[st]), 0);
                 wait(&M.w_full[st], ph);
                 wait(&M.s_ready, now);
                 tc_fence_after();
-                const unsigned long long w = turned_desc(su32(M.w[st]), 0), q = sw128_desc(su32(M.q[st]));
 #pragma unroll
                 for (int product = 0; product < 3; ++product)  // lo hi, hi lo, hi hi
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
                         mma_f16_ts(tmem + kZ, tmem + (product == 0 ? kSLo : kS) + k * 8, w + (product == 1) * kLoTile + k * 128, turned_idesc(128, 64),
                                    product || k);
-                mma_commit(&M.w_empty[st]);
                 mma_commit(&M.z_done);
-                wait(&M.q_full[st], ph);
+                mma_commit(&M.w_empty[st]);
+                wait(&M.q_full, ph1);
                 wait(&M.r_free, now);
                 tc_fence_after();
 #pragma unroll
@@ -147,188 +179,191 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
                     for (int k = 0; k < D / 16; ++k)
                         mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8, q + (product == 1) * kLoTile + k / 4 * 512 + k % 4 * 2,
                                    idesc_f16(128, 64), product || k);
-                mma_commit(&M.q_empty[st]);
-                mma_commit(&M.r_done);
-                wait(&M.k_full, c & 1);
+                mma_commit(&M.q_empty);
+                wait(&M.k_full, ph1);
                 wait(&M.d_ready, now);
                 tc_fence_after();
-                const unsigned long long keys = turned_desc(su32(M.k[0]), 8192), g = sw128_desc(su32(M.g[0]));
 #pragma unroll
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + kNew, tmem + kD + (product == 0) * 32 + k * 8, keys + (product == 1) * kLoTile + k * 128, turned_idesc(128, D),
+                        mma_f16_ts(tmem + kNew, tmem + kE + (product == 0) * 32 + k * 8, keys + (product == 1) * kLoTile + k * 128, turned_idesc(128, D),
                                    product || k);
-                mma_commit(&M.k_empty);
                 mma_commit(&M.d_done);
-                wait(&M.g_full, c & 1);
+                mma_commit(&M.k_empty);
+                wait(&M.g_full, ph1);
                 wait(&M.y_ready, now);
                 tc_fence_after();
 #pragma unroll
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + kY, tmem + kS + (product == 0) * 32 + k * 8, g + (product == 1) * 512 + k * 2, idesc_f16(128, 64), product || k);
-                mma_commit(&M.g_empty);
+                        mma_f16_ts(tmem + kY, tmem + kZ + (product == 0) * 32 + k * 8, g + (product == 1) * 512 + k * 2, idesc_f16(128, 64), product || k);
                 mma_commit(&M.y_done);
+                mma_commit(&M.g_empty);
             }
         }
         __syncwarp();
-    } else if (warp < kFetchWarp) {
+    } else {
         const int w4 = warp & 3, part = warp >> 2, v = w4 * 32 + lane;
         const unsigned lanes = tmem + ((unsigned)(w4 * 32) << 16);
         const bool in = v < n.dim;
+        const int keys = in ? n.dim - part * kPart : 0;  // how many of the thread's there are, or more
         const auto arrive = [&](unsigned long long *b) {
             __syncwarp();
             if (lane == 0) bar_arrive(b);
         };
         float *state = n.state + ((long long)me.sequence * n.dim + part * kPart) * vw + (long long)h * n.dim + v;
-        float S[kPart];
+        unsigned long long S[kPart / 2];
+        const auto load_state = [&] {
 #pragma unroll
-        for (int i = 0; i < kPart; ++i) S[i] = in && part * kPart + i < n.dim ? state[i * vw] : 0.0f;
+            for (int i = 0; i < kPart / 2; ++i)
+                S[i] = pack2(2 * i < keys ? state[2 * i * vw] : 0.0f, 2 * i + 1 < keys ? state[(2 * i + 1) * vw] : 0.0f);
+        };
+        const auto store_state = [&] {
+#pragma unroll
+            for (int i = 0; i < kPart / 2; ++i) {
+                float a, b;
+                unpack2(S[i], a, b);
+                if (2 * i < keys) state[2 * i * vw] = a;
+                if (2 * i + 1 < keys) state[(2 * i + 1) * vw] = b;
+            }
+        };
+        load_state();
         unsigned live = 0;
-        bool owed = false;            // the chunk before has results in TMEM
-        float inv_r = 0, inv_y = 0;   // their scales taken back
+        bool owed = false;           // the chunk before has results in TMEM
+        float inv_r = 0, inv_y = 0;  // their scales taken back
         // results of chunk c: its tokens part * 16 ..
         const auto write_y = [&](int c) {
-            const float4 *fq = reinterpret_cast<const float4 *>(M.factors[c & 1].q + part * 16);
-            const float4 *fa = reinterpret_cast<const float4 *>(M.factors[c & 1].attn + part * 16);
+            const DeltaFactors &f = M.row[c & 1].f;
             const int t0 = begin + c * kChunk + part * 16, left = in ? me.tokens - t0 : 0;
-            float *y = A.y + (first + t0) * vw + (long long)h * n.dim + v;
-            float R[16], Y[16];
-            tmem_read(lanes + kR + part * 16, R);
-            tmem_read(lanes + kY + part * 16, Y);
+            // (uniform row addresses and a lane's offset)
+            const char *row = reinterpret_cast<const char *>(A.y + (first + t0) * vw + (long long)h * n.dim);
+            const long long next = vw * 4;
+            const unsigned at = v * 4;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 q = fq[i], a = fa[i];
-                R[4 * i] = fmaf(R[4 * i] * inv_r, q.x, Y[4 * i] * inv_y * a.x);
-                R[4 * i + 1] = fmaf(R[4 * i + 1] * inv_r, q.y, Y[4 * i + 1] * inv_y * a.y);
-                R[4 * i + 2] = fmaf(R[4 * i + 2] * inv_r, q.z, Y[4 * i + 2] * inv_y * a.z);
-                R[4 * i + 3] = fmaf(R[4 * i + 3] * inv_r, q.w, Y[4 * i + 3] * inv_y * a.w);
+            for (int half = 0; half < 2; ++half) {
+                float R[8], Y[8];
+                tmem_read8(lanes + kR + part * 16 + half * 8, R);
+                tmem_read8(lanes + kY + part * 16 + half * 8, Y);
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    const float4 q = *reinterpret_cast<const float4 *>(f.q + part * 16 + half * 8 + i);
+                    const float4 a = *reinterpret_cast<const float4 *>(f.attn + part * 16 + half * 8 + i);
+                    R[i] = fmaf(R[i] * inv_r, q.x, Y[i] * inv_y * a.x), R[i + 1] = fmaf(R[i + 1] * inv_r, q.y, Y[i + 1] * inv_y * a.y);
+                    R[i + 2] = fmaf(R[i + 2] * inv_r, q.z, Y[i + 2] * inv_y * a.z), R[i + 3] = fmaf(R[i + 3] * inv_r, q.w, Y[i + 3] * inv_y * a.w);
+                }
+                if (left >= 16) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i, row += next) *reinterpret_cast<float *>(const_cast<char *>(row) + at) = R[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i, row += next)
+                        if (half * 8 + i < left) *reinterpret_cast<float *>(const_cast<char *>(row) + at) = R[i];
+                }
             }
-            if (left >= 16) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i, y += vw) *y = R[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i, y += vw)
-                    if (i < left) *y = R[i];
-            }
-            arrive(&M.f_empty[c & 1]);
         };
+#pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
             const int st = c & 1;
-            wait(&M.f_full[st], c >> 1 & 1);
-            const DeltaFactors &f = M.factors[st];
-            if (owed) wait(&M.y_done, (live - 1) & 1), tc_fence_after();
+            wait(&M.row_full[st], c >> 1 & 1);
+            const DeltaFactors &f = M.row[st].f;
             if (f.walk) {
-                if (owed) write_y(c - 1);
-                owed = false;
-                // token by token: a channel's four threads add up their parts of the keys
-                const int t0 = begin + c * kChunk, tokens = min(kChunk, me.tokens - t0);
-                for (int t = 0; t < tokens; ++t) {
-                    const long long row = first + t0 + t;
-                    // (volatile: one after another, not 128 registers of them)
-                    const volatile float *kp = A.k + row * A.k_stride + (long long)(slab.head0 + head_l) * n.dim + part * kPart;
-                    const volatile float *qp = A.q + row * A.q_stride + (long long)(slab.head0 + head_l) * n.dim + part * kPart;
-                    const float a = A.decay[row * n.value_heads + h], b = A.beta[row * n.value_heads + h];
-                    const float value = in ? A.v[row * A.v_stride + (long long)h * n.dim + v] : 0.0f;
-                    float p = 0.0f, y = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kPart; ++i) {
-                        S[i] *= a;
-                        p = fmaf(S[i], part * kPart + i < n.dim ? kp[i] : 0.0f, p);
-                    }
-                    M.d_max[part][v].x = p;
-                    lane_sync(w4);
-                    const float d = b * (value - ((M.d_max[0][v].x + M.d_max[1][v].x) + (M.d_max[2][v].x + M.d_max[3][v].x)));
-#pragma unroll
-                    for (int i = 0; i < kPart; ++i) {
-                        if (part * kPart + i < n.dim) {
-                            S[i] = fmaf(kp[i], d, S[i]);
-                            y = fmaf(S[i], qp[i], y);
-                        }
-                    }
-                    M.d_max[part][v].y = y;
-                    lane_sync(w4);
-                    if (part == 0 && in)
-                        A.y[row * vw + (long long)h * n.dim + v] = (M.d_max[0][v].y + M.d_max[1][v].y) + (M.d_max[2][v].y + M.d_max[3][v].y);
+                if (owed) {
+                    wait(&M.y_done, (live - 1) & 1);
+                    tc_fence_after();
+                    write_y(c - 1);
+                    arrive(&M.row_empty[st ^ 1]);
+                    owed = false;
                 }
-                arrive(&M.f_empty[st]);
-                wait(&M.u_full, c & 1);
-                arrive(&M.u_empty);
+                const int t0 = begin + c * kChunk;
+                store_state();
+                walk_chunk(n, A, M, state, first + t0, min(kChunk, me.tokens - t0), h, part, v);
+                load_state();
+                arrive(&M.row_empty[st]);
                 continue;
             }
             const unsigned now = live & 1;
             ++live;
             // the state as an operand
-            M.s_max[part][v] = largest(0.0f, S);
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPart / 2; ++i) most = larger2(most, S[i]);
+            M.s_max[part][v] = most;
             lane_sync(w4);
             const int es = exponent_of(larger(larger(M.s_max[0][v], M.s_max[1][v], M.s_max[2][v]), M.s_max[3][v], 0.0f));
             const float inv_s = unscale_of(es);
 #pragma unroll
-            for (int i = 0; i < kPart; i += 16) {
-                float x[16];
+            for (int i = 0; i < kPart / 2; i += 8) {
                 unsigned hi[8], lo[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = S[i + e];
-                split(x, scale_of(es), hi, lo);
-                tmem_write(lanes + kS + (part * kPart + i) / 2, hi);
-                tmem_write(lanes + kSLo + (part * kPart + i) / 2, lo);
+                for (int e = 0; e < 8; ++e) split2(S[i + e], both(scale_of(es)), hi[e], lo[e]);
+                tmem_write(lanes + kS + part * (kPart / 2) + i, hi);
+                tmem_write(lanes + kSLo + part * (kPart / 2) + i, lo);
             }
             tmem_written();
             arrive(&M.s_ready);
             if (owed) {
+                wait(&M.y_done, now ^ 1);
+                tc_fence_after();
                 write_y(c - 1);
                 tc_fence_before();
+                arrive(&M.row_empty[st ^ 1]);
             }
             arrive(&M.r_free);
             inv_r = inv_s;
             // differences, and as the decays to the chunk's end leave them
-            wait(&M.u_full, c & 1);
+            const float *u = M.row[st].u + part * 16 * D + (v < D ? v : 0);
+            const float by = v < D ? -inv_s : 0.0f;
+            float d[16];
             wait(&M.z_done, now);
             tc_fence_after();
-            float d[16], e[16];
-            const float *u = M.u + part * 16 * D + (v < D ? v : 0);
-            const float4 *fz = reinterpret_cast<const float4 *>(f.z + part * 16), *fk = reinterpret_cast<const float4 *>(f.k + part * 16);
-            const float by = v < D ? -inv_s : 0.0f, keep = v < D ? 1.0f : 0.0f;
             tmem_read(lanes + kZ + part * 16, d);
+            unsigned long long x[8];
+            float most_d = 0.0f, most_e = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-                const float4 z = fz[i / 4], k = fk[i / 4];
-                d[i] = fmaf(d[i] * by, z.x, u[i * D] * keep), d[i + 1] = fmaf(d[i + 1] * by, z.y, u[i * D + D] * keep);
-                d[i + 2] = fmaf(d[i + 2] * by, z.z, u[i * D + 2 * D] * keep), d[i + 3] = fmaf(d[i + 3] * by, z.w, u[i * D + 3 * D] * keep);
-                e[i] = d[i] * k.x, e[i + 1] = d[i + 1] * k.y, e[i + 2] = d[i + 2] * k.z, e[i + 3] = d[i + 3] * k.w;
+                const ulonglong2 z = *reinterpret_cast<const ulonglong2 *>(f.z + part * 16 + i), k = *reinterpret_cast<const ulonglong2 *>(f.k + part * 16 + i);
+                x[i / 2] = fma2(mul2_rn(pack2(d[i], d[i + 1]), both(by)), z.x, pack2(u[i * D], u[i * D + D]));
+                x[i / 2 + 1] = fma2(mul2_rn(pack2(d[i + 2], d[i + 3]), both(by)), z.y, pack2(u[i * D + 2 * D], u[i * D + 3 * D]));
+                most_d = larger2(larger2(most_d, x[i / 2]), x[i / 2 + 1]);
+                most_e = larger2(larger2(most_e, mul2_rn(x[i / 2], k.x)), mul2_rn(x[i / 2 + 1], k.y));
             }
-            arrive(&M.u_empty);
-            M.d_max[part][v] = float2{largest(0.0f, d), largest(0.0f, e)};
-            lane_sync(w4);
+            M.d_max[part][v] = float2{most_d, most_e};
+            tc_fence_before();
+            lane_sync(w4);  // Z's lanes have been read, too
+            tc_fence_after();
             const float2 m0 = M.d_max[0][v], m1 = M.d_max[1][v], m2 = M.d_max[2][v], m3 = M.d_max[3][v];
-            const int ed = exponent_of(larger(larger(m0.x, m1.x, m2.x), m3.x, 0.0f)), ee = exponent_of(larger(larger(m0.y, m1.y, m2.y), m3.y, 0.0f));
+            const int ee = exponent_of(larger(larger(m0.y, m1.y, m2.y), m3.y, 0.0f)), ed = exponent_of(larger(larger(m0.x, m1.x, m2.x), m3.x, 0.0f));
             unsigned hi[8], lo[8];
-            split(e, scale_of(ee), hi, lo);
-            tmem_write(lanes + kD + part * 8, hi);
-            tmem_write(lanes + kD + 32 + part * 8, lo);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(f.k + part * 16 + 2 * i);
+                split2(mul2_rn(x[i], k.x), both(scale_of(ee)), hi[i], lo[i]);
+                split2(mul2_rn(x[i + 1], k.y), both(scale_of(ee)), hi[i + 1], lo[i + 1]);
+            }
+            tmem_write(lanes + kE + part * 8, hi);
+            tmem_write(lanes + kE + 32 + part * 8, lo);
             tmem_written();
             arrive(&M.d_ready);
-            split(d, scale_of(ed), hi, lo);
-            wait(&M.r_done, now);  // the state's halves have been read
-            tc_fence_after();
-            tmem_write(lanes + kS + part * 8, hi);
-            tmem_write(lanes + kS + 32 + part * 8, lo);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) split2(x[i], both(scale_of(ed)), hi[i], lo[i]);
+            tmem_write(lanes + kZ + part * 8, hi);
+            tmem_write(lanes + kZ + 32 + part * 8, lo);
             tmem_written();
             arrive(&M.y_ready);
             inv_y = unscale_of(ed);
             // the new state
-            wait(&M.d_done, now);
-            tc_fence_after();
             const float inv_e = unscale_of(ee), end = f.end;
 #pragma unroll
-            for (int i = 0; i < kPart; i += 16) {
-                float x[16];
-                tmem_read(lanes + kNew + part * kPart + i, x);
+            for (int i = 0; i < kPart / 2; ++i) S[i] = mul2_rn(S[i], both(end));
+            wait(&M.d_done, now);
+            tc_fence_after();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) S[i + e] = fmaf(x[e], inv_e, S[i + e] * end);
+            for (int i = 0; i < kPart; i += 16) {
+                tmem_read(lanes + kNew + part * kPart + i, d);
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) S[(i + e) / 2] = fma2(pack2(d[e], d[e + 1]), both(inv_e), S[(i + e) / 2]);
             }
             tc_fence_before();
             owed = true;
@@ -339,11 +374,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(DeltaNet n, De
             write_y(chunks - 1);
         }
         work_sync();
-        if (!*(volatile int *)&M.abort_flag) {
-#pragma unroll
-            for (int i = 0; i < kPart; ++i)
-                if (in && part * kPart + i < n.dim) state[i * vw] = S[i];
-        }
+        if (!*(volatile int *)&M.abort_flag) store_state();
     }
     tc_fence_before();
     __syncthreads();

@@ -66,6 +66,14 @@ __device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[16]) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_read8(unsigned taddr, float (&v)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
 __device__ __forceinline__ void tmem_write(unsigned taddr, const unsigned (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
@@ -107,24 +115,34 @@ __device__ __forceinline__ float warp_largest(float x) {
     return r;
 }
 __device__ __forceinline__ bool past(float largest) { return !(largest <= kDeltaLarge); }
-// x times a power of two as pairs of FP16 halves, hi and lo
+// Pairs of F32 as one 64-bit register pair.
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long both(float x) { return pack2(x, x); }
+// A pair times powers of two as FP16 halves, hi and lo.
+__device__ __forceinline__ void split2(unsigned long long x, unsigned long long by, unsigned &hi, unsigned &lo) {
+    const unsigned long long s = mul2_rn(x, by);
+    float a, b;
+    unpack2(s, a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    unpack2(fma2(pack2(f.x, f.y), both(-1.0f), s), a, b);
+    const __half2 l = __floats2half2_rn(a, b);
+    hi = *reinterpret_cast<const unsigned *>(&h);
+    lo = *reinterpret_cast<const unsigned *>(&l);
+}
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[N], float scale, unsigned (&hi)[N / 2], unsigned (&lo)[N / 2]) {
-    const unsigned long long by = pack2(scale, scale), less = pack2(-1.0f, -1.0f);
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-        const unsigned long long s = mul2_rn(pack2(x[2 * i], x[2 * i + 1]), by);
-        float a, b;
-        unpack2(s, a, b);
-        const __half2 h = __floats2half2_rn(a, b);
-        const float2 f = __half22float2(h);
-        unsigned long long d;
-        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pack2(f.x, f.y)), "l"(less), "l"(s));
-        unpack2(d, a, b);
-        const __half2 l = __floats2half2_rn(a, b);
-        hi[i] = *reinterpret_cast<const unsigned *>(&h);
-        lo[i] = *reinterpret_cast<const unsigned *>(&l);
-    }
+    for (int i = 0; i < N / 2; ++i) split2(pack2(x[2 * i], x[2 * i + 1]), both(scale), hi[i], lo[i]);
+}
+__device__ __forceinline__ float larger2(float m, unsigned long long x) {
+    float a, b;
+    unpack2(x, a, b);
+    return larger(m, a, b);
 }
 // Byte of 16-byte piece c of row r: rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ int piece(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
