@@ -24,8 +24,7 @@ constexpr int kWork = 512, kChainThreads = kWork + 64, kFetchWarp = 16, kIssueWa
 template <int D>
 struct __align__(1024) ChainSmem {
     unsigned char w[2][2][D * 128];         // by stage: hi, lo; rows are key channels
-    unsigned char q[2 * D / 64][64 * 128];  // hi panels, lo panels
-    unsigned char k[2 * D / 64][64 * 128];
+    unsigned char qk[2][D / 64][128 * 128];  // hi, lo: panels of 64 channels; rows 0-63 Q, 64-127 K
     unsigned char g[2][64 * 128];  // hi, lo
     struct {
         float u[64 * D];
@@ -33,7 +32,7 @@ struct __align__(1024) ChainSmem {
     } row[2];  // by stage, as they follow one another in a slot
     float s_max[4][128];
     float2 d_max[4][128];  // also the sums of chunks that are walked
-    unsigned long long w_full[2], w_empty[2], row_full[2], row_empty[2], q_full, q_empty, k_full, k_empty, g_full, g_empty;
+    unsigned long long w_full[2], w_empty[2], row_full[2], row_empty[2], qk_full, qk_empty, g_full, g_empty;
     unsigned long long s_ready, r_free, d_ready, y_ready, z_done, d_done, y_done;
     unsigned tmem;
     int abort_flag;
@@ -98,7 +97,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             bar_init(&M.w_full[i], 1), bar_init(&M.w_empty[i], 1);
             bar_init(&M.row_full[i], 1), bar_init(&M.row_empty[i], kWork / 32 + 1);
         }
-        bar_init(&M.q_full, 1), bar_init(&M.q_empty, 1), bar_init(&M.k_full, 1), bar_init(&M.k_empty, 1), bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
+        bar_init(&M.qk_full, 1), bar_init(&M.qk_empty, 1), bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
         bar_init(&M.s_ready, kWork / 32), bar_init(&M.r_free, kWork / 32), bar_init(&M.d_ready, kWork / 32), bar_init(&M.y_ready, kWork / 32);
         bar_init(&M.z_done, 1), bar_init(&M.d_done, 1), bar_init(&M.y_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -131,10 +130,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 fetch(M.w[st], slot + mine + Slot::w, Slot::tile, &M.w_full[st]);
                 wait(&M.row_empty[st], again);
                 fetch(&M.row[st], slot + mine + Slot::uu, sizeof M.row[st], &M.row_full[st]);
-                wait(&M.q_empty, again1);
-                fetch(M.q, slot + Slot::q, Slot::tile, &M.q_full);
-                wait(&M.k_empty, again1);
-                fetch(M.k, slot + Slot::k, Slot::tile, &M.k_full);
+                wait(&M.qk_empty, again1);
+                fetch(M.qk, slot, 2 * Slot::tile, &M.qk_full);
                 wait(&M.g_empty, again1);
                 fetch(M.g, slot + mine + Slot::g, Slot::attn, &M.g_full);
             }
@@ -142,8 +139,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
         __syncwarp();
     } else if (warp == kIssueWarp) {
         if (elect_one()) {
-            constexpr unsigned kLoTile = D / 64 * 512;  // from a tile's hi panels to its lo ones, in 16-byte units
-            const unsigned long long q = sw128_desc(su32(M.q)), keys = turned_desc(su32(M.k), 8192), g = sw128_desc(su32(M.g));
+            constexpr unsigned kLoW = D * 8, kLoQk = D / 64 * 1024;  // from hi to lo, in 16-byte units
+            const unsigned long long q = sw128_desc(su32(M.qk)), keys = turned_desc(su32(M.qk) + 8192, 16384), g = sw128_desc(su32(M.g));
             unsigned live = 0;  // chunks on the tensor cores so far
             for (int c = 0; c < chunks; ++c) {
                 const int st = c & 1;
@@ -152,8 +149,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 const bool walk = M.row[st].f.walk != 0;
                 bar_arrive(&M.row_empty[st]);
                 if (walk) {  // nothing of it is used
-                    wait(&M.w_full[st], ph), wait(&M.q_full, ph1), wait(&M.k_full, ph1), wait(&M.g_full, ph1);
-                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.q_empty), bar_arrive(&M.k_empty), bar_arrive(&M.g_empty);
+                    wait(&M.w_full[st], ph), wait(&M.qk_full, ph1), wait(&M.g_full, ph1);
+                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.qk_empty), bar_arrive(&M.g_empty);
                     continue;
                 }
                 const unsigned now = live & 1;
@@ -166,31 +163,29 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 for (int product = 0; product < 3; ++product)  // lo hi, hi lo, hi hi
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        mma_f16_ts(tmem + kZ, tmem + (product == 0 ? kSLo : kS) + k * 8, w + (product == 1) * kLoTile + k * 128, turned_idesc(128, 64),
+                        mma_f16_ts(tmem + kZ, tmem + (product == 0 ? kSLo : kS) + k * 8, w + (product == 1) * kLoW + k * 128, turned_idesc(128, 64),
                                    product || k);
                 mma_commit(&M.z_done);
                 mma_commit(&M.w_empty[st]);
-                wait(&M.q_full, ph1);
+                wait(&M.qk_full, ph1);
                 wait(&M.r_free, now);
                 tc_fence_after();
 #pragma unroll
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8, q + (product == 1) * kLoTile + k / 4 * 512 + k % 4 * 2,
+                        mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8, q + (product == 1) * kLoQk + k / 4 * 1024 + k % 4 * 2,
                                    idesc_f16(128, 64), product || k);
-                mma_commit(&M.q_empty);
-                wait(&M.k_full, ph1);
                 wait(&M.d_ready, now);
                 tc_fence_after();
 #pragma unroll
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + kNew, tmem + kE + (product == 0) * 32 + k * 8, keys + (product == 1) * kLoTile + k * 128, turned_idesc(128, D),
+                        mma_f16_ts(tmem + kNew, tmem + kE + (product == 0) * 32 + k * 8, keys + (product == 1) * kLoQk + k * 128, turned_idesc(128, D),
                                    product || k);
                 mma_commit(&M.d_done);
-                mma_commit(&M.k_empty);
+                mma_commit(&M.qk_empty);
                 wait(&M.g_full, ph1);
                 wait(&M.y_ready, now);
                 tc_fence_after();
@@ -266,11 +261,11 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
             const int st = c & 1;
-            wait(&M.row_full[st], c >> 1 & 1);
+            wait.warp(&M.row_full[st], c >> 1 & 1, lane);
             const DeltaFactors &f = M.row[st].f;
             if (f.walk) {
                 if (owed) {
-                    wait(&M.y_done, (live - 1) & 1);
+                    wait.warp(&M.y_done, (live - 1) & 1, lane);
                     tc_fence_after();
                     write_y(c - 1);
                     arrive(&M.row_empty[st ^ 1]);
@@ -304,7 +299,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             tmem_written();
             arrive(&M.s_ready);
             if (owed) {
-                wait(&M.y_done, now ^ 1);
+                wait.warp(&M.y_done, now ^ 1, lane);
                 tc_fence_after();
                 write_y(c - 1);
                 tc_fence_before();
@@ -316,7 +311,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             const float *u = M.row[st].u + part * 16 * D + (v < D ? v : 0);
             const float by = v < D ? -inv_s : 0.0f;
             float d[16];
-            wait(&M.z_done, now);
+            wait.warp(&M.z_done, now, lane);
             tc_fence_after();
             tmem_read(lanes + kZ + part * 16, d);
             unsigned long long x[8];
@@ -357,7 +352,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             const float inv_e = unscale_of(ee), end = f.end;
 #pragma unroll
             for (int i = 0; i < kPart / 2; ++i) S[i] = mul2_rn(S[i], both(end));
-            wait(&M.d_done, now);
+            wait.warp(&M.d_done, now, lane);
             tc_fence_after();
 #pragma unroll
             for (int i = 0; i < kPart; i += 16) {
@@ -369,7 +364,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             owed = true;
         }
         if (owed) {
-            wait(&M.y_done, (live - 1) & 1);
+            wait.warp(&M.y_done, (live - 1) & 1, lane);
             tc_fence_after();
             write_y(chunks - 1);
         }

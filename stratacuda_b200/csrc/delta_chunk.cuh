@@ -13,7 +13,7 @@
 // off in the 2-norm, so it is 2.8e-7).
 //
 // Workspace: a slot for each run, key head and chunk of a slab, in the layout that the second kernel's tensor-core operands
-// have in shared memory (rows of 128 bytes, 128-byte swizzle): Q and K [64 tokens][D], hi and lo; then for each of the key
+// have in shared memory (rows of 128 bytes, 128-byte swizzle): Q above K [2 x 64 tokens][D], hi and lo; then for each of the key
 // head's value heads W^T [D][64], hi and lo, the products G (q . k) [64][64], hi and lo, U [64][D] in F32 and the rows' factors.
 #pragma once
 #include "mixers.cuh"
@@ -42,7 +42,7 @@ struct DeltaSlab {  // runs, key heads and chunks [first, first + n) of a call
 template <int D>
 struct DeltaSlot {
     static constexpr int tile = 64 * D * 2 * 2, attn = 64 * 64 * 2 * 2, u = 64 * D * 4;  // bytes; hi and lo
-    static constexpr int q = 0, k = tile, heads = 2 * tile;
+    static constexpr int heads = 2 * tile;  // behind Q and K
     static constexpr int w = 0, g = tile, uu = tile + attn, factors = uu + u, head_bytes = factors + (int)sizeof(DeltaFactors);
     __host__ __device__ static long long bytes(int ratio) { return heads + (long long)ratio * head_bytes; }
 };
@@ -122,15 +122,14 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
     return d;
 }
 __device__ __forceinline__ unsigned long long both(float x) { return pack2(x, x); }
-// A pair times powers of two as FP16 halves, hi and lo.
+// A pair times powers of two as FP16 halves, hi and lo. (The subtraction is not paired: paired operations and conversions
+// from FP16 share one pipe, which bounds a split.)
 __device__ __forceinline__ void split2(unsigned long long x, unsigned long long by, unsigned &hi, unsigned &lo) {
-    const unsigned long long s = mul2_rn(x, by);
     float a, b;
-    unpack2(s, a, b);
+    unpack2(mul2_rn(x, by), a, b);
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    unpack2(fma2(pack2(f.x, f.y), both(-1.0f), s), a, b);
-    const __half2 l = __floats2half2_rn(a, b);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
     hi = *reinterpret_cast<const unsigned *>(&h);
     lo = *reinterpret_cast<const unsigned *>(&l);
 }
@@ -176,7 +175,13 @@ struct Waits {
             }
         }
     }
+    // The same of a whole warp: one lane looks (32 that look at one barrier take 15 clocks each way, 16 warps of them 250).
+    __device__ __forceinline__ void warp(unsigned long long *b, unsigned parity, int lane) const {
+        if (lane == 0) (*this)(b, parity);
+        __syncwarp();
+    }
 };
+
 // After a wait has run out: time for copies and products in flight, before shared memory and TMEM go.
 __device__ __forceinline__ void settle(const int *abort_flag) {
     if (!*(volatile const int *)abort_flag) return;

@@ -3,14 +3,15 @@
 // A block has a run's chunk and key head, and takes the head's value heads one after another:
 //   [Q; K] K^T      128 rows by 64, once for all of them
 //   A, G (q . k)    a row's two threads have half of its columns each, from their TMEM lane
-//   T = (I + A)^-1  of blocks of 16 by substitution, a column a lane, then of blocks twice as large twice, F32 throughout
+//   T = (I + A)^-1  of blocks of 32 by substitution, a column a lane, then -T22 (A21 T11), F32 throughout
 //   U^T = V^T (T diag(beta))^T      a lane a value channel
 //   W^T = K^T (T diag(beta P))^T    a lane a key channel; K's tile as it lies, read the other way round
-// Bound by instructions, most of them the splits into halves, and by the way from one step to the next: two blocks a
-// multiprocessor, 100 KB and half of TMEM each, so that one's steps run in the other's waits. What becomes operands goes
-// through shared memory and bulk copies. Code that a block runs once comes slower than it executes, so it is kept short: with a
-// thread for a whole row, all 64 columns unrolled, a prompt of 2048 tokens over 32 heads of 128 took 210 us, most of them
-// without an instruction to issue.
+// Bound by instructions, most of them the splits into halves, and by the way from one step to the next: two blocks of eight
+// warps a multiprocessor, 100 KB and half of TMEM each, so that one's steps run in the other's waits (blocks of sixteen warps
+// were slower: 87 us where this took 68). What becomes operands goes
+// through shared memory and bulk copies, few and large ones. Code that a block runs once comes slower than it executes, so it is
+// kept short. A prompt of 2048 tokens over 32 heads of 128 took 210 us with a thread for a whole row, all 64 columns unrolled,
+// most of them without an instruction to issue.
 #include "delta_chunk.cuh"
 
 #include <atomic>
@@ -27,18 +28,17 @@ template <int D>
 struct __align__(1024) PrepareSmem {
     unsigned char qk[2][D / 64][128 * 128];  // hi, lo: panels of 64 channels; rows 0-63 Q, 64-127 K
     unsigned char more[D == 64 ? 4 : 1][D == 64 ? 64 * 128 : 16];
-    union {  // a value head's V, until it is in TMEM; A, then T; W^T, hi and lo
-        float v[64 * D];
-        float a[64 * kPitch];
+    union {
+        float a[64 * kPitch];  // A, then T
         unsigned char w[2][D * 128];
     };
     float inv[128];  // Q's and K's scales taken back
-    // decays; products of decays up to a token in its half; strengths, and times decays up to the token over K's scale; K's
+    // decays; their products up to a token in its half; strengths, and times decays up to the token over K's scale; K's
     // scales taken back, the lower half's times the decays after a token in it
     float decay[64], upto[64], beta[64], beta_w[64], inv_k[64];
     float inv_tu[64];
     float most[2][2][128];  // a row's largest values, by warpgroup; two that are used in turn
-    int bad_key, bad, abort_flag;
+    int bad_key, bad[2], abort_flag;  // by turn
     unsigned tmem;
     unsigned long long done;
 
@@ -47,20 +47,16 @@ struct __align__(1024) PrepareSmem {
     __device__ __forceinline__ unsigned char *tile(int i) { return D == 128 ? qk[i >> 1][i & 1] : more[i]; }
 };
 
-__device__ __forceinline__ void add2(unsigned long long &d, unsigned long long a, unsigned long long b) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
-}
-__device__ __forceinline__ ulonglong2 load22(const float *p) { return *reinterpret_cast<const ulonglong2 *>(p); }
 __device__ __forceinline__ void bulk_out(void *to, const void *from, unsigned bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(su32(from)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void bulk_out_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_out_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
-// x of (I + L) x = e_c, L the strictly lower part of 16 rows at l
-__device__ __forceinline__ void substitute(const float *l, int c, float (&x)[16]) {
+// x of (I + L) x = e_c, L the strictly lower part of 32 rows at l
+__device__ __forceinline__ void substitute(const float *l, int c, float (&x)[32]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 32; ++i) {
         float s[4] = {i == c ? 1.0f : 0.0f, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < i; j += 4) {
@@ -73,21 +69,20 @@ __device__ __forceinline__ void substitute(const float *l, int c, float (&x)[16]
         x[i] = (s[0] + s[1]) + (s[2] + s[3]);
     }
 }
-// Four columns from c of row r of sign X Y: rows of X at x, Y at y; `terms` (a multiple of 4) of X's row count
-__device__ __forceinline__ void times(const float *x, const float *y, int r, int c, int terms, float sign, float *to) {
-    unsigned long long s0 = 0, s1 = 0;
+// Rows r, r + 1 and four columns from c of X Y, 32 by 32, rows of X at x, Y at y; `terms` (a multiple of 4) of X's rows count.
+__device__ __forceinline__ void times(const float *x, const float *y, int r, int c, int terms, float4 (&out)[2]) {
+    out[0] = out[1] = float4{0, 0, 0, 0};
 #pragma unroll 2
     for (int j = 0; j < terms; j += 4) {
-        const float4 f = *reinterpret_cast<const float4 *>(x + r * kPitch + j);
-        const float g[4] = {f.x * sign, f.y * sign, f.z * sign, f.w * sign};
+        const float4 f0 = *reinterpret_cast<const float4 *>(x + r * kPitch + j), f1 = *reinterpret_cast<const float4 *>(x + (r + 1) * kPitch + j);
+        const float a[4] = {f0.x, f0.y, f0.z, f0.w}, b[4] = {f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const ulonglong2 b = load22(y + (j + e) * kPitch + c);
-            add2(s0, pack2(g[e], g[e]), b.x);
-            add2(s1, pack2(g[e], g[e]), b.y);
+            const float4 g = *reinterpret_cast<const float4 *>(y + (j + e) * kPitch + c);
+            out[0].x = fmaf(a[e], g.x, out[0].x), out[0].y = fmaf(a[e], g.y, out[0].y), out[0].z = fmaf(a[e], g.z, out[0].z), out[0].w = fmaf(a[e], g.w, out[0].w);
+            out[1].x = fmaf(b[e], g.x, out[1].x), out[1].y = fmaf(b[e], g.y, out[1].y), out[1].z = fmaf(b[e], g.z, out[1].z), out[1].w = fmaf(b[e], g.w, out[1].w);
         }
     }
-    *reinterpret_cast<ulonglong2 *>(to + r * kPitch + c) = ulonglong2{s0, s1};
 }
 // Products over lanes: of this one's and those before, and of those after.
 __device__ __forceinline__ float product_upto(float x, int lane) {
@@ -109,11 +104,12 @@ __device__ __forceinline__ float product_after(float x, int lane) {
     return x;
 }
 
-// VEC: rows of q, k and v can be read four channels at a time.
+// VEC: rows of q and k can be read four channels at a time.
 template <int D, bool VEC>
-__global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n, DeltaRule A, MixRuns r, DeltaSlab slab) {
+__global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A,
+                                                                      const __grid_constant__ MixRuns r, const __grid_constant__ DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
-    constexpr int kPanels = D / 64;
+    constexpr int kPanels = D / 64, kBulk = 32;  // the thread that copies out
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     PrepareSmem<D> &M = *reinterpret_cast<PrepareSmem<D> *>(smem_raw);
     // half of the columns, row
@@ -127,21 +123,24 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
     const long long row0 = (long long)run * r.count + t0;
     unsigned char *slot = slab.slots + blockIdx.x * slab.slot_bytes;
 
-    // V's rows of a value head to shared memory; zeros behind the run's end and past dim
-    const auto fetch_v = [&](int h) {
-        const float *from = A.v + row0 * A.v_stride + (long long)h * n.dim;
-        constexpr int kPiece = VEC ? 4 : 1;
-#pragma unroll 4
-        for (int at = tid * kPiece; at < 64 * D; at += kPrepareThreads * kPiece) {
-            const int j = at / D, c = at % D;
-            const bool in = j < tokens && c < n.dim;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(su32(&M.v[at])), "l"(in ? from + j * A.v_stride + c : A.v), "n"(kPiece * 4),
-                         "r"(in ? kPiece * 4 : 0)
-                         : "memory");
+    // Q's and K's rows: sixteen a warp
+    constexpr int kLanes = D / 4, kRows = 32 / kLanes, kPasses = 16 / kRows;
+    const int ch = 4 * (lane % kLanes);
+    float f[kPasses][4];
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+        const int row = warp * 16 + u * kRows + lane / kLanes, t = row & 63;
+        f[u][0] = f[u][1] = f[u][2] = f[u][3] = 0.0f;
+        if (t >= tokens || ch >= n.dim) continue;
+        const float *p = (row < 64 ? A.q + (row0 + t) * A.q_stride : A.k + (row0 + t) * A.k_stride) + (long long)head * n.dim + ch;
+        if (VEC) {
+            const float4 x = *reinterpret_cast<const float4 *>(p);
+            f[u][0] = x.x, f[u][1] = x.y, f[u][2] = x.z, f[u][3] = x.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[u][e] = ch + e < n.dim ? p[e] : 0.0f;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    fetch_v(head);
+    }
     if (tid == 0) {
         bar_init(&M.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -158,53 +157,40 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
     constexpr unsigned kRaw = 0, kV = 64, kU = 128, kW = 192;  // columns: [Q; K] K^T; V's halves; U^T; W^T
     const Waits wait{&M.abort_flag, n.err};
     unsigned phase = 0;
-
-    // Q's and K's rows, a power of two each: 16 a warp
-    constexpr int kLanes = D / 4, kRows = 32 / kLanes;
-#pragma unroll 1
-    for (int at = 0; at < 16; at += 8 * kRows) {
-        float f[8][4];
-        const int ch = 4 * (lane % kLanes);
+    // a power of two a row
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int row = warp * 16 + at + u * kRows + lane / kLanes, t = row & 63;
-            f[u][0] = f[u][1] = f[u][2] = f[u][3] = 0.0f;
-            if (t >= tokens || ch >= n.dim) continue;
-            const float *p = (row < 64 ? A.q + (row0 + t) * A.q_stride : A.k + (row0 + t) * A.k_stride) + (long long)head * n.dim + ch;
-            if (VEC) {
-                const float4 x = *reinterpret_cast<const float4 *>(p);
-                f[u][0] = x.x, f[u][1] = x.y, f[u][2] = x.z, f[u][3] = x.w;
-            } else {
+    for (int u = 0; u < kPasses; ++u) {
+        const int row = warp * 16 + u * kRows + lane / kLanes;
+        float m = largest(0.0f, f[u]);
+        if (kLanes == 32) {
+            m = warp_largest(m);
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[u][e] = ch + e < n.dim ? p[e] : 0.0f;
-            }
+            for (int s = kLanes / 2; s > 0; s >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, s), 0.0f);
         }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int row = warp * 16 + at + u * kRows + lane / kLanes;
-            float m = largest(0.0f, f[u]);
-            if (kLanes == 32) {
-                m = warp_largest(m);
-            } else {
-#pragma unroll
-                for (int s = kLanes / 2; s > 0; s >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, s), 0.0f);
-            }
-            const int e = exponent_of(m);
-            if (lane % kLanes == 0) M.inv[row] = unscale_of(e);
-            if (past(m)) M.bad_key = 1;
-            unsigned hi[2], lo[2];
-            split(f[u], scale_of(e), hi, lo);
-            const int to = piece(row, ch % 64 / 8) + ch % 8 * 2;
-            *reinterpret_cast<uint2 *>(&M.qk[0][ch / 64][to]) = uint2{hi[0], hi[1]};
-            *reinterpret_cast<uint2 *>(&M.qk[1][ch / 64][to]) = uint2{lo[0], lo[1]};
-        }
+        const int e = exponent_of(m);
+        if (lane % kLanes == 0) M.inv[row] = unscale_of(e);
+        if (past(m)) M.bad_key = 1;
+        unsigned hi[2], lo[2];
+        split(f[u], scale_of(e), hi, lo);
+        const int to = piece(row, ch % 64 / 8) + ch % 8 * 2;
+        *reinterpret_cast<uint2 *>(&M.qk[0][ch / 64][to]) = uint2{hi[0], hi[1]};
+        *reinterpret_cast<uint2 *>(&M.qk[1][ch / 64][to]) = uint2{lo[0], lo[1]};
     }
+    // V's column of this lane, 32 tokens
+    float v[32];
+    const auto load_v = [&](int h) {
+        const float *p = A.v + (row0 + half * 32) * A.v_stride + (long long)h * n.dim + gt;
+#pragma unroll
+        for (int j = 0; j < 32; ++j, p += A.v_stride) v[j] = gt < n.dim && half * 32 + j < tokens ? *p : 0.0f;
+    };
+    load_v(head);
     to_async();
     __syncthreads();
     if (warp == 0) {
         if (elect_one()) {
             const unsigned long long q = sw128_desc(su32(M.qk[0][0]));
-#pragma unroll 1
+#pragma unroll
             for (int product = 0; product < 3; ++product) {  // lo hi, hi lo, hi hi
                 const unsigned long long x = q + (product == 0) * (kPanels * 1024), y = q + 512 + (product == 1) * (kPanels * 1024);
 #pragma unroll
@@ -213,14 +199,11 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
             }
             mma_commit(&M.done);
         }
-        if (lane == 0) {
-            for (int i = 0; i < 4 * kPanels; ++i) {  // Q: hi, lo; K: hi, lo
-                const int part = i % (2 * kPanels);
-                bulk_out(slot + i * 8192, M.qk[part / kPanels][part % kPanels] + (i / (2 * kPanels)) * 8192, 8192);
-            }
-            bulk_out_commit();
-        }
         __syncwarp();
+    }
+    if (tid == kBulk) {
+        bulk_out(slot, M.qk, 2 * Slot::tile);
+        bulk_out_commit();
     }
 
 #pragma unroll 1
@@ -228,10 +211,9 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
         const int h = head + m * n.key_heads;
         unsigned char *out = slot + Slot::heads + (long long)m * Slot::head_bytes;
         DeltaFactors *factors = reinterpret_cast<DeltaFactors *>(out + Slot::factors);
-        if (tid == 0) M.bad = 0;
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();  // V is there, and bad has been cleared
-        if (warp == 0) {
+        if (warp == 4) {
+            if (lane == 0) M.bad[m & 1] = 0;
+            __syncwarp();
             // decays and strengths, two tokens a lane; rows behind the run's end change nothing
             float a[2], b[2];
 #pragma unroll
@@ -241,7 +223,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
                 a[e] = in ? A.decay[at] : 1.0f;
                 b[e] = in ? A.beta[at] : 0.0f;
             }
-            if (past(larger(larger(a[0], a[1], b[0]), b[1], 0.0f))) M.bad = 1;
+            if (past(larger(larger(a[0], a[1], b[0]), b[1], 0.0f))) M.bad[m & 1] = 1;
             const float upto[2] = {product_upto(a[0], lane), product_upto(a[1], lane)};
             const float after[2] = {product_after(a[0], lane), product_after(a[1], lane)};
             const float low = __shfl_sync(0xffffffffu, upto[0], 31), high = __shfl_sync(0xffffffffu, upto[1], 31);
@@ -259,126 +241,110 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
                 if (t == 63) factors->end = p;
             }
         }
-        float inv_v;
-        {  // V's column of this lane to TMEM, 32 tokens
-            const float *column = M.v + half * 32 * D + (gt < D ? gt : 0);
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = column[j * D];
-            M.most[0][half][gt] = largest(0.0f, v);
-            __syncthreads();  // the decays are there, too
-            const float most = larger(M.most[0][0][gt], M.most[0][1][gt], 0.0f);
-            const int e = exponent_of(most);
-            inv_v = unscale_of(e);
-            if (past(most)) M.bad = 1;
+        M.most[0][half][gt] = largest(0.0f, v);
+        if (tid == kBulk) bulk_out_read();  // Q's tile, or the last head's W
+        __syncthreads();
+        const float most_v = larger(M.most[0][0][gt], M.most[0][1][gt], 0.0f);
+        const float inv_v = unscale_of(exponent_of(most_v));
+        {
+            if (past(most_v)) M.bad[m & 1] = 1;
             unsigned hi[16], lo[16];
-            split(v, scale_of(e), hi, lo);
+            split(v, scale_of(exponent_of(most_v)), hi, lo);
             tmem_write(mine + kV + half * 16, hi);
             tmem_write(mine + kV + 32 + half * 16, lo);
             tmem_written();
         }
-        if (m == 0) wait(&M.done, phase & 1), ++phase;
+        if (m == 0) wait.warp(&M.done, phase & 1, lane), ++phase;
         tc_fence_after();
-        if (tid == 0) bulk_out_read();  // Q's tile, or the last head's T
-        {
-            // Rows 0-63: products of queries, 64-127: of keys, each times G over the column's scale. Where row and column are of the
-            // same half of the tokens, the product of decays grows from the diagonal; else it is that up to the row in its half times
-            // that after the column in its own. Columns of the upper half mean nothing to rows of the lower one.
-            const int i = gt & 63;
-            const bool key = gt >= 64, upper = w4 & 1, empty = !upper && half;
-            float *a_row = &M.a[i * kPitch + 32 * half];
-            float x[32], most = 0.0f;
-            if (!empty) {
-                tmem_read(mine + kRaw + 32 * half, x);
-                if (upper && !half) {
-                    const float far = M.upto[i];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 c = *reinterpret_cast<const float4 *>(&M.inv_k[j]);
-                        x[j] *= c.x * far, x[j + 1] *= c.y * far, x[j + 2] *= c.z * far, x[j + 3] *= c.w * far;
-                    }
-                } else {
-                    const int row = i & 31, limit = key ? row - 1 : row;
-                    const float *decay = &M.decay[32 * half], *inv = &M.inv[64 + 32 * half];
-                    float p = 1.0f;
-#pragma unroll
-                    for (int j = 31; j >= 0; --j) {
-                        if (j < row) p *= decay[j + 1 < 32 ? j + 1 : 31];
-                        x[j] = j <= limit ? x[j] * inv[j] * p : 0.0f;
-                    }
-                }
-                if (key) {
-                    const float f = M.inv[gt] * M.beta[i];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(a_row + j) = float4{x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
-                } else {
-                    most = largest(0.0f, x);
-                }
-            }
-            M.most[1][half][gt] = most;
-            __syncthreads();
-            if (!key) {
-                const int e = exponent_of(larger(M.most[1][0][gt], M.most[1][1][gt], 0.0f));
-                unsigned hi[16] = {}, lo[16] = {};
-                if (!empty) split(x, scale_of(e), hi, lo);
-                put_pieces(M.tile(0), i, half * 4, hi);
-                put_pieces(M.tile(1), i, half * 4, lo);
-                if (!half) factors->attn[i] = unscale_of(e) * M.inv[i];
-                to_async();
-            }
-        }
-        {
-            // T: inverses of the four blocks of 16 on the diagonal, by two warps; then of pairs of them: the lower left of
-            // [B 0; A C]^-1 is -C^-1 (A B^-1), whose second factor waits in the upper right
-            float *a = M.a;
-            const auto at = [&](int row, int col) { return a + row * kPitch + col; };
-            if (warp == 2 || warp == 3) {
-                const int block = 32 * (warp - 2) + (lane & 16);
-                float c[16];
-                substitute(at(block, block), lane & 15, c);
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) *at(block + j, block + (lane & 15)) = c[j];
-            }
-            __syncthreads();
-            if (tid == 0) {
-                bulk_out(out + Slot::g, M.tile(0), 8192);
-                bulk_out(out + Slot::g + 8192, M.tile(1), 8192);
-                bulk_out_commit();
-            }
-            const int two = gt >> 6, row16 = (gt & 63) >> 2, col16 = (gt & 3) * 4;  // 64 threads each of two pairs
-            float *b = at(32 * two, 32 * two);
-            if (half) times(b + 16 * kPitch, b, row16, col16, 16, 1.0f, b + 16);
-            __syncthreads();
-            if (half) times(b + 16 * kPitch + 16, b + 16, row16, col16, 16, -1.0f, b + 16 * kPitch);
-            __syncthreads();
-            if (half) *reinterpret_cast<float4 *>(b + 16 + row16 * kPitch + col16) = float4{0, 0, 0, 0};
-            __syncthreads();
-            const int row = tid >> 3, col = (tid & 7) * 4;
-            times(at(32, 0), at(0, 0), row, col, 32, 1.0f, at(0, 32));
-            __syncthreads();
-            times(at(32, 32), at(0, 32), row, col, warp * 4 + 4, -1.0f, at(32, 0));
-            if (tid == 0) bulk_out_read();  // G
-            __syncthreads();
-        }
-        {
-            // T's rows as operands: threads 0-63 for U, 64-127 for W
-            const int i = gt & 63;
-            const bool key = gt >= 64, empty = !(w4 & 1) && half;
-            const float *a_row = &M.a[i * kPitch + 32 * half], *by = (key ? M.beta_w : M.beta) + 32 * half;
-            float x[32], most = 0.0f;
-            if (!empty) {
+        // Rows 0-63: products of queries, 64-127: of keys, each times G over the column's scale. Where row and column are of the
+        // same half of the tokens, the product of decays grows from the diagonal; else it is that up to the row in its half times
+        // that after the column in its own. Columns of the upper half mean nothing to rows of the lower one.
+        const int i = gt & 63;
+        const bool key = gt >= 64, upper = w4 & 1, empty = !upper && half;
+        float *a_row = &M.a[i * kPitch + 32 * half];
+        float x[32], most = 0.0f;
+        if (!empty) {
+            tmem_read(mine + kRaw + 32 * half, x);
+            if (upper && !half) {
+                const float far = M.upto[i];
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
-                    const float4 t = *reinterpret_cast<const float4 *>(a_row + j), b = *reinterpret_cast<const float4 *>(by + j);
-                    x[j] = t.x * b.x, x[j + 1] = t.y * b.y, x[j + 2] = t.z * b.z, x[j + 3] = t.w * b.w;
+                    const float4 c = *reinterpret_cast<const float4 *>(&M.inv_k[j]);
+                    x[j] *= c.x * far, x[j + 1] *= c.y * far, x[j + 2] *= c.z * far, x[j + 3] *= c.w * far;
                 }
+            } else {
+                const int row = i & 31, limit = key ? row - 1 : row;
+                const float *decay = &M.decay[32 * half], *inv = &M.inv[64 + 32 * half];
+                float p = 1.0f;
+#pragma unroll
+                for (int j = 31; j >= 0; --j) {
+                    if (j < row) p *= decay[j + 1 < 32 ? j + 1 : 31];
+                    x[j] = j <= limit ? x[j] * inv[j] * p : 0.0f;
+                }
+            }
+            if (key) {
+                const float f = M.inv[gt] * M.beta[i];
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(a_row + j) = float4{x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
+            } else {
                 most = largest(0.0f, x);
             }
-            M.most[0][half][gt] = most;
-            __syncthreads();
-            most = larger(M.most[0][0][gt], M.most[0][1][gt], 0.0f);
-            if (past(most)) M.bad = 1;
+        }
+        M.most[1][half][gt] = most;
+        __syncthreads();
+        if (!key) {
+            const int e = exponent_of(larger(M.most[1][0][gt], M.most[1][1][gt], 0.0f));
+            unsigned hi[16] = {}, lo[16] = {};
+            if (!empty) split(x, scale_of(e), hi, lo);
+            put_pieces(M.tile(0), i, half * 4, hi);
+            put_pieces(M.tile(1), i, half * 4, lo);
+            if (!half) factors->attn[i] = unscale_of(e) * M.inv[i];
+            to_async();
+        } else if (!half) {
+            // T: the inverses of the two blocks of 32 on the diagonal, a warp each
+            float *block = M.a + (w4 == 2 ? 0 : 32 * kPitch + 32), c[32];
+            substitute(block, lane, c);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) block[j * kPitch + lane] = c[j];
+        }
+        __syncthreads();
+        if (tid == 128 + kBulk) {
+            bulk_out(out + Slot::g, M.tile(0), 8192);
+            bulk_out(out + Slot::g + 8192, M.tile(1), 8192);
+            bulk_out_commit();
+            bulk_out_read();
+        }
+        if (!half) {
+            // the lower left is -T22 (A21 T11); the second factor waits in the upper right
+            const int row = (gt >> 3) * 2, col = (gt & 7) * 4;
+            float *a12 = M.a + 32, *a21 = M.a + 32 * kPitch, *a22 = a21 + 32;
+            float4 o[2];
+            times(a21, M.a, row, col, 32, o);
+            *reinterpret_cast<float4 *>(a12 + row * kPitch + col) = o[0];
+            *reinterpret_cast<float4 *>(a12 + (row + 1) * kPitch + col) = o[1];
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            times(a22, a12, row, col, 8 * w4 + 8, o);
+            *reinterpret_cast<float4 *>(a21 + row * kPitch + col) = float4{-o[0].x, -o[0].y, -o[0].z, -o[0].w};
+            *reinterpret_cast<float4 *>(a21 + (row + 1) * kPitch + col) = float4{-o[1].x, -o[1].y, -o[1].z, -o[1].w};
+        }
+        __syncthreads();
+        // T's rows as operands: threads 0-63 for U, 64-127 for W
+        most = 0.0f;
+        if (!empty) {  // (the upper right holds what is no part of T)
+            const float *by = (key ? M.beta_w : M.beta) + 32 * half;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const float4 t = *reinterpret_cast<const float4 *>(a_row + j), b = *reinterpret_cast<const float4 *>(by + j);
+                x[j] = t.x * b.x, x[j + 1] = t.y * b.y, x[j + 2] = t.z * b.z, x[j + 3] = t.w * b.w;
+            }
+            most = largest(0.0f, x);
+        }
+        M.most[0][half][gt] = most;
+        __syncthreads();
+        most = larger(M.most[0][0][gt], M.most[0][1][gt], 0.0f);
+        if (past(most)) M.bad[m & 1] = 1;
+        {
             const int e = exponent_of(most);
             unsigned hi[16] = {}, lo[16] = {};
             if (!empty) split(x, scale_of(e), hi, lo);
@@ -414,17 +380,17 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
             }
             __syncwarp();
         }
-        wait(&M.done, phase & 1), ++phase;
+        if (m + 1 < slab.ratio) load_v(h + n.key_heads);
+        wait.warp(&M.done, phase & 1, lane), ++phase;
         tc_fence_after();
         if (w4 < D / 32) {
-            float x[32];
             tmem_read(mine + kU + half * 32, x);
             float *to = reinterpret_cast<float *>(out + Slot::uu) + half * 32 * D + gt;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(&M.inv_tu[half * 32 + i]);
-                to[i * D] = x[i] * inv_v * f.x, to[i * D + D] = x[i + 1] * inv_v * f.y;
-                to[i * D + 2 * D] = x[i + 2] * inv_v * f.z, to[i * D + 3 * D] = x[i + 3] * inv_v * f.w;
+            for (int j = 0; j < 32; j += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(&M.inv_tu[half * 32 + j]);
+                to[j * D] = x[j] * inv_v * f.x, to[j * D + D] = x[j + 1] * inv_v * f.y;
+                to[j * D + 2 * D] = x[j + 2] * inv_v * f.z, to[j * D + 3 * D] = x[j + 3] * inv_v * f.w;
             }
             unsigned hi[16], lo[16];
             tmem_read(mine + kW + half * 32, x);
@@ -436,18 +402,14 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(DeltaNet n
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        if (tid == 0) {
-            factors->walk = M.bad | M.bad_key;
-            bulk_out(out + Slot::w, M.w[0], Slot::tile);
+        if (tid == kBulk) {
+            factors->walk = M.bad[m & 1] | M.bad_key;
+            bulk_out(out + Slot::w, M.w, Slot::tile);
             bulk_out_commit();
         }
-        if (m + 1 < slab.ratio) {
-            if (tid == 0) bulk_out_read();
-            __syncthreads();
-            fetch_v(h + n.key_heads);
-        }
+        __syncwarp();
     }
-    if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (tid == kBulk || tid == 128 + kBulk) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     settle(&M.abort_flag);
