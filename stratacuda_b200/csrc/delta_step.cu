@@ -40,7 +40,8 @@ __device__ __forceinline__ void add_to(float4 &a, float b, const float4 &c) {
 
 // VEC: rows of the state, of v and of y can be read four columns at a time.
 template <int ROWS, bool VEC>
-__global__ void __launch_bounds__(kStepThreads) k_delta_step(DeltaNet n, DeltaRule A, MixRuns r) {
+__global__ void __launch_bounds__(kStepThreads, ROWS <= 8 ? 6 : 3)
+    k_delta_step(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A, const __grid_constant__ MixRuns r) {
     kv8_enter();
     constexpr int D = ROWS * 16;  // keys there is room for
     __shared__ float kq[2][2][D];
@@ -57,22 +58,46 @@ __global__ void __launch_bounds__(kStepThreads) k_delta_step(DeltaNet n, DeltaRu
         return;
     }
     if (!me.tokens) return;
+    // A token's rows are fetched while the token before it is worked on: key and query, a channel or two a thread, through
+    // shared memory, decay, strength and this thread's columns of v in registers
+    constexpr int E = (D + kStepThreads - 1) / kStepThreads;
+    struct Next {
+        float k[E], q[E], a, b;
+        float4 v;
+    };
+    const float *kp = A.k + first * A.k_stride + kat, *qp = A.q + first * A.q_stride + kat, *vp = A.v + first * A.v_stride + vat;
+    const float *ap = A.decay + first * n.value_heads + h, *bp = A.beta + first * n.value_heads + h;
+    const auto fetch = [&](int t, Next &x) {
+        if (t >= me.tokens) return;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = tid + e * kStepThreads;
+            x.k[e] = i < n.dim ? kp[t * A.k_stride + i] : 0.0f;
+            x.q[e] = i < n.dim ? qp[t * A.q_stride + i] : 0.0f;
+        }
+        x.a = ap[(long long)t * n.value_heads], x.b = bp[(long long)t * n.value_heads];
+        x.v = load4<VEC>(vp + t * A.v_stride, left);
+    };
+    const auto stage = [&](int t, const Next &x) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = tid + e * kStepThreads;
+            if (D % kStepThreads == 0 || i < D) kq[t & 1][0][i] = x.k[e], kq[t & 1][1][i] = x.q[e];
+        }
+    };
+    Next x{};
+    fetch(0, x);
     float *sp = n.state + ((long long)me.sequence * n.dim + row0) * vw + vat;
     float4 S[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) S[i] = row0 + i < n.dim ? load4<VEC>(sp + i * vw, left) : float4{0, 0, 0, 0};
-    const auto stage = [&](int t) {  // keys and query of token t
-        for (int i = tid; i < D; i += kStepThreads) {
-            const bool in = i < n.dim;
-            kq[t & 1][0][i] = in ? A.k[(first + t) * A.k_stride + kat + i] : 0.0f;
-            kq[t & 1][1][i] = in ? A.q[(first + t) * A.q_stride + kat + i] : 0.0f;
-        }
-    };
-    stage(0);
+    float *yp = A.y + first * vw + vat;
+    stage(0, x);
     __syncthreads();
     for (int t = 0; t < me.tokens; ++t) {
-        const float a = A.decay[(first + t) * n.value_heads + h], b = A.beta[(first + t) * n.value_heads + h];
-        const float4 v = load4<VEC>(A.v + (first + t) * A.v_stride + vat, left);
+        const float a = x.a, b = x.b;
+        const float4 v = x.v;
+        fetch(t + 1, x);
         float k[ROWS], dot = 0.0f;
         float4 p{0, 0, 0, 0}, y{0, 0, 0, 0};
 #pragma unroll
@@ -91,25 +116,24 @@ __global__ void __launch_bounds__(kStepThreads) k_delta_step(DeltaNet n, DeltaRu
             part[t & 1][warp][1][lane] = y;
         }
         if (lane == 0) part_kq[t & 1][warp] = dot;
-        if (t + 1 < me.tokens) stage(t + 1);
+        if (t + 1 < me.tokens) stage(t + 1, x);
         __syncthreads();
         p = y = float4{0, 0, 0, 0};
         dot = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             add_to(p, 1.0f, part[t & 1][w][0][lane & 7]);
-            add_to(y, 1.0f, part[t & 1][w][1][lane & 7]);
+            if (warp == 0) add_to(y, 1.0f, part[t & 1][w][1][lane & 7]);
             dot += part_kq[t & 1][w];
         }
         const float4 d{b * (v.x - a * p.x), b * (v.y - a * p.y), b * (v.z - a * p.z), b * (v.w - a * p.w)};
+        if (group == 0)
+            store4<VEC>(yp + t * vw, left, float4{fmaf(dot, d.x, a * y.x), fmaf(dot, d.y, a * y.y), fmaf(dot, d.z, a * y.z), fmaf(dot, d.w, a * y.w)});
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
             S[i] = float4{a * S[i].x, a * S[i].y, a * S[i].z, a * S[i].w};
             add_to(S[i], k[i], d);
         }
-        if (group == 0)
-            store4<VEC>(A.y + (first + t) * vw + vat, left,
-                        float4{fmaf(dot, d.x, a * y.x), fmaf(dot, d.y, a * y.y), fmaf(dot, d.z, a * y.z), fmaf(dot, d.w, a * y.w)});
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
