@@ -14,7 +14,7 @@ constexpr int kRowThreads = 256, kTile = 16, kMaxTaps = 8;
 
 // C: groups of VEC channels a lane.
 template <int TAPS, int VEC, int C, int LANES>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, TAPS == 4 && VEC == 4 && C == 1 ? 3 : 1)
     k_delta_inputs(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaInputs A, const __grid_constant__ MixRuns r) {
     kv8_enter();
     constexpr int W = VEC * C, ROOM = TAPS > 0 ? TAPS : kMaxTaps;
@@ -62,117 +62,104 @@ __global__ void __launch_bounds__(kRowThreads)
     if (t0 >= me.tokens) return;
     const long long c0 = (long long)head * n.dim;
     const float *x = A.x + first * A.row_stride + c0;
-    float w[ROOM][W], past[ROOM][W];  // past[m]: the row m tokens back, [0] the token's own
     float *history = n.history + ((long long)me.sequence * n.channels() + c0) * (taps - 1);
     constexpr bool kWide = TAPS == 4 && VEC == 4;  // four channels' weights are four vectors, their histories three
+    constexpr int kAhead = W <= 4 ? 4 : 1;         // rows in flight
+    float w[ROOM][W], row[ROOM - 1 + kAhead][W];   // row[i] is token t + i - (ROOM - 1); fewer taps than ROOM are the last ones
+    const int skip = ROOM - taps;
     if constexpr (kWide) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             const float4 f = channel(i) < n.dim ? reinterpret_cast<const float4 *>(n.weight)[c0 + channel(i)] : float4{0, 0, 0, 0};
-            w[3][i] = f.x, w[2][i] = f.y, w[1][i] = f.z, w[0][i] = f.w;
+            w[0][i] = f.x, w[1][i] = f.y, w[2][i] = f.z, w[3][i] = f.w;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < W; ++i)
 #pragma unroll
-            for (int m = 0; m < ROOM; ++m) w[m][i] = m < taps && channel(i) < n.dim ? n.weight[(c0 + channel(i)) * taps + taps - 1 - m] : 0.0f;
+            for (int m = 0; m < ROOM; ++m) w[m][i] = m >= skip && channel(i) < n.dim ? n.weight[(c0 + channel(i)) * taps + m - skip] : 0.0f;
     }
-    float old[kWide ? 3 * W : 1];  // the history of lanes that have the run's first tile: three values a channel
-    if constexpr (kWide) {
-        if (t0 == 0) {
+    // The rows before the tile. The first tile's lanes alone read the history, and leave the run's last taps - 1 rows in its place.
+    if (t0 > 0) {
 #pragma unroll
-            for (int i = 0; i < W; i += 4)
+        for (int m = 0; m < ROOM - 1; ++m)
+            if (m >= skip) load(x + (t0 + m - (ROOM - 1)) * A.row_stride, row[m]);
+    } else if constexpr (kWide) {
 #pragma unroll
-                for (int e = 0; e < 3; ++e) {
-                    const float4 f = channel(i) < n.dim ? reinterpret_cast<const float4 *>(history + 3 * channel(i))[e] : float4{0, 0, 0, 0};
-                    old[3 * i + 4 * e] = f.x, old[3 * i + 4 * e + 1] = f.y, old[3 * i + 4 * e + 2] = f.z, old[3 * i + 4 * e + 3] = f.w;
+        for (int i = 0; i < W; i += 4) {
+            if (channel(i) >= n.dim) {
+#pragma unroll
+                for (int m = 0; m < 3; ++m) row[m][i] = row[m][i + 1] = row[m][i + 2] = row[m][i + 3] = 0.0f;
+                continue;
+            }
+            float4 *at = reinterpret_cast<float4 *>(history + 3 * channel(i));
+            const float4 f = at[0], g = at[1], h = at[2];
+            row[0][i] = f.x, row[1][i] = f.y, row[2][i] = f.z, row[0][i + 1] = f.w;
+            row[1][i + 1] = g.x, row[2][i + 1] = g.y, row[0][i + 2] = g.z, row[1][i + 2] = g.w;
+            row[2][i + 2] = h.x, row[0][i + 3] = h.y, row[1][i + 3] = h.z, row[2][i + 3] = h.w;
+            float now[3][4];
+#pragma unroll
+            for (int m = 0; m < 3; ++m) {
+                const int t = me.tokens - 3 + m;
+                if (t >= 0) {
+                    const float4 v = *reinterpret_cast<const float4 *>(x + t * A.row_stride + channel(i));
+                    now[m][0] = v.x, now[m][1] = v.y, now[m][2] = v.z, now[m][3] = v.w;
+                } else {  // a short run moves its history down
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) now[m][e] = t == -3 ? row[0][i + e] : t == -2 ? row[1][i + e] : row[2][i + e];
                 }
+            }
+            at[0] = float4{now[0][0], now[1][0], now[2][0], now[0][1]};
+            at[1] = float4{now[1][1], now[2][1], now[0][2], now[1][2]};
+            at[2] = float4{now[2][2], now[0][3], now[1][3], now[2][3]};
         }
-    }
+    } else {
 #pragma unroll
-    for (int m = 1; m < ROOM; ++m) {  // rows before the tile: past[m - 1] is t0 - m here
-        if (m >= taps) break;
-        if (t0 - m >= 0) {
-            load(x + (t0 - m) * A.row_stride, past[m - 1]);
-        } else if constexpr (kWide) {
+        for (int i = 0; i < W; ++i) {
+            const int c = channel(i);
+            float *mine = history + (long long)c * (taps - 1);
 #pragma unroll
-            for (int i = 0; i < W; ++i) past[m - 1][i] = old[3 * i + 3 - m];
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-                past[m - 1][i] = channel(i) < n.dim ? history[(long long)channel(i) * (taps - 1) + taps - 1 - m + t0] : 0.0f;
+            for (int m = 0; m < ROOM - 1; ++m)
+                row[m][i] = m >= skip && c < n.dim ? mine[m - skip] : 0.0f;
+            if (c >= n.dim) continue;
+            for (int m = 0; m < taps - 1; ++m) {  // ascending: a short run moves its history down
+                const int t = me.tokens - (taps - 1) + m;
+                mine[m] = t >= 0 ? x[t * A.row_stride + c] : mine[m + me.tokens];
+            }
         }
     }
     const int end = min(me.tokens, t0 + kTile);
-    constexpr int kAhead = W <= 4 ? 4 : 1;  // rows in flight
-    for (int t1 = t0; t1 < end; t1 += kAhead) {
-        float ahead[kAhead][W];
+    const float scale = is_q ? A.q_scale : 1.0f;
+#pragma unroll 1
+    for (int t = t0; t < end; t += kAhead) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-            if (t1 + u < end) load(x + (t1 + u) * A.row_stride, ahead[u]);
+            if (t + u < end) load(x + (t + u) * A.row_stride, row[ROOM - 1 + u]);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (t1 + u >= end) break;
-#pragma unroll
-            for (int m = ROOM - 1; m > 0; --m)
-#pragma unroll
-                for (int i = 0; i < W; ++i) past[m][i] = past[m - 1][i];
             float s[W], sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                past[0][i] = ahead[u][i];
                 s[i] = 0.0f;
 #pragma unroll
-                for (int m = ROOM - 1; m >= 0; --m)
-                    if (m < taps) s[i] = fmaf(w[m][i], past[m][i], s[i]);
+                for (int m = 0; m < ROOM; ++m)
+                    if (TAPS > 0 || m >= skip) s[i] = fmaf(w[m][i], row[u + m][i], s[i]);
                 s[i] = __fdividef(s[i], 1.0f + expf(-s[i]));
                 sum = fmaf(s[i], s[i], sum);
             }
             if (normed) {
 #pragma unroll
                 for (int m = LANES / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(mates, sum, m);
-                const float inv = (is_q ? A.q_scale : 1.0f) / sqrtf(sum + A.epsilon);
+                const float inv = scale * rsqrtf(sum + A.epsilon);
 #pragma unroll
                 for (int i = 0; i < W; ++i) s[i] *= inv;
             }
-            store(out + (first + t1 + u) * ow, s);
-        }
-    }
-    if (t0 == 0 && taps > 1) {
-        // the first tile's lanes alone have read the history: they leave the run's last taps - 1 rows in its place
-        if constexpr (kWide) {
-#pragma unroll
-            for (int i = 0; i < W; i += 4) {
-                if (channel(i) >= n.dim) continue;
-                float now[3][4];
-#pragma unroll
-                for (int m = 0; m < 3; ++m) {
-                    const int t = me.tokens - 3 + m;
-                    if (t >= 0) {
-                        const float4 f = *reinterpret_cast<const float4 *>(x + t * A.row_stride + channel(i));
-                        now[m][0] = f.x, now[m][1] = f.y, now[m][2] = f.z, now[m][3] = f.w;
-                    } else {  // a short run moves its history down
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) now[m][e] = t == -3 ? old[3 * (i + e)] : t == -2 ? old[3 * (i + e) + 1] : old[3 * (i + e) + 2];
-                    }
-                }
-                float4 *to = reinterpret_cast<float4 *>(history + 3 * channel(i));
-                to[0] = float4{now[0][0], now[1][0], now[2][0], now[0][1]};
-                to[1] = float4{now[1][1], now[2][1], now[0][2], now[1][2]};
-                to[2] = float4{now[2][2], now[0][3], now[1][3], now[2][3]};
-            }
-            return;
+            if (t + u < end) store(out + (first + t + u) * ow, s);
         }
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const int c = channel(i);
-            if (c >= n.dim) continue;
-            float *mine = history + (long long)c * (taps - 1);
-            for (int m = 0; m < taps - 1; ++m) {  // ascending: a short run moves its history down
-                const int t = me.tokens - (taps - 1) + m;
-                mine[m] = t >= 0 ? x[t * A.row_stride + c] : mine[m + me.tokens];
-            }
-        }
+        for (int m = 0; m < ROOM - 1; ++m)
+#pragma unroll
+            for (int i = 0; i < W; ++i) row[m][i] = row[m + kAhead][i];
     }
 }
 

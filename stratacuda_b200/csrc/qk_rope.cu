@@ -1,7 +1,7 @@
 // Norms of queries and keys for each head with the position's rotation in the same pass (strata_qk_rope).
 //
 // Bound by bytes: a group of LANES lanes has a head row, reads it once from memory (what a channel is paired with comes from
-// L1), and writes it once.
+// L1), and writes it once. A block has heads of one token, so that no index is divided.
 #include "mixers.cuh"
 
 namespace strata {
@@ -11,13 +11,12 @@ constexpr int kQkThreads = 256;
 
 // C: groups of VEC channels a lane.
 template <int VEC, int C, int LANES>
-__global__ void __launch_bounds__(kQkThreads) k_qk_rope(QkRope W, QkRopeRows A, MixRuns r) {
+__global__ void __launch_bounds__(kQkThreads)
+    k_qk_rope(const __grid_constant__ QkRope W, const __grid_constant__ QkRopeRows A, const __grid_constant__ MixRuns r) {
     kv8_enter();
     constexpr int N = VEC * C;
-    const int sub = threadIdx.x % LANES, all = W.heads + W.kv_heads, run = blockIdx.y;
-    const long long item = (long long)blockIdx.x * (kQkThreads / LANES) + threadIdx.x / LANES;
-    const int t = (int)(item / all), head = (int)(item % all);
-    if (t >= r.count) return;
+    const int sub = threadIdx.x % LANES, run = blockIdx.z, t = blockIdx.x, head = blockIdx.y * (kQkThreads / LANES) + threadIdx.x / LANES;
+    if (head >= W.heads + W.kv_heads) return;
     const unsigned mates = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << ((threadIdx.x & 31) / LANES * LANES);
     const MixRun me = mix_run(r, W.sequences, run, W.err);
     const long long row = (long long)run * r.count + t;
@@ -56,7 +55,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_rope(QkRope W, QkRopeRows A, 
     }
 #pragma unroll
     for (int m = LANES / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(mates, sum, m);
-    const float inv = 1.0f / sqrtf(sum / (float)W.dim + A.epsilon);
+    const float inv = rsqrtf(__fdividef(sum, (float)W.dim) + A.epsilon);
 #pragma unroll
     for (int i = 0; i < N; i += VEC) {
         const int c = channel(i);
@@ -94,10 +93,9 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_rope(QkRope W, QkRopeRows A, 
 
 template <int VEC, int C, int LANES>
 cudaError_t launch_qk(const QkRope &w, const QkRopeRows &a, const MixRuns &r, cudaStream_t s) {
-    const long long items = (long long)r.count * (w.heads + w.kv_heads), per = kQkThreads / LANES;
-    const long long blocks = (items + per - 1) / per;
-    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    return kv8_launch(k_qk_rope<VEC, C, LANES>, dim3((unsigned)blocks, r.segments), dim3(kQkThreads), 0, 1, s, w, a, r);
+    const int per = kQkThreads / LANES;
+    return kv8_launch(k_qk_rope<VEC, C, LANES>, dim3((unsigned)r.count, (unsigned)((w.heads + w.kv_heads + per - 1) / per), (unsigned)r.segments),
+                      dim3(kQkThreads), 0, 1, s, w, a, r);
 }
 
 }  // namespace
