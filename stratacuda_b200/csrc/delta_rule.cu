@@ -7,7 +7,13 @@
 namespace strata {
 namespace {
 
-constexpr int kShortRun = 32;  // rows of a run up to which the state walks token by token
+// Rows of a run up to which it is taken token by token. A call in chunks takes 35 us however short its runs are (25 us with heads
+// of 64), token by token 0.7 us a row, and with more state than the multiprocessors walk at once as much longer as chunks get:
+// 16 sessions of 32 heads of 128 92 us in chunks, 106 us token by token at 32 rows; 64 of 8 heads of 64 57 us, 34 us at 32 rows.
+int short_run(const DeltaNet &n, const MixRuns &r) {
+    if (n.dim <= 64) return 48;
+    return (long long)r.segments * n.value_heads <= 148 / 2 ? 44 : 28;
+}
 
 }  // namespace
 
@@ -15,7 +21,7 @@ cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, 
     const int ratio = n.value_heads / n.key_heads;
     const long long bytes = n.dim <= 64 ? DeltaSlot<64>::bytes(ratio) : DeltaSlot<128>::bytes(ratio);
     const int room = (int)((long long)STRATA_DELTA_WORKSPACE_BYTES / bytes);  // slots
-    if (n.dim > 128 || r.count <= kShortRun || room < 1) return delta_step(n, a, r, s);
+    if (n.dim > 128 || r.count <= short_run(n, r) || room < 1) return delta_step(n, a, r, s);
     const bool vec = n.dim % 4 == 0 && a.q_stride % 4 == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 && mix_aligned16(a.q) &&
                      mix_aligned16(a.k) && mix_aligned16(a.v);
     // Whole runs where they fit; else as many runs as give each multiprocessor two value heads, and their chunks in turn.

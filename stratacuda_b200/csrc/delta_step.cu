@@ -3,13 +3,20 @@
 // With the state S [key][value] of a value head before the token, and decay a, strength b:
 //   d = b (v - a S^T k),  y = a S^T q + (k . q) d,  S <- a S + k d^T
 // so that prediction and result come from one pass over the state as it was: one exchange between warps a token.
-// A block has 32 value columns of a head (columns do not meet), its 128 threads 4 columns by ROWS keys each, in registers.
+// A block has 32 value columns of a head (columns do not meet), a thread of its WARPS warps 4 columns by ROWS keys, in registers.
+//
+// Single tokens of many sequences are bound by the states' bytes (64 sessions of 32 heads of 128: 54 us, 5 TB/s of 268 MB), runs by
+// instructions and the way from token to token: rows come through asynchronous copies kAhead tokens ahead, keys and queries twice
+// so that products are paired (one session, 0.7 us a token; 0.83 with rows fetched one token ahead).
 #include "delta_chunk.cuh"
 
 namespace strata {
 namespace {
 
-constexpr int kStepThreads = 128, kStepCols = 32;
+constexpr int kStepCols = 32, kAhead = 4, kRing = 8;
+// Of heads of more than 64 keys, blocks up to which four warps share one: with few blocks the way from token to token is shorter (one
+// session of 32 heads of 128, 32 tokens: 25 us against 32), with many two warps need fewer instructions (16 sessions 106 us against 117).
+constexpr int kFewBlocks = 2 * 148;
 
 template <bool VEC>
 __device__ __forceinline__ float4 load4(const float *p, int left) {
@@ -31,127 +38,159 @@ __device__ __forceinline__ float sum_groups(float x) {  // over the warp's four 
     x += __shfl_xor_sync(0xffffffffu, x, 8);
     return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
-__device__ __forceinline__ void add_to(float4 &a, float b, const float4 &c) {
-    a.x = fmaf(b, c.x, a.x);
-    a.y = fmaf(b, c.y, a.y);
-    a.z = fmaf(b, c.z, a.z);
-    a.w = fmaf(b, c.w, a.w);
+// Pairs of F32 in one register pair.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ float4 sum_groups(Pair x, Pair y) {
+    float4 f;
+    unpack2(x, f.x, f.y);
+    unpack2(y, f.z, f.w);
+    return float4{sum_groups(f.x), sum_groups(f.y), sum_groups(f.z), sum_groups(f.w)};
+}
+__device__ __forceinline__ void copy4(float *to, const float *from, bool in) {  // zero where not `in`
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(to))), "l"(from), "r"(in ? 4 : 0)
+                 : "memory");
 }
 
-// VEC: rows of the state, of v and of y can be read four columns at a time.
-template <int ROWS, bool VEC>
-__global__ void __launch_bounds__(kStepThreads, ROWS <= 8 ? 6 : 3)
+// VEC: rows of the state and of y can be read and written four columns at a time.
+template <int ROWS, int WARPS, bool VEC>
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 2 ? 8 : ROWS <= 8 ? 6 : 3)
     k_delta_step(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A, const __grid_constant__ MixRuns r) {
     kv8_enter();
-    constexpr int D = ROWS * 16;  // keys there is room for
-    __shared__ float kq[2][2][D];
-    __shared__ float4 part[2][4][2][8];
-    __shared__ float part_kq[2][4];
-    const int slices = (n.dim + kStepCols - 1) / kStepCols, h = blockIdx.x / slices, run = blockIdx.y;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = warp * 4 + (lane >> 3);
-    const int col = (int)(blockIdx.x % slices) * kStepCols + 4 * (lane & 7), row0 = group * ROWS, left = n.dim - col;
+    constexpr int D = ROWS * 4 * WARPS, kStepThreads = 32 * WARPS;  // keys there is room for
+    struct Token {
+        float2 k[D], q[D];  // each twice, as a pair
+        float v[kStepCols], a, b, pad[2];
+    };
+    __shared__ __align__(16) Token ring[kRing];
+    __shared__ float4 part[2][2][WARPS][8];
+    __shared__ float part_kq[2][WARPS];
+    const int slices = (n.dim + kStepCols - 1) / kStepCols, h = blockIdx.x / slices, run = blockIdx.y, col0 = (int)(blockIdx.x % slices) * kStepCols;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = warp * 4 + (lane >> 3), mine = 4 * (lane & 7);
+    const int row0 = group * ROWS, left = n.dim - col0 - mine;
     const long long first = (long long)run * r.count;  // the run's first row
     const MixRun me = mix_run_alone(r, n.sequences, run, n.err);
-    const long long vw = (long long)n.value_heads * n.dim, vat = (long long)h * n.dim + col, kat = (long long)(h % n.key_heads) * n.dim;
+    const long long vw = (long long)n.value_heads * n.dim, vat = (long long)h * n.dim + col0, kat = (long long)(h % n.key_heads) * n.dim;
+    float *yp = A.y + first * vw + vat + mine;
     if (me.sequence < 0) {
-        for (long long t = group; t < r.count; t += 16) store4<VEC>(A.y + (first + t) * vw + vat, left, float4{0, 0, 0, 0});
+        for (long long t = group; t < r.count; t += 4 * WARPS) store4<VEC>(yp + t * vw, left, float4{0, 0, 0, 0});
         return;
     }
     if (!me.tokens) return;
-    // A token's rows are fetched while the token before it is worked on: key and query, a channel or two a thread, through
-    // shared memory, decay, strength and this thread's columns of v in registers
-    constexpr int E = (D + kStepThreads - 1) / kStepThreads;
-    struct Next {
-        float k[E], q[E], a, b;
-        float4 v;
-    };
     const float *kp = A.k + first * A.k_stride + kat, *qp = A.q + first * A.q_stride + kat, *vp = A.v + first * A.v_stride + vat;
     const float *ap = A.decay + first * n.value_heads + h, *bp = A.beta + first * n.value_heads + h;
-    const auto fetch = [&](int t, Next &x) {
-        if (t >= me.tokens) return;
+    const auto fetch = [&](int t) {
+        if (t < me.tokens) {
+            Token &x = ring[t % kRing];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = tid + e * kStepThreads;
-            x.k[e] = i < n.dim ? kp[t * A.k_stride + i] : 0.0f;
-            x.q[e] = i < n.dim ? qp[t * A.q_stride + i] : 0.0f;
+            for (int i = tid; i < D; i += kStepThreads) {
+                const bool in = i < n.dim;
+                const float *k = in ? kp + t * A.k_stride + i : kp, *q = in ? qp + t * A.q_stride + i : qp;
+                copy4(&x.k[i].x, k, in), copy4(&x.k[i].y, k, in);
+                copy4(&x.q[i].x, q, in), copy4(&x.q[i].y, q, in);
+            }
+            if (tid < kStepCols) copy4(&x.v[tid], col0 + tid < n.dim ? vp + t * A.v_stride + tid : vp, col0 + tid < n.dim);
+            if (tid == 32) copy4(&x.a, ap + (long long)t * n.value_heads, true);
+            if (tid == 33) copy4(&x.b, bp + (long long)t * n.value_heads, true);
         }
-        x.a = ap[(long long)t * n.value_heads], x.b = bp[(long long)t * n.value_heads];
-        x.v = load4<VEC>(vp + t * A.v_stride, left);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const auto stage = [&](int t, const Next &x) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = tid + e * kStepThreads;
-            if (D % kStepThreads == 0 || i < D) kq[t & 1][0][i] = x.k[e], kq[t & 1][1][i] = x.q[e];
-        }
-    };
-    Next x{};
-    fetch(0, x);
-    float *sp = n.state + ((long long)me.sequence * n.dim + row0) * vw + vat;
-    float4 S[ROWS];
+    for (int t = 0; t < kAhead; ++t) fetch(t);
+    float *sp = n.state + ((long long)me.sequence * n.dim + row0) * vw + vat + mine;
+    Pair S[ROWS][2];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) S[i] = row0 + i < n.dim ? load4<VEC>(sp + i * vw, left) : float4{0, 0, 0, 0};
-    float *yp = A.y + first * vw + vat;
-    stage(0, x);
+    for (int i = 0; i < ROWS; ++i) {
+        const float4 f = row0 + i < n.dim ? load4<VEC>(sp + i * vw, left) : float4{0, 0, 0, 0};
+        S[i][0] = pack2(f.x, f.y), S[i][1] = pack2(f.z, f.w);
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
     __syncthreads();
+#pragma unroll 1
     for (int t = 0; t < me.tokens; ++t) {
-        const float a = x.a, b = x.b;
-        const float4 v = x.v;
-        fetch(t + 1, x);
-        float k[ROWS], dot = 0.0f;
-        float4 p{0, 0, 0, 0}, y{0, 0, 0, 0};
+        const Token &x = ring[t % kRing];
+        const int turn = t & 1;
+        fetch(t + kAhead);
+        Pair p0 = 0, p1 = 0, y0 = 0, y1 = 0;
+        float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            k[i] = kq[t & 1][0][row0 + i];
-            const float q = kq[t & 1][1][row0 + i];
-            dot = fmaf(k[i], q, dot);
-            add_to(p, k[i], S[i]);
-            add_to(y, q, S[i]);
+        for (int i = 0; i < ROWS; i += 2) {
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(&x.k[row0 + i]), q = *reinterpret_cast<const ulonglong2 *>(&x.q[row0 + i]);
+            p0 = fma_pair(k.x, S[i][0], p0), p1 = fma_pair(k.x, S[i][1], p1);
+            y0 = fma_pair(q.x, S[i][0], y0), y1 = fma_pair(q.x, S[i][1], y1);
+            p0 = fma_pair(k.y, S[i + 1][0], p0), p1 = fma_pair(k.y, S[i + 1][1], p1);
+            y0 = fma_pair(q.y, S[i + 1][0], y0), y1 = fma_pair(q.y, S[i + 1][1], y1);
+            float a, b, c, d, same;
+            unpack2(k.x, a, same), unpack2(q.x, b, same), unpack2(k.y, c, same), unpack2(q.y, d, same);
+            dot = fmaf(a, b, fmaf(c, d, dot));
         }
-        p = float4{sum_groups(p.x), sum_groups(p.y), sum_groups(p.z), sum_groups(p.w)};
-        y = float4{sum_groups(y.x), sum_groups(y.y), sum_groups(y.z), sum_groups(y.w)};
+        const float4 p = sum_groups(p0, p1), y = sum_groups(y0, y1);
         dot = sum_groups(dot);
         if (lane < 8) {
-            part[t & 1][warp][0][lane] = p;
-            part[t & 1][warp][1][lane] = y;
+            part[turn][0][warp][lane] = p;
+            part[turn][1][warp][lane] = y;
         }
-        if (lane == 0) part_kq[t & 1][warp] = dot;
-        if (t + 1 < me.tokens) stage(t + 1, x);
+        if (lane == 0) part_kq[turn][warp] = dot;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");  // the next token's rows
         __syncthreads();
-        p = y = float4{0, 0, 0, 0};
-        dot = 0.0f;
+        const float a = x.a, b = x.b;
+        const float4 v = *reinterpret_cast<const float4 *>(&x.v[mine]);
+        const auto total = [&](int which) {
+            const float4 *f = &part[turn][which][0][lane & 7];
+            float4 s = f[0];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            add_to(p, 1.0f, part[t & 1][w][0][lane & 7]);
-            if (warp == 0) add_to(y, 1.0f, part[t & 1][w][1][lane & 7]);
-            dot += part_kq[t & 1][w];
+            for (int w = 1; w < WARPS; ++w) s.x += f[8 * w].x, s.y += f[8 * w].y, s.z += f[8 * w].z, s.w += f[8 * w].w;
+            return s;
+        };
+        const float4 s = total(0);
+        const float4 d{b * (v.x - a * s.x), b * (v.y - a * s.y), b * (v.z - a * s.z), b * (v.w - a * s.w)};
+        const Pair d0 = pack2(d.x, d.y), d1 = pack2(d.z, d.w), aa = pack2(a, a);
+#pragma unroll
+        for (int i = 0; i < ROWS; i += 2) {
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(&x.k[row0 + i]);
+            S[i][0] = fma_pair(k.x, d0, mul2_rn(aa, S[i][0])), S[i][1] = fma_pair(k.x, d1, mul2_rn(aa, S[i][1]));
+            S[i + 1][0] = fma_pair(k.y, d0, mul2_rn(aa, S[i + 1][0])), S[i + 1][1] = fma_pair(k.y, d1, mul2_rn(aa, S[i + 1][1]));
         }
-        const float4 d{b * (v.x - a * p.x), b * (v.y - a * p.y), b * (v.z - a * p.z), b * (v.w - a * p.w)};
-        if (group == 0)
-            store4<VEC>(yp + t * vw, left, float4{fmaf(dot, d.x, a * y.x), fmaf(dot, d.y, a * y.y), fmaf(dot, d.z, a * y.z), fmaf(dot, d.w, a * y.w)});
+        if (warp == t % WARPS && lane < 8) {
+            const float4 z = total(1);
+            float c = part_kq[turn][0];
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            S[i] = float4{a * S[i].x, a * S[i].y, a * S[i].z, a * S[i].w};
-            add_to(S[i], k[i], d);
+            for (int w = 1; w < WARPS; ++w) c += part_kq[turn][w];
+            store4<VEC>(yp + t * vw, left, float4{fmaf(c, d.x, a * z.x), fmaf(c, d.y, a * z.y), fmaf(c, d.z, a * z.z), fmaf(c, d.w, a * z.w)});
         }
     }
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-        if (row0 + i < n.dim) store4<VEC>(sp + i * vw, left, S[i]);
+    for (int i = 0; i < ROWS; ++i) {
+        float4 f;
+        unpack2(S[i][0], f.x, f.y);
+        unpack2(S[i][1], f.z, f.w);
+        if (row0 + i < n.dim) store4<VEC>(sp + i * vw, left, f);
+    }
 }
 
+template <int ROWS, int WARPS, bool VEC>
+cudaError_t launch_step(dim3 grid, const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s) {
+    return kv8_launch(k_delta_step<ROWS, WARPS, VEC>, grid, dim3(32 * WARPS), 0, 1, s, n, a, r);
+}
 template <bool VEC>
-cudaError_t launch_step(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s) {
+cudaError_t pick_step(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s) {
     const dim3 grid((unsigned)n.value_heads * ((n.dim + kStepCols - 1) / kStepCols), (unsigned)r.segments);
-    const auto kernel = n.dim <= 32 ? k_delta_step<2, VEC> : n.dim <= 64 ? k_delta_step<4, VEC> : n.dim <= 128 ? k_delta_step<8, VEC> : k_delta_step<16, VEC>;
-    return kv8_launch(kernel, grid, dim3(kStepThreads), 0, 1, s, n, a, r);
+    if (n.dim > 128) return launch_step<16, 4, VEC>(grid, n, a, r, s);
+    if (n.dim <= 32) return launch_step<4, 2, VEC>(grid, n, a, r, s);
+    if (n.dim <= 64) return launch_step<8, 2, VEC>(grid, n, a, r, s);
+    if ((long long)grid.x * grid.y > kFewBlocks) return launch_step<16, 2, VEC>(grid, n, a, r, s);
+    return launch_step<8, 4, VEC>(grid, n, a, r, s);
 }
 
 }  // namespace
 
 cudaError_t delta_step(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s) {
-    const bool vec = n.dim % 4 == 0 && a.v_stride % 4 == 0 && mix_aligned16(n.state) && mix_aligned16(a.v) && mix_aligned16(a.y);
-    return vec ? launch_step<true>(n, a, r, s) : launch_step<false>(n, a, r, s);
+    const bool vec = n.dim % 4 == 0 && mix_aligned16(n.state) && mix_aligned16(a.y);
+    return vec ? pick_step<true>(n, a, r, s) : pick_step<false>(n, a, r, s);
 }
 
 }  // namespace strata
