@@ -30,6 +30,11 @@ engine its resident buffers and one fused Q2 mixture-of-experts layer per layer;
 runs each layer's experts as one strata_moe_forward call (src/engine.js:133-156 and
 src/prefill.js:52-78 collapsed into one dispatch, with no host read of the routed ids).
 
+With ``mixers=1`` the token mixers' inner parts run as the run entries of stratacuda_b200.mixers: the delta-rule layer's
+convolution, slices and norms as one dispatch and its rule as another (chunked on the tensor cores for prompt chunks), the norms and
+rotation of queries and keys as one. Values then agree with the reference's entries to F32 rounding instead of bit for bit, and
+prompt chunks may have up to 1024 tokens.
+
 The engine takes any backend with the reference protocol (src/backend.js:58-206): ``alloc``,
 ``write``, ``read``, ``copy``, ``zero``, ``free``, ``run``, ``idle``. On a B200 that is
 ``stratacuda_b200.backend.CudaBackend``.
@@ -72,6 +77,66 @@ def gdn_gates(o, b, g, p: str, x, tokens: int):
         b.run("strata_gdn_gates_batch", dict(Alpha=alpha, Beta=beta, A=o.vector(p + "ssm_a"), Dt=o.vector(p + "ssm_dt.bias"), Decay=decay,
                                              Strength=strength, heads=heads, tokens=tokens), grid(tokens * heads))
     return decay, strength
+
+
+class RunMixers:
+    """The run forms of the token mixers (stratacuda_b200.mixers) of the layers of an engine (one sequence) or a batch: a layer's
+    state and history are the ones that the other entries use, the layers share a workspace."""
+
+    def __init__(self, ops, states, sequences: int, sequence=None):
+        self.o, self.b, self.g, self.states, self.sequences = ops, ops.b, ops.g, states, sequences
+        self.nets, self.ropes, self.owned = {}, {}, []
+        try:
+            from . import _lib as L
+            self.workspace = self._keep(L.DELTA_WORKSPACE_BYTES // 4, "u32", False)
+            self.sequence = sequence
+            if sequence is None:
+                self.sequence = self._keep(sequences, "i32", True)
+                self.b.write(self.sequence, np.arange(sequences, dtype=np.int32))
+        except BaseException:  # nobody else has them
+            self.free()
+            raise
+
+    def _keep(self, n: int, type: str, zero: bool):
+        buf = self.b.alloc(n, type, zero=zero)
+        self.owned.append(buf)
+        return buf
+
+    def gdn(self, layer: int, x, segments: int, count: int):
+        """The delta-rule layer's output projection of `segments` runs of `count` tokens x."""
+        from .mixers import DeltaNet
+        g, o, n, p = self.g, self.o, segments * count, f"blk.{layer}."
+        if layer not in self.nets:
+            st = self.states[layer]
+            self.nets[layer] = DeltaNet(self.b, g["keyHeads"], g["valueHeads"], g["ssmDim"], self.sequences, 4, st["state"], st["conv"],
+                                        o.vector(p + "ssm_conv1d.weight"), self.workspace)
+        net, kd, vd = self.nets[layer], n * g["keyHeads"] * g["ssmDim"], n * g["valueHeads"] * g["ssmDim"]
+        qkv = o.mat(p + "attn_qkv.weight", x, n)
+        q, k, v, y = o.alloc(kd), o.alloc(kd), o.alloc(vd), o.alloc(vd)
+        net.inputs(qkv, q, k, v, self.sequence, segments, count)
+        decay, strength = gdn_gates(o, self.b, g, p, x, n)
+        net.rule(q, k, v, decay, strength, y, self.sequence, segments, count)
+        z = o.mat(p + "attn_gate.weight", x, n)
+        norm = o.norm(y, o.vector(p + "ssm_norm.weight"), g["ssmDim"], n * g["valueHeads"])
+        return o.mat(p + "ssm_out.weight", o.elem(norm, z, 4), n)
+
+    def qk(self, layer: int, full, k, start, segments: int, count: int):
+        """Normed and rotated heads of the [query | gate] rows `full` and the key rows `k`; run i stands at start[i]."""
+        from .mixers import QkRope
+        g, o, p, hd = self.g, self.o, f"blk.{layer}.", self.g["headDim"]
+        if layer not in self.ropes:
+            cos, sin = o.rope_tables()
+            self.ropes[layer] = QkRope(self.b, g["heads"], g["kvHeads"], hd, g["rotary"], g["context"], o.vector(p + "attn_q_norm.weight"),
+                                       o.vector(p + "attn_k_norm.weight"), cos, sin)
+        n = segments * count
+        yq, yk = o.alloc(n * g["heads"] * hd), o.alloc(n * g["kvHeads"] * hd)
+        self.ropes[layer].apply(full, k, yq, yk, start, segments, count, q_head_stride=2 * hd)
+        return yq, yk
+
+    def free(self) -> None:
+        for buf in self.owned:
+            self.b.free(buf)
+        self.owned = []
 
 
 class Ops:
@@ -246,8 +311,13 @@ class Ops:
 class StrataEngine:
     """src/engine.js:7-222 for one backend (no CPU expert lane: every expert runs on the device)."""
 
-    def __init__(self, store, backend, moe_mode: int = 0, graph: bool = False):
+    def __init__(self, store, backend, moe_mode: int = 0, graph: bool = False, mixers: int = 0):
+        require_integer(mixers, "mixers", 0, 1)
+        if mixers and getattr(backend, "kind", None) != "cuda":
+            raise ValueError("The token mixers over runs need the CUDA backend")
         self.moe_mode = moe_mode  # fused layers only: 0 exact (bit-identical), 1 fast (tensor cores)
+        self.mixers = mixers      # 0 the reference's entries (bit-identical), 1 the run forms (stratacuda_b200.mixers)
+        self.runs = None
         # Decode steps replayed from one captured CUDA graph (needs a store with fused layers: a
         # step then reads nothing back until its argmax).
         self.use_graph = bool(graph)
@@ -277,8 +347,8 @@ class StrataEngine:
                 self.moe_trace.append(dict(position=position + t, layer=layer, y=v[t].copy()))
 
     @classmethod
-    def create(cls, store, backend, moe_mode: int = 0, graph: bool = False) -> "StrataEngine":
-        engine = cls(store, backend, moe_mode, graph)
+    def create(cls, store, backend, moe_mode: int = 0, graph: bool = False, mixers: int = 0) -> "StrataEngine":
+        engine = cls(store, backend, moe_mode, graph, **({"mixers": mixers} if mixers else {}))  # (subclasses may not take it)
         try:
             engine.initialize()
         except Exception:
@@ -369,6 +439,14 @@ class StrataEngine:
                 self.states.append(dict(keys=self.keep(kv), values=self.keep(kv)))
             else:
                 self.states.append(dict(state=self.keep(g["ssmDim"] * g["valueHeads"] * g["ssmDim"]), conv=self.keep(c * 3)))
+        if self.mixers:
+            self.runs = RunMixers(self.ops, self.states, 1)
+
+    def position_on_device(self):
+        """The position as a device scalar: the captured steps' own, else written now."""
+        if not self._dev_mode:
+            self.b.write(self._device_scalars()["position"], np.array([self.position], np.int32))
+        return self._dev["position"]
 
     # ---- one token (src/engine.js:73-156)
     def hc(self, prefix: str, inject: bool = True):
@@ -415,6 +493,8 @@ class StrataEngine:
         b.run("strata_ple_add", dict(Residual=self.residual, Gated=gated, Conv=conv, n=hc), grid(hc))
 
     def gdn(self, layer: int, x):
+        if self.runs is not None:
+            return self.runs.gdn(layer, x, 1, 1)
         g, o, b = self.g, self.ops, self.b
         p, st = f"blk.{layer}.", self.states[layer]
         qk, vn = g["ssmDim"] * g["keyHeads"], g["ssmDim"] * g["valueHeads"]
@@ -446,10 +526,13 @@ class StrataEngine:
         p, st, hd = f"blk.{layer}.", self.states[layer], g["headDim"]
         dpos = self._dev["position"] if self._dev_mode else None
         full = o.mat(p + "attn_q.weight", x)
-        qr = o.slice(full, hd, g["heads"], hd * 2)
-        q = o.rotate(o.norm(qr, o.vector(p + "attn_q_norm.weight"), hd, g["heads"]), g["heads"], self.position, device_position=dpos)
-        kr = o.mat(p + "attn_k.weight", x)
-        k = o.rotate(o.norm(kr, o.vector(p + "attn_k_norm.weight"), hd, g["kvHeads"]), g["kvHeads"], self.position, device_position=dpos)
+        if self.runs is not None:
+            q, k = self.runs.qk(layer, full, o.mat(p + "attn_k.weight", x), self.position_on_device(), 1, 1)
+        else:
+            qr = o.slice(full, hd, g["heads"], hd * 2)
+            q = o.rotate(o.norm(qr, o.vector(p + "attn_q_norm.weight"), hd, g["heads"]), g["heads"], self.position, device_position=dpos)
+            kr = o.mat(p + "attn_k.weight", x)
+            k = o.rotate(o.norm(kr, o.vector(p + "attn_k_norm.weight"), hd, g["kvHeads"]), g["kvHeads"], self.position, device_position=dpos)
         v = o.mat(p + "attn_v.weight", x)
         if dpos is not None:  # the same three dispatches with the position read on the device
             attn, gated = o.alloc(g["heads"] * hd), o.alloc(g["heads"] * hd)
@@ -688,7 +771,7 @@ class StrataEngine:
             require_integer(t, "token", 0, self.g["vocab"] - 1)
         if self.position + len(tokens) > self.g["context"]:
             raise ValueError("Context capacity reached")
-        require_integer(chunk_size, "prompt chunk size", 1, 64)
+        require_integer(chunk_size, "prompt chunk size", 1, 1024 if self.mixers else 64)
         if logits and not predict:
             raise ValueError("Logits require prediction")
         self.stats["routes"] = []
@@ -755,6 +838,10 @@ class StrataEngine:
         for buf in (self._dev or {}).values():
             self.b.free(buf)
         self._dev = None
+        if self.runs is not None:
+            self.b.idle()
+            self.runs.free()
+            self.runs = None
         self.ops.dispose()
         for buf in self.persistent:
             self.b.free(buf)
@@ -823,6 +910,8 @@ class PromptBatch:
         b.run("strata_ple_add", dict(Residual=self.residual, Gated=gated, Conv=conv, n=n * hc), grid(n * hc))
 
     def gdn(self, layer: int, x):
+        if self.e.runs is not None:
+            return self.e.runs.gdn(layer, x, 1, self.n)
         g, o, b, n, e = self.g, self.o, self.b, self.n, self.e
         p, st = f"blk.{layer}.", e.states[layer]
         qk, vn = g["ssmDim"] * g["keyHeads"], g["ssmDim"] * g["valueHeads"]
@@ -847,10 +936,14 @@ class PromptBatch:
         p, st, hd = f"blk.{layer}.", e.states[layer], g["headDim"]
         dpos = e._dev["position"] if self.device is not None else None
         full = self.mat(p + "attn_q.weight", x)
-        qr = o.slice(full, hd, n * g["heads"], hd * 2)
-        q = o.rotate(o.norm(qr, o.vector(p + "attn_q_norm.weight"), hd, n * g["heads"]), g["heads"], self.position, n, dpos)
-        kr = self.mat(p + "attn_k.weight", x)
-        k = o.rotate(o.norm(kr, o.vector(p + "attn_k_norm.weight"), hd, n * g["kvHeads"]), g["kvHeads"], self.position, n, dpos)
+        if e.runs is not None:
+            start = dpos if dpos is not None else e.position_on_device()
+            q, k = e.runs.qk(layer, full, self.mat(p + "attn_k.weight", x), start, 1, n)
+        else:
+            qr = o.slice(full, hd, n * g["heads"], hd * 2)
+            q = o.rotate(o.norm(qr, o.vector(p + "attn_q_norm.weight"), hd, n * g["heads"]), g["heads"], self.position, n, dpos)
+            kr = self.mat(p + "attn_k.weight", x)
+            k = o.rotate(o.norm(kr, o.vector(p + "attn_k_norm.weight"), hd, n * g["kvHeads"]), g["kvHeads"], self.position, n, dpos)
         v = self.mat(p + "attn_v.weight", x)
         if dpos is not None:  # the same dispatches with the position read on the device
             attn = o.alloc(n * g["heads"] * hd)
@@ -957,7 +1050,9 @@ class SequenceBatch(PromptBatch):
     quarter of the memory): each step appends to the cache and attends over it. With ``top`` as well, a
     token attends to the ``top`` blocks of 64 tokens that strata_kv8_select picks for each key/value
     head. A slot's values then differ from its own engine's by the cache's rounding, and a slot
-    cannot be exported."""
+    cannot be exported.
+
+    A batch of an engine with ``mixers`` uses the run forms of the token mixers, too."""
 
     def __init__(self, engine: StrataEngine, capacity: int, graph: bool = False, kv8: bool = False, top: int = 0):
         require_integer(capacity, "batch capacity", 1, 1024)
@@ -974,7 +1069,7 @@ class SequenceBatch(PromptBatch):
         self.persistent, self.caches = [], []
         self._graph = self._graph_head = None
         self.disposed = False
-        self.kv8, self.top = bool(kv8), top
+        self.kv8, self.top, self.runs = bool(kv8), top, None
         hc, c = g["width"] * g["streams"], (2 * g["keyHeads"] + g["valueHeads"]) * g["ssmDim"]
         try:
             self.residual = self._keep(capacity * hc)
@@ -998,6 +1093,8 @@ class SequenceBatch(PromptBatch):
             if kv8:  # the sequences of a step, and the one that is being admitted
                 self.dev.update(sequences=self._keep(capacity, "i32"), admitted=self._keep(1, "i32"), begin=self._keep(1, "i32"))
                 b.write(self.dev["sequences"], np.arange(capacity, dtype=np.int32))
+            if getattr(engine, "mixers", 0):
+                self.runs = RunMixers(self.o, self.states, capacity, self.dev.get("sequences"))
         except Exception:
             self.dispose()
             raise
@@ -1078,6 +1175,8 @@ class SequenceBatch(PromptBatch):
         b.run("strata_ple_add", dict(Residual=self.residual, Gated=gated, Conv=conv, n=n * hc), grid(n * hc))
 
     def gdn(self, layer: int, x):
+        if self.runs is not None:
+            return self.runs.gdn(layer, x, self.n, 1)
         g, o, b, n = self.g, self.o, self.b, self.n
         p, st = f"blk.{layer}.", self.states[layer]
         qk, vn = g["ssmDim"] * g["keyHeads"], g["ssmDim"] * g["valueHeads"]
@@ -1110,10 +1209,13 @@ class SequenceBatch(PromptBatch):
             return y
 
         full = self.mat(p + "attn_q.weight", x)
-        qr = o.slice(full, hd, n * g["heads"], hd * 2)
-        q = rotate(o.norm(qr, o.vector(p + "attn_q_norm.weight"), hd, n * g["heads"]), g["heads"])
-        kr = self.mat(p + "attn_k.weight", x)
-        k = rotate(o.norm(kr, o.vector(p + "attn_k_norm.weight"), hd, n * g["kvHeads"]), g["kvHeads"])
+        if self.runs is not None:
+            q, k = self.runs.qk(layer, full, self.mat(p + "attn_k.weight", x), pos, n, 1)
+        else:
+            qr = o.slice(full, hd, n * g["heads"], hd * 2)
+            q = rotate(o.norm(qr, o.vector(p + "attn_q_norm.weight"), hd, n * g["heads"]), g["heads"])
+            kr = self.mat(p + "attn_k.weight", x)
+            k = rotate(o.norm(kr, o.vector(p + "attn_k_norm.weight"), hd, n * g["kvHeads"]), g["kvHeads"])
         v = self.mat(p + "attn_v.weight", x)
         attn = o.alloc(n * g["heads"] * hd)
         if self.kv8:
@@ -1213,6 +1315,9 @@ class SequenceBatch(PromptBatch):
             self.b.graph_free(self._graph)
             self._graph = None
         self.b.idle()
+        if self.runs is not None:
+            self.runs.free()
+            self.runs = None
         for cache in self.caches[::-1]:  # (the first one's workspace is shared)
             cache.free()
         self.caches = []
