@@ -36,6 +36,7 @@ struct DeltaFactors {  // of a chunk's rows, for one value head
 struct DeltaSlab {  // runs, key heads and chunks [first, first + n) of a call
     int run0, runs, head0, heads, chunk0, chunks;
     int ratio;  // value heads of a key head
+    int ahead;  // the first kernel runs while the slab before is on its way through the second
     unsigned char *slots;
     long long slot_bytes;
 };

@@ -114,11 +114,16 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
     PrepareSmem<D> &M = *reinterpret_cast<PrepareSmem<D> *>(smem_raw);
     // half of the columns, row
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = tid >> 7, gt = tid & 127, w4 = warp & 3;
-    kv8_enter();
+    if (slab.ahead) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    else kv8_enter();
+    // Of a slab ahead, this block makes the kernel end after the second one of the slab before.
+    const auto leave = [&] {
+        if (slab.ahead && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+    };
     const int chunk = slab.chunk0 + (int)(blockIdx.x % slab.chunks), head = slab.head0 + (int)(blockIdx.x / slab.chunks % slab.heads);
     const int run = slab.run0 + (int)(blockIdx.x / slab.chunks / slab.heads), t0 = chunk * kChunk;
     const MixRun me = mix_run_alone(r, n.sequences, run, n.err);
-    if (me.sequence < 0 || t0 >= me.tokens) return;
+    if (me.sequence < 0 || t0 >= me.tokens) return leave();
     const int tokens = min(kChunk, me.tokens - t0);
     const long long row0 = (long long)run * r.count + t0;
     unsigned char *slot = slab.slots + blockIdx.x * slab.slot_bytes;
@@ -414,6 +419,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
     __syncthreads();
     settle(&M.abort_flag);
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+    leave();
 }
 
 template <int D, bool VEC>

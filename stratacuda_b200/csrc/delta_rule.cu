@@ -7,12 +7,14 @@
 namespace strata {
 namespace {
 
+constexpr int kSms = 148;
+
 // Rows of a run up to which it is taken token by token. A call in chunks takes 35 us however short its runs are (25 us with heads
 // of 64), token by token 0.7 us a row, and with more state than the multiprocessors walk at once as much longer as chunks get:
 // 16 sessions of 32 heads of 128 92 us in chunks, 106 us token by token at 32 rows; 64 of 8 heads of 64 57 us, 34 us at 32 rows.
 int short_run(const DeltaNet &n, const MixRuns &r) {
     if (n.dim <= 64) return 48;
-    return (long long)r.segments * n.value_heads <= 148 / 2 ? 44 : 28;
+    return (long long)r.segments * n.value_heads <= kSms / 2 ? 44 : 28;
 }
 
 }  // namespace
@@ -24,18 +26,43 @@ cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, 
     if (n.dim > 128 || r.count <= short_run(n, r) || room < 1) return delta_step(n, a, r, s);
     const bool vec = n.dim % 4 == 0 && a.q_stride % 4 == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 && mix_aligned16(a.q) &&
                      mix_aligned16(a.k) && mix_aligned16(a.v);
+    const int all = (r.count + kChunk - 1) / kChunk;
+    DeltaSlab slab{0, 0, 0, 0, 0, 0, ratio, 0, static_cast<unsigned char *>(n.workspace), bytes};
+    const auto one = [&] {
+        cudaError_t e = delta_prepare(n, a, r, slab, vec, s);
+        return e == cudaSuccess ? delta_chain(n, a, r, slab, s) : e;
+    };
+    // Few states leave most multiprocessors idle in the second kernel: there the next slab's first one runs meanwhile, on the
+    // workspace's other half. The first slab gives each multiprocessor two blocks, the next ones those that are left. One prompt
+    // of 2048 tokens over 32 heads of 128 194 -> 182 us, of 8191 over 48 937 -> 680 us, two of 1024 over 32 140 -> 132 us; three
+    // would take 227 us in place of 189: with more states than half of the multiprocessors one slab after another.
+    if ((long long)r.segments * n.value_heads <= kSms / 2) {
+        const int chains = r.segments * n.value_heads, per = r.segments * n.key_heads, most = room / 2 / per;  // chunks of a half
+        const int first = std::min(most, 2 * kSms / per), next = std::min(most, std::max(1, 2 * (kSms - chains) / per));
+        if (most > 0 && first < all) {
+            slab.runs = r.segments, slab.heads = n.key_heads, slab.chunks = first;
+            while (slab.chunk0 < all) {
+                const cudaError_t e = one();
+                if (e != cudaSuccess) return e;
+                slab.chunk0 += slab.chunks, slab.chunks = std::min(next, all - slab.chunk0);
+                slab.slots = static_cast<unsigned char *>(n.workspace) + (slab.slots == n.workspace ? room / 2 * bytes : 0);
+                slab.ahead = 1;
+            }
+            return cudaSuccess;
+        }
+    }
     // Whole runs where they fit; else as many runs as give each multiprocessor two value heads, and their chunks in turn.
-    const int all = (r.count + kChunk - 1) / kChunk, heads = std::min(n.key_heads, room);
-    int runs = std::max(1, std::min({r.segments, room / heads, (2 * 148 + heads * ratio - 1) / (heads * ratio)}));
+    const int heads = std::min(n.key_heads, room);
+    int runs = std::max(1, std::min({r.segments, room / heads, (2 * kSms + heads * ratio - 1) / (heads * ratio)}));
     const int chunks = std::min(all, room / (runs * heads));
     if (chunks == all) runs = std::min(r.segments, room / (heads * chunks));
     for (int run0 = 0; run0 < r.segments; run0 += runs)
         for (int head0 = 0; head0 < n.key_heads; head0 += heads)
             for (int chunk0 = 0; chunk0 < all; chunk0 += chunks) {
-                const DeltaSlab slab{run0, std::min(runs, r.segments - run0), head0, std::min(heads, n.key_heads - head0), chunk0,
-                                     std::min(chunks, all - chunk0), ratio, static_cast<unsigned char *>(n.workspace), bytes};
-                cudaError_t e = delta_prepare(n, a, r, slab, vec, s);
-                if (e == cudaSuccess) e = delta_chain(n, a, r, slab, s);
+                slab.run0 = run0, slab.runs = std::min(runs, r.segments - run0);
+                slab.head0 = head0, slab.heads = std::min(heads, n.key_heads - head0);
+                slab.chunk0 = chunk0, slab.chunks = std::min(chunks, all - chunk0);
+                const cudaError_t e = one();
                 if (e != cudaSuccess) return e;
             }
     return cudaSuccess;

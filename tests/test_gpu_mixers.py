@@ -289,6 +289,39 @@ def test_rule_of_more_chunks_than_the_workspace_holds(torch):
     check_rule(torch, 8, 8, 128, 40, 321, lengths=[321 - 7 * i for i in range(40)])
 
 
+@pytest.mark.parametrize("lengths,sequence", [(None, None), ([1250, 1250], [1, 0]), ([1200, 3], None), ([700, 1250], [2, -1]), ([0, 64 * 9], None)])
+def test_rule_of_few_long_runs(torch, lengths, sequence):
+    """Parts of a prompt follow one another, the next one's first kernel beside the last one's second; runs end in all of them."""
+    check_rule(torch, 16, 32, 64, 2, 1250, sequence, lengths, 3)
+
+
+def test_rule_of_few_long_runs_repeats_and_replays(torch):
+    """Two calls in a row, eagerly and from a graph: bit for bit the same, on one workspace."""
+    kh, vh, dim, count = 16, 32, 128, 2500
+    c = R.rule_case(np.random.default_rng(3), kh, vh, dim, 1, 1, count)
+    net = Net(torch, kh, vh, dim, 1, c)
+    start = torch.tensor(c["state"], device="cuda")
+    args = [net.t[n] for n in ("q", "k", "v", "decay", "beta")]
+    ys, sequence = [torch.zeros(count, vh * dim, device="cuda") for _ in range(2)], net.ints([0])
+
+    def twice():
+        for y in ys:
+            net.net.rule(*args, y, sequence, 1, count, stream=torch.cuda.current_stream().cuda_stream)
+
+    twice()
+    torch.cuda.synchronize()
+    first, after = [y.cpu().numpy() for y in ys], net.state()
+    assert not np.array_equal(first[0], first[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        twice()
+    for again in (twice, graph.replay, graph.replay):
+        net.t["state"].copy_(start)
+        again()
+        torch.cuda.synchronize()
+        assert all(np.array_equal(y.cpu().numpy(), f) for y, f in zip(ys, first)) and np.array_equal(net.state(), after)
+
+
 # ---------------------------------------------------------------- inputs
 
 @pytest.mark.parametrize("count", [1, 2, 3, 4, 15, 16, 17, 100])
