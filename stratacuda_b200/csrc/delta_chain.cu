@@ -33,7 +33,9 @@ struct __align__(1024) ChainSmem {
     float s_max[4][128];
     float2 d_max[4][128];  // also the sums of chunks that are walked
     unsigned long long w_full[2], w_empty[2], row_full[2], row_empty[2], qk_full, qk_empty, g_full, g_empty;
-    unsigned long long s_ready, r_free, d_ready, y_ready, z_done, d_done, y_done;
+    unsigned long long s_hi, s_ready, r_free, d_hi, d_ready, y_ready, z_done, d_done, y_done;
+    float *to;  // where the state goes and is walked, rows to_next floats apart
+    long long to_next;
     unsigned tmem;
     int abort_flag;
 };
@@ -42,35 +44,38 @@ __device__ __forceinline__ void lane_sync(int w4) { asm volatile("bar.sync %0, 1
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
 
 // A chunk token by token, on the state in memory: a channel's four threads add up their parts of the keys.
-template <int D>
-__device__ __noinline__ void walk_chunk(const DeltaNet &n, const DeltaRule &A, ChainSmem<D> &M, float *state, long long row, int tokens, int h, int part, int v) {
+template <int D, bool ENDS>
+__device__ __noinline__ void walk_chunk(const DeltaNet &n, const DeltaRule &A, ChainSmem<D> &M, long long row, int tokens, int h, int part, int v, bool values) {
     constexpr int kPart = D / 4;
     const long long vw = (long long)n.value_heads * n.dim, key = (long long)(h % n.key_heads) * n.dim + part * kPart;
     const bool in = v < n.dim;
     const int keys = in ? min(kPart, n.dim - part * kPart) : 0;
+    const long long next = M.to_next;
+    float *const state = M.to + part * kPart * next + v;
     for (int t = 0; t < tokens; ++t, ++row) {
         const float *kp = A.k + row * A.k_stride + key, *qp = A.q + row * A.q_stride + key;
         const float a = A.decay[row * n.value_heads + h], b = A.beta[row * n.value_heads + h];
         float p = 0.0f, y = 0.0f;
         for (int i = 0; i < keys; ++i) {
-            state[i * vw] *= a;
-            p = fmaf(state[i * vw], kp[i], p);
+            state[i * next] *= a;
+            p = fmaf(state[i * next], kp[i], p);
         }
         M.d_max[part][v].x = p;
         lane_sync(v >> 5);
-        const float d = b * ((in ? A.v[row * A.v_stride + (long long)h * n.dim + v] : 0.0f) -
+        const float d = b * ((in && values ? A.v[row * A.v_stride + (long long)h * n.dim + v] : 0.0f) -
                              ((M.d_max[0][v].x + M.d_max[1][v].x) + (M.d_max[2][v].x + M.d_max[3][v].x)));
         for (int i = 0; i < keys; ++i) {
-            state[i * vw] = fmaf(kp[i], d, state[i * vw]);
-            y = fmaf(state[i * vw], qp[i], y);
+            state[i * next] = fmaf(kp[i], d, state[i * next]);
+            if (!ENDS) y = fmaf(state[i * next], qp[i], y);
         }
         M.d_max[part][v].y = y;
         lane_sync(v >> 5);
-        if (part == 0 && in) A.y[row * vw + (long long)h * n.dim + v] = (M.d_max[0][v].y + M.d_max[1][v].y) + (M.d_max[2][v].y + M.d_max[3][v].y);
+        if (!ENDS && part == 0 && in) A.y[row * vw + (long long)h * n.dim + v] = (M.d_max[0][v].y + M.d_max[1][v].y) + (M.d_max[2][v].y + M.d_max[3][v].y);
     }
 }
 
-template <int D>
+// ENDS: nothing but where parts of runs end, from zeros and (their transition) without values from the identity.
+template <int D, bool ENDS>
 __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A,
                                                                   const __grid_constant__ MixRuns r, const __grid_constant__ DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
@@ -79,18 +84,44 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
     ChainSmem<D> &M = *reinterpret_cast<ChainSmem<D> *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     kv8_enter();
-    const int m = (int)(blockIdx.x % slab.ratio), head_l = (int)(blockIdx.x / slab.ratio % slab.heads), run_l = (int)(blockIdx.x / slab.ratio / slab.heads);
+    int block = (int)blockIdx.x;
+    bool transition = false;
+    int part = 0;
+    if (ENDS) transition = block & 1, block >>= 1;
+    if (slab.parts > 1) part = block % (slab.parts - ENDS), block /= slab.parts - ENDS;
+    const int chain = block, m = block % slab.ratio, head_l = block / slab.ratio % slab.heads, run_l = block / slab.ratio / slab.heads;
     const int h = slab.head0 + head_l + m * n.key_heads, run = slab.run0 + run_l;
     const MixRun me = mix_run_alone(r, n.sequences, run, n.err);
     const long long first = (long long)run * r.count, vw = (long long)n.value_heads * n.dim;
-    const int begin = slab.chunk0 * kChunk;
+    int begin = slab.chunk0 * kChunk;
     if (me.sequence < 0) {
+        if (ENDS || part > 0) return;
         const long long end = min((long long)r.count, (long long)begin + (long long)slab.chunks * kChunk), rows = end - begin;
         for (long long i = tid; i < rows * n.dim; i += kChainThreads) A.y[(first + begin + i / n.dim) * vw + (long long)h * n.dim + i % n.dim] = 0.0f;
         return;
     }
     if (begin >= me.tokens) return;
-    const int chunks = min(slab.chunks, (me.tokens - begin + kChunk - 1) / kChunk);
+    int chunks = min(slab.chunks, (me.tokens - begin + kChunk - 1) / kChunk), chunk = 0;
+    // where the state comes from (null: zeros or the identity), and where it goes
+    float *const real = n.state + (long long)me.sequence * n.dim * vw + (long long)h * n.dim;
+    float *from = real, *to = real;
+    long long from_next = vw, to_next = vw;
+    if (slab.parts > 1) {
+        const int last = (chunks - 1) / slab.part_chunks;
+        float *const own = slab.states + (long long)chain * (slab.parts - 1) * (2 * D * D);
+        if (ENDS) {
+            if (part >= last || (transition && part == 0)) return;
+            if (part > 0) from = nullptr;
+            to = own + (2 * part + !transition) * (D * D), to_next = D;
+        } else {
+            const bool whole = slab.whole[chain] != 0;
+            if (part > (whole ? 0 : last)) return;
+            from = own + (part ? 2 * part - 1 : 0) * (D * D), from_next = D;
+            if (!whole && part < last) to = from, to_next = D;
+            if (whole) part = -1;
+        }
+        if (part >= 0) chunk = part * slab.part_chunks, chunks = min(slab.part_chunks, chunks - chunk), begin += chunk * kChunk;
+    }
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -98,10 +129,11 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             bar_init(&M.row_full[i], 1), bar_init(&M.row_empty[i], kWork / 32 + 1);
         }
         bar_init(&M.qk_full, 1), bar_init(&M.qk_empty, 1), bar_init(&M.g_full, 1), bar_init(&M.g_empty, 1);
-        bar_init(&M.s_ready, kWork / 32), bar_init(&M.r_free, kWork / 32), bar_init(&M.d_ready, kWork / 32), bar_init(&M.y_ready, kWork / 32);
+        bar_init(&M.s_hi, kWork / 32), bar_init(&M.d_hi, kWork / 32), bar_init(&M.s_ready, kWork / 32), bar_init(&M.r_free, kWork / 32), bar_init(&M.d_ready, kWork / 32), bar_init(&M.y_ready, kWork / 32);
         bar_init(&M.z_done, 1), bar_init(&M.d_done, 1), bar_init(&M.y_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         M.abort_flag = 0;
+        M.to = to, M.to_next = to_next;  // (there: seldom used, and the chunks' loop has no registers to spare)
     }
     if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&M.tmem)) : "memory");
@@ -117,7 +149,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
 
     if (warp == kFetchWarp) {
         if (lane == 0) {
-            const unsigned char *slot = slab.slots + ((long long)run_l * slab.heads + head_l) * slab.chunks * slab.slot_bytes;
+            const unsigned char *slot = slab.slots + (((long long)run_l * slab.heads + head_l) * slab.chunks + chunk) * slab.slot_bytes;
             const long long mine = Slot::heads + (long long)m * Slot::head_bytes;
             const auto fetch = [&](void *to, const unsigned char *from, unsigned bytes, unsigned long long *full) {
                 bar_expect(full, bytes);
@@ -132,6 +164,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 fetch(&M.row[st], slot + mine + Slot::uu, sizeof M.row[st], &M.row_full[st]);
                 wait(&M.qk_empty, again1);
                 fetch(M.qk, slot, 2 * Slot::tile, &M.qk_full);
+                if (ENDS) continue;
                 wait(&M.g_empty, again1);
                 fetch(M.g, slot + mine + Slot::g, Slot::attn, &M.g_full);
             }
@@ -149,43 +182,59 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 const bool walk = M.row[st].f.walk != 0;
                 bar_arrive(&M.row_empty[st]);
                 if (walk) {  // nothing of it is used
-                    wait(&M.w_full[st], ph), wait(&M.qk_full, ph1), wait(&M.g_full, ph1);
-                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.qk_empty), bar_arrive(&M.g_empty);
+                    wait(&M.w_full[st], ph), wait(&M.qk_full, ph1);
+                    bar_arrive(&M.w_empty[st]), bar_arrive(&M.qk_empty);
+                    if (ENDS) continue;
+                    wait(&M.g_full, ph1);
+                    bar_arrive(&M.g_empty);
                     continue;
                 }
                 const unsigned now = live & 1;
                 ++live;
                 const unsigned long long w = turned_desc(su32(M.w[st]), 0);
                 wait(&M.w_full[st], ph);
-                wait(&M.s_ready, now);
+                wait(&M.s_hi, now);
                 tc_fence_after();
 #pragma unroll
-                for (int product = 0; product < 3; ++product)  // lo hi, hi lo, hi hi
+                for (int product = 0; product < 3; ++product) {  // hi lo, lo hi, hi hi
+                    if (product == 1) {
+                        wait(&M.s_ready, now);
+                        tc_fence_after();
+                    }
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        mma_f16_ts(tmem + kZ, tmem + (product == 0 ? kSLo : kS) + k * 8, w + (product == 1) * kLoW + k * 128, turned_idesc(128, 64),
+                        mma_f16_ts(tmem + kZ, tmem + (product == 1 ? kSLo : kS) + k * 8, w + (product == 0) * kLoW + k * 128, turned_idesc(128, 64),
                                    product || k);
+                }
                 mma_commit(&M.z_done);
                 mma_commit(&M.w_empty[st]);
                 wait(&M.qk_full, ph1);
-                wait(&M.r_free, now);
+                if (!ENDS) {
+                    wait(&M.r_free, now);
+                    tc_fence_after();
+#pragma unroll
+                    for (int product = 0; product < 3; ++product)
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k)
+                            mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8, q + (product == 1) * kLoQk + k / 4 * 1024 + k % 4 * 2,
+                                       idesc_f16(128, 64), product || k);
+                }
+                wait(&M.d_hi, now);
                 tc_fence_after();
 #pragma unroll
-                for (int product = 0; product < 3; ++product)
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_f16_ts(tmem + kR, tmem + (product == 0 ? kSLo : kS) + k * 8, q + (product == 1) * kLoQk + k / 4 * 1024 + k % 4 * 2,
-                                   idesc_f16(128, 64), product || k);
-                wait(&M.d_ready, now);
-                tc_fence_after();
-#pragma unroll
-                for (int product = 0; product < 3; ++product)
+                for (int product = 0; product < 3; ++product) {  // hi lo, lo hi, hi hi
+                    if (product == 1) {
+                        wait(&M.d_ready, now);
+                        tc_fence_after();
+                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + kNew, tmem + kE + (product == 0) * 32 + k * 8, keys + (product == 1) * kLoQk + k * 128, turned_idesc(128, D),
+                        mma_f16_ts(tmem + kNew, tmem + kE + (product == 1) * 32 + k * 8, keys + (product == 0) * kLoQk + k * 128, turned_idesc(128, D),
                                    product || k);
+                }
                 mma_commit(&M.d_done);
                 mma_commit(&M.qk_empty);
+                if (ENDS) continue;
                 wait(&M.g_full, ph1);
                 wait(&M.y_ready, now);
                 tc_fence_after();
@@ -200,38 +249,44 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
         }
         __syncwarp();
     } else {
-        const int w4 = warp & 3, part = warp >> 2, v = w4 * 32 + lane;
+        const int w4 = warp & 3, quarter = warp >> 2, v = w4 * 32 + lane;
         const unsigned lanes = tmem + ((unsigned)(w4 * 32) << 16);
         const bool in = v < n.dim;
-        const int keys = in ? n.dim - part * kPart : 0;  // how many of the thread's there are, or more
+        const int keys = in ? n.dim - quarter * kPart : 0;  // how many of the thread's there are, or more
         const auto arrive = [&](unsigned long long *b) {
             __syncwarp();
             if (lane == 0) bar_arrive(b);
         };
-        float *state = n.state + ((long long)me.sequence * n.dim + part * kPart) * vw + (long long)h * n.dim + v;
         unsigned long long S[kPart / 2];
-        const auto load_state = [&] {
+        const auto load_state = [&](const float *p, long long next) {
 #pragma unroll
-            for (int i = 0; i < kPart / 2; ++i)
-                S[i] = pack2(2 * i < keys ? state[2 * i * vw] : 0.0f, 2 * i + 1 < keys ? state[(2 * i + 1) * vw] : 0.0f);
+            for (int i = 0; i < kPart / 2; ++i, p += 2 * next) S[i] = pack2(2 * i < keys ? p[0] : 0.0f, 2 * i + 1 < keys ? p[next] : 0.0f);
         };
         const auto store_state = [&] {
+            const long long next = M.to_next;
+            float *p = M.to + quarter * kPart * next + v;
 #pragma unroll
-            for (int i = 0; i < kPart / 2; ++i) {
+            for (int i = 0; i < kPart / 2; ++i, p += 2 * next) {
                 float a, b;
                 unpack2(S[i], a, b);
-                if (2 * i < keys) state[2 * i * vw] = a;
-                if (2 * i + 1 < keys) state[(2 * i + 1) * vw] = b;
+                if (2 * i < keys) p[0] = a;
+                if (2 * i + 1 < keys) p[next] = b;
             }
         };
-        load_state();
+        if (!ENDS || from) {
+            load_state(from + quarter * kPart * from_next + v, from_next);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPart / 2; ++i)
+                S[i] = pack2(transition && quarter * kPart + 2 * i == v ? 1.0f : 0.0f, transition && quarter * kPart + 2 * i + 1 == v ? 1.0f : 0.0f);
+        }
         unsigned live = 0;
         bool owed = false;           // the chunk before has results in TMEM
         float inv_r = 0, inv_y = 0;  // their scales taken back
-        // results of chunk c: its tokens part * 16 ..
+        // results of chunk c: its tokens quarter * 16 ..
         const auto write_y = [&](int c) {
             const DeltaFactors &f = M.row[c & 1].f;
-            const int t0 = begin + c * kChunk + part * 16, left = in ? me.tokens - t0 : 0;
+            const int t0 = begin + c * kChunk + quarter * 16, left = in ? me.tokens - t0 : 0;
             // (uniform row addresses and a lane's offset)
             const char *row = reinterpret_cast<const char *>(A.y + (first + t0) * vw + (long long)h * n.dim);
             const long long next = vw * 4;
@@ -239,12 +294,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 float R[8], Y[8];
-                tmem_read8(lanes + kR + part * 16 + half * 8, R);
-                tmem_read8(lanes + kY + part * 16 + half * 8, Y);
+                tmem_read8(lanes + kR + quarter * 16 + half * 8, R);
+                tmem_read8(lanes + kY + quarter * 16 + half * 8, Y);
 #pragma unroll
                 for (int i = 0; i < 8; i += 4) {
-                    const float4 q = *reinterpret_cast<const float4 *>(f.q + part * 16 + half * 8 + i);
-                    const float4 a = *reinterpret_cast<const float4 *>(f.attn + part * 16 + half * 8 + i);
+                    const float4 q = *reinterpret_cast<const float4 *>(f.q + quarter * 16 + half * 8 + i);
+                    const float4 a = *reinterpret_cast<const float4 *>(f.attn + quarter * 16 + half * 8 + i);
                     R[i] = fmaf(R[i] * inv_r, q.x, Y[i] * inv_y * a.x), R[i + 1] = fmaf(R[i + 1] * inv_r, q.y, Y[i + 1] * inv_y * a.y);
                     R[i + 2] = fmaf(R[i + 2] * inv_r, q.z, Y[i + 2] * inv_y * a.z), R[i + 3] = fmaf(R[i + 3] * inv_r, q.w, Y[i + 3] * inv_y * a.w);
                 }
@@ -273,8 +328,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 }
                 const int t0 = begin + c * kChunk;
                 store_state();
-                walk_chunk(n, A, M, state, first + t0, min(kChunk, me.tokens - t0), h, part, v);
-                load_state();
+                walk_chunk<D, ENDS>(n, A, M, first + t0, min(kChunk, me.tokens - t0), h, quarter, v, !transition);
+                load_state(M.to + quarter * kPart * M.to_next + v, M.to_next);
                 arrive(&M.row_empty[st]);
                 continue;
             }
@@ -284,17 +339,22 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < kPart / 2; ++i) most = larger2(most, S[i]);
-            M.s_max[part][v] = most;
+            M.s_max[quarter][v] = most;
             lane_sync(w4);
             const int es = exponent_of(larger(larger(M.s_max[0][v], M.s_max[1][v], M.s_max[2][v]), M.s_max[3][v], 0.0f));
             const float inv_s = unscale_of(es);
+            const unsigned long long by_s = both(scale_of(es));
+            unsigned hi[kPart / 2], lo[8];
+#pragma unroll
+            for (int i = 0; i < kPart / 2; ++i) hi[i] = split_hi(S[i], by_s);
+            tmem_write(lanes + kS + quarter * (kPart / 2), hi);
+            tmem_written();
+            arrive(&M.s_hi);
 #pragma unroll
             for (int i = 0; i < kPart / 2; i += 8) {
-                unsigned hi[8], lo[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) split2(S[i + e], both(scale_of(es)), hi[e], lo[e]);
-                tmem_write(lanes + kS + part * (kPart / 2) + i, hi);
-                tmem_write(lanes + kSLo + part * (kPart / 2) + i, lo);
+                for (int e = 0; e < 8; ++e) lo[e] = split_lo(S[i + e], by_s, hi[i + e]);
+                tmem_write(lanes + kSLo + quarter * (kPart / 2) + i, lo);
             }
             tmem_written();
             arrive(&M.s_ready);
@@ -305,49 +365,59 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 tc_fence_before();
                 arrive(&M.row_empty[st ^ 1]);
             }
-            arrive(&M.r_free);
+            if (!ENDS) arrive(&M.r_free);
             inv_r = inv_s;
             // differences, and as the decays to the chunk's end leave them
-            const float *u = M.row[st].u + part * 16 * D + (v < D ? v : 0);
+            const float *u = M.row[st].u + quarter * 16 * D + (v < D ? v : 0);
             const float by = v < D ? -inv_s : 0.0f;
             float d[16];
+            unsigned long long x[8];  // U, before Z is there
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = ENDS && transition ? 0 : pack2(u[2 * i * D], u[2 * i * D + D]);
             wait.warp(&M.z_done, now, lane);
             tc_fence_after();
-            tmem_read(lanes + kZ + part * 16, d);
-            unsigned long long x[8];
+            tmem_read(lanes + kZ + quarter * 16, d);
             float most_d = 0.0f, most_e = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-                const ulonglong2 z = *reinterpret_cast<const ulonglong2 *>(f.z + part * 16 + i), k = *reinterpret_cast<const ulonglong2 *>(f.k + part * 16 + i);
-                x[i / 2] = fma2(mul2_rn(pack2(d[i], d[i + 1]), both(by)), z.x, pack2(u[i * D], u[i * D + D]));
-                x[i / 2 + 1] = fma2(mul2_rn(pack2(d[i + 2], d[i + 3]), both(by)), z.y, pack2(u[i * D + 2 * D], u[i * D + 3 * D]));
+                const ulonglong2 z = *reinterpret_cast<const ulonglong2 *>(f.z + quarter * 16 + i), k = *reinterpret_cast<const ulonglong2 *>(f.k + quarter * 16 + i);
+                x[i / 2] = fma2(mul2_rn(pack2(d[i], d[i + 1]), both(by)), z.x, x[i / 2]);
+                x[i / 2 + 1] = fma2(mul2_rn(pack2(d[i + 2], d[i + 3]), both(by)), z.y, x[i / 2 + 1]);
                 most_d = larger2(larger2(most_d, x[i / 2]), x[i / 2 + 1]);
                 most_e = larger2(larger2(most_e, mul2_rn(x[i / 2], k.x)), mul2_rn(x[i / 2 + 1], k.y));
             }
-            M.d_max[part][v] = float2{most_d, most_e};
+            M.d_max[quarter][v] = float2{most_d, most_e};
             tc_fence_before();
             lane_sync(w4);  // Z's lanes have been read, too
             tc_fence_after();
             const float2 m0 = M.d_max[0][v], m1 = M.d_max[1][v], m2 = M.d_max[2][v], m3 = M.d_max[3][v];
             const int ee = exponent_of(larger(larger(m0.y, m1.y, m2.y), m3.y, 0.0f)), ed = exponent_of(larger(larger(m0.x, m1.x, m2.x), m3.x, 0.0f));
-            unsigned hi[8], lo[8];
+            const unsigned long long by_e = both(scale_of(ee));
+            unsigned long long e[8];
+            unsigned h[8];
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(f.k + part * 16 + 2 * i);
-                split2(mul2_rn(x[i], k.x), both(scale_of(ee)), hi[i], lo[i]);
-                split2(mul2_rn(x[i + 1], k.y), both(scale_of(ee)), hi[i + 1], lo[i + 1]);
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(f.k + quarter * 16 + 2 * i);
+                e[i] = mul2_rn(x[i], k.x), e[i + 1] = mul2_rn(x[i + 1], k.y);
+                h[i] = split_hi(e[i], by_e), h[i + 1] = split_hi(e[i + 1], by_e);
             }
-            tmem_write(lanes + kE + part * 8, hi);
-            tmem_write(lanes + kE + 32 + part * 8, lo);
+            tmem_write(lanes + kE + quarter * 8, h);
+            tmem_written();
+            arrive(&M.d_hi);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) lo[i] = split_lo(e[i], by_e, h[i]);
+            tmem_write(lanes + kE + 32 + quarter * 8, lo);
             tmem_written();
             arrive(&M.d_ready);
+            if (!ENDS) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) split2(x[i], both(scale_of(ed)), hi[i], lo[i]);
-            tmem_write(lanes + kZ + part * 8, hi);
-            tmem_write(lanes + kZ + 32 + part * 8, lo);
-            tmem_written();
-            arrive(&M.y_ready);
-            inv_y = unscale_of(ed);
+                for (int i = 0; i < 8; ++i) split2(x[i], both(scale_of(ed)), h[i], lo[i]);
+                tmem_write(lanes + kZ + quarter * 8, h);
+                tmem_write(lanes + kZ + 32 + quarter * 8, lo);
+                tmem_written();
+                arrive(&M.y_ready);
+                inv_y = unscale_of(ed);
+            }
             // the new state
             const float inv_e = unscale_of(ee), end = f.end;
 #pragma unroll
@@ -356,12 +426,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             tc_fence_after();
 #pragma unroll
             for (int i = 0; i < kPart; i += 16) {
-                tmem_read(lanes + kNew + part * kPart + i, d);
+                tmem_read(lanes + kNew + quarter * kPart + i, d);
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) S[(i + e) / 2] = fma2(pack2(d[e], d[e + 1]), both(inv_e), S[(i + e) / 2]);
             }
             tc_fence_before();
-            owed = true;
+            if (ENDS) arrive(&M.row_empty[st]);
+            owed = !ENDS;
         }
         if (owed) {
             wait.warp(&M.y_done, (live - 1) & 1, lane);
@@ -377,25 +448,28 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
     if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <int D>
+template <int D, bool ENDS>
 cudaError_t launch_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
     constexpr int kDevices = 64;
     static std::atomic<bool> done[kDevices];
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess && (device >= kDevices || !done[device].load(std::memory_order_relaxed))) {
-        e = cudaFuncSetAttribute(k_delta_chain<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChainSmem<D>));
+        e = cudaFuncSetAttribute(k_delta_chain<D, ENDS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChainSmem<D>));
         if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
     }
     if (e != cudaSuccess) return e;
-    return kv8_launch(k_delta_chain<D>, dim3((unsigned)(slab.runs * slab.heads * slab.ratio)), dim3(kChainThreads), sizeof(ChainSmem<D>), 1, s, n, a, r,
-                      slab);
+    const int blocks = slab.runs * slab.heads * slab.ratio * (ENDS ? 2 * (slab.parts - 1) : slab.parts);
+    return kv8_launch(k_delta_chain<D, ENDS>, dim3((unsigned)blocks), dim3(kChainThreads), sizeof(ChainSmem<D>), 1, s, n, a, r, slab);
 }
 
 }  // namespace
 
 cudaError_t delta_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
-    return n.dim <= 64 ? launch_chain<64>(n, a, r, slab, s) : launch_chain<128>(n, a, r, slab, s);
+    return n.dim <= 64 ? launch_chain<64, false>(n, a, r, slab, s) : launch_chain<128, false>(n, a, r, slab, s);
+}
+cudaError_t delta_ends(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
+    return n.dim <= 64 ? launch_chain<64, true>(n, a, r, slab, s) : launch_chain<128, true>(n, a, r, slab, s);
 }
 
 }  // namespace strata

@@ -6,6 +6,9 @@
 // The first line needs no state: all chunks of all heads at once. The second goes from chunk to chunk. Products of decays are
 // formed by multiplication alone, so that zero decays need no care.
 //
+// Runs of few states are taken in parts at once: a state goes into a part and out of it as  S' = F S + N, with F and N where the identity
+// without values and zeros end; then the parts follow from the states before them.                  delta_chain.cu, delta_join.cu
+//
 // Products. Each F32 factor is two FP16 halves, times a power of two that brings the largest value of its row (or of its
 // TMEM lane, or tile) to 2^13: 22 bits for whatever is within 2^-17 of that, and 2^-38 of it below. lo hi + hi lo + hi hi are three
 // FP16 products with F32 sums; lo lo would be 2^-22 of the result. The large product comes last: sums in TMEM are cut, not
@@ -39,6 +42,12 @@ struct DeltaSlab {  // runs, key heads and chunks [first, first + n) of a call
     int ahead;  // the first kernel runs while the slab before is on its way through the second
     unsigned char *slots;
     long long slot_bytes;
+    // Runs in parts of part_chunks chunks that are on their way at once (parts > 1): of each run and head, for each part p but the
+    // last, its transition and its end without it ([dim D][dim D] each), then the end with it; in the first one's transition's place
+    // the state before it. And whether a run and head has to be taken whole.
+    int parts, part_chunks;
+    float *states;
+    int *whole;
 };
 template <int D>
 struct DeltaSlot {
@@ -51,6 +60,8 @@ struct DeltaSlot {
 cudaError_t delta_step(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s);
 cudaError_t delta_prepare(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, bool vec, cudaStream_t s);
 cudaError_t delta_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s);
+cudaError_t delta_ends(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s);  // transitions and ends of parts
+cudaError_t delta_join(const DeltaNet &n, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s);                     // states before them
 
 #ifdef __CUDACC__
 namespace delta {
@@ -133,6 +144,20 @@ __device__ __forceinline__ void split2(unsigned long long x, unsigned long long 
     const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
     hi = *reinterpret_cast<const unsigned *>(&h);
     lo = *reinterpret_cast<const unsigned *>(&l);
+}
+// The same one after the other, where products with hi begin before lo is there.
+__device__ __forceinline__ unsigned split_hi(unsigned long long x, unsigned long long by) {
+    float a, b;
+    unpack2(mul2_rn(x, by), a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+__device__ __forceinline__ unsigned split_lo(unsigned long long x, unsigned long long by, unsigned hi) {
+    float a, b;
+    unpack2(mul2_rn(x, by), a, b);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    return *reinterpret_cast<const unsigned *>(&l);
 }
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[N], float scale, unsigned (&hi)[N / 2], unsigned (&lo)[N / 2]) {

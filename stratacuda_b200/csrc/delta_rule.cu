@@ -17,6 +17,23 @@ int short_run(const DeltaNet &n, const MixRuns &r) {
     return (long long)r.segments * n.value_heads <= kSms / 2 ? 44 : 28;
 }
 
+// States up to which runs are taken in parts: with N of them, (148 / N + 3) / 2 parts fill the multiprocessors (of a part but the last
+// its end and, but for the first, its transition; then all parts once more, from the states that these give). One prompt of 8191 tokens over
+// 2 heads of 128 487 -> 138 us, over 16 560 -> 355 us, over 24 588 -> 530 us; of 2048 over 8 of 64 114 -> 65 us, over 24 of 128
+// 171 -> 154 us. Over 32 three parts are left: 2048 tokens 174 -> 172 us, 8191 611 -> 678 us.
+constexpr int kSplitStates = 24;
+
+// Parts of a run's chunks, by tenths of microseconds: 3.7 us a chunk as one, 7.1 us a part's chunk twice, 1.5 us to join a part and 15 us
+// of two more kernels. (1000 tokens over 4 heads of 128: 86 us as one, 83 in 3 parts, 72 in 4, 70 in 8; 640 over 8: 64 and 62 us.)
+int parts_of(int chunks, int most) {
+    int best = 1, least = chunks * 37;
+    for (int k = 3; k <= std::min(most, chunks); ++k) {
+        const int time = (chunks + k - 1) / k * 71 + k * 15 + 150;
+        if (time < least) best = k, least = time;
+    }
+    return best;
+}
+
 }  // namespace
 
 cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, cudaStream_t s) {
@@ -27,14 +44,38 @@ cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, 
     const bool vec = n.dim % 4 == 0 && a.q_stride % 4 == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 && mix_aligned16(a.q) &&
                      mix_aligned16(a.k) && mix_aligned16(a.v);
     const int all = (r.count + kChunk - 1) / kChunk;
-    DeltaSlab slab{0, 0, 0, 0, 0, 0, ratio, 0, static_cast<unsigned char *>(n.workspace), bytes};
+    DeltaSlab slab{0, 0, 0, 0, 0, 0, ratio, 0, static_cast<unsigned char *>(n.workspace), bytes, 1, 0, nullptr, nullptr};
     const auto one = [&] {
         cudaError_t e = delta_prepare(n, a, r, slab, vec, s);
+        if (slab.parts > 1) {
+            if (e == cudaSuccess) e = delta_ends(n, a, r, slab, s);
+            if (e == cudaSuccess) e = delta_join(n, r, slab, s);
+        }
         return e == cudaSuccess ? delta_chain(n, a, r, slab, s) : e;
     };
+    const int D = n.dim <= 64 ? 64 : 128;
+    if ((long long)r.segments * n.value_heads <= kSplitStates) {
+        const int states = r.segments * n.value_heads, per = r.segments * n.key_heads, most = (kSms / states + 3) / 2;
+        const long long state = 2ll * D * D * sizeof(float) * states, behind = STRATA_DELTA_WORKSPACE_BYTES - state * (most - 1) - 1024;
+        const int chunks = std::min<long long>(all, behind / (bytes * per));
+        if (chunks > 0 && parts_of(chunks, most) > 1) {
+            slab.runs = r.segments, slab.heads = n.key_heads;
+            for (; slab.chunk0 < all; slab.chunk0 += slab.chunks) {
+                slab.chunks = std::min(chunks, all - slab.chunk0);
+                const int parts = parts_of(slab.chunks, most);
+                slab.part_chunks = (slab.chunks + parts - 1) / parts;
+                slab.parts = (slab.chunks + slab.part_chunks - 1) / slab.part_chunks;
+                slab.states = reinterpret_cast<float *>(slab.slots + slab.chunks * per * bytes);
+                slab.whole = reinterpret_cast<int *>(slab.states + state / sizeof(float) * (slab.parts - 1));
+                const cudaError_t e = one();
+                if (e != cudaSuccess) return e;
+            }
+            return cudaSuccess;
+        }
+    }
     // Few states leave most multiprocessors idle in the second kernel: there the next slab's first one runs meanwhile, on the
     // workspace's other half. The first slab gives each multiprocessor two blocks, the next ones those that are left. One prompt
-    // of 2048 tokens over 32 heads of 128 194 -> 182 us, of 8191 over 48 937 -> 680 us, two of 1024 over 32 140 -> 132 us; three
+    // of 2048 tokens over 32 heads of 128 185 -> 174 us, of 8191 over 48 900 -> 645 us, two of 1024 over 32 140 -> 132 us; three
     // would take 227 us in place of 189: with more states than half of the multiprocessors one slab after another.
     if ((long long)r.segments * n.value_heads <= kSms / 2) {
         const int chains = r.segments * n.value_heads, per = r.segments * n.key_heads, most = room / 2 / per;  // chunks of a half
