@@ -53,20 +53,22 @@ __device__ __forceinline__ void bulk_out(void *to, const void *from, unsigned by
 __device__ __forceinline__ void bulk_out_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_out_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
-// x of (I + L) x = e_c, L the strictly lower part of 32 rows at l
+// x of (I + L) x = e_c, L the strictly lower part of 32 rows; at l its negative, by columns. Once x_j is known all later rows have
+// their term (the rows' sums one after another took 3200 clocks, a chain of up to 8 products a row).
 __device__ __forceinline__ void substitute(const float *l, int c, float (&x)[32]) {
+    unsigned long long s[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        float s[4] = {i == c ? 1.0f : 0.0f, 0, 0, 0};
+    for (int i = 0; i < 16; ++i) s[i] = pack2(2 * i == c ? 1.0f : 0.0f, 2 * i + 1 == c ? 1.0f : 0.0f);
 #pragma unroll
-        for (int j = 0; j < i; j += 4) {
-            const float4 r = *reinterpret_cast<const float4 *>(l + i * kPitch + j);
-            s[0] = fmaf(-r.x, x[j], s[0]);
-            if (j + 1 < i) s[1] = fmaf(-r.y, x[j + 1], s[1]);
-            if (j + 2 < i) s[2] = fmaf(-r.z, x[j + 2], s[2]);
-            if (j + 3 < i) s[3] = fmaf(-r.w, x[j + 3], s[3]);
+    for (int j = 0; j < 32; ++j) {
+        unpack2(s[j / 2], x[j & ~1], x[j | 1]);
+        const unsigned long long by = both(x[j]);
+#pragma unroll
+        for (int i = (j + 1) / 4; i < 8 && j < 31; ++i) {  // (the pair of x_j itself: its term is zero)
+            const ulonglong2 r = *reinterpret_cast<const ulonglong2 *>(l + j * kPitch + 4 * i);
+            if (4 * i + 1 > j) s[2 * i] = fma2(r.x, by, s[2 * i]);
+            s[2 * i + 1] = fma2(r.y, by, s[2 * i + 1]);
         }
-        x[i] = (s[0] + s[1]) + (s[2] + s[3]);
     }
 }
 // Rows r, r + 1 and four columns from c of X Y, 32 by 32, rows of X at x, Y at y; `terms` (a multiple of 4) of X's rows count.
@@ -290,7 +292,15 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
             if (key) {
                 const float f = M.inv[gt] * M.beta[i];
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(a_row + j) = float4{x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 a{x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
+                    if (upper && !half) {
+                        *reinterpret_cast<float4 *>(a_row + j) = a;
+                    } else {  // what is substituted: by columns, its negative
+                        float *to = &M.a[(32 * half + j) * kPitch + i];
+                        to[0] = -a.x, to[kPitch] = -a.y, to[2 * kPitch] = -a.z, to[3 * kPitch] = -a.w;
+                    }
+                }
             } else {
                 most = largest(0.0f, x);
             }
