@@ -12,6 +12,8 @@
 namespace strata {
 namespace {
 
+using delta::both;
+using delta::fma2;
 using delta::larger;
 
 constexpr float kLargest = 2.0f;
@@ -49,47 +51,56 @@ __global__ void __launch_bounds__(D *COLS / EACH) k_delta_join(const __grid_cons
     asm volatile("cp.async.commit_group;" ::: "memory");
     // the state before the first part moves here: the last part's block writes the real one
     const float *real = n.state + ((long long)me.sequence * n.dim + row) * n.value_heads * n.dim + (long long)h * n.dim + col;
-    float4 end[kVec];
-#pragma unroll
-    for (int c = 0; c < EACH; ++c) reinterpret_cast<float *>(end)[c] = row < n.dim && col + c < n.dim ? real[c] : 0.0f;
+    ulonglong2 end[kVec], next[kVec];  // four columns each
 #pragma unroll
     for (int c = 0; c < kVec; ++c) {
-        float4 *at = reinterpret_cast<float4 *>(own + row * D + col) + c;
-        *at = end[c];
-        if (last > 0) end[c] = at[D * D / 4];
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = row < n.dim && col + 4 * c + e < n.dim ? real[4 * c + e] : 0.0f;
+        *reinterpret_cast<float4 *>(own + row * D + col + 4 * c) = float4{x[0], x[1], x[2], x[3]};
+    }
+    const auto ends = [&](int p) { return reinterpret_cast<ulonglong2 *>(own + (2 * p + 1) * (D * D) + row * D + col); };
+#pragma unroll
+    for (int c = 0; c < kVec; ++c) {
+        if (last > 0) end[c] = ends(0)[c];
+        if (last > 1) next[c] = ends(1)[c];
     }
     float most = 0.0f;
     for (int p = 1; p < last; ++p) {
-        float4 *at = reinterpret_cast<float4 *>(own + (2 * p + 1) * (D * D) + row * D + col), sum[kVec];
+        ulonglong2 sum[kVec];
 #pragma unroll
         for (int c = 0; c < kVec; ++c) {
             // rows past the head's channels hold nothing
-            reinterpret_cast<float4 *>(&M.s[p & 1][row][group * EACH])[c] = row < n.dim ? end[c] : float4{0, 0, 0, 0};
-            end[c] = at[c];
-            sum[c] = float4{0, 0, 0, 0};
+            reinterpret_cast<ulonglong2 *>(&M.s[p & 1][row][group * EACH])[c] = row < n.dim ? end[c] : ulonglong2{0, 0};
+            sum[c] = next[c];
+            if (p + 1 < last) next[c] = ends(p + 1)[c];
         }
         if (p + 1 < last) fetch(p + 1);
         asm volatile("cp.async.commit_group;" ::: "memory");
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncthreads();
         const float *f = M.f[p & 1][row];
-#pragma unroll 4
-        for (int j = 0; j < n.dim; j += 4) {
-            const float4 a = *reinterpret_cast<const float4 *>(f + j);
-            const float w[4] = {a.x, j + 1 < n.dim ? a.y : 0.0f, j + 2 < n.dim ? a.z : 0.0f, j + 3 < n.dim ? a.w : 0.0f};
+        const auto four = [&](int j, float4 a) {
+            const float w[4] = {a.x, a.y, a.z, a.w};
             most = larger(larger(most, w[0], w[1]), w[2], w[3]);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int c = 0; c < kVec; ++c) {
-                    const float4 s = reinterpret_cast<const float4 *>(&M.s[p & 1][j + e][group * EACH])[c];
-                    sum[c].x = fmaf(w[e], s.x, sum[c].x), sum[c].y = fmaf(w[e], s.y, sum[c].y);
-                    sum[c].z = fmaf(w[e], s.z, sum[c].z), sum[c].w = fmaf(w[e], s.w, sum[c].w);
+                    const ulonglong2 s = reinterpret_cast<const ulonglong2 *>(&M.s[p & 1][j + e][group * EACH])[c];
+                    sum[c].x = fma2(both(w[e]), s.x, sum[c].x), sum[c].y = fma2(both(w[e]), s.y, sum[c].y);
                 }
+        };
+        const int whole = n.dim & ~3;
+#pragma unroll 4
+        for (int j = 0; j < whole; j += 4) four(j, *reinterpret_cast<const float4 *>(f + j));
+        if (whole < n.dim) {
+            const float4 a = *reinterpret_cast<const float4 *>(f + whole);
+            four(whole, float4{a.x, whole + 1 < n.dim ? a.y : 0.0f, whole + 2 < n.dim ? a.z : 0.0f, 0.0f});
         }
         if (row >= n.dim) most = 0.0f;
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) at[c] = end[c] = float4{end[c].x + sum[c].x, end[c].y + sum[c].y, end[c].z + sum[c].z, end[c].w + sum[c].w};
+        for (int c = 0; c < kVec; ++c) ends(p)[c] = end[c] = sum[c];
         __syncthreads();  // the buffers' next turn
     }
     const int large = __syncthreads_or(!(most <= kLargest));
