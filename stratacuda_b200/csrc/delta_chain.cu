@@ -8,8 +8,10 @@
 //   Y^T = D^T G^T;  y = P R + Y          128 by 64 tokens
 // One warp fetches, one issues; results of a chunk are written while the next one's first product runs.
 //
-// Bound by the way round: a product, its differences, the next product and the new state cannot overlap one another. The four
-// products take 2700 clocks of the tensor cores a chunk of 128 channels, half of them on that way.
+// Bound by the way round: a product, its differences, the next product and the new state cannot overlap one another. A chunk of 128
+// channels takes 6900 clocks (3.5 us): the four products 2700 of the tensor cores, half of them on that way, the rest splits, scales and
+// hand-overs. Products begin with the upper half of their 128-row operand while the lower one is made (2048 tokens over 32 heads
+// 183 -> 175 us).
 #include "delta_chunk.cuh"
 
 #include <atomic>
