@@ -794,7 +794,7 @@ int strata_delta_rule(strata_ctx *ctx, const strata_delta_net *net, strata_buf q
                                   {"decay", decay, rows * n.value_heads, (void **)&a.decay, false},
                                   {"beta", beta, rows * n.value_heads, (void **)&a.beta, false},
                                   {"y", y, rows * vd, (void **)&a.y, false},
-                                  {"state", net->state, n.sequences * n.dim * vd, (void **)&n.state, false},
+                                  {"state", net->state, (long long)n.sequences * n.dim * vd, (void **)&n.state, false},
                                   {"workspace", net->workspace, STRATA_DELTA_WORKSPACE_BYTES / 4, &n.workspace, false}}))
         return e;
     cudaError_t e = delta_rule(n, a, r, ctx->stream);

@@ -507,3 +507,25 @@ def test_handles_run_a_layer(torch, count):
         b.idle()
     b.idle()
     net.free()
+
+
+def test_handles_refuse_buffers_that_are_too_short(torch):
+    """Sizes are counted in 64 bits: numbers of sequences whose states would be 2^31 rows or more do not wrap round."""
+    from stratacuda_b200.backend import CudaBackend, StrataError
+    from stratacuda_b200.mixers import DeltaNet
+    b = CudaBackend(0)
+    kh, vh, dim = 1, 1, 256
+    f, seq, work = b.alloc(8 * dim), b.alloc(np.zeros(1, np.int32), "i32"), b.alloc(L.DELTA_WORKSPACE_BYTES // 4, "u32", zero=False)
+    state = b.alloc(dim * dim)
+    for sequences in (2, 1 << 23, 1 << 24, (1 << 31) - 1):
+        net = DeltaNet(b, kh, vh, dim, sequences, state=state, history=f, weight=f, workspace=work)
+        with pytest.raises(StrataError, match="state needs"):
+            net.rule(f, f, f, f, f, f, seq)
+        with pytest.raises(StrataError, match="history needs"):
+            net.inputs(f, f, f, f, seq)
+    net = DeltaNet(b, kh, vh, dim, 1, state=state, history=f, weight=f, workspace=work)
+    for short in ("q", "v", "y"):
+        with pytest.raises(StrataError, match=short + " needs"):
+            net.rule(**{**dict(q=f, k=f, v=f, decay=f, beta=f, y=f), short: seq}, sequence=seq)
+    with pytest.raises(StrataError, match="workspace needs"):
+        DeltaNet(b, kh, vh, dim, 1, state=state, history=f, weight=f, workspace=f).rule(f, f, f, f, f, f, seq)
