@@ -121,6 +121,22 @@ def test_refuses_tensors_that_are_not_as_they_should_be():
     assert refuse(StrataError, "CUDA device", lambda: net(state=torch.zeros(3 * 64 * 4 * 64))) == L.ERR_LAYOUT
 
 
+def test_refuses_the_default_stream_of_another_device(monkeypatch):
+    torch = pytest.importorskip("torch")
+
+    class Elsewhere:  # what is looked at of a tensor on device 1
+        def __init__(self, dtype=torch.float32):
+            self.dtype = dtype
+        get_device, numel, is_contiguous, data_ptr = lambda _: 1, lambda _: 1 << 40, lambda _: True, lambda _: A
+        element_size = lambda _: 4  # noqa: E731
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    x = Elsewhere()
+    for call, make in ((inputs, lambda: net(state=x, history=x, weight=x)), (rule, lambda: net(state=x, history=x, weight=x)),
+                       (apply, lambda: rope(q_weight=x, k_weight=x, cos=x, sin=x))):
+        assert refuse(StrataError, "default stream", lambda: call(make())) == L.ERR_LAYOUT
+
+
 def test_other_backends_are_refused():
     class Other:
         kind = "checker"
