@@ -514,10 +514,10 @@ def test_handles_refuse_buffers_that_are_too_short(torch):
     from stratacuda_b200.backend import CudaBackend, StrataError
     from stratacuda_b200.mixers import DeltaNet
     b = CudaBackend(0)
-    kh, vh, dim = 1, 1, 256
-    f, seq, work = b.alloc(8 * dim), b.alloc(np.zeros(1, np.int32), "i32"), b.alloc(L.DELTA_WORKSPACE_BYTES // 4, "u32", zero=False)
+    kh, vh, dim = 1, 1, 128
+    f, seq, work = b.alloc(16 * dim), b.alloc(np.zeros(1, np.int32), "i32"), b.alloc(L.DELTA_WORKSPACE_BYTES // 4, "u32", zero=False)
     state = b.alloc(dim * dim)
-    for sequences in (2, 1 << 23, 1 << 24, (1 << 31) - 1):
+    for sequences in (2, 1 << 24, 1 << 25, (1 << 31) - 1):
         net = DeltaNet(b, kh, vh, dim, sequences, state=state, history=f, weight=f, workspace=work)
         with pytest.raises(StrataError, match="state needs"):
             net.rule(f, f, f, f, f, f, seq)
