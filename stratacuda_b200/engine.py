@@ -33,7 +33,8 @@ src/prefill.js:52-78 collapsed into one dispatch, with no host read of the route
 With ``mixers=1`` the token mixers' inner parts run as the run entries of stratacuda_b200.mixers: the delta-rule layer's
 convolution, slices and norms as one dispatch and its rule as another (chunked on the tensor cores for prompt chunks), the norms and
 rotation of queries and keys as one. Values then agree with the reference's entries to F32 rounding instead of bit for bit, and
-prompt chunks may have up to 1024 tokens.
+prompt chunks may have up to 1024 tokens; chunks of more than 64 take the fast mixture of experts (``moe_mode=1``) through its FP16
+form, 2e-3 a layer.
 
 The engine takes any backend with the reference protocol (src/backend.js:58-206): ``alloc``,
 ``write``, ``read``, ``copy``, ``zero``, ``free``, ``run``, ``idle``. On a B200 that is
