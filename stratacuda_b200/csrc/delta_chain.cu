@@ -39,7 +39,7 @@ struct __align__(1024) ChainSmem {
     float *to;  // where the state goes and is walked, rows to_next floats apart
     long long to_next;
     unsigned tmem;
-    int abort_flag;
+    int abort_flag, picked;
 };
 
 __device__ __forceinline__ void lane_sync(int w4) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w4) : "memory"); }  // of the same lanes
@@ -76,8 +76,9 @@ __device__ __noinline__ void walk_chunk(const DeltaNet &n, const DeltaRule &A, C
     }
 }
 
-// ENDS: nothing but where parts of runs end, from zeros and (their transition) without values from the identity.
-template <int D, bool ENDS>
+// ENDS: nothing but where parts of runs end, from zeros and (their transition) without values from the identity. SORTED: a kernel of its own,
+// since a run's number from memory takes registers that the other form has not to spare (2% of its time).
+template <int D, bool ENDS, bool SORTED>
 __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A,
                                                                   const __grid_constant__ MixRuns r, const __grid_constant__ DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
@@ -91,7 +92,21 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
     int part = 0;
     if (ENDS) transition = block & 1, block >>= 1;
     if (slab.parts > 1) part = block % (slab.parts - ENDS), block /= slab.parts - ENDS;
-    const int chain = block, m = block % slab.ratio, head_l = block / slab.ratio % slab.heads, run_l = block / slab.ratio / slab.heads;
+    const int chain = block, m = block % slab.ratio, head_l = block / slab.ratio % slab.heads;
+    int run_l = block / slab.ratio / slab.heads;
+    if (SORTED) {  // the run with the run_l-th most tokens
+        int *tokens = reinterpret_cast<int *>(M.s_max);
+        const int i = slab.run0 + tid;
+        if (tid < slab.runs) tokens[tid] = r.sequence[i] < 0 ? 0 : r.lengths[i];
+        __syncthreads();
+        if (tid < slab.runs) {
+            int rank = 0;
+            for (int j = 0; j < slab.runs; ++j) rank += tokens[j] > tokens[tid] || (tokens[j] == tokens[tid] && j < tid);
+            if (rank == run_l) M.picked = tid;
+        }
+        __syncthreads();
+        run_l = M.picked;
+    }
     const int h = slab.head0 + head_l + m * n.key_heads, run = slab.run0 + run_l;
     const MixRun me = mix_run_alone(r, n.sequences, run, n.err);
     const long long first = (long long)run * r.count, vw = (long long)n.value_heads * n.dim;
@@ -450,24 +465,25 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
     if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <int D, bool ENDS>
+template <int D, bool ENDS, bool SORTED = false>
 cudaError_t launch_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
     constexpr int kDevices = 64;
     static std::atomic<bool> done[kDevices];
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess && (device >= kDevices || !done[device].load(std::memory_order_relaxed))) {
-        e = cudaFuncSetAttribute(k_delta_chain<D, ENDS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChainSmem<D>));
+        e = cudaFuncSetAttribute(k_delta_chain<D, ENDS, SORTED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChainSmem<D>));
         if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
     }
     if (e != cudaSuccess) return e;
     const int blocks = slab.runs * slab.heads * slab.ratio * (ENDS ? 2 * (slab.parts - 1) : slab.parts);
-    return kv8_launch(k_delta_chain<D, ENDS>, dim3((unsigned)blocks), dim3(kChainThreads), sizeof(ChainSmem<D>), 1, s, n, a, r, slab);
+    return kv8_launch(k_delta_chain<D, ENDS, SORTED>, dim3((unsigned)blocks), dim3(kChainThreads), sizeof(ChainSmem<D>), 1, s, n, a, r, slab);
 }
 
 }  // namespace
 
 cudaError_t delta_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
+    if (slab.sorted) return n.dim <= 64 ? launch_chain<64, false, true>(n, a, r, slab, s) : launch_chain<128, false, true>(n, a, r, slab, s);
     return n.dim <= 64 ? launch_chain<64, false>(n, a, r, slab, s) : launch_chain<128, false>(n, a, r, slab, s);
 }
 cudaError_t delta_ends(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {

@@ -25,6 +25,7 @@
 namespace strata {
 
 constexpr int kChunk = 64;
+constexpr int kSortedRuns = 128;        // at most, where runs are taken by their lengths
 constexpr float kDeltaLarge = 0x1p60f;  // past this, or not finite: the chunk is walked token by token
 
 struct DeltaFactors {  // of a chunk's rows, for one value head
@@ -38,7 +39,8 @@ struct DeltaFactors {  // of a chunk's rows, for one value head
 };
 struct DeltaSlab {  // runs, key heads and chunks [first, first + n) of a call
     int run0, runs, head0, heads, chunk0, chunks;
-    int ratio;  // value heads of a key head
+    int ratio;   // value heads of a key head
+    int sorted;  // the second kernel takes long runs first
     int ahead;  // the first kernel runs while the slab before is on its way through the second
     unsigned char *slots;
     long long slot_bytes;

@@ -349,6 +349,20 @@ def test_rule_of_few_long_runs_repeats_and_replays(torch):
         assert all(np.array_equal(y.cpu().numpy(), f) for y, f in zip(ys, first)) and np.array_equal(net.state(), after)
 
 
+@pytest.mark.parametrize("dim,count", [(64, 200), (128, 131)])
+def test_rule_takes_long_runs_first(torch, dim, count):
+    """More states than multiprocessors, runs of all lengths and of equal ones, idle ones, numbers outside and one sequence twice."""
+    sequence = [(7 * i + 3) % 24 for i in range(24)]
+    lengths = [(37 * i) % (count + 1) for i in range(24)]
+    lengths[5] = lengths[6] = lengths[20] = count
+    lengths[9] = 0
+    sequence[11] = -1
+    check_rule(torch, 4, 8, dim, 24, count, sequence, lengths, 24)
+    sequence[3] = sequence[1]
+    sequence[17], lengths[2], lengths[4] = 99, -5, count + 7
+    check_rule(torch, 4, 8, dim, 24, count, sequence, lengths, 24, status=1)
+
+
 # ---------------------------------------------------------------- inputs
 
 @pytest.mark.parametrize("count", [1, 2, 3, 4, 15, 16, 17, 100])
