@@ -36,8 +36,11 @@ struct __align__(1024) ChainSmem {
     float2 d_max[4][128];  // also the sums of chunks that are walked
     unsigned long long w_full[2], w_empty[2], row_full[2], row_empty[2], qk_full, qk_empty, g_full, g_empty;
     unsigned long long s_hi, s_ready, r_free, d_hi, d_ready, y_ready, z_done, d_done, y_done;
-    float *to;  // where the state goes and is walked, rows to_next floats apart
-    long long to_next;
+    // What a chunk needs seldom: its loop has no registers to spare. Where the state goes and is walked, rows to_next floats apart;
+    // the part's first row, its tokens, the value head.
+    float *to;
+    long long to_next, row0;
+    int tokens, head;
     unsigned tmem;
     int abort_flag, picked;
 };
@@ -82,6 +85,7 @@ template <int D, bool ENDS, bool SORTED>
 __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A,
                                                                   const __grid_constant__ MixRuns r, const __grid_constant__ DeltaSlab slab) {
     using Slot = DeltaSlot<D>;
+    constexpr bool kEarlyU = D == 64 || ENDS;
     constexpr int kPart = D / 4;  // keys of a thread; and 16 tokens
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     ChainSmem<D> &M = *reinterpret_cast<ChainSmem<D> *>(smem_raw);
@@ -150,7 +154,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
         bar_init(&M.z_done, 1), bar_init(&M.d_done, 1), bar_init(&M.y_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         M.abort_flag = 0;
-        M.to = to, M.to_next = to_next;  // (there: seldom used, and the chunks' loop has no registers to spare)
+        M.to = to, M.to_next = to_next;
+        M.row0 = first + begin, M.tokens = me.tokens - begin, M.head = h;
     }
     if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&M.tmem)) : "memory");
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
         // results of chunk c: its tokens quarter * 16 ..
         const auto write_y = [&](int c) {
             const DeltaFactors &f = M.row[c & 1].f;
-            const int t0 = begin + c * kChunk + quarter * 16, left = in ? me.tokens - t0 : 0;
+            const int t0 = begin + c * kChunk + quarter * 16, left = in ? M.tokens - c * kChunk - quarter * 16 : 0;
             // (uniform row addresses and a lane's offset)
             const char *row = reinterpret_cast<const char *>(A.y + (first + t0) * vw + (long long)h * n.dim);
             const long long next = vw * 4;
@@ -315,10 +320,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 tmem_read8(lanes + kY + quarter * 16 + half * 8, Y);
 #pragma unroll
                 for (int i = 0; i < 8; i += 4) {
-                    const float4 q = *reinterpret_cast<const float4 *>(f.q + quarter * 16 + half * 8 + i);
-                    const float4 a = *reinterpret_cast<const float4 *>(f.attn + quarter * 16 + half * 8 + i);
-                    R[i] = fmaf(R[i] * inv_r, q.x, Y[i] * inv_y * a.x), R[i + 1] = fmaf(R[i + 1] * inv_r, q.y, Y[i + 1] * inv_y * a.y);
-                    R[i + 2] = fmaf(R[i + 2] * inv_r, q.z, Y[i + 2] * inv_y * a.z), R[i + 3] = fmaf(R[i + 3] * inv_r, q.w, Y[i + 3] * inv_y * a.w);
+                    const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(f.q + quarter * 16 + half * 8 + i);
+                    const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(f.attn + quarter * 16 + half * 8 + i);
+                    const auto sum = [&](int j, unsigned long long q, unsigned long long a) {
+                        const unsigned long long r = mul2_rn(pack2(R[j], R[j + 1]), both(inv_r)), y = mul2_rn(pack2(Y[j], Y[j + 1]), both(inv_y));
+                        unpack2(fma2(r, q, mul2_rn(y, a)), R[j], R[j + 1]);
+                    };
+                    sum(i, q.x, a.x), sum(i + 2, q.y, a.y);
                 }
                 if (left >= 16) {
 #pragma unroll
@@ -343,9 +351,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                     arrive(&M.row_empty[st ^ 1]);
                     owed = false;
                 }
-                const int t0 = begin + c * kChunk;
                 store_state();
-                walk_chunk<D, ENDS>(n, A, M, first + t0, min(kChunk, me.tokens - t0), h, quarter, v, !transition);
+                walk_chunk<D, ENDS>(n, A, M, M.row0 + c * kChunk, min(kChunk, M.tokens - c * kChunk), M.head, quarter, v, !transition);
                 load_state(M.to + quarter * kPart * M.to_next + v, M.to_next);
                 arrive(&M.row_empty[st]);
                 continue;
@@ -388,20 +395,26 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             const float *u = M.row[st].u + quarter * 16 * D + (v < D ? v : 0);
             const float by = v < D ? -inv_s : 0.0f;
             float d[16];
-            unsigned long long x[8];  // U, before Z is there
+            unsigned long long x[8];  // U, before Z is there; with 128 channels that takes registers from the rest (2048 tokens 169.6 -> 164.7 us after it)
+            const auto load_u = [&] {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = ENDS && transition ? 0 : pack2(u[2 * i * D], u[2 * i * D + D]);
+                for (int i = 0; i < 8; ++i) x[i] = ENDS && transition ? 0 : pack2(u[2 * i * D], u[2 * i * D + D]);
+            };
+            if (kEarlyU) load_u();
             wait.warp(&M.z_done, now, lane);
+            if (!kEarlyU) load_u();
             tc_fence_after();
             tmem_read(lanes + kZ + quarter * 16, d);
             float most_d = 0.0f, most_e = 0.0f;
+            unsigned long long e[8];
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const ulonglong2 z = *reinterpret_cast<const ulonglong2 *>(f.z + quarter * 16 + i), k = *reinterpret_cast<const ulonglong2 *>(f.k + quarter * 16 + i);
                 x[i / 2] = fma2(mul2_rn(pack2(d[i], d[i + 1]), both(by)), z.x, x[i / 2]);
                 x[i / 2 + 1] = fma2(mul2_rn(pack2(d[i + 2], d[i + 3]), both(by)), z.y, x[i / 2 + 1]);
                 most_d = larger2(larger2(most_d, x[i / 2]), x[i / 2 + 1]);
-                most_e = larger2(larger2(most_e, mul2_rn(x[i / 2], k.x)), mul2_rn(x[i / 2 + 1], k.y));
+                e[i / 2] = mul2_rn(x[i / 2], k.x), e[i / 2 + 1] = mul2_rn(x[i / 2 + 1], k.y);
+                most_e = larger2(larger2(most_e, e[i / 2]), e[i / 2 + 1]);
             }
             M.d_max[quarter][v] = float2{most_d, most_e};
             tc_fence_before();
@@ -410,14 +423,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             const float2 m0 = M.d_max[0][v], m1 = M.d_max[1][v], m2 = M.d_max[2][v], m3 = M.d_max[3][v];
             const int ee = exponent_of(larger(larger(m0.y, m1.y, m2.y), m3.y, 0.0f)), ed = exponent_of(larger(larger(m0.x, m1.x, m2.x), m3.x, 0.0f));
             const unsigned long long by_e = both(scale_of(ee));
-            unsigned long long e[8];
             unsigned h[8];
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(f.k + quarter * 16 + 2 * i);
-                e[i] = mul2_rn(x[i], k.x), e[i + 1] = mul2_rn(x[i + 1], k.y);
-                h[i] = split_hi(e[i], by_e), h[i + 1] = split_hi(e[i + 1], by_e);
-            }
+            for (int i = 0; i < 8; ++i) h[i] = split_hi(e[i], by_e);
             tmem_write(lanes + kE + quarter * 8, h);
             tmem_written();
             arrive(&M.d_hi);
