@@ -9,9 +9,10 @@
 // One warp fetches, one issues; results of a chunk are written while the next one's first product runs.
 //
 // Bound by the way round: a product, its differences, the next product and the new state cannot overlap one another. A chunk of 128
-// channels takes 6900 clocks (3.5 us): the four products 2700 of the tensor cores, half of them on that way, the rest splits, scales and
+// channels takes 6100 clocks (3.1 us): the four products 2700 of the tensor cores, half of them on that way, the rest splits, scales and
 // hand-overs. Products begin with the upper half of their 128-row operand while the lower one is made (2048 tokens over 32 heads
-// 183 -> 175 us).
+// 183 -> 175 us). 18 warps leave 96 registers a thread, which the loop over chunks needs all: what it needs seldom is in shared memory
+// (173 -> 160 us).
 #include "delta_chunk.cuh"
 
 #include <atomic>
