@@ -139,7 +139,7 @@ def test_refuses_the_default_stream_of_another_device(monkeypatch):
 
 def test_other_backends_are_refused():
     class Other:
-        kind = "checker"
+        kind = "other"
     for make in (lambda: mixers.DeltaNet(Other(), 1, 1, 64, 1), lambda: mixers.QkRope(Other(), 1, 1, 64, 32, 8, None, None)):
         assert refuse(StrataRangeError, "CUDA backend", make) == L.ERR_RANGE
 
