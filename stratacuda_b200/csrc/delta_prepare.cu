@@ -6,9 +6,9 @@
 //   T = (I + A)^-1  of blocks of 32 by substitution, a column a lane, then -T22 (A21 T11), F32 throughout
 //   U^T = V^T (T diag(beta))^T      a lane a value channel
 //   W^T = K^T (T diag(beta P))^T    a lane a key channel; K's tile as it lies, read the other way round
-// Bound by instructions (19.5 k of a warp a chunk and value head), most of them the splits into halves, and by the way from one step to
+// Bound by instructions (19 k of a warp a chunk and value head), most of them the splits into halves, and by the way from one step to
 // the next: two blocks of eight warps a multiprocessor, 100 KB and half of TMEM each, so that one's steps run in the other's waits (a
-// prompt of 2048 tokens over 32 heads of 128: 63 us; blocks of sixteen warps 87 us where this took 68; a thread for a whole row, all 64 columns
+// prompt of 2048 tokens over 32 heads of 128: 57 us; blocks of sixteen warps 87 us where this took 68; a thread for a whole row, all 64 columns
 // unrolled, 210 us, most of them without an instruction to issue). What becomes operands goes through shared memory and bulk copies, few
 // and large ones. Code that a block runs once comes slower than it executes, so it is kept short.
 // Of a slab ahead the kernel runs beside the second one of the slab before it.

@@ -9,23 +9,23 @@ namespace {
 
 constexpr int kSms = 148;
 
-// Rows of a run up to which it is taken token by token. A call in chunks takes 31 us however short its runs are (25 us with heads
+// Rows of a run up to which it is taken token by token. A call in chunks takes 29 us however short its runs are (23 us with heads
 // of 64), token by token 0.7 us a row, and with more state than the multiprocessors walk at once as much longer as chunks get. 32 heads of
-// 128: one session 31 us in chunks and 34 us token by token at 44 rows, two 31 and 32 us at 36, four 33 and 36 us at 28, 16 74 and 82 us at 24;
-// 8 heads of 64: one session 25 and 26 us at 48 rows, 64 of them 50 and 49 us.
+// 128: one session 29 us in chunks and 34 us token by token at 44 rows, two 29 and 32 us at 36, four 30 and 36 us at 28, 16 72 and 82 us at 24;
+// 8 heads of 64: one session 23 and 26 us at 48 rows, 64 of them 48 and 49 us.
 int short_run(const DeltaNet &n, const MixRuns &r) {
-    if (n.dim <= 64) return 48;
-    return (long long)r.segments * n.value_heads <= kSms / 2 ? 37 : 22;
+    if (n.dim <= 64) return 44;
+    return (long long)r.segments * n.value_heads <= kSms / 2 ? 34 : 21;
 }
 
 // States up to which runs are taken in parts: with N of them, (148 / N + 3) / 2 parts fill the multiprocessors (of a part but the last
 // its end and, but for the first, its transition; then all parts once more, from the states that these give). One prompt of 8191 tokens over
-// 2 heads of 128 442 -> 132 us, over 16 497 -> 337 us, over 24 527 -> 504 us; of 2048 over 8 of 64 114 -> 63 us, over 24 of 128
-// 156 -> 146 us. Over 32 three parts are left: 2048 tokens 158 -> 164 us, 8191 550 -> 646 us.
+// 2 heads of 128 440 -> 130 us, over 16 494 -> 330 us, over 24 523 -> 490 us; of 2048 over 8 of 64 112 -> 61 us, over 24 of 128
+// 154 -> 141 us. Over 32 three parts are left: 2048 tokens 156 -> 159 us, 8191 546 -> 627 us.
 constexpr int kSplitStates = 24;
 
 // Parts of a run's chunks, by tenths of microseconds: 3.7 us a chunk as one, 7.1 us a part's chunk twice, 1.5 us to join a part and 15 us
-// of two more kernels. (1000 tokens over 4 heads of 128: 80 us as one, 66 in 8 parts; 640 over 8: 60 and 59 us.)
+// of two more kernels. (1000 tokens over 4 heads of 128: 77 us as one, 64 in 8 parts; 640 over 8: 58 and 57 us.)
 int parts_of(int chunks, int most) {
     int best = 1, least = chunks * 37;
     for (int k = 3; k <= std::min(most, chunks); ++k) {
@@ -76,8 +76,8 @@ cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, 
     }
     // Few states leave most multiprocessors idle in the second kernel: there the next slab's first one runs meanwhile, on the
     // workspace's other half. The first slab gives each multiprocessor two blocks, the next ones those that are left. One prompt
-    // of 2048 tokens over 32 heads of 128 176 -> 158 us, of 8191 over 48 857 -> 594 us, two of 1024 over 32 125 -> 117 us; three
-    // would take 213 us in place of 169: with more states than half of the multiprocessors one slab after another.
+    // of 2048 tokens over 32 heads of 128 172 -> 156 us, of 8191 over 48 825 -> 585 us, two of 1024 over 32 121 -> 112 us; three
+    // would take 200 us in place of 163: with more states than half of the multiprocessors one slab after another.
     if ((long long)r.segments * n.value_heads <= kSms / 2) {
         const int chains = r.segments * n.value_heads, per = r.segments * n.key_heads, most = room / 2 / per;  // chunks of a half
         const int first = std::min(most, 2 * kSms / per), next = std::min(most, std::max(1, 2 * (kSms - chains) / per));
