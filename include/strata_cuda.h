@@ -399,10 +399,12 @@ int strata_kv8_call_dev(const strata_kv8_call *call);
  * delta_rule: with the state S [dim key][dim value] of each value head of the run's sequence, token after token
  *     S <- decay S;  d = beta (v - S^T k);  S <- S + k d^T;  y = S^T q
  *   Value head h reads key head h % key_heads. decay, beta [rows][value_heads]; y [rows][value_heads * dim]. Runs of many
- *   tokens are taken in chunks of 64 on the tensor cores: factors keep 22 bits of what is largest in their row or tile, sums
- *   are F32. A chunk in which a value is not finite (or past 2^60 in magnitude) is walked token by token, so that no token before it
- *   sees it. How a call is taken goes by its segments, count and heads alone: it repeats bit for bit, and tokens that are cut into
- *   other calls differ in their last bits.
+ *   tokens over heads of at most 128 channels are taken in chunks of 64 on the tensor cores, all others token by token. A chunk's factors keep
+ *   22 bits down to 2^-27 of what is largest in their row (a token's k or q; a value channel's state over its keys), sums are F32: a token's
+ *   result is off by what 22 bits lose of what its state holds, not by the size of what comes later or of what a decay has taken away. A chunk
+ *   where that would not hold, or in which a value is not finite (or past 2^60 in magnitude), is walked token by token, so that no token before
+ *   it sees it; 0.05 to 0.4 ms a chunk. How a call is taken goes by its segments, count, heads and dim, and by the values: it repeats bit for
+ *   bit, and tokens that are cut into other calls differ in their last bits.
  * qk_rope: for each head of q and k x / sqrt(mean x^2 + epsilon) times the kind's weight [dim], its first `rotary` channels
  *   rotated (channel d with d + rotary / 2) by the row start[i] + j of cos and sin [cells][rotary / 2], as strata_norm and then
  *   strata_rope_position. Heads of q may lie q_head_stride floats apart (0: dim), as in a projection of [q | gate] for each head.

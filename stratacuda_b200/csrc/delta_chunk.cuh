@@ -10,10 +10,13 @@
 // without values and zeros end; then the parts follow from the states before them.                  delta_chain.cu, delta_join.cu
 //
 // Products. Each F32 factor is two FP16 halves, times a power of two that brings the largest value of its row (or of its
-// TMEM lane, or tile) to 2^13: 22 bits for whatever is within 2^-17 of that, and 2^-38 of it below. lo hi + hi lo + hi hi are three
-// FP16 products with F32 sums; lo lo would be 2^-22 of the result. The large product comes last: sums in TMEM are cut, not
-// rounded, and each step at full size costs up to 2^-24 of the sum, always towards zero (with hi hi first a prompt's result was 9.4e-7
-// off in the 2-norm, so it is 2.8e-7).
+// TMEM lane, or tile) to 2^13; lo is held 2^11 times as large as it is. That is 22 bits for whatever is within 2^-27 of the largest, and
+// 2^-49 of it below. lo hi + hi lo + hi hi are three FP16 products with F32 sums; lo lo would be 2^-22 of the result. The large product
+// comes last, its first step takes the sum so far times 2^-11: sums in TMEM are cut, not rounded, and each step at full size costs up to
+// 2^-24 of the sum, always towards zero (with hi hi first a prompt's result was 9.4e-7 off in the 2-norm, so it is 2.8e-7).
+//
+// What a lane holds of a chunk's 64 tokens has one power of two, also of tokens that are to come, or that a decay has taken away. A chunk in
+// which that hides a value of V, or a difference, from a token whose state holds nothing larger is walked token by token.
 //
 // Workspace: a slot for each run, key head and chunk of a slab, in the layout that the second kernel's tensor-core operands
 // have in shared memory (rows of 128 bytes, 128-byte swizzle): Q above K [2 x 64 tokens][D], hi and lo; then for each of the key
@@ -117,6 +120,13 @@ __device__ __forceinline__ float larger(float a, float b, float c) {
     asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ float smaller(float a, float b, float c) {  // of magnitudes
+    float d;
+    asm("min.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Below this magnitude a value has less than 22 bits beside a largest one of exponent e. (Where that is as small as it gets, F32 ends first.)
+__device__ __forceinline__ float hidden_below(int e) { return e > -113 ? unscale_of(e) * 0x1p-14f : 0.0f; }
 template <int N>
 __device__ __forceinline__ float largest(float m, const float (&x)[N]) {
 #pragma unroll
@@ -136,18 +146,16 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
     return d;
 }
 __device__ __forceinline__ unsigned long long both(float x) { return pack2(x, x); }
-// A pair times powers of two as FP16 halves, hi and lo. (The subtraction is not paired: paired operations and conversions
-// from FP16 share one pipe, which bounds a split.)
-__device__ __forceinline__ void split2(unsigned long long x, unsigned long long by, unsigned &hi, unsigned &lo) {
-    float a, b;
-    unpack2(mul2_rn(x, by), a, b);
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const unsigned *>(&h);
-    lo = *reinterpret_cast<const unsigned *>(&l);
+// A pair times powers of two as FP16 halves, hi first where products with it begin before lo is there. lo is held kLow times as
+// large: it keeps 11 bits where hi itself is as small as FP16 gets. (What hi leaves is a sum of an F32 and an FP16 number in one
+// instruction: conversions back to F32 share a pipe with paired operations, which bounds a split; with them and products by kLow one by one
+// 2048 tokens over 32 heads took 170 us, so 158.)
+constexpr float kLow = 0x1p11f;
+__device__ __forceinline__ float less_half(float x, unsigned short negative) {
+    float d;
+    asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(d) : "h"(negative), "f"(x));
+    return d;
 }
-// The same one after the other, where products with hi begin before lo is there.
 __device__ __forceinline__ unsigned split_hi(unsigned long long x, unsigned long long by) {
     float a, b;
     unpack2(mul2_rn(x, by), a, b);
@@ -157,10 +165,12 @@ __device__ __forceinline__ unsigned split_hi(unsigned long long x, unsigned long
 __device__ __forceinline__ unsigned split_lo(unsigned long long x, unsigned long long by, unsigned hi) {
     float a, b;
     unpack2(mul2_rn(x, by), a, b);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    const unsigned h = hi ^ 0x80008000u;
+    unpack2(mul2_rn(pack2(less_half(a, (unsigned short)h), less_half(b, (unsigned short)(h >> 16))), both(kLow)), a, b);
+    const __half2 l = __floats2half2_rn(a, b);
     return *reinterpret_cast<const unsigned *>(&l);
 }
+__device__ __forceinline__ void split2(unsigned long long x, unsigned long long by, unsigned &hi, unsigned &lo) { hi = split_hi(x, by), lo = split_lo(x, by, hi); }
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[N], float scale, unsigned (&hi)[N / 2], unsigned (&lo)[N / 2]) {
 #pragma unroll
@@ -170,6 +180,11 @@ __device__ __forceinline__ float larger2(float m, unsigned long long x) {
     float a, b;
     unpack2(x, a, b);
     return larger(m, a, b);
+}
+__device__ __forceinline__ float smaller2(float m, unsigned long long x) {
+    float a, b;
+    unpack2(x, a, b);
+    return smaller(m, a, b);
 }
 // Byte of 16-byte piece c of row r: rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ int piece(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
@@ -186,6 +201,26 @@ __device__ __forceinline__ unsigned long long turned_desc(unsigned smem_addr, un
 }
 __device__ __forceinline__ unsigned turned_idesc(int M, int N) { return idesc_f16(M, N) | (1u << 16); }  // the narrow operand
 constexpr unsigned kTurnedWide = 1u << 15;                                                                // the 128-row one
+
+// Step k of product 0 (lo hi), 1 (hi lo) or 2 (hi hi) of a sum; the last one's first step takes what the others gave times 2^-11, 1 / kLow.
+__device__ __forceinline__ void mma_step(unsigned tmem_d, unsigned long long a, unsigned long long b, unsigned idesc, int product, int k) {
+    if (product < 2 || k) return mma_f16(tmem_d, a, b, idesc, product || k);
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n\t}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_step_ts(unsigned tmem_d, unsigned tmem_a, unsigned long long b, unsigned idesc, int product, int k) {
+    if (product < 2 || k) return mma_f16_ts(tmem_d, tmem_a, b, idesc, product || k);
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, 11;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(b), "r"(idesc)
+        : "memory");
+}
 
 // Waits of a block's threads, with a limit; past it, all of them let everything through and the block reports.
 struct Waits {

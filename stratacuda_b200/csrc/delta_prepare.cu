@@ -106,6 +106,25 @@ __device__ __forceinline__ float product_after(float x, int lane) {
     return x;
 }
 
+// Whether a channel has a token that sees nothing of `limit` or more: not its own value, nor what the state still has of earlier ones
+// (a few of the chunk before count, too). One in 2^24 of normally distributed values makes a thread ask, and then only a run's first tokens
+// see nothing larger; tokens of zeros and of strong decays.
+__device__ __noinline__ bool value_hidden(const DeltaRule &A, int heads, long long row0, int before, int tokens, int h, long long channel, float limit) {
+    float held = 0.0f;
+    bool any = false;
+    const int from = -min(before, 8);
+#pragma unroll 8
+    for (int t = from; t < tokens; ++t) {  // (to the end: so that loads of many rows are in flight)
+        const long long row = row0 + t;
+        const float x = fabsf(A.v[row * A.v_stride + channel]);
+        held *= fminf(fabsf(A.decay[row * heads + h]), 1.0f);
+        const float seen = fmaxf(x, held);
+        any |= t >= 0 && seen > 0.0f && seen < limit;
+        held = fmaxf(held, x * fminf(fabsf(A.beta[row * heads + h]), 1.0f));
+    }
+    return any;
+}
+
 // VEC: rows of q and k can be read four channels at a time.
 template <int D, bool VEC>
 __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __grid_constant__ DeltaNet n, const __grid_constant__ DeltaRule A,
@@ -203,7 +222,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
                 const unsigned long long x = q + (product == 0) * (kPanels * 1024), y = q + 512 + (product == 1) * (kPanels * 1024);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_f16(tmem + kRaw, x + k / 4 * 1024 + k % 4 * 2, y + k / 4 * 1024 + k % 4 * 2, idesc_f16(128, 64), product || k);
+                    mma_step(tmem + kRaw, x + k / 4 * 1024 + k % 4 * 2, y + k / 4 * 1024 + k % 4 * 2, idesc_f16(128, 64), product, k);
             }
             mma_commit(&M.done);
         }
@@ -256,6 +275,18 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
         const float inv_v = unscale_of(exponent_of(most_v));
         {
             if (past(most_v)) M.bad[m & 1] = 1;
+            if (most_v > 0.0f) {  // (lanes past the head's channels hold zeros)
+                float least = most_v;
+                if (tokens == kChunk) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) least = smaller(least, v[j], v[j + 1]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) least = half * 32 + j < tokens ? smaller(least, v[j], least) : least;
+                }
+                const float limit = hidden_below(exponent_of(most_v));
+                if (least < limit && value_hidden(A, n.value_heads, row0, t0, tokens, h, (long long)h * n.dim + gt, limit)) M.bad[m & 1] = 1;
+            }
             unsigned hi[16], lo[16];
             split(v, scale_of(exponent_of(most_v)), hi, lo);
             tmem_write(mine + kV + half * 16, hi);
@@ -385,13 +416,13 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + kU, tmem + kV + (product == 0) * 32 + k * 8, tu[product == 1] + k * 2, idesc_f16(128, 64), product || k);
+                        mma_step_ts(tmem + kU, tmem + kV + (product == 0) * 32 + k * 8, tu[product == 1] + k * 2, idesc_f16(128, 64), product, k);
 #pragma unroll
                 for (int product = 0; product < 3; ++product)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16(tmem + kW, keys + (product == 0) * (kPanels * 1024) + k * 128, tw[product == 1] + k * 2, idesc_f16(128, 64) | kTurnedWide,
-                                product || k);
+                        mma_step(tmem + kW, keys + (product == 0) * (kPanels * 1024) + k * 128, tw[product == 1] + k * 2, idesc_f16(128, 64) | kTurnedWide,
+                                 product, k);
                 mma_commit(&M.done);
             }
             __syncwarp();
