@@ -23,6 +23,8 @@ using namespace delta;
 
 constexpr int kPrepareThreads = 256, kPitch = 68;
 constexpr float kWScale = 0x1p-19f;  // of W's sums, which are 2^34 at most: 64 terms of two factors below 2^14
+// Of G (q . k), with q at up to 2^14: past it F32 ends, though what it weighs may be small. (G (k . k) shows in T.)
+constexpr float kLargestWeight = 0x1p100f;
 
 template <int D>
 struct __align__(1024) PrepareSmem {
@@ -340,7 +342,9 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
         M.most[1][half][gt] = most;
         __syncthreads();
         if (!key) {
-            const int e = exponent_of(larger(M.most[1][0][gt], M.most[1][1][gt], 0.0f));
+            const float weight = larger(M.most[1][0][gt], M.most[1][1][gt], 0.0f);
+            if (!(weight <= kLargestWeight)) M.bad[m & 1] = 1;
+            const int e = exponent_of(weight);
             unsigned hi[16] = {}, lo[16] = {};
             if (!empty) split(x, scale_of(e), hi, lo);
             put_pieces(M.tile(0), i, half * 4, hi);

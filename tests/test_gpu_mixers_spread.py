@@ -158,3 +158,23 @@ def test_runs_that_begin_from_nothing(torch, form):
         for i in range(segments):
             c["v"][i * count + 1] *= 1e-14
     check(torch, kh, vh, dim, segments, count, edit, [count - i % 7 for i in range(segments)])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("growing", [36, 40, 60])
+def test_growth_that_only_queries_see(torch, dim, growing):
+    """Keys that do not meet, and a value of 2^-100 that decays of 8 bring back: what a token weighs it by, 8^40 and more times a query's
+    and a key's factors, passes F32's range, the result does not."""
+    kh, vh, count = 1, 2, 64
+
+    def edit(c):
+        c["state"][:] = 0
+        c["decay"][:] = 1
+        c["decay"][0] = 0
+        c["decay"][1:growing] = 8
+        c["k"][:] = np.eye(dim)[np.arange(count) % dim]
+        c["q"][:] = c["k"][:1] / 8
+        c["beta"][:] = 1
+        c["v"] *= 2.0 ** -100
+        c["v"][1:] = 0
+    check(torch, kh, vh, dim, 1, count, edit)
