@@ -141,12 +141,13 @@ class _Device:
         return _strided(x, what, rows, width, stride, self._device) if stride else self._floats(x, what, rows * width)
 
     def _here(self) -> None:
-        """The default stream is the current device's: refused where that is not the one that holds the parts. (A stream of another
-        device is refused by the launch.)"""
+        """Calls go to a stream of the current device: refused where that is not the one that holds the parts. (A launch refuses a stream of
+        another device than the current one.)"""
         if self._device is not None:
             import torch
-            if torch.cuda.current_device() != self._device:
-                raise StrataError(L.ERR_LAYOUT, f"the parts are on device {self._device}, the default stream is device {torch.cuda.current_device()}'s")
+            if (now := torch.cuda.current_device()) != self._device:
+                raise StrataError(L.ERR_LAYOUT, f"the parts are on device {self._device}, the current device is {now}: its default stream, or "
+                                                "another of its streams, is where the call would go")
 
     def _run(self, entry, pack, *values) -> None:
         try:
@@ -187,8 +188,7 @@ class DeviceDeltaNet(_Device):
     def inputs(self, x, q, k, v, sequence, segments: int = 1, count: int = 1, lengths=None, row_stride: int = 0, q_scale: float = 0.0,
                epsilon: float = 1e-6, stream: int = 0) -> None:
         n = segments * count
-        if not stream:
-            self._here()
+        self._here()
         self._run(self._inputs, _pack_inputs, self._at, self._rows(x, "x", n, 2 * self.kd + self.vd, row_stride), row_stride,
                   self._ints(sequence, "sequence", segments), 0 if lengths is None else self._ints(lengths, "lengths", segments),
                   self._floats(q, "q", n * self.kd), self._floats(k, "k", n * self.kd), self._floats(v, "v", n * self.vd), stream, _message.at,
@@ -197,8 +197,7 @@ class DeviceDeltaNet(_Device):
     def rule(self, q, k, v, decay, beta, y, sequence, segments: int = 1, count: int = 1, lengths=None, q_stride: int = 0, k_stride: int = 0,
              v_stride: int = 0, stream: int = 0) -> None:
         n = segments * count
-        if not stream:
-            self._here()
+        self._here()
         self._run(self._rule, _pack_rule, self._at, self._rows(q, "q", n, self.kd, q_stride), self._rows(k, "k", n, self.kd, k_stride),
                   self._rows(v, "v", n, self.vd, v_stride), q_stride, k_stride, v_stride, self._floats(decay, "decay", n * self.value_heads),
                   self._floats(beta, "beta", n * self.value_heads), self._ints(sequence, "sequence", segments),
@@ -226,8 +225,7 @@ class DeviceQkRope(_Device):
     def apply(self, q, k, yq, yk, start, segments: int = 1, count: int = 1, sequence=None, lengths=None, q_stride: int = 0,
               q_head_stride: int = 0, k_stride: int = 0, epsilon: float = 1e-6, stream: int = 0) -> None:
         n, apart = segments * count, q_head_stride or self.dim
-        if not stream:
-            self._here()
+        self._here()
         reach = (self.heads - 1) * apart + self.dim  # from a row's first head to the end of its last
         if q_stride:
             pq = _strided(q, "q", n, reach, q_stride, self._device)

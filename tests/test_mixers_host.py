@@ -137,6 +137,24 @@ def test_refuses_the_default_stream_of_another_device(monkeypatch):
         assert refuse(StrataError, "default stream", lambda: call(make())) == L.ERR_LAYOUT
 
 
+@pytest.mark.parametrize("stream", [0, 0x7000])
+def test_refuses_streams_of_a_device_that_is_not_the_parts(monkeypatch, stream):
+    """A stream goes with the current device (the launch refuses others), so that is the one that has to hold the parts."""
+    torch = pytest.importorskip("torch")
+
+    class There:  # what is looked at of a tensor on device 1
+        dtype = torch.float32
+        get_device, numel, is_contiguous, data_ptr, element_size = lambda _: 1, lambda _: 1 << 40, lambda _: True, lambda _: A, lambda _: 4
+
+    x = There()
+    for call, make in ((inputs, lambda: net(state=x, history=x, weight=x)), (rule, lambda: net(state=x, history=x, weight=x)),
+                       (apply, lambda: rope(q_weight=x, k_weight=x, cos=x, sin=x))):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+        assert refuse(StrataError, "default stream", lambda: call(make(), stream=stream)) == L.ERR_LAYOUT
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+        assert refuse(StrataRangeError, "segments", lambda: call(make(), segments=0, stream=stream)) == L.ERR_RANGE  # past that check
+
+
 def test_other_backends_are_refused():
     class Other:
         kind = "other"
