@@ -18,6 +18,8 @@ from __future__ import annotations
 import ctypes as C
 import struct
 
+import numpy as np
+
 from . import _lib as L
 from .backend import StrataError, StrataRangeError
 from .kv8 import _Types, _address, _int32, _message, _strided, _words
@@ -38,6 +40,12 @@ def _cuda(backend):
 
 def _handle(buf) -> int:
     return 0 if buf is None else buf.handle
+
+
+def _strides(**values) -> None:
+    for name, x in values.items():
+        if not isinstance(x, (int, np.integer)) or not 0 <= x < 1 << 64:
+            raise StrataRangeError(L.ERR_RANGE, f"{name} must be an integer in [0, 2^64)")
 
 
 class DeltaNet:
@@ -77,6 +85,7 @@ class DeltaNet:
                epsilon: float = 1e-6) -> None:
         """q, k, v from projection rows x (strata_delta_inputs). `q_scale` 0 is 1 / sqrt(dim)."""
         _int32(segments=segments, count=count)
+        _strides(row_stride=row_stride)
         self.b._check(self.b.lib.strata_delta_inputs(self.b.ctx, C.byref(self._struct()), x.handle, row_stride, segments, count,
                                                      sequence.handle, _handle(lengths), q_scale, epsilon, q.handle, k.handle, v.handle))
 
@@ -84,6 +93,7 @@ class DeltaNet:
              v_stride: int = 0) -> None:
         """y, and the sequences' new states, from rows q, k, v, decay and beta (strata_delta_rule)."""
         _int32(segments=segments, count=count)
+        _strides(q_stride=q_stride, k_stride=k_stride, v_stride=v_stride)
         self.b._check(self.b.lib.strata_delta_rule(self.b.ctx, C.byref(self._struct()), q.handle, q_stride, k.handle, k_stride, v.handle,
                                                    v_stride, decay.handle, beta.handle, segments, count, sequence.handle, _handle(lengths),
                                                    y.handle))
@@ -110,6 +120,7 @@ class QkRope:
               q_head_stride: int = 0, k_stride: int = 0, epsilon: float = 1e-6) -> None:
         """yq, yk: the normed and rotated heads of rows q and k (strata_qk_rope)."""
         _int32(segments=segments, count=count)
+        _strides(q_stride=q_stride, q_head_stride=q_head_stride, k_stride=k_stride)
         self.b._check(self.b.lib.strata_qk_rope(self.b.ctx, C.byref(self._weights), q.handle, q_stride, q_head_stride, k.handle, k_stride,
                                                 segments, count, _handle(sequence), start.handle, _handle(lengths), epsilon, yq.handle,
                                                 yk.handle))

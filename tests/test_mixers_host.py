@@ -188,3 +188,28 @@ def test_a_net_gives_its_buffers_back_when_a_later_one_fails():
 def test_sizes():
     assert mixers.sizes(16, 32, 128, 3) == dict(state=3 * 128 * 32 * 128, history=3 * 64 * 128 * 3, weight=64 * 128 * 4, workspace=32 << 20)
     assert C.sizeof(L.StrataDeltaNetDev) == 64 and C.sizeof(L.StrataQkRopeWeightsDev) == 64
+
+
+def test_handles_refuse_strides_that_64_bits_do_not_hold():
+    """ctypes cuts integers down to 64 bits without a word: 2^64 + 512 would pass for rows 512 floats apart."""
+    class Lib:
+        def __getattr__(self, name):
+            def entry(*args):
+                raise AssertionError(f"{name} was reached")
+            return entry
+
+    class Buf:
+        handle = 1
+
+    class Backend:
+        kind, lib, ctx = "cuda", Lib(), None
+        alloc = lambda *_, **__: Buf()  # noqa: E731
+
+    x = Buf()
+    delta, qk = mixers.DeltaNet(Backend(), 2, 4, 64, 3, weight=x), mixers.QkRope(Backend(), 4, 2, 64, 32, 10, x, x, x, x)
+    for bad in ((1 << 64) + 512, -1, -(1 << 64) + 512, 1 << 64, 512.0):
+        calls = [lambda: delta.inputs(x, x, x, x, x, row_stride=bad)]
+        calls += [lambda n=n: delta.rule(x, x, x, x, x, x, x, **{n: bad}) for n in ("q_stride", "k_stride", "v_stride")]
+        calls += [lambda n=n: qk.apply(x, x, x, x, x, **{n: bad}) for n in ("q_stride", "q_head_stride", "k_stride")]
+        for call in calls:
+            assert refuse(StrataRangeError, "stride", call) == L.ERR_RANGE
