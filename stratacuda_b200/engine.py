@@ -82,14 +82,15 @@ def gdn_gates(o, b, g, p: str, x, tokens: int):
 
 class RunMixers:
     """The run forms of the token mixers (stratacuda_b200.mixers) of the layers of an engine (one sequence) or a batch: a layer's
-    state and history are the ones that the other entries use, the layers share a workspace."""
+    state and history are the ones that the other entries use; all layers of all engines and batches of a backend, whose calls follow one
+    another on its stream, share a workspace."""
 
     def __init__(self, ops, states, sequences: int, sequence=None):
         self.o, self.b, self.g, self.states, self.sequences = ops, ops.b, ops.g, states, sequences
-        self.nets, self.ropes, self.owned = {}, {}, []
+        self.nets, self.ropes, self.owned, self.workspace = {}, {}, [], None
         try:
-            from . import _lib as L
-            self.workspace = self._keep(L.DELTA_WORKSPACE_BYTES // 4, "u32", False)
+            from .mixers import borrow_workspace
+            self.workspace = borrow_workspace(self.b)
             self.sequence = sequence
             if sequence is None:
                 self.sequence = self._keep(sequences, "i32", True)
@@ -135,9 +136,13 @@ class RunMixers:
         return yq, yk
 
     def free(self) -> None:
+        from .mixers import return_workspace
         for buf in self.owned:
             self.b.free(buf)
         self.owned = []
+        if self.workspace is not None:
+            return_workspace(self.b)
+            self.workspace = None
 
 
 class Ops:

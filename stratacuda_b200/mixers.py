@@ -32,6 +32,24 @@ def sizes(key_heads: int, value_heads: int, dim: int, sequences: int, taps: int 
                 workspace=L.DELTA_WORKSPACE_BYTES // 4)
 
 
+def borrow_workspace(backend):
+    """The workspace that users of a backend share, whose calls follow one another on its stream: made for the first of them, freed when the
+    last one gives it back (``return_workspace``)."""
+    shared = getattr(backend, "_delta_workspace", None)
+    if shared is None:
+        shared = backend._delta_workspace = [backend.alloc(L.DELTA_WORKSPACE_BYTES // 4, "u32", zero=False), 0]
+    shared[1] += 1
+    return shared[0]
+
+
+def return_workspace(backend) -> None:
+    shared = backend._delta_workspace
+    shared[1] -= 1
+    if not shared[1]:
+        backend._delta_workspace = None
+        backend.free(shared[0])
+
+
 def _cuda(backend):
     if getattr(backend, "kind", None) != "cuda":
         raise StrataRangeError(L.ERR_RANGE, "the token mixers over runs need the CUDA backend")

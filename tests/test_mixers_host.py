@@ -213,3 +213,70 @@ def test_handles_refuse_strides_that_64_bits_do_not_hold():
         calls += [lambda n=n: qk.apply(x, x, x, x, x, **{n: bad}) for n in ("q_stride", "q_head_stride", "k_stride")]
         for call in calls:
             assert refuse(StrataRangeError, "stride", call) == L.ERR_RANGE
+
+
+class Counting:
+    """A backend that only counts what it has handed out; `room` allocations of any size."""
+    kind = "cuda"
+
+    def __init__(self, room=1 << 30):
+        self.live, self.room = {}, room
+
+    def alloc(self, length, type="f32", zero=True):
+        if not self.room:
+            raise MemoryError("no more")
+        self.room -= 1
+        buf = object()
+        self.live[id(buf)] = (buf, length)
+        return buf
+
+    def write(self, buf, data):
+        assert id(buf) in self.live
+
+    def free(self, buf):
+        del self.live[id(buf)]
+
+    def words(self):
+        return sum(n for _, n in self.live.values())
+
+
+def run_mixers(b, sequences=1):
+    from types import SimpleNamespace
+
+    from stratacuda_b200.engine import RunMixers
+    return RunMixers(SimpleNamespace(b=b, g={}), [], sequences)
+
+
+def test_sessions_of_a_backend_share_a_workspace():
+    """Engines and batches of one backend follow one another on its stream: 64 sessions need one workspace, not 8 GB of them."""
+    b, other = Counting(), Counting()
+    held = [run_mixers(b) for _ in range(64)]
+    apart = run_mixers(other)
+    assert b.words() == L.DELTA_WORKSPACE_BYTES // 4 + 64
+    assert len({id(r.workspace) for r in held}) == 1 and apart.workspace is not held[0].workspace
+    for r in held[:-1]:
+        r.free()
+        r.free()  # twice: as once
+    assert b.words() == L.DELTA_WORKSPACE_BYTES // 4 + 1
+    again = run_mixers(b)
+    assert again.workspace is held[-1].workspace
+    held[-1].free(), again.free()
+    assert not b.live
+    new = run_mixers(b)  # the last one's is gone
+    assert id(new.workspace) in b.live
+    new.free(), apart.free()
+    assert not b.live and not other.live
+
+
+def test_a_session_that_cannot_be_made_leaves_the_workspace_to_the_others():
+    b = Counting(room=2)
+    first = run_mixers(b)
+    with pytest.raises(MemoryError):
+        run_mixers(b)
+    assert id(first.workspace) in b.live
+    first.free()
+    assert not b.live
+    b.room = 1  # the workspace, and then nothing
+    with pytest.raises(MemoryError):
+        run_mixers(b)
+    assert not b.live
