@@ -448,10 +448,13 @@ class StrataEngine:
         if self.mixers:
             self.runs = RunMixers(self.ops, self.states, 1)
 
+    _position_there = False  # since the eager step or chunk began
+
     def position_on_device(self):
-        """The position as a device scalar: the captured steps' own, else written now."""
-        if not self._dev_mode:
+        """The position as a device scalar: the captured steps' own, else written by the step's or chunk's first layer that asks."""
+        if not self._dev_mode and not self._position_there:
             self.b.write(self._device_scalars()["position"], np.array([self.position], np.int32))
+            self._position_there = True
         return self._dev["position"]
 
     # ---- one token (src/engine.js:73-156)
@@ -675,7 +678,7 @@ class StrataEngine:
                 result = self._graph_step(token, logits)
             else:
                 self.ops.embedding(token, self.residual)
-                self._token = token
+                self._token, self._position_there = token, False
                 for layer in range(self.g["layers"]):
                     self._layer(layer)
                 result = dict(position=self.position)
@@ -1016,6 +1019,7 @@ class PromptBatch:
                 b.run("strata_embed_token", dict(Table=o.weight("token_embd.weight"), Token=self.device["tokens"], Residual=self.residual,
                                                  width=g["width"], streams=g["streams"], vocab=g["vocab"], tokens=n), grid(n * g["width"]))
             else:
+                e._position_there = False
                 for t, token in enumerate(self.tokens):
                     o.embedding(token, self.residual, t * hc)
             for layer in range(g["layers"]):
