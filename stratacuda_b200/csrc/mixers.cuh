@@ -25,6 +25,7 @@ __device__ __forceinline__ MixRun mix_run(const MixRuns &r, int sequences, int i
 // too is reported, and the later run is idle.
 __device__ __forceinline__ MixRun mix_run_alone(const MixRuns &r, int sequences, int i, unsigned *err) {
     MixRun a = mix_run(r, sequences, i, err);
+    if (r.once) return a;
     bool twice = false;
     if (a.sequence >= 0)
         for (int j = threadIdx.x; j < i; j += blockDim.x) twice |= r.sequence[j] == a.sequence;

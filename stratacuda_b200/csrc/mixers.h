@@ -1,6 +1,6 @@
 // Internal interface of the token mixers over runs of many sequences: the delta-rule layer's inputs, the gated delta rule, and
-// the norms of queries and keys with their rotation (delta_rows.cu, delta_step.cu, qk_rope.cu; checked by mixers_api.cu and
-// api.cu). The operators' definitions are in include/strata_cuda.h.
+// the norms of queries and keys with their rotation (delta_rows.cu; delta_rule.cu with delta_step.cu, delta_prepare.cu, delta_chain.cu and
+// delta_join.cu; qk_rope.cu; checked by mixers_api.cu and api.cu). The operators' definitions are in include/strata_cuda.h.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -13,6 +13,7 @@ namespace strata {
 struct MixRuns {
     int segments, count;
     const int *sequence, *lengths;
+    bool once = false;  // no sequence is outside or there twice: a kernel of the call has made the list so
 };
 // Device view of one delta-rule layer.
 struct DeltaNet {
