@@ -108,18 +108,25 @@ __device__ __noinline__ void walk_chunk(const DeltaNet &n, const DeltaRule &A, C
     }
 }
 
-// Whether a channel has a token, of `count` from t0, that sees nothing of `limit` or more: not its own difference without the state, nor what
-// the state, `held` before the chunk, still has of earlier ones. Seldom called, as the first kernel's value_hidden.
+// Whether a channel has a token, of a quarter's, that sees nothing of `limit` or more: not its own difference without the state, nor what the
+// state, `held` before the chunk, still has of earlier ones; by a whole warp. Seldom called, as the first kernel's value_hidden. A token whose
+// query weighs nothing has a result of zeros exactly.
 template <int D>
-__device__ __noinline__ bool difference_hidden(const DeltaRule &A, int heads, long long row, int h, const float *u, float held, int t0, int count, float limit) {
-    bool any = false;
-#pragma unroll 8
-    for (int t = 0; t < t0 + count; ++t, u += D) {
-        held *= fminf(fabsf(A.decay[(row + t) * heads + h]), 1.0f);
-        held = fmaxf(held, fabsf(*u));
-        any |= t >= t0 && held > 0.0f && held < limit;
+__device__ __forceinline__ bool difference_hidden(const DeltaRule &A, int heads, long long row, int h, const float *u, const DeltaFactors &f, float held, int quarter,
+                                                  float limit) {
+    const int lane = threadIdx.x & 31;
+    float x[2], size[2], decay[2];
+    bool wanted[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int t = lane + 32 * e;
+        const bool in = t < f.counted;
+        x[e] = in ? fabsf(u[t * D]) : 0.0f;
+        size[e] = f.keyed[e] >> lane & 1 ? x[e] : 0.0f;
+        decay[e] = in ? fminf(fabsf(A.decay[(row + t) * heads + h]), 1.0f) : 1.0f;
+        wanted[e] = in & (t >> 4 == quarter) & (f.attn[t] > 0x1p-120f);
     }
-    return any;
+    return see_less(size, decay, x, wanted, held, limit, lane);
 }
 
 // ENDS: nothing but where parts of runs end, from zeros and (their transition) without values from the identity. SORTED: a kernel of its own,
@@ -488,7 +495,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                 inv_y = unscale_of(ed);
                 // A difference that the largest of its channel hides: the chunk is walked, from the state as it was. (While the products run.)
                 const float limit = hidden_below(ed);
-                const int left = M.tokens - c * kChunk - quarter * 16;
+                const int left = f.counted - quarter * 16;
                 float least = limit;
                 if (left >= 16) {
 #pragma unroll
@@ -501,20 +508,22 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
                         least = i < left ? smaller(least, p[i & 1], least) : least;
                     }
                 }
-                const bool small = least < limit && in && left > 0;
-                if (any_work(small)) {  // seldom: all of the block's threads look closer, the state in memory meanwhile
-                    store_state();
-                    const float held = larger(larger(M.s_max[0][v], M.s_max[1][v], M.s_max[2][v]), M.s_max[3][v], 0.0f);
-                    const bool hidden = any_work(small && difference_hidden<D>(A, n.value_heads, M.row0 + c * kChunk, M.head, M.row[st].u + v, held,
-                                                                              quarter * 16, min(left, 16), limit));
-                    if (hidden) {
+                const bool closer = least < limit && in && left > 0;
+                if (any_work(closer)) {  // mostly a difference near zero beside others
+                    bool hidden = false;
+                    const float most_s = larger(larger(M.s_max[0][v], M.s_max[1][v], M.s_max[2][v]), M.s_max[3][v], 0.0f);
+                    for (unsigned ask = __ballot_sync(0xffffffffu, closer); ask && !hidden; ask &= ask - 1) {
+                        const int who = __ffs(ask) - 1;
+                        hidden = difference_hidden<D>(A, n.value_heads, M.row0 + c * kChunk, M.head, M.row[st].u + w4 * 32 + who, f,
+                                                      __shfl_sync(0xffffffffu, most_s, who), quarter, __shfl_sync(0xffffffffu, limit, who));
+                    }
+                    if (any_work(hidden)) {
                         wait.warp(&M.d_done, now, lane);
                         wait.warp(&M.y_done, now, lane);
                         tc_fence_after();
+                        store_state();
                         walk(c);
-                    }
-                    load_state(M.to + quarter * kPart * M.to_next + v, M.to_next);
-                    if (hidden) {
+                        load_state(M.to + quarter * kPart * M.to_next + v, M.to_next);
                         arrive(&M.row_empty[st]);
                         owed = false;
                         continue;

@@ -38,7 +38,9 @@ struct DeltaFactors {  // of a chunk's rows, for one value head
     float k[64];       // E over K's scale
     float end;         // P of the last token
     int walk;          // token by token
-    int pad[30];
+    int counted;       // tokens up to the last one with a query or a key: rows that fill up a batch have neither
+    unsigned keyed[2]; // tokens, by bits, whose key is large enough that the state holds what is large of them
+    int pad[27];
 };
 struct DeltaSlab {  // runs, key heads and chunks [first, first + n) of a call
     int run0, runs, head0, heads, chunk0, chunks;
@@ -220,6 +222,30 @@ __device__ __forceinline__ void mma_step_ts(unsigned tmem_d, unsigned tmem_a, un
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, 11;\n\t}" ::"r"(tmem_d),
         "r"(tmem_a), "l"(b), "r"(idesc)
         : "memory");
+}
+
+// Of a key's scale taken back: from it on what a token adds to the state, times the key, is no less than the 2^-27 of its value or difference
+// that 22 bits reach down to.
+constexpr float kKeyed = 0x1p-40f;
+// A channel's 64 tokens over a warp, two a lane: what each adds to the state of it (size[0] of token `lane`, size[1] of lane + 32), what is left
+// of the state at it (decay, up to one), and `held` before them. Whether there is a token among `wanted` (bits as sizes) that sees less than
+// limit but something: neither of its own (`seen`) nor of what the state holds.
+__device__ __forceinline__ bool see_less(const float (&size)[2], const float (&decay)[2], const float (&seen)[2], const bool (&wanted)[2], float held, float limit, int lane) {
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        float d = decay[e], b = size[e];  // over tokens so far: held after them is max(d held, b)
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const float d0 = __shfl_up_sync(0xffffffffu, d, s), b0 = __shfl_up_sync(0xffffffffu, b, s);
+            if (lane >= s) b = fmaxf(d * b0, b), d *= d0;
+        }
+        const float after = fmaxf(d * held, b), before = __shfl_up_sync(0xffffffffu, after, 1);
+        const float most = fmaxf(seen[e], decay[e] * (lane ? before : held));
+        any |= wanted[e] & (most > 0.0f) & (most < limit);
+        held = __shfl_sync(0xffffffffu, after, 31);
+    }
+    return __any_sync(0xffffffffu, any);
 }
 
 // Waits of a block's threads, with a limit; past it, all of them let everything through and the block reports.

@@ -41,6 +41,7 @@ struct __align__(1024) PrepareSmem {
     float inv_tu[64];
     float most[2][2][128];  // a row's largest values, by warpgroup; two that are used in turn
     int bad_key, bad[2], abort_flag;  // by turn
+    int counted;  // as in the factors
     unsigned tmem;
     unsigned long long done;
 
@@ -108,23 +109,31 @@ __device__ __forceinline__ float product_after(float x, int lane) {
     return x;
 }
 
-// Whether a channel has a token that sees nothing of `limit` or more: not its own value, nor what the state still has of earlier ones
-// (a few of the chunk before count, too). One in 2^24 of normally distributed values makes a thread ask, and then only a run's first tokens
-// see nothing larger; tokens of zeros and of strong decays.
-__device__ __noinline__ bool value_hidden(const DeltaRule &A, int heads, long long row0, int before, int tokens, int h, long long channel, float limit) {
-    float held = 0.0f;
-    bool any = false;
-    const int from = -min(before, 8);
-#pragma unroll 8
-    for (int t = from; t < tokens; ++t) {  // (to the end: so that loads of many rows are in flight)
+// Whether a channel has a token that sees nothing of `limit` or more: not its own value, nor what the state still has of earlier ones (one
+// before the chunk counts, too); by a whole warp. One in 2^25 of normally distributed values makes a thread ask, and then only a run's first
+// tokens see nothing larger; tokens of zeros and of strong decays. What a token without a key is given goes nowhere.
+__device__ __noinline__ bool value_hidden(const DeltaNet &n, const DeltaRule &A, long long row0, int before, int tokens, int h, int channel, const float *key_scales,
+                                          float limit) {
+    const int lane = threadIdx.x & 31;
+    const float *v = A.v + (long long)h * n.dim + channel, *decays = A.decay + h, *strengths = A.beta + h;
+    float x[2], size[2], decay[2], held = 0.0f;
+    bool wanted[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int t = lane + 32 * e;
         const long long row = row0 + t;
-        const float x = fabsf(A.v[row * A.v_stride + channel]);
-        held *= fminf(fabsf(A.decay[row * heads + h]), 1.0f);
-        const float seen = fmaxf(x, held);
-        any |= t >= 0 && seen > 0.0f && seen < limit;
-        held = fmaxf(held, x * fminf(fabsf(A.beta[row * heads + h]), 1.0f));
+        const bool in = t < tokens;
+        x[e] = in ? fabsf(v[row * A.v_stride]) : 0.0f;
+        decay[e] = in ? fminf(fabsf(decays[row * n.value_heads]), 1.0f) : 1.0f;
+        size[e] = in & (key_scales[t] >= kKeyed) ? x[e] * fminf(fabsf(strengths[row * n.value_heads]), 1.0f) : 0.0f;
+        wanted[e] = in & (key_scales[t] > unscale_of(-113));
     }
-    return any;
+    if (before) {
+        float key = 0.0f;
+        for (int i = lane; i < n.dim; i += 32) key = larger(key, A.k[(row0 - 1) * A.k_stride + (long long)(h % n.key_heads) * n.dim + i], 0.0f);
+        if (warp_largest(key) >= kKeyed * 0x1p13f) held = fabsf(v[(row0 - 1) * A.v_stride]) * fminf(fabsf(strengths[(row0 - 1) * n.value_heads]), 1.0f);
+    }
+    return see_less(size, decay, x, wanted, held, limit, lane);
 }
 
 // VEC: rows of q and k can be read four channels at a time.
@@ -269,6 +278,11 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
                 factors->k[t] = (e ? after[1] : after[0] * high) * inv_k;
                 if (t == 63) factors->end = p;
             }
+            const unsigned low_rows = __ballot_sync(0xffffffffu, larger(M.inv[lane], M.inv[64 + lane], 0.0f) > unscale_of(-113));
+            const unsigned high_rows = __ballot_sync(0xffffffffu, larger(M.inv[32 + lane], M.inv[96 + lane], 0.0f) > unscale_of(-113));
+            const unsigned low_keys = __ballot_sync(0xffffffffu, M.inv[64 + lane] >= kKeyed), high_keys = __ballot_sync(0xffffffffu, M.inv[96 + lane] >= kKeyed);
+            if (lane == 0) factors->keyed[0] = low_keys, factors->keyed[1] = high_keys;
+            if (lane == 0) factors->counted = M.counted = high_rows ? 64 - __clz(high_rows) : 32 - __clz(low_rows);
         }
         M.most[0][half][gt] = largest(0.0f, v);
         if (tid == kBulk) bulk_out_read();  // Q's tile, or the last head's W
@@ -277,17 +291,21 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
         const float inv_v = unscale_of(exponent_of(most_v));
         {
             if (past(most_v)) M.bad[m & 1] = 1;
-            if (most_v > 0.0f) {  // (lanes past the head's channels hold zeros)
-                float least = most_v;
-                if (tokens == kChunk) {
+            float least = most_v;
+            if (M.counted == kChunk) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) least = smaller(least, v[j], v[j + 1]);
-                } else {
+                for (int j = 0; j < 32; j += 2) least = smaller(least, v[j], v[j + 1]);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) least = half * 32 + j < tokens ? smaller(least, v[j], least) : least;
+                for (int j = 0; j < 32; ++j) least = half * 32 + j < M.counted ? smaller(least, v[j], least) : least;
+            }
+            const float limit = hidden_below(exponent_of(most_v));  // (zero where a lane has zeros)
+            for (unsigned ask = __ballot_sync(0xffffffffu, least < limit); ask; ask &= ask - 1) {
+                const int who = __ffs(ask) - 1;
+                if (value_hidden(n, A, row0, t0, tokens, h, w4 * 32 + who, M.inv + 64, __shfl_sync(0xffffffffu, limit, who))) {
+                    M.bad[m & 1] = 1;
+                    break;
                 }
-                const float limit = hidden_below(exponent_of(most_v));
-                if (least < limit && value_hidden(A, n.value_heads, row0, t0, tokens, h, (long long)h * n.dim + gt, limit)) M.bad[m & 1] = 1;
             }
             unsigned hi[16], lo[16];
             split(v, scale_of(exponent_of(most_v)), hi, lo);

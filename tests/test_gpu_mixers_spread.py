@@ -178,3 +178,20 @@ def test_growth_that_only_queries_see(torch, dim, growing):
         c["v"] *= 2.0 ** -100
         c["v"][1:] = 0
     check(torch, kh, vh, dim, 1, count, edit)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("where", ["behind", "before", "between", "keys alone", "queries alone"])
+def test_rows_of_zeros(torch, form, where):
+    """Rows that fill up a batch without lengths: no key, query and value (or one of the first two), beside tokens that are large."""
+    kh, vh, dim, segments, count = form
+    t = np.tile(np.arange(count), segments)
+    rows = {"behind": t >= count - count // 3, "before": t < count // 3, "between": (t % 7 == 3) | ((t > 20) & (t < 40))}.get(where, t % 5 == 2)
+
+    def edit(c):
+        c["v"][t == 50 % count] *= 1e10
+        for n in {"keys alone": "k", "queries alone": "q"}.get(where, "qkv"):  # (each letter a name)
+            c[n][rows] = 0
+        if where == "keys alone":  # what such a token is given goes nowhere
+            c["v"][rows] *= (10.0 ** np.random.default_rng(1).uniform(-12, 12, (rows.sum(), 1))).astype(np.float32)
+    check(torch, kh, vh, dim, segments, count, edit)
