@@ -115,18 +115,17 @@ template <int D>
 __device__ __forceinline__ bool difference_hidden(const DeltaRule &A, int heads, long long row, int h, const float *u, const DeltaFactors &f, float held, int quarter,
                                                   float limit) {
     const int lane = threadIdx.x & 31;
-    float x[2], size[2], decay[2];
+    float x[2], decay[2];
     bool wanted[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int t = lane + 32 * e;
         const bool in = t < f.counted;
         x[e] = in ? fabsf(u[t * D]) : 0.0f;
-        size[e] = f.keyed[e] >> lane & 1 ? x[e] : 0.0f;
         decay[e] = in ? fminf(fabsf(A.decay[(row + t) * heads + h]), 1.0f) : 1.0f;
         wanted[e] = in & (t >> 4 == quarter) & (f.attn[t] > 0x1p-120f);
     }
-    return see_less(size, decay, x, wanted, held, limit, lane);
+    return see_less(x, decay, x, wanted, held, limit, lane);
 }
 
 // ENDS: nothing but where parts of runs end, from zeros and (their transition) without values from the identity. SORTED: a kernel of its own,

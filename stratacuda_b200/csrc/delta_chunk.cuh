@@ -3,6 +3,8 @@
 // With P_i the product of a chunk's decays up to token i, G_ij that of those after j up to i, E_i that of those after i:
 //   A_ij = beta_i G_ij (k_i . k_j) for j < i,   T = (I + A)^-1,   U = T diag(beta) V,   W = T diag(beta P) K        delta_prepare.cu
 //   D = U - W S,   y_i = P_i q_i S + sum_{j <= i} G_ij (q_i . k_j) D_j,   S <- P_63 S + sum_i E_i k_i D_i^T          delta_chain.cu
+// (with keys as they are scaled for the products, by a power of two e_i each: k_i 2^-e_i, beta_i 2^2e_i, and as V and D what they add to the
+// state, beta_i 2^e_i v_i and 2^e_i d_i; so that keys and strengths of all sizes meet in factors of one size.)
 // The first line needs no state: all chunks of all heads at once. The second goes from chunk to chunk. Products of decays are
 // formed by multiplication alone, so that zero decays need no care.
 //
@@ -35,12 +37,11 @@ struct DeltaFactors {  // of a chunk's rows, for one value head
     float z[64];       // W's scale taken back
     float q[64];       // P over Q's scale
     float attn[64];    // G (q . k)'s scale taken back
-    float k[64];       // E over K's scale
+    float k[64];       // E over 2^13
     float end;         // P of the last token
     int walk;          // token by token
     int counted;       // tokens up to the last one with a query or a key: rows that fill up a batch have neither
-    unsigned keyed[2]; // tokens, by bits, whose key is large enough that the state holds what is large of them
-    int pad[27];
+    int pad[29];
 };
 struct DeltaSlab {  // runs, key heads and chunks [first, first + n) of a call
     int run0, runs, head0, heads, chunk0, chunks;
@@ -224,9 +225,6 @@ __device__ __forceinline__ void mma_step_ts(unsigned tmem_d, unsigned tmem_a, un
         : "memory");
 }
 
-// Of a key's scale taken back: from it on what a token adds to the state, times the key, is no less than the 2^-27 of its value or difference
-// that 22 bits reach down to.
-constexpr float kKeyed = 0x1p-40f;
 // A channel's 64 tokens over a warp, two a lane: what each adds to the state of it (size[0] of token `lane`, size[1] of lane + 32), what is left
 // of the state at it (decay, up to one), and `held` before them. Whether there is a token among `wanted` (bits as sizes) that sees less than
 // limit but something: neither of its own (`seen`) nor of what the state holds.

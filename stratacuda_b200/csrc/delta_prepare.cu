@@ -4,7 +4,7 @@
 //   [Q; K] K^T      128 rows by 64, once for all of them
 //   A, G (q . k)    a row's two threads have half of its columns each, from their TMEM lane
 //   T = (I + A)^-1  of blocks of 32 by substitution, a column a lane, then -T22 (A21 T11), F32 throughout
-//   U^T = V^T (T diag(beta))^T      a lane a value channel
+//   U^T = (diag(beta) V)^T T^T      a lane a value channel
 //   W^T = K^T (T diag(beta P))^T    a lane a key channel; K's tile as it lies, read the other way round
 // Bound by instructions (19 k of a warp a chunk and value head), most of them the splits into halves, and by the way from one step to
 // the next: two blocks of eight warps a multiprocessor, 100 KB and half of TMEM each, so that one's steps run in the other's waits (a
@@ -22,9 +22,10 @@ namespace {
 using namespace delta;
 
 constexpr int kPrepareThreads = 256, kPitch = 68;
+constexpr float kKey = 0x1p-13f;     // keys are scaled to 2^13, and of size one to all but the products
 constexpr float kWScale = 0x1p-19f;  // of W's sums, which are 2^34 at most: 64 terms of two factors below 2^14
 // Of G (q . k), with q at up to 2^14: past it F32 ends, though what it weighs may be small. (G (k . k) shows in T.)
-constexpr float kLargestWeight = 0x1p100f;
+constexpr float kLargestWeight = 0x1p110f;
 
 template <int D>
 struct __align__(1024) PrepareSmem {
@@ -35,13 +36,13 @@ struct __align__(1024) PrepareSmem {
         unsigned char w[2][D * 128];
     };
     float inv[128];  // Q's and K's scales taken back
-    // decays; their products up to a token in its half; strengths, and times decays up to the token over K's scale; K's
-    // scales taken back, the lower half's times the decays after a token in it
-    float decay[64], upto[64], beta[64], beta_w[64], inv_k[64];
+    // decays; their products up to a token in its half; what a value is added to the state times; strengths, and times decays up to the
+    // token (of keys by their power of two); decays after a token in its half, for the lower one, over keys' 2^13
+    float decay[64], upto[64], gain[64], beta[64], beta_w[64], behind[64];
     float inv_tu[64];
     float most[2][2][128];  // a row's largest values, by warpgroup; two that are used in turn
     int bad_key, bad[2], abort_flag;  // by turn
-    int counted;  // as in the factors
+    int counted;  // tokens up to the last one with a key and a strength
     unsigned tmem;
     unsigned long long done;
 
@@ -109,31 +110,31 @@ __device__ __forceinline__ float product_after(float x, int lane) {
     return x;
 }
 
-// Whether a channel has a token that sees nothing of `limit` or more: not its own value, nor what the state still has of earlier ones (one
-// before the chunk counts, too); by a whole warp. One in 2^25 of normally distributed values makes a thread ask, and then only a run's first
-// tokens see nothing larger; tokens of zeros and of strong decays. What a token without a key is given goes nowhere.
+// Whether a channel has a token that sees nothing of `limit` or more: not what itself adds to the state, nor what that still has of earlier
+// ones (one before the chunk counts, too); by a whole warp. One in 2^25 of normally distributed values makes a thread ask, and then only a
+// run's first tokens see nothing larger; tokens of zeros and of strong decays. A token without a key or a strength leaves the state alone.
 __device__ __noinline__ bool value_hidden(const DeltaNet &n, const DeltaRule &A, long long row0, int before, int tokens, int h, int channel, const float *key_scales,
                                           float limit) {
     const int lane = threadIdx.x & 31;
     const float *v = A.v + (long long)h * n.dim + channel, *decays = A.decay + h, *strengths = A.beta + h;
-    float x[2], size[2], decay[2], held = 0.0f;
+    float x[2], decay[2], held = 0.0f;
     bool wanted[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int t = lane + 32 * e;
         const long long row = row0 + t;
         const bool in = t < tokens;
-        x[e] = in ? fabsf(v[row * A.v_stride]) : 0.0f;
+        const float gain = in ? fabsf(strengths[row * n.value_heads] * (key_scales[t] * 0x1p13f)) : 0.0f;
+        x[e] = in ? fabsf(v[row * A.v_stride]) * gain : 0.0f;
         decay[e] = in ? fminf(fabsf(decays[row * n.value_heads]), 1.0f) : 1.0f;
-        size[e] = in & (key_scales[t] >= kKeyed) ? x[e] * fminf(fabsf(strengths[row * n.value_heads]), 1.0f) : 0.0f;
-        wanted[e] = in & (key_scales[t] > unscale_of(-113));
+        wanted[e] = in & (gain > 0x1p-100f);
     }
     if (before) {
         float key = 0.0f;
         for (int i = lane; i < n.dim; i += 32) key = larger(key, A.k[(row0 - 1) * A.k_stride + (long long)(h % n.key_heads) * n.dim + i], 0.0f);
-        if (warp_largest(key) >= kKeyed * 0x1p13f) held = fabsf(v[(row0 - 1) * A.v_stride]) * fminf(fabsf(strengths[(row0 - 1) * n.value_heads]), 1.0f);
+        held = fabsf(v[(row0 - 1) * A.v_stride] * (strengths[(row0 - 1) * n.value_heads] * (warp_largest(key) * 0.5f)));
     }
-    return see_less(size, decay, x, wanted, held, limit, lane);
+    return see_less(x, decay, x, wanted, held, limit, lane);
 }
 
 // VEC: rows of q and k can be read four channels at a time.
@@ -268,24 +269,33 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int t = lane + 32 * e;
-                const float p = e ? upto[1] * low : upto[0], inv_k = M.inv[64 + t];
+                const float p = e ? upto[1] * low : upto[0], key = M.inv[64 + t] * 0x1p13f;
                 M.decay[t] = a[e];
                 M.upto[t] = upto[e];
-                M.beta[t] = b[e];
-                M.beta_w[t] = b[e] * p * inv_k;
-                M.inv_k[t] = e ? inv_k : inv_k * after[0];
+                M.gain[t] = b[e] * key;
+                M.beta[t] = b[e] * key * key;
+                M.beta_w[t] = M.beta[t] * p * kKey;
+                M.behind[t] = e ? kKey : kKey * after[0];
                 factors->q[t] = p * M.inv[t];
-                factors->k[t] = (e ? after[1] : after[0] * high) * inv_k;
+                factors->k[t] = (e ? after[1] : after[0] * high) * kKey;
                 if (t == 63) factors->end = p;
             }
             const unsigned low_rows = __ballot_sync(0xffffffffu, larger(M.inv[lane], M.inv[64 + lane], 0.0f) > unscale_of(-113));
             const unsigned high_rows = __ballot_sync(0xffffffffu, larger(M.inv[32 + lane], M.inv[96 + lane], 0.0f) > unscale_of(-113));
-            const unsigned low_keys = __ballot_sync(0xffffffffu, M.inv[64 + lane] >= kKeyed), high_keys = __ballot_sync(0xffffffffu, M.inv[96 + lane] >= kKeyed);
-            if (lane == 0) factors->keyed[0] = low_keys, factors->keyed[1] = high_keys;
-            if (lane == 0) factors->counted = M.counted = high_rows ? 64 - __clz(high_rows) : 32 - __clz(low_rows);
+            const unsigned low_gains = __ballot_sync(0xffffffffu, fabsf(M.gain[lane]) > 0x1p-100f), high_gains = __ballot_sync(0xffffffffu, fabsf(M.gain[32 + lane]) > 0x1p-100f);
+            if (lane == 0) M.counted = high_gains ? 64 - __clz(high_gains) : 32 - __clz(low_gains);
+            if (lane == 0) factors->counted = high_rows ? 64 - __clz(high_rows) : 32 - __clz(low_rows);
+        }
+        if (tid == kBulk) bulk_out_read();  // Q's tile, or the last head's W
+        __syncthreads();
+        // values as what they add to the state
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const ulonglong2 g = *reinterpret_cast<const ulonglong2 *>(&M.gain[half * 32 + j]);
+            unpack2(mul2_rn(pack2(v[j], v[j + 1]), g.x), v[j], v[j + 1]);
+            unpack2(mul2_rn(pack2(v[j + 2], v[j + 3]), g.y), v[j + 2], v[j + 3]);
         }
         M.most[0][half][gt] = largest(0.0f, v);
-        if (tid == kBulk) bulk_out_read();  // Q's tile, or the last head's W
         __syncthreads();
         const float most_v = larger(M.most[0][0][gt], M.most[0][1][gt], 0.0f);
         const float inv_v = unscale_of(exponent_of(most_v));
@@ -328,21 +338,21 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
                 const float far = M.upto[i];
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
-                    const float4 c = *reinterpret_cast<const float4 *>(&M.inv_k[j]);
+                    const float4 c = *reinterpret_cast<const float4 *>(&M.behind[j]);
                     x[j] *= c.x * far, x[j + 1] *= c.y * far, x[j + 2] *= c.z * far, x[j + 3] *= c.w * far;
                 }
             } else {
                 const int row = i & 31, limit = key ? row - 1 : row;
-                const float *decay = &M.decay[32 * half], *inv = &M.inv[64 + 32 * half];
-                float p = 1.0f;
+                const float *decay = &M.decay[32 * half];
+                float p = kKey;
 #pragma unroll
                 for (int j = 31; j >= 0; --j) {
                     if (j < row) p *= decay[j + 1 < 32 ? j + 1 : 31];
-                    x[j] = j <= limit ? x[j] * inv[j] * p : 0.0f;
+                    x[j] = j <= limit ? x[j] * p : 0.0f;
                 }
             }
             if (key) {
-                const float f = M.inv[gt] * M.beta[i];
+                const float f = kKey * M.beta[i];
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
                     const float4 a{x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
@@ -401,11 +411,17 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
         // T's rows as operands: threads 0-63 for U, 64-127 for W
         most = 0.0f;
         if (!empty) {  // (the upper right holds what is no part of T)
-            const float *by = (key ? M.beta_w : M.beta) + 32 * half;
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
-                const float4 t = *reinterpret_cast<const float4 *>(a_row + j), b = *reinterpret_cast<const float4 *>(by + j);
-                x[j] = t.x * b.x, x[j + 1] = t.y * b.y, x[j + 2] = t.z * b.z, x[j + 3] = t.w * b.w;
+                const float4 t = *reinterpret_cast<const float4 *>(a_row + j);
+                x[j] = t.x, x[j + 1] = t.y, x[j + 2] = t.z, x[j + 3] = t.w;
+            }
+            if (key) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 b = *reinterpret_cast<const float4 *>(&M.beta_w[32 * half + j]);
+                    x[j] *= b.x, x[j + 1] *= b.y, x[j + 2] *= b.z, x[j + 3] *= b.w;
+                }
             }
             most = largest(0.0f, x);
         }

@@ -195,3 +195,21 @@ def test_rows_of_zeros(torch, form, where):
         if where == "keys alone":  # what such a token is given goes nowhere
             c["v"][rows] *= (10.0 ** np.random.default_rng(1).uniform(-12, 12, (rows.sum(), 1))).astype(np.float32)
     check(torch, kh, vh, dim, segments, count, edit)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("what", ["keys", "short keys", "short keys, large values"])
+def test_keys_of_all_sizes(torch, form, what):
+    """Every token's key of a size of its own: with a strength that goes with it (beta |k|^2 as before), or shorter alone."""
+    kh, vh, dim, segments, count = form
+    rng = np.random.default_rng(7)
+
+    def edit(c):
+        by = 10.0 ** rng.uniform(-6, 6 if what == "keys" else 0, (len(c["k"]), 1))
+        c["k"] *= by
+        if what == "keys":
+            c["beta"] /= by * by
+            c["v"] *= by
+        elif what != "short keys":
+            c["v"] /= by * by
+    check(torch, kh, vh, dim, segments, count, edit)
