@@ -15,8 +15,6 @@
 // (173 -> 160 us).
 #include "delta_chunk.cuh"
 
-#include <atomic>
-
 namespace strata {
 namespace {
 
@@ -561,14 +559,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
 
 template <int D, bool ENDS, bool SORTED = false>
 cudaError_t launch_chain(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
-    constexpr int kDevices = 64;
-    static std::atomic<bool> done[kDevices];
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess && (device >= kDevices || !done[device].load(std::memory_order_relaxed))) {
-        e = cudaFuncSetAttribute(k_delta_chain<D, ENDS, SORTED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChainSmem<D>));
-        if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
-    }
+    const cudaError_t e = mix_shared_memory<k_delta_chain<D, ENDS, SORTED>>(sizeof(ChainSmem<D>));
     if (e != cudaSuccess) return e;
     const int blocks = slab.runs * slab.heads * slab.ratio * (ENDS ? 2 * (slab.parts - 1) : slab.parts);
     return kv8_launch(k_delta_chain<D, ENDS, SORTED>, dim3((unsigned)blocks), dim3(kChainThreads), sizeof(ChainSmem<D>), 1, s, n, a, r, slab);

@@ -76,7 +76,7 @@ namespace delta {
 
 using namespace pf;
 
-// 16 or 32 columns of this thread's TMEM lane, and 8 or more written.
+// 8, 16 or 32 columns of this thread's TMEM lane, and 8 or 16 written.
 __device__ __forceinline__ void tmem_read(unsigned taddr, float (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
@@ -101,12 +101,6 @@ __device__ __forceinline__ void tmem_write(unsigned taddr, const unsigned (&r)[8
                  : "memory");
 }
 __device__ __forceinline__ void tmem_write(unsigned taddr, const unsigned (&r)[16]) { tmem_st16(taddr, r); }
-__device__ __forceinline__ void tmem_write(unsigned taddr, const float (&v)[16]) {
-    unsigned r[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
-    tmem_st16(taddr, r);
-}
 __device__ __forceinline__ void tmem_written() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     tc_fence_before();

@@ -7,8 +7,6 @@
 // kLargest, or not finite, differences of large terms could lose what the state keeps: that run and head is taken whole.
 #include "delta_chunk.cuh"
 
-#include <atomic>
-
 namespace strata {
 namespace {
 
@@ -109,14 +107,7 @@ __global__ void __launch_bounds__(D *COLS / EACH) k_delta_join(const __grid_cons
 
 template <int D, int COLS, int EACH>
 cudaError_t launch_join(const DeltaNet &n, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
-    constexpr int kDevices = 64;
-    static std::atomic<bool> done[kDevices];
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess && (device >= kDevices || !done[device].load(std::memory_order_relaxed))) {
-        e = cudaFuncSetAttribute(k_delta_join<D, COLS, EACH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinSmem<D, COLS>));
-        if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
-    }
+    const cudaError_t e = mix_shared_memory<k_delta_join<D, COLS, EACH>>(sizeof(JoinSmem<D, COLS>));
     if (e != cudaSuccess) return e;
     return kv8_launch(k_delta_join<D, COLS, EACH>, dim3((unsigned)(slab.runs * slab.heads * slab.ratio * (D / COLS))), dim3(D * COLS / EACH), sizeof(JoinSmem<D, COLS>), 1, s, n, r, slab);
 }

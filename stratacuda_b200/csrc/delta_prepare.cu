@@ -14,8 +14,6 @@
 // Of a slab ahead the kernel runs beside the second one of the slab before it.
 #include "delta_chunk.cuh"
 
-#include <atomic>
-
 namespace strata {
 namespace {
 
@@ -504,14 +502,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
 
 template <int D, bool VEC>
 cudaError_t launch_prepare(const DeltaNet &n, const DeltaRule &a, const MixRuns &r, const DeltaSlab &slab, cudaStream_t s) {
-    constexpr int kDevices = 64;
-    static std::atomic<bool> done[kDevices];
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess && (device >= kDevices || !done[device].load(std::memory_order_relaxed))) {
-        e = cudaFuncSetAttribute(k_delta_prepare<D, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PrepareSmem<D>));
-        if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
-    }
+    const cudaError_t e = mix_shared_memory<k_delta_prepare<D, VEC>>(sizeof(PrepareSmem<D>));
     if (e != cudaSuccess) return e;
     return kv8_launch(k_delta_prepare<D, VEC>, dim3((unsigned)(slab.runs * slab.heads * slab.chunks)), dim3(kPrepareThreads), sizeof(PrepareSmem<D>), 1, s,
                       n, a, r, slab);

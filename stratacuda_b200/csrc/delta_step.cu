@@ -13,6 +13,9 @@
 namespace strata {
 namespace {
 
+using delta::both;
+using delta::fma2;
+
 constexpr int kStepCols = 32, kAhead = 4, kRing = 8;
 // Of heads of more than 64 keys, blocks up to which four warps share one: with few blocks the way from token to token is shorter (one
 // session of 32 heads of 128, 32 tokens: 25 us against 32), with many two warps need fewer instructions (16 sessions 106 us against 117).
@@ -38,13 +41,7 @@ __device__ __forceinline__ float sum_groups(float x) {  // over the warp's four 
     x += __shfl_xor_sync(0xffffffffu, x, 8);
     return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
-// Pairs of F32 in one register pair.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
+using Pair = unsigned long long;  // of F32, in one register pair
 __device__ __forceinline__ float4 sum_groups(Pair x, Pair y) {
     float4 f;
     unpack2(x, f.x, f.y);
@@ -120,10 +117,10 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 2 ? 8 : ROWS <= 8 ? 6 : 3
 #pragma unroll
         for (int i = 0; i < ROWS; i += 2) {
             const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(&x.k[row0 + i]), q = *reinterpret_cast<const ulonglong2 *>(&x.q[row0 + i]);
-            p0 = fma_pair(k.x, S[i][0], p0), p1 = fma_pair(k.x, S[i][1], p1);
-            y0 = fma_pair(q.x, S[i][0], y0), y1 = fma_pair(q.x, S[i][1], y1);
-            p0 = fma_pair(k.y, S[i + 1][0], p0), p1 = fma_pair(k.y, S[i + 1][1], p1);
-            y0 = fma_pair(q.y, S[i + 1][0], y0), y1 = fma_pair(q.y, S[i + 1][1], y1);
+            p0 = fma2(k.x, S[i][0], p0), p1 = fma2(k.x, S[i][1], p1);
+            y0 = fma2(q.x, S[i][0], y0), y1 = fma2(q.x, S[i][1], y1);
+            p0 = fma2(k.y, S[i + 1][0], p0), p1 = fma2(k.y, S[i + 1][1], p1);
+            y0 = fma2(q.y, S[i + 1][0], y0), y1 = fma2(q.y, S[i + 1][1], y1);
             float a, b, c, d, same;
             unpack2(k.x, a, same), unpack2(q.x, b, same), unpack2(k.y, c, same), unpack2(q.y, d, same);
             dot = fmaf(a, b, fmaf(c, d, dot));
@@ -148,12 +145,12 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 2 ? 8 : ROWS <= 8 ? 6 : 3
         };
         const float4 s = total(0);
         const float4 d{b * (v.x - a * s.x), b * (v.y - a * s.y), b * (v.z - a * s.z), b * (v.w - a * s.w)};
-        const Pair d0 = pack2(d.x, d.y), d1 = pack2(d.z, d.w), aa = pack2(a, a);
+        const Pair d0 = pack2(d.x, d.y), d1 = pack2(d.z, d.w), aa = both(a);
 #pragma unroll
         for (int i = 0; i < ROWS; i += 2) {
             const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(&x.k[row0 + i]);
-            S[i][0] = fma_pair(k.x, d0, mul2_rn(aa, S[i][0])), S[i][1] = fma_pair(k.x, d1, mul2_rn(aa, S[i][1]));
-            S[i + 1][0] = fma_pair(k.y, d0, mul2_rn(aa, S[i + 1][0])), S[i + 1][1] = fma_pair(k.y, d1, mul2_rn(aa, S[i + 1][1]));
+            S[i][0] = fma2(k.x, d0, mul2_rn(aa, S[i][0])), S[i][1] = fma2(k.x, d1, mul2_rn(aa, S[i][1]));
+            S[i + 1][0] = fma2(k.y, d0, mul2_rn(aa, S[i + 1][0])), S[i + 1][1] = fma2(k.y, d1, mul2_rn(aa, S[i + 1][1]));
         }
         if (warp == t % WARPS && lane < 8) {
             const float4 z = total(1);

@@ -1,5 +1,7 @@
 // Device helpers of the token mixers.
 #pragma once
+#include <atomic>
+
 #include "kv8.cuh"
 #include "mixers.h"
 
@@ -34,6 +36,19 @@ __device__ __forceinline__ MixRun mix_run_alone(const MixRuns &r, int sequences,
         a.sequence = -1;
     }
     return a;
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory: once a device, from whatever thread.
+template <auto kKernel>
+cudaError_t mix_shared_memory(size_t bytes) {
+    constexpr int kDevices = 64;
+    static std::atomic<bool> done[kDevices];
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < kDevices && done[device].load(std::memory_order_relaxed))) return e;
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < kDevices) done[device].store(true, std::memory_order_relaxed);
+    return e;
 }
 
 inline bool mix_aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
