@@ -404,7 +404,8 @@ int strata_kv8_call_dev(const strata_kv8_call *call);
  *   result is off by what 22 bits lose of what its state holds, not by the size of what comes later or of what a decay has taken away. A chunk
  *   where that would not hold, or in which a value is not finite (or past 2^60 in magnitude), is walked token by token, so that no token before
  *   it sees it; 0.05 to 0.4 ms a chunk. How a call is taken goes by its segments, count, heads and dim, and by the values: it repeats bit for
- *   bit, and tokens that are cut into other calls differ in their last bits.
+ *   bit, and tokens that are cut into other calls differ in their last bits. Token by token S^T k and S^T q are formed before the decay
+ *   and have to stay in F32's range there.
  * qk_rope: for each head of q and k x / sqrt(mean x^2 + epsilon) times the kind's weight [dim], its first `rotary` channels
  *   rotated (channel d with d + rotary / 2) by the row start[i] + j of cos and sin [cells][rotary / 2], as strata_norm and then
  *   strata_rope_position. Heads of q may lie q_head_stride floats apart (0: dim), as in a projection of [q | gate] for each head.

@@ -10,9 +10,8 @@
 //
 // Bound by the way round: a product, its differences, the next product and the new state cannot overlap one another. A chunk of 128
 // channels takes 6100 clocks (3.1 us): the four products 2700 of the tensor cores, half of them on that way, the rest splits, scales and
-// hand-overs. Products begin with the upper half of their 128-row operand while the lower one is made (2048 tokens over 32 heads
-// 183 -> 175 us). 18 warps leave 96 registers a thread, which the loop over chunks needs all: what it needs seldom is in shared memory
-// (173 -> 160 us).
+// hand-overs. Products begin with the upper half of their 128-row operand while the lower one is made (5% of the time). 18 warps leave 96
+// registers a thread, which the loop over chunks needs all: what it needs seldom is in shared memory (8%).
 #include "delta_chunk.cuh"
 
 namespace strata {
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) k_delta_chain(const __grid_c
             const float *u = M.row[st].u + quarter * 16 * D + (v < D ? v : 0);
             const float by = v < D ? -inv_s : 0.0f;
             float d[16];
-            unsigned long long x[8];  // U, before Z is there; with 128 channels that takes registers from the rest (2048 tokens 169.6 -> 164.7 us after it)
+            unsigned long long x[8];  // U, before Z is there; with 128 channels that takes registers from the rest, so there after it (3% of the time)
             const auto load_u = [&] {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = ENDS && transition ? 0 : pack2(u[2 * i * D], u[2 * i * D + D]);

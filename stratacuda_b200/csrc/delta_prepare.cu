@@ -7,10 +7,9 @@
 //   U^T = (diag(beta) V)^T T^T      a lane a value channel
 //   W^T = K^T (T diag(beta P))^T    a lane a key channel; K's tile as it lies, read the other way round
 // Bound by instructions (19 k of a warp a chunk and value head), most of them the splits into halves, and by the way from one step to
-// the next: two blocks of eight warps a multiprocessor, 100 KB and half of TMEM each, so that one's steps run in the other's waits (a
-// prompt of 2048 tokens over 32 heads of 128: 57 us; blocks of sixteen warps 87 us where this took 68; a thread for a whole row, all 64 columns
-// unrolled, 210 us, most of them without an instruction to issue). What becomes operands goes through shared memory and bulk copies, few
-// and large ones. Code that a block runs once comes slower than it executes, so it is kept short.
+// the next: two blocks of eight warps a multiprocessor, 100 KB and half of TMEM each, so that one's steps run in the other's waits (288
+// chunks of a prompt over 32 heads of 128: 34 us; blocks of sixteen warps take 1.3 times as long). What becomes operands goes through shared
+// memory and bulk copies, few and large ones. Code that a block runs once comes slower than it executes, so it is kept short.
 // Of a slab ahead the kernel runs beside the second one of the slab before it.
 #include "delta_chunk.cuh"
 
@@ -56,7 +55,7 @@ __device__ __forceinline__ void bulk_out_commit() { asm volatile("cp.async.bulk.
 __device__ __forceinline__ void bulk_out_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 // x of (I + L) x = e_c, L the strictly lower part of 32 rows; at l its negative, by columns. Once x_j is known all later rows have
-// their term (the rows' sums one after another took 3200 clocks, a chain of up to 8 products a row).
+// their term, so that no row waits for a sum of its own.
 __device__ __forceinline__ void substitute(const float *l, int c, float (&x)[32]) {
     unsigned long long s[16];
 #pragma unroll
@@ -143,8 +142,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_delta_prepare(const __gr
     constexpr int kPanels = D / 64, kBulk = 32;  // the thread that copies out
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     PrepareSmem<D> &M = *reinterpret_cast<PrepareSmem<D> *>(smem_raw);
-    // half of the columns, row; the warp's number comes from one lane, so that what follows from it is the whole warp's (80 -> 76.5 us for 24
-    // prompts of up to 531 tokens over 8 heads of 64)
+    // half of the columns, row; the warp's number comes from one lane, so that what follows from it is the whole warp's (5% of the kernel)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, half = warp >> 2, gt = tid & 127, w4 = warp & 3;
     if (slab.ahead) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     else kv8_enter();

@@ -67,8 +67,8 @@ __global__ void __launch_bounds__(kRowThreads, TAPS == 4 && VEC == 4 && C == 1 ?
     float *history = n.history + ((long long)me.sequence * n.channels() + c0) * (taps - 1);
     constexpr bool kWide = TAPS == 4 && VEC == 4;  // four channels' weights are four vectors, their histories three
     constexpr int kAhead = W <= 4 ? 4 : 1;         // rows in flight
-    // Of the widths that have registers for it, the next rows while these are worked on: 4096 tokens of 8192 channels, heads of 256, 72 -> 67 us,
-    // of 4096 channels with three taps 49 -> 43 us. (Four taps of a vector a lane would have two blocks a multiprocessor in place of three, 133 -> 135 us.)
+    // Of the widths that have registers for it, the next rows while these are worked on: 4096 tokens of 8192 channels, heads of 256, 67 us
+    // (72 without), of 4096 channels with three taps 43 (49). Four taps of a vector a lane would have two blocks a multiprocessor in place of three.
     constexpr bool kNext = !(TAPS == 4 && W == 4);
     float w[ROOM][W], row[ROOM - 1 + kAhead][W];   // row[i] is token t + i - (ROOM - 1); fewer taps than ROOM are the last ones
     const int skip = ROOM - taps;

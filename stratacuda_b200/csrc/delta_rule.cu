@@ -9,23 +9,23 @@ namespace {
 
 constexpr int kSms = 148;
 
-// Rows of a run up to which it is taken token by token. A call in chunks takes 29 us however short its runs are (23 us with heads
-// of 64), token by token 0.7 us a row, and with more state than the multiprocessors walk at once as much longer as chunks get. 32 heads of
-// 128: one session 29 us in chunks and 34 us token by token at 44 rows, two 29 and 32 us at 36, four 30 and 36 us at 28, 16 72 and 82 us at 24;
-// 8 heads of 64: one session 23 and 26 us at 48 rows, 64 of them 48 and 49 us.
+// Rows of a run up to which it is taken token by token. A call in chunks takes 31 us however short its runs are (24 us with heads
+// of 64), token by token 0.75 us a row, and with more state than the multiprocessors walk at once as much longer as chunks get. 32 heads of
+// 128, in chunks and token by token: one session of 34 rows 31 and 26 us, of 44 31 and 34; two of 36 31 and 32; four of 21 33 and 27, of 28 33
+// and 35; 16 of 21 76 and 71, of 24 76 and 81; 8 heads of 64: one of 40 24 and 22 us, of 48 24 and 25; 64 of 40 50 and 41, of 56 51 and 57.
 int short_run(const DeltaNet &n, const MixRuns &r) {
     if (n.dim <= 64) return 44;
     return (long long)r.segments * n.value_heads <= kSms / 2 ? 34 : 21;
 }
 
 // States up to which runs are taken in parts: with N of them, (148 / N + 3) / 2 parts fill the multiprocessors (of a part but the last
-// its end and, but for the first, its transition; then all parts once more, from the states that these give). One prompt of 8191 tokens over
-// 2 heads of 128 440 -> 130 us, over 16 494 -> 330 us, over 24 523 -> 490 us; of 2048 over 8 of 64 112 -> 61 us, over 24 of 128
-// 154 -> 141 us. Over 32 three parts are left: 2048 tokens 156 -> 159 us, 8191 546 -> 627 us.
+// its end and, but for the first, its transition; then all parts once more, from the states that these give). As one and in parts: one prompt of
+// 8191 tokens over 2 heads of 128 444 and 135 us, over 16 505 and 347, over 24 536 and 518; of 2048 over 8 of 64 114 and 63 us, over 24 of 128 160
+// and 148. Over 32 three parts are left: 2048 tokens 164 and 167 us, 8191 562 and 661.
 constexpr int kSplitStates = 24;
 
 // Parts of a run's chunks, by tenths of microseconds: 3.7 us a chunk as one, 7.1 us a part's chunk twice, 1.5 us to join a part and 15 us
-// of two more kernels. (1000 tokens over 4 heads of 128: 77 us as one, 64 in 8 parts; 640 over 8: 58 and 57 us.)
+// of two more kernels. (1000 tokens over 4 heads of 128: 80 us as one, 66 in 8 parts; 640 over 8: 60 and 58 us.)
 int parts_of(int chunks, int most) {
     int best = 1, least = chunks * 37;
     for (int k = 3; k <= std::min(most, chunks); ++k) {
@@ -140,9 +140,9 @@ cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &giv
         }
     }
     // Few states leave most multiprocessors idle in the second kernel: there the next slab's first one runs meanwhile, on the
-    // workspace's other half. The first slab gives each multiprocessor two blocks, the next ones those that are left. One prompt
-    // of 2048 tokens over 32 heads of 128 172 -> 156 us, of 8191 over 48 825 -> 585 us, two of 1024 over 32 121 -> 112 us; three
-    // would take 200 us in place of 163: with more states than half of the multiprocessors one slab after another.
+    // workspace's other half. The first slab gives each multiprocessor two blocks, the next ones those that are left. One after another and
+    // side by side: one prompt of 2048 tokens over 32 heads of 128 177 and 164 us, of 8191 over 48 876 and 606, two of 1024 over 32 129 and 121;
+    // three 179 and 218: with more states than half of the multiprocessors one slab after another.
     if ((long long)r.segments * n.value_heads <= kSms / 2) {
         const int chains = r.segments * n.value_heads, per = r.segments * n.key_heads, most = room / 2 / per;  // chunks of a half
         const int first = std::min(most, 2 * kSms / per), next = std::min(most, std::max(1, 2 * (kSms - chains) / per));
@@ -159,7 +159,7 @@ cudaError_t delta_rule(const DeltaNet &n, const DeltaRule &a, const MixRuns &giv
         }
     }
     // Of somewhat more states than multiprocessors those of long runs go first, so that none of them begins when others end (24 runs of
-    // up to 531 tokens, 8 heads of 64: 88.5 -> 80.5 us; with two states or more for each multiprocessor it gains nothing and costs 2%).
+    // up to 531 tokens, 8 heads of 64: 88 us without, 80 with it; with two states or more for each multiprocessor it gains nothing and costs 2%).
     // Whole runs where they fit; else as many runs as give each multiprocessor two value heads, and their chunks in turn.
     const int heads = std::min(n.key_heads, room);
     int runs = std::max(1, std::min({r.segments, room / heads, (2 * kSms + heads * ratio - 1) / (heads * ratio)}));

@@ -1,7 +1,7 @@
 // Norms of queries and keys for each head with the position's rotation in the same pass (strata_qk_rope).
 //
 // Bound by bytes: a group of LANES lanes has a head row, reads it once from memory (what a channel is paired with comes from
-// L1), and writes it once. A block has heads of one token, so that no index is divided (90 -> 84 us). 8191 tokens of 24 + 2 heads of
+// L1), and writes it once. A block has heads of one token, so that no index is divided. 8191 tokens of 24 + 2 heads of
 // 256: 84 us, 5.2 TB/s; partners through shuffles took 94 us.
 #include "mixers.cuh"
 

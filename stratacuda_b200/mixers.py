@@ -195,8 +195,8 @@ class DeviceDeltaNet(_Device):
     """A delta-rule layer in caller-owned device memory: torch tensors, Buffers or addresses of the layouts in
     include/strata_cuda.h. Tensors are checked for their type, device, order and size and Buffers for their size; addresses are the
     caller's word. ``inputs`` needs `weight` and (with taps > 1) `history`, ``rule`` needs `state` and `workspace`. Calls go to
-    `stream` (a cudaStream_t as an integer; 0 is the default stream) of the current device, allocate nothing and do not
-    synchronise. `status`, where given, is a zeroed 32-bit device word that device-side errors are added to. The parts must stay
+    `stream` (a cudaStream_t as an integer; 0 is the default stream) of the current device, which has to be the parts', allocate
+    nothing and do not synchronise. `status`, where given, is a zeroed 32-bit device word that device-side errors are added to. The parts must stay
     alive."""
 
     def __init__(self, key_heads: int, value_heads: int, dim: int, sequences: int, taps: int = 4, state=None, history=None, weight=None,
