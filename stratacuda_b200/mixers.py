@@ -147,7 +147,7 @@ class QkRope:
 class _Device:
     """What both views of caller-owned memory do with tensors, Buffers and addresses."""
 
-    _device = None
+    _device = _cuda = None
 
     # most calls' tensors are as they should be: these look at that at once, and leave the rest to _address
     def _floats(self, x, what: str, need: int):
@@ -169,14 +169,20 @@ class _Device:
     def _rows(self, x, what: str, rows: int, width: int, stride: int):
         return _strided(x, what, rows, width, stride, self._device) if stride else self._floats(x, what, rows * width)
 
+    def _where(self):
+        """The parts' device, if a tensor among them tells. The only device there is is the current one: nothing to look at in calls."""
+        self._device = next((x.get_device() for x in self.parts if hasattr(x, "get_device")), None)
+        if self._device is not None:
+            import torch
+            self._cuda = None if self._device == 0 and torch.cuda.device_count() == 1 else torch.cuda
+        return self._device
+
     def _here(self) -> None:
         """Calls go to a stream of the current device: refused where that is not the one that holds the parts. (A launch refuses a stream of
         another device than the current one.)"""
-        if self._device is not None:
-            import torch
-            if (now := torch.cuda.current_device()) != self._device:
-                raise StrataError(L.ERR_LAYOUT, f"the parts are on device {self._device}, the current device is {now}: its default stream, or "
-                                                "another of its streams, is where the call would go")
+        if self._cuda is not None and (now := self._cuda.current_device()) != self._device:
+            raise StrataError(L.ERR_LAYOUT, f"the parts are on device {self._device}, the current device is {now}: its default stream, or "
+                                            "another of its streams, is where the call would go")
 
     def _run(self, entry, pack, *values) -> None:
         try:
@@ -205,7 +211,7 @@ class DeviceDeltaNet(_Device):
         self._inputs, self._rule = lib.strata_delta_inputs_dev, lib.strata_delta_rule_dev
         _int32(key_heads=key_heads, value_heads=value_heads, dim=dim, sequences=sequences, taps=taps)
         self.parts = (state, history, weight, workspace, status)
-        self._device = d = next((x.get_device() for x in self.parts if hasattr(x, "get_device")), None)
+        d = self._where()
         n = sizes(key_heads, value_heads, dim, sequences, taps)
         self.kd, self.vd, self.value_heads = key_heads * dim, value_heads * dim, value_heads
         self._net = L.StrataDeltaNetDev(key_heads, value_heads, dim, taps, sequences, _address(state, "state", n["state"], "float32", d),
@@ -243,7 +249,7 @@ class DeviceQkRope(_Device):
         self._entry = L.load().strata_qk_rope_dev
         _int32(heads=heads, kv_heads=kv_heads, dim=dim, rotary=rotary, cells=cells, sequences=sequences)
         self.parts = (q_weight, k_weight, cos, sin, status)
-        self._device = d = next((x.get_device() for x in self.parts if hasattr(x, "get_device")), None)
+        d = self._where()
         self.heads, self.dim, self.kw = heads, dim, kv_heads * dim
         self._weights = L.StrataQkRopeWeightsDev(heads, kv_heads, dim, rotary, cells, sequences,
                                                  _address(q_weight, "q_weight", dim, "float32", d), _address(k_weight, "k_weight", dim, "float32", d),
